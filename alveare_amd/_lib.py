@@ -25,6 +25,8 @@ ALV_ACT_SILU = 1
 # Every symbol include/alveare_q4.h declares: name -> (restype, argtypes).
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
+_l = ctypes.c_int64
+_f = ctypes.c_float
 SIGNATURES: dict[str, tuple] = {
     "alv_last_error": (ctypes.c_char_p, []),
     "alv_version": (ctypes.c_char_p, []),
@@ -69,6 +71,14 @@ SIGNATURES: dict[str, tuple] = {
     "alv_q4_tiled_bytes": (ctypes.c_uint64, [_i, _i]),
     "alv_q4_tile": (_i, [_vp, _vp, _i, _i, _vp]),
     "alv_chain_run": (_i, [_vp, _i, _i, _vp]),
+    "alv_qkv_post_paged": (_i, [_vp, _l, _i, _i, _i, _i, _i, _vp, _vp, _i, _i, _i, _f, _vp, _i, _l, _i, _i, _i, _vp, _l,
+                                _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _l, _l, _vp, _l, _vp]),
+    "alv_attention_paged_workspace": (ctypes.c_uint64, [_i, _i, _i, _i, _i, _i]),
+    "alv_attention_paged": (_i, [_vp, _l, _vp, _vp, _l, _l, _i, _i, _vp, _l, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i,
+                                 _f, _vp, _l, _vp, ctypes.c_uint64, _vp]),
+    "alv_copy_pages": (_i, [_vp, _i, _l, _l, _i, _vp, _vp, _i, _vp]),
+    "alv_sample_workspace": (ctypes.c_uint64, [_i, _i]),
+    "alv_sample": (_i, [_vp, _l, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _vp, _vp, _vp, ctypes.c_uint64, _vp]),
     "alv_glu": (_i, [_vp, _vp, _vp, ctypes.c_int64, _i, _vp]),
 }
 

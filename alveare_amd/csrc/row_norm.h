@@ -82,7 +82,7 @@ struct PwFrame {
     float left;
 };
 
-__device__ float pw_serial_sq(const float* a, int n, PwFrame* st) {
+__device__ __attribute__((unused)) float pw_serial_sq(const float* a, int n, PwFrame* st) {
     int sp = 0;
     st[0] = {0, n, 0, 0.0f};
     float ret = 0.0f;

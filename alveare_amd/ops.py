@@ -451,6 +451,63 @@ def chain_run(ops, M: int = 1) -> None:
         check(lib().alv_chain_run(arr, len(ops), M, torch.cuda.current_stream(dev).cuda_stream), "alv_chain_run")
 
 
+def _per_row(v, name: str, B: int, dtype: torch.dtype, dev: torch.device):
+    """(device array, number) of a parameter given as a tensor of B values or one number."""
+    if isinstance(v, torch.Tensor):
+        if v.dtype != dtype or v.device != dev or not v.is_contiguous():
+            raise TypeError(f"{name} must be a number or a contiguous {dtype} tensor on the logits' device")
+        if v.numel() < B:
+            raise ValueError(f"{name} holds {v.numel()} values for {B} rows")
+        return v.data_ptr(), 0
+    return None, int(v) if dtype == torch.int32 else float(v)
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           token: torch.Tensor | None = None, prob: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """One token per row of ``logits`` (float32, (B, vocab) or (vocab,), rows
+    contiguous in themselves) from the uniform numbers ``u`` (float32, one per
+    row, in [0, 1)): temperature, then the ``top_k`` largest, of those the
+    smallest set of the likeliest whose probability reaches ``top_p``, of those
+    the ones at least ``min_p`` times as likely as the likeliest (alv_sample has
+    the exact definition). Parameters are numbers or one value per row on the
+    device (float32; ``top_k`` int32). temperature 0: greedy, as ``lm_head``.
+    Returns (token int32 [B], the token's probability among those kept, float32
+    [B]); a row of nothing but -inf gives token -1."""
+    dev = _need_gpu(logits, u)
+    if logits.dtype != torch.float32 or logits.dim() not in (1, 2) or logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        raise TypeError("logits must be float32, (B, vocab) or (vocab,), contiguous along the vocabulary")
+    B, V = (1, logits.shape[0]) if logits.dim() == 1 else logits.shape
+    ld = V if logits.dim() == 1 or B <= 1 else logits.stride(0)
+    if u.dtype != torch.float32 or not u.is_contiguous():
+        raise TypeError("u must be a contiguous float32 tensor")
+    if u.numel() < B:
+        raise ValueError(f"u holds {u.numel()} numbers for {B} rows")
+    params = (*_per_row(temperature, "temperature", B, torch.float32, dev), *_per_row(top_k, "top_k", B, torch.int32, dev),
+              *_per_row(top_p, "top_p", B, torch.float32, dev), *_per_row(min_p, "min_p", B, torch.float32, dev))
+    if token is None:
+        token = torch.empty(B, dtype=torch.int32, device=dev)
+    elif token.dtype != torch.int32 or token.device != dev or not token.is_contiguous() or token.numel() < B:
+        raise TypeError(f"token must be a contiguous int32 tensor of {B} on the logits' device")
+    if prob is None:
+        prob = torch.empty(B, dtype=torch.float32, device=dev)
+    elif prob.dtype != torch.float32 or prob.device != dev or not prob.is_contiguous() or prob.numel() < B:
+        raise TypeError(f"prob must be a contiguous float32 tensor of {B} on the logits' device")
+    with _on(dev):
+        ws = _workspace(lib().alv_sample_workspace(B, V), dev)
+        check(lib().alv_sample(logits.data_ptr(), ld, B, V, u.data_ptr(), *params, token.data_ptr(), prob.data_ptr(),
+                               *ws[1:], _stream(logits)), "alv_sample")
+    return token, prob
+
+
+def _workspace(n: int, dev: torch.device):
+    """(tensor, address, bytes) of a call's temporaries, from torch's allocator: a captured call's live in its
+    graph's own pool, so two graphs share none."""
+    if n == 0:
+        return None, None, 0
+    t = torch.empty(n, dtype=torch.uint8, device=dev)
+    return t, t.data_ptr(), n
+
+
 def lm_head(W: "Q4Weight", x: torch.Tensor, vocab: int | None = None, softcap: float = 30.0,
             logits: torch.Tensor | None = None, token: torch.Tensor | None = None,
             pos: torch.Tensor | None = None, max_pos: int = 0) -> tuple[torch.Tensor, torch.Tensor]:

@@ -1,0 +1,341 @@
+"""Batches of sequences over a paged KV cache: prompts, drafts and decode steps.
+
+``alveare_amd.layer`` steps one sequence by one token over a cache in one
+piece. Here a call takes a packed batch: sequence b owns rows ``q_start[b] ..
+q_start[b + 1] - 1`` of every activation, the last of its ``kv_len[b]``
+positions (the new ones included), and position p is slot ``p % S`` of page
+``page_table[b, p // S]``. The three are int32 tensors on the device, read by
+the kernels, so a captured step replays with whatever they hold then. Pages are
+``(pages, kv_heads, S, D)`` bfloat16, S a power of two from 16 to 1024; a table
+entry outside ``[0, pages)`` holds no positions (pages a window has left behind
+may be given up by writing -1 there).
+
+===================  ========================================================
+``qkv_post_paged``   q/k/v norms + RoPE + insert of every new token, in the
+                     bits of ``layer.qkv_post``
+``attention_paged``  attention of every new token: causal, sliding window,
+                     first tokens that stay visible
+``copy_pages``       pages copied within each of many caches
+``PagedCache``       the layers' pages and the tables of a set of sequences:
+                     reserve, fork, truncate, free, compact
+===================  ========================================================
+"""
+from __future__ import annotations
+
+import ctypes
+import heapq
+
+import numpy as np
+import torch
+
+from ._lib import check, lib
+from .layer import _GEMMA_EPS, _f32, _ptr
+from .ops import _need_gpu, _on, _stream, _workspace
+
+
+def _rows(t: torch.Tensor, name: str, width: int, dev: torch.device) -> torch.Tensor:
+    """A (T, >= width) bfloat16 tensor, contiguous along its rows."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 2 or t.device != dev:
+        raise TypeError(f"{name} must be a 2-D bfloat16 tensor on {dev}")
+    if t.shape[1] < width or t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} rows must be contiguous and hold {width} values, got shape {tuple(t.shape)} "
+                         f"strides {t.stride()}")
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _pages(kpages: torch.Tensor, vpages: torch.Tensor, dev: torch.device):
+    """(pages, kv_heads, S, D, page strides) of the two pools: each page contiguous in itself."""
+    for t, name in ((kpages, "kpages"), (vpages, "vpages")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 4 or t.device != dev:
+            raise TypeError(f"{name} must be a (pages, kv_heads, page_size, D) bfloat16 tensor on {dev}")
+        _, H, S, D = t.shape
+        if t.stride(3) != 1 or t.stride(2) != D or H > 1 and t.stride(1) != S * D:
+            raise ValueError(f"{name}: each page must be contiguous, got strides {t.stride()}")
+    if kpages.shape != vpages.shape:
+        raise ValueError(f"kpages and vpages differ: {tuple(kpages.shape)} and {tuple(vpages.shape)}")
+    n, H, S, D = kpages.shape
+    return n, H, S, D, *(t.stride(0) if n > 1 else H * S * D for t in (kpages, vpages))
+
+
+def _batch(page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, dev: torch.device):
+    """(B, max_pages, row stride of the table)."""
+    for t, name, dim in ((page_table, "page_table", 2), (q_start, "q_start", 1), (kv_len, "kv_len", 1)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or t.device != dev:
+            raise TypeError(f"{name} must be a {dim}-D int32 tensor on {dev}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name} must be contiguous along its rows")
+    B, W = page_table.shape
+    if kv_len.shape[0] != B or q_start.shape[0] != B + 1:
+        raise ValueError(f"a table of {B} sequences needs kv_len of {B} and q_start of {B + 1}, got {kv_len.shape[0]} "
+                         f"and {q_start.shape[0]}")
+    return B, W, page_table.stride(0) if B > 1 else W
+
+
+def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
+                   q_start: torch.Tensor, kv_len: torch.Tensor, *, heads: int, k_off: int, v_off: int, q_w=None,
+                   k_w=None, norm_q: bool = True, norm_k: bool = True, norm_v: bool = True, eps: float = _GEMMA_EPS,
+                   rope: torch.Tensor | None = None, cos_off: int = 0, sin_off: int | None = None,
+                   half: int | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``layer.qkv_post`` for every row of ``qkv`` (T, [q | k | v]): per-head
+    norms, RoPE of q and k at the row's position, k and v into their pages.
+    ``rope`` is the (positions, width) bfloat16 table, by default [cos | sin]
+    halves of its rows. Returns q (T, heads * D); rows past the last sequence are
+    left as they are in ``q_out``, zeros for a sequence that does not fit its
+    table (or the rope table)."""
+    dev = _need_gpu(qkv)
+    pages, kv_heads, S, D, ks, vs = _pages(kpages, vpages, dev)
+    B, W, ldt = _batch(page_table, q_start, kv_len, dev)
+    _rows(qkv, "qkv", (k_off if v_off < 0 else v_off) + kv_heads * D, dev)
+    T = qkv.shape[0]
+    q_w, k_w = _f32(q_w, "q_w", D, dev), _f32(k_w, "k_w", D, dev)
+    rope_rows = ldr = 0
+    if rope is not None:
+        _rows(rope, "rope", 2, dev)
+        rope_rows, ldr = rope.shape[0], _ld(rope)
+        half = rope.shape[1] // 2 if half is None else half
+        sin_off = half if sin_off is None else sin_off
+    if q_out is None:
+        q_out = torch.empty(T, heads * D, dtype=torch.bfloat16, device=dev)
+    elif _rows(q_out, "q_out", heads * D, dev).shape[0] < T:
+        raise ValueError(f"q_out has {q_out.shape[0]} rows, qkv {T}")
+    with _on(dev):
+        check(lib().alv_qkv_post_paged(qkv.data_ptr(), _ld(qkv), k_off, v_off, heads, kv_heads, D, _ptr(q_w), _ptr(k_w),
+                                       norm_q, norm_k, norm_v, eps, _ptr(rope), rope_rows, ldr, cos_off, sin_off or 0,
+                                       half or 0, page_table.data_ptr(), ldt, W, q_start.data_ptr(), kv_len.data_ptr(),
+                                       B, T, pages, S, kpages.data_ptr(), vpages.data_ptr(), ks, vs, q_out.data_ptr(),
+                                       _ld(q_out), _stream(qkv)), "alv_qkv_post_paged")
+    return q_out
+
+
+def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
+                    q_start: torch.Tensor, kv_len: torch.Tensor, *, heads: int, window: int = 0, sinks: int = 0,
+                    scale: float = 1.0, max_q: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of every row of ``q`` (T, heads * D) over the positions up to
+    its own: all of them, or with ``window`` the last ``window`` and the first
+    ``sinks``. A row that sees no position gets zeros; rows past the last
+    sequence are left as they are in ``out``. ``max_q``, the most rows any
+    sequence owns, where the caller knows it, lets the call choose how to spread
+    the work (1 for a decode step); it does not change what is computed."""
+    dev = _need_gpu(q)
+    pages, kv_heads, S, D, ks, vs = _pages(kpages, vpages, dev)
+    B, W, ldt = _batch(page_table, q_start, kv_len, dev)
+    _rows(q, "q", heads * D, dev)
+    T = q.shape[0]
+    if out is None:
+        out = torch.empty(T, heads * D, dtype=torch.bfloat16, device=dev)
+    elif _rows(out, "out", heads * D, dev).shape[0] < T:
+        raise ValueError(f"out has {out.shape[0]} rows, q {T}")
+    L = lib()
+    with _on(dev):
+        ws = _workspace(L.alv_attention_paged_workspace(heads, kv_heads, D, B, T, max_q), dev)
+        check(L.alv_attention_paged(q.data_ptr(), _ld(q), kpages.data_ptr(), vpages.data_ptr(), ks, vs, pages, S,
+                                    page_table.data_ptr(), ldt, W, q_start.data_ptr(), kv_len.data_ptr(), B, T, max_q,
+                                    heads, kv_heads, D, window, sinks, scale, out.data_ptr(), _ld(out), *ws[1:],
+                                    _stream(q)), "alv_attention_paged")
+    return out
+
+
+def _host_i32(v, name: str) -> np.ndarray:
+    """Page numbers as a host int32 array."""
+    if isinstance(v, torch.Tensor):
+        if v.device.type != "cpu":
+            raise ValueError(f"{name} must be on the host: it is checked before anything is copied")
+        v = v.numpy()
+    a = np.asarray(v)
+    if a.size == 0:
+        return np.empty(0, np.int32)
+    if a.dtype.kind not in "iu" or a.ndim != 1:
+        raise TypeError(f"{name} must be a sequence of integers, got {a.dtype} of {a.ndim} dimensions")
+    if a.min() < 0 or a.max() > 0x7FFFFFFF:
+        raise ValueError(f"{name} holds page numbers out of range")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def copy_pages(caches, src, dst) -> None:
+    """In every cache (tensors of one shape whose first dimension counts pages,
+    each page contiguous): page ``dst[i]`` = page ``src[i]``. ``src`` and ``dst``
+    are host sequences; a page may be the destination of one copy and then the
+    source of none."""
+    caches = list(caches)
+    if not caches:
+        return
+    first = caches[0]
+    dev = _need_gpu(*caches)
+    shape, strides, esize = first.shape, first.stride(), first.element_size()
+    if first.dim() < 2 or first.numel() == 0:
+        raise ValueError(f"a cache must be (pages, ...), got shape {tuple(shape)}")
+    for t in caches:
+        if t.shape != shape or t.stride() != strides or t.dtype != first.dtype:
+            raise ValueError(f"the caches differ: {t.dtype} {tuple(t.shape)} {t.stride()} and {first.dtype} "
+                             f"{tuple(shape)} {strides}")
+    if not first[0].is_contiguous():
+        raise ValueError(f"each page must be contiguous, got strides {strides}")
+    src, dst = _host_i32(src, "src"), _host_i32(dst, "dst")
+    if len(src) != len(dst):
+        raise ValueError(f"{len(src)} sources and {len(dst)} destinations")
+    n = first[0].numel() * esize
+    ptrs = (ctypes.c_void_p * len(caches))(*[t.data_ptr() for t in caches])
+    with _on(dev):
+        check(lib().alv_copy_pages(ptrs, len(caches), n, strides[0] * esize if shape[0] > 1 else n, shape[0],
+                                   src.ctypes.data, dst.ctypes.data, len(src), _stream(first)), "alv_copy_pages")
+
+
+class PagedCache:
+    """The K and V pages of a model's layers and the tables of up to ``slots``
+    sequences. One page number stands for that page of every layer, K and V.
+
+    The bookkeeping (which slot holds which pages, how often a page is shared)
+    is the host's; only page copies and the tables go to the device, in the
+    order of the current stream. ``batch`` gives the tensors the kernels take.
+    A call that needs more pages than are free raises ``MemoryError`` and changes
+    nothing."""
+
+    def __init__(self, *, layers: int, kv_heads: int, D: int, pages: int, page_size: int, slots: int, max_pages: int,
+                 device):
+        if min(layers, kv_heads, D, pages, slots, max_pages) < 1:
+            raise ValueError("layers, kv_heads, D, pages, slots and max_pages must be positive")
+        if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
+            raise ValueError(f"page_size={page_size}: a power of two from 16 to 1024")
+        self.device = torch.device(device)
+        self.page_size, self.pages, self.slots, self.max_pages = page_size, pages, slots, max_pages
+        self.pool = torch.zeros((layers, 2, pages, kv_heads, page_size, D), dtype=torch.bfloat16, device=self.device)
+        self.k = [self.pool[i, 0] for i in range(layers)]
+        self.v = [self.pool[i, 1] for i in range(layers)]
+        self._table: list[list[int]] = [[] for _ in range(slots)]
+        self._len = [0] * slots
+        self._shared = [0] * pages  # slots that hold the page
+        self._free = list(range(pages))  # a heap: the lowest page first
+
+    def _slot(self, slot: int) -> int:
+        if not 0 <= slot < self.slots:
+            raise IndexError(f"slot {slot} of {self.slots}")
+        return slot
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, slot: int) -> int:
+        return self._len[self._slot(slot)]
+
+    def table(self, slot: int) -> list[int]:
+        """The slot's pages, in the order of its positions."""
+        return list(self._table[self._slot(slot)])
+
+    def _copy(self, src: list[int], dst: list[int]) -> None:
+        copy_pages(self.k + self.v, src, dst)
+
+    def _take(self) -> int:
+        p = heapq.heappop(self._free)
+        self._shared[p] = 1
+        return p
+
+    def _drop(self, page: int) -> None:
+        self._shared[page] -= 1
+        if self._shared[page] == 0:
+            heapq.heappush(self._free, page)
+
+    def reserve(self, slots, n) -> None:
+        """Room for ``n`` more positions in each slot (one number or one per
+        slot), counted in its length: a last page that is partly filled and
+        shared is copied first, so that what is inserted reaches no other slot."""
+        slots = [self._slot(s) for s in slots]
+        n = [n] * len(slots) if isinstance(n, int) else list(n)
+        if len(n) != len(slots) or len(set(slots)) != len(slots):
+            raise ValueError("one count per slot, each slot once")
+        if any(m < 0 for m in n):
+            raise ValueError("counts must not be negative")
+        S = self.page_size
+        need, left = 0, {}
+        for s, m in zip(slots, n):
+            total = -(-(self._len[s] + m) // S)
+            if total > self.max_pages:
+                raise ValueError(f"slot {s}: {self._len[s] + m} positions, its table holds {self.max_pages * S}")
+            need += total - len(self._table[s])
+            if m and self._len[s] % S:
+                last = self._table[s][-1]
+                left[last] = left.get(last, self._shared[last]) - 1
+                need += left[last] > 0  # the last to write keeps the page
+        if need > len(self._free):
+            raise MemoryError(f"{need} pages needed, {len(self._free)} free")
+        src, dst = [], []
+        for s, m in zip(slots, n):
+            t = self._table[s]
+            if m and self._len[s] % S and self._shared[t[-1]] > 1:
+                src.append(t[-1])
+                self._shared[t[-1]] -= 1
+                t[-1] = self._take()
+                dst.append(t[-1])
+            self._len[s] += m
+            while len(t) * S < self._len[s]:
+                t.append(self._take())
+        if src:
+            self._copy(src, dst)
+
+    def fork(self, src: int, dst: int) -> None:
+        """``dst`` (empty) gets the positions of ``src``: its pages, shared until
+        one of the two extends into them."""
+        src, dst = self._slot(src), self._slot(dst)
+        if self._table[dst] or src == dst:
+            raise ValueError(f"slot {dst} is in use")
+        self._table[dst] = list(self._table[src])
+        self._len[dst] = self._len[src]
+        for p in self._table[dst]:
+            self._shared[p] += 1
+
+    def truncate(self, slot: int, length: int) -> None:
+        """Only the first ``length`` positions stay (rejected drafts go)."""
+        slot = self._slot(slot)
+        if not 0 <= length <= self._len[slot]:
+            raise ValueError(f"slot {slot} holds {self._len[slot]} positions, not {length}")
+        keep = -(-length // self.page_size)
+        for p in self._table[slot][keep:]:
+            self._drop(p)
+        del self._table[slot][keep:]
+        self._len[slot] = length
+
+    def free(self, slot: int) -> None:
+        self.truncate(slot, 0)
+
+    def compact(self) -> int:
+        """Every page in use into the lowest numbers; returns how many moved."""
+        used = [p for p in range(self.pages) if self._shared[p]]
+        n = len(used)
+        src = [p for p in used if p >= n]
+        dst = [p for p in range(n) if not self._shared[p]]
+        if not src:
+            return 0
+        self._copy(src, dst)
+        to = dict(zip(src, dst))
+        for t in self._table:
+            t[:] = [to.get(p, p) for p in t]
+        for a, b in to.items():
+            self._shared[b], self._shared[a] = self._shared[a], 0
+        self._free = list(range(n, self.pages))
+        return len(src)
+
+    def batch(self, slots, n):
+        """(page_table, q_start, kv_len) on the device for a packed batch of the
+        last ``n`` positions (one number or one per slot) of each slot."""
+        slots = [self._slot(s) for s in slots]
+        n = [n] * len(slots) if isinstance(n, int) else list(n)
+        if len(n) != len(slots):
+            raise ValueError("one count per slot")
+        for s, m in zip(slots, n):
+            if not 0 <= m <= self._len[s]:
+                raise ValueError(f"slot {s} holds {self._len[s]} positions, not {m} new ones")
+        B = len(slots)
+        host = torch.full((B * self.max_pages + 2 * B + 1,), -1, dtype=torch.int32)
+        a = host.numpy()
+        for i, s in enumerate(slots):
+            a[i * self.max_pages:i * self.max_pages + len(self._table[s])] = self._table[s]
+        a[B * self.max_pages] = 0
+        a[B * self.max_pages + 1:B * self.max_pages + 1 + B] = np.cumsum(n)
+        a[B * self.max_pages + 1 + B:] = [self._len[s] for s in slots]
+        d = host.to(self.device)
+        t, q, k = d.split([B * self.max_pages, B + 1, B])
+        return t.view(B, self.max_pages), q, k

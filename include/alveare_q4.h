@@ -428,6 +428,106 @@ int alv_embed(const uint16_t* table_f16, int vocab, int H, const int32_t* token_
               void* stream);
 
 /*
+ * ---- serving: a paged KV cache and a batch of sequences --------------------------
+ * No counterpart in the reference, whose cache holds one sequence in one piece
+ * and takes one token per step.
+ *
+ * K and V pages are (page, kv head, slot, column) bf16, consecutive pages
+ * k_stride / v_stride values apart (at least kv_heads * page_size * D);
+ * page_size a power of two from 16 to 1024. Position p of sequence b is slot
+ * p % page_size of page page_table[b * ld_table + p / page_size] (max_pages
+ * entries per sequence). An entry outside [0, pages) holds no positions:
+ * nothing is read from it, and nothing written to it.
+ *
+ * Sequence b < B owns the packed rows q_start[b] .. q_start[b + 1] - 1 (B + 1
+ * entries, not decreasing, q_start[B] <= T), and these are the last of its
+ * kv_len[b] positions: kv_len counts the new rows. A sequence may own no row.
+ * page_table, q_start and kv_len are int32 device memory, read by the kernels,
+ * so a captured graph replays with whatever they hold then. A sequence whose
+ * kv_len is less than its rows or more than max_pages * page_size gets zeros
+ * for its rows, and nothing in the cache changes; rows past the last sequence
+ * (padding up to T, at most 2^22) are not touched.
+ */
+
+/*
+ * alv_qkv_post for every row of a batch: per-head RMSNorm of q, k and (norm_v)
+ * v, RoPE of q and k at the row's position, q to q_out (rows ld_q apart), k and
+ * v into their pages. Row t's values are qkv + t * ld_qkv: q at 0, k at k_off,
+ * v at v_off (v_off < 0: v is the un-normalised k). The arithmetic, roundings
+ * included, is alv_qkv_post's: each value has the bits that a step of one token
+ * writes. rope holds rope_rows rows, rope_stride apart (NULL: no rotation); a
+ * sequence longer than that counts as one longer than its table for the rows
+ * past it. D one of 64, 128, 256, 512. Two sequences must not insert into the
+ * same slot.
+ */
+int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off, int heads, int kv_heads, int D,
+                       const float* q_w, const float* k_w, int norm_q, int norm_k, int norm_v, float eps,
+                       const uint16_t* rope, int rope_rows, int64_t rope_stride, int cos_off, int sin_off, int half,
+                       const int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* q_start,
+                       const int32_t* kv_len, int B, int T, int pages, int page_size, uint16_t* kpages,
+                       uint16_t* vpages, int64_t k_stride, int64_t v_stride, uint16_t* q_out, int64_t ld_q,
+                       void* stream);
+
+/*
+ * out[t, h] = softmax(scale * K q[t, h]) V for every row t of a batch over the
+ * positions p <= the row's own that its window holds: all of them, or with
+ * window > 0 the last `window` and the first `sinks`. float32 scores and
+ * softmax; bf16 out. A row that sees no position (all its pages are missing)
+ * gets zeros. K and V of a position that a row does not see do not reach it,
+ * whatever they hold. Scores that are all -infinity count as unseen. D one of
+ * 64, 128, 256, 512; scale finite, not negative; q, its rows, the pages and
+ * their strides 16-byte aligned, out and its rows 8-byte.
+ *
+ * max_q: the most rows that any sequence owns, if the caller knows (0: not
+ * known). It decides how the work is spread, not what is computed: a value too
+ * small costs time. workspace: alv_attention_paged_workspace bytes for the same
+ * arguments, 16-byte aligned (NULL if that is 0); contents are not kept between
+ * calls, and calls that may run at the same time need one each, graph replays
+ * included.
+ */
+uint64_t alv_attention_paged_workspace(int heads, int kv_heads, int D, int B, int T, int max_q);
+int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16_t* kpages, const uint16_t* vpages,
+                        int64_t k_stride, int64_t v_stride, int pages, int page_size, const int32_t* page_table,
+                        int64_t ld_table, int max_pages, const int32_t* q_start, const int32_t* kv_len, int B, int T,
+                        int max_q, int heads, int kv_heads, int D, int window, int sinks, float scale, uint16_t* out,
+                        int64_t ld_out, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/*
+ * In each of `ncaches` caches (host array of device pointers; pages of
+ * page_bytes bytes, stride_bytes apart, both multiples of 16, caches 16-byte
+ * aligned): page dst[i] = page src[i] for i < npairs. src and dst are HOST
+ * arrays, read before the call returns. Every copy may run beside every other:
+ * a page that is the destination of two pairs, or of one pair and the source of
+ * any, is refused with ALV_ERR_ARG before anything is enqueued.
+ */
+int alv_copy_pages(void* const* caches, int ncaches, int64_t page_bytes, int64_t stride_bytes, int pages,
+                   const int32_t* src, const int32_t* dst, int npairs, void* stream);
+
+/*
+ * One token per row of float32 logits (rows ld apart) from the row's uniform
+ * number u in [0, 1), beside the greedy pick of alv_lm_head. Tokens are ordered
+ * by logit, largest first, equal ones by index; w_r = exp((l_r - l_0) /
+ * temperature). Kept are the first top_k; of those the r with
+ * sum_{j<r} w_j < top_p * (their sum), the first always; of those the ones with
+ * w_r >= min_p. The token is the first r with sum_{j<=r} w_j > u * (sum of the
+ * kept), and prob (optional) its share of that sum. u = 0 gives the likeliest.
+ * Sums and weights are 64 bits wide.
+ *
+ * Each parameter comes as a device array of B values, or (NULL) as one number:
+ * temperature not above 0: greedy, first index of equal logits; top_k <= 0 or
+ * > V: no cut; top_p not below 1: no cut; min_p not above 0: no cut, above 1
+ * as 1. u outside [0, 1) counts as the nearest number inside. A row with a NaN
+ * gives its first NaN's index and probability NaN (alv_lm_head's argmax); a row
+ * of nothing but -infinity gives -1 and 0; +infinities share the weight.
+ * B <= 65536, V <= 2^24. workspace as for alv_attention_paged.
+ */
+uint64_t alv_sample_workspace(int B, int V);
+int alv_sample(const float* logits, int64_t ld, int B, int V, const float* u, const float* temperature_dev,
+               float temperature, const int32_t* top_k_dev, int top_k, const float* top_p_dev, float top_p,
+               const float* min_p_dev, float min_p, int32_t* token, float* prob, void* workspace,
+               uint64_t workspace_bytes, void* stream);
+
+/*
  * One op of a chain: a registered projection (y = W x) or a registered FFN
  * layer (y = ffn(x)); exactly one of `weight` and `ffn` is set. x and y are
  * device fp32 buffers of M rows (leading dimension K, resp. N or H). dep is

@@ -1,0 +1,201 @@
+"""Sampling against its definition in 64 bits: tokens are equal, probabilities
+within float32's rounding (2^-24 of the float64 quotient, and the fixed-point
+weights' 2^-36)."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def check(dev, logits, u, **kw):
+    import alveare_amd as aa
+
+    B = logits.shape[0]
+    dt = {"top_k": torch.int32}
+    full = {k: v if isinstance(v, list) else [v] * B for k, v in kw.items()}
+    args = {k: torch.tensor(v, dtype=dt.get(k, torch.float32), device=dev) if isinstance(kw[k], list) else kw[k]
+            for k, v in full.items()}
+    token, prob = aa.sample(logits.to(dev), torch.tensor(u, dtype=torch.float32, device=dev), **args)
+    for b in range(B):
+        want, p = R.sample(logits[b], u[b], **{k: v[b] for k, v in full.items()})
+        assert int(token[b]) == want, (b, int(token[b]), want, {k: v[b] for k, v in full.items()}, u[b])
+        if math.isnan(p):
+            assert math.isnan(float(prob[b]))
+        else:
+            assert abs(float(prob[b]) - p) <= p * (2.0 ** -24 + 2.0 ** -35) + 2.0 ** -149
+    return token
+
+
+def normal(B, V, seed=0, std=3.0):
+    return torch.randn(B, V, generator=torch.Generator().manual_seed(seed)) * std
+
+
+@pytest.mark.parametrize("V", [1, 2, 63, 64, 1000, 1025, 32000, 128256, 262144, 300001])
+def test_sizes(dev, V):
+    x = normal(6, V, V)
+    u = [0.0, 0.25, 0.5, 0.77, 0.999, 1 - 2.0 ** -24]
+    check(dev, x, u)
+    check(dev, x, u, temperature=0.7, top_k=50, top_p=0.9, min_p=0.02)
+    check(dev, x, u, top_p=0.95)
+
+
+@pytest.mark.parametrize("top_k", [0, 1, 2, 17, 1000, 5000, 40000, 10 ** 6])
+@pytest.mark.parametrize("top_p", [1.0, 0.0, 0.3, 0.9, 0.9999])
+@pytest.mark.parametrize("min_p", [0.0, 0.1, 1.0])
+def test_cuts(dev, top_k, top_p, min_p):
+    x = normal(4, 50000, 7, 2.0)
+    check(dev, x, [0.01, 0.4, 0.8, 0.9999], temperature=1.2, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+def test_parameters_per_row(dev):
+    x = normal(7, 20011, 3)
+    check(dev, x, [0.5, 0.1, 0.9, 0.3, 0.6, 0.99, 0.2], temperature=[0.0, 1.0, 0.5, -1.0, 2.0, math.nan, math.inf],
+          top_k=[5, 0, 3, -1, 100, 7, 4], top_p=[0.5, 2.0, 1.0, 0.1, -3.0, 0.9, 0.95],
+          min_p=[0.0, -1.0, 0.3, 2.0, 0.001, 0.0, 0.0])
+
+
+@pytest.mark.parametrize("V", [5, 4096, 100000])
+def test_ties(dev, V):
+    """Equal logits keep their order by index across every cut, zeros of both signs alike."""
+    x = torch.zeros(6, V)
+    x[1, V // 2:] = -0.0
+    x[2, ::2] = 1.0
+    x[3, V // 3:] = -2.0
+    x[4] = torch.arange(V).remainder(3).float()
+    x[5] = 5.0
+    x[5, 0] = -math.inf
+    for u in (0.0, 0.3, 0.5, 0.75, 0.999):
+        check(dev, x, [u] * 6)
+        check(dev, x, [u] * 6, top_p=0.5)
+        check(dev, x, [u] * 6, top_k=max(1, V // 4))
+        check(dev, x, [u] * 6, min_p=0.5, top_k=3, top_p=0.7)
+
+
+@pytest.mark.parametrize("V", [100, 5000, 262144])
+def test_extreme_values(dev, V):
+    inf = math.inf
+    big = 3.0e38
+    x = normal(8, V, 5)
+    x[0, 1:] = -inf                 # one token left
+    x[1, :] = -inf                  # none
+    x[2, 7] = inf                   # one infinity
+    x[3, [3, V - 1]] = inf          # two share the weight
+    x[4, V // 2] = math.nan
+    x[5, ::2] = -big                # masked by the type's lowest values
+    x[5, 1] = big
+    x[6, V // 3:] = torch.finfo(torch.float32).min
+    x[7, :] = torch.where(torch.arange(V) % 2 == 0, 1e30, -1e30)
+    for kw in ({}, dict(top_k=20), dict(top_p=0.8), dict(min_p=0.2), dict(temperature=1e-30), dict(temperature=1e30),
+               dict(temperature=0.0)):
+        check(dev, x, [0.6, 0.3, 0.1, 0.7, 0.5, 0.2, 0.9, 0.4], **kw)
+
+
+def test_one_bin_distributions(dev):
+    """Logits that differ in their last bits only, and outliers far above the rest."""
+    V = 60000
+    x = torch.empty(3, V)
+    x[0] = 1.0 + torch.arange(V).float() * 2.0 ** -23
+    x[1] = normal(1, V, 1, 1e-6)[0]
+    x[1, 5] = 40.0
+    x[2] = normal(1, V, 2, 50.0)[0]
+    for kw in ({}, dict(top_k=30000), dict(top_p=0.4), dict(top_k=50000, top_p=0.6), dict(temperature=100.0, top_p=0.9)):
+        for u in (0.001, 0.5, 0.97):
+            check(dev, x, [u] * 3, **kw)
+
+
+def test_strided_rows_and_given_outputs(dev):
+    import alveare_amd as aa
+
+    x = normal(5, 3000, 9).to(dev)
+    u = torch.rand(5, generator=torch.Generator().manual_seed(1)).to(dev)
+    want = aa.sample(x[:, :2500].contiguous(), u, top_k=100)
+    token, prob = torch.full((8,), 9, dtype=torch.int32, device=dev), torch.full((8,), 9.0, device=dev)
+    got = aa.sample(x[:, :2500], u, top_k=100, token=token, prob=prob)
+    assert got[0] is token and torch.equal(token[:5], want[0]) and (token[5:] == 9).all()
+    assert torch.equal(prob[:5], want[1]) and (prob[5:] == 9).all()
+    one = aa.sample(x[2, :2500], u[2:3], top_k=100)
+    assert int(one[0]) == int(want[0][2])
+    assert aa.sample(x[:0], u)[0].shape == (0,)
+    for off in (1, 2, 3):  # rows that start off a 16-byte boundary
+        y = aa.sample(x[:, off:2500], u, top_p=0.9)
+        z = aa.sample(x[:, off:2500].contiguous(), u, top_p=0.9)
+        assert torch.equal(y[0], z[0]) and torch.equal(y[1], z[1])
+
+
+def test_large_batch(dev):
+    import alveare_amd as aa
+
+    x = normal(300, 777, 2)
+    u = torch.rand(300, generator=torch.Generator().manual_seed(5))
+    check(dev, x, u.tolist(), top_p=0.9, temperature=0.8)
+    a = aa.sample(x.to(dev), u.to(dev))
+    for _ in range(2):
+        b = aa.sample(x.to(dev), u.to(dev))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_frequencies(dev):
+    """Even numbers over [0, 1) give every token its share: of N, token r is drawn
+    within one of N times its probability (an interval of u)."""
+    import alveare_amd as aa
+
+    x = torch.tensor([[0.0, 1.0, -1.0, 2.0, 0.5, -3.0]])
+    N = 4096
+    u = (torch.arange(N, dtype=torch.float32) + 0.5) / N
+    token, _ = aa.sample(x.expand(N, 6).contiguous().to(dev), u.to(dev))
+    share = torch.softmax(x[0].double(), 0) * N
+    assert ((torch.bincount(token.cpu(), minlength=6) - share).abs() <= 1).all()
+
+
+def test_graphs_and_streams(dev):
+    import alveare_amd as aa
+
+    made = []
+    for seed, V in ((1, 262144), (2, 5000)):
+        x = normal(3, V, seed).to(dev)
+        u = torch.rand(3, device=dev)
+        s = torch.cuda.Stream(dev)
+        s.wait_stream(torch.cuda.current_stream(dev))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = aa.sample(x, u, top_k=300, top_p=0.9)
+        made.append((x, u, s, g, out))
+    for turn in range(5):
+        for i, (x, u, s, g, out) in enumerate(made):
+            x.copy_(normal(3, x.shape[1], 20 + turn + i))
+            u.uniform_()
+        torch.cuda.synchronize()
+        for x, u, s, g, out in made:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for x, u, s, g, out in made:
+            want = aa.sample(x, u, top_k=300, top_p=0.9)
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_greedy_is_the_heads_argmax(dev):
+    import alveare_amd as aa
+    import numpy as np
+
+    x = normal(4, 9000, 6)
+    x[1, 400] = x[1].max()
+    x[2, [70, 8000]] = math.nan
+    token, _ = aa.sample(x.to(dev), torch.rand(4, device=dev), temperature=0.0)
+    assert token.tolist() == [int(np.argmax(r)) for r in x.numpy()]
+
+
+def test_refusals(dev):
+    import alveare_amd as aa
+
+    x, u = normal(2, 100).to(dev), torch.rand(2, device=dev)
+    for a, b, kw in ((x.double(), u, {}), (x.cpu(), u, {}), (x, u.double(), {}), (x, u[:1], {}), (x.t(), u, {}),
+                     (x, u, dict(top_k=torch.zeros(2, device=dev))), (x, u, dict(temperature=u[:1])),
+                     (x, u, dict(top_p=torch.zeros(2))), (x, u, dict(token=torch.zeros(2, device=dev))),
+                     (x, u, dict(prob=torch.zeros(1, device=dev))), (x[:, :0], u, {})):
+        with pytest.raises((TypeError, ValueError)):
+            aa.sample(a, b, **kw)
