@@ -22,6 +22,7 @@ struct PagedAttnArgs {
     uint16_t* out;
     int64_t ld_out;
     int64_t row_limit;  // sequences of more rows (tokens times q heads per kv head) are not this launch's
+    int nsplit;         // parts of a tile's positions
     float* part;
 };
 
@@ -104,16 +105,16 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 v) {
     return (nonfinite_bits(v[0]) | nonfinite_bits(v[1]) | nonfinite_bits(v[2]) | nonfinite_bits(v[3])) != 0;
 }
 
-// LDS pieces of a row are stored at (piece ^ swizzle of the row): the K reads (16
-// rows, the same piece) and the transposing V reads (4 rows, two pieces) then
-// fall on different banks.
+// LDS pieces of a row are stored at (piece ^ swizzle of the row): the 16 lanes
+// that read K at once (16 rows, the same piece) and the 32 that read V (8 rows of
+// two pieces, or 4 of four) then fall on different banks.
 template <int D>
 __device__ __forceinline__ int k_swz(int row) {
     return D == 64 ? (row >> 1) & 7 : row & 15;
 }
 template <int D>
 __device__ __forceinline__ int v_swz(int row) {
-    return D == 64 ? ((row >> 1) & 3) * 2 : (row & 7) * 2;
+    return D == 64 ? ((row >> 1) & 1) * 4 + ((row >> 2) & 1) * 2 : (row & 3) * 4 + ((row >> 2) & 1) * 2;
 }
 
 // The offset of piece c of a row as what is xored into a swizzled offset (the
@@ -127,35 +128,6 @@ __device__ __forceinline__ constexpr uint32_t piece_far(int c) {
     return (c & ~(D == 64 ? 7 : 15)) * 16;
 }
 
-// Where value d (a multiple of 4) of V's row p stands in its tile.
-template <int D>
-__device__ __forceinline__ uint32_t v_at(int p, int d) {
-    return p * (2 * D) + (((d >> 3) ^ v_swz<D>(p)) * 16) + (d & 4) * 2;
-}
-
-// o += w v for the four values at `p` that are infinite or NaN, for a lane whose
-// row sees them.
-__device__ __forceinline__ void add_nonfinite(f32x4& o, const unsigned char* p, bool see, float w) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    const uint32_t n0 = nonfinite_bits(v.x), n1 = nonfinite_bits(v.y);
-    float x0 = o[0], x1 = o[1], x2 = o[2], x3 = o[3];
-    if (see && (n0 & 0x8000u)) x0 = __builtin_fmaf(w, bf16_bits_to_f32(v.x & 0xFFFFu), x0);
-    if (see && (n0 >> 31)) x1 = __builtin_fmaf(w, bf16_bits_to_f32(v.x >> 16), x1);
-    if (see && (n1 & 0x8000u)) x2 = __builtin_fmaf(w, bf16_bits_to_f32(v.y & 0xFFFFu), x2);
-    if (see && (n1 >> 31)) x3 = __builtin_fmaf(w, bf16_bits_to_f32(v.y >> 16), x3);
-    o = f32x4{x0, x1, x2, x3};
-}
-// The eight values at `p`, zeros for those that are infinite or NaN.
-__device__ __forceinline__ void zero_nonfinite(unsigned char* p) {
-    u32x4 v = *reinterpret_cast<u32x4*>(p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint32_t w = v[e], n = nonfinite_bits(w);
-        v[e] = w & ~((n >> 15) * 0xFFFFu);
-    }
-    *reinterpret_cast<u32x4*>(p) = v;
-}
-
 __device__ __forceinline__ s16x4 read_tr(const unsigned char* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
 }
@@ -165,14 +137,11 @@ __device__ __forceinline__ bool sees(const PagedAttnArgs& a, int p, int t) {
     return p <= t && (a.window <= 0 || p > t - a.window || p < a.sinks);
 }
 
-__device__ __forceinline__ void store4(uint16_t* dst, f32x4 v, float l) {
-    uint16_t b[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float x = v[e];
-        b[e] = l == 0.0f ? (uint16_t)0 : bf16_rne_bits(x / l);
-    }
-    *reinterpret_cast<uint2*>(dst) = uint2{b[0] | ((uint32_t)b[1] << 16), b[2] | ((uint32_t)b[3] << 16)};
+// 1 / l of a row, 0 for one that saw nothing.
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+__device__ __forceinline__ void store4(uint16_t* dst, f32x4 v, float inv) {
+    *reinterpret_cast<s16x4*>(dst) = pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
 }
 
 constexpr float kNoMax = -3.0e38f;  // running maximum of a row that has seen nothing
@@ -182,6 +151,62 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // powers of two: weights up to 2^8 lose nothing in float32 or bf16, and most
 // blocks then need neither a maximum over the lanes nor a rescaled output.
 constexpr float kSlack = 8.0f;
+
+// One row's part (maximum, sum, output: RW values per lane) over units u0 .. u1 - 1
+// of its tile, by one wave in plain float32 steps. The matrix products give a
+// value of V that is infinite or NaN to every row they compute, seen or not (0
+// times it is NaN); a wave that meets one in a block that some row does not see
+// whole does its rows again with this.
+template <int D>
+__device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16_t* q, int pos, int us, int ulo, int unit,
+                          int u0, int u1, int lane, float (&acc)[D / 64], float& m, float& l) {
+    constexpr int RW = D / 64;
+    const float c = fmaxf(a.scale * kLog2e, kMinScale);
+    m = kNoMax;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < RW; ++e) acc[e] = 0.0f;
+    for (int u = u0; u < u1; ++u) {
+        const int base = (u < us ? u : u - us + ulo) * unit;
+        for (int pb = base; pb < base + unit; pb += 64) {
+            const int p = pb + lane;
+            int page = -1;
+            if (p < base + unit && sees(a, p, pos)) page = page_of(a.b, seq, p);
+            float s = -__builtin_inff();
+            const int64_t off = (((int64_t)kvh << a.b.shift) + (p & ((1 << a.b.shift) - 1))) * D;
+            if (page >= 0) {
+                const u32x4* k = reinterpret_cast<const u32x4*>(a.kpages + page * a.k_stride + off);
+                s = 0.0f;
+                for (int i = 0; i < D / 8; ++i) {
+                    const u32x4 kv = k[i], qv = reinterpret_cast<const u32x4*>(q)[i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t kw = kv[e], qw = qv[e];
+                        s = __builtin_fmaf(bf16_bits_to_f32(kw & 0xFFFFu), bf16_bits_to_f32(qw & 0xFFFFu), s);
+                        s = __builtin_fmaf(bf16_bits_to_f32(kw >> 16), bf16_bits_to_f32(qw >> 16), s);
+                    }
+                }
+            }
+            float top = s;
+            for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+            const float mn = fmaxf(m, top * c), fac = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            float w = page >= 0 ? __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -mn)) : 0.0f, sum = w;
+            for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+            l = l * fac + sum;
+#pragma unroll
+            for (int e = 0; e < RW; ++e) acc[e] *= fac;
+            for (uint64_t left = __ballot(page >= 0); left; left &= left - 1) {
+                const int j = __builtin_ctzll(left), pj = pb + j;
+                const float wj = __shfl(w, j);
+                const uint16_t* v = a.vpages + __shfl(page, j) * a.v_stride +
+                                    (((int64_t)kvh << a.b.shift) + (pj & ((1 << a.b.shift) - 1))) * D + RW * lane;
+#pragma unroll
+                for (int e = 0; e < RW; ++e) acc[e] = __builtin_fmaf(wj, bf16_bits_to_f32(v[e]), acc[e]);
+            }
+        }
+    }
+}
 
 // ---- few rows: a workgroup streams positions -------------------------------------------
 //
@@ -217,10 +242,10 @@ constexpr bool rows_q_lds(int D, int QT) { return QT * D > 256; }
 constexpr int rows_lds(int D, int QT) {
     const int ring = rows_waves(D) * rows_stages(D) * rows_stage(D);
     const int outs = rows_waves(D) * 16 * QT * (rows_out_ld(D) * 4);
-    return (ring > outs ? ring : outs) + 2 * rows_waves(D) * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0);
+    return (ring > outs ? ring : outs) + 2 * rows_waves(D) * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0) + 16;
 }
 constexpr int rows_mls(int D, int QT) {  // where the waves' maxima and sums stand; q behind them
-    return rows_lds(D, QT) - 2 * rows_waves(D) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
+    return rows_lds(D, QT) - 16 - 2 * rows_waves(D) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
 }
 // Floats of one workspace place: outputs, maxima, sums.
 constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
@@ -353,6 +378,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
     unsigned char* ring = smem + wave * NS * rows_stage(D);
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
     float* mls = reinterpret_cast<float*>(smem + rows_mls(D, QT));  // [wave][max | sum][row]
+    int* odds = reinterpret_cast<int*>(smem + rows_lds(D, QT) - 16);
     const float c = fmaxf(a.scale * kLog2e, kMinScale);
     const int S = 1 << a.b.shift;
     // Byte offsets that stay: this lane's piece of a load (memory side), of a K
@@ -430,6 +456,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
         const int pos_hi = f.s.len - f.s.n + (f.rt * ROWS + nrows - 1) / a.g;
         f32x4 o[QT][D / 16];
         float m[QT], l[QT];
+        bool odd = false;  // a value of V that is no number, where some row may not see it
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             m[t] = kNoMax;
@@ -447,8 +474,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
                 wait_vm<(NS - 1) * 2 * NI>();
             else
                 wait_vm<0>();
-            unsigned char* kt = ring + (j % NS) * rows_stage(D);
-            unsigned char* vt = kt + HALF;
+            const unsigned char* kt = ring + (j % NS) * rows_stage(D);
+            const unsigned char* vt = kt + HALF;
             f32x4 s[QT];
 #pragma unroll
             for (int t = 0; t < QT; ++t) s[t] = f32x4{0, 0, 0, 0};
@@ -500,30 +527,9 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
                 return read_tr(vt + (rd_v ^ piece<D>(2 * d)) + piece_far<D>(2 * d));
             };
             if (masked) {
-                // A weight of zero does not keep a value that is no number from
-                // the rows that do not see it: such values go to the rows that
-                // do one by one, and are zeros for the products.
-                bool odd = false;
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
                     odd |= any_nonfinite(*reinterpret_cast<const u32x4*>(vt + 1024 * i + 16 * lane));
-                if (__any(odd)) {
-#pragma unroll 1
-                    for (int p = 0; p < 16; ++p) {
-#pragma unroll
-                        for (int t = 0; t < QT; ++t) {
-                            const uint64_t w64 = __builtin_bit_cast(uint64_t, pw[t]);
-                            const uint32_t w32 = __shfl((int)(uint32_t)(p & 2 ? w64 >> 32 : w64), (p >> 2) * 16 + col);
-                            const float w = bf16_bits_to_f32(p & 1 ? w32 >> 16 : w32 & 0xFFFFu);
-                            const bool see = !gone && sees(a, p0 + p, pos[t]);
-#pragma unroll
-                            for (int d = 0; d < D / 16; ++d)
-                                add_nonfinite(o[t][d], vt + v_at<D>(p, 16 * d + 4 * G), see, w);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < NI; ++i) zero_nonfinite(vt + 1024 * i + 16 * lane);
-                }
             }
             constexpr int VB = D / 16 < 8 ? D / 16 : 8;  // V reads on their way at once
 #pragma unroll
@@ -552,7 +558,37 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
                 mls[(wave * 2 + 1) * ROWS + 16 * t + col] = l[t];
             }
         }
+        if (lane == 0) odds[wave] = 0;
+        if (__any(odd) && lane == 0) odds[wave] = 1;
         __syncthreads();  // and every wave is done with its ring
+        bool again = false;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) again |= odds[w] != 0;
+        const bool whole = u0 == 0 && u1 == f.s.nu;
+        float* part = a.part + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * rows_part(D, QT);
+        if (again) {
+            for (int r = wave; r < nrows; r += NW) {
+                const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
+                float acc[D / 64], mr, lr;
+                plain_row<D>(a, f.seq, f.kvh, a.q + (int64_t)(f.s.first + tok) * a.ld_q + h * D, f.s.len - f.s.n + tok,
+                             f.s.us, f.s.ulo, UNIT, u0, u1, lane, acc, mr, lr);
+                const float inv = inverse(lr);
+                uint16_t* dst = a.out + (int64_t)(f.s.first + tok) * a.ld_out + h * D + D / 64 * lane;
+#pragma unroll
+                for (int e = 0; e < D / 64; ++e) {
+                    if (whole)
+                        dst[e] = bf16_rne_bits(acc[e] * inv);
+                    else
+                        part[(size_t)r * D + D / 64 * lane + e] = acc[e];
+                }
+                if (!whole && lane == 0) {
+                    part[ROWS * D + r] = mr;
+                    part[ROWS * (D + 1) + r] = lr;
+                }
+            }
+            __syncthreads();
+            continue;
+        }
         float* outs = reinterpret_cast<float*>(smem);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
@@ -565,8 +601,6 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
             for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(row + 16 * d) = o[t][d] * fac;
         }
         __syncthreads();
-        const bool whole = u0 == 0 && u1 == f.s.nu;
-        float* part = a.part + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * rows_part(D, QT);
         for (int e = tid; e < nrows * (D / 4); e += 64 * NW) {
             const int r = e / (D / 4), d = 4 * (e - r * (D / 4));
             f32x4 v = *reinterpret_cast<const f32x4*>(outs + (size_t)r * rows_out_ld(D) + d);
@@ -581,7 +615,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
             }
             if (whole) {
                 const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
-                store4(a.out + (int64_t)(f.s.first + tok) * a.ld_out + h * D + d, v, ls);
+                store4(a.out + (int64_t)(f.s.first + tok) * a.ld_out + h * D + d, v, inverse(ls));
             } else {
                 *reinterpret_cast<f32x4*>(part + (size_t)r * D + d) = v;
                 if (d == 0) {
@@ -630,9 +664,394 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
         for (int e = 0; e < RW; ++e) acc[e] = __builtin_fmaf(t[e], fac, acc[e]);
     }
     const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
+    const float inv = inverse(ls);
     uint16_t* dst = a.out + (int64_t)(f.s.first + tok) * a.ld_out + h * D + RW * lane;
 #pragma unroll
-    for (int e = 0; e < RW; ++e) dst[e] = ls == 0.0f ? (uint16_t)0 : bf16_rne_bits(acc[e] / ls);
+    for (int e = 0; e < RW; ++e) dst[e] = bf16_rne_bits(acc[e] * inv);
+}
+
+// ---- many rows: a workgroup shares K and V tiles ------------------------------------------
+//
+// A tile is TR rows of one (sequence, kv head), 32 per wave (v_mfma_f32_32x32x16),
+// against BN positions at a time, K and V in LDS for all waves, the next ones on
+// their way while these are used. D = 512: a wave's output would be 256 registers;
+// two waves share 32 rows instead, each with half the columns: half of every
+// score's products, exchanged through LDS, and half of the output.
+// Where there are fewer tiles than compute units each tile's positions are split
+// and the parts joined by a second launch.
+constexpr int tile_ds(int D) { return D == 512 ? 2 : 1; }      // waves that share 32 rows
+constexpr int tile_waves(int D) { return D == 512 ? 8 : 4; }
+constexpr int tile_rows(int D) { return 32 * tile_waves(D) / tile_ds(D); }
+constexpr int tile_bn(int D) { return D <= 128 ? 64 : 32; }
+constexpr int tile_kbufs(int D) { return D == 512 ? 1 : 2; }
+constexpr int tile_bytes(int D) { return tile_bn(D) * 2 * D; }  // of K, of V
+constexpr int tile_xch(int D) { return D == 512 ? tile_waves(D) * 4096 : 0; }
+constexpr int tile_lds(int D) { return (tile_kbufs(D) + 2) * tile_bytes(D) + tile_xch(D) + 16; }
+
+typedef float f32x16 __attribute__((__vector_size__(16 * sizeof(float))));
+
+// Tiles of the sequences of more rows than row_limit, up to and with each
+// lane's, in one step of 64 sequences.
+struct TileScan {
+    int first, n, len;
+    bool ok;
+    int tiles, incl, sum;
+};
+template <int TR>
+__device__ __forceinline__ TileScan tile_scan(const PagedAttnArgs& a, int b0, int lane) {
+    TileScan t{};
+    const int b = b0 + lane;
+    if (b < a.b.B) {
+        t.first = a.b.q_start[b];
+        t.n = a.b.q_start[b + 1] - t.first;
+        t.len = a.b.kv_len[b];
+        const bool here = t.first >= 0 && t.n > 0 && (int64_t)t.first + t.n <= a.b.T;
+        t.ok = t.n <= t.len && t.len <= a.b.max_pos;
+        const int64_t rows = here ? (int64_t)t.n * a.g : 0;
+        if (rows > a.row_limit) t.tiles = (int)((rows + TR - 1) / TR);
+    }
+    int x = t.tiles;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(x, o);
+        if (lane >= o) x += u;
+    }
+    t.incl = x;
+    t.sum = __builtin_amdgcn_readlane(x, 63);
+    return t;
+}
+
+// The positions tile rt of a sequence runs over, in units of BN.
+struct TileSpan {
+    int rows;            // of the tile
+    int pos_lo, pos_hi;  // of its first and last row
+    int us, ulo, nu;
+};
+template <int TR, int BN>
+__device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int len, bool ok, int rt) {
+    TileSpan s;
+    const int64_t r0 = (int64_t)rt * TR, all = (int64_t)n * a.g;
+    s.rows = (int)min((int64_t)TR, all - r0);
+    s.pos_lo = len - n + (int)(r0 / a.g);
+    s.pos_hi = len - n + (int)((r0 + s.rows - 1) / a.g);
+    const int lo = a.window > 0 ? max(0, s.pos_lo + 1 - a.window) : 0;
+    s.ulo = lo / BN;
+    s.us = min((min(a.sinks, lo) + BN - 1) / BN, s.ulo);
+    s.nu = ok ? s.us + s.pos_hi / BN + 1 - s.ulo : 0;
+    return s;
+}
+
+template <int D>
+__global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kernel(PagedAttnArgs a) {
+    constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D), KB = tile_kbufs(D);
+    constexpr int DW = D / DS;            // this wave's columns of the output (and of its scores' products)
+    constexpr int TB = tile_bytes(D), NC = D / 8, RPL = 512 / D;
+    constexpr int LR = BN / NW;           // positions a wave loads: within one page
+    constexpr int NL = LR / RPL;          // its loads of K (of V)
+    extern __shared__ __align__(16) unsigned char smem[];
+    unsigned char* kbuf = smem;
+    unsigned char* vbuf = smem + KB * TB;
+    float* xch = reinterpret_cast<float*>(smem + (KB + 2) * TB);
+    int* tags = reinterpret_cast<int*>(smem + (KB + 2) * TB + tile_xch(D));
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rg = wave / DS, dh = wave % DS;
+    const int col = lane & 31, h = lane >> 5;
+
+    // Item: heaviest (last) tiles first, kv heads side by side, so that the
+    // workgroups an XCD gets in turn share theirs where there are eight.
+    int all = 0;
+    for (int b0 = 0; b0 < a.b.B; b0 += 64) all += tile_scan<TR>(a, b0, lane).sum;
+    const int item = all * a.kv_heads - 1 - (int)(blockIdx.x / (uint32_t)a.nsplit);
+    const int split = (int)(blockIdx.x % (uint32_t)a.nsplit);
+    if (item < 0) return;
+    const int gt = item / a.kv_heads, kvh = item - gt * a.kv_heads;
+    int base = 0, b0 = 0;
+    TileScan sc = tile_scan<TR>(a, 0, lane);
+    while (gt >= base + sc.sum) {
+        base += sc.sum;
+        b0 += 64;
+        sc = tile_scan<TR>(a, b0, lane);
+    }
+    const int l0 = __builtin_ctzll(__ballot(base + sc.incl > gt));
+    const int seq = b0 + l0;
+    const int first = __builtin_amdgcn_readlane(sc.first, l0), n = __builtin_amdgcn_readlane(sc.n, l0);
+    const int len = __builtin_amdgcn_readlane(sc.len, l0);
+    const bool ok = __builtin_amdgcn_readlane((int)sc.ok, l0) != 0;
+    const int rt = gt - base - __builtin_amdgcn_readlane(sc.incl - sc.tiles, l0);
+    const TileSpan sp = tile_span<TR, BN>(a, n, len, ok, rt);
+    const int u0 = uniform((int)((int64_t)sp.nu * split / a.nsplit));
+    const int u1 = uniform((int)((int64_t)sp.nu * (split + 1) / a.nsplit));
+    if (a.nsplit > 1 && u0 == u1) return;  // the merge skips it too
+
+    const int32_t* table = a.b.table + (int64_t)seq * a.b.ld_table;
+    auto unit_pos = [&](int u) { return (u < sp.us ? u : u - sp.us + sp.ulo) * BN; };
+    int pages = -1, pages0 = u0;
+    auto load_pages = [&](int v0) {
+        pages0 = v0;
+        const int p = unit_pos(v0 + lane) + wave * LR;
+        pages = v0 + lane < u1 && p < len ? table[p >> a.b.shift] : -1;
+        if ((unsigned)pages >= (unsigned)a.b.pages) pages = -1;
+    };
+    const uint32_t kb_lds = __builtin_amdgcn_readfirstlane(lds_addr(kbuf)) + wave * LR * (2 * D);
+    const uint32_t vb_lds = __builtin_amdgcn_readfirstlane(lds_addr(vbuf)) + wave * LR * (2 * D);
+    // The wave's rows start at a multiple of 4, not of 16: their bits of the
+    // swizzles are part of the lane's offset.
+    const uint32_t dma_k = (lane / NC) * (2 * D) + ((lane % NC) ^ k_swz<D>(wave * LR + lane / NC)) * 16;
+    const uint32_t dma_v = (lane / NC) * (2 * D) + ((lane % NC) ^ v_swz<D>(wave * LR + lane / NC)) * 16;
+    auto issue = [&](int u) {
+        if (u - pages0 >= 64) load_pages(u);
+        const int page = __builtin_amdgcn_readlane(pages, u - pages0), p = unit_pos(u) + wave * LR;
+        const uint32_t bytes = page < 0 ? 0u : (uint32_t)max(0, min(LR, len - p)) * (2 * D);
+        if (page < 0 && p < len && lane == 0) tags[u & 1] = u;
+        const int64_t off = (((int64_t)kvh << a.b.shift) + (p & ((1 << a.b.shift) - 1))) * D;
+        const __amdgpu_buffer_rsrc_t rk = wave_rsrc(a.kpages + max(page, 0) * a.k_stride + off, bytes);
+        const __amdgpu_buffer_rsrc_t rv = wave_rsrc(a.vpages + max(page, 0) * a.v_stride + off, bytes);
+        const uint32_t kd = kb_lds + (KB == 2 ? (u & 1) * TB : 0), vd = vb_lds + (u & 1) * TB;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) load_lds16(rk, dma_k ^ (k_swz<D>(RPL * i) * 16), 1024 * i, kd + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) load_lds16(rv, dma_v ^ (v_swz<D>(RPL * i) * 16), 1024 * i, vd + 1024 * i);
+    };
+
+    // This lane's row: column col of the wave's 32.
+    const int64_t r0 = (int64_t)rt * TR + 32 * rg;
+    const int nrows = (int)max((int64_t)0, min((int64_t)32, (int64_t)n * a.g - r0));
+    const int64_t row = r0 + min(col, max(nrows - 1, 0));
+    const int tok = min((int)(row / a.g), n - 1), head = kvh * a.g + (int)(row % a.g);
+    const int pos = len - n + tok;
+    const int wpos_lo = len - n + (int)(r0 / a.g);
+    const int wpos_hi = len - n + (int)((r0 + max(nrows, 1) - 1) / a.g);
+    const float c = fmaxf(a.scale * kLog2e, kMinScale);
+    bf16x8 q[DW / 16];
+    {
+        const uint16_t* qr = a.q + (int64_t)(first + tok) * a.ld_q + head * D + dh * DW + 8 * h;
+#pragma unroll
+        for (int i = 0; i < DW / 16; ++i) q[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qr + 16 * i));
+    }
+    f32x16 o[DW / 32];
+#pragma unroll
+    for (int d = 0; d < DW / 32; ++d) o[d] = f32x16{};
+    float m = kNoMax, l = 0.0f;
+    bool odd = false;  // a value of V that is no number, where some row may not see it
+
+    const int vrow = 4 * h + ((lane & 15) >> 2);
+    const uint32_t rd_k = col * (2 * D) + (h ^ k_swz<D>(col)) * 16;
+    const uint32_t rd_v = vrow * (2 * D) + ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_swz<D>(vrow)) * 16 + (lane & 1) * 8;
+
+    if (tid < 2) tags[tid] = -1;
+    __syncthreads();
+    if (u1 > u0) {
+        load_pages(u0);
+        issue(u0);
+    }
+#pragma unroll 1
+    for (int u = u0; u < u1; ++u) {
+        wait_vm<0>();
+        __syncthreads();
+        if (KB == 2 && u + 1 < u1) issue(u + 1);
+        const bool holes = tags[u & 1] == u;
+        const unsigned char* kt = kbuf + (KB == 2 ? (u & 1) * TB : 0);
+        const unsigned char* vt = vbuf + (u & 1) * TB;
+        const int pt = unit_pos(u);
+#pragma unroll 1
+        for (int sub = 0; sub < BN / 32; ++sub) {
+            const int p0 = pt + 32 * sub;
+            const bool skip = nrows == 0 || p0 > wpos_hi;
+            if (DS == 1 && skip) break;
+            f32x16 s{};
+            if (!skip) {
+                const unsigned char* ks = kt + sub * 64 * D;
+#pragma unroll
+                for (int i0 = 0; i0 < DW / 16; i0 += 4) {
+                    bf16x8 k[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        k[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
+                            ks + (rd_k ^ piece<D>(2 * (i0 + i))) + piece_far<D>((dh * DW + 16 * (i0 + i)) / 8 & ~15)));
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i], q[i0 + i], s, 0, 0, 0);
+                }
+            }
+            if constexpr (DS == 2) {
+                // The other half's products; the sum is the same in both waves.
+                f32x4* mine = reinterpret_cast<f32x4*>(xch + wave * 1024) + lane;
+                const f32x4* other = reinterpret_cast<const f32x4*>(xch + (wave ^ 1) * 1024) + lane;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mine[64 * i] = f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+                __syncthreads();
+                if (u + 1 < u1) issue(u + 1);
+                if (skip) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 x = other[64 * i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[4 * i + e] += x[e];
+                }
+            }
+            const bool masked = holes || p0 + 31 > wpos_lo ||
+                                (a.window > 0 && p0 <= wpos_hi - a.window && p0 + 31 >= a.sinks);
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int p = p0 + 8 * (i / 4) + 4 * h + i % 4;
+                    bool see = sees(a, p, pos);
+                    if (holes && see) see = page_of(a.b, seq, p) >= 0;
+                    if (!see) s[i] = -__builtin_inff();
+                }
+            }
+            float top = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+            if (__any(__builtin_fmaf(top, c, -m) > kSlack)) {
+                const uint32_t tb = __builtin_bit_cast(uint32_t, top);
+                auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
+                const uint32_t t0 = sw[0], t1 = sw[1];
+                const float mn = fmaxf(m, fmaxf(__builtin_bit_cast(float, t0), __builtin_bit_cast(float, t1)) * c);
+                const float fac = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= fac;
+#pragma unroll
+                for (int d = 0; d < DW / 32; ++d) o[d] *= fac;
+            }
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float si = s[i];
+                w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(si, c, -m));
+            }
+            l += (((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]))) +
+                 (((w[8] + w[9]) + (w[10] + w[11])) + ((w[12] + w[13]) + (w[14] + w[15])));
+            // Weights as bf16, the matrix cores' type (see the streaming kernel).
+            bf16x8 pw[2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pw[i >> 3][i & 7] = (__bf16)w[i];
+            const unsigned char* vs = vt + sub * 64 * D;
+            // Columns 32 d .. of this wave, positions 16 k + 8 e + 4 h .. + 3.
+            auto read_v = [&](int d, int k) __attribute__((always_inline)) {
+                const unsigned char* v = vs + (rd_v ^ piece<D>(4 * d)) + piece_far<D>((dh * DW + 32 * d) / 8 & ~15) + k * 32 * D;
+                const s16x4 lo = read_tr(v), hi = read_tr(v + 16 * D);
+                return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            if (masked) {
+#pragma unroll
+                for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) odd |= any_nonfinite(__builtin_bit_cast(u32x4, read_v(d, k)));
+                asm volatile("" ::: "memory");  // V is read again, not kept
+            }
+#pragma unroll
+            for (int d = 0; d < DW / 32; d += 2) {
+                bf16x8 v[2][2];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k >> 1][k & 1] = read_v(d + (k >> 1), k & 1);
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    o[d + (k & 1)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k & 1][k >> 1], pw[k >> 1], o[d + (k & 1)], 0, 0, 0);
+            }
+        }
+    }
+
+    float* part = a.part + ((int64_t)item * a.nsplit + split) * (TR * (D + 2));
+    if (__any(odd)) {  // see plain_row; with two waves per row, one does it
+        for (int r = 0; dh == 0 && r < nrows; ++r) {
+            const int64_t rr = r0 + r;
+            const int tk = (int)(rr / a.g), hd = kvh * a.g + (int)(rr % a.g);
+            float acc[D / 64], mr, lr;
+            plain_row<D>(a, seq, kvh, a.q + (int64_t)(first + tk) * a.ld_q + hd * D, len - n + tk, sp.us, sp.ulo, BN, u0, u1,
+                         lane, acc, mr, lr);
+            const float inv = inverse(lr);
+            uint16_t* dst = a.out + (int64_t)(first + tk) * a.ld_out + hd * D + D / 64 * lane;
+            float* pr = part + (32 * rg + r) * D + D / 64 * lane;
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) {
+                if (a.nsplit == 1)
+                    dst[e] = bf16_rne_bits(acc[e] * inv);
+                else
+                    pr[e] = acc[e];
+            }
+            if (a.nsplit > 1 && lane == 0) {
+                part[TR * D + 32 * rg + r] = mr;
+                part[TR * (D + 1) + 32 * rg + r] = lr;
+            }
+        }
+        return;
+    }
+    l += __shfl_xor(l, 32);
+    if (col >= nrows) return;
+    if (a.nsplit == 1) {
+        const float inv = inverse(l);
+        uint16_t* dst = a.out + (int64_t)(first + tok) * a.ld_out + head * D + dh * DW + 4 * h;
+#pragma unroll
+        for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                store4(dst + 32 * d + 8 * k, f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]}, inv);
+    } else {
+        float* dst = part + (32 * rg + col) * D + dh * DW + 4 * h;
+#pragma unroll
+        for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * k) =
+                    f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+        if (dh == 0 && h == 0) {
+            part[TR * D + 32 * rg + col] = m;
+            part[TR * (D + 1) + 32 * rg + col] = l;
+        }
+    }
+}
+
+// The splits of the tiles joined: a wave per (packed row, q head).
+template <int D>
+__global__ void __launch_bounds__(64) attn_paged_tile_merge_kernel(PagedAttnArgs a) {
+    constexpr int TR = tile_rows(D), BN = tile_bn(D), RW = D / 64;
+    const int lane = threadIdx.x, t = blockIdx.x, head = blockIdx.y;
+    int base = 0;
+    for (int b0 = 0; b0 < a.b.B; b0 += 64) {
+        const TileScan sc = tile_scan<TR>(a, b0, lane);
+        const uint64_t mine = __ballot(sc.tiles > 0 && sc.first <= t && t < sc.first + sc.n);
+        if (!mine) {
+            base += sc.sum;
+            continue;
+        }
+        const int l0 = __builtin_ctzll(mine);
+        const int first = __builtin_amdgcn_readlane(sc.first, l0), n = __builtin_amdgcn_readlane(sc.n, l0);
+        const int len = __builtin_amdgcn_readlane(sc.len, l0);
+        const bool ok = __builtin_amdgcn_readlane((int)sc.ok, l0) != 0;
+        const int kvh = head / a.g;
+        const int64_t row = (int64_t)(t - first) * a.g + (head - kvh * a.g);
+        const int rt = (int)(row / TR), r = (int)(row % TR);
+        const int gt = base + __builtin_amdgcn_readlane(sc.incl - sc.tiles, l0) + rt;
+        const TileSpan sp = tile_span<TR, BN>(a, n, len, ok, rt);
+        const float* part = a.part + ((int64_t)gt * a.kv_heads + kvh) * a.nsplit * (TR * (D + 2));
+        auto there = [&](int s) {
+            return (int)((int64_t)sp.nu * s / a.nsplit) < (int)((int64_t)sp.nu * (s + 1) / a.nsplit);
+        };
+        float mx = kNoMax;
+        for (int s = lane; s < a.nsplit; s += 64)
+            if (there(s)) mx = fmaxf(mx, part[(int64_t)s * (TR * (D + 2)) + TR * D + r]);
+        for (int k = 32; k; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
+        float acc[RW] = {}, ls = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < a.nsplit; ++s) {
+            if (!there(s)) continue;
+            const float* p = part + (int64_t)s * (TR * (D + 2));
+            const float fac = __builtin_amdgcn_exp2f(p[TR * D + r] - mx);
+            ls = __builtin_fmaf(p[TR * (D + 1) + r], fac, ls);
+            float v[RW];
+            __builtin_memcpy(v, p + r * D + RW * lane, sizeof(v));
+#pragma unroll
+            for (int e = 0; e < RW; ++e) acc[e] = __builtin_fmaf(v[e], fac, acc[e]);
+        }
+        const float inv = inverse(ls);
+        uint16_t* dst = a.out + (int64_t)t * a.ld_out + head * D + RW * lane;
+#pragma unroll
+        for (int e = 0; e < RW; ++e) dst[e] = bf16_rne_bits(acc[e] * inv);
+        return;
+    }
 }
 
 }  // namespace
@@ -646,21 +1065,38 @@ namespace {
 
 // How a call's work is spread.
 struct AttnPlan {
-    int qt;      // row tiles of 16 in the streaming kernel
-    int64_t row_limit;
-    int grid;
-    uint64_t part_bytes;
+    int qt;              // row tiles of 16 in the streaming kernel (0: not launched)
+    int64_t row_limit;   // sequences of at most this many rows are its, the others the tile kernel's
+    int grid;            // its workgroups
+    int64_t tiles;       // most tiles times kv heads of the tile kernel (0: not launched)
+    int nsplit;
+    uint64_t rows_bytes, part_bytes;
 };
 
 AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     AttnPlan p{};
     const int64_t g = heads / kv_heads;
-    const int64_t rows = (max_q > 0 ? std::min(max_q, T) : (T + B - 1) / B) * g;
     const int qt_max = D <= 128 ? 4 : (D == 256 ? 2 : 1);
-    p.qt = std::min(qt_max, rows <= 16 ? 1 : (rows <= 32 ? 2 : 4));
-    p.row_limit = INT64_MAX;
-    p.grid = device_cus();
-    p.part_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
+    const int64_t most = (max_q > 0 ? std::min(max_q, T) : T) * g;          // rows of a sequence at most
+    const int64_t rows = (max_q > 0 ? std::min(max_q, T) : (T + B - 1) / B) * g;  // as far as is known
+    const bool tiles = B == 1 ? most > 16 * qt_max : rows > 16 * qt_max;
+    const bool stream = !(B == 1 && tiles);
+    if (stream) {
+        const int64_t r = tiles ? g : rows;
+        p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
+        p.row_limit = tiles ? 16 * p.qt : INT64_MAX;
+        p.grid = device_cus();
+        p.rows_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
+    }
+    p.nsplit = 1;
+    p.part_bytes = p.rows_bytes;
+    if (tiles) {
+        const int tr = D == 512 ? tile_rows(512) : tile_rows(64);
+        p.tiles = (T * g / tr + std::min((int64_t)B, T * g / (p.row_limit + 1) + 1)) * kv_heads;
+        const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2);
+        p.nsplit = (int)std::max((int64_t)1, std::min((int64_t)64, slots / p.tiles));
+        if (p.nsplit > 1) p.part_bytes += (uint64_t)p.tiles * p.nsplit * tr * (D + 2) * sizeof(float);
+    }
     return p;
 }
 
@@ -678,11 +1114,32 @@ int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
 }
 
 template <int D>
-int launch_d(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
+int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
+    constexpr int lds = tile_lds(D);
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    const void* k = reinterpret_cast<const void*>(&attn_paged_tile_kernel<D>);
+    if (int rc = hip_check(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute"))
+        return rc;
+    hipLaunchKernelGGL((attn_paged_tile_kernel<D>), dim3((uint32_t)(p.tiles * p.nsplit)), dim3(64 * tile_waves(D)), lds, s, a);
+    if (int rc = hip_check(hipGetLastError(), "attn_paged_tile_kernel launch")) return rc;
+    if (p.nsplit == 1) return ALV_OK;
+    hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D>), dim3(a.b.T, a.heads), dim3(64), 0, s, a);
+    return hip_check(hipGetLastError(), "attn_paged_tile_merge_kernel launch");
+}
+
+template <int D>
+int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
+    float* part = a.part;
+    if (p.tiles) {
+        a.part = part + p.rows_bytes / sizeof(float);
+        if (int rc = launch_tiles<D>(a, p, s)) return rc;
+    }
+    a.part = part;
     if (p.qt == 1) return launch_rows<D, 1>(a, p, s);
     if constexpr (D <= 256)
         if (p.qt == 2) return launch_rows<D, 2>(a, p, s);
-    if constexpr (D <= 128) return launch_rows<D, 4>(a, p, s);
+    if constexpr (D <= 128)
+        if (p.qt == 4) return launch_rows<D, 4>(a, p, s);
     return ALV_OK;
 }
 
@@ -721,12 +1178,13 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
     a.heads = heads, a.kv_heads = kv_heads, a.g = heads / kv_heads, a.window = window, a.sinks = sinks, a.scale = scale;
     a.out = out, a.ld_out = ld_out;
     const AttnPlan p = attn_plan(heads, kv_heads, D, B, T, max_q);
-    if (!workspace || workspace_bytes < p.part_bytes)
+    if (p.part_bytes && (!workspace || workspace_bytes < p.part_bytes))
         return fail(ALV_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
                     (unsigned long long)p.part_bytes);
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(ALV_ERR_ALIGN, "workspace needs 16-byte alignment");
     a.part = static_cast<float*>(workspace);
     a.row_limit = p.row_limit;
+    a.nsplit = p.nsplit;
     const hipStream_t s = (hipStream_t)stream;
     switch (D) {
         case 64: return launch_d<64>(a, p, s);
