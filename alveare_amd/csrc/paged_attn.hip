@@ -679,13 +679,13 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
 // score's products, exchanged through LDS, and half of the output.
 // Where there are fewer tiles than compute units each tile's positions are split
 // and the parts joined by a second launch.
-constexpr int tile_ds(int D) { return D == 512 ? 2 : 1; }      // waves that share 32 rows
-constexpr int tile_waves(int D) { return D == 512 ? 8 : 4; }
+constexpr int tile_ds(int D) { return D >= 256 ? 2 : 1; }      // waves that share 32 rows
+constexpr int tile_waves(int D) { return D >= 256 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D) / tile_ds(D); }
 constexpr int tile_bn(int D) { return D <= 128 ? 64 : 32; }
-constexpr int tile_kbufs(int D) { return D == 512 ? 1 : 2; }
+constexpr int tile_kbufs(int D) { return D >= 256 ? 1 : 2; }
 constexpr int tile_bytes(int D) { return tile_bn(D) * 2 * D; }  // of K, of V
-constexpr int tile_xch(int D) { return D == 512 ? tile_waves(D) * 4096 : 0; }
+constexpr int tile_xch(int D) { return D >= 256 ? tile_waves(D) * 4096 : 0; }
 constexpr int tile_lds(int D) { return (tile_kbufs(D) + 2) * tile_bytes(D) + tile_xch(D) + 16; }
 
 typedef float f32x16 __attribute__((__vector_size__(16 * sizeof(float))));
@@ -1093,7 +1093,7 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     if (tiles) {
         const int tr = D == 512 ? tile_rows(512) : tile_rows(64);
         p.tiles = (T * g / tr + std::min((int64_t)B, T * g / (p.row_limit + 1) + 1)) * kv_heads;
-        const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2);
+        const int64_t slots = (int64_t)device_cus() * (D >= 256 ? 1 : 2);
         p.nsplit = (int)std::max((int64_t)1, std::min((int64_t)64, slots / p.tiles));
         if (p.nsplit > 1) p.part_bytes += (uint64_t)p.tiles * p.nsplit * tr * (D + 2) * sizeof(float);
     }
