@@ -35,6 +35,8 @@ struct SampleArgs {
     int shift;  // fixed-point bits of a weight
     int32_t* token;
     float* prob;
+    unsigned char* work;
+    int pieces;  // of a row; 0: a row is one workgroup's
 };
 
 struct RowParams {
@@ -70,11 +72,37 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+// exp(-x), x >= 0: with n = rint(x / ln 2) and y = n ln 2 - x, |y| <= 0.347, it
+// is 2^-n times the Taylor sum of exp(y) to y^12 / 12! (the rest is below 2^-52).
+// The float64 library function, exact to the last bit, takes twice as long.
+__device__ __forceinline__ double exp_neg(double x) {
+    const double n = rint(x * 1.4426950408889634);
+    const double y = fma(n, 0.6931471805599453, -x);
+    double p = 1.0 / 479001600.0;
+    p = fma(p, y, 1.0 / 39916800.0);
+    p = fma(p, y, 1.0 / 3628800.0);
+    p = fma(p, y, 1.0 / 362880.0);
+    p = fma(p, y, 1.0 / 40320.0);
+    p = fma(p, y, 1.0 / 5040.0);
+    p = fma(p, y, 1.0 / 720.0);
+    p = fma(p, y, 1.0 / 120.0);
+    p = fma(p, y, 1.0 / 24.0);
+    p = fma(p, y, 1.0 / 6.0);
+    p = fma(p, y, 0.5);
+    p = fma(p, y, 1.0);
+    p = fma(p, y, 1.0);
+    return x < 700.0 ? __builtin_ldexp(p, -(int)n) : 0.0;
+}
 // exp((l - m) / T): 1 for l = m also where both are infinite.
 __device__ __forceinline__ double weight(float l, float m, double inv_t) {
-    return l == m ? 1.0 : exp(((double)l - (double)m) * inv_t);
+    return l == m ? 1.0 : exp_neg(((double)m - (double)l) * inv_t);
 }
 __device__ __forceinline__ uint64_t fixed(double w, double scale) { return (uint64_t)rint(w * scale); }
+
+// Targets of the three crossings. top-p keeps what begins below ceil(p S); a
+// token is drawn at floor(u Z).
+__device__ __forceinline__ uint64_t topp_target(double p, uint64_t S) { return max((uint64_t)1, (uint64_t)ceil(p * (double)S)); }
+__device__ __forceinline__ uint64_t draw_target(double u, uint64_t Z) { return min((uint64_t)(u * (double)Z), Z - 1); }
 
 constexpr int kRowThreads = 1024;
 constexpr int kBins = 2048;
@@ -147,12 +175,10 @@ __device__ Pick pick(const float* l, int V, float m, double inv_t, double scale,
     return p;
 }
 
-// One workgroup per row, any values.
-__global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a) {
-    __shared__ RowShared s;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
+// A row by one workgroup from the logits alone, whatever their values.
+__device__ void sample_row(const SampleArgs& a, int b, const RowParams& rp, RowShared& s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* l = a.logits + b * a.ld;
-    const RowParams rp = row_params(a, b);
     // The largest logit and its first index; a NaN counts as largest.
     float m = -__builtin_inff();
     int mi = a.V;
@@ -203,21 +229,26 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a) {
     __syncthreads();
     uint64_t Z = S;
     auto own_weight = [&](uint32_t key) { return fixed(weight(logit_of(key), m, rp.inv_t), scale); };
-    if (rp.topk < a.V) {
-        const Pick p = pick(l, a.V, m, rp.inv_t, scale, true, (uint64_t)rp.topk - 1, s);
-        Z = p.sum + (uint64_t)(rp.topk - (int)p.cnt) * own_weight(p.key);
-    }
-    if (rp.topp < 1.0) {
-        const uint64_t target = max((uint64_t)1, (uint64_t)ceil(rp.topp * (double)Z));
-        if (target < Z) {
-            const Pick p = pick(l, a.V, m, rp.inv_t, scale, false, target - 1, s);
-            const uint64_t w = own_weight(p.key);
-            Z = min(Z, p.sum + ((target - 1 - p.sum) / w + 1) * w);
+    Pick p{};
+    uint64_t x = 0;
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {  // top-k, top-p, the draw
+        if (step == 0) {
+            if (rp.topk >= a.V) continue;
+            x = (uint64_t)rp.topk - 1;
+        } else if (step == 1) {
+            const uint64_t target = topp_target(rp.topp, Z);
+            if (rp.topp >= 1.0 || target >= Z) continue;
+            x = target - 1;
+        } else {
+            Z = min(Z, Sm);
+            x = draw_target(rp.u, Z);
         }
+        p = pick(l, a.V, m, rp.inv_t, scale, step == 0, x, s);
+        const uint64_t w = own_weight(p.key);
+        if (step == 0) Z = p.sum + (uint64_t)(rp.topk - (int)p.cnt) * w;
+        if (step == 1) Z = min(Z, p.sum + ((x - p.sum) / w + 1) * w);
     }
-    Z = min(Z, Sm);
-    const uint64_t x = min((uint64_t)(rp.u * (double)Z), Z - 1);
-    const Pick p = pick(l, a.V, m, rp.inv_t, scale, false, x, s);
     const uint64_t w = own_weight(p.key);
     int skip = (int)((x - p.sum) / w);  // equal logits ahead of the token, by index
     // The token: the skip-th with that value.
@@ -242,13 +273,628 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a) {
     }
 }
 
+// ---- several workgroups per row -----------------------------------------------------
+//
+// Five launches: the pieces' largest logits; a histogram of each piece over x =
+// (l_0 - l) / T, from 0 to where a weight rounds to nothing (or the row's range);
+// the row's sum of them, which tells the bins in which the three crossings can
+// fall; the collection of those bins' tokens; the crossings among those, by
+// comparison where they are few, else by a finer histogram first. Every step
+// moves integers, so no order of atomics shows. A row whose bins hold too many
+// (logits all alike but for a few far ones) is done by sample_row.
+//
+// What bounds it: one row is a chain of launches, each a trip or two to memory;
+// many rows, the float64 exponentials (two per logit's weight, 12 terms).
+constexpr int kPieceThreads = 256;
+constexpr int kWaves = kPieceThreads / 64;
+constexpr int kPiece = 16 * kPieceThreads;  // logits per workgroup
+constexpr int kCoarse = 1024;     // bins
+constexpr int kFine = 2048;       // finer bins of the collected ones
+constexpr int kCand = 4096;       // tokens collected per row
+constexpr int kLast = 128;        // tokens compared one with another (256 take 30 us, 128 in the finer histogram 9)
+
+struct RowWork {  // per row
+    float* top;         // [pieces] largest logit
+    float* low;         // [pieces] smallest logit above -infinity
+    int* at;            // [pieces] first index of the largest
+    unsigned long long* minp;   // [pieces] weight that min-p keeps
+    unsigned long long* sum;    // [kCoarse] weight of each bin, then its prefix [kCoarse + 1]
+    uint32_t* cnt;              // [kCoarse] count of each bin, then its prefix [kCoarse + 1]
+    unsigned long long* cw;     // [kCand] collected weights,
+    float* cl;          // logits,
+    float* cp;          // places in the histogram
+    int* ci;            // and indices
+    uint32_t* want;     // [kCoarse / 32] a bit per bin to collect
+    uint32_t* n;        // collected; kCand + 1 and above: too many
+};
+
+__host__ __device__ inline uint64_t up16(uint64_t v) { return (v + 15) & ~(uint64_t)15; }
+__host__ __device__ inline uint64_t row_bytes(int pieces) {
+    return up16(8ull * (pieces + 2 * kCoarse + 1 + kCand) + 4ull * (3ull * pieces + 2 * kCoarse + 1 + 3 * kCand + kCoarse / 32 + 1));
+}
+__device__ __forceinline__ RowWork row_work(const SampleArgs& a, int b) {
+    RowWork w;
+    unsigned char* p = a.work + (uint64_t)b * row_bytes(a.pieces);
+    w.sum = reinterpret_cast<unsigned long long*>(p);
+    w.cw = w.sum + 2 * kCoarse + 1;
+    w.minp = w.cw + kCand;
+    w.cnt = reinterpret_cast<uint32_t*>(w.minp + a.pieces);
+    w.cl = reinterpret_cast<float*>(w.cnt + 2 * kCoarse + 1);
+    w.cp = w.cl + kCand;
+    w.ci = reinterpret_cast<int*>(w.cp + kCand);
+    w.want = reinterpret_cast<uint32_t*>(w.ci + kCand);
+    w.n = w.want + kCoarse / 32;
+    w.top = reinterpret_cast<float*>(w.n + 1);
+    w.low = w.top + a.pieces;
+    w.at = reinterpret_cast<int*>(w.low + a.pieces);
+    return w;
+}
+
+// (value, index) a before b in numpy's argmax order: NaN first, then the larger,
+// then the lower index.
+__device__ __forceinline__ bool ahead(float va, int ia, float vb, int ib) {
+    const bool na = va != va, nb = vb != vb;
+    if (na != nb) return na;
+    return va > vb || ((va == vb || na) && ia < ib);
+}
+
+// This thread's 16 logits of the piece, in 4 groups of 4 (index i0 + 4 kPieceThreads
+// g + e); -infinity past the row.
+__device__ __forceinline__ void load_piece(const float* l, int V, int base, int tid, float (&v)[16]) {
+    if ((reinterpret_cast<uintptr_t>(l) & 15) == 0 && base + kPiece <= V) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 f = *reinterpret_cast<const float4*>(l + base + 4 * kPieceThreads * g + 4 * tid);
+            v[4 * g] = f.x, v[4 * g + 1] = f.y, v[4 * g + 2] = f.z, v[4 * g + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = base + 4 * kPieceThreads * g + 4 * tid + e;
+                v[4 * g + e] = i < V ? l[i] : -__builtin_inff();
+            }
+    }
+}
+__device__ __forceinline__ int piece_index(int base, int tid, int k) {
+    return base + 4 * kPieceThreads * (k >> 2) + 4 * tid + (k & 3);
+}
+
+__global__ void __launch_bounds__(kPieceThreads) sample_top_kernel(SampleArgs a) {
+    __shared__ float st[kWaves], sl[kWaves];
+    __shared__ int si[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.y, base = blockIdx.x * kPiece;
+    const RowWork rw = row_work(a, b);
+    float v[16];
+    load_piece(a.logits + b * a.ld, a.V, base, tid, v);
+    float m = v[0], lo = __builtin_inff();
+    int mi = piece_index(base, tid, 0);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        if (k && ahead(v[k], piece_index(base, tid, k), m, mi)) m = v[k], mi = piece_index(base, tid, k);
+        if (v[k] > -__builtin_inff()) lo = fminf(lo, v[k]);
+    }
+    for (int o = 32; o; o >>= 1) {
+        const float u = __shfl_xor(m, o);
+        const int ui = __shfl_xor(mi, o);
+        if (ahead(u, ui, m, mi)) m = u, mi = ui;
+        lo = fminf(lo, __shfl_xor(lo, o));
+    }
+    if (lane == 0) st[wave] = m, si[wave] = mi, sl[wave] = lo;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kWaves; ++w) {
+            if (ahead(st[w], si[w], m, mi)) m = st[w], mi = si[w];
+            lo = fminf(lo, sl[w]);
+        }
+        rw.top[blockIdx.x] = m;
+        rw.at[blockIdx.x] = mi;
+        rw.low[blockIdx.x] = lo;
+    }
+    // The row's histogram, clear for the next launch.
+    for (int i = blockIdx.x * kPieceThreads + tid; i < kCoarse; i += a.pieces * kPieceThreads) {
+        rw.cnt[i] = 0;
+        rw.sum[i] = 0;
+    }
+}
+
+// What a row's largest and smallest logits decide.
+struct RowRange {
+    float m;
+    int at;
+    bool done;      // the token is `at` (or there is none)
+    float bins;     // bins per unit of x
+    float end;      // x from which a weight is nothing
+};
+__device__ __forceinline__ RowRange row_range(const SampleArgs& a, const RowWork& rw, const RowParams& rp, int lane) {
+    float m = -__builtin_inff(), lo = __builtin_inff();
+    int at = 0x7FFFFFFF;
+    for (int i = lane; i < a.pieces; i += 64) {
+        if (ahead(rw.top[i], rw.at[i], m, at)) m = rw.top[i], at = rw.at[i];
+        lo = fminf(lo, rw.low[i]);
+    }
+    for (int o = 32; o; o >>= 1) {
+        const float u = __shfl_xor(m, o);
+        const int ui = __shfl_xor(at, o);
+        if (ahead(u, ui, m, at)) m = u, at = ui;
+        lo = fminf(lo, __shfl_xor(lo, o));
+    }
+    RowRange r;
+    r.m = m;
+    r.at = at;
+    r.done = m != m || m == -__builtin_inff() || rp.topk == 1;
+    r.end = (float)(a.shift + 1) * 0.693147182464599609375f;
+    const float range = (float)(((double)m - (double)lo) * rp.inv_t);
+    r.bins = (float)kCoarse / fmaxf(fminf(range, r.end), 1e-30f);  // NaN range (infinities): the whole
+    return r;
+}
+// x in bins, from 0; a value of kCoarse or more in the last. The same for equal
+// logits and never smaller for a smaller one.
+__device__ __forceinline__ double x_of(float l, const RowRange& r, double inv_t) {
+    return l == r.m ? 0.0 : ((double)r.m - (double)l) * inv_t;
+}
+__device__ __forceinline__ float place_of(double x, const RowRange& r) { return fminf((float)x * r.bins, (float)kCoarse - 0.00390625f); }
+
+__global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(SampleArgs a) {
+    __shared__ uint32_t cnt[kCoarse];
+    __shared__ unsigned long long sum[kCoarse];
+    __shared__ unsigned long long smin[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.y, base = blockIdx.x * kPiece;
+    const RowWork rw = row_work(a, b);
+    float v[16];
+    load_piece(a.logits + b * a.ld, a.V, base, tid, v);
+    const RowParams rp = row_params(a, b);
+    const RowRange rr = row_range(a, rw, rp, lane);
+    if (rr.done) return;
+    for (int i = tid; i < kCoarse; i += kPieceThreads) {
+        cnt[i] = 0;
+        sum[i] = 0;
+    }
+    __syncthreads();
+    const double scale = __builtin_ldexp(1.0, a.shift);
+    uint64_t kept = 0;
+#pragma unroll 4
+    for (int k = 0; k < 16; ++k) {
+        const double x = x_of(v[k], rr, rp.inv_t);
+        if (!(x < rr.end)) continue;
+        const double w = exp_neg(x);
+        const uint64_t f = fixed(w, scale);
+        if (w >= rp.minp) kept += f;
+        const int bin = (int)place_of(x, rr);
+        atomicAdd(&cnt[bin], 1u);
+        atomicAdd(&sum[bin], (unsigned long long)f);
+    }
+    for (int o = 32; o; o >>= 1) kept += __shfl_xor((unsigned long long)kept, o);
+    if (lane == 0) smin[wave] = kept;
+    __syncthreads();
+    for (int i = tid; i < kCoarse; i += kPieceThreads) {
+        // (added up here rather than kept per piece: reading 64 pieces'
+        // histograms takes one workgroup 30 us)
+        if (cnt[i]) {
+            atomicAdd(rw.cnt + i, cnt[i]);
+            atomicAdd(rw.sum + i, sum[i]);
+        }
+    }
+    if (tid == 0) {
+        kept = 0;
+        for (int i = 0; i < kWaves; ++i) kept += smin[i];
+        rw.minp[blockIdx.x] = kept;
+    }
+}
+
+// One workgroup per row, a bin per thread: the row's histogram and its prefix,
+// and the bins in which the crossings can fall.
+__global__ void __launch_bounds__(kCoarse) sample_plan_kernel(SampleArgs a) {
+    constexpr int NW = kCoarse / 64;
+    __shared__ unsigned long long wsum[NW], pre[kCoarse + 1];
+    __shared__ uint32_t wcnt[NW], prec[kCoarse + 1];
+    __shared__ int hit;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
+    const RowWork rw = row_work(a, b);
+    const RowParams rp = row_params(a, b);
+    const RowRange rr = row_range(a, rw, rp, lane);
+    if (rr.done) return;
+    uint32_t c = rw.cnt[tid];
+    uint64_t w = rw.sum[tid], Sm = 0;
+    for (int g = lane; g < a.pieces; g += 64) Sm += rw.minp[g];
+    for (int o = 32; o; o >>= 1) Sm += __shfl_xor((unsigned long long)Sm, o);
+    const uint32_t c0 = c;
+    const uint64_t w0 = w;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t cu = __shfl_up(c, o);
+        const uint64_t wu = __shfl_up((unsigned long long)w, o);
+        if (lane >= o) c += cu, w += wu;
+    }
+    if (lane == 63) wcnt[wave] = c, wsum[wave] = w;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) c += wcnt[i], w += wsum[i];
+    prec[tid + 1] = c;
+    pre[tid + 1] = w;
+    if (tid == 0) prec[0] = 0, pre[0] = 0;
+    const uint32_t cb = c - c0;
+    const uint64_t wb = w - w0;
+    __syncthreads();
+    const uint64_t S = pre[kCoarse];
+    bool want = false;
+    // The bin in which a count or a sum of x crosses.
+    auto bin_at = [&](bool by_count, uint64_t x) {
+        __syncthreads();
+        if (by_count ? (cb <= x && x < c) : (wb <= x && x < w)) hit = tid;
+        __syncthreads();
+        return hit;
+    };
+    uint64_t lo = S, hi = S;  // between what the sum of the kept lies
+    if ((uint32_t)rp.topk < prec[kCoarse]) {
+        const int t = bin_at(true, (uint64_t)rp.topk - 1);
+        lo = pre[t];
+        hi = pre[t + 1];
+        want = tid == t;
+    }
+    if (rp.topp < 1.0) {
+        const uint64_t p0 = topp_target(rp.topp, lo), p1 = topp_target(rp.topp, hi);
+        const int t0 = bin_at(false, p0 - 1), t1 = p1 == p0 ? t0 : bin_at(false, p1 - 1);
+        want |= tid >= t0 && tid <= t1;
+        lo = min(lo, (uint64_t)pre[t0]);
+        hi = min(hi, (uint64_t)pre[t1 + 1]);
+    }
+    lo = max(min(lo, Sm), (uint64_t)1);
+    hi = max(min(hi, Sm), (uint64_t)1);
+    const int d0 = bin_at(false, draw_target(rp.u, lo)), d1 = lo == hi ? d0 : bin_at(false, draw_target(rp.u, hi));
+    want |= tid >= d0 && tid <= d1;
+    const uint64_t bits = __ballot(want);
+    uint32_t total = want ? c0 : 0;
+    for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
+    __syncthreads();
+    if (lane == 0) {
+        wcnt[wave] = total;
+        rw.want[2 * wave] = (uint32_t)bits;
+        rw.want[2 * wave + 1] = (uint32_t)(bits >> 32);
+    }
+    rw.cnt[kCoarse + tid] = cb;
+    rw.sum[kCoarse + tid] = wb;
+    __syncthreads();
+    if (tid == 0) {
+        rw.cnt[2 * kCoarse] = prec[kCoarse];
+        rw.sum[2 * kCoarse] = S;
+        total = 0;
+        for (int i = 0; i < NW; ++i) total += wcnt[i];
+        *rw.n = total > kCand ? kCand + 1 : 0;
+    }
+}
+
+__global__ void __launch_bounds__(kPieceThreads) sample_collect_kernel(SampleArgs a) {
+    __shared__ uint32_t want[kCoarse / 32];
+    __shared__ uint32_t found, at0;
+    const int tid = threadIdx.x, lane = tid & 63, b = blockIdx.y, base = blockIdx.x * kPiece;
+    const RowWork rw = row_work(a, b);
+    float v[16];
+    load_piece(a.logits + b * a.ld, a.V, base, tid, v);
+    const RowParams rp = row_params(a, b);
+    const RowRange rr = row_range(a, rw, rp, lane);
+    if (rr.done || *rw.n > kCand) return;  // (while others add to it, n stays at kCand or below)
+    if (tid < kCoarse / 32) want[tid] = rw.want[tid];
+    if (tid == 0) found = 0;
+    __syncthreads();
+    uint32_t mine = 0, mask = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const double x = x_of(v[k], rr, rp.inv_t);
+        if (!(x < rr.end)) continue;
+        const int bin = (int)place_of(x, rr);
+        if (want[bin >> 5] >> (bin & 31) & 1) mask |= 1u << k, ++mine;
+    }
+    uint32_t at = mine ? atomicAdd(&found, mine) : 0;
+    __syncthreads();
+    if (tid == 0) at0 = found ? atomicAdd(rw.n, found) : 0;
+    __syncthreads();
+    at += at0;
+    const double scale = __builtin_ldexp(1.0, a.shift);
+#pragma unroll 1
+    for (int k = 0; __any(mask >> k); ++k) {
+        if (!(mask >> k & 1)) continue;
+        float l = v[0];
+#pragma unroll
+        for (int q = 1; q < 16; ++q) l = q == k ? v[q] : l;
+        rw.cl[at] = l;
+        rw.cp[at] = place_of(x_of(l, rr, rp.inv_t), rr);
+        rw.cw[at] = fixed(weight(l, rr.m, rp.inv_t), scale);
+        rw.ci[at] = piece_index(base, tid, k);
+        ++at;
+    }
+}
+
+constexpr int kPer = kCand / kRowThreads;  // collected tokens of a thread
+struct LastShared {
+    // the collected bins, each cut into kFine / (their number) fine ones
+    uint32_t cnt[kFine], pcnt[kFine];
+    unsigned long long sum[kFine], psum[kFine];
+    uint32_t base_cnt[kCoarse];            // by collected bin: what comes before it
+    unsigned long long base_sum[kCoarse];
+    uint32_t want[kCoarse / 32];
+    unsigned long long wsum[kRowThreads / 64];
+    uint32_t wcnt[kRowThreads / 64];
+    // the tokens of one fine bin
+    float el[kLast];
+    int ei[kLast];
+    unsigned long long ew[kLast];
+    int ne, f;
+    uint32_t before_cnt;
+    unsigned long long before_sum;
+    // the token found, and the weight up to and with it
+    float rl;
+    int ri;
+    unsigned long long through;
+};
+union SampleShared {
+    RowShared row;
+    LastShared last;
+};
+
+// A thread's collected tokens, and its two fine bins.
+struct LastRegs {
+    float l[kPer];
+    int i[kPer], f[kPer];
+    unsigned long long w[kPer];
+    uint32_t cb[2], c[2];
+    unsigned long long wb[2], ws[2];
+};
+
+// The token at which the running count or weight crosses x; false where a fine
+// bin holds too many to compare.
+__device__ bool cross(const LastRegs& r, bool by_count, uint64_t x, LastShared& s) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int e = 0; e < kFine / kRowThreads; ++e) {
+        const uint64_t b = by_count ? r.cb[e] : r.wb[e], own = by_count ? r.c[e] : r.ws[e];
+        if (b <= x && x < b + own) s.f = tid * (kFine / kRowThreads) + e, s.before_cnt = r.cb[e], s.before_sum = r.wb[e];
+    }
+    if (tid == 0) s.ne = 0;
+    __syncthreads();
+    const int f = s.f;
+    if (s.cnt[f] > kLast) return false;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        if (r.f[q] != f) continue;
+        const int e = atomicAdd(&s.ne, 1);
+        s.el[e] = r.l[q];
+        s.ei[e] = r.i[q];
+        s.ew[e] = r.w[q];
+    }
+    __syncthreads();
+    const int ne = s.ne;
+    if (tid < ne) {
+        uint64_t before = by_count ? s.before_cnt : s.before_sum, bsum = s.before_sum;
+        const float l = s.el[tid];
+        const int id = s.ei[tid];
+#pragma unroll 8
+        for (int e = 0; e < ne; ++e) {
+            const float le = s.el[e];
+            const int ie = s.ei[e];
+            const uint64_t we = s.ew[e];
+            const bool first = (le > l) | ((le == l) & (ie < id));
+            before += first ? (by_count ? 1 : we) : 0;
+            bsum += first ? we : 0;
+        }
+        const uint64_t mine = by_count ? 1 : s.ew[tid];
+        if (before <= x && x < before + mine) s.rl = l, s.ri = id, s.through = bsum + s.ew[tid];
+    }
+    __syncthreads();
+    return true;
+}
+
+// The token from what was collected; false where that is too much.
+__device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const RowWork rw = row_work(a, b);
+    const RowRange rr = row_range(a, rw, rp, lane);
+    if (rr.done) {
+        if (tid == 0) {
+            const bool none = rr.m == -__builtin_inff();
+            a.token[b] = none ? -1 : rr.at;
+            if (a.prob) a.prob[b] = rr.m != rr.m ? rr.m : (none ? 0.0f : 1.0f);
+        }
+        return true;
+    }
+    const uint32_t n = *rw.n;
+    const uint32_t all = rw.cnt[2 * kCoarse];
+    uint64_t Z = rw.sum[2 * kCoarse], Sm = 0;
+    for (int g = lane; g < a.pieces; g += 64) Sm += rw.minp[g];
+    if (n > kCand) return false;
+    const double scale = __builtin_ldexp(1.0, a.shift);
+    for (int o = 32; o; o >>= 1) Sm += __shfl_xor((unsigned long long)Sm, o);
+    const bool cut = (uint32_t)rp.topk < all;
+    if (n <= kLast) {
+        // Few: each token's place among all, hence what comes before it, at once.
+        const uint32_t* cnt = rw.cnt + kCoarse;
+        const unsigned long long* sum = rw.sum + kCoarse;
+        uint32_t bc = 0;
+        uint64_t bs = 0, own = 0;
+        float l = 0.0f;
+        int id = 0, bin = 0;
+        if (tid < (int)n) {
+            l = rw.cl[tid];
+            id = rw.ci[tid];
+            bin = (int)rw.cp[tid];
+            own = rw.cw[tid];
+            s.el[tid] = l;
+            s.ei[tid] = id;
+            s.ew[tid] = own;
+            s.cnt[tid] = bin;
+            bc = cnt[bin];
+            bs = sum[bin];
+        }
+        __syncthreads();
+        if (tid < (int)n)
+#pragma unroll 8
+            for (int e = 0; e < (int)n; ++e) {
+                const float le = s.el[e];
+                const int ie = s.ei[e];
+                const bool first = ((int)s.cnt[e] == bin) & ((le > l) | ((le == l) & (ie < id)));
+                const uint64_t we = s.ew[e];
+                bc += first ? 1 : 0;
+                bs += first ? we : 0;
+            }
+        if (cut) {
+            if (tid < (int)n && bc == (uint32_t)rp.topk - 1) s.through = bs + own;
+            __syncthreads();
+            Z = s.through;
+        }
+        if (rp.topp < 1.0) {
+            const uint64_t target = topp_target(rp.topp, Z);
+            if (target < Z) {
+                __syncthreads();
+                if (tid < (int)n && bs < target && target <= bs + own) s.through = bs + own;
+                __syncthreads();
+                Z = min(Z, (uint64_t)s.through);
+            }
+        }
+        Z = min(Z, Sm);
+        const uint64_t x = draw_target(rp.u, Z);
+        if (tid < (int)n && bs <= x && x < bs + own) {
+            a.token[b] = id;
+            if (a.prob) a.prob[b] = (float)(weight(l, rr.m, rp.inv_t) / ((double)Z / scale));
+        }
+        return true;
+    }
+    LastRegs r;
+    float place[kPer];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int e = tid + q * kRowThreads;
+        place[q] = -1.0f;
+        r.w[q] = 0;
+        if (e < (int)n) {
+            place[q] = rw.cp[e];
+            r.w[q] = rw.cw[e];
+            r.l[q] = rw.cl[e];
+            r.i[q] = rw.ci[e];
+        }
+    }
+    const uint32_t bc = rw.cnt[kCoarse + tid];
+    const uint64_t bs = rw.sum[kCoarse + tid];
+    if (tid < kCoarse / 32) s.want[tid] = rw.want[tid];
+#pragma unroll
+    for (int e = 0; e < kFine / kRowThreads; ++e) {
+        s.cnt[tid + e * kRowThreads] = 0;
+        s.sum[tid + e * kRowThreads] = 0;
+    }
+    __syncthreads();
+    // The place of each collected bin among them.
+    auto rank = [&](int bin) {
+        int k = __popc(s.want[bin >> 5] & ((1u << (bin & 31)) - 1));
+        for (int i = 0; i < (bin >> 5); ++i) k += __popc(s.want[i]);
+        return k;
+    };
+    int slots = 0;
+    for (int i = 0; i < kCoarse / 32; ++i) slots += __popc(s.want[i]);
+    const int F = kFine / slots;
+    if (s.want[tid >> 5] >> (tid & 31) & 1) {
+        const int k = rank(tid);
+        s.base_cnt[k] = bc;
+        s.base_sum[k] = bs;
+    }
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        r.f[q] = -1;
+        if (place[q] < 0.0f) continue;
+        const int bin = (int)place[q];
+        r.f[q] = rank(bin) * F + min((int)((place[q] - (float)bin) * (float)F), F - 1);
+        atomicAdd(&s.cnt[r.f[q]], 1u);
+        atomicAdd(&s.sum[r.f[q]], r.w[q]);
+    }
+    __syncthreads();
+    {
+        constexpr int E = kFine / kRowThreads;
+        uint32_t c = 0;
+        uint64_t w = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            r.c[e] = s.cnt[E * tid + e];
+            r.ws[e] = s.sum[E * tid + e];
+            c += r.c[e];
+            w += r.ws[e];
+        }
+        const uint32_t c0 = c;
+        const uint64_t w0 = w;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t cu = __shfl_up(c, o);
+            const uint64_t wu = __shfl_up((unsigned long long)w, o);
+            if (lane >= o) c += cu, w += wu;
+        }
+        if (lane == 63) s.wcnt[tid >> 6] = c, s.wsum[tid >> 6] = w;
+        __syncthreads();
+        c -= c0;
+        w -= w0;
+        for (int i = 0; i < (tid >> 6); ++i) c += s.wcnt[i], w += s.wsum[i];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            s.pcnt[E * tid + e] = r.cb[e] = c;
+            s.psum[E * tid + e] = r.wb[e] = w;
+            c += r.c[e];
+            w += r.ws[e];
+        }
+        __syncthreads();
+        // From the sum over the collected bins to the one over the row's.
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int k = (E * tid + e) / F;
+            if (k >= slots) continue;  // (holds nothing)
+            r.cb[e] += s.base_cnt[k] - s.pcnt[k * F];
+            r.wb[e] += s.base_sum[k] - s.psum[k * F];
+        }
+    }
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {  // top-k, top-p, the draw
+        uint64_t x;
+        if (step == 0) {
+            if (!cut) continue;
+            x = (uint64_t)rp.topk - 1;
+        } else if (step == 1) {
+            const uint64_t target = topp_target(rp.topp, Z);
+            if (rp.topp >= 1.0 || target >= Z) continue;
+            x = target - 1;
+        } else {
+            Z = min(Z, Sm);
+            x = draw_target(rp.u, Z);
+        }
+        if (!cross(r, step == 0, x, s)) return false;
+        if (step < 2) Z = min(Z, (uint64_t)s.through);
+    }
+    if (tid == 0) {
+        a.token[b] = s.ri;
+        if (a.prob) a.prob[b] = (float)(weight(s.rl, rr.m, rp.inv_t) / ((double)Z / scale));
+    }
+    return true;
+}
+
+// One workgroup per row: the token.
+__global__ void __launch_bounds__(kRowThreads) sample_last_kernel(SampleArgs a) {
+    __shared__ SampleShared sh;
+    const int b = blockIdx.x;
+    const RowParams rp = row_params(a, b);
+    if (a.pieces > 0 && sample_collected(a, b, rp, sh.last)) return;
+    __syncthreads();
+    sample_row(a, b, rp, sh.row);
+}
 }  // namespace
 
 }  // namespace alv
 
 using namespace alv;
 
-extern "C" uint64_t alv_sample_workspace(int B, int V) { return 0; }
+namespace alv {
+namespace {
+// Short rows are one workgroup's work.
+int sample_pieces(int V) { return V <= 4096 ? 0 : (V + kPiece - 1) / kPiece; }
+}  // namespace
+}  // namespace alv
+
+extern "C" uint64_t alv_sample_workspace(int B, int V) {
+    if (B < 1 || V < 1) return 0;
+    const int pieces = sample_pieces(V);
+    return pieces ? (uint64_t)B * row_bytes(pieces) : 0;
+}
 
 extern "C" int alv_sample(const float* logits, int64_t ld, int B, int V, const float* u, const float* temperature_dev,
                           float temperature, const int32_t* top_k_dev, int top_k, const float* top_p_dev, float top_p,
@@ -257,7 +903,8 @@ extern "C" int alv_sample(const float* logits, int64_t ld, int B, int V, const f
     if (B < 0 || V < 1 || ld < V) return fail(ALV_ERR_ARG, "bad logits shape B=%d vocab=%d ld=%lld", B, V, (long long)ld);
     if (B == 0) return ALV_OK;
     if (!logits || !u || !token) return fail(ALV_ERR_ARG, "null pointer");
-    if (V > 1 << 24 || B > 1 << 16) return fail(ALV_ERR_RANGE, "%d rows of %d logits (at most 65536 of 2^24)", B, V);
+    if (V > 1 << 24 || B > 65535 || (int64_t)B * sample_pieces(V) > 1 << 23)
+        return fail(ALV_ERR_RANGE, "%d rows of %d logits (at most 65535 rows, 2^24 logits in one, 2^35 in all)", B, V);
     for (const void* p : {(const void*)logits, (const void*)u, (const void*)temperature_dev, (const void*)top_k_dev,
                           (const void*)top_p_dev, (const void*)min_p_dev, (const void*)token, (const void*)prob})
         if (reinterpret_cast<uintptr_t>(p) % 4) return fail(ALV_ERR_ALIGN, "logits, parameters and outputs need 4-byte alignment");
@@ -269,6 +916,21 @@ extern "C" int alv_sample(const float* logits, int64_t ld, int B, int V, const f
     while ((1 << bits) < V) ++bits;
     a.shift = std::min(52, 62 - bits);
     a.token = token, a.prob = prob;
-    hipLaunchKernelGGL(sample_row_kernel, dim3(B), dim3(kRowThreads), 0, (hipStream_t)stream, a);
-    return hip_check(hipGetLastError(), "sample_row_kernel launch");
+    a.pieces = sample_pieces(V);
+    const uint64_t need = alv_sample_workspace(B, V);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(ALV_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
+                    (unsigned long long)need);
+    if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(ALV_ERR_ALIGN, "workspace needs 16-byte alignment");
+    a.work = static_cast<unsigned char*>(workspace);
+    const hipStream_t st = (hipStream_t)stream;
+    if (a.pieces) {
+        const dim3 grid(a.pieces, B);
+        hipLaunchKernelGGL(sample_top_kernel, grid, dim3(kPieceThreads), 0, st, a);
+        hipLaunchKernelGGL(sample_hist_kernel, grid, dim3(kPieceThreads), 0, st, a);
+        hipLaunchKernelGGL(sample_plan_kernel, dim3(B), dim3(kCoarse), 0, st, a);
+        hipLaunchKernelGGL(sample_collect_kernel, grid, dim3(kPieceThreads), 0, st, a);
+    }
+    hipLaunchKernelGGL(sample_last_kernel, dim3(B), dim3(kRowThreads), 0, st, a);
+    return hip_check(hipGetLastError(), "sample kernels' launch");
 }

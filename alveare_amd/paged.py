@@ -22,7 +22,7 @@ may be given up by writing -1 there).
 """
 from __future__ import annotations
 
-import ctypes
+import array
 import heapq
 
 import numpy as np
@@ -33,32 +33,32 @@ from .layer import _GEMMA_EPS, _f32, _ptr
 from .ops import _need_gpu, _on, _stream, _workspace
 
 
-def _rows(t: torch.Tensor, name: str, width: int, dev: torch.device) -> torch.Tensor:
-    """A (T, >= width) bfloat16 tensor, contiguous along its rows."""
+def _rows(t: torch.Tensor, name: str, width: int, dev: torch.device) -> int:
+    """Checks a (T, >= width) bfloat16 tensor, contiguous along its rows; returns how far apart they are."""
     if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 2 or t.device != dev:
         raise TypeError(f"{name} must be a 2-D bfloat16 tensor on {dev}")
-    if t.shape[1] < width or t.shape[1] > 1 and t.stride(1) != 1:
+    (T, w), (ld, one) = t.shape, t.stride()
+    if w < width or one != 1 and w > 1:
         raise ValueError(f"{name} rows must be contiguous and hold {width} values, got shape {tuple(t.shape)} "
                          f"strides {t.stride()}")
-    return t
+    return ld if T > 1 else w
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _page_stride(t: torch.Tensor, name: str, dev: torch.device) -> int:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 4 or t.device != dev:
+        raise TypeError(f"{name} must be a (pages, kv_heads, page_size, D) bfloat16 tensor on {dev}")
+    (n, H, S, D), (s0, s1, s2, s3) = t.shape, t.stride()
+    if s3 != 1 or s2 != D or s1 != S * D and H > 1:
+        raise ValueError(f"{name}: each page must be contiguous, got strides {t.stride()}")
+    return s0 if n > 1 else H * S * D
 
 
 def _pages(kpages: torch.Tensor, vpages: torch.Tensor, dev: torch.device):
-    """(pages, kv_heads, S, D, page strides) of the two pools: each page contiguous in itself."""
-    for t, name in ((kpages, "kpages"), (vpages, "vpages")):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 4 or t.device != dev:
-            raise TypeError(f"{name} must be a (pages, kv_heads, page_size, D) bfloat16 tensor on {dev}")
-        _, H, S, D = t.shape
-        if t.stride(3) != 1 or t.stride(2) != D or H > 1 and t.stride(1) != S * D:
-            raise ValueError(f"{name}: each page must be contiguous, got strides {t.stride()}")
+    """(shape, page strides) of the two pools: each page contiguous in itself."""
+    ks, vs = _page_stride(kpages, "kpages", dev), _page_stride(vpages, "vpages", dev)
     if kpages.shape != vpages.shape:
         raise ValueError(f"kpages and vpages differ: {tuple(kpages.shape)} and {tuple(vpages.shape)}")
-    n, H, S, D = kpages.shape
-    return n, H, S, D, *(t.stride(0) if n > 1 else H * S * D for t in (kpages, vpages))
+    return kpages.shape, ks, vs
 
 
 def _batch(page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, dev: torch.device):
@@ -66,7 +66,7 @@ def _batch(page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor
     for t, name, dim in ((page_table, "page_table", 2), (q_start, "q_start", 1), (kv_len, "kv_len", 1)):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or t.device != dev:
             raise TypeError(f"{name} must be a {dim}-D int32 tensor on {dev}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
             raise ValueError(f"{name} must be contiguous along its rows")
     B, W = page_table.shape
     if kv_len.shape[0] != B or q_start.shape[0] != B + 1:
@@ -87,27 +87,28 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
     left as they are in ``q_out``, zeros for a sequence that does not fit its
     table (or the rope table)."""
     dev = _need_gpu(qkv)
-    pages, kv_heads, S, D, ks, vs = _pages(kpages, vpages, dev)
+    (pages, kv_heads, S, D), ks, vs = _pages(kpages, vpages, dev)
     B, W, ldt = _batch(page_table, q_start, kv_len, dev)
-    _rows(qkv, "qkv", (k_off if v_off < 0 else v_off) + kv_heads * D, dev)
-    T = qkv.shape[0]
+    ldqkv = _rows(qkv, "qkv", (k_off if v_off < 0 else v_off) + kv_heads * D, dev)
+    T, ldq = qkv.shape[0], heads * D
     q_w, k_w = _f32(q_w, "q_w", D, dev), _f32(k_w, "k_w", D, dev)
     rope_rows = ldr = 0
     if rope is not None:
-        _rows(rope, "rope", 2, dev)
-        rope_rows, ldr = rope.shape[0], _ld(rope)
+        rope_rows, ldr = rope.shape[0], _rows(rope, "rope", 2, dev)
         half = rope.shape[1] // 2 if half is None else half
         sin_off = half if sin_off is None else sin_off
     if q_out is None:
-        q_out = torch.empty(T, heads * D, dtype=torch.bfloat16, device=dev)
-    elif _rows(q_out, "q_out", heads * D, dev).shape[0] < T:
-        raise ValueError(f"q_out has {q_out.shape[0]} rows, qkv {T}")
+        q_out = torch.empty((T, ldq), dtype=torch.bfloat16, device=dev)
+    else:
+        ldq = _rows(q_out, "q_out", ldq, dev)
+        if q_out.shape[0] < T:
+            raise ValueError(f"q_out has {q_out.shape[0]} rows, qkv {T}")
     with _on(dev):
-        check(lib().alv_qkv_post_paged(qkv.data_ptr(), _ld(qkv), k_off, v_off, heads, kv_heads, D, _ptr(q_w), _ptr(k_w),
+        check(lib().alv_qkv_post_paged(qkv.data_ptr(), ldqkv, k_off, v_off, heads, kv_heads, D, _ptr(q_w), _ptr(k_w),
                                        norm_q, norm_k, norm_v, eps, _ptr(rope), rope_rows, ldr, cos_off, sin_off or 0,
                                        half or 0, page_table.data_ptr(), ldt, W, q_start.data_ptr(), kv_len.data_ptr(),
                                        B, T, pages, S, kpages.data_ptr(), vpages.data_ptr(), ks, vs, q_out.data_ptr(),
-                                       _ld(q_out), _stream(qkv)), "alv_qkv_post_paged")
+                                       ldq, _stream(qkv)), "alv_qkv_post_paged")
     return q_out
 
 
@@ -121,38 +122,38 @@ def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     sequence owns, where the caller knows it, lets the call choose how to spread
     the work (1 for a decode step); it does not change what is computed."""
     dev = _need_gpu(q)
-    pages, kv_heads, S, D, ks, vs = _pages(kpages, vpages, dev)
+    (pages, kv_heads, S, D), ks, vs = _pages(kpages, vpages, dev)
     B, W, ldt = _batch(page_table, q_start, kv_len, dev)
-    _rows(q, "q", heads * D, dev)
-    T = q.shape[0]
+    ldq = _rows(q, "q", heads * D, dev)
+    T, ldo = q.shape[0], heads * D
     if out is None:
-        out = torch.empty(T, heads * D, dtype=torch.bfloat16, device=dev)
-    elif _rows(out, "out", heads * D, dev).shape[0] < T:
-        raise ValueError(f"out has {out.shape[0]} rows, q {T}")
+        out = torch.empty((T, ldo), dtype=torch.bfloat16, device=dev)
+    else:
+        ldo = _rows(out, "out", ldo, dev)
+        if out.shape[0] < T:
+            raise ValueError(f"out has {out.shape[0]} rows, q {T}")
     L = lib()
     with _on(dev):
         ws = _workspace(L.alv_attention_paged_workspace(heads, kv_heads, D, B, T, max_q), dev)
-        check(L.alv_attention_paged(q.data_ptr(), _ld(q), kpages.data_ptr(), vpages.data_ptr(), ks, vs, pages, S,
+        check(L.alv_attention_paged(q.data_ptr(), ldq, kpages.data_ptr(), vpages.data_ptr(), ks, vs, pages, S,
                                     page_table.data_ptr(), ldt, W, q_start.data_ptr(), kv_len.data_ptr(), B, T, max_q,
-                                    heads, kv_heads, D, window, sinks, scale, out.data_ptr(), _ld(out), *ws[1:],
+                                    heads, kv_heads, D, window, sinks, scale, out.data_ptr(), ldo, *ws[1:],
                                     _stream(q)), "alv_attention_paged")
     return out
 
 
-def _host_i32(v, name: str) -> np.ndarray:
+def _host_i32(v, name: str) -> array.array:
     """Page numbers as a host int32 array."""
-    if isinstance(v, torch.Tensor):
-        if v.device.type != "cpu":
-            raise ValueError(f"{name} must be on the host: it is checked before anything is copied")
-        v = v.numpy()
-    a = np.asarray(v)
-    if a.size == 0:
-        return np.empty(0, np.int32)
-    if a.dtype.kind not in "iu" or a.ndim != 1:
-        raise TypeError(f"{name} must be a sequence of integers, got {a.dtype} of {a.ndim} dimensions")
-    if a.min() < 0 or a.max() > 0x7FFFFFFF:
-        raise ValueError(f"{name} holds page numbers out of range")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    if isinstance(v, torch.Tensor) and v.device.type != "cpu":
+        raise ValueError(f"{name} must be on the host: it is checked before anything is copied")
+    if isinstance(v, (torch.Tensor, np.ndarray)):
+        v = v.tolist()
+    try:
+        return array.array("i", v)
+    except OverflowError as e:
+        raise ValueError(f"{name} holds page numbers out of range") from e
+    except TypeError as e:
+        raise TypeError(f"{name} must be a sequence of integers: {e}") from e
 
 
 def copy_pages(caches, src, dst) -> None:
@@ -164,24 +165,28 @@ def copy_pages(caches, src, dst) -> None:
     if not caches:
         return
     first = caches[0]
-    dev = _need_gpu(*caches)
-    shape, strides, esize = first.shape, first.stride(), first.element_size()
-    if first.dim() < 2 or first.numel() == 0:
+    dev = _need_gpu(first)
+    shape, strides, dtype = first.shape, first.stride(), first.dtype
+    if len(shape) < 2 or first.numel() == 0:
         raise ValueError(f"a cache must be (pages, ...), got shape {tuple(shape)}")
     for t in caches:
-        if t.shape != shape or t.stride() != strides or t.dtype != first.dtype:
-            raise ValueError(f"the caches differ: {t.dtype} {tuple(t.shape)} {t.stride()} and {first.dtype} "
+        if not isinstance(t, torch.Tensor) or t.device != dev:
+            raise ValueError(f"the caches must be tensors on one GPU, {dev}")
+        if t.shape != shape or t.stride() != strides or t.dtype != dtype:
+            raise ValueError(f"the caches differ: {t.dtype} {tuple(t.shape)} {t.stride()} and {dtype} "
                              f"{tuple(shape)} {strides}")
-    if not first[0].is_contiguous():
+    page = first[0]
+    if not page.is_contiguous():
         raise ValueError(f"each page must be contiguous, got strides {strides}")
     src, dst = _host_i32(src, "src"), _host_i32(dst, "dst")
     if len(src) != len(dst):
         raise ValueError(f"{len(src)} sources and {len(dst)} destinations")
-    n = first[0].numel() * esize
-    ptrs = (ctypes.c_void_p * len(caches))(*[t.data_ptr() for t in caches])
+    n, esize = page.numel() * first.element_size(), first.element_size()
+    ptrs = array.array("Q", [t.data_ptr() for t in caches])
     with _on(dev):
-        check(lib().alv_copy_pages(ptrs, len(caches), n, strides[0] * esize if shape[0] > 1 else n, shape[0],
-                                   src.ctypes.data, dst.ctypes.data, len(src), _stream(first)), "alv_copy_pages")
+        check(lib().alv_copy_pages(ptrs.buffer_info()[0], len(caches), n, strides[0] * esize if shape[0] > 1 else n,
+                                   shape[0], src.buffer_info()[0], dst.buffer_info()[0], len(src), _stream(first)),
+              "alv_copy_pages")
 
 
 class PagedCache:

@@ -519,7 +519,7 @@ int alv_copy_pages(void* const* caches, int ncaches, int64_t page_bytes, int64_t
  * as 1. u outside [0, 1) counts as the nearest number inside. A row with a NaN
  * gives its first NaN's index and probability NaN (alv_lm_head's argmax); a row
  * of nothing but -infinity gives -1 and 0; +infinities share the weight.
- * B <= 65536, V <= 2^24. workspace as for alv_attention_paged.
+ * B <= 65535, V <= 2^24, B * V <= 2^35. workspace as for alv_attention_paged.
  */
 uint64_t alv_sample_workspace(int B, int V);
 int alv_sample(const float* logits, int64_t ld, int B, int V, const float* u, const float* temperature_dev,
