@@ -42,60 +42,171 @@ struct PostPagedArgs {
     int64_t k_stride, v_stride;
 };
 
+// One workgroup per packed row (token). Eight lanes per 128 columns (per head of
+// 64), so a wave takes 2 to 8 heads at once: that is the layout in which numpy's
+// order of a row's sum of squares (row_norm.h: eight interleaved accumulators
+// per 128 values) needs no step on fewer lanes. A lane loads and stores 16-byte
+// octets; the float rows in LDS turn octets into accumulators' columns and bring
+// a rotated pair's other half.
+//
+// What bounds it: one token, three dependent trips to memory (the sequence, its
+// page and RoPE row, the stores); many, the bytes. 16 + 2 x 8 heads of 256: 4939
+// tokens, a wave per head and two-byte accesses 86 us.
 constexpr int kPostMaxWaves = 8;
+constexpr int kLeafPad = 8;  // floats: leaves then start eight banks apart
 
-// One workgroup per packed row (token); a wave takes one head row at a time.
 template <int D>
-__global__ void __launch_bounds__(64 * kPostMaxWaves) qkv_post_paged_kernel(PostPagedArgs a) {
-    constexpr int RW = D / 64;
-    __shared__ __align__(16) float rows[kPostMaxWaves][D];
+struct PostGeom {
+    static constexpr int Leaf = D < 128 ? D : 128, Leaves = D / Leaf;
+    static constexpr int Lanes = 8 * Leaves;      // of a head
+    static constexpr int Heads = 64 / Lanes;      // of a wave
+    static constexpr int Oct = Leaf / 64;         // octets of a lane
+    static constexpr int Row = Leaves * (Leaf + kLeafPad);  // floats of a head in LDS
+    // Float of a head's row that holds column c.
+    static __device__ __forceinline__ int at(int c) { return c + (c / Leaf) * kLeafPad; }
+};
+
+// WIDE: every row 16-byte aligned, a rotated half whole octets.
+template <int D, bool WIDE>
+__global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post_paged_kernel(PostPagedArgs a) {
+    using G = PostGeom<D>;
+    __shared__ __align__(16) float rows[kPostMaxWaves][G::Heads * G::Row];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = blockDim.x >> 6;
     const int t = blockIdx.x;
+    const int total = a.heads + 2 * a.kv_heads;
+    const int hw = lane / G::Lanes, hl = lane % G::Lanes;  // head of the wave, lane of the head
+    float* row = rows[wave] + hw * G::Row;
+    const uint16_t* xt = a.qkv + (int64_t)t * a.ld_qkv;
+
+    struct Head {
+        int role, h;
+        bool in;
+        const uint16_t* x;
+        const float* w;
+    };
+    auto head = [&](int r0) {
+        Head d;
+        const int r = r0 * G::Heads + hw;
+        d.in = r < total;
+        const int rc = d.in ? r : total - 1;
+        d.role = rc < a.heads ? 0 : (rc < a.heads + a.kv_heads ? 1 : 2);
+        d.h = d.role == 0 ? rc : (d.role == 1 ? rc - a.heads : rc - a.heads - a.kv_heads);
+        d.x = xt + (d.role == 0 ? 0 : (d.role == 1 || a.v_off < 0 ? a.k_off : a.v_off)) + d.h * D;
+        d.w = d.role == 0 ? a.q_w : (d.role == 1 ? a.k_w : nullptr);
+        return d;
+    };
+    // Octet e of a lane: columns 8 (hl + Lanes e).
+    auto load_x = [&](const Head& d, uint4 (&x)[G::Oct]) {
+#pragma unroll
+        for (int e = 0; e < G::Oct; ++e) {
+            const uint16_t* p = d.x + 8 * (hl + G::Lanes * e);
+            if constexpr (WIDE)
+                x[e] = *reinterpret_cast<const uint4*>(p);
+            else
+                __builtin_memcpy(&x[e], p, sizeof(x[e]));
+        }
+    };
+    Head d = head(wave);
+    uint4 x[G::Oct];
+    load_x(d, x);  // on its way while the sequence is looked up
     const SeqRows sr = find_row(a.b, t, lane);
     if (sr.seq < 0) return;
     const int pos = sr.len - sr.n + (t - sr.first);
     const bool ok = sr.ok && pos < a.rope_rows;
     const int page = ok ? page_of(a.b, sr.seq, pos) : -1;
     const int slot = pos & ((1 << a.b.shift) - 1);
-    const int total = a.heads + 2 * a.kv_heads;
-    float* row = rows[wave];
-    for (int r = wave; r < total; r += nw) {
-        const int role = r < a.heads ? 0 : (r < a.heads + a.kv_heads ? 1 : 2);
-        const int h = role == 0 ? r : (role == 1 ? r - a.heads : r - a.heads - a.kv_heads);
-        if (role && page < 0) continue;
-        uint16_t* dst = role == 0 ? a.q_out + (int64_t)t * a.ld_q + h * D
-                                  : (role == 1 ? a.kpages + page * a.k_stride : a.vpages + page * a.v_stride) +
-                                        (((int64_t)h << a.b.shift) + slot) * D;
-        if (!ok) {
-            for (int e = 0; e < RW; ++e) dst[RW * lane + e] = 0;
-            continue;
+    const uint16_t* rr = ok && a.rope ? a.rope + pos * a.rope_stride : nullptr;
+
+    for (int r0 = wave; r0 * G::Heads < total; r0 += nw) {
+        if (r0 != wave) {
+            d = head(r0);
+            load_x(d, x);
         }
-        const int src = role == 0 ? h * D : (role == 1 || a.v_off < 0 ? a.k_off + h * D : a.v_off + h * D);
-        const uint16_t* x = a.qkv + (int64_t)t * a.ld_qkv + src;
-        const int norm = role == 0 ? a.norm_q : (role == 1 ? a.norm_k : a.norm_v);
-        const float* w = role == 0 ? a.q_w : (role == 1 ? a.k_w : nullptr);
-        for (int e = 0; e < RW; ++e) row[RW * lane + e] = bf16_bits_to_f32(x[RW * lane + e]);
-        if (norm) {
-            const float inv = rms_inv_wave(row, D, a.eps, lane);
-            for (int e = 0; e < RW; ++e) {
-                const int d = RW * lane + e;
-                const float v = mul_rn(row[d], inv);
-                row[d] = bf16r(w ? mul_rn(v, w[d]) : v);
+        float f[G::Oct][8];
+        const int norm = d.role == 0 ? a.norm_q : (d.role == 1 ? a.norm_k : a.norm_v);
+#pragma unroll
+        for (int e = 0; e < G::Oct; ++e) {
+            unpack8(x[e], f[e]);
+            float4* p = reinterpret_cast<float4*>(row + G::at(8 * (hl + G::Lanes * e)));
+            p[0] = float4{f[e][0], f[e][1], f[e][2], f[e][3]};
+            p[1] = float4{f[e][4], f[e][5], f[e][6], f[e][7]};
+        }
+        // Leaf hl / 8 by its eight lanes, then the leaves in the recursion's tree.
+        float sum = leaf8_sq_n<G::Leaf / 8>(row + (hl >> 3) * (G::Leaf + kLeafPad), hl & 7);
+        if (G::Leaves > 1) sum = add_rn(sum, dpp_f<0x140>(sum));
+        if (G::Leaves > 2) sum = add_rn(sum, __shfl_xor(sum, 16));
+        const float inv = __fdiv_rn(1.0f, sqrtf(add_rn(__fdiv_rn(sum, (float)D), a.eps)));
+        const bool rot = d.role < 2 && rr;
+#pragma unroll
+        for (int e = 0; e < G::Oct; ++e) {
+            const int c0 = 8 * (hl + G::Lanes * e);
+            if (norm) {
+                float w[8];
+                load_w8(d.w, c0 / 8, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = mul_rn(f[e][i], inv);
+                    f[e][i] = bf16r(d.w ? mul_rn(v, w[i]) : v);
+                }
+            }
+            if (rr) {  // the whole wave: a head's rows hold what its pairs read
+                float4* p = reinterpret_cast<float4*>(row + G::at(c0));
+                p[0] = float4{f[e][0], f[e][1], f[e][2], f[e][3]};
+                p[1] = float4{f[e][4], f[e][5], f[e][6], f[e][7]};
             }
         }
-        const uint16_t* rr = role < 2 && a.rope ? a.rope + pos * a.rope_stride : nullptr;
-        for (int e = 0; e < RW; ++e) {
-            const int d = RW * lane + e;
-            float y = row[d];
-            if (rr && d < 2 * a.half) {
-                const int i = d < a.half ? d : d - a.half;
-                const float c = bf16_bits_to_f32(rr[a.cos_off + i]), s = bf16_bits_to_f32(rr[a.sin_off + i]);
-                y = d < a.half ? sub_rn(mul_rn(row[i], c), mul_rn(row[i + a.half], s))
-                               : add_rn(mul_rn(row[d], c), mul_rn(row[i], s));
+        uint16_t* dst = d.role == 0 ? a.q_out + (int64_t)t * a.ld_q + d.h * D
+                                    : (d.role == 1 ? a.kpages + max(page, 0) * a.k_stride : a.vpages + max(page, 0) * a.v_stride) +
+                                          (((int64_t)d.h << a.b.shift) + slot) * D;
+        const bool put = d.in && (d.role == 0 || page >= 0);
+#pragma unroll
+        for (int e = 0; e < G::Oct; ++e) {
+            const int c0 = 8 * (hl + G::Lanes * e);
+            uint16_t out[8];
+            if (rot && c0 < 2 * a.half) {
+                // run_rope_cpu_gemma (model.py:549-575): y1 = x1 c - x2 s, y2 = x2 c + x1 s.
+                if constexpr (WIDE) {
+                    const bool low = c0 < a.half;
+                    const int i0 = low ? c0 : c0 - a.half;
+                    const float4* op = reinterpret_cast<const float4*>(row + G::at(low ? c0 + a.half : i0));
+                    const float4 o0 = op[0], o1 = op[1];
+                    const float o[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
+                    float cr[8], sn[8];
+                    unpack8(*reinterpret_cast<const uint4*>(rr + a.cos_off + i0), cr);
+                    unpack8(*reinterpret_cast<const uint4*>(rr + a.sin_off + i0), sn);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float xc = mul_rn(f[e][i], cr[i]), os = mul_rn(o[i], sn[i]);
+                        out[i] = bf16_rne_bits(low ? sub_rn(xc, os) : add_rn(xc, os));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int c = c0 + i, k = c < a.half ? c : c - a.half;
+                        float y = f[e][i];
+                        if (c < 2 * a.half) {
+                            const float xc = mul_rn(y, bf16_bits_to_f32(rr[a.cos_off + k]));
+                            const float os = mul_rn(row[G::at(c < a.half ? c + a.half : k)], bf16_bits_to_f32(rr[a.sin_off + k]));
+                            y = c < a.half ? sub_rn(xc, os) : add_rn(xc, os);
+                        }
+                        out[i] = bf16_rne_bits(y);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) out[i] = bf16_rne_bits(f[e][i]);
             }
-            dst[d] = bf16_rne_bits(y);
+            if (!ok)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) out[i] = 0;
+            if (!put) continue;
+            const uint4 o8 = pack8(out);
+            if constexpr (WIDE)
+                *reinterpret_cast<uint4*>(dst + c0) = o8;
+            else
+                __builtin_memcpy(dst + c0, &o8, sizeof(o8));
         }
     }
 }
@@ -158,16 +269,25 @@ extern "C" int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off
     a.rope = rope, a.rope_stride = rope_stride, a.cos_off = cos_off, a.sin_off = sin_off, a.half = half;
     a.q_out = q_out, a.ld_q = ld_q, a.kpages = kpages, a.vpages = vpages, a.k_stride = k_stride, a.v_stride = v_stride;
     a.rope_rows = rope ? rope_rows : INT_MAX;
-    const int threads = 64 * std::min(kPostMaxWaves, heads + 2 * kv_heads);
+    auto rows16 = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
+    const bool wide = rows16(qkv, ld_qkv) && rows16(q_out, ld_q) && rows16(kpages, k_stride) && rows16(vpages, v_stride) &&
+             k_off % 8 == 0 && (v_off < 0 || v_off % 8 == 0) &&
+                      (!rope || (rows16(rope, rope_stride) && cos_off % 8 == 0 && sin_off % 8 == 0 && half % 8 == 0));
+    if (reinterpret_cast<uintptr_t>(qkv) % 2 || reinterpret_cast<uintptr_t>(q_out) % 2 || reinterpret_cast<uintptr_t>(rope) % 2 ||
+        reinterpret_cast<uintptr_t>(kpages) % 2 || reinterpret_cast<uintptr_t>(vpages) % 2 ||
+        reinterpret_cast<uintptr_t>(q_w) % 16 || reinterpret_cast<uintptr_t>(k_w) % 16)
+        return fail(ALV_ERR_ALIGN, "q_w and k_w need 16-byte alignment, the bf16 arrays 2-byte");
+    const int per_wave = D <= 128 ? 8 : 1024 / D;  // heads
+    const int threads = 64 * std::min(kPostMaxWaves, (heads + 2 * kv_heads + per_wave - 1) / per_wave);
     auto go = [&](auto k) {
         hipLaunchKernelGGL(k, dim3(T), dim3(threads), 0, (hipStream_t)stream, a);
         return hip_check(hipGetLastError(), "qkv_post_paged_kernel launch");
     };
     switch (D) {
-        case 64: return go(qkv_post_paged_kernel<64>);
-        case 128: return go(qkv_post_paged_kernel<128>);
-        case 256: return go(qkv_post_paged_kernel<256>);
-        default: return go(qkv_post_paged_kernel<512>);
+        case 64: return wide ? go(qkv_post_paged_kernel<64, true>) : go(qkv_post_paged_kernel<64, false>);
+        case 128: return wide ? go(qkv_post_paged_kernel<128, true>) : go(qkv_post_paged_kernel<128, false>);
+        case 256: return wide ? go(qkv_post_paged_kernel<256, true>) : go(qkv_post_paged_kernel<256, false>);
+        default: return wide ? go(qkv_post_paged_kernel<512, true>) : go(qkv_post_paged_kernel<512, false>);
     }
 }
 

@@ -75,6 +75,12 @@ def _batch(page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor
     return B, W, page_table.stride(0) if B > 1 else W
 
 
+def _weights(w, name: str, n: int, dev: torch.device) -> torch.Tensor | None:
+    """Norm weights on a 16-byte boundary."""
+    w = _f32(w, name, n, dev)
+    return w.clone() if w is not None and w.data_ptr() & 15 else w
+
+
 def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
                    q_start: torch.Tensor, kv_len: torch.Tensor, *, heads: int, k_off: int, v_off: int, q_w=None,
                    k_w=None, norm_q: bool = True, norm_k: bool = True, norm_v: bool = True, eps: float = _GEMMA_EPS,
@@ -91,7 +97,7 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
     B, W, ldt = _batch(page_table, q_start, kv_len, dev)
     ldqkv = _rows(qkv, "qkv", (k_off if v_off < 0 else v_off) + kv_heads * D, dev)
     T, ldq = qkv.shape[0], heads * D
-    q_w, k_w = _f32(q_w, "q_w", D, dev), _f32(k_w, "k_w", D, dev)
+    q_w, k_w = _weights(q_w, "q_w", D, dev), _weights(k_w, "k_w", D, dev)
     rope_rows = ldr = 0
     if rope is not None:
         rope_rows, ldr = rope.shape[0], _rows(rope, "rope", 2, dev)

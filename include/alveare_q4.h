@@ -457,8 +457,8 @@ int alv_embed(const uint16_t* table_f16, int vocab, int H, const int32_t* token_
  * included, is alv_qkv_post's: each value has the bits that a step of one token
  * writes. rope holds rope_rows rows, rope_stride apart (NULL: no rotation); a
  * sequence longer than that counts as one longer than its table for the rows
- * past it. D one of 64, 128, 256, 512. Two sequences must not insert into the
- * same slot.
+ * past it. D one of 64, 128, 256, 512; q_w and k_w 16-byte aligned. Two sequences
+ * must not insert into the same slot.
  */
 int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off, int heads, int kv_heads, int D,
                        const float* q_w, const float* k_w, int norm_q, int norm_k, int norm_v, float eps,
