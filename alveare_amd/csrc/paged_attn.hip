@@ -1,5 +1,6 @@
 // Attention of the newest tokens of a batch of sequences over a paged KV cache.
 #include <algorithm>
+#include <atomic>
 
 #include "paged.h"
 #include "q4_device.h"
@@ -230,7 +231,7 @@ struct RowsSeq {
     int us, ulo, nu;  // units of first tokens; first unit of the window; units in all
 };
 
-constexpr int rows_waves(int D) { return D == 512 ? 2 : 4; }
+constexpr int rows_waves(int D) { return D == 512 ? 2 : (D == 64 ? 8 : 4); }
 constexpr int rows_stage(int D) { return 64 * D; }  // bytes of 16 positions' K and V
 constexpr int rows_stages(int D) { return 131072 / (rows_waves(D) * rows_stage(D)); }
 constexpr int rows_unit(int D) { return 16 * rows_waves(D); }
@@ -250,11 +251,14 @@ constexpr int rows_mls(int D, int QT) {  // where the waves' maxima and sums sta
 // Floats of one workspace place: outputs, maxima, sums.
 constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
 
+constexpr int kPartsPerTile = 64;
+
 struct Scan {
     RowsSeq s;          // this lane's sequence
     uint64_t incl;      // work of the sequences of this step up to and with this lane's
     uint64_t base, sum; // work before this step; of this step
     int b0;             // the step's first sequence
+    uint32_t tiles;     // of the whole batch, no more than 2^31 (scan_all)
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -307,11 +311,15 @@ template <int ROWS, int UNIT>
 __device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, Scan& sc) {
     scan_step<ROWS, UNIT>(a, 0, lane, 0, sc);
     uint64_t total = sc.sum;
+    uint32_t tiles = sc.s.nu ? min(sc.s.tiles, kPartsPerTile) : 0;
     for (int b0 = 64; b0 < a.b.B; b0 += 64) {
         Scan t;
         scan_step<ROWS, UNIT>(a, b0, lane, 0, t);
         total += t.sum;
+        tiles = min(tiles + (t.s.nu ? min(t.s.tiles, kPartsPerTile) : 0), 1u << 24);
     }
+    for (int k = 32; k; k >>= 1) tiles += __shfl_xor(tiles, k);
+    sc.tiles = uniform(min(tiles, 1u << 24) * (uint32_t)min(a.kv_heads, 64));
     return total;
 }
 
@@ -353,8 +361,10 @@ __device__ __forceinline__ uint64_t part_begin(uint64_t total, uint32_t parts, u
     const uint64_t q = total / parts, r = total - q * parts;
     return q * w + min((uint64_t)w, r);
 }
-__device__ __forceinline__ uint32_t part_count(uint64_t total, int grid) {
-    return (uint32_t)min((uint64_t)grid, total);
+// At most kPartsPerTile parts per tile on average: the merge reads them all (one
+// token over 8000 positions on one kv head of 512: 250 parts 117 us, 125 40, 64 XX).
+__device__ __forceinline__ uint32_t part_count(uint64_t total, const Scan& sc, int grid) {
+    return (uint32_t)min((uint64_t)min((uint32_t)grid, sc.tiles * kPartsPerTile), total);
 }
 
 template <int D, int QT>
@@ -370,7 +380,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
     const int col = lane & 15, G = lane >> 4;
     Scan sc;
     const uint64_t total = scan_all<ROWS, UNIT>(a, lane, sc);
-    const uint32_t parts = part_count(total, gridDim.x);
+    const uint32_t parts = part_count(total, sc, gridDim.x);
     if (blockIdx.x >= parts) return;
     uint64_t x = part_begin(total, parts, blockIdx.x);
     const uint64_t end = part_begin(total, parts, blockIdx.x + 1);
@@ -628,6 +638,43 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
     }
 }
 
+// acc, l of n parts rescaled to the largest maximum and added in order, by one
+// wave: the maxima and sums 64 parts at a time, a part per lane (ml(v) points to
+// part v's maximum, its sum `gap` floats behind), then eight parts' outputs (o(v)
+// points to this lane's) on their way at once.
+template <int RW, class ML, class O>
+__device__ __forceinline__ void join_parts(int n, int lane, ML ml, int gap, O o, float (&acc)[RW], float& mx, float& l) {
+    for (int v0 = 0; v0 < n; v0 += 64) {
+        const int c = min(64, n - v0);
+        float m = kNoMax, s = 0.0f;
+        if (lane < c) {
+            const float* p = ml(v0 + lane);
+            m = p[0];
+            s = p[gap];
+        }
+        float top = m;
+        for (int k = 32; k; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
+        const float mn = fmaxf(mx, top), old = __builtin_amdgcn_exp2f(mx - mn);
+        mx = mn;
+        const float fac = lane < c ? __builtin_amdgcn_exp2f(m - mn) : 0.0f;
+        l *= old;
+#pragma unroll
+        for (int e = 0; e < RW; ++e) acc[e] *= old;
+        for (int q0 = 0; q0 < c; q0 += 8) {
+            float t[8][RW];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) __builtin_memcpy(t[q], o(v0 + min(q0 + q, c - 1)), sizeof(t[q]));
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float f = q0 + q < c ? lane_f(fac, min(q0 + q, c - 1)) : 0.0f;
+                l = __builtin_fmaf(lane_f(s, min(q0 + q, c - 1)), f, l);
+#pragma unroll
+                for (int e = 0; e < RW; ++e) acc[e] = q0 + q < c ? __builtin_fmaf(t[q][e], f, acc[e]) : acc[e];
+            }
+        }
+    }
+}
+
 // The cut tiles: wave (boundary, row) joins the parts of the tile in which
 // boundary blockIdx.x + 1 is the first, in the order of the line.
 template <int D, int QT>
@@ -637,7 +684,7 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
     const int r = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
     Scan sc;
     const uint64_t total = scan_all<ROWS, UNIT>(a, lane, sc);
-    const uint32_t parts = part_count(total, grid), w = blockIdx.x + 1;
+    const uint32_t parts = part_count(total, sc, grid), w = blockIdx.x + 1;
     if (w >= parts) return;
     const uint64_t x = part_begin(total, parts, w);
     const Found f = scan_find<ROWS, UNIT>(a, lane, sc, x);
@@ -649,20 +696,11 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
     auto place = [&](uint32_t v) { return a.part + (size_t)(2 * v + (v == w - 1 ? 1 : 0)) * rows_part(D, QT); };
     uint32_t last = w;
     while (last + 1 < parts && part_begin(total, parts, last + 1) < tile1) ++last;
-    float mx = kNoMax;
-    for (uint32_t v = w - 1 + lane; v <= last; v += 64) mx = fmaxf(mx, place(v)[ROWS * D + r]);
-    for (int k = 32; k; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
-    float acc[RW] = {}, ls = 0.0f;
-#pragma unroll 4
-    for (uint32_t v = w - 1; v <= last; ++v) {
-        const float* p = place(v);
-        const float fac = __builtin_amdgcn_exp2f(p[ROWS * D + r] - mx);
-        ls = __builtin_fmaf(p[ROWS * (D + 1) + r], fac, ls);
-        float t[RW];
-        __builtin_memcpy(t, p + (size_t)r * D + RW * lane, sizeof(t));
-#pragma unroll
-        for (int e = 0; e < RW; ++e) acc[e] = __builtin_fmaf(t[e], fac, acc[e]);
-    }
+    const int n = (int)(last - w + 2);
+    float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
+    join_parts<RW>(
+        n, lane, [&](int v) { return place(w - 1 + v) + ROWS * D + r; }, ROWS,
+        [&](int v) { return place(w - 1 + v) + (size_t)r * D + RW * lane; }, acc, mx, ls);
     const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
     const float inv = inverse(ls);
     uint16_t* dst = a.out + (int64_t)(f.s.first + tok) * a.ld_out + h * D + RW * lane;
@@ -1027,25 +1065,15 @@ __global__ void __launch_bounds__(64) attn_paged_tile_merge_kernel(PagedAttnArgs
         const int gt = base + __builtin_amdgcn_readlane(sc.incl - sc.tiles, l0) + rt;
         const TileSpan sp = tile_span<TR, BN>(a, n, len, ok, rt);
         const float* part = a.part + ((int64_t)gt * a.kv_heads + kvh) * a.nsplit * (TR * (D + 2));
-        auto there = [&](int s) {
-            return (int)((int64_t)sp.nu * s / a.nsplit) < (int)((int64_t)sp.nu * (s + 1) / a.nsplit);
+        // (a tile of fewer units than splits leaves some empty: spread over nu of them)
+        const int np = min(a.nsplit, sp.nu);
+        auto at = [&](int v) {
+            return part + (int64_t)(np == a.nsplit ? v : ((int64_t)(v + 1) * a.nsplit - 1) / sp.nu) * (TR * (D + 2));
         };
-        float mx = kNoMax;
-        for (int s = lane; s < a.nsplit; s += 64)
-            if (there(s)) mx = fmaxf(mx, part[(int64_t)s * (TR * (D + 2)) + TR * D + r]);
-        for (int k = 32; k; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
-        float acc[RW] = {}, ls = 0.0f;
-#pragma unroll 4
-        for (int s = 0; s < a.nsplit; ++s) {
-            if (!there(s)) continue;
-            const float* p = part + (int64_t)s * (TR * (D + 2));
-            const float fac = __builtin_amdgcn_exp2f(p[TR * D + r] - mx);
-            ls = __builtin_fmaf(p[TR * (D + 1) + r], fac, ls);
-            float v[RW];
-            __builtin_memcpy(v, p + r * D + RW * lane, sizeof(v));
-#pragma unroll
-            for (int e = 0; e < RW; ++e) acc[e] = __builtin_fmaf(v[e], fac, acc[e]);
-        }
+        float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
+        join_parts<RW>(
+            np, lane, [&](int v) { return at(v) + TR * D + r; }, TR, [&](int v) { return at(v) + r * D + RW * lane; }, acc, mx,
+            ls);
         const float inv = inverse(ls);
         uint16_t* dst = a.out + (int64_t)t * a.ld_out + head * D + RW * lane;
 #pragma unroll
@@ -1100,13 +1128,23 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     return p;
 }
 
+// Dynamic LDS past 64 KiB, asked for once per kernel and device.
+int allow_lds(const void* k, int lds, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (int rc = hip_check(hipGetDevice(&dev), "hipGetDevice")) return rc;
+    if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return ALV_OK;
+    if (int rc = hip_check(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute"))
+        return rc;
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return ALV_OK;
+}
+
 template <int D, int QT>
 int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     constexpr int lds = rows_lds(D, QT);
     static_assert(lds <= 160 * 1024, "LDS of a CU");
-    const void* k = reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT>);
-    if (int rc = hip_check(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute"))
-        return rc;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT>), lds, done)) return rc;
     hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT>), dim3(p.grid), dim3(64 * rows_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_rows_kernel launch")) return rc;
     hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a, p.grid);
@@ -1117,9 +1155,8 @@ template <int D>
 int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     constexpr int lds = tile_lds(D);
     static_assert(lds <= 160 * 1024, "LDS of a CU");
-    const void* k = reinterpret_cast<const void*>(&attn_paged_tile_kernel<D>);
-    if (int rc = hip_check(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute"))
-        return rc;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D>), lds, done)) return rc;
     hipLaunchKernelGGL((attn_paged_tile_kernel<D>), dim3((uint32_t)(p.tiles * p.nsplit)), dim3(64 * tile_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_tile_kernel launch")) return rc;
     if (p.nsplit == 1) return ALV_OK;
