@@ -75,6 +75,43 @@ def _batch(page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor
     return B, W, page_table.stride(0) if B > 1 else W
 
 
+_BF16, _I32 = torch.bfloat16, torch.int32
+
+
+def _args(t: torch.Tensor, name: str, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
+          q_start: torch.Tensor, kv_len: torch.Tensor, dev: torch.device):
+    """((pages, kv_heads, S, D), page strides, B, max_pages, table's row stride, T, t's width and row stride): the
+    checks that every call shares. Contiguous tensors, as most are, take one test each (the others' take 6 us of a
+    call whose kernel may take 5)."""
+    i = dev.index
+    try:
+        if (t.dtype is _BF16 and kpages.dtype is _BF16 and vpages.dtype is _BF16 and page_table.dtype is _I32
+                and q_start.dtype is _I32 and kv_len.dtype is _I32 and t.is_contiguous() and kpages.is_contiguous()
+                and vpages.is_contiguous() and page_table.is_contiguous() and q_start.is_contiguous()
+                and kv_len.is_contiguous() and kpages.get_device() == i and vpages.get_device() == i
+                and page_table.get_device() == i and q_start.get_device() == i and kv_len.get_device() == i
+                and t.dim() == 2 and q_start.dim() == 1 and kv_len.dim() == 1):
+            shape = kpages.shape
+            _, H, S, D = shape
+            B, W = page_table.shape
+            if vpages.shape == shape and q_start.numel() == B + 1 and kv_len.numel() == B:
+                T, w = t.shape
+                n = H * S * D
+                return shape, n, n, B, W, W, T, w, w
+    except (AttributeError, ValueError):
+        pass
+    return *_pages(kpages, vpages, dev), *_batch(page_table, q_start, kv_len, dev), *_shape2(t, name, dev)
+
+
+def _shape2(t: torch.Tensor, name: str, dev: torch.device):
+    ld = _rows(t, name, 0, dev)
+    return *t.shape, ld
+
+
+def _narrow(name: str, have: int, width: int) -> None:
+    raise ValueError(f"{name} rows must hold {width} values, got {have}")
+
+
 def _weights(w, name: str, n: int, dev: torch.device) -> torch.Tensor | None:
     """Norm weights on a 16-byte boundary."""
     w = _f32(w, name, n, dev)
@@ -93,10 +130,11 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
     left as they are in ``q_out``, zeros for a sequence that does not fit its
     table (or the rope table)."""
     dev = _need_gpu(qkv)
-    (pages, kv_heads, S, D), ks, vs = _pages(kpages, vpages, dev)
-    B, W, ldt = _batch(page_table, q_start, kv_len, dev)
-    ldqkv = _rows(qkv, "qkv", (k_off if v_off < 0 else v_off) + kv_heads * D, dev)
-    T, ldq = qkv.shape[0], heads * D
+    (pages, kv_heads, S, D), ks, vs, B, W, ldt, T, width, ldqkv = _args(qkv, "qkv", kpages, vpages, page_table, q_start,
+                                                                        kv_len, dev)
+    if width < (k_off if v_off < 0 else v_off) + kv_heads * D:
+        _narrow("qkv", width, (k_off if v_off < 0 else v_off) + kv_heads * D)
+    ldq = heads * D
     q_w, k_w = _weights(q_w, "q_w", D, dev), _weights(k_w, "k_w", D, dev)
     rope_rows = ldr = 0
     if rope is not None:
@@ -104,7 +142,7 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
         half = rope.shape[1] // 2 if half is None else half
         sin_off = half if sin_off is None else sin_off
     if q_out is None:
-        q_out = torch.empty((T, ldq), dtype=torch.bfloat16, device=dev)
+        q_out = qkv.new_empty((T, ldq))
     else:
         ldq = _rows(q_out, "q_out", ldq, dev)
         if q_out.shape[0] < T:
@@ -128,12 +166,13 @@ def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     sequence owns, where the caller knows it, lets the call choose how to spread
     the work (1 for a decode step); it does not change what is computed."""
     dev = _need_gpu(q)
-    (pages, kv_heads, S, D), ks, vs = _pages(kpages, vpages, dev)
-    B, W, ldt = _batch(page_table, q_start, kv_len, dev)
-    ldq = _rows(q, "q", heads * D, dev)
-    T, ldo = q.shape[0], heads * D
+    (pages, kv_heads, S, D), ks, vs, B, W, ldt, T, width, ldq = _args(q, "q", kpages, vpages, page_table, q_start, kv_len,
+                                                                      dev)
+    ldo = heads * D
+    if width < ldo:
+        _narrow("q", width, ldo)
     if out is None:
-        out = torch.empty((T, ldo), dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(q) if width == ldo == ldq else q.new_empty((T, ldo))
     else:
         ldo = _rows(out, "out", ldo, dev)
         if out.shape[0] < T:
@@ -172,15 +211,13 @@ def copy_pages(caches, src, dst) -> None:
         return
     first = caches[0]
     dev = _need_gpu(first)
-    shape, strides, dtype = first.shape, first.stride(), first.dtype
+    shape, strides, dtype, index = first.shape, first.stride(), first.dtype, dev.index
     if len(shape) < 2 or first.numel() == 0:
         raise ValueError(f"a cache must be (pages, ...), got shape {tuple(shape)}")
-    for t in caches:
-        if not isinstance(t, torch.Tensor) or t.device != dev:
-            raise ValueError(f"the caches must be tensors on one GPU, {dev}")
-        if t.shape != shape or t.stride() != strides or t.dtype != dtype:
-            raise ValueError(f"the caches differ: {t.dtype} {tuple(t.shape)} {t.stride()} and {dtype} "
-                             f"{tuple(shape)} {strides}")
+    if not all([isinstance(t, torch.Tensor) for t in caches]) or {t.get_device() for t in caches} != {index}:
+        raise ValueError(f"the caches must be tensors on one GPU, {dev}")
+    if len({t.dtype for t in caches}) + len({t.shape for t in caches}) + len({t.stride() for t in caches}) != 3:
+        raise ValueError(f"the caches must be alike: {dtype} {tuple(shape)} {strides}, and not all are")
     page = first[0]
     if not page.is_contiguous():
         raise ValueError(f"each page must be contiguous, got strides {strides}")
