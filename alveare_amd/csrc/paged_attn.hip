@@ -1,4 +1,6 @@
 // Attention of the newest tokens of a batch of sequences over a paged KV cache.
+#include <limits.h>
+
 #include <algorithm>
 #include <atomic>
 
@@ -23,7 +25,8 @@ struct PagedAttnArgs {
     uint16_t* out;
     int64_t ld_out;
     int64_t row_limit;  // sequences of more rows (tokens times q heads per kv head) are not this launch's
-    int nsplit;         // parts of a tile's positions
+    int nsplit;         // parts of a tile's positions, unless there are more than max_items tiles
+    int max_items;
     float* part;
 };
 
@@ -70,6 +73,13 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p);
 }
 
+// The value, as if it were new here: what is computed from it is computed again
+// in each turn of a loop rather than kept in registers throughout.
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // The larger (sum) of a value over the lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float max_groups(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -102,8 +112,8 @@ __device__ __forceinline__ s16x4 pack4(float a, float b, float c, float d) {
 __device__ __forceinline__ uint32_t nonfinite_bits(uint32_t w) {
     return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
 }
-__device__ __forceinline__ bool any_nonfinite(u32x4 v) {
-    return (nonfinite_bits(v[0]) | nonfinite_bits(v[1]) | nonfinite_bits(v[2]) | nonfinite_bits(v[3])) != 0;
+__device__ __forceinline__ uint32_t nonfinite_bits4(u32x4 v) {
+    return nonfinite_bits(v[0]) | nonfinite_bits(v[1]) | nonfinite_bits(v[2]) | nonfinite_bits(v[3]);
 }
 
 // LDS pieces of a row are stored at (piece ^ swizzle of the row): the 16 lanes
@@ -461,12 +471,21 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
                 }
             }
         }
-        if (QL) __syncthreads();
+        if constexpr (QL) {
+            __syncthreads();
+        } else {
+            // Waited for here: the compiler would else wait at their first use, in
+            // the loop, each time, for whatever is on its way to LDS by then.
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) asm volatile("" : "+v"(q[t][i]));
+        }
         const int pos_lo = f.s.len - f.s.n + (f.rt * ROWS) / a.g;
         const int pos_hi = f.s.len - f.s.n + (f.rt * ROWS + nrows - 1) / a.g;
         f32x4 o[QT][D / 16];
         float m[QT], l[QT];
-        bool odd = false;  // a value of V that is no number, where some row may not see it
+        uint32_t odd = 0;  // not 0: a value of V that is no number, where some row may not see it
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             m[t] = kNoMax;
@@ -539,7 +558,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
-                    odd |= any_nonfinite(*reinterpret_cast<const u32x4*>(vt + 1024 * i + 16 * lane));
+                    odd |= nonfinite_bits4(*reinterpret_cast<const u32x4*>(vt + 1024 * i + 16 * lane));
             }
             constexpr int VB = D / 16 < 8 ? D / 16 : 8;  // V reads on their way at once
 #pragma unroll
@@ -569,7 +588,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
             }
         }
         if (lane == 0) odds[wave] = 0;
-        if (__any(odd) && lane == 0) odds[wave] = 1;
+        if (__any(odd != 0) && lane == 0) odds[wave] = 1;
         __syncthreads();  // and every wave is done with its ring
         bool again = false;
 #pragma unroll
@@ -721,10 +740,9 @@ constexpr int tile_ds(int D) { return D >= 256 ? 2 : 1; }      // waves that sha
 constexpr int tile_waves(int D) { return D >= 256 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D) / tile_ds(D); }
 constexpr int tile_bn(int D) { return D <= 128 ? 64 : 32; }
-constexpr int tile_kbufs(int D) { return D >= 256 ? 1 : 2; }
 constexpr int tile_bytes(int D) { return tile_bn(D) * 2 * D; }  // of K, of V
 constexpr int tile_xch(int D) { return D >= 256 ? tile_waves(D) * 4096 : 0; }
-constexpr int tile_lds(int D) { return (tile_kbufs(D) + 2) * tile_bytes(D) + tile_xch(D) + 16; }
+constexpr int tile_lds(int D) { return 4 * tile_bytes(D) + tile_xch(D); }
 
 typedef float f32x16 __attribute__((__vector_size__(16 * sizeof(float))));
 
@@ -779,30 +797,35 @@ __device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int
     return s;
 }
 
+// Items (tiles times kv heads, times splits) and where each is found: heaviest
+// (last) tiles first, kv heads side by side, so that the workgroups an XCD gets
+// in turn share theirs where there are eight.
+template <int TR>
+__device__ __forceinline__ int tile_count(const PagedAttnArgs& a, int lane) {
+    int all = 0;
+    for (int b0 = 0; b0 < a.b.B; b0 += 64) all += tile_scan<TR>(a, b0, lane).sum;
+    return all * a.kv_heads;
+}
+// Splits per tile: as planned, unless there are more tiles than the plan knew of.
+__device__ __forceinline__ int tile_splits(const PagedAttnArgs& a, int items) { return items <= a.max_items ? a.nsplit : 1; }
+
 template <int D>
-__global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kernel(PagedAttnArgs a) {
-    constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D), KB = tile_kbufs(D);
+__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int split, int nsplit, unsigned char* smem) {
+    constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D);
     constexpr int DW = D / DS;            // this wave's columns of the output (and of its scores' products)
     constexpr int TB = tile_bytes(D), NC = D / 8, RPL = 512 / D;
-    constexpr int LR = BN / NW;           // positions a wave loads: within one page
+    constexpr int LR = BN / NW;           // positions a wave loads: within one block of 16
     constexpr int NL = LR / RPL;          // its loads of K (of V)
-    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int NB = BN / 16;
+    constexpr int KR = 4, VR = 4;         // operands of K, of V on their way from LDS
     unsigned char* kbuf = smem;
-    unsigned char* vbuf = smem + KB * TB;
-    float* xch = reinterpret_cast<float*>(smem + (KB + 2) * TB);
-    int* tags = reinterpret_cast<int*>(smem + (KB + 2) * TB + tile_xch(D));
+    unsigned char* vbuf = smem + 2 * TB;
+    float* xch = reinterpret_cast<float*>(smem + 4 * TB);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = wave / DS, dh = wave % DS;
     const int col = lane & 31, h = lane >> 5;
 
-    // Item: heaviest (last) tiles first, kv heads side by side, so that the
-    // workgroups an XCD gets in turn share theirs where there are eight.
-    int all = 0;
-    for (int b0 = 0; b0 < a.b.B; b0 += 64) all += tile_scan<TR>(a, b0, lane).sum;
-    const int item = all * a.kv_heads - 1 - (int)(blockIdx.x / (uint32_t)a.nsplit);
-    const int split = (int)(blockIdx.x % (uint32_t)a.nsplit);
-    if (item < 0) return;
     const int gt = item / a.kv_heads, kvh = item - gt * a.kv_heads;
     int base = 0, b0 = 0;
     TileScan sc = tile_scan<TR>(a, 0, lane);
@@ -818,38 +841,56 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
     const bool ok = __builtin_amdgcn_readlane((int)sc.ok, l0) != 0;
     const int rt = gt - base - __builtin_amdgcn_readlane(sc.incl - sc.tiles, l0);
     const TileSpan sp = tile_span<TR, BN>(a, n, len, ok, rt);
-    const int u0 = uniform((int)((int64_t)sp.nu * split / a.nsplit));
-    const int u1 = uniform((int)((int64_t)sp.nu * (split + 1) / a.nsplit));
-    if (a.nsplit > 1 && u0 == u1) return;  // the merge skips it too
+    const int u0 = uniform((int)((int64_t)sp.nu * split / nsplit));
+    const int u1 = uniform((int)((int64_t)sp.nu * (split + 1) / nsplit));
+    if (nsplit > 1 && u0 == u1) return;  // the merge skips it too
 
     const int32_t* table = a.b.table + (int64_t)seq * a.b.ld_table;
     auto unit_pos = [&](int u) { return (u < sp.us ? u : u - sp.us + sp.ulo) * BN; };
+    // The pages of 64 units' positions that this wave loads, one per lane; a bit
+    // per unit for each of its blocks of 16 that has none.
     int pages = -1, pages0 = u0;
-    auto load_pages = [&](int v0) {
+    uint64_t gone[NB] = {};
+    auto load_pages = [&](int v0) __attribute__((always_inline)) {
         pages0 = v0;
-        const int p = unit_pos(v0 + lane) + wave * LR;
-        pages = v0 + lane < u1 && p < len ? table[p >> a.b.shift] : -1;
-        if ((unsigned)pages >= (unsigned)a.b.pages) pages = -1;
+        const int p = unit_pos(v0 + lane);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const bool in = v0 + lane < u1 && p + 16 * k < len;
+            int e = in ? table[(p + 16 * k) >> a.b.shift] : -1;
+            if ((unsigned)e >= (unsigned)a.b.pages) e = -1;
+            gone[k] = __ballot(in && e < 0);
+            pages = k == wave * LR / 16 ? e : pages;
+        }
     };
+    uint32_t holes = 0;  // NB bits by unit modulo 4
     const uint32_t kb_lds = __builtin_amdgcn_readfirstlane(lds_addr(kbuf)) + wave * LR * (2 * D);
     const uint32_t vb_lds = __builtin_amdgcn_readfirstlane(lds_addr(vbuf)) + wave * LR * (2 * D);
     // The wave's rows start at a multiple of 4, not of 16: their bits of the
     // swizzles are part of the lane's offset.
     const uint32_t dma_k = (lane / NC) * (2 * D) + ((lane % NC) ^ k_swz<D>(wave * LR + lane / NC)) * 16;
     const uint32_t dma_v = (lane / NC) * (2 * D) + ((lane % NC) ^ v_swz<D>(wave * LR + lane / NC)) * 16;
-    auto issue = [&](int u) {
+    // Starts unit u's K (then its V) on the way to LDS; K before V, units in order.
+    auto issue = [&](int u, bool v) __attribute__((always_inline)) {
         if (u - pages0 >= 64) load_pages(u);
         const int page = __builtin_amdgcn_readlane(pages, u - pages0), p = unit_pos(u) + wave * LR;
         const uint32_t bytes = page < 0 ? 0u : (uint32_t)max(0, min(LR, len - p)) * (2 * D);
-        if (page < 0 && p < len && lane == 0) tags[u & 1] = u;
         const int64_t off = (((int64_t)kvh << a.b.shift) + (p & ((1 << a.b.shift) - 1))) * D;
-        const __amdgpu_buffer_rsrc_t rk = wave_rsrc(a.kpages + max(page, 0) * a.k_stride + off, bytes);
-        const __amdgpu_buffer_rsrc_t rv = wave_rsrc(a.vpages + max(page, 0) * a.v_stride + off, bytes);
-        const uint32_t kd = kb_lds + (KB == 2 ? (u & 1) * TB : 0), vd = vb_lds + (u & 1) * TB;
+        if (!v) {
+            uint32_t now = 0;
 #pragma unroll
-        for (int i = 0; i < NL; ++i) load_lds16(rk, dma_k ^ (k_swz<D>(RPL * i) * 16), 1024 * i, kd + 1024 * i);
+            for (int k = 0; k < NB; ++k) now |= (uint32_t)(gone[k] >> (u - pages0) & 1) << k;
+            const int at = NB * (u & 3);
+            holes = (holes & ~(((1u << NB) - 1) << at)) | (now << at);
+        }
+        const uint16_t* src = v ? a.vpages + max(page, 0) * a.v_stride : a.kpages + max(page, 0) * a.k_stride;
+        const __amdgpu_buffer_rsrc_t r = wave_rsrc(src + off, bytes);
+        const uint32_t dst = (v ? vb_lds : kb_lds) + (u & 1) * TB, at = here(v ? dma_v : dma_k);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) load_lds16(rv, dma_v ^ (v_swz<D>(RPL * i) * 16), 1024 * i, vd + 1024 * i);
+        for (int i = 0; i < NL; ++i) {
+            const uint32_t x = v ? (uint32_t)v_swz<D>(RPL * i) : (uint32_t)k_swz<D>(RPL * i);
+            load_lds16(r, at ^ (x * 16), 1024 * i, dst + 1024 * i);
+        }
     };
 
     // This lane's row: column col of the wave's 32.
@@ -866,134 +907,185 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
         const uint16_t* qr = a.q + (int64_t)(first + tok) * a.ld_q + head * D + dh * DW + 8 * h;
 #pragma unroll
         for (int i = 0; i < DW / 16; ++i) q[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qr + 16 * i));
+        // Waited for here: the compiler would else wait at their first use, in
+        // the loop, each time, for whatever is on its way to LDS by then.
+#pragma unroll
+        for (int i = 0; i < DW / 16; ++i) asm volatile("" : "+v"(q[i]));
     }
     f32x16 o[DW / 32];
 #pragma unroll
     for (int d = 0; d < DW / 32; ++d) o[d] = f32x16{};
     float m = kNoMax, l = 0.0f;
-    bool odd = false;  // a value of V that is no number, where some row may not see it
+    uint32_t odd = 0;  // not 0: a value of V that is no number, where some row may not see it
 
     const int vrow = 4 * h + ((lane & 15) >> 2);
     const uint32_t rd_k = col * (2 * D) + (h ^ k_swz<D>(col)) * 16;
     const uint32_t rd_v = vrow * (2 * D) + ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_swz<D>(vrow)) * 16 + (lane & 1) * 8;
 
-    if (tid < 2) tags[tid] = -1;
-    __syncthreads();
+    // Rows that see nothing of 32 positions at p0 (or are none) are done with them.
+    auto skip = [&](int p0) { return nrows == 0 || p0 > wpos_hi; };
+    // K q of the 32 positions whose rows begin at ks, over this wave's columns.
+    auto scores = [&](const unsigned char* ks) __attribute__((always_inline)) {
+        f32x16 s{};
+        const uint32_t at = here(rd_k);
+        auto read_k = [&](int i) __attribute__((always_inline)) {
+            return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
+                ks + (at ^ piece<D>(2 * i)) + piece_far<D>((dh * DW + 16 * i) / 8 & ~15)));
+        };
+        bf16x8 k[KR];
+#pragma unroll
+        for (int i = 0; i < KR; ++i) k[i] = read_k(i);
+#pragma unroll
+        for (int i = 0; i < DW / 16; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i % KR], q[i], s, 0, 0, 0);
+            if (i + KR < DW / 16) k[i % KR] = read_k(i + KR);
+        }
+        return s;
+    };
+    // Their weights, and the output's share of V.
+    auto absorb = [&](const f32x16& sv, int p0, const unsigned char* vs, uint32_t hole) __attribute__((always_inline)) {
+        hole &= 3;  // of its two blocks of 16
+        float s[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = sv[i];
+        const bool masked = hole || p0 + 31 > wpos_lo || (a.window > 0 && p0 <= wpos_hi - a.window && p0 + 31 >= a.sinks);
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int p = p0 + 8 * (i / 4) + 4 * h + i % 4;
+                if (!sees(a, p, pos) || (hole >> (i / 8) & 1)) s[i] = -__builtin_inff();
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        if (__any(__builtin_fmaf(top, c, -m) > kSlack)) {
+            const uint32_t tb = __builtin_bit_cast(uint32_t, top);
+            auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
+            const uint32_t t0 = sw[0], t1 = sw[1];
+            const float mn = fmaxf(m, fmaxf(__builtin_bit_cast(float, t0), __builtin_bit_cast(float, t1)) * c);
+            const float fac = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= fac;
+#pragma unroll
+            for (int d = 0; d < DW / 32; ++d) {
+                o[d] *= fac;
+                asm volatile("" : "+v"(o[d]));  // in place, one after the other
+            }
+        }
+        float w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float si = s[i];
+            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(si, c, -m));
+        }
+        l += (((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]))) +
+             (((w[8] + w[9]) + (w[10] + w[11])) + ((w[12] + w[13]) + (w[14] + w[15])));
+        // Weights as bf16, the matrix cores' type (see the streaming kernel).
+        bf16x8 pw[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pw[i >> 3][i & 7] = (__bf16)w[i];
+        // Columns 32 d .. of this wave, positions 16 k + 8 e + 4 h .. + 3.
+        const uint32_t at = here(rd_v);
+        auto read_v = [&](int d, int k) __attribute__((always_inline)) {
+            const unsigned char* v = vs + (at ^ piece<D>(4 * d)) + piece_far<D>((dh * DW + 32 * d) / 8 & ~15) + k * 32 * D;
+            const s16x4 lo = read_tr(v), hi = read_tr(v + 16 * D);
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        if (masked) {
+#pragma unroll
+            for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    // (tied down one by one: few registers at a time, and V is read again below, not kept)
+                    odd |= nonfinite_bits4(__builtin_bit_cast(u32x4, read_v(d, k)));
+                    asm volatile("" : "+v"(odd)::"memory");
+                }
+        }
+        // Operand j: two blocks of columns in turn, then their second 16 positions.
+        constexpr int NV = DW / 16;
+        auto blk = [](int j) { return (j & ~3) / 2 + (j & 1); };
+        bf16x8 v[VR];
+#pragma unroll
+        for (int j = 0; j < VR; ++j) v[j] = read_v(blk(j), j >> 1 & 1);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            o[blk(j)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[j % VR], pw[j >> 1 & 1], o[blk(j)], 0, 0, 0);
+            if (j + VR < NV) v[j % VR] = read_v(blk(j + VR), (j + VR) >> 1 & 1);
+        }
+    };
+
     if (u1 > u0) {
         load_pages(u0);
-        issue(u0);
+        issue(u0, false);
+        issue(u0, true);
     }
+    if constexpr (DS == 1) {
 #pragma unroll 1
-    for (int u = u0; u < u1; ++u) {
-        wait_vm<0>();
-        __syncthreads();
-        if (KB == 2 && u + 1 < u1) issue(u + 1);
-        const bool holes = tags[u & 1] == u;
-        const unsigned char* kt = kbuf + (KB == 2 ? (u & 1) * TB : 0);
-        const unsigned char* vt = vbuf + (u & 1) * TB;
-        const int pt = unit_pos(u);
-#pragma unroll 1
-        for (int sub = 0; sub < BN / 32; ++sub) {
-            const int p0 = pt + 32 * sub;
-            const bool skip = nrows == 0 || p0 > wpos_hi;
-            if (DS == 1 && skip) break;
-            f32x16 s{};
-            if (!skip) {
-                const unsigned char* ks = kt + sub * 64 * D;
-#pragma unroll
-                for (int i0 = 0; i0 < DW / 16; i0 += 4) {
-                    bf16x8 k[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        k[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
-                            ks + (rd_k ^ piece<D>(2 * (i0 + i))) + piece_far<D>((dh * DW + 16 * (i0 + i)) / 8 & ~15)));
-                    asm volatile("" ::: "memory");
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i], q[i0 + i], s, 0, 0, 0);
-                }
+        for (int u = u0; u < u1; ++u) {
+            wait_vm<0>();
+            __syncthreads();
+            if (u + 1 < u1) {
+                issue(u + 1, false);
+                issue(u + 1, true);
             }
-            if constexpr (DS == 2) {
-                // The other half's products; the sum is the same in both waves.
-                f32x4* mine = reinterpret_cast<f32x4*>(xch + wave * 1024) + lane;
-                const f32x4* other = reinterpret_cast<const f32x4*>(xch + (wave ^ 1) * 1024) + lane;
+            const int pt = unit_pos(u);
+            const unsigned char* kt = kbuf + (u & 1) * TB;
+            const unsigned char* vt = vbuf + (u & 1) * TB;
+#pragma unroll 1
+            for (int sub = 0; sub < BN / 32 && !skip(pt + 32 * sub); ++sub)
+                absorb(scores(kt + sub * 64 * D), pt + 32 * sub, vt + sub * 64 * D, holes >> (NB * (u & 3) + 2 * sub));
+        }
+    } else {
+        // Two groups of waves, one of each per SIMD, half a unit apart: while one
+        // multiplies K the other has its softmax and V, so the matrix cores, the
+        // vector ALUs and LDS all have work (in step, each waits for the others:
+        // 4096 tokens, 16 heads of 512, 342 us). Phase p, between two barriers:
+        // even p = 2 k is unit k's K for group 0 and unit k - 1's V for group 1, odd
+        // p the reverse; loads run two phases ahead, unit k's K needed from phase
+        // 2 k, its V from 2 k + 1, and each buffer is filled again when its last
+        // reader has passed a barrier.
+        const int grp = wave / (NW / 2), nu = u1 - u0;
+        f32x4* mine = reinterpret_cast<f32x4*>(xch + wave * 1024) + lane;
+        const f32x4* other = reinterpret_cast<const f32x4*>(xch + (wave ^ 1) * 1024) + lane;
+        auto begin = [&](int phase) __attribute__((always_inline)) {
+            if (phase + 1 < 2 * nu)
+                wait_vm<NL>();  // the loads issued in the last phase may still be on their way
+            else
+                wait_vm<0>();
+            __syncthreads();
+            if (phase + 2 < 2 * nu) issue(u0 + ((phase + 2) >> 1), phase & 1);
+        };
+        if (nu > 0 && grp == 1) begin(0);
+#pragma unroll 1
+        for (int u = u0; u < u1; ++u) {
+            const int p0 = unit_pos(u);
+            f32x16 s{};
+            begin(2 * (u - u0) + grp);
+            if (!skip(p0)) {
+                s = scores(kbuf + (u & 1) * TB);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mine[64 * i] = f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
-                __syncthreads();
-                if (u + 1 < u1) issue(u + 1);
-                if (skip) continue;
+            }
+            begin(2 * (u - u0) + grp + 1);
+            if (!skip(p0)) {
+                // With the other half's products; the sum is the same in both waves.
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const f32x4 x = other[64 * i];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[4 * i + e] += x[e];
                 }
-            }
-            const bool masked = holes || p0 + 31 > wpos_lo ||
-                                (a.window > 0 && p0 <= wpos_hi - a.window && p0 + 31 >= a.sinks);
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int p = p0 + 8 * (i / 4) + 4 * h + i % 4;
-                    bool see = sees(a, p, pos);
-                    if (holes && see) see = page_of(a.b, seq, p) >= 0;
-                    if (!see) s[i] = -__builtin_inff();
-                }
-            }
-            float top = s[0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-            if (__any(__builtin_fmaf(top, c, -m) > kSlack)) {
-                const uint32_t tb = __builtin_bit_cast(uint32_t, top);
-                auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
-                const uint32_t t0 = sw[0], t1 = sw[1];
-                const float mn = fmaxf(m, fmaxf(__builtin_bit_cast(float, t0), __builtin_bit_cast(float, t1)) * c);
-                const float fac = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= fac;
-#pragma unroll
-                for (int d = 0; d < DW / 32; ++d) o[d] *= fac;
-            }
-            float w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float si = s[i];
-                w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(si, c, -m));
-            }
-            l += (((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]))) +
-                 (((w[8] + w[9]) + (w[10] + w[11])) + ((w[12] + w[13]) + (w[14] + w[15])));
-            // Weights as bf16, the matrix cores' type (see the streaming kernel).
-            bf16x8 pw[2];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pw[i >> 3][i & 7] = (__bf16)w[i];
-            const unsigned char* vs = vt + sub * 64 * D;
-            // Columns 32 d .. of this wave, positions 16 k + 8 e + 4 h .. + 3.
-            auto read_v = [&](int d, int k) __attribute__((always_inline)) {
-                const unsigned char* v = vs + (rd_v ^ piece<D>(4 * d)) + piece_far<D>((dh * DW + 32 * d) / 8 & ~15) + k * 32 * D;
-                const s16x4 lo = read_tr(v), hi = read_tr(v + 16 * D);
-                return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            };
-            if (masked) {
-#pragma unroll
-                for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) odd |= any_nonfinite(__builtin_bit_cast(u32x4, read_v(d, k)));
-                asm volatile("" ::: "memory");  // V is read again, not kept
-            }
-#pragma unroll
-            for (int d = 0; d < DW / 32; d += 2) {
-                bf16x8 v[2][2];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k >> 1][k & 1] = read_v(d + (k >> 1), k & 1);
-                asm volatile("" ::: "memory");
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    o[d + (k & 1)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k & 1][k >> 1], pw[k >> 1], o[d + (k & 1)], 0, 0, 0);
+                absorb(s, p0, vbuf + (u & 1) * TB, holes >> (NB * (u & 3)));
             }
         }
+        if (nu > 0 && grp == 0) begin(2 * nu);
     }
 
-    float* part = a.part + ((int64_t)item * a.nsplit + split) * (TR * (D + 2));
-    if (__any(odd)) {  // see plain_row; with two waves per row, one does it
+    float* part = a.part + ((int64_t)item * nsplit + split) * (TR * (D + 2));
+    if (__any(odd != 0)) {  // see plain_row; with two waves per row, one does it
         for (int r = 0; dh == 0 && r < nrows; ++r) {
             const int64_t rr = r0 + r;
             const int tk = (int)(rr / a.g), hd = kvh * a.g + (int)(rr % a.g);
@@ -1005,12 +1097,12 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
             float* pr = part + (32 * rg + r) * D + D / 64 * lane;
 #pragma unroll
             for (int e = 0; e < D / 64; ++e) {
-                if (a.nsplit == 1)
+                if (nsplit == 1)
                     dst[e] = bf16_rne_bits(acc[e] * inv);
                 else
                     pr[e] = acc[e];
             }
-            if (a.nsplit > 1 && lane == 0) {
+            if (nsplit > 1 && lane == 0) {
                 part[TR * D + 32 * rg + r] = mr;
                 part[TR * (D + 1) + 32 * rg + r] = lr;
             }
@@ -1019,7 +1111,7 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
     }
     l += __shfl_xor(l, 32);
     if (col >= nrows) return;
-    if (a.nsplit == 1) {
+    if (nsplit == 1) {
         const float inv = inverse(l);
         uint16_t* dst = a.out + (int64_t)(first + tok) * a.ld_out + head * D + dh * DW + 4 * h;
 #pragma unroll
@@ -1042,11 +1134,22 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
     }
 }
 
+template <int D>
+__global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kernel(PagedAttnArgs a) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int items = tile_count<tile_rows(D)>(a, threadIdx.x & 63);
+    const int nsplit = tile_splits(a, items);
+    const int item = items - 1 - (int)(blockIdx.x / (uint32_t)nsplit);
+    if (item >= 0) tile_item<D>(a, item, (int)(blockIdx.x % (uint32_t)nsplit), nsplit, smem);
+}
+
 // The splits of the tiles joined: a wave per (packed row, q head).
 template <int D>
 __global__ void __launch_bounds__(64) attn_paged_tile_merge_kernel(PagedAttnArgs a) {
     constexpr int TR = tile_rows(D), BN = tile_bn(D), RW = D / 64;
     const int lane = threadIdx.x, t = blockIdx.x, head = blockIdx.y;
+    const int nsplit = tile_splits(a, tile_count<TR>(a, lane));
+    if (nsplit == 1) return;
     int base = 0;
     for (int b0 = 0; b0 < a.b.B; b0 += 64) {
         const TileScan sc = tile_scan<TR>(a, b0, lane);
@@ -1064,11 +1167,11 @@ __global__ void __launch_bounds__(64) attn_paged_tile_merge_kernel(PagedAttnArgs
         const int rt = (int)(row / TR), r = (int)(row % TR);
         const int gt = base + __builtin_amdgcn_readlane(sc.incl - sc.tiles, l0) + rt;
         const TileSpan sp = tile_span<TR, BN>(a, n, len, ok, rt);
-        const float* part = a.part + ((int64_t)gt * a.kv_heads + kvh) * a.nsplit * (TR * (D + 2));
+        const float* part = a.part + ((int64_t)gt * a.kv_heads + kvh) * nsplit * (TR * (D + 2));
         // (a tile of fewer units than splits leaves some empty: spread over nu of them)
-        const int np = min(a.nsplit, sp.nu);
+        const int np = min(nsplit, sp.nu);
         auto at = [&](int v) {
-            return part + (int64_t)(np == a.nsplit ? v : ((int64_t)(v + 1) * a.nsplit - 1) / sp.nu) * (TR * (D + 2));
+            return part + (int64_t)(np == nsplit ? v : ((int64_t)(v + 1) * nsplit - 1) / sp.nu) * (TR * (D + 2));
         };
         float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
         join_parts<RW>(
@@ -1096,7 +1199,8 @@ struct AttnPlan {
     int qt;              // row tiles of 16 in the streaming kernel (0: not launched)
     int64_t row_limit;   // sequences of at most this many rows are its, the others the tile kernel's
     int grid;            // its workgroups
-    int64_t tiles;       // most tiles times kv heads of the tile kernel (0: not launched)
+    int64_t grid_tiles;  // tiles times kv heads of the tile kernel at most (0: not launched),
+    int64_t tiles;       // and at most as far as max_q tells
     int nsplit;
     uint64_t rows_bytes, part_bytes;
 };
@@ -1119,8 +1223,10 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     p.nsplit = 1;
     p.part_bytes = p.rows_bytes;
     if (tiles) {
-        const int tr = D == 512 ? tile_rows(512) : tile_rows(64);
-        p.tiles = (T * g / tr + std::min((int64_t)B, T * g / (p.row_limit + 1) + 1)) * kv_heads;
+        static_assert(tile_rows(64) == 128 && tile_rows(128) == 128 && tile_rows(256) == 128 && tile_rows(512) == 128, "");
+        const int tr = 128;
+        p.grid_tiles = (T * g / tr + std::min((int64_t)B, T * g / (p.row_limit + 1) + 1)) * kv_heads;
+        p.tiles = max_q > 0 ? std::min(p.grid_tiles, (int64_t)B * ((max_q * g + tr - 1) / tr) * kv_heads) : p.grid_tiles;
         const int64_t slots = (int64_t)device_cus() * (D >= 256 ? 1 : 2);
         p.nsplit = (int)std::max((int64_t)1, std::min((int64_t)64, slots / p.tiles));
         if (p.nsplit > 1) p.part_bytes += (uint64_t)p.tiles * p.nsplit * tr * (D + 2) * sizeof(float);
@@ -1157,7 +1263,7 @@ int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D>), lds, done)) return rc;
-    hipLaunchKernelGGL((attn_paged_tile_kernel<D>), dim3((uint32_t)(p.tiles * p.nsplit)), dim3(64 * tile_waves(D)), lds, s, a);
+    hipLaunchKernelGGL((attn_paged_tile_kernel<D>), dim3((uint32_t)(p.grid_tiles * p.nsplit)), dim3(64 * tile_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_tile_kernel launch")) return rc;
     if (p.nsplit == 1) return ALV_OK;
     hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D>), dim3(a.b.T, a.heads), dim3(64), 0, s, a);
@@ -1167,7 +1273,7 @@ int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
 template <int D>
 int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
     float* part = a.part;
-    if (p.tiles) {
+    if (p.grid_tiles) {
         a.part = part + p.rows_bytes / sizeof(float);
         if (int rc = launch_tiles<D>(a, p, s)) return rc;
     }
@@ -1222,6 +1328,7 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
     a.part = static_cast<float*>(workspace);
     a.row_limit = p.row_limit;
     a.nsplit = p.nsplit;
+    a.max_items = (int)std::min(p.tiles, (int64_t)INT_MAX);
     const hipStream_t s = (hipStream_t)stream;
     switch (D) {
         case 64: return launch_d<64>(a, p, s);
