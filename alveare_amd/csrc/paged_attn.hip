@@ -736,12 +736,12 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
 // score's products, exchanged through LDS, and half of the output.
 // Where there are fewer tiles than compute units each tile's positions are split
 // and the parts joined by a second launch.
-constexpr int tile_ds(int D) { return D >= 256 ? 2 : 1; }      // waves that share 32 rows
-constexpr int tile_waves(int D) { return D >= 256 ? 8 : 4; }
+constexpr int tile_ds(int D) { return D == 512 ? 2 : 1; }      // waves that share 32 rows
+constexpr int tile_waves(int D) { return D == 512 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D) / tile_ds(D); }
 constexpr int tile_bn(int D) { return D <= 128 ? 64 : 32; }
 constexpr int tile_bytes(int D) { return tile_bn(D) * 2 * D; }  // of K, of V
-constexpr int tile_xch(int D) { return D >= 256 ? tile_waves(D) * 4096 : 0; }
+constexpr int tile_xch(int D) { return D == 512 ? tile_waves(D) * 4096 : 0; }
 constexpr int tile_lds(int D) { return 4 * tile_bytes(D) + tile_xch(D); }
 
 typedef float f32x16 __attribute__((__vector_size__(16 * sizeof(float))));
@@ -1227,7 +1227,7 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
         const int tr = 128;
         p.grid_tiles = (T * g / tr + std::min((int64_t)B, T * g / (p.row_limit + 1) + 1)) * kv_heads;
         p.tiles = max_q > 0 ? std::min(p.grid_tiles, (int64_t)B * ((max_q * g + tr - 1) / tr) * kv_heads) : p.grid_tiles;
-        const int64_t slots = (int64_t)device_cus() * (D >= 256 ? 1 : 2);
+        const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2);
         p.nsplit = (int)std::max((int64_t)1, std::min((int64_t)64, slots / p.tiles));
         if (p.nsplit > 1) p.part_bytes += (uint64_t)p.tiles * p.nsplit * tr * (D + 2) * sizeof(float);
     }
