@@ -333,6 +333,10 @@ __device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, S
     return total;
 }
 
+__device__ __forceinline__ uint64_t div32(uint64_t a, uint64_t b) {  // (32 bits take a third of the steps)
+    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
+}
+
 struct Found {
     RowsSeq s;
     int seq, kvh, rt;
@@ -358,7 +362,7 @@ __device__ __forceinline__ Found scan_find(const PagedAttnArgs& a, int lane, Sca
     const uint64_t seq_work = (uint64_t)f.s.tiles * a.kv_heads * f.s.nu;
     const uint64_t start = sc.base + lane_u64(sc.incl, l) - seq_work;
     const uint64_t in = x - start;
-    const uint64_t tile = in >> 32 ? in / (uint32_t)f.s.nu : (uint32_t)in / (uint32_t)f.s.nu;
+    const uint64_t tile = div32(in, (uint32_t)f.s.nu);
     f.u = uniform((int)(in - tile * f.s.nu));
     f.tile0 = start + tile * f.s.nu;
     f.kvh = uniform((int)((uint32_t)tile / (uint32_t)f.s.tiles));
@@ -366,13 +370,26 @@ __device__ __forceinline__ Found scan_find(const PagedAttnArgs& a, int lane, Sca
     return f;
 }
 
-// Where part w of the line begins.
-__device__ __forceinline__ uint64_t part_begin(uint64_t total, uint32_t parts, uint32_t w) {
-    const uint64_t q = total / parts, r = total - q * parts;
-    return q * w + min((uint64_t)w, r);
+// The line of `total` units cut into n parts, the first r of them a unit longer.
+struct Cut {
+    uint64_t q;
+    uint32_t r, n;
+    __device__ __forceinline__ uint64_t begin(uint32_t w) const { return q * w + min(w, r); }
+    __device__ __forceinline__ uint32_t part_of(uint64_t x) const {  // that holds place x
+        const uint64_t longer = (q + 1) * r;
+        return (uint32_t)(x < longer ? div32(x, q + 1) : r + div32(x - longer, q));
+    }
+};
+__device__ __forceinline__ Cut make_cut(uint64_t total, uint32_t n) {
+    Cut c;
+    c.n = n;
+    c.q = n ? div32(total, n) : 0;
+    c.r = (uint32_t)(total - c.q * n);
+    return c;
 }
+
 // At most kPartsPerTile parts per tile on average: the merge reads them all (one
-// token over 8000 positions on one kv head of 512: 250 parts 117 us, 125 40, 64 XX).
+// token over 8000 positions on one kv head of 512: 250 parts 117 us, 125 40, 64 33).
 __device__ __forceinline__ uint32_t part_count(uint64_t total, const Scan& sc, int grid) {
     return (uint32_t)min((uint64_t)min((uint32_t)grid, sc.tiles * kPartsPerTile), total);
 }
@@ -390,10 +407,10 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
     const int col = lane & 15, G = lane >> 4;
     Scan sc;
     const uint64_t total = scan_all<ROWS, UNIT>(a, lane, sc);
-    const uint32_t parts = part_count(total, sc, gridDim.x);
-    if (blockIdx.x >= parts) return;
-    uint64_t x = part_begin(total, parts, blockIdx.x);
-    const uint64_t end = part_begin(total, parts, blockIdx.x + 1);
+    const Cut cut = make_cut(total, part_count(total, sc, gridDim.x));
+    if (blockIdx.x >= cut.n) return;
+    uint64_t x = cut.begin(blockIdx.x);
+    const uint64_t end = cut.begin(blockIdx.x + 1);
 
     unsigned char* ring = smem + wave * NS * rows_stage(D);
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
@@ -703,18 +720,16 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
     const int r = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
     Scan sc;
     const uint64_t total = scan_all<ROWS, UNIT>(a, lane, sc);
-    const uint32_t parts = part_count(total, sc, grid), w = blockIdx.x + 1;
-    if (w >= parts) return;
-    const uint64_t x = part_begin(total, parts, w);
-    const Found f = scan_find<ROWS, UNIT>(a, lane, sc, x);
-    if (f.u == 0 || part_begin(total, parts, w - 1) > f.tile0) return;
+    const Cut cut = make_cut(total, part_count(total, sc, grid));
+    const uint32_t w = blockIdx.x + 1;
+    if (w >= cut.n) return;
+    const Found f = scan_find<ROWS, UNIT>(a, lane, sc, cut.begin(w));
+    if (f.u == 0 || cut.begin(w - 1) > f.tile0) return;
     if (r >= min(ROWS, f.s.n * a.g - f.rt * ROWS)) return;
-    const uint64_t tile1 = f.tile0 + f.s.nu;
     // Part w - 1 holds the tile's begin in its second place, the later ones
     // theirs in the first.
     auto place = [&](uint32_t v) { return a.part + (size_t)(2 * v + (v == w - 1 ? 1 : 0)) * rows_part(D, QT); };
-    uint32_t last = w;
-    while (last + 1 < parts && part_begin(total, parts, last + 1) < tile1) ++last;
+    const uint32_t last = cut.part_of(f.tile0 + f.s.nu - 1);
     const int n = (int)(last - w + 2);
     float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
     join_parts<RW>(
@@ -935,12 +950,17 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
         bf16x8 k[KR];
 #pragma unroll
         for (int i = 0; i < KR; ++i) k[i] = read_k(i);
+        // The products go ahead of the other workgroup's softmax (three chunks in a
+        // 1024 window at D = 256: 78 -> 75 us, 8192 tokens 532 -> 509). At D = 512 the
+        // two groups of waves already take turns, and it costs: 4096 tokens 323 -> 331.
+        if constexpr (DS == 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < DW / 16; ++i) {
             __builtin_amdgcn_sched_barrier(0);
             s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i % KR], q[i], s, 0, 0, 0);
             if (i + KR < DW / 16) k[i % KR] = read_k(i + KR);
         }
+        if constexpr (DS == 1) __builtin_amdgcn_s_setprio(0);
         return s;
     };
     // Their weights, and the output's share of V.
@@ -1009,12 +1029,14 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
         bf16x8 v[VR];
 #pragma unroll
         for (int j = 0; j < VR; ++j) v[j] = read_v(blk(j), j >> 1 & 1);
+        if constexpr (DS == 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             __builtin_amdgcn_sched_barrier(0);
             o[blk(j)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[j % VR], pw[j >> 1 & 1], o[blk(j)], 0, 0, 0);
             if (j + VR < NV) v[j % VR] = read_v(blk(j + VR), (j + VR) >> 1 & 1);
         }
+        if constexpr (DS == 1) __builtin_amdgcn_s_setprio(0);
     };
 
     if (u1 > u0) {
@@ -1212,7 +1234,9 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     const int64_t most = (max_q > 0 ? std::min(max_q, T) : T) * g;          // rows of a sequence at most
     const int64_t rows = (max_q > 0 ? std::min(max_q, T) : (T + B - 1) / B) * g;  // as far as is known
     const bool tiles = B == 1 ? most > 16 * qt_max : rows > 16 * qt_max;
-    const bool stream = !(B == 1 && tiles);
+    // No sequence is left for the streaming kernel where there is one, or all have
+    // max_q rows (should they not, the tile kernel takes them all the same).
+    const bool stream = !(tiles && (B == 1 || (max_q > 0 && (int64_t)B * max_q <= T)));
     if (stream) {
         const int64_t r = tiles ? g : rows;
         p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
