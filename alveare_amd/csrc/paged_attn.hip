@@ -824,6 +824,31 @@ __device__ __forceinline__ int tile_count(const PagedAttnArgs& a, int lane) {
 // Splits per tile: as planned, unless there are more tiles than the plan knew of.
 __device__ __forceinline__ int tile_splits(const PagedAttnArgs& a, int items) { return items <= a.max_items ? a.nsplit : 1; }
 
+// Where item `item` is.
+template <int TR, int BN>
+struct TileAt {
+    int seq, kvh, rt, first, n, len;
+    TileSpan sp;
+    __device__ __forceinline__ TileAt(const PagedAttnArgs& a, int item, int lane) {
+        const int gt = item / a.kv_heads;
+        kvh = item - gt * a.kv_heads;
+        int base = 0, b0 = 0;
+        TileScan sc = tile_scan<TR>(a, 0, lane);
+        while (gt >= base + sc.sum) {
+            base += sc.sum;
+            b0 += 64;
+            sc = tile_scan<TR>(a, b0, lane);
+        }
+        const int l = __builtin_ctzll(__ballot(base + sc.incl > gt));
+        seq = b0 + l;
+        first = __builtin_amdgcn_readlane(sc.first, l);
+        n = __builtin_amdgcn_readlane(sc.n, l);
+        len = __builtin_amdgcn_readlane(sc.len, l);
+        rt = gt - base - __builtin_amdgcn_readlane(sc.incl - sc.tiles, l);
+        sp = tile_span<TR, BN>(a, n, len, __builtin_amdgcn_readlane((int)sc.ok, l) != 0, rt);
+    }
+};
+
 template <int D>
 __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int split, int nsplit, unsigned char* smem) {
     constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D);
@@ -841,21 +866,10 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
     const int rg = wave / DS, dh = wave % DS;
     const int col = lane & 31, h = lane >> 5;
 
-    const int gt = item / a.kv_heads, kvh = item - gt * a.kv_heads;
-    int base = 0, b0 = 0;
-    TileScan sc = tile_scan<TR>(a, 0, lane);
-    while (gt >= base + sc.sum) {
-        base += sc.sum;
-        b0 += 64;
-        sc = tile_scan<TR>(a, b0, lane);
-    }
-    const int l0 = __builtin_ctzll(__ballot(base + sc.incl > gt));
-    const int seq = b0 + l0;
-    const int first = __builtin_amdgcn_readlane(sc.first, l0), n = __builtin_amdgcn_readlane(sc.n, l0);
-    const int len = __builtin_amdgcn_readlane(sc.len, l0);
-    const bool ok = __builtin_amdgcn_readlane((int)sc.ok, l0) != 0;
-    const int rt = gt - base - __builtin_amdgcn_readlane(sc.incl - sc.tiles, l0);
-    const TileSpan sp = tile_span<TR, BN>(a, n, len, ok, rt);
+    const TileAt<TR, BN> at_item(a, item, lane);
+    const int seq = at_item.seq, kvh = at_item.kvh, rt = at_item.rt;
+    const int first = at_item.first, n = at_item.n, len = at_item.len;
+    const TileSpan sp = at_item.sp;
     const int u0 = uniform((int)((int64_t)sp.nu * split / nsplit));
     const int u1 = uniform((int)((int64_t)sp.nu * (split + 1) / nsplit));
     if (nsplit > 1 && u0 == u1) return;  // the merge skips it too
@@ -1107,6 +1121,14 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
     }
 
     float* part = a.part + ((int64_t)item * nsplit + split) * (TR * (D + 2));
+    if constexpr (DS == 2) {  // found in either half's columns
+        int* odds = reinterpret_cast<int*>(xch);
+        __syncthreads();
+        if (lane == 0) odds[wave] = 0;
+        if (__any(odd != 0) && lane == 0) odds[wave] = 1;
+        __syncthreads();
+        odd = odds[wave] | odds[wave ^ 1];
+    }
     if (__any(odd != 0)) {  // see plain_row; with two waves per row, one does it
         for (int r = 0; dh == 0 && r < nrows; ++r) {
             const int64_t rr = r0 + r;
@@ -1165,45 +1187,61 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
     if (item >= 0) tile_item<D>(a, item, (int)(blockIdx.x % (uint32_t)nsplit), nsplit, smem);
 }
 
-// The splits of the tiles joined: a wave per (packed row, q head).
+// The splits of the tiles joined, `groups` workgroups to a tile, merge_rows(D) of
+// its rows at a time: the parts' factors first, a row per wave and a part per
+// lane, into LDS, then the outputs, 16 bytes per lane and part.
+constexpr int merge_rows(int D) { return 1024 / D; }
 template <int D>
-__global__ void __launch_bounds__(64) attn_paged_tile_merge_kernel(PagedAttnArgs a) {
-    constexpr int TR = tile_rows(D), BN = tile_bn(D), RW = D / 64;
-    const int lane = threadIdx.x, t = blockIdx.x, head = blockIdx.y;
-    const int nsplit = tile_splits(a, tile_count<TR>(a, lane));
-    if (nsplit == 1) return;
-    int base = 0;
-    for (int b0 = 0; b0 < a.b.B; b0 += 64) {
-        const TileScan sc = tile_scan<TR>(a, b0, lane);
-        const uint64_t mine = __ballot(sc.tiles > 0 && sc.first <= t && t < sc.first + sc.n);
-        if (!mine) {
-            base += sc.sum;
-            continue;
-        }
-        const int l0 = __builtin_ctzll(mine);
-        const int first = __builtin_amdgcn_readlane(sc.first, l0), n = __builtin_amdgcn_readlane(sc.n, l0);
-        const int len = __builtin_amdgcn_readlane(sc.len, l0);
-        const bool ok = __builtin_amdgcn_readlane((int)sc.ok, l0) != 0;
-        const int kvh = head / a.g;
-        const int64_t row = (int64_t)(t - first) * a.g + (head - kvh * a.g);
-        const int rt = (int)(row / TR), r = (int)(row % TR);
-        const int gt = base + __builtin_amdgcn_readlane(sc.incl - sc.tiles, l0) + rt;
-        const TileSpan sp = tile_span<TR, BN>(a, n, len, ok, rt);
-        const float* part = a.part + ((int64_t)gt * a.kv_heads + kvh) * nsplit * (TR * (D + 2));
-        // (a tile of fewer units than splits leaves some empty: spread over nu of them)
-        const int np = min(nsplit, sp.nu);
-        auto at = [&](int v) {
-            return part + (int64_t)(np == nsplit ? v : ((int64_t)(v + 1) * nsplit - 1) / sp.nu) * (TR * (D + 2));
-        };
-        float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
-        join_parts<RW>(
-            np, lane, [&](int v) { return at(v) + TR * D + r; }, TR, [&](int v) { return at(v) + r * D + RW * lane; }, acc, mx,
-            ls);
-        const float inv = inverse(ls);
-        uint16_t* dst = a.out + (int64_t)t * a.ld_out + head * D + RW * lane;
+__global__ void __launch_bounds__(256) attn_paged_tile_merge_kernel(PagedAttnArgs a, int groups) {
+    constexpr int TR = tile_rows(D), BN = tile_bn(D), R = merge_rows(D), C = D / 4;  // 16-byte pieces of a row
+    __shared__ float fac[R][64];
+    __shared__ float inv[R];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int items = tile_count<TR>(a, lane), nsplit = tile_splits(a, items);
+    const int item = blockIdx.x / groups;
+    if (nsplit == 1 || item >= items) return;
+    const TileAt<TR, BN> t(a, item, lane);
+    const float* part = a.part + (int64_t)item * nsplit * (TR * (D + 2));
+    // (a tile of fewer units than splits leaves some empty: spread over nu of them)
+    const int np = min(nsplit, t.sp.nu);
+    auto at = [&](int v) { return part + (np == nsplit ? v : ((v + 1) * nsplit - 1) / max(np, 1)) * (TR * (D + 2)); };
+    const float* mine = at(max(min(lane, np - 1), 0));
+    for (int r0 = blockIdx.x % groups * R; r0 < t.sp.rows; r0 += groups * R) {
+        const int rows = min(R, t.sp.rows - r0), r = tid / C, c = tid % C;
+        f32x4 acc{}, x[8];
+        auto load = [&](int v0) {
 #pragma unroll
-        for (int e = 0; e < RW; ++e) dst[e] = bf16_rne_bits(acc[e] * inv);
-        return;
+            for (int q = 0; q < 8; ++q)
+                x[q] = v0 + q < np && r < rows ? *reinterpret_cast<const f32x4*>(at(v0 + q) + (r0 + r) * D + 4 * c)
+                                               : f32x4{0, 0, 0, 0};
+        };
+        load(0);
+#pragma unroll
+        for (int w = wave; w < R; w += 4) {
+            const int rr = r0 + min(w, rows - 1);
+            const float m = lane < np ? mine[TR * D + rr] : kNoMax, l = lane < np ? mine[TR * (D + 1) + rr] : 0.0f;
+            float top = m;
+#pragma unroll
+            for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+            const float f = __builtin_amdgcn_exp2f(m - top);
+            float sum = l * f;
+#pragma unroll
+            for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+            fac[w][lane] = f;
+            if (lane == 0) inv[w] = inverse(sum);
+        }
+        __syncthreads();
+        for (int v0 = 0; v0 < np; v0 += 8) {
+            if (v0) load(v0);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) acc += x[q] * fac[r][v0 + q];
+        }
+        if (r < rows) {
+            const int64_t rr = (int64_t)t.rt * TR + r0 + r;
+            const int tok = (int)(rr / a.g), head = t.kvh * a.g + (int)(rr % a.g);
+            store4(a.out + (int64_t)(t.first + tok) * a.ld_out + head * D + 4 * c, acc, inv[r]);
+        }
+        __syncthreads();
     }
 }
 
@@ -1290,7 +1328,9 @@ int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     hipLaunchKernelGGL((attn_paged_tile_kernel<D>), dim3((uint32_t)(p.grid_tiles * p.nsplit)), dim3(64 * tile_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_tile_kernel launch")) return rc;
     if (p.nsplit == 1) return ALV_OK;
-    hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D>), dim3(a.b.T, a.heads), dim3(64), 0, s, a);
+    // Few tiles are joined by as many workgroups as they have rows for, many by fewer each.
+    const int groups = (int)std::max((int64_t)1, std::min((int64_t)tile_rows(D) / merge_rows(D), 1024 / p.tiles));
+    hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D>), dim3((uint32_t)p.tiles * groups), dim3(256), 0, s, a, groups);
     return hip_check(hipGetLastError(), "attn_paged_tile_merge_kernel launch");
 }
 

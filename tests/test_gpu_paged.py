@@ -491,3 +491,50 @@ def test_cache_contents_follow_the_bookkeeping(dev):
                 if held[w]:
                     got = x[t].transpose(1, 2).reshape(-1, H * D)[:len(held[w]), :2].long()
                     assert (got[:, 0] + 128 * got[:, 1]).tolist() == held[w], (step, act)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("part", [0.0, 0.5, 0.999])
+@pytest.mark.parametrize("n,total", [(5, 70), (150, 150), (150, 1500)])
+def test_attention_an_infinity_in_one_column_of_v(dev, D, part, n, total):
+    """The last token's v, which only its own row may see."""
+    from alveare_amd import attention_paged
+
+    heads, col = 2, int(part * D)
+    b = R.Batch([n], [total], kv_heads=1, D=D, page=32, dev=dev)
+    b.kp[int(b.table[0, (total - 1) // 32]), 0, (total - 1) % 32] = 0  # its weight is no zero
+    b.k[0][total - 1] = 0
+    q = rows(n, heads * D, dev, 5)
+    want, tol = R.attention(q, b, heads, scale=0.05)
+    b.vp[int(b.table[0, (total - 1) // 32]), 0, (total - 1) % 32, col] = math.inf
+    for mq in (0, n):
+        got = attention_paged(q, *b.args(), heads=heads, scale=0.05, max_q=mq).double().cpu().view_as(want)
+        hit = torch.zeros_like(want, dtype=torch.bool)
+        hit[-1, :, col] = True
+        assert (got[hit] == math.inf).all()
+        assert torch.isfinite(got[~hit]).all()
+        assert ((got - want).abs() <= tol)[~hit].all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,D", [(8, 2, 64), (4, 1, 128), (4, 2, 256), (8, 1, 512)])
+@pytest.mark.parametrize("n,past", [([200, 1, 1, 2, 1, 1], [0, 500, 33, 128, 0, 64]), ([1, 130, 150], [900, 20, 0]),
+                                    ([70, 70, 70], [0, 10, 200])])
+def test_attention_chunks_and_single_tokens(dev, heads, kv_heads, D, n, past):
+    """Both kinds of sequences in one call, and every max_q: a wrong one costs time alone."""
+    b = R.Batch(n, [a + c for a, c in zip(n, past)], kv_heads=kv_heads, D=D, page=32, dev=dev)
+    q = rows(b.T, heads * D, dev, 6)
+    want, tol = R.attention(q, b, heads, scale=0.1)
+    from alveare_amd import attention_paged
+
+    for mq in (0, 1, 17, max(n) // 2, max(n) - 1, max(n), 10 * max(n)):
+        got = attention_paged(q, *b.args(), heads=heads, scale=0.1, max_q=mq).double().cpu().view_as(want)
+        assert ((got - want).abs() <= tol).all(), f"max_q={mq}"
+
+
+@pytest.mark.parametrize("D", [64, 512])
+def test_attention_seventy_chunks(dev, D):
+    """More sequences than lanes, of one tile each and more, with empty ones among them."""
+    n = [(7 * i) % 53 for i in range(70)]
+    past = [(11 * i) % 90 for i in range(70)]
+    b = R.Batch(n, [a + c for a, c in zip(n, past)], kv_heads=1, D=D, page=16, dev=dev)
+    check_attention(b, 4, dev)
