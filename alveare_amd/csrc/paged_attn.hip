@@ -25,6 +25,7 @@ struct PagedAttnArgs {
     uint16_t* out;
     int64_t ld_out;
     int64_t row_limit;  // sequences of more rows (tokens times q heads per kv head) are not this launch's
+    int max_tiles;      // tiles of all sequences, per kv head, at most
     int nsplit;         // parts of a tile's positions, unless there are more than max_items tiles
     int max_items;
     float* part;
@@ -325,7 +326,7 @@ __device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, S
     for (int b0 = 64; b0 < a.b.B; b0 += 64) {
         Scan t;
         scan_step<ROWS, UNIT>(a, b0, lane, 0, t);
-        total += t.sum;
+        total = min(total + t.sum, (uint64_t)1 << 62);  // (sequences that overlap: no wrap)
         tiles = min(tiles + (t.s.nu ? min(t.s.tiles, kPartsPerTile) : 0), 1u << 24);
     }
     for (int k = 32; k; k >>= 1) tiles += __shfl_xor(tiles, k);
@@ -818,7 +819,8 @@ __device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int
 template <int TR>
 __device__ __forceinline__ int tile_count(const PagedAttnArgs& a, int lane) {
     int all = 0;
-    for (int b0 = 0; b0 < a.b.B; b0 += 64) all += tile_scan<TR>(a, b0, lane).sum;
+    // (no more than there can be: sequences that overlap must not carry the sum away)
+    for (int b0 = 0; b0 < a.b.B; b0 += 64) all = min(all + tile_scan<TR>(a, b0, lane).sum, a.max_tiles);
     return all * a.kv_heads;
 }
 // Splits per tile: as planned, unless there are more tiles than the plan knew of.
@@ -1384,7 +1386,11 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
     a.q = q, a.ld_q = ld_q, a.kpages = kpages, a.vpages = vpages, a.k_stride = k_stride, a.v_stride = v_stride;
     a.heads = heads, a.kv_heads = kv_heads, a.g = heads / kv_heads, a.window = window, a.sinks = sinks, a.scale = scale;
     a.out = out, a.ld_out = ld_out;
+    if ((int64_t)T * heads > (int64_t)1 << 30)  // (the largest launch: 2^32 threads)
+        return fail(ALV_ERR_RANGE, "%d rows of %d heads in one call (at most 2^30 rows times heads)", T, heads);
     const AttnPlan p = attn_plan(heads, kv_heads, D, B, T, max_q);
+    if (p.grid_tiles * p.nsplit * 512 > (int64_t)UINT32_MAX)
+        return fail(ALV_ERR_RANGE, "%d rows of %d heads in %d sequences: too many tiles for one call", T, heads, B);
     if (p.part_bytes && (!workspace || workspace_bytes < p.part_bytes))
         return fail(ALV_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
                     (unsigned long long)p.part_bytes);
@@ -1393,6 +1399,7 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
     a.row_limit = p.row_limit;
     a.nsplit = p.nsplit;
     a.max_items = (int)std::min(p.tiles, (int64_t)INT_MAX);
+    a.max_tiles = (int)(p.grid_tiles / kv_heads);
     const hipStream_t s = (hipStream_t)stream;
     switch (D) {
         case 64: return launch_d<64>(a, p, s);

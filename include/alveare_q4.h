@@ -476,7 +476,8 @@ int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off
  * gets zeros. K and V of a position that a row does not see do not reach it,
  * whatever they hold. Scores that are all -infinity count as unseen. D one of
  * 64, 128, 256, 512; scale finite, not negative; q, its rows, the pages and
- * their strides 16-byte aligned, out and its rows 8-byte.
+ * their strides 16-byte aligned, out and its rows 8-byte; T * heads at most
+ * 2^30; out does not overlap q.
  *
  * max_q: the most rows that any sequence owns, if the caller knows (0: not
  * known). It decides how the work is spread, not what is computed: a value too

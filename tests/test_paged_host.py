@@ -42,6 +42,7 @@ def test_attention_arguments(L):
                dict(table=ctypes.c_void_p((1 << 20) + 1))):
         assert attn(L, **ch) == ALV_ERR_ALIGN, ch
     assert attn(L, T=(1 << 22) + 1) == ALV_ERR_RANGE
+    assert attn(L, T=1 << 22, heads=512, ld_q=1 << 15, ldo=1 << 15) == ALV_ERR_RANGE
     assert attn(L, W=1 << 27, ldt=1 << 27) == ALV_ERR_RANGE
     assert attn(L, T=0, q=None, out=None) == ALV_OK
 
