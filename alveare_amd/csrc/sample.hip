@@ -72,7 +72,7 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// exp(-x), x >= 0: with n = rint(x / ln 2) and y = n ln 2 - x, |y| <= 0.347, it
+// exp(-x), 0 <= x < 700: with n = rint(x / ln 2) and y = n ln 2 - x, |y| <= 0.347, it
 // is 2^-n times the Taylor sum of exp(y) to y^12 / 12! (the rest is below 2^-52).
 // The float64 library function, exact to the last bit, takes twice as long.
 __device__ __forceinline__ double exp_neg(double x) {
@@ -91,13 +91,17 @@ __device__ __forceinline__ double exp_neg(double x) {
     p = fma(p, y, 0.5);
     p = fma(p, y, 1.0);
     p = fma(p, y, 1.0);
-    return x < 700.0 ? __builtin_ldexp(p, -(int)n) : 0.0;
+    return __builtin_ldexp(p, -(int)n);
 }
 // exp((l - m) / T): 1 for l = m also where both are infinite.
 __device__ __forceinline__ double weight(float l, float m, double inv_t) {
-    return l == m ? 1.0 : exp_neg(((double)m - (double)l) * inv_t);
+    const double x = l == m ? 0.0 : ((double)m - (double)l) * inv_t;
+    return x < 700.0 ? exp_neg(x) : 0.0;
 }
-__device__ __forceinline__ uint64_t fixed(double w, double scale) { return (uint64_t)rint(w * scale); }
+// w * scale to the nearest integer, at most 2^52: the last bits of 2^52 plus it.
+__device__ __forceinline__ uint64_t fixed(double w, double scale) {
+    return __builtin_bit_cast(uint64_t, fma(w, scale, 0x1p52)) - __builtin_bit_cast(uint64_t, 0x1p52);
+}
 
 // Targets of the three crossings. top-p keeps what begins below ceil(p S); a
 // token is drawn at floor(u Z).
@@ -275,19 +279,19 @@ __device__ void sample_row(const SampleArgs& a, int b, const RowParams& rp, RowS
 
 // ---- several workgroups per row -----------------------------------------------------
 //
-// Five launches: the pieces' largest logits; a histogram of each piece over x =
-// (l_0 - l) / T, from 0 to where a weight rounds to nothing (or the row's range);
-// the row's sum of them, which tells the bins in which the three crossings can
-// fall; the collection of those bins' tokens; the crossings among those, by
-// comparison where they are few, else by a finer histogram first. Every step
-// moves integers, so no order of atomics shows. A row whose bins hold too many
-// (logits all alike but for a few far ones) is done by sample_row.
+// Four launches: the pieces' largest logits; a histogram of the row over x = (l_0 -
+// l) / T, from 0 to where a weight rounds to nothing (or the row's range); from
+// its prefix sums the bins in which the three crossings can fall, and the
+// collection of those bins' tokens; the crossings among those, by comparison
+// where they are few, else by a finer histogram first. Every step moves integers,
+// so no order of atomics shows. A row whose bins hold too many (logits all alike
+// but for a few far ones) is done by sample_row.
 //
 // What bounds it: one row is a chain of launches, each a trip or two to memory;
-// many rows, the float64 exponentials (two per logit's weight, 12 terms).
+// many rows, the histograms' atomics and the float64 exponentials.
 constexpr int kPieceThreads = 256;
 constexpr int kWaves = kPieceThreads / 64;
-constexpr int kPiece = 16 * kPieceThreads;  // logits per workgroup
+constexpr int kPiece = 16 * kPieceThreads;  // logits per workgroup (2 or 4 times as many are slower by a half: too few loads on their way)
 constexpr int kCoarse = 1024;     // bins
 constexpr int kFine = 2048;       // finer bins of the collected ones
 constexpr int kCand = 4096;       // tokens collected per row
@@ -305,26 +309,28 @@ struct RowWork {  // per row
     float* cp;          // places in the histogram
     int* ci;            // and indices
     uint32_t* want;     // [kCoarse / 32] a bit per bin to collect
-    uint32_t* n;        // collected; kCand + 1 and above: too many
+    uint32_t* n;        // collected
+    uint32_t* over;     // not 0: those bins hold more than kCand
 };
 
-__host__ __device__ inline uint64_t up16(uint64_t v) { return (v + 15) & ~(uint64_t)15; }
+// (offsets of 16 bytes up to where the pieces' values begin)
 __host__ __device__ inline uint64_t row_bytes(int pieces) {
-    return up16(8ull * (pieces + 2 * kCoarse + 1 + kCand) + 4ull * (3ull * pieces + 2 * kCoarse + 1 + 3 * kCand + kCoarse / 32 + 1));
+    return 8ull * (2 * kCoarse + 2 + kCand) + 4ull * (2 * kCoarse + 4 + 3 * kCand + kCoarse / 32 + 4) + (20ull * pieces + 15 & ~15ull);
 }
 __device__ __forceinline__ RowWork row_work(const SampleArgs& a, int b) {
     RowWork w;
     unsigned char* p = a.work + (uint64_t)b * row_bytes(a.pieces);
     w.sum = reinterpret_cast<unsigned long long*>(p);
-    w.cw = w.sum + 2 * kCoarse + 1;
-    w.minp = w.cw + kCand;
-    w.cnt = reinterpret_cast<uint32_t*>(w.minp + a.pieces);
-    w.cl = reinterpret_cast<float*>(w.cnt + 2 * kCoarse + 1);
+    w.cw = w.sum + 2 * kCoarse + 2;
+    w.cnt = reinterpret_cast<uint32_t*>(w.cw + kCand);
+    w.cl = reinterpret_cast<float*>(w.cnt + 2 * kCoarse + 4);
     w.cp = w.cl + kCand;
     w.ci = reinterpret_cast<int*>(w.cp + kCand);
     w.want = reinterpret_cast<uint32_t*>(w.ci + kCand);
     w.n = w.want + kCoarse / 32;
-    w.top = reinterpret_cast<float*>(w.n + 1);
+    w.over = w.n + 1;
+    w.minp = reinterpret_cast<unsigned long long*>(w.n + 4);
+    w.top = reinterpret_cast<float*>(w.minp + a.pieces);
     w.low = w.top + a.pieces;
     w.at = reinterpret_cast<int*>(w.low + a.pieces);
     return w;
@@ -338,8 +344,8 @@ __device__ __forceinline__ bool ahead(float va, int ia, float vb, int ib) {
     return va > vb || ((va == vb || na) && ia < ib);
 }
 
-// This thread's 16 logits of the piece, in 4 groups of 4 (index i0 + 4 kPieceThreads
-// g + e); -infinity past the row.
+// This thread's 16 logits of the piece, in 4 groups of 4 (index base + 4
+// kPieceThreads g + 4 tid + e); -infinity past the row.
 __device__ __forceinline__ void load_piece(const float* l, int V, int base, int tid, float (&v)[16]) {
     if ((reinterpret_cast<uintptr_t>(l) & 15) == 0 && base + kPiece <= V) {
 #pragma unroll
@@ -391,6 +397,7 @@ __global__ void __launch_bounds__(kPieceThreads) sample_top_kernel(SampleArgs a)
         rw.top[blockIdx.x] = m;
         rw.at[blockIdx.x] = mi;
         rw.low[blockIdx.x] = lo;
+        if (blockIdx.x == 0) *rw.n = 0;
     }
     // The row's histogram, clear for the next launch.
     for (int i = blockIdx.x * kPieceThreads + tid; i < kCoarse; i += a.pieces * kPieceThreads) {
@@ -483,122 +490,135 @@ __global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(SampleArgs a
     }
 }
 
-// One workgroup per row, a bin per thread: the row's histogram and its prefix,
-// and the bins in which the crossings can fall.
-__global__ void __launch_bounds__(kCoarse) sample_plan_kernel(SampleArgs a) {
-    constexpr int NW = kCoarse / 64;
-    __shared__ unsigned long long wsum[NW], pre[kCoarse + 1];
-    __shared__ uint32_t wcnt[NW], prec[kCoarse + 1];
-    __shared__ int hit;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
-    const RowWork rw = row_work(a, b);
-    const RowParams rp = row_params(a, b);
-    const RowRange rr = row_range(a, rw, rp, lane);
-    if (rr.done) return;
-    uint32_t c = rw.cnt[tid];
-    uint64_t w = rw.sum[tid], Sm = 0;
-    for (int g = lane; g < a.pieces; g += 64) Sm += rw.minp[g];
-    for (int o = 32; o; o >>= 1) Sm += __shfl_xor((unsigned long long)Sm, o);
-    const uint32_t c0 = c;
-    const uint64_t w0 = w;
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t cu = __shfl_up(c, o);
-        const uint64_t wu = __shfl_up((unsigned long long)w, o);
-        if (lane >= o) c += cu, w += wu;
+// The prefix of a row's histogram, and the bins in which the crossings can fall.
+struct PlanShared {
+    unsigned long long pre[kCoarse + 1], wsum[kWaves];
+    uint32_t prec[kCoarse + 1], wcnt[kWaves], want[kCoarse / 32];
+    int hit;
+};
+// The tokens those bins hold. Each thread has kCoarse / kPieceThreads bins.
+__device__ __forceinline__ uint32_t row_plan(const SampleArgs& a, const RowWork& rw, const RowParams& rp, PlanShared& s) {
+    constexpr int E = kCoarse / kPieceThreads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t c[E + 1], own = 0;  // before bin E tid + e
+    uint64_t w[E + 1], ownw = 0, Sm = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        c[e] = rw.cnt[E * tid + e];
+        w[e] = rw.sum[E * tid + e];
     }
-    if (lane == 63) wcnt[wave] = c, wsum[wave] = w;
+    for (int g = lane; g < a.pieces; g += 64) Sm += rw.minp[g];
+    if (tid < kCoarse / 32) s.want[tid] = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) own += c[e], ownw += w[e];
+    for (int o = 32; o; o >>= 1) Sm += __shfl_xor((unsigned long long)Sm, o);
+    uint32_t ci = own;
+    uint64_t wi = ownw;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t cu = __shfl_up(ci, o);
+        const uint64_t wu = __shfl_up((unsigned long long)wi, o);
+        if (lane >= o) ci += cu, wi += wu;
+    }
+    if (lane == 63) s.wcnt[wave] = ci, s.wsum[wave] = wi;
     __syncthreads();
-    for (int i = 0; i < wave; ++i) c += wcnt[i], w += wsum[i];
-    prec[tid + 1] = c;
-    pre[tid + 1] = w;
-    if (tid == 0) prec[0] = 0, pre[0] = 0;
-    const uint32_t cb = c - c0;
-    const uint64_t wb = w - w0;
+    ci -= own, wi -= ownw;
+    for (int i = 0; i < wave; ++i) ci += s.wcnt[i], wi += s.wsum[i];
+#pragma unroll
+    for (int e = 0; e <= E; ++e) {
+        const uint32_t cn = e < E ? c[e] : 0;
+        const uint64_t wn = e < E ? w[e] : 0;
+        c[e] = ci, w[e] = wi;
+        if (e < E || tid == kPieceThreads - 1) s.prec[E * tid + e] = ci, s.pre[E * tid + e] = wi;
+        ci += cn, wi += wn;
+    }
     __syncthreads();
-    const uint64_t S = pre[kCoarse];
-    bool want = false;
+    const uint64_t S = s.pre[kCoarse];
     // The bin in which a count or a sum of x crosses.
     auto bin_at = [&](bool by_count, uint64_t x) {
         __syncthreads();
-        if (by_count ? (cb <= x && x < c) : (wb <= x && x < w)) hit = tid;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (by_count ? (c[e] <= x && x < c[e + 1]) : (w[e] <= x && x < w[e + 1])) s.hit = E * tid + e;
         __syncthreads();
-        return hit;
+        return s.hit;
     };
     uint64_t lo = S, hi = S;  // between what the sum of the kept lies
-    if ((uint32_t)rp.topk < prec[kCoarse]) {
-        const int t = bin_at(true, (uint64_t)rp.topk - 1);
-        lo = pre[t];
-        hi = pre[t + 1];
-        want = tid == t;
+    int t = -1, t0 = -1, t1 = -1;
+    if ((uint32_t)rp.topk < s.prec[kCoarse]) {
+        t = bin_at(true, (uint64_t)rp.topk - 1);
+        lo = s.pre[t];
+        hi = s.pre[t + 1];
     }
     if (rp.topp < 1.0) {
         const uint64_t p0 = topp_target(rp.topp, lo), p1 = topp_target(rp.topp, hi);
-        const int t0 = bin_at(false, p0 - 1), t1 = p1 == p0 ? t0 : bin_at(false, p1 - 1);
-        want |= tid >= t0 && tid <= t1;
-        lo = min(lo, (uint64_t)pre[t0]);
-        hi = min(hi, (uint64_t)pre[t1 + 1]);
+        t0 = bin_at(false, p0 - 1), t1 = p1 == p0 ? t0 : bin_at(false, p1 - 1);
+        lo = min(lo, (uint64_t)s.pre[t0]);
+        hi = min(hi, (uint64_t)s.pre[t1 + 1]);
     }
     lo = max(min(lo, Sm), (uint64_t)1);
     hi = max(min(hi, Sm), (uint64_t)1);
     const int d0 = bin_at(false, draw_target(rp.u, lo)), d1 = lo == hi ? d0 : bin_at(false, draw_target(rp.u, hi));
-    want |= tid >= d0 && tid <= d1;
-    const uint64_t bits = __ballot(want);
-    uint32_t total = want ? c0 : 0;
+    uint32_t bits = 0, total = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = E * tid + e;
+        if (i == t || (i >= t0 && i <= t1) || (i >= d0 && i <= d1)) bits |= 1u << e, total += c[e + 1] - c[e];
+    }
+    if (bits) atomicOr(&s.want[E * tid >> 5], bits << (E * tid & 31));
     for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
+    if (lane == 0) s.wcnt[wave] = total;
     __syncthreads();
-    if (lane == 0) {
-        wcnt[wave] = total;
-        rw.want[2 * wave] = (uint32_t)bits;
-        rw.want[2 * wave + 1] = (uint32_t)(bits >> 32);
-    }
-    rw.cnt[kCoarse + tid] = cb;
-    rw.sum[kCoarse + tid] = wb;
-    __syncthreads();
-    if (tid == 0) {
-        rw.cnt[2 * kCoarse] = prec[kCoarse];
-        rw.sum[2 * kCoarse] = S;
-        total = 0;
-        for (int i = 0; i < NW; ++i) total += wcnt[i];
-        *rw.n = total > kCand ? kCand + 1 : 0;
-    }
+    total = 0;
+    for (int i = 0; i < kWaves; ++i) total += s.wcnt[i];
+    return total;
 }
 
+// Each workgroup finds the bins for itself, 12 KB in cache: a launch less.
 __global__ void __launch_bounds__(kPieceThreads) sample_collect_kernel(SampleArgs a) {
-    __shared__ uint32_t want[kCoarse / 32];
-    __shared__ uint32_t found, at0;
+    __shared__ PlanShared s;
     const int tid = threadIdx.x, lane = tid & 63, b = blockIdx.y, base = blockIdx.x * kPiece;
     const RowWork rw = row_work(a, b);
     float v[16];
     load_piece(a.logits + b * a.ld, a.V, base, tid, v);
     const RowParams rp = row_params(a, b);
     const RowRange rr = row_range(a, rw, rp, lane);
-    if (rr.done || *rw.n > kCand) return;  // (while others add to it, n stays at kCand or below)
-    if (tid < kCoarse / 32) want[tid] = rw.want[tid];
-    if (tid == 0) found = 0;
-    __syncthreads();
+    if (rr.done) return;
+    const bool over = row_plan(a, rw, rp, s) > kCand;
+    if (blockIdx.x == 0) {  // for the last launch
+        for (int i = tid; i <= kCoarse; i += kPieceThreads) {
+            rw.cnt[kCoarse + i] = s.prec[i];
+            rw.sum[kCoarse + i] = s.pre[i];
+        }
+        if (tid < kCoarse / 32) rw.want[tid] = s.want[tid];
+        if (tid == 0) *rw.over = over;
+    }
+    if (over) return;
+    const double scale = __builtin_ldexp(1.0, a.shift);
     uint32_t mine = 0, mask = 0;
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
         const double x = x_of(v[k], rr, rp.inv_t);
         if (!(x < rr.end)) continue;
         const int bin = (int)place_of(x, rr);
-        if (want[bin >> 5] >> (bin & 31) & 1) mask |= 1u << k, ++mine;
+        if (s.want[bin >> 5] >> (bin & 31) & 1) mask |= 1u << k, ++mine;
     }
-    uint32_t at = mine ? atomicAdd(&found, mine) : 0;
-    __syncthreads();
-    if (tid == 0) at0 = found ? atomicAdd(rw.n, found) : 0;
-    __syncthreads();
-    at += at0;
-    const double scale = __builtin_ldexp(1.0, a.shift);
+    if (!__any(mine != 0)) return;
+    uint32_t at = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t u = __shfl_up(at, o);
+        if (lane >= o) at += u;
+    }
+    uint32_t first = lane == 63 ? atomicAdd(rw.n, at) : 0;
+    at += __shfl(first, 63) - mine;
 #pragma unroll 1
     for (int k = 0; __any(mask >> k); ++k) {
         if (!(mask >> k & 1)) continue;
-        float l = v[0];
+        float lk = v[0];
 #pragma unroll
-        for (int q = 1; q < 16; ++q) l = q == k ? v[q] : l;
-        rw.cl[at] = l;
-        rw.cp[at] = place_of(x_of(l, rr, rp.inv_t), rr);
-        rw.cw[at] = fixed(weight(l, rr.m, rp.inv_t), scale);
+        for (int q = 1; q < 16; ++q) lk = q == k ? v[q] : lk;
+        rw.cl[at] = lk;
+        rw.cp[at] = place_of(x_of(lk, rr, rp.inv_t), rr);
+        rw.cw[at] = fixed(weight(lk, rr.m, rp.inv_t), scale);
         rw.ci[at] = piece_index(base, tid, k);
         ++at;
     }
@@ -696,11 +716,11 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
         }
         return true;
     }
-    const uint32_t n = *rw.n;
+    const uint32_t n = *rw.n, over = *rw.over;
     const uint32_t all = rw.cnt[2 * kCoarse];
     uint64_t Z = rw.sum[2 * kCoarse], Sm = 0;
     for (int g = lane; g < a.pieces; g += 64) Sm += rw.minp[g];
-    if (n > kCand) return false;
+    if (over) return false;
     const double scale = __builtin_ldexp(1.0, a.shift);
     for (int o = 32; o; o >>= 1) Sm += __shfl_xor((unsigned long long)Sm, o);
     const bool cut = (uint32_t)rp.topk < all;
@@ -886,7 +906,7 @@ using namespace alv;
 namespace alv {
 namespace {
 // Short rows are one workgroup's work.
-int sample_pieces(int V) { return V <= 4096 ? 0 : (V + kPiece - 1) / kPiece; }
+int sample_pieces(int V) { return V <= kPiece ? 0 : (V + kPiece - 1) / kPiece; }
 }  // namespace
 }  // namespace alv
 
@@ -928,7 +948,6 @@ extern "C" int alv_sample(const float* logits, int64_t ld, int B, int V, const f
         const dim3 grid(a.pieces, B);
         hipLaunchKernelGGL(sample_top_kernel, grid, dim3(kPieceThreads), 0, st, a);
         hipLaunchKernelGGL(sample_hist_kernel, grid, dim3(kPieceThreads), 0, st, a);
-        hipLaunchKernelGGL(sample_plan_kernel, dim3(B), dim3(kCoarse), 0, st, a);
         hipLaunchKernelGGL(sample_collect_kernel, grid, dim3(kPieceThreads), 0, st, a);
     }
     hipLaunchKernelGGL(sample_last_kernel, dim3(B), dim3(kRowThreads), 0, st, a);
