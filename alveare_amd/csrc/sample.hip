@@ -72,31 +72,9 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// exp(-x), 0 <= x < 700: with n = rint(x / ln 2) and y = n ln 2 - x, |y| <= 0.347, it
-// is 2^-n times the Taylor sum of exp(y) to y^12 / 12! (the rest is below 2^-52).
-// The float64 library function, exact to the last bit, takes twice as long.
-__device__ __forceinline__ double exp_neg(double x) {
-    const double n = rint(x * 1.4426950408889634);
-    const double y = fma(n, 0.6931471805599453, -x);
-    double p = 1.0 / 479001600.0;
-    p = fma(p, y, 1.0 / 39916800.0);
-    p = fma(p, y, 1.0 / 3628800.0);
-    p = fma(p, y, 1.0 / 362880.0);
-    p = fma(p, y, 1.0 / 40320.0);
-    p = fma(p, y, 1.0 / 5040.0);
-    p = fma(p, y, 1.0 / 720.0);
-    p = fma(p, y, 1.0 / 120.0);
-    p = fma(p, y, 1.0 / 24.0);
-    p = fma(p, y, 1.0 / 6.0);
-    p = fma(p, y, 0.5);
-    p = fma(p, y, 1.0);
-    p = fma(p, y, 1.0);
-    return __builtin_ldexp(p, -(int)n);
-}
 // exp((l - m) / T): 1 for l = m also where both are infinite.
 __device__ __forceinline__ double weight(float l, float m, double inv_t) {
-    const double x = l == m ? 0.0 : ((double)m - (double)l) * inv_t;
-    return x < 700.0 ? exp_neg(x) : 0.0;
+    return l == m ? 1.0 : exp(((double)l - (double)m) * inv_t);
 }
 // w * scale to the nearest integer, at most 2^52: the last bits of 2^52 plus it.
 __device__ __forceinline__ uint64_t fixed(double w, double scale) {
@@ -465,7 +443,7 @@ __global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(SampleArgs a
     for (int k = 0; k < 16; ++k) {
         const double x = x_of(v[k], rr, rp.inv_t);
         if (!(x < rr.end)) continue;
-        const double w = exp_neg(x);
+        const double w = exp(-x);
         const uint64_t f = fixed(w, scale);
         if (w >= rp.minp) kept += f;
         const int bin = (int)place_of(x, rr);
