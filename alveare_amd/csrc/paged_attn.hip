@@ -108,15 +108,6 @@ __device__ __forceinline__ s16x4 pack4(float a, float b, float c, float d) {
     return __builtin_bit_cast(s16x4, v);
 }
 
-// Whether one of the two bf16 values of a word is infinite or NaN: its exponent
-// of ones carries into the bit above.
-__device__ __forceinline__ uint32_t nonfinite_bits(uint32_t w) {
-    return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-}
-__device__ __forceinline__ uint32_t nonfinite_bits4(u32x4 v) {
-    return nonfinite_bits(v[0]) | nonfinite_bits(v[1]) | nonfinite_bits(v[2]) | nonfinite_bits(v[3]);
-}
-
 // LDS pieces of a row are stored at (piece ^ swizzle of the row): the 16 lanes
 // that read K at once (16 rows, the same piece) and the 32 that read V (8 rows of
 // two pieces, or 4 of four) then fall on different banks.
@@ -167,8 +158,8 @@ constexpr float kSlack = 8.0f;
 // One row's part (maximum, sum, output: RW values per lane) over units u0 .. u1 - 1
 // of its tile, by one wave in plain float32 steps. The matrix products give a
 // value of V that is infinite or NaN to every row they compute, seen or not (0
-// times it is NaN); a wave that meets one in a block that some row does not see
-// whole does its rows again with this.
+// times it is NaN, and no later step makes that a number again); a wave that ends
+// with such an output does its rows again with this.
 template <int D>
 __device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16_t* q, int pos, int us, int ulo, int unit,
                           int u0, int u1, int lane, float (&acc)[D / 64], float& m, float& l) {
@@ -503,7 +494,6 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
         const int pos_hi = f.s.len - f.s.n + (f.rt * ROWS + nrows - 1) / a.g;
         f32x4 o[QT][D / 16];
         float m[QT], l[QT];
-        uint32_t odd = 0;  // not 0: a value of V that is no number, where some row may not see it
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             m[t] = kNoMax;
@@ -573,11 +563,6 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
             auto read_v = [&](int d) __attribute__((always_inline)) {
                 return read_tr(vt + (rd_v ^ piece<D>(2 * d)) + piece_far<D>(2 * d));
             };
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < NI; ++i)
-                    odd |= nonfinite_bits4(*reinterpret_cast<const u32x4*>(vt + 1024 * i + 16 * lane));
-            }
             constexpr int VB = D / 16 < 8 ? D / 16 : 8;  // V reads on their way at once
 #pragma unroll
             for (int d0 = 0; d0 < D / 16; d0 += VB) {
@@ -605,8 +590,15 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
                 mls[(wave * 2 + 1) * ROWS + 16 * t + col] = l[t];
             }
         }
+        float odd = 0.0f;
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd = __builtin_fmaf(o[t][d][e], 0.0f, odd);
         if (lane == 0) odds[wave] = 0;
-        if (__any(odd != 0) && lane == 0) odds[wave] = 1;
+        if (__any(odd != 0.0f) && lane == 0) odds[wave] = 1;
         __syncthreads();  // and every wave is done with its ring
         bool again = false;
 #pragma unroll
@@ -947,7 +939,6 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
 #pragma unroll
     for (int d = 0; d < DW / 32; ++d) o[d] = f32x16{};
     float m = kNoMax, l = 0.0f;
-    uint32_t odd = 0;  // not 0: a value of V that is no number, where some row may not see it
 
     const int vrow = 4 * h + ((lane & 15) >> 2);
     const uint32_t rd_k = col * (2 * D) + (h ^ k_swz<D>(col)) * 16;
@@ -987,10 +978,12 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
         for (int i = 0; i < 16; ++i) s[i] = sv[i];
         const bool masked = hole || p0 + 31 > wpos_lo || (a.window > 0 && p0 <= wpos_hi - a.window && p0 + 31 >= a.sinks);
         if (masked) {
+            // Relative to p0 + 4 h, so that positions are constants.
+            const int at = pos - p0 - 4 * h, lo = a.window > 0 ? at - a.window : INT_MIN, sk = a.sinks - p0 - 4 * h;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int p = p0 + 8 * (i / 4) + 4 * h + i % 4;
-                if (!sees(a, p, pos) || (hole >> (i / 8) & 1)) s[i] = -__builtin_inff();
+                const int p = 8 * (i / 4) + i % 4, hi = hole >> (i / 8) & 1 ? -1 : at;
+                s[i] = (p <= hi) & ((p > lo) | (p < sk)) ? s[i] : -__builtin_inff();
             }
         }
         float top = s[0];
@@ -1029,16 +1022,6 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
             const s16x4 lo = read_tr(v), hi = read_tr(v + 16 * D);
             return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         };
-        if (masked) {
-#pragma unroll
-            for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    // (tied down one by one: few registers at a time, and V is read again below, not kept)
-                    odd |= nonfinite_bits4(__builtin_bit_cast(u32x4, read_v(d, k)));
-                    asm volatile("" : "+v"(odd)::"memory");
-                }
-        }
         // Operand j: two blocks of columns in turn, then their second 16 positions.
         constexpr int NV = DW / 16;
         auto blk = [](int j) { return (j & ~3) / 2 + (j & 1); };
@@ -1123,15 +1106,20 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
     }
 
     float* part = a.part + ((int64_t)item * nsplit + split) * (TR * (D + 2));
-    if constexpr (DS == 2) {  // found in either half's columns
+    float no = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) no = __builtin_fmaf(o[d][i], 0.0f, no);
+    bool odd = __any(no != 0.0f);
+    if constexpr (DS == 2) {  // in either half's columns
         int* odds = reinterpret_cast<int*>(xch);
         __syncthreads();
-        if (lane == 0) odds[wave] = 0;
-        if (__any(odd != 0) && lane == 0) odds[wave] = 1;
+        if (lane == 0) odds[wave] = odd;
         __syncthreads();
         odd = odds[wave] | odds[wave ^ 1];
     }
-    if (__any(odd != 0)) {  // see plain_row; with two waves per row, one does it
+    if (odd) {  // see plain_row; with two waves per row, one does it
         for (int r = 0; dh == 0 && r < nrows; ++r) {
             const int64_t rr = r0 + r;
             const int tk = (int)(rr / a.g), hd = kvh * a.g + (int)(rr % a.g);
@@ -1384,7 +1372,8 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
         return fail(ALV_ERR_ALIGN, "q, kpages and vpages and their rows need 16-byte alignment, out and its rows 8-byte");
     if (T == 0) return ALV_OK;
     a.q = q, a.ld_q = ld_q, a.kpages = kpages, a.vpages = vpages, a.k_stride = k_stride, a.v_stride = v_stride;
-    a.heads = heads, a.kv_heads = kv_heads, a.g = heads / kv_heads, a.window = window, a.sinks = sinks, a.scale = scale;
+    a.heads = heads, a.kv_heads = kv_heads, a.g = heads / kv_heads, a.sinks = sinks, a.scale = scale;
+    a.window = window < a.b.max_pos ? window : 0;  // (all positions are within it)
     a.out = out, a.ld_out = ld_out;
     if ((int64_t)T * heads > (int64_t)1 << 30)  // (the largest launch: 2^32 threads)
         return fail(ALV_ERR_RANGE, "%d rows of %d heads in one call (at most 2^30 rows times heads)", T, heads);
