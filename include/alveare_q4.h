@@ -496,7 +496,7 @@ int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16_t* kpages,
 /*
  * In each of `ncaches` caches (host array of device pointers; pages of
  * page_bytes bytes, stride_bytes apart, both multiples of 16, caches 16-byte
- * aligned): page dst[i] = page src[i] for i < npairs. src and dst are HOST
+ * aligned, none overlapping): page dst[i] = page src[i], i < npairs. src and dst are HOST
  * arrays, read before the call returns. Every copy may run beside every other:
  * a page that is the destination of two pairs, or of one pair and the source of
  * any, is refused with ALV_ERR_ARG before anything is enqueued.
