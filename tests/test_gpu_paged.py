@@ -538,3 +538,163 @@ def test_attention_seventy_chunks(dev, D):
     past = [(11 * i) % 90 for i in range(70)]
     b = R.Batch(n, [a + c for a, c in zip(n, past)], kv_heads=1, D=D, page=16, dev=dev)
     check_attention(b, 4, dev)
+
+
+@pytest.mark.parametrize("half", [1, 3, 12, 29])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_post_odd_halves_and_rows_off_their_alignment(dev, half, shift):
+    """As the one-token op, where no eight columns share a path or a 16-byte access."""
+    from alveare_amd import layer as L, qkv_post_paged
+
+    heads, kv_heads, D = 3, 1, 64
+    n, total = [5, 1], [5, 20]
+    b = R.Batch(n, total, kv_heads=kv_heads, D=D, page=16, dev=dev)
+    width = (heads + 2) * D
+    qkv = rows(b.T, width + 3, dev, 4)[:, shift:shift + width]
+    rope = rows(20, 2 * half + 1, dev, 8)
+    got = qkv_post_paged(qkv, b.kp, b.vp, b.table, b.q_start, b.kv_len, heads=heads, k_off=heads * D,
+                         v_off=(heads + 1) * D, rope=rope, sin_off=half, half=half)
+    kc, vc = (torch.zeros(kv_heads, 20, D, dtype=bf, device=dev) for _ in range(2))
+    for t, (s, pos) in enumerate([(0, 0), (0, 1), (0, 2), (0, 3), (0, 4), (1, 19)]):
+        want = L.qkv_post(qkv[t].clone(), torch.tensor([pos], dtype=torch.int32, device=dev), kc, vc, heads=heads,
+                          kv_heads=kv_heads, D=D, k_off=heads * D, v_off=(heads + 1) * D,
+                          rope=rope[:, :2 * half].contiguous().view(-1), rope_stride=2 * half, sin_off=half, half=half)
+        pg, sl = int(b.table[s, pos // 16]), pos % 16
+        assert torch.equal(got[t], want)
+        assert torch.equal(b.kp[pg, :, sl], kc[:, pos]) and torch.equal(b.vp[pg, :, sl], vc[:, pos])
+
+
+# ---- the operators together --------------------------------------------------------------
+
+def test_prompts_forks_drafts_and_decode_steps(dev):
+    """A small model served as these operators are meant to be used: prompts in
+    chunks, two continuations of one prompt, drafts of which some are taken back,
+    sampled decode steps, a sequence freed and the pool compacted. Each call is
+    checked on the inputs it got, and the cache against what was inserted."""
+    import types
+
+    from alveare_amd import PagedCache, attention_paged, qkv_post_paged, sample
+
+    heads, kv_heads, D, hidden, vocab, layers, page = 4, 2, 64, 96, 5000, 2, 16
+    g = torch.Generator().manual_seed(9)
+    mat = lambda *s: (torch.randn(*s, generator=g) / math.sqrt(s[0])).to(bf).to(dev)  # noqa: E731
+    emb = mat(vocab, hidden) * 8
+    w_qkv, w_o, w_head = ([mat(hidden, (heads + 2 * kv_heads) * D) for _ in range(layers)],
+                          [mat(heads * D, hidden) for _ in range(layers)], mat(hidden, vocab) * 4)
+    rope = rows(200, D, dev, 3)
+    c = PagedCache(layers=layers, kv_heads=kv_heads, D=D, pages=40, page_size=page, slots=4, max_pages=12, device=dev)
+    kept = [[([], []) for _ in range(layers)] for _ in range(4)]  # by slot and layer, each position's k and v
+
+    def step(slots, tokens):
+        """tokens: a list per slot. Returns the logits of each slot's last token."""
+        n = [len(t) for t in tokens]
+        c.reserve(slots, n)
+        table, q_start, kv_len = c.batch(slots, n)
+        x = emb[torch.tensor(sum(tokens, []), device=dev)]
+        for i in range(layers):
+            qkv = x @ w_qkv[i]
+            q = qkv_post_paged(qkv, c.k[i], c.v[i], table, q_start, kv_len, heads=heads, k_off=heads * D,
+                               v_off=(heads + kv_heads) * D, rope=rope)
+            at = 0
+            for s, m in zip(slots, n):
+                for j in range(m):
+                    pos = c.length(s) - m + j
+                    _, k, v = R.post(qkv[at], types.SimpleNamespace(D=D, kv_heads=kv_heads), pos, heads=heads,
+                                     k_off=heads * D, v_off=(heads + kv_heads) * D, q_w=None, k_w=None, norm=(1, 1, 1),
+                                     eps=1e-6, rope=rope, half=D // 2, cos_off=0, sin_off=D // 2)
+                    pg, sl = c.table(s)[pos // page], pos % page
+                    for got, want, keep in ((c.k[i][pg, :, sl], k, kept[s][i][0]), (c.v[i][pg, :, sl], v, kept[s][i][1])):
+                        got = got.double().cpu()
+                        # (as in test_post_against_the_formula)
+                        scale = want.abs() + want.abs().amax(-1, keepdim=True) * 2
+                        assert ((got - want).abs() <= R.BF16 * (want.abs() + 2 * scale)).all()
+                        keep.append(got)
+                    at += 1
+            out = attention_paged(q, c.k[i], c.v[i], table, q_start, kv_len, heads=heads, scale=0.125, max_q=max(n))
+            b = types.SimpleNamespace(n=n, total=[c.length(s) for s in slots], page=page, kv_heads=kv_heads, D=D,
+                                      k=[torch.stack(kept[s][i][0]) for s in slots],
+                                      v=[torch.stack(kept[s][i][1]) for s in slots])
+            want, tol = R.attention(q, b, heads, scale=0.125)
+            assert ((out.double().cpu().view_as(want) - want).abs() <= tol).all()
+            x = x + out @ w_o[i]
+        last = torch.tensor([sum(n[:k + 1]) - 1 for k in range(len(n))], device=dev)
+        return (x[last] @ w_head).float()
+
+    def draw(logits):
+        u = torch.rand(len(logits), generator=g).to(dev)
+        token, prob = sample(logits, u, temperature=0.9, top_k=50, top_p=0.95, min_p=0.01)
+        for k in range(len(logits)):
+            assert R.sample(logits[k], float(u[k]), 0.9, 50, 0.95, 0.01)[0] == int(token[k])
+        assert ((prob > 0) & (prob <= 1)).all()
+        return token.tolist()
+
+    prompts = [torch.randint(vocab, (m,), generator=g).tolist() for m in (75, 18, 3)]
+    step([0, 1], [prompts[0][:40], prompts[1]])
+    logits = step([0, 2], [prompts[0][40:], prompts[2]])
+    c.fork(0, 3)  # a second continuation
+    kept[3] = [([*k], [*v]) for k, v in kept[0]]
+    tokens = draw(logits[[0, 1, 0]])
+    for _ in range(3):
+        tokens = draw(step([0, 2, 3], [[t] for t in tokens]))
+    step([0, 1], [[tokens[0], 5, 6, 7], [9, 8]])  # drafts: two of the first's are taken back
+    c.truncate(0, c.length(0) - 2)
+    for k, v in kept[0]:
+        del k[-2:], v[-2:]
+    c.free(2)
+    kept[2] = [([], []) for _ in range(layers)]
+    assert c.compact() >= 0
+    tokens = draw(step([3, 0, 1], [[4], [5], [6]]))
+    draw(step([2, 3, 1, 0], [prompts[2] * 9, [tokens[0]], [], [tokens[1]]])[[0, 1, 3]])
+    for s in range(4):
+        t = c.table(s)
+        for i in range(layers):
+            for pool, keep in ((c.k[i], kept[s][i][0]), (c.v[i], kept[s][i][1])):
+                got = pool[t].transpose(1, 2).reshape(-1, kv_heads, D)[:c.length(s)]
+                assert torch.equal(got.double().cpu(), torch.stack(keep))
+
+
+def test_a_captured_decode_step(dev):
+    """Insert, attention and sampling of a batch in one graph, replayed while the
+    sequences grow over pages, against the same calls made one by one."""
+    from alveare_amd import PagedCache, attention_paged, qkv_post_paged, sample
+
+    heads, kv_heads, D, vocab, B = 4, 2, 64, 6000, 3
+    g = torch.Generator().manual_seed(1)
+    emb, w = rows(vocab, (heads + 2 * kv_heads) * D, dev, 1), rows(heads * D, vocab, dev, 2, std=0.3)
+    caches = [PagedCache(layers=1, kv_heads=kv_heads, D=D, pages=30, page_size=16, slots=B, max_pages=6, device=dev)
+              for _ in range(2)]
+    for c in caches:
+        c.reserve(range(B), [14, 1, 40])
+        c.pool.copy_(torch.randn(c.pool.shape, generator=torch.Generator().manual_seed(5)).to(bf))
+        c.truncate(1, 0)
+    table = torch.full((B, 6), -1, dtype=torch.int32, device=dev)
+    q_start, kv_len = torch.arange(B + 1, dtype=torch.int32, device=dev), torch.zeros(B, dtype=torch.int32, device=dev)
+    u = torch.zeros(B, device=dev)
+    token = torch.tensor([3, 4, 5], dtype=torch.int32, device=dev)
+    prob = torch.zeros(B, device=dev)
+
+    def step(c, table, q_start, kv_len, token, prob):
+        q = qkv_post_paged(emb[token.long()], c.k[0], c.v[0], table, q_start, kv_len, heads=heads, k_off=heads * D,
+                           v_off=(heads + kv_heads) * D)
+        out = attention_paged(q, c.k[0], c.v[0], table, q_start, kv_len, heads=heads, scale=0.125, max_q=1)
+        sample((out @ w).float(), u, temperature=1.2, top_k=100, top_p=0.9, token=token, prob=prob)
+
+    eager_token, eager_prob = token.clone(), prob.clone()
+    s = torch.cuda.Stream(dev)
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s):
+        step(caches[0], table, q_start, kv_len, token.clone(), prob.clone())  # nothing fits: no page changes
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        step(caches[0], table, q_start, kv_len, token, prob)
+    for _ in range(6):
+        for c in caches:
+            c.reserve(range(B), [1] * B)
+        t, q, k = caches[0].batch(range(B), [1] * B)
+        u.copy_(torch.rand(B, generator=g))
+        table.copy_(t), kv_len.copy_(k)
+        graph.replay()
+        step(caches[1], *caches[1].batch(range(B), [1] * B), eager_token, eager_prob)
+        torch.cuda.synchronize()
+        assert torch.equal(token, eager_token) and torch.equal(prob, eager_prob)
+        assert torch.equal(caches[0].pool, caches[1].pool)

@@ -181,3 +181,13 @@ def test_operators_refuse_host_tensors():
                  lambda: aa.copy_pages([pg], [0], [1]), lambda: aa.sample(z.float(), z[0, :1].float())):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+def test_attention_workspace(L):
+    from alveare_amd._lib import ALV_ERR_ALIGN, ALV_ERR_ARG
+
+    need = L.alv_attention_paged_workspace(4, 2, 64, 2, 3, 0)
+    assert need > 0 and L.alv_attention_paged_workspace(4, 3, 64, 2, 3, 0) == 0
+    assert attn(L) == ALV_ERR_ARG and attn(L, ws=P, wb=need - 1) == ALV_ERR_ARG
+    assert attn(L, ws=ctypes.c_void_p((1 << 20) + 8), wb=need) == ALV_ERR_ALIGN
+    assert L.alv_sample_workspace(1, 4096) == 0 < L.alv_sample_workspace(1, 4097) < L.alv_sample_workspace(2, 4097)
