@@ -1,4 +1,16 @@
 // Attention of the newest tokens of a batch of sequences over a paged KV cache.
+//
+// out = sum_p w_p v_p / sum_p w_p with w_p = exp(scale q.k_p - m), the maximum m
+// and both sums kept running in float32 over one pass of K and V. Both kernels
+// compute the transposes, S' = K Q' and O' = V' P': a lane then has one row's
+// scores for several positions, which as bf16 are the next product's operand as
+// they stand, and a row's maximum and sum are one lane's (pair's, group's) own.
+//
+// Two kernels, by how many rows (tokens times q heads of the group) a sequence
+// brings: up to 64 at D <= 128, 32 at 256, 16 at 512 stream K and V past a few
+// resident rows, bound by memory; more rows share tiles of K and V, bound by the
+// matrix cores. The host plans with max_q (or the average) and the kernels sort
+// the sequences by their own counts, so a batch may hold both kinds.
 #include <limits.h>
 
 #include <algorithm>
@@ -225,6 +237,12 @@ __device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16
 // NW, ...) through a ring of LDS buffers that only it uses: no barrier until the
 // tile's end, and 64 to 128 KiB in flight per CU, which is what the memory needs
 // to run at its rate. 16 positions never cross a page.
+//
+// Bound by memory where there is work enough: 64 sequences of 1000 to 4000
+// positions, one token each, read K and V at 4.8 TB/s (32 q heads of 64 on 8: 70
+// us), 5.2 (16 of 128 on 8: 128 us), 5.6 (16 of 256 on 8: 240 us) and 4.0 (16 of
+// 512 on 1: 85 us); a large copy moves 4.9 on this card, reads alone more. One
+// sequence of 300 positions is two launches, 14 us with the host's part.
 
 // A sequence's place in the line, per lane of the scan.
 struct RowsSeq {
@@ -383,7 +401,7 @@ __device__ __forceinline__ Cut make_cut(uint64_t total, uint32_t n) {
 // At most kPartsPerTile parts per tile on average: the merge reads them all (one
 // token over 8000 positions on one kv head of 512: 250 parts 117 us, 125 40, 64 33).
 __device__ __forceinline__ uint32_t part_count(uint64_t total, const Scan& sc, int grid) {
-    return (uint32_t)min((uint64_t)min((uint32_t)grid, sc.tiles * kPartsPerTile), total);
+    return (uint32_t)min(min((uint64_t)grid, (uint64_t)sc.tiles * kPartsPerTile), total);
 }
 
 template <int D, int QT>
@@ -742,8 +760,17 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
 // their way while these are used. D = 512: a wave's output would be 256 registers;
 // two waves share 32 rows instead, each with half the columns: half of every
 // score's products, exchanged through LDS, and half of the output.
-// Where there are fewer tiles than compute units each tile's positions are split
-// and the parts joined by a second launch.
+// Where there are tiles for less than half of the workgroups that fit, each tile's
+// positions are split and the parts joined by a second launch.
+//
+// Bound by the matrix cores and the vector ALUs in turn: a wave's 32 x 32 scores
+// take 2 D / 16 matrix instructions and some 70 vector ones (half as many cycles
+// as D = 256's products, as many as D = 64's), and LDS delivers K and V to four
+// waves in the time of their products. Prompts of 8192 tokens: 32 heads of 64 on
+// 8 376 us (732 TFLOP/s), 16 of 128 on 8 329 us (837), 16 of 256 on 8 500 us
+// (1100), 16 of 512 on 1 1220 us (900). BN = 32 at D = 128 gains there (310 us)
+// and loses on the shorter ones (4096 tokens 120 -> 134 us, 2048 in a 1024 window
+// 52 -> 58); reading K ahead of the next loads' addresses costs 2 to 8 % at D <= 128.
 constexpr int tile_ds(int D) { return D == 512 ? 2 : 1; }      // waves that share 32 rows
 constexpr int tile_waves(int D) { return D == 512 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D) / tile_ds(D); }
@@ -1063,7 +1090,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
         // Two groups of waves, one of each per SIMD, half a unit apart: while one
         // multiplies K the other has its softmax and V, so the matrix cores, the
         // vector ALUs and LDS all have work (in step, each waits for the others:
-        // 4096 tokens, 16 heads of 512, 342 us). Phase p, between two barriers:
+        // 4096 tokens, 16 heads of 512, 342 us; so 328). Phase p, between two barriers:
         // even p = 2 k is unit k's K for group 0 and unit k - 1's V for group 1, odd
         // p the reverse; loads run two phases ahead, unit k's K needed from phase
         // 2 k, its V from 2 k + 1, and each buffer is filled again when its last
@@ -1318,7 +1345,9 @@ int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     hipLaunchKernelGGL((attn_paged_tile_kernel<D>), dim3((uint32_t)(p.grid_tiles * p.nsplit)), dim3(64 * tile_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_tile_kernel launch")) return rc;
     if (p.nsplit == 1) return ALV_OK;
-    // Few tiles are joined by as many workgroups as they have rows for, many by fewer each.
+    // Few tiles are joined by as many workgroups as they have rows for, many by fewer
+    // each: 1024 tokens of 16 heads of 512 (128 tiles) 23 us with 64 workgroups each,
+    // 16 with 8; drafts over 4 long contexts (4 tiles) 6 us less than with 32.
     const int groups = (int)std::max((int64_t)1, std::min((int64_t)tile_rows(D) / merge_rows(D), 1024 / p.tiles));
     hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D>), dim3((uint32_t)p.tiles * groups), dim3(256), 0, s, a, groups);
     return hip_check(hipGetLastError(), "attn_paged_tile_merge_kernel launch");

@@ -265,8 +265,10 @@ __device__ void sample_row(const SampleArgs& a, int b, const RowParams& rp, RowS
 // so no order of atomics shows. A row whose bins hold too many (logits all alike
 // but for a few far ones) is done by sample_row.
 //
-// What bounds it: one row is a chain of launches, each a trip or two to memory;
-// many rows, the histograms' atomics and the float64 exponentials.
+// What bounds it: one row is a chain of launches, each a trip or two to memory (one
+// row of 262144: 25 us, of them 4 + 8 + 9 + 4 in the kernels); many rows, the
+// histogram (48 rows of 128256, 52 us: 9 + 18 + 16 + 10; reading the logits three
+// times is 15 of them).
 constexpr int kPieceThreads = 256;
 constexpr int kWaves = kPieceThreads / 64;
 constexpr int kPiece = 16 * kPieceThreads;  // logits per workgroup (2 or 4 times as many are slower by a half: too few loads on their way)
