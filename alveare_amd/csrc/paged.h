@@ -30,6 +30,8 @@ struct PagedBatch {
 constexpr int kPageMin = 16, kPageMax = 1024;
 constexpr int kMaxRows = 1 << 22;  // 512 threads a row stay within a launch's 2^32 threads
 
+constexpr int kMaxHeads = 1 << 16;  // a row's offsets stay within 32 bits
+
 inline int page_shift(int page_size) { return 31 - __builtin_clz((unsigned)page_size); }
 
 // Checks of the arguments every paged entry point shares, and the batch.

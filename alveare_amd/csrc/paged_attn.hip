@@ -1390,6 +1390,7 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
         sinks < 0 || max_q < 0 || ld_q < (int64_t)heads * D || ld_out < (int64_t)heads * D)
         return fail(ALV_ERR_ARG, "bad attention shape heads=%d kv_heads=%d D=%d window=%d sinks=%d ld_q=%lld ld_out=%lld "
                     "(D one of 64, 128, 256, 512)", heads, kv_heads, D, window, sinks, (long long)ld_q, (long long)ld_out);
+    if (heads > kMaxHeads) return fail(ALV_ERR_RANGE, "%d heads (at most %d)", heads, kMaxHeads);
     if (!(scale >= 0.0f) || scale > 3e38f) return fail(ALV_ERR_ARG, "scale %g: finite and not negative", (double)scale);
     const int64_t page_values = (int64_t)kv_heads * page_size * D;
     if (k_stride < page_values || v_stride < page_values)

@@ -255,11 +255,12 @@ extern "C" int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off
     PostPagedArgs a{};
     if (int rc = paged_batch(page_table, ld_table, max_pages, q_start, kv_len, B, T, pages, page_size, &a.b)) return rc;
     if (!kpages || !vpages || (T > 0 && (!qkv || !q_out))) return fail(ALV_ERR_ARG, "null pointer");
-    if (heads < 1 || kv_heads < 1 || heads % kv_heads || (D != 64 && D != 128 && D != 256 && D != 512) ||
-        k_off < heads * D || (v_off >= 0 && v_off < k_off + kv_heads * D) ||
-        ld_qkv < (v_off < 0 ? k_off : v_off) + kv_heads * D || ld_q < heads * D)
+    const int64_t qw = (int64_t)heads * D, kw = (int64_t)kv_heads * D;
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads || (D != 64 && D != 128 && D != 256 && D != 512) || k_off < qw ||
+        (v_off >= 0 && v_off < k_off + kw) || ld_qkv < (v_off < 0 ? k_off : v_off) + kw || ld_q < qw)
         return fail(ALV_ERR_ARG, "bad qkv layout heads=%d kv_heads=%d D=%d k_off=%d v_off=%d (D one of 64, 128, 256, 512)",
                     heads, kv_heads, D, k_off, v_off);
+    if (heads > kMaxHeads) return fail(ALV_ERR_RANGE, "%d heads (at most %d)", heads, kMaxHeads);
     const int64_t page_values = (int64_t)kv_heads * page_size * D;
     if (k_stride < page_values || v_stride < page_values)
         return fail(ALV_ERR_ARG, "page strides %lld and %lld hold fewer than the page's %lld values", (long long)k_stride,

@@ -459,7 +459,7 @@ def _per_row(v, name: str, B: int, dtype: torch.dtype, dev: torch.device):
         if v.numel() < B:
             raise ValueError(f"{name} holds {v.numel()} values for {B} rows")
         return v.data_ptr(), 0
-    return None, int(v) if dtype == torch.int32 else float(v)
+    return None, max(-1, min(int(v), 2 ** 31 - 1)) if dtype == torch.int32 else float(v)
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,

@@ -76,6 +76,7 @@ def _batch(page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor
 
 
 _BF16, _I32 = torch.bfloat16, torch.int32
+_INT_MAX = 2 ** 31 - 1
 
 
 def _args(t: torch.Tensor, name: str, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
@@ -141,6 +142,8 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
         rope_rows, ldr = rope.shape[0], _rows(rope, "rope", 2, dev)
         half = rope.shape[1] // 2 if half is None else half
         sin_off = half if sin_off is None else sin_off
+        if not (0 <= cos_off <= rope.shape[1] - half and 0 <= sin_off <= rope.shape[1] - half):
+            raise ValueError(f"rope rows of {rope.shape[1]} values hold no {half} at cos_off={cos_off} and sin_off={sin_off}")
     if q_out is None:
         q_out = qkv.new_empty((T, ldq))
     else:
@@ -171,6 +174,7 @@ def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     ldo = heads * D
     if width < ldo:
         _narrow("q", width, ldo)
+    window, sinks, max_q = min(window, _INT_MAX), min(sinks, _INT_MAX), min(max_q, _INT_MAX)
     if out is None:
         out = torch.empty_like(q) if width == ldo == ldq else q.new_empty((T, ldo))
     else:
@@ -251,9 +255,9 @@ class PagedCache:
             raise ValueError("layers, kv_heads, D, pages, slots and max_pages must be positive")
         if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
             raise ValueError(f"page_size={page_size}: a power of two from 16 to 1024")
-        self.device = torch.device(device)
         self.page_size, self.pages, self.slots, self.max_pages = page_size, pages, slots, max_pages
-        self.pool = torch.zeros((layers, 2, pages, kv_heads, page_size, D), dtype=torch.bfloat16, device=self.device)
+        self.pool = torch.zeros((layers, 2, pages, kv_heads, page_size, D), dtype=torch.bfloat16, device=device)
+        self.device = self.pool.device
         self.k = [self.pool[i, 0] for i in range(layers)]
         self.v = [self.pool[i, 1] for i in range(layers)]
         self._table: list[list[int]] = [[] for _ in range(slots)]
@@ -374,8 +378,8 @@ class PagedCache:
         last ``n`` positions (one number or one per slot) of each slot."""
         slots = [self._slot(s) for s in slots]
         n = [n] * len(slots) if isinstance(n, int) else list(n)
-        if len(n) != len(slots):
-            raise ValueError("one count per slot")
+        if len(n) != len(slots) or len(set(slots)) != len(slots):
+            raise ValueError("one count per slot, each slot once")
         for s, m in zip(slots, n):
             if not 0 <= m <= self._len[s]:
                 raise ValueError(f"slot {s} holds {self._len[s]} positions, not {m} new ones")

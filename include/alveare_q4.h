@@ -446,7 +446,7 @@ int alv_embed(const uint16_t* table_f16, int vocab, int H, const int32_t* token_
  * so a captured graph replays with whatever they hold then. A sequence whose
  * kv_len is less than its rows or more than max_pages * page_size gets zeros
  * for its rows, and nothing in the cache changes; rows past the last sequence
- * (padding up to T, at most 2^22) are not touched.
+ * (padding up to T, at most 2^22) are not touched. heads at most 2^16.
  */
 
 /*

@@ -698,3 +698,20 @@ def test_a_captured_decode_step(dev):
         torch.cuda.synchronize()
         assert torch.equal(token, eager_token) and torch.equal(prob, eager_prob)
         assert torch.equal(caches[0].pool, caches[1].pool)
+
+
+def test_numbers_past_32_bits(dev):
+    """A window or a max_q of any size counts as no limit; offsets are refused."""
+    from alveare_amd import attention_paged, qkv_post_paged
+
+    b = R.Batch([3, 40], [300, 40], kv_heads=1, D=64, page=16, dev=dev)
+    q = rows(b.T, 128, dev)
+    want = attention_paged(q, *b.args(), heads=2, scale=0.1)
+    for big in (2 ** 31 - 1, 2 ** 32 + 1, 2 ** 40):
+        assert torch.equal(attention_paged(q, *b.args(), heads=2, scale=0.1, window=big, sinks=big), want)
+        R_max = attention_paged(q, *b.args(), heads=2, scale=0.1, max_q=big)
+        assert torch.equal(R_max, attention_paged(q, *b.args(), heads=2, scale=0.1, max_q=2 ** 31 - 1))
+    rope, qkv = rows(300, 64, dev), rows(b.T, 256, dev)
+    for kw in (dict(cos_off=2 ** 32), dict(sin_off=2 ** 32), dict(half=2 ** 32 + 8), dict(cos_off=-8)):
+        with pytest.raises(ValueError):
+            qkv_post_paged(qkv, *b.args(), heads=2, k_off=128, v_off=192, rope=rope, **kw)

@@ -199,3 +199,13 @@ def test_refusals(dev):
                      (x, u, dict(prob=torch.zeros(1, device=dev))), (x[:, :0], u, {})):
         with pytest.raises((TypeError, ValueError)):
             aa.sample(a, b, **kw)
+
+
+def test_top_k_of_any_size(dev):
+    import alveare_amd as aa
+
+    x, u = normal(4, 5000).to(dev), torch.tensor([0.1, 0.5, 0.9, 0.999], device=dev)
+    want = aa.sample(x, u)
+    for k in (5000, 2 ** 31, 2 ** 32 + 1, -2 ** 40):
+        for a, b in zip(aa.sample(x, u, top_k=k), want):
+            assert torch.equal(a, b)

@@ -42,13 +42,14 @@ def test_attention_arguments(L):
                dict(table=ctypes.c_void_p((1 << 20) + 1))):
         assert attn(L, **ch) == ALV_ERR_ALIGN, ch
     assert attn(L, T=(1 << 22) + 1) == ALV_ERR_RANGE
+    assert attn(L, T=1, heads=1 << 17, ld_q=1 << 23, ldo=1 << 23) == ALV_ERR_RANGE
     assert attn(L, T=1 << 22, heads=512, ld_q=1 << 15, ldo=1 << 15) == ALV_ERR_RANGE
     assert attn(L, W=1 << 27, ldt=1 << 27) == ALV_ERR_RANGE
     assert attn(L, T=0, q=None, out=None) == ALV_OK
 
 
 def test_post_arguments(L):
-    from alveare_amd._lib import ALV_ERR_ARG, ALV_OK
+    from alveare_amd._lib import ALV_ERR_ARG, ALV_ERR_RANGE, ALV_OK
 
     def post(**ch):
         a = dict(qkv=P, ld=512, k_off=256, v_off=384, heads=4, kv=2, D=64, qw=None, kw=None, nq=1, nk=1, nv=1, eps=1e-6,
@@ -61,6 +62,11 @@ def test_post_arguments(L):
                dict(v_off=300), dict(D=32), dict(heads=5), dict(half=33), dict(half=0), dict(sin=40), dict(rows=0),
                dict(cos=-1), dict(S=17), dict(ks=2047), dict(ldq=255)):
         assert post(**ch) == ALV_ERR_ARG, ch
+    # heads times D, and offsets plus it, past 32 bits
+    for ch in (dict(heads=1 << 26), dict(heads=1 << 27, kv=1 << 26), dict(k_off=2 ** 31 - 64, v_off=-1),
+               dict(v_off=2 ** 31 - 64)):
+        assert post(**ch) == ALV_ERR_ARG, ch
+    assert post(heads=1 << 17, k_off=1 << 23, v_off=-1, ld=1 << 24, ldq=1 << 24) == ALV_ERR_RANGE
     assert post(T=0, qkv=None, q=None) == ALV_OK
 
 
@@ -168,6 +174,8 @@ def test_cache_truncate_and_compact(cache):
     assert q.tolist() == [0, 5, 5, 23] and k.tolist() == [33, 0, 18]
     with pytest.raises(ValueError):
         c.batch([1], [19])
+    with pytest.raises(ValueError):
+        c.batch([1, 1], [1, 1])
 
 
 def test_operators_refuse_host_tensors():
