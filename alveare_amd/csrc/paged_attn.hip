@@ -38,8 +38,9 @@ struct PagedAttnArgs {
     int64_t ld_out;
     int64_t row_limit;  // sequences of more rows (tokens times q heads per kv head) are not this launch's
     int max_tiles;      // tiles of all sequences, per kv head, at most
-    int nsplit;         // parts of a tile's positions, unless there are more than max_items tiles
-    int max_items;
+    int max_items;      // tiles (times kv heads) that may be split: no more than slots; 0: none
+    int slots;          // parts that run at once
+    int* tab;           // for the merge: how many tiles, then kTabInts for each
     float* part;
 };
 
@@ -760,8 +761,8 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
 // their way while these are used. D = 512: a wave's output would be 256 registers;
 // two waves share 32 rows instead, each with half the columns: half of every
 // score's products, exchanged through LDS, and half of the output.
-// Where there are tiles for less than half of the workgroups that fit, each tile's
-// positions are split and the parts joined by a second launch.
+// Where there are tiles for less than half of the workgroups that fit, the longer
+// ones' positions are split and the parts joined by a second launch.
 //
 // Bound by the matrix cores and the vector ALUs in turn: a wave's 32 x 32 scores
 // take 2 D / 16 matrix instructions and some 70 vector ones (half as many cycles
@@ -821,10 +822,10 @@ struct TileSpan {
 template <int TR, int BN>
 __device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int len, bool ok, int rt) {
     TileSpan s;
-    const int64_t r0 = (int64_t)rt * TR, all = (int64_t)n * a.g;
-    s.rows = (int)min((int64_t)TR, all - r0);
-    s.pos_lo = len - n + (int)(r0 / a.g);
-    s.pos_hi = len - n + (int)((r0 + s.rows - 1) / a.g);
+    const int r0 = rt * TR;  // (rows, of one kv head too, stay below 2^30)
+    s.rows = min(TR, n * a.g - r0);
+    s.pos_lo = len - n + r0 / a.g;
+    s.pos_hi = len - n + (r0 + s.rows - 1) / a.g;
     const int lo = a.window > 0 ? max(0, s.pos_lo + 1 - a.window) : 0;
     s.ulo = lo / BN;
     s.us = min((min(a.sinks, lo) + BN - 1) / BN, s.ulo);
@@ -832,29 +833,25 @@ __device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int
     return s;
 }
 
-// Items (tiles times kv heads, times splits) and where each is found: heaviest
+// Items (tiles times kv heads, times their parts) and where each is found: heaviest
 // (last) tiles first, kv heads side by side, so that the workgroups an XCD gets
 // in turn share theirs where there are eight.
 template <int TR>
-__device__ __forceinline__ int tile_count(const PagedAttnArgs& a, int lane) {
-    int all = 0;
+__device__ __forceinline__ int tile_count(const PagedAttnArgs& a, const TileScan& sc0, int lane) {  // per kv head
     // (no more than there can be: sequences that overlap must not carry the sum away)
-    for (int b0 = 0; b0 < a.b.B; b0 += 64) all = min(all + tile_scan<TR>(a, b0, lane).sum, a.max_tiles);
-    return all * a.kv_heads;
+    int all = min(sc0.sum, a.max_tiles);
+    for (int b0 = 64; b0 < a.b.B; b0 += 64) all = min(all + tile_scan<TR>(a, b0, lane).sum, a.max_tiles);
+    return all;
 }
-// Splits per tile: as planned, unless there are more tiles than the plan knew of.
-__device__ __forceinline__ int tile_splits(const PagedAttnArgs& a, int items) { return items <= a.max_items ? a.nsplit : 1; }
 
-// Where item `item` is.
+// Where tile gt is (sc0: the first 64 sequences, read once for all that needs them).
 template <int TR, int BN>
 struct TileAt {
-    int seq, kvh, rt, first, n, len;
+    int seq, rt, first, n, len;
     TileSpan sp;
-    __device__ __forceinline__ TileAt(const PagedAttnArgs& a, int item, int lane) {
-        const int gt = item / a.kv_heads;
-        kvh = item - gt * a.kv_heads;
+    __device__ __forceinline__ TileAt(const PagedAttnArgs& a, const TileScan& sc0, int gt, int lane) {
         int base = 0, b0 = 0;
-        TileScan sc = tile_scan<TR>(a, 0, lane);
+        TileScan sc = sc0;
         while (gt >= base + sc.sum) {
             base += sc.sum;
             b0 += 64;
@@ -870,8 +867,84 @@ struct TileAt {
     }
 };
 
+// ---- fewer tiles than workgroups that fit: their positions in parts
+//
+// A causal prompt's tiles run over 1 to n units: as many parts of each would leave
+// most workgroups idle at the end, so no part has more than `cap` units instead.
+// Uneven tiles: three quarters of the average workgroup's units and five more, what
+// a part costs beside them, the light tiles filling in behind the heavy. Even ones:
+// the total over the workgroups that rounding up leaves, half as many again where
+// that makes more parts than run at once, else none is split. (1024 tokens: 16
+// heads of 512 74 -> 61 us, 32 of 64 35 -> 31 against two parts each; 512 tokens
+// of 16 of 256 37 -> 29 against four; drafts over 4 long contexts 82 -> 77.)
+constexpr int kSplitTiles = 512;  // at most, of one kv head
+constexpr int kMaxParts = 64;     // of a tile: a lane each in the merge
+constexpr int kMinCap = 4;
+constexpr int kTabInts = 8;       // entry of part 0, parts, first row of the sequence, tile, rows, kv head
+
+__device__ __forceinline__ int sum64(int v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return uniform(v);
+}
+
+// Units of every tile, into LDS, by all waves.
+template <int TR, int BN, int NW>
+__device__ __forceinline__ void tile_units(const PagedAttnArgs& a, const TileScan& sc0, int tiles, int lane, int wave, int* nu) {
+    int base = 0, turn = 0;
+    for (int b0 = 0; b0 < a.b.B && base < tiles; b0 += 64) {
+        const TileScan sc = b0 ? tile_scan<TR>(a, b0, lane) : sc0;
+        for (int x0 = 0; x0 < sc.sum && base + x0 < tiles; x0 += 64, ++turn) {
+            if (turn % NW != wave) continue;
+            const int x = x0 + lane;
+            int l = 0;  // the sequence: the first lane whose tiles end behind x
+#pragma unroll
+            for (int o = 32; o; o >>= 1)
+                if (__shfl(sc.incl, l + o - 1) <= x) l += o;
+            l = min(l, 63);
+            const int before = __shfl(sc.incl - sc.tiles, l), n = __shfl(sc.n, l), len = __shfl(sc.len, l);
+            const bool ok = __shfl((int)sc.ok, l) != 0;
+            if (x < sc.sum && base + x < tiles) nu[base + x] = tile_span<TR, BN>(a, n, len, ok, x - before).nu;
+        }
+        base += sc.sum;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ int tile_parts(int nu, int cap) { return max(1, (nu + cap - 1) / cap); }
+// Parts of all tiles of a kv head.
+__device__ __forceinline__ int tile_parts_sum(const int* nu, int tiles, int lane, int cap) {
+    int c = 0;
+    for (int t = lane; t < tiles; t += 64) c += tile_parts(nu[t], cap);
+    return sum64(c);
+}
+__device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, int tiles, int lane, int& parts) {
+    int total = 0, most = 0;
+    for (int t = lane; t < tiles; t += 64) {
+        total += nu[t];
+        most = max(most, nu[t]);
+    }
+    total = sum64(total);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
+    most = uniform(most);
+    const int slots = a.slots / a.kv_heads;  // of a kv head
+    const int least = max(kMinCap, (most + kMaxParts - 1) / kMaxParts);
+    if ((int64_t)total * 5 <= (int64_t)most * tiles * 3) {  // uneven: the light ones fill in behind the heavy
+        const int cap = max(least, (int)((int64_t)total * 3 / (4 * slots)) + 5);
+        parts = tile_parts_sum(nu, tiles, lane, cap);
+        if (parts <= 2 * slots) return cap;
+    }
+    int cap = max(least, (total + slots - tiles / 2 - 1) / max(1, slots - tiles / 2));
+    for (int turn = 0; turn < 2; ++turn, cap += cap / 2) {
+        parts = tile_parts_sum(nu, tiles, lane, cap);
+        if (parts <= slots) return cap;
+    }
+    parts = tiles;
+    return INT_MAX / 2;
+}
+
 template <int D>
-__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int split, int nsplit, unsigned char* smem) {
+__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan& sc0, int gt, int kvh, int split, int nsplit, int entry, unsigned char* smem) {
     constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D);
     constexpr int DW = D / DS;            // this wave's columns of the output (and of its scores' products)
     constexpr int TB = tile_bytes(D), NC = D / 8, RPL = 512 / D;
@@ -887,13 +960,16 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
     const int rg = wave / DS, dh = wave % DS;
     const int col = lane & 31, h = lane >> 5;
 
-    const TileAt<TR, BN> at_item(a, item, lane);
-    const int seq = at_item.seq, kvh = at_item.kvh, rt = at_item.rt;
+    const TileAt<TR, BN> at_item(a, sc0, gt, lane);
+    const int seq = at_item.seq, rt = at_item.rt;
     const int first = at_item.first, n = at_item.n, len = at_item.len;
     const TileSpan sp = at_item.sp;
     const int u0 = uniform((int)((int64_t)sp.nu * split / nsplit));
     const int u1 = uniform((int)((int64_t)sp.nu * (split + 1) / nsplit));
-    if (nsplit > 1 && u0 == u1) return;  // the merge skips it too
+    if (a.tab && split == 0 && tid == 0) {
+        int* e = a.tab + kTabInts * (1 + gt * a.kv_heads + kvh);
+        e[0] = entry, e[1] = nsplit, e[2] = first, e[3] = rt, e[4] = sp.rows, e[5] = kvh;
+    }
 
     const int32_t* table = a.b.table + (int64_t)seq * a.b.ld_table;
     auto unit_pos = [&](int u) { return (u < sp.us ? u : u - sp.us + sp.ulo) * BN; };
@@ -944,13 +1020,13 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
     };
 
     // This lane's row: column col of the wave's 32.
-    const int64_t r0 = (int64_t)rt * TR + 32 * rg;
-    const int nrows = (int)max((int64_t)0, min((int64_t)32, (int64_t)n * a.g - r0));
-    const int64_t row = r0 + min(col, max(nrows - 1, 0));
-    const int tok = min((int)(row / a.g), n - 1), head = kvh * a.g + (int)(row % a.g);
+    const int r0 = rt * TR + 32 * rg;
+    const int nrows = max(0, min(32, n * a.g - r0));
+    const int row = r0 + min(col, max(nrows - 1, 0));
+    const int tok = min(row / a.g, n - 1), head = kvh * a.g + row % a.g;
     const int pos = len - n + tok;
-    const int wpos_lo = len - n + (int)(r0 / a.g);
-    const int wpos_hi = len - n + (int)((r0 + max(nrows, 1) - 1) / a.g);
+    const int wpos_lo = len - n + r0 / a.g;
+    const int wpos_hi = len - n + (r0 + max(nrows, 1) - 1) / a.g;
     const float c = fmaxf(a.scale * kLog2e, kMinScale);
     bf16x8 q[DW / 16];
     {
@@ -1132,7 +1208,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
         if (nu > 0 && grp == 0) begin(2 * nu);
     }
 
-    float* part = a.part + ((int64_t)item * nsplit + split) * (TR * (D + 2));
+    float* part = a.part + (int64_t)(entry + split * a.kv_heads) * (TR * (D + 2));
     float no = 0.0f;
 #pragma unroll
     for (int d = 0; d < DW / 32; ++d)
@@ -1148,8 +1224,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
     }
     if (odd) {  // see plain_row; with two waves per row, one does it
         for (int r = 0; dh == 0 && r < nrows; ++r) {
-            const int64_t rr = r0 + r;
-            const int tk = (int)(rr / a.g), hd = kvh * a.g + (int)(rr % a.g);
+            const int rr = r0 + r, tk = rr / a.g, hd = kvh * a.g + rr % a.g;
             float acc[D / 64], mr, lr;
             plain_row<D>(a, seq, kvh, a.q + (int64_t)(first + tk) * a.ld_q + hd * D, len - n + tk, sp.us, sp.ulo, BN, u0, u1,
                          lane, acc, mr, lr);
@@ -1198,34 +1273,73 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, int item, int 
 template <int D>
 __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kernel(PagedAttnArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
-    const int items = tile_count<tile_rows(D)>(a, threadIdx.x & 63);
-    const int nsplit = tile_splits(a, items);
-    const int item = items - 1 - (int)(blockIdx.x / (uint32_t)nsplit);
-    if (item >= 0) tile_item<D>(a, item, (int)(blockIdx.x % (uint32_t)nsplit), nsplit, smem);
+    constexpr int TR = tile_rows(D), BN = tile_bn(D);
+    static_assert(tile_lds(D) >= 4 * kSplitTiles, "the tiles' units");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const TileScan sc0 = tile_scan<TR>(a, 0, lane);
+    const int tiles = tile_count<TR>(a, sc0, lane), items = tiles * a.kv_heads;
+    const bool split = items <= a.max_items;
+    if (a.tab && blockIdx.x == 0 && tid == 0) a.tab[0] = split ? items : 0;
+    int gt, kvh, part = 0, parts = 1, entry = 0;
+    if (split) {
+        int* nu = reinterpret_cast<int*>(smem);
+        tile_units<TR, BN, tile_waves(D)>(a, sc0, tiles, lane, wave, nu);
+        int all;
+        const int cap = tile_cap(a, nu, tiles, lane, all);
+        const int e = all * a.kv_heads - 1 - (int)blockIdx.x;
+        if (e < 0) return;
+        int base = 0, t0 = 0, p, incl;
+        while (true) {
+            p = t0 + lane < tiles ? tile_parts(nu[t0 + lane], cap) : 0;
+            incl = p;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int u = __shfl_up(incl, o);
+                if (lane >= o) incl += u;
+            }
+            const int sum = __builtin_amdgcn_readlane(incl, 63);
+            if (e < (base + sum) * a.kv_heads) break;
+            base += sum;
+            t0 += 64;
+        }
+        const int l = __builtin_ctzll(__ballot((base + incl) * a.kv_heads > e));
+        gt = t0 + l;
+        parts = __builtin_amdgcn_readlane(p, l);
+        entry = (base + __builtin_amdgcn_readlane(incl, l) - parts) * a.kv_heads;
+        part = (e - entry) / a.kv_heads;
+        kvh = e - entry - part * a.kv_heads;
+        entry += kvh;
+        __syncthreads();  // nu gives way to K and V
+    } else {
+        const int item = items - 1 - (int)blockIdx.x;
+        if (item < 0) return;
+        gt = item / a.kv_heads;
+        kvh = item - gt * a.kv_heads;
+    }
+    tile_item<D>(a, sc0, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), smem);
 }
 
-// The splits of the tiles joined, `groups` workgroups to a tile, merge_rows(D) of
+// The parts of the tiles joined, `groups` workgroups to a tile, merge_rows(D) of
 // its rows at a time: the parts' factors first, a row per wave and a part per
 // lane, into LDS, then the outputs, 16 bytes per lane and part.
 constexpr int merge_rows(int D) { return 1024 / D; }
 template <int D, int PG>
 __global__ void __launch_bounds__((256 * PG)) attn_paged_tile_merge_kernel(PagedAttnArgs a, int groups) {
-    constexpr int TR = tile_rows(D), BN = tile_bn(D), R = merge_rows(D), C = D / 4;  // 16-byte pieces of a row
+    constexpr int TR = tile_rows(D), R = merge_rows(D), C = D / 4;  // 16-byte pieces of a row
     __shared__ float fac[R][64];
     __shared__ float inv[R];
     __shared__ f32x4 sums[PG > 1 ? PG - 1 : 1][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int items = tile_count<TR>(a, lane), nsplit = tile_splits(a, items);
     const int item = blockIdx.x / groups;
-    if (nsplit == 1 || item >= items) return;
-    const TileAt<TR, BN> t(a, item, lane);
-    const float* part = a.part + (int64_t)item * nsplit * (TR * (D + 2));
-    // (a tile of fewer units than splits leaves some empty: spread over nu of them)
-    const int np = min(nsplit, t.sp.nu);
-    auto at = [&](int v) { return part + (np == nsplit ? v : ((v + 1) * nsplit - 1) / max(np, 1)) * (TR * (D + 2)); };
-    const float* mine = at(max(min(lane, np - 1), 0));
-    for (int r0 = blockIdx.x % groups * R; r0 < t.sp.rows; r0 += groups * R) {
-        const int rows = min(R, t.sp.rows - r0), r = tid % 256 / C, c = tid % C;
+    if (item >= a.tab[0]) return;
+    const int* e = a.tab + kTabInts * (1 + item);
+    const int np = e[1], first = e[2], rt = e[3], tile_n = e[4], kvh = e[5];
+    if (np == 1) return;
+    const float* part = a.part + (int64_t)e[0] * (TR * (D + 2));
+    auto at = [&](int v) { return part + (int64_t)v * a.kv_heads * (TR * (D + 2)); };
+    const float* mine = at(min(lane, np - 1));
+    for (int r0 = blockIdx.x % groups * R; r0 < tile_n; r0 += groups * R) {
+        const int rows = min(R, tile_n - r0), r = tid % 256 / C, c = tid % C;
         const int vlo = tid / 256 * np / PG, vhi = (tid / 256 + 1) * np / PG;  // this group's parts
         f32x4 acc{}, x[8];
         auto load = [&](int v0) {
@@ -1262,9 +1376,8 @@ __global__ void __launch_bounds__((256 * PG)) attn_paged_tile_merge_kernel(Paged
             for (int k = 0; k < PG - 1; ++k) acc += sums[k][tid % 256];
         }
         if (r < rows && tid < 256) {
-            const int64_t rr = (int64_t)t.rt * TR + r0 + r;
-            const int tok = (int)(rr / a.g), head = t.kvh * a.g + (int)(rr % a.g);
-            store4(a.out + (int64_t)(t.first + tok) * a.ld_out + head * D + 4 * c, acc, inv[r]);
+            const int rr = rt * TR + r0 + r, tok = rr / a.g, head = kvh * a.g + rr % a.g;
+            store4(a.out + (int64_t)(first + tok) * a.ld_out + head * D + 4 * c, acc, inv[r]);
         }
         __syncthreads();
     }
@@ -1286,8 +1399,8 @@ struct AttnPlan {
     int grid;            // its workgroups
     int64_t grid_tiles;  // tiles times kv heads of the tile kernel at most (0: not launched),
     int64_t tiles;       // and at most as far as max_q tells
-    int nsplit;
-    uint64_t rows_bytes, part_bytes;
+    int slots;           // parts of tiles; 0: none is split
+    uint64_t rows_bytes, tab_bytes, part_bytes;
 };
 
 AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
@@ -1307,7 +1420,6 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
         p.grid = device_cus();
         p.rows_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
     }
-    p.nsplit = 1;
     p.part_bytes = p.rows_bytes;
     if (tiles) {
         static_assert(tile_rows(64) == 128 && tile_rows(128) == 128 && tile_rows(256) == 128 && tile_rows(512) == 128, "");
@@ -1315,8 +1427,13 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
         p.grid_tiles = (T * g / tr + std::min((int64_t)B, T * g / (p.row_limit + 1) + 1)) * kv_heads;
         p.tiles = max_q > 0 ? std::min(p.grid_tiles, (int64_t)B * ((max_q * g + tr - 1) / tr) * kv_heads) : p.grid_tiles;
         const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2);
-        p.nsplit = (int)std::max((int64_t)1, std::min((int64_t)64, slots / p.tiles));
-        if (p.nsplit > 1) p.part_bytes += (uint64_t)p.tiles * p.nsplit * tr * (D + 2) * sizeof(float);
+        // (up to half: 1800 tokens of 32 heads of 64, 450 tiles for 512 workgroups, 46 us
+        // in parts, 41 whole; 16 of 128, 232 tiles, 42 against 49)
+        if (p.tiles <= slots / 2 && p.tiles <= kSplitTiles) {
+            p.slots = (int)slots;
+            p.tab_bytes = (uint64_t)(p.tiles + 1) * kTabInts * sizeof(int);
+            p.part_bytes += p.tab_bytes + std::min((uint64_t)slots * 2, (uint64_t)p.tiles * kMaxParts) * tr * (D + 2) * sizeof(float);
+        }
     }
     return p;
 }
@@ -1350,16 +1467,15 @@ int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D>), lds, done)) return rc;
-    hipLaunchKernelGGL((attn_paged_tile_kernel<D>), dim3((uint32_t)(p.grid_tiles * p.nsplit)), dim3(64 * tile_waves(D)), lds, s, a);
+    hipLaunchKernelGGL((attn_paged_tile_kernel<D>), dim3((uint32_t)std::max(p.grid_tiles, (int64_t)p.slots * 2)), dim3(64 * tile_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_tile_kernel launch")) return rc;
-    if (p.nsplit == 1) return ALV_OK;
+    if (p.slots == 0) return ALV_OK;
     // Few tiles are joined by as many workgroups as they have rows for, many by fewer
-    // each: 1024 tokens of 16 heads of 512 (128 tiles) 23 us with 64 workgroups each,
-    // 16 with 8; drafts over 4 long contexts (4 tiles) 6 us less than with 32.
-    const int groups = (int)std::max((int64_t)1, std::min((int64_t)tile_rows(D) / merge_rows(D), 1024 / p.tiles));
+    // each (a tile in one part costs its workgroups two loads).
+    const int groups = (int)std::max((int64_t)1, std::min((int64_t)tile_rows(D) / merge_rows(D), 4096 / p.tiles));
     // Four groups of threads share many parts (drafts over 4 long contexts, 64 parts:
     // 12.5 -> 10.5 us; 16 parts of 32 tiles, D = 256: 15.5 -> 21.4).
-    if (p.nsplit >= 32)
+    if (p.slots / p.tiles >= 32)
         hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D, 4>), dim3((uint32_t)p.tiles * groups), dim3(1024), 0, s, a, groups);
     else
         hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D, 1>), dim3((uint32_t)p.tiles * groups), dim3(256), 0, s, a, groups);
@@ -1370,7 +1486,8 @@ template <int D>
 int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
     float* part = a.part;
     if (p.grid_tiles) {
-        a.part = part + p.rows_bytes / sizeof(float);
+        if (p.slots) a.tab = reinterpret_cast<int*>(part + p.rows_bytes / sizeof(float));
+        a.part = part + (p.rows_bytes + p.tab_bytes) / sizeof(float);
         if (int rc = launch_tiles<D>(a, p, s)) return rc;
     }
     a.part = part;
@@ -1421,7 +1538,7 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
     if ((int64_t)T * heads > (int64_t)1 << 30)  // (the largest launch: 2^32 threads)
         return fail(ALV_ERR_RANGE, "%d rows of %d heads in one call (at most 2^30 rows times heads)", T, heads);
     const AttnPlan p = attn_plan(heads, kv_heads, D, B, T, max_q);
-    if (p.grid_tiles * p.nsplit * 512 > (int64_t)UINT32_MAX)
+    if (p.grid_tiles * 512 > (int64_t)UINT32_MAX)
         return fail(ALV_ERR_RANGE, "%d rows of %d heads in %d sequences: too many tiles for one call", T, heads, B);
     if (p.part_bytes && (!workspace || workspace_bytes < p.part_bytes))
         return fail(ALV_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
@@ -1429,8 +1546,8 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(ALV_ERR_ALIGN, "workspace needs 16-byte alignment");
     a.part = static_cast<float*>(workspace);
     a.row_limit = p.row_limit;
-    a.nsplit = p.nsplit;
-    a.max_items = (int)std::min(p.tiles, (int64_t)INT_MAX);
+    a.slots = p.slots;
+    a.max_items = p.slots ? (int)p.tiles : 0;
     a.max_tiles = (int)(p.grid_tiles / kv_heads);
     const hipStream_t s = (hipStream_t)stream;
     switch (D) {

@@ -715,3 +715,13 @@ def test_numbers_past_32_bits(dev):
     for kw in (dict(cos_off=2 ** 32), dict(sin_off=2 ** 32), dict(half=2 ** 32 + 8), dict(cos_off=-8)):
         with pytest.raises(ValueError):
             qkv_post_paged(qkv, *b.args(), heads=2, k_off=128, v_off=192, rope=rope, **kw)
+
+
+@pytest.mark.parametrize("heads,kv_heads,D,n,past", [(16, 1, 64, [560, 0, 300, 1], [0, 5, 40, 900]), (4, 1, 512, [450], [0]),
+                                                     (8, 4, 128, [150, 290], [700, 0]), (6, 2, 256, [333], [31])])
+def test_attention_tiles_in_parts_of_unequal_number(dev, heads, kv_heads, D, n, past):
+    """Causal prompts whose late tiles are cut and whose early ones are not, more
+    than a wave's lanes of them, with and without a window."""
+    b = R.Batch(n, [a + c for a, c in zip(n, past)], kv_heads=kv_heads, D=D, page=64, dev=dev, extra_rows=2)
+    check_attention(b, heads, dev)
+    check_attention(b, heads, dev, window=170, sinks=40)
