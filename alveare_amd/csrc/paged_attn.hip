@@ -879,7 +879,7 @@ struct TileAt {
 // of 16 of 256 37 -> 29 against four; drafts over 4 long contexts 82 -> 77.)
 constexpr int kSplitTiles = 512;  // at most, of one kv head
 constexpr int kMaxParts = 64;     // of a tile: a lane each in the merge
-constexpr int kMinCap = 4;
+constexpr int kMinCap = 2;        // (4: 380 tokens of 32 heads of 64 in 3 sequences 27 us for 21)
 constexpr int kTabInts = 8;       // entry of part 0, parts, first row of the sequence, tile, rows, kv head
 
 __device__ __forceinline__ int sum64(int v) {
