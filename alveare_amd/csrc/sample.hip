@@ -11,7 +11,7 @@
 // Weights are fixed-point 64-bit integers, exp in float64 scaled by 2^(62 -
 // log2 of the vocabulary): integer sums do not depend on their order, so atomics
 // change no result, and the roundings of 2^18 weights add up to about 2^-36 of the
-// largest (2^-28 if all went one way), where float32 would shift every border
+// largest (2^-27 if all went one way), where float32 would shift every border
 // between two tokens by 2^-24.
 #include <algorithm>
 

@@ -512,7 +512,7 @@ int alv_copy_pages(void* const* caches, int ncaches, int64_t page_bytes, int64_t
  * sum_{j<r} w_j < top_p * (their sum), the first always; of those the ones with
  * w_r >= min_p. The token is the first r with sum_{j<=r} w_j > u * (sum of the
  * kept), and prob (optional) its share of that sum. u = 0 gives the likeliest.
- * Weights are exp in float64, summed as 64-bit integers (each to within 2^-46 of
+ * Weights are exp in float64, summed as 64-bit integers (each to within 2^-45 of
  * the largest at 2^18 logits).
  *
  * Each parameter comes as a device array of B values, or (NULL) as one number:
