@@ -10,7 +10,8 @@
 // brings: up to 64 at D <= 128, 32 at 256, 16 at 512 stream K and V past a few
 // resident rows, bound by memory; more rows share tiles of K and V, bound by the
 // matrix cores. The host plans with max_q (or the average) and the kernels sort
-// the sequences by their own counts, so a batch may hold both kinds.
+// the sequences by their own counts, so a batch may hold both kinds; a small batch
+// with more rows is the tile kernel's alone.
 #include <limits.h>
 
 #include <algorithm>
@@ -1411,8 +1412,19 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     const int64_t rows = (max_q > 0 ? std::min(max_q, T) : (T + B - 1) / B) * g;  // as far as is known
     const bool tiles = B == 1 ? most > 16 * qt_max : rows > 16 * qt_max;
     // No sequence is left for the streaming kernel where there is one, or all have
-    // max_q rows (should they not, the tile kernel takes them all the same).
-    const bool stream = !(tiles && (B == 1 || (max_q > 0 && (int64_t)B * max_q <= T)));
+    // max_q rows (should they not, the tile kernel takes them all the same), or where
+    // all tiles are few enough to be cut: two launches less, and the tile kernel's
+    // parts read long contexts as fast (0 to 6 tokens each over up to 4000 positions,
+    // 10 sequences of 16 heads of 512 63 -> 35 us; 0 to 20, 16 of 32 heads of 64 49 ->
+    // 36; 0 to 12, 2 of 4 heads of 256 24 -> 19).
+    const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2);
+    const int64_t tr = 128;
+    auto tiles_of = [&](int64_t row_limit) {  // that sequences of more rows than that have at most
+        return (T * g / tr + std::min((int64_t)B, T * g / (row_limit + 1) + 1)) * kv_heads;
+    };
+    auto tiles_known = [&](int64_t n) { return max_q > 0 ? std::min(n, (int64_t)B * ((max_q * g + tr - 1) / tr) * kv_heads) : n; };
+    const bool few = tiles_known(tiles_of(0)) <= slots / 2;
+    const bool stream = !(tiles && (B == 1 || few || (max_q > 0 && (int64_t)B * max_q <= T)));
     if (stream) {
         const int64_t r = tiles ? g : rows;
         p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
@@ -1423,10 +1435,8 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     p.part_bytes = p.rows_bytes;
     if (tiles) {
         static_assert(tile_rows(64) == 128 && tile_rows(128) == 128 && tile_rows(256) == 128 && tile_rows(512) == 128, "");
-        const int tr = 128;
-        p.grid_tiles = (T * g / tr + std::min((int64_t)B, T * g / (p.row_limit + 1) + 1)) * kv_heads;
-        p.tiles = max_q > 0 ? std::min(p.grid_tiles, (int64_t)B * ((max_q * g + tr - 1) / tr) * kv_heads) : p.grid_tiles;
-        const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2);
+        p.grid_tiles = tiles_of(p.row_limit);
+        p.tiles = tiles_known(p.grid_tiles);
         // (up to half: 1800 tokens of 32 heads of 64, 450 tiles for 512 workgroups, 46 us
         // in parts, 41 whole; 16 of 128, 232 tiles, 42 against 49)
         if (p.tiles <= slots / 2 && p.tiles <= kSplitTiles) {
