@@ -7,11 +7,11 @@
 // they stand, and a row's maximum and sum are one lane's (pair's, group's) own.
 //
 // Two kernels, by how many rows (tokens times q heads of the group) a sequence
-// brings: up to 64 at D <= 128, 32 at 256, 16 at 512 stream K and V past a few
-// resident rows, bound by memory; more rows share tiles of K and V, bound by the
-// matrix cores. The host plans with max_q (or the average) and the kernels sort
-// the sequences by their own counts, so a batch may hold both kinds; a small batch
-// with more rows is the tile kernel's alone.
+// brings: up to 64 at D <= 128, 32 at 256, 16 at 512 (16 of them in a small batch)
+// stream K and V past resident rows, bound by memory; more rows share tiles of K
+// and V, bound by the matrix cores. The host plans with max_q (or the average) and
+// the kernels sort the sequences by their own counts, so a batch may hold both
+// kinds; a small batch with more rows is the tile kernel's alone.
 #include <limits.h>
 
 #include <algorithm>
@@ -1410,20 +1410,23 @@ AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     const int qt_max = D <= 128 ? 4 : (D == 256 ? 2 : 1);
     const int64_t most = (max_q > 0 ? std::min(max_q, T) : T) * g;          // rows of a sequence at most
     const int64_t rows = (max_q > 0 ? std::min(max_q, T) : (T + B - 1) / B) * g;  // as far as is known
-    const bool tiles = B == 1 ? most > 16 * qt_max : rows > 16 * qt_max;
-    // No sequence is left for the streaming kernel where there is one, or all have
-    // max_q rows (should they not, the tile kernel takes them all the same), or where
-    // all tiles are few enough to be cut: two launches less, and the tile kernel's
-    // parts read long contexts as fast (0 to 6 tokens each over up to 4000 positions,
-    // 10 sequences of 16 heads of 512 63 -> 35 us; 0 to 20, 16 of 32 heads of 64 49 ->
-    // 36; 0 to 12, 2 of 4 heads of 256 24 -> 19).
     const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2);
     const int64_t tr = 128;
     auto tiles_of = [&](int64_t row_limit) {  // that sequences of more rows than that have at most
         return (T * g / tr + std::min((int64_t)B, T * g / (row_limit + 1) + 1)) * kv_heads;
     };
     auto tiles_known = [&](int64_t n) { return max_q > 0 ? std::min(n, (int64_t)B * ((max_q * g + tr - 1) / tr) * kv_heads) : n; };
+    // A batch of tiles few enough to be cut is the tile kernel's alone, without the
+    // other's two launches: its parts read long contexts as fast (0 to 6 tokens each
+    // over up to 4000 positions, 10 sequences of 16 heads of 512 63 -> 35 us; a chunk of
+    // 300 and eight single tokens over 2000, 16 heads of 256 65 -> 40). And that from
+    // more than 16 rows on (32 rows over up to 16000 positions, 6 sequences, D = 256
+    // 40 -> 28 us, 128 29 -> 23; 16 rows 31 -> 28 and 20 -> 21, D = 64 36 -> 40), at
+    // D = 512 from 16 on (52 -> 40).
     const bool few = tiles_known(tiles_of(0)) <= slots / 2;
+    const bool tiles = (B == 1 ? most : rows) > (few ? (D == 512 ? 15 : 16) : 16 * qt_max);
+    // No sequence is left for the streaming kernel there, nor where there is one, or
+    // all have max_q rows (should they not, the tile kernel takes them all the same).
     const bool stream = !(tiles && (B == 1 || few || (max_q > 0 && (int64_t)B * max_q <= T)));
     if (stream) {
         const int64_t r = tiles ? g : rows;

@@ -725,3 +725,26 @@ def test_attention_tiles_in_parts_of_unequal_number(dev, heads, kv_heads, D, n, 
     b = R.Batch(n, [a + c for a, c in zip(n, past)], kv_heads=kv_heads, D=D, page=64, dev=dev, extra_rows=2)
     check_attention(b, heads, dev)
     check_attention(b, heads, dev, window=170, sinks=40)
+
+
+@pytest.mark.parametrize("D,most", [(64, 10), (64, 20), (128, 10), (128, 20), (256, 5), (256, 10)])
+def test_attention_many_drafts(dev, D, most):
+    """So many sequences that drafts of 16, 32 and 64 rows stream past K and V."""
+    n = [1 + (5 * i) % most for i in range(132)]
+    n[7] = 0
+    past = [(29 * i) % 150 for i in range(132)]
+    b = R.Batch(n, [a + c for a, c in zip(n, past)], kv_heads=2, D=D, page=16, dev=dev, extra_rows=1)
+    check_attention(b, 6, dev)
+    if D == 128:
+        check_attention(b, 6, dev, window=60, sinks=5)
+    # a value that is no number in the last token's v of one sequence
+    from alveare_amd import attention_paged
+
+    q = rows(b.T, 6 * D, dev, 3)
+    want, tol = R.attention(q, b, 6, scale=0.1)
+    s = 60
+    b.put(s, b.total[s] - 1, v=math.nan)
+    got = attention_paged(q, *b.args(), heads=6, scale=0.1, max_q=most)[:want.shape[0]].double().cpu().view_as(want)
+    hit = torch.zeros(len(want), dtype=torch.bool)
+    hit[sum(n[:s + 1]) - 1] = True
+    assert torch.isnan(got[hit]).all() and ((got - want).abs() <= tol)[~hit].all()
