@@ -37,7 +37,7 @@ struct SampleArgs {
     int32_t* token;
     float* prob;
     unsigned char* work;
-    int pieces;  // of a row; 0: a row is one workgroup's
+    int pieces;  // of a row; 0: a row is one workgroup's alone
 };
 
 struct RowParams {
@@ -387,6 +387,9 @@ __global__ void __launch_bounds__(kPieceThreads) sample_top_kernel(SampleArgs a)
     }
 }
 
+// x from which a weight rounds to nothing.
+__device__ __forceinline__ float weightless(const SampleArgs& a) { return (float)(a.shift + 1) * 0.693147182464599609375f; }
+
 // What a row's largest and smallest logits decide.
 struct RowRange {
     float m;
@@ -412,7 +415,7 @@ __device__ __forceinline__ RowRange row_range(const SampleArgs& a, const RowWork
     r.m = m;
     r.at = at;
     r.done = m != m || m == -__builtin_inff() || rp.topk == 1;
-    r.end = (float)(a.shift + 1) * 0.693147182464599609375f;
+    r.end = weightless(a);
     const float range = (float)(((double)m - (double)lo) * rp.inv_t);
     r.bins = (float)kCoarse / fmaxf(fminf(range, r.end), 1e-30f);  // NaN range (infinities): the whole
     return r;
@@ -684,6 +687,70 @@ __device__ bool cross(const LastRegs& r, bool by_count, uint64_t x, LastShared& 
     return true;
 }
 
+// The prefix of the fine histogram, two bins per thread.
+__device__ __forceinline__ void fine_prefix(LastRegs& r, LastShared& s) {
+    constexpr int E = kFine / kRowThreads;
+    const int tid = threadIdx.x, lane = tid & 63;
+    uint32_t c = 0;
+    uint64_t w = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        r.c[e] = s.cnt[E * tid + e];
+        r.ws[e] = s.sum[E * tid + e];
+        c += r.c[e];
+        w += r.ws[e];
+    }
+    const uint32_t c0 = c;
+    const uint64_t w0 = w;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t cu = __shfl_up(c, o);
+        const uint64_t wu = __shfl_up((unsigned long long)w, o);
+        if (lane >= o) c += cu, w += wu;
+    }
+    if (lane == 63) s.wcnt[tid >> 6] = c, s.wsum[tid >> 6] = w;
+    __syncthreads();
+    c -= c0;
+    w -= w0;
+    for (int i = 0; i < (tid >> 6); ++i) c += s.wcnt[i], w += s.wsum[i];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        r.cb[e] = c;
+        r.wb[e] = w;
+        c += r.c[e];
+        w += r.ws[e];
+    }
+}
+
+// The three crossings and the token; false where a fine bin holds too many. Z:
+// the weight of all (cut: of which top-k leaves some out), Sm of what min-p keeps.
+__device__ __forceinline__ bool finish(const SampleArgs& a, int b, const RowParams& rp, const LastRegs& r, float m, uint64_t Z,
+                                       uint64_t Sm, bool cut, LastShared& s) {
+    const int tid = threadIdx.x;
+    const double scale = __builtin_ldexp(1.0, a.shift);
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {  // top-k, top-p, the draw
+        uint64_t x;
+        if (step == 0) {
+            if (!cut) continue;
+            x = (uint64_t)rp.topk - 1;
+        } else if (step == 1) {
+            const uint64_t target = topp_target(rp.topp, Z);
+            if (rp.topp >= 1.0 || target >= Z) continue;
+            x = target - 1;
+        } else {
+            Z = min(Z, Sm);
+            x = draw_target(rp.u, Z);
+        }
+        if (!cross(r, step == 0, x, s)) return false;
+        if (step < 2) Z = min(Z, (uint64_t)s.through);
+    }
+    if (tid == 0) {
+        a.token[b] = s.ri;
+        if (a.prob) a.prob[b] = (float)(weight(s.rl, m, rp.inv_t) / ((double)Z / scale));
+    }
+    return true;
+}
+
 // The token from what was collected; false where that is too much.
 __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
     const int tid = threadIdx.x, lane = tid & 63;
@@ -805,35 +872,13 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
         atomicAdd(&s.sum[r.f[q]], r.w[q]);
     }
     __syncthreads();
+    fine_prefix(r, s);
     {
         constexpr int E = kFine / kRowThreads;
-        uint32_t c = 0;
-        uint64_t w = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            r.c[e] = s.cnt[E * tid + e];
-            r.ws[e] = s.sum[E * tid + e];
-            c += r.c[e];
-            w += r.ws[e];
-        }
-        const uint32_t c0 = c;
-        const uint64_t w0 = w;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t cu = __shfl_up(c, o);
-            const uint64_t wu = __shfl_up((unsigned long long)w, o);
-            if (lane >= o) c += cu, w += wu;
-        }
-        if (lane == 63) s.wcnt[tid >> 6] = c, s.wsum[tid >> 6] = w;
-        __syncthreads();
-        c -= c0;
-        w -= w0;
-        for (int i = 0; i < (tid >> 6); ++i) c += s.wcnt[i], w += s.wsum[i];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            s.pcnt[E * tid + e] = r.cb[e] = c;
-            s.psum[E * tid + e] = r.wb[e] = w;
-            c += r.c[e];
-            w += r.ws[e];
+            s.pcnt[E * tid + e] = r.cb[e];
+            s.psum[E * tid + e] = r.wb[e];
         }
         __syncthreads();
         // From the sum over the collected bins to the one over the row's.
@@ -845,28 +890,91 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
             r.wb[e] += s.base_sum[k] - s.psum[k * F];
         }
     }
-#pragma unroll 1
-    for (int step = 0; step < 3; ++step) {  // top-k, top-p, the draw
-        uint64_t x;
-        if (step == 0) {
-            if (!cut) continue;
-            x = (uint64_t)rp.topk - 1;
-        } else if (step == 1) {
-            const uint64_t target = topp_target(rp.topp, Z);
-            if (rp.topp >= 1.0 || target >= Z) continue;
-            x = target - 1;
-        } else {
-            Z = min(Z, Sm);
-            x = draw_target(rp.u, Z);
+    return finish(a, b, rp, r, rr.m, Z, Sm, cut, s);
+}
+
+// A row of at most kCand logits by one workgroup, held in registers: the fine
+// histogram over the whole range at once (4000 logits with cuts XX us, by sample_row
+// alone 44). False where a bin holds too many.
+__device__ __forceinline__ bool sample_small(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float* row = a.logits + b * a.ld;
+    LastRegs r;
+    float m = -__builtin_inff(), lo = __builtin_inff();
+    int at = 0x7FFFFFFF;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int i = tid + q * kRowThreads;
+        r.i[q] = i;
+        r.l[q] = i < a.V ? row[i] : -__builtin_inff();
+        if (i < a.V && ahead(r.l[q], i, m, at)) m = r.l[q], at = i;
+        if (r.l[q] > -__builtin_inff()) lo = fminf(lo, r.l[q]);
+    }
+    for (int o = 32; o; o >>= 1) {
+        const float u = __shfl_xor(m, o);
+        const int ui = __shfl_xor(at, o);
+        if (ahead(u, ui, m, at)) m = u, at = ui;
+        lo = fminf(lo, __shfl_xor(lo, o));
+    }
+    if (lane == 0) s.el[wave] = m, s.ei[wave] = at, s.el[64 + wave] = lo;
+#pragma unroll
+    for (int e = 0; e < kFine / kRowThreads; ++e) {
+        s.cnt[tid + e * kRowThreads] = 0;
+        s.sum[tid + e * kRowThreads] = 0;
+    }
+    __syncthreads();
+    for (int i = 0; i < kRowThreads / 64; ++i) {
+        if (ahead(s.el[i], s.ei[i], m, at)) m = s.el[i], at = s.ei[i];
+        lo = fminf(lo, s.el[64 + i]);
+    }
+    if (m != m || m == -__builtin_inff() || rp.topk == 1) {
+        if (tid == 0) {
+            const bool none = m == -__builtin_inff();
+            a.token[b] = none ? -1 : at;
+            if (a.prob) a.prob[b] = m != m ? m : (none ? 0.0f : 1.0f);
         }
-        if (!cross(r, step == 0, x, s)) return false;
-        if (step < 2) Z = min(Z, (uint64_t)s.through);
+        return true;
     }
-    if (tid == 0) {
-        a.token[b] = s.ri;
-        if (a.prob) a.prob[b] = (float)(weight(s.rl, rr.m, rp.inv_t) / ((double)Z / scale));
+    const double scale = __builtin_ldexp(1.0, a.shift);
+    const float end = weightless(a);
+    const float bins = (float)kFine / fmaxf(fminf((float)(((double)m - (double)lo) * rp.inv_t), end), 1e-30f);
+    uint64_t Z = 0, Sm = 0;
+    uint32_t all = 0;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const double x = r.l[q] == m ? 0.0 : ((double)m - (double)r.l[q]) * rp.inv_t;
+        r.f[q] = -1;
+        r.w[q] = 0;
+        if (r.i[q] >= a.V || !(x < end)) continue;
+        const double w = exp(-x);
+        r.w[q] = fixed(w, scale);
+        r.f[q] = min((int)((float)x * bins), kFine - 1);
+        Z += r.w[q];
+        if (w >= rp.minp) Sm += r.w[q];
+        ++all;
+        atomicAdd(&s.cnt[r.f[q]], 1u);
+        atomicAdd(&s.sum[r.f[q]], r.w[q]);
     }
-    return true;
+    for (int o = 32; o; o >>= 1) {
+        Z += __shfl_xor((unsigned long long)Z, o);
+        Sm += __shfl_xor((unsigned long long)Sm, o);
+        all += __shfl_xor(all, o);
+    }
+    __syncthreads();  // and every wave has read el
+    if (lane == 0) s.base_sum[wave] = Z, s.base_sum[64 + wave] = Sm, s.base_cnt[wave] = all;
+    fine_prefix(r, s);
+    Z = Sm = 0;
+    all = 0;
+    for (int i = 0; i < kRowThreads / 64; ++i) Z += s.base_sum[i], Sm += s.base_sum[64 + i], all += s.base_cnt[i];
+    return finish(a, b, rp, r, m, Z, Sm, (uint32_t)rp.topk < all, s);
+}
+__global__ void __launch_bounds__(kRowThreads) sample_small_kernel(SampleArgs a) {
+    __shared__ SampleShared sh;
+    const int b = blockIdx.x;
+    const RowParams rp = row_params(a, b);
+    if (sample_small(a, b, rp, sh.last)) return;
+    __syncthreads();
+    sample_row(a, b, rp, sh.row);
 }
 
 // One workgroup per row: the token.
@@ -874,7 +982,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_last_kernel(SampleArgs a) 
     __shared__ SampleShared sh;
     const int b = blockIdx.x;
     const RowParams rp = row_params(a, b);
-    if (a.pieces > 0 && sample_collected(a, b, rp, sh.last)) return;
+    if (sample_collected(a, b, rp, sh.last)) return;
     __syncthreads();
     sample_row(a, b, rp, sh.row);
 }
@@ -887,6 +995,7 @@ using namespace alv;
 namespace alv {
 namespace {
 // Short rows are one workgroup's work.
+static_assert(kPiece == kCand, "a row in registers");
 int sample_pieces(int V) { return V <= kPiece ? 0 : (V + kPiece - 1) / kPiece; }
 }  // namespace
 }  // namespace alv
@@ -931,6 +1040,9 @@ extern "C" int alv_sample(const float* logits, int64_t ld, int B, int V, const f
         hipLaunchKernelGGL(sample_hist_kernel, grid, dim3(kPieceThreads), 0, st, a);
         hipLaunchKernelGGL(sample_collect_kernel, grid, dim3(kPieceThreads), 0, st, a);
     }
-    hipLaunchKernelGGL(sample_last_kernel, dim3(B), dim3(kRowThreads), 0, st, a);
+    if (a.pieces)
+        hipLaunchKernelGGL(sample_last_kernel, dim3(B), dim3(kRowThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(sample_small_kernel, dim3(B), dim3(kRowThreads), 0, st, a);
     return hip_check(hipGetLastError(), "sample kernels' launch");
 }
