@@ -636,17 +636,19 @@ union SampleShared {
 };
 
 // A thread's collected tokens, and its two fine bins.
+template <int PER>
 struct LastRegs {
-    float l[kPer];
-    int i[kPer], f[kPer];
-    unsigned long long w[kPer];
+    float l[PER];
+    int i[PER], f[PER];
+    unsigned long long w[PER];
     uint32_t cb[2], c[2];
     unsigned long long wb[2], ws[2];
 };
 
 // The token at which the running count or weight crosses x; false where a fine
 // bin holds too many to compare.
-__device__ bool cross(const LastRegs& r, bool by_count, uint64_t x, LastShared& s) {
+template <int PER>
+__device__ bool cross(const LastRegs<PER>& r, bool by_count, uint64_t x, LastShared& s) {
     const int tid = threadIdx.x;
 #pragma unroll
     for (int e = 0; e < kFine / kRowThreads; ++e) {
@@ -658,7 +660,7 @@ __device__ bool cross(const LastRegs& r, bool by_count, uint64_t x, LastShared& 
     const int f = s.f;
     if (s.cnt[f] > kLast) return false;
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) {
+    for (int q = 0; q < PER; ++q) {
         if (r.f[q] != f) continue;
         const int e = atomicAdd(&s.ne, 1);
         s.el[e] = r.l[q];
@@ -688,7 +690,8 @@ __device__ bool cross(const LastRegs& r, bool by_count, uint64_t x, LastShared& 
 }
 
 // The prefix of the fine histogram, two bins per thread.
-__device__ __forceinline__ void fine_prefix(LastRegs& r, LastShared& s) {
+template <int PER>
+__device__ __forceinline__ void fine_prefix(LastRegs<PER>& r, LastShared& s) {
     constexpr int E = kFine / kRowThreads;
     const int tid = threadIdx.x, lane = tid & 63;
     uint32_t c = 0;
@@ -723,8 +726,9 @@ __device__ __forceinline__ void fine_prefix(LastRegs& r, LastShared& s) {
 
 // The three crossings and the token; false where a fine bin holds too many. Z:
 // the weight of all (cut: of which top-k leaves some out), Sm of what min-p keeps.
-__device__ __forceinline__ bool finish(const SampleArgs& a, int b, const RowParams& rp, const LastRegs& r, float m, uint64_t Z,
-                                       uint64_t Sm, bool cut, LastShared& s) {
+template <int PER>
+__device__ __forceinline__ bool finish(const SampleArgs& a, int b, const RowParams& rp, const LastRegs<PER>& r, float m,
+                                       uint64_t Z, uint64_t Sm, bool cut, LastShared& s) {
     const int tid = threadIdx.x;
     const double scale = __builtin_ldexp(1.0, a.shift);
 #pragma unroll 1
@@ -825,7 +829,7 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
         }
         return true;
     }
-    LastRegs r;
+    LastRegs<kPer> r;
     float place[kPer];
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
@@ -893,17 +897,19 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
     return finish(a, b, rp, r, rr.m, Z, Sm, cut, s);
 }
 
-// A row of at most kCand logits by one workgroup, held in registers: the fine
-// histogram over the whole range at once (4000 logits with cuts XX us, by sample_row
-// alone 44). False where a bin holds too many.
+// A row by one workgroup, PER logits of it in each thread's registers: the fine
+// histogram over the whole range at once. One launch, bound by its chain of barriers:
+// 4096 logits with cuts 13 us (sample_row 44), 16384 21 (the four launches above 24),
+// 256 such rows 24 (48). False where a bin holds too many.
+template <int PER>
 __device__ __forceinline__ bool sample_small(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* row = a.logits + b * a.ld;
-    LastRegs r;
+    LastRegs<PER> r;
     float m = -__builtin_inff(), lo = __builtin_inff();
     int at = 0x7FFFFFFF;
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) {
+    for (int q = 0; q < PER; ++q) {
         const int i = tid + q * kRowThreads;
         r.i[q] = i;
         r.l[q] = i < a.V ? row[i] : -__builtin_inff();
@@ -941,7 +947,7 @@ __device__ __forceinline__ bool sample_small(const SampleArgs& a, int b, const R
     uint64_t Z = 0, Sm = 0;
     uint32_t all = 0;
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) {
+    for (int q = 0; q < PER; ++q) {
         const double x = r.l[q] == m ? 0.0 : ((double)m - (double)r.l[q]) * rp.inv_t;
         r.f[q] = -1;
         r.w[q] = 0;
@@ -968,11 +974,12 @@ __device__ __forceinline__ bool sample_small(const SampleArgs& a, int b, const R
     for (int i = 0; i < kRowThreads / 64; ++i) Z += s.base_sum[i], Sm += s.base_sum[64 + i], all += s.base_cnt[i];
     return finish(a, b, rp, r, m, Z, Sm, (uint32_t)rp.topk < all, s);
 }
+template <int PER>
 __global__ void __launch_bounds__(kRowThreads) sample_small_kernel(SampleArgs a) {
     __shared__ SampleShared sh;
     const int b = blockIdx.x;
     const RowParams rp = row_params(a, b);
-    if (sample_small(a, b, rp, sh.last)) return;
+    if (sample_small<PER>(a, b, rp, sh.last)) return;
     __syncthreads();
     sample_row(a, b, rp, sh.row);
 }
@@ -994,9 +1001,18 @@ using namespace alv;
 
 namespace alv {
 namespace {
-// Short rows are one workgroup's work.
-static_assert(kPiece == kCand, "a row in registers");
-int sample_pieces(int V) { return V <= kPiece ? 0 : (V + kPiece - 1) / kPiece; }
+// Short rows, as many logits as fit the registers of one workgroup.
+constexpr int kSmall = 16 * kRowThreads;
+int sample_pieces(int V) { return V <= kSmall ? 0 : (V + kPiece - 1) / kPiece; }
+template <class F>
+void small_row(int V, F go) {
+    if (V <= 4 * kRowThreads)
+        go(sample_small_kernel<4>);
+    else if (V <= 8 * kRowThreads)
+        go(sample_small_kernel<8>);
+    else
+        go(sample_small_kernel<16>);
+}
 }  // namespace
 }  // namespace alv
 
@@ -1043,6 +1059,6 @@ extern "C" int alv_sample(const float* logits, int64_t ld, int B, int V, const f
     if (a.pieces)
         hipLaunchKernelGGL(sample_last_kernel, dim3(B), dim3(kRowThreads), 0, st, a);
     else
-        hipLaunchKernelGGL(sample_small_kernel, dim3(B), dim3(kRowThreads), 0, st, a);
+        small_row(V, [&](auto k) { hipLaunchKernelGGL(k, dim3(B), dim3(kRowThreads), 0, st, a); });
     return hip_check(hipGetLastError(), "sample kernels' launch");
 }
