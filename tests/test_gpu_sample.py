@@ -209,3 +209,18 @@ def test_top_k_of_any_size(dev):
     for k in (5000, 2 ** 31, 2 ** 32 + 1, -2 ** 40):
         for a, b in zip(aa.sample(x, u, top_k=k), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("V", [1024, 1025, 4095, 4097, 8192, 8193, 16383, 16384, 16385])
+def test_sizes_around_the_variants_ends(dev, V):
+    """Cuts of every kind, ties past what a bin compares, and -infinity among them."""
+    x = normal(6, V, seed=V)
+    x[1] = (x[1] * 2).round() / 2       # a few dozen values
+    x[2, ::3] = -math.inf
+    x[3] = 0.25                         # one value
+    x[4] = x[4] * 1e-3
+    x[4, V // 2] = 40.0                 # one far above the rest
+    u = [0.3, 0.7, 0.999, 0.5, 0.9999999, 0.0]
+    check(dev, x, u, temperature=0.7, top_k=[0, 50, 0, 700, 0, 3], top_p=[0.95, 1.0, 0.6, 0.9, 0.999999, 0.5],
+          min_p=[0.0, 0.0, 0.05, 0.0, 0.0, 0.2])
+    check(dev, x, u)
