@@ -217,7 +217,7 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
 // thread; pointers and pairs come in the kernel's arguments, so a call is one
 // launch and no transfer. Bound by memory: 450 pages of 64 KB in 64
 // caches 370 us, 5.1 TB/s read and written; 6 pages of 64 KB in 24 caches, 4.4 us,
-// by the launch (16 us with the checks of 24 tensors on the host).
+// by the launch (14 us with the checks of 24 tensors on the host).
 constexpr int kCopyCaches = 128;  // per launch
 constexpr int kCopyPairs = 256;
 constexpr int kCopyChunk = 16384;  // bytes per workgroup

@@ -218,11 +218,16 @@ def copy_pages(caches, src, dst) -> None:
     shape, strides, dtype, index = first.shape, first.stride(), first.dtype, dev.index
     if len(shape) < 2 or first.numel() == 0:
         raise ValueError(f"a cache must be (pages, ...), got shape {tuple(shape)}")
-    if not all([isinstance(t, torch.Tensor) for t in caches]) or {t.get_device() for t in caches} != {index}:
+    T = torch.Tensor
+    try:  # (the methods mapped, and strides only where some are not contiguous: these tests are most of a small call)
+        one = set(map(T.get_device, caches)) == {index}
+        whole = all(map(T.is_contiguous, caches))
+        ptrs = array.array("Q", map(T.data_ptr, caches))
+    except TypeError:
+        one = False
+    if not one:
         raise ValueError(f"the caches must be tensors on one GPU, {dev}")
-    # (one test each where all are contiguous: strides cost 0.3 us a cache)
-    whole = all([t.is_contiguous() for t in caches])
-    if len({t.dtype for t in caches}) + len({t.shape for t in caches}) != 2 or (
+    if len({t.dtype for t in caches}) + len(set(map(T.size, caches))) != 2 or (
             not whole and len({t.stride() for t in caches}) != 1):
         raise ValueError(f"the caches must be alike: {dtype} {tuple(shape)} {strides}, and not all are")
     if not whole and not first[0].is_contiguous():
@@ -232,7 +237,6 @@ def copy_pages(caches, src, dst) -> None:
         raise ValueError(f"{len(src)} sources and {len(dst)} destinations")
     esize = first.element_size()
     n = first.numel() // shape[0] * esize
-    ptrs = array.array("Q", [t.data_ptr() for t in caches])
     with _on(dev):
         check(lib().alv_copy_pages(ptrs.buffer_info()[0], len(caches), n, strides[0] * esize if shape[0] > 1 else n,
                                    shape[0], src.buffer_info()[0], dst.buffer_info()[0], len(src), _stream(first)),

@@ -748,3 +748,13 @@ def test_attention_many_drafts(dev, D, most):
     hit = torch.zeros(len(want), dtype=torch.bool)
     hit[sum(n[:s + 1]) - 1] = True
     assert torch.isnan(got[hit]).all() and ((got - want).abs() <= tol)[~hit].all()
+
+
+def test_copy_pages_refuses_what_is_no_cache(dev):
+    from alveare_amd import copy_pages
+
+    c = torch.zeros(4, 2, 16, 64, dtype=bf, device=dev)
+    for bad in ([c, 1], [c, None], [c, c.cpu()], [c, c[:2]], [c, c.float()], [c, c.transpose(1, 2)]):
+        with pytest.raises(ValueError):
+            copy_pages(bad, [0], [1])
+    assert (c == 0).all()
