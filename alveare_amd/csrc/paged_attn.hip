@@ -945,7 +945,7 @@ __device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, i
 }
 
 template <int D>
-__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan& sc0, int gt, int kvh, int split, int nsplit, int entry, unsigned char* smem) {
+__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan& sc0, int gt, int kvh, int split, int nsplit, int entry, int* tab, unsigned char* smem) {
     constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D);
     constexpr int DW = D / DS;            // this wave's columns of the output (and of its scores' products)
     constexpr int TB = tile_bytes(D), NC = D / 8, RPL = 512 / D;
@@ -967,8 +967,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     const TileSpan sp = at_item.sp;
     const int u0 = uniform((int)((int64_t)sp.nu * split / nsplit));
     const int u1 = uniform((int)((int64_t)sp.nu * (split + 1) / nsplit));
-    if (a.tab && split == 0 && tid == 0) {
-        int* e = a.tab + kTabInts * (1 + gt * a.kv_heads + kvh);
+    if (tab && split == 0 && tid == 0) {
+        int* e = tab + kTabInts * (1 + gt * a.kv_heads + kvh);
         e[0] = entry, e[1] = nsplit, e[2] = first, e[3] = rt, e[4] = sp.rows, e[5] = kvh;
     }
 
@@ -1317,7 +1317,8 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
         gt = item / a.kv_heads;
         kvh = item - gt * a.kv_heads;
     }
-    tile_item<D>(a, sc0, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), smem);
+    // (tiles of more rows than max_q told of may be more than tab has entries for: they are not split)
+    tile_item<D>(a, sc0, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), split ? a.tab : nullptr, smem);
 }
 
 // The parts of the tiles joined, `groups` workgroups to a tile, merge_rows(D) of

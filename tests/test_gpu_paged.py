@@ -758,3 +758,31 @@ def test_copy_pages_refuses_what_is_no_cache(dev):
         with pytest.raises(ValueError):
             copy_pages(bad, [0], [1])
     assert (c == 0).all()
+
+
+def test_attention_more_tiles_than_max_q_tells_of(dev):
+    """max_q = 1 for a sequence of 68000 rows of 128 heads: the merge's table has one entry, the call 68000
+    tiles. Nothing behind the workspace is written, and the rows are right."""
+    import ctypes
+
+    from alveare_amd import lib
+
+    T, heads, D, window = 68000, 128, 64, 16
+    b = R.Batch([T], [T], kv_heads=1, D=D, page=1024, dev=dev)
+    q = torch.randn(T, heads * D, generator=torch.Generator(dev).manual_seed(1), device=dev).to(bf)
+    out = torch.full_like(q, 7.0)
+    need = lib().alv_attention_paged_workspace(heads, 1, D, 1, T, 1)
+    ws = torch.full((need + (4 << 20),), 0xA5, dtype=torch.uint8, device=dev)
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    rc = lib().alv_attention_paged(ptr(q), heads * D, ptr(b.kp), ptr(b.vp), 1024 * D, 1024 * D, b.pages, 1024, ptr(b.table),
+                                   b.table.shape[1], b.table.shape[1], ptr(b.q_start), ptr(b.kv_len), 1, T, 1, heads, 1, D,
+                                   window, 0, 0.1, ptr(out), heads * D, ptr(ws), need,
+                                   ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+    assert rc == 0
+    assert (ws[need:] == 0xA5).all()
+    for t in (0, 1, 15, 16, 17, 1023, 1024, 33333, T - 2, T - 1):
+        lo = max(0, t + 1 - window)
+        one = R.Batch([1], [t + 1 - lo], kv_heads=1, D=D, page=16, dev="cpu")
+        one.k[0], one.v[0] = b.k[0][lo:t + 1], b.v[0][lo:t + 1]
+        want, tol = R.attention(q[t:t + 1], one, heads, scale=0.1)
+        assert ((out[t].double().cpu().view_as(want[0]) - want[0]).abs() <= tol[0]).all(), t
