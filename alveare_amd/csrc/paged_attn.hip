@@ -1281,6 +1281,7 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
     const int tiles = tile_count<TR>(a, sc0, lane), items = tiles * a.kv_heads;
     const bool split = items <= a.max_items;
     if (a.tab && blockIdx.x == 0 && tid == 0) a.tab[0] = split ? items : 0;
+    if (items == 0) return;  // (the streaming kernel's all; there may be no slots to plan for)
     int gt, kvh, part = 0, parts = 1, entry = 0;
     if (split) {
         int* nu = reinterpret_cast<int*>(smem);

@@ -786,3 +786,11 @@ def test_attention_more_tiles_than_max_q_tells_of(dev):
         one.k[0], one.v[0] = b.k[0][lo:t + 1], b.v[0][lo:t + 1]
         want, tol = R.attention(q[t:t + 1], one, heads, scale=0.1)
         assert ((out[t].double().cpu().view_as(want[0]) - want[0]).abs() <= tol[0]).all(), t
+
+
+@pytest.mark.parametrize("D,pad", [(64, 1200), (64, 100), (128, 1200), (256, 6000), (512, 6000)])
+def test_attention_mostly_padding(dev, D, pad):
+    """Rows enough for many tiles, of which the sequences own a few: the tile kernel is launched and has none
+    (pad = 100: few enough that it takes the batch alone)."""
+    b = R.Batch([1, 2, 0, 1], [300, 2, 40, 1], kv_heads=8, D=D, page=16, dev=dev, extra_rows=pad)
+    check_attention(b, 64 if D <= 128 else 8, dev, max_q=0)
