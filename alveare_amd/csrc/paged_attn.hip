@@ -1409,9 +1409,10 @@ struct AttnPlan {
 AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
     AttnPlan p{};
     const int64_t g = heads / kv_heads;
+    max_q = std::min(max_q, T);  // (and its products stay within 64 bits)
     const int qt_max = D <= 128 ? 4 : (D == 256 ? 2 : 1);
-    const int64_t most = (max_q > 0 ? std::min(max_q, T) : T) * g;          // rows of a sequence at most
-    const int64_t rows = (max_q > 0 ? std::min(max_q, T) : (T + B - 1) / B) * g;  // as far as is known
+    const int64_t most = (max_q > 0 ? max_q : T) * g;          // rows of a sequence at most
+    const int64_t rows = (max_q > 0 ? max_q : ((int64_t)T + B - 1) / B) * g;  // as far as is known
     const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2);
     const int64_t tr = 128;
     auto tiles_of = [&](int64_t row_limit) {  // that sequences of more rows than that have at most

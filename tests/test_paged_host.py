@@ -199,3 +199,13 @@ def test_attention_workspace(L):
     assert attn(L) == ALV_ERR_ARG and attn(L, ws=P, wb=need - 1) == ALV_ERR_ARG
     assert attn(L, ws=ctypes.c_void_p((1 << 20) + 8), wb=need) == ALV_ERR_ALIGN
     assert L.alv_sample_workspace(1, 1000) == 0 < L.alv_sample_workspace(1, 32000) < L.alv_sample_workspace(2, 32000)
+
+
+def test_attention_workspace_of_any_hint(L):
+    """No sequence owns more than T rows: a larger max_q is T, whatever it is multiplied by."""
+    for heads, kv, D, B, T in ((65536, 1, 64, 1 << 24, 100), (65536, 1, 512, (1 << 31) - 1, 100), (16, 8, 256, 3, 7),
+                               (512, 512, 64, (1 << 31) - 1, 1 << 21)):
+        want = L.alv_attention_paged_workspace(heads, kv, D, B, T, T)
+        assert want < 1 << 40
+        for mq in (T + 1, 1 << 20, (1 << 31) - 1):
+            assert L.alv_attention_paged_workspace(heads, kv, D, B, T, max(mq, T)) == want
