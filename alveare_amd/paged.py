@@ -251,7 +251,7 @@ class PagedCache:
     is the host's; only page copies and the tables go to the device, in the
     order of the current stream. ``batch`` gives the tensors the kernels take.
     A call that needs more pages than are free raises ``MemoryError`` and changes
-    nothing."""
+    nothing, nor does one whose copies raise."""
 
     def __init__(self, *, layers: int, kv_heads: int, D: int, pages: int, page_size: int, slots: int, max_pages: int,
                  device):
@@ -288,11 +288,6 @@ class PagedCache:
     def _copy(self, src: list[int], dst: list[int]) -> None:
         copy_pages(self.k + self.v, src, dst)
 
-    def _take(self) -> int:
-        p = heapq.heappop(self._free)
-        self._shared[p] = 1
-        return p
-
     def _drop(self, page: int) -> None:
         self._shared[page] -= 1
         if self._shared[page] == 0:
@@ -309,31 +304,46 @@ class PagedCache:
         if any(m < 0 for m in n):
             raise ValueError("counts must not be negative")
         S = self.page_size
-        need, left = 0, {}
+        need, left, plan = 0, {}, []
         for s, m in zip(slots, n):
             total = -(-(self._len[s] + m) // S)
             if total > self.max_pages:
                 raise ValueError(f"slot {s}: {self._len[s] + m} positions, its table holds {self.max_pages * S}")
-            need += total - len(self._table[s])
+            more, copied = total - len(self._table[s]), False
             if m and self._len[s] % S:
                 last = self._table[s][-1]
                 left[last] = left.get(last, self._shared[last]) - 1
-                need += left[last] > 0  # the last to write keeps the page
+                copied = left[last] > 0  # the last to write keeps the page
+            plan.append((s, m, copied, more))
+            need += copied + more
         if need > len(self._free):
             raise MemoryError(f"{need} pages needed, {len(self._free)} free")
-        src, dst = [], []
-        for s, m in zip(slots, n):
-            t = self._table[s]
-            if m and self._len[s] % S and self._shared[t[-1]] > 1:
-                src.append(t[-1])
-                self._shared[t[-1]] -= 1
-                t[-1] = self._take()
-                dst.append(t[-1])
-            self._len[s] += m
-            while len(t) * S < self._len[s]:
-                t.append(self._take())
+        taken = [heapq.heappop(self._free) for _ in range(need)]
+        src, dst, at = [], [], 0  # (a slot's copy, then the pages it grows by)
+        for s, m, copied, more in plan:
+            if copied:
+                src.append(self._table[s][-1])
+                dst.append(taken[at])
+            at += copied + more
         if src:
-            self._copy(src, dst)
+            try:
+                self._copy(src, dst)
+            except BaseException:
+                for p in taken:
+                    heapq.heappush(self._free, p)
+                raise
+        for p in src:
+            self._shared[p] -= 1
+        for p in taken:
+            self._shared[p] = 1
+        at = 0
+        for s, m, copied, more in plan:
+            t = self._table[s]
+            if copied:
+                t.pop()
+            t += taken[at:at + copied + more]
+            at += copied + more
+            self._len[s] += m
 
     def fork(self, src: int, dst: int) -> None:
         """``dst`` (empty) gets the positions of ``src``: its pages, shared until

@@ -209,3 +209,36 @@ def test_attention_workspace_of_any_hint(L):
         assert want < 1 << 40
         for mq in (T + 1, 1 << 20, (1 << 31) - 1):
             assert L.alv_attention_paged_workspace(heads, kv, D, B, T, max(mq, T)) == want
+
+
+def test_cache_is_unchanged_where_a_copy_fails(cache, monkeypatch):
+    """A reserve or compaction whose copies raise leaves tables, lengths, shares and free pages as they were."""
+    from alveare_amd import paged
+
+    c = cache
+    c.reserve([0, 3], [20, 33])
+    c.fork(0, 1)
+    c.fork(0, 2)
+    state = lambda: ([c.table(s) for s in range(4)], [c.length(s) for s in range(4)], c.free_pages,  # noqa: E731
+                     list(c._shared), sorted(c._free))
+    before = state()
+
+    def fail(*_):
+        raise RuntimeError("no copy")
+
+    with monkeypatch.context() as m:
+        m.setattr(paged, "copy_pages", fail)
+        with pytest.raises(RuntimeError, match="no copy"):
+            c.reserve([3, 0, 1], [5, 13, 1])
+        assert state() == before
+        c.free(0)  # slots 1 and 2 hold pages 0 and 1, slot 3 pages 2, 3 and 4
+        c.free(1)
+        c.free(2)
+        before = state()
+        with pytest.raises(RuntimeError, match="no copy"):
+            c.compact()
+        assert state() == before
+    assert c.compact() == 2 and c.copies == [([3, 4], [0, 1])] and c.table(3) == [2, 0, 1]
+    c.fork(3, 1)
+    c.reserve([1], 1)
+    assert c.copies[-1] == ([1], [3]) and c.table(1) == [2, 0, 3] and c.free_pages == 4
