@@ -109,6 +109,10 @@ def _shape2(t: torch.Tensor, name: str, dev: torch.device):
     return *t.shape, ld
 
 
+def _far(**numbers: int) -> None:
+    raise ValueError("past 32 bits: " + ", ".join(f"{k}={v}" for k, v in numbers.items()))
+
+
 def _narrow(name: str, have: int, width: int) -> None:
     raise ValueError(f"{name} rows must hold {width} values, got {have}")
 
@@ -133,6 +137,9 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
     dev = _need_gpu(qkv)
     (pages, kv_heads, S, D), ks, vs, B, W, ldt, T, width, ldqkv = _args(qkv, "qkv", kpages, vpages, page_table, q_start,
                                                                         kv_len, dev)
+    v_off = max(v_off, -1)
+    if max(heads, k_off, v_off) > _INT_MAX or min(heads, k_off, half or 0) < -_INT_MAX:
+        _far(heads=heads, k_off=k_off, v_off=v_off, half=half)
     if width < (k_off if v_off < 0 else v_off) + kv_heads * D:
         _narrow("qkv", width, (k_off if v_off < 0 else v_off) + kv_heads * D)
     ldq = heads * D
@@ -175,6 +182,8 @@ def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     if width < ldo:
         _narrow("q", width, ldo)
     window, sinks, max_q = min(window, _INT_MAX), min(sinks, _INT_MAX), min(max_q, _INT_MAX)
+    if min(heads, window, sinks, max_q) < -_INT_MAX:
+        _far(heads=heads, window=window, sinks=sinks, max_q=max_q)
     if out is None:
         out = torch.empty_like(q) if width == ldo == ldq else q.new_empty((T, ldo))
     else:

@@ -242,3 +242,44 @@ def test_cache_is_unchanged_where_a_copy_fails(cache, monkeypatch):
     c.fork(3, 1)
     c.reserve([1], 1)
     assert c.copies[-1] == ([1], [3]) and c.table(1) == [2, 0, 3] and c.free_pages == 4
+
+
+def test_negative_numbers_past_32_bits(monkeypatch):
+    """What a C int would turn into another number is refused before the call; any negative v_off means the raw k."""
+    from alveare_amd import paged
+
+    class Reached(Exception):
+        pass
+
+    def reach(*a):
+        raise Reached(a)
+
+    class Fake:
+        alv_attention_paged = alv_qkv_post_paged = staticmethod(reach)
+        alv_attention_paged_workspace = staticmethod(lambda *a: 0)
+
+    monkeypatch.setattr(paged, "lib", Fake)
+    monkeypatch.setattr(paged, "_need_gpu", lambda t: t.device)
+    monkeypatch.setattr(paged, "_on", lambda dev: torch.no_grad())
+    monkeypatch.setattr(paged, "_stream", lambda t: 0)
+    bf = torch.bfloat16
+    qkv, pg = torch.zeros(3, 256, dtype=bf), torch.zeros(4, 1, 16, 64, dtype=bf)
+    batch = pg, pg, torch.zeros(2, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    out, wrap = torch.zeros(3, 128, dtype=bf), 2 ** 32
+    attend = lambda **kw: paged.attention_paged(qkv[:, :128], *batch, out=out, **{"heads": 2, **kw})  # noqa: E731
+    post = lambda **kw: paged.qkv_post_paged(qkv, *batch, q_out=out, rope=torch.zeros(9, 64, dtype=bf),  # noqa: E731
+                                             **{"heads": 2, "k_off": 128, "v_off": 192, **kw})
+    with pytest.raises(Reached):
+        attend(window=5, sinks=1, max_q=3)
+    with pytest.raises(Reached):
+        post()
+    for kw in (dict(window=-wrap), dict(window=-wrap + 7), dict(sinks=-wrap), dict(max_q=-wrap + 1), dict(heads=2 - wrap)):
+        with pytest.raises(ValueError):
+            attend(**kw)
+    for kw in (dict(heads=2 - wrap), dict(k_off=128 - wrap), dict(k_off=128 + wrap), dict(half=32 - wrap)):
+        with pytest.raises(ValueError):
+            post(**kw)
+    for v_off in (-1, -wrap, 192 - wrap):
+        with pytest.raises(Reached) as e:
+            post(v_off=v_off)
+        assert e.value.args[0][3] == -1
