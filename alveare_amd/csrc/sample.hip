@@ -263,8 +263,8 @@ __device__ void sample_row(const SampleArgs& a, int b, const RowParams& rp, RowS
 // its prefix sums the bins in which the three crossings can fall, and the
 // collection of those bins' tokens; the crossings among those, by comparison
 // where they are few, else by a finer histogram first. Every step moves integers,
-// so no order of atomics shows. A row whose bins hold too many (logits all alike
-// but for a few far ones) is done by sample_row.
+// so no order of atomics shows. A row whose bins hold more than kCand tokens (thousands
+// of one value, or more than a million logits) is done by sample_row.
 //
 // What bounds it: one row is a chain of launches, each a trip or two to memory (one
 // row of 262144: 25 us, of them 4 + 8 + 9 + 4 in the kernels); many rows, the
@@ -625,6 +625,7 @@ struct LastShared {
     int ne, f;
     uint32_t before_cnt;
     unsigned long long before_sum;
+    unsigned long long lo, hi;  // the first and last of its places in the order
     // the token found, and the weight up to and with it
     float rl;
     int ri;
@@ -635,36 +636,178 @@ union SampleShared {
     LastShared last;
 };
 
-// A thread's collected tokens, and its two fine bins.
-template <int PER>
+// A thread's two bins: counts and weights (c, ws), and what comes before them (cb, wb).
+struct BinPair {
+    uint32_t cb[kFine / kRowThreads], c[kFine / kRowThreads];
+    unsigned long long wb[kFine / kRowThreads], ws[kFine / kRowThreads];
+};
+// A thread's collected tokens.
+// LINE: token q is index i[0] + 1024 q, else i[q].
+template <int PER, bool LINE>
 struct LastRegs {
     float l[PER];
-    int i[PER], f[PER];
+    int i[LINE ? 1 : PER];
+    uint32_t two[PER / 2];  // the fine bins of two tokens each (of none: 0xFFFF)
     unsigned long long w[PER];
-    uint32_t cb[2], c[2];
-    unsigned long long wb[2], ws[2];
+    __device__ __forceinline__ int bin(int q) const { return two[q / 2] >> 16 * (q & 1) & 0xFFFFu; }
+    __device__ __forceinline__ void set_bin(int q, int f) {
+        two[q / 2] = q & 1 ? (two[q / 2] & 0xFFFFu) | (uint32_t)f << 16 : (two[q / 2] & 0xFFFF0000u) | (uint32_t)f;
+    }
+    __device__ __forceinline__ void no_bins() {
+#pragma unroll
+        for (int q = 0; q < PER / 2; ++q) two[q] = ~0u;
+    }
+    __device__ __forceinline__ int index(int q) const {
+        if constexpr (!LINE) return i[q];
+        int first = i[0];
+        asm volatile("" : "+v"(first));  // (as below)
+        return first + q * kRowThreads;
+    }
 };
 
-// The token at which the running count or weight crosses x; false where a fine
-// bin holds too many to compare.
-template <int PER>
-__device__ bool cross(const LastRegs<PER>& r, bool by_count, uint64_t x, LastShared& s) {
-    const int tid = threadIdx.x;
+// A histogram's two bins of this thread, `c0` and `w0` ahead of the first bin.
+__device__ __forceinline__ void bin_prefix(const uint32_t* cnt, const unsigned long long* sum, uint32_t c0, uint64_t w0,
+                                           BinPair& r, LastShared& s) {
+    constexpr int E = kFine / kRowThreads;
+    const int tid = threadIdx.x, lane = tid & 63;
+    uint32_t own = 0;
+    uint64_t ownw = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        r.c[e] = cnt[E * tid + e];
+        r.ws[e] = sum[E * tid + e];
+        own += r.c[e];
+        ownw += r.ws[e];
+    }
+    uint32_t c = own;
+    uint64_t w = ownw;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t cu = __shfl_up(c, o);
+        const uint64_t wu = __shfl_up((unsigned long long)w, o);
+        if (lane >= o) c += cu, w += wu;
+    }
+    if (lane == 63) s.wcnt[tid >> 6] = c, s.wsum[tid >> 6] = w;
+    __syncthreads();
+    c += c0 - own;
+    w += w0 - ownw;
+    for (int i = 0; i < (tid >> 6); ++i) c += s.wcnt[i], w += s.wsum[i];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        r.cb[e] = c;
+        r.wb[e] = w;
+        c += r.c[e];
+        w += r.ws[e];
+    }
+}
+// The bin in which the running count or weight crosses x, and what comes before it, for all threads behind the
+// next barrier.
+__device__ __forceinline__ void find_bin(const BinPair& r, bool by_count, uint64_t x, LastShared& s) {
 #pragma unroll
     for (int e = 0; e < kFine / kRowThreads; ++e) {
         const uint64_t b = by_count ? r.cb[e] : r.wb[e], own = by_count ? r.c[e] : r.ws[e];
-        if (b <= x && x < b + own) s.f = tid * (kFine / kRowThreads) + e, s.before_cnt = r.cb[e], s.before_sum = r.wb[e];
+        if (b <= x && x < b + own)
+            s.f = threadIdx.x * (kFine / kRowThreads) + e, s.before_cnt = r.cb[e], s.before_sum = r.wb[e];
     }
-    if (tid == 0) s.ne = 0;
-    __syncthreads();
-    const int f = s.f;
-    if (s.cnt[f] > kLast) return false;
+}
+
+// A token's place in the order (logit descending, index ascending) as one number, the logit's 32 bits above the
+// index's (V needs no more than 62 - shift). Computed anew in each turn of a loop: kept, it is two registers a
+// token, and 16 tokens leave none (256 rows of 16384 logits 26 -> 44 us, with indices and bins kept too).
+__device__ __forceinline__ uint64_t place_in_order(float l, int i, int shift) {
+    asm volatile("" : "+v"(l));
+    return (uint64_t)~key_of(l) << (62 - shift) | (uint32_t)i;
+}
+
+// The tokens of fine bin f (logits that differ in their last bits, or not at all: those rounded to bf16 have
+// hundreds of each value) cut to at most kLast around the crossing: their places [lo, hi] into kFine equal parts,
+// until the one that holds it has no more. Places differ by one at least, so that ends; two or three times for a
+// bin of a few values. A row of 262144 logits with top-p, rounded to bf16 41 us (not rounded 34; by one workgroup
+// from the logits, which tied bins went to once, 700).
+template <int PER, bool LINE>
+__device__ __forceinline__ void narrow(const LastRegs<PER, LINE>& r, int shift, bool by_count, uint64_t x, int f, uint64_t& lo,
+                                       uint64_t& hi, LastShared& s) {
+    const int tid = threadIdx.x;
+    unsigned long long first = ~0ull, last = 0;
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
-        if (r.f[q] != f) continue;
+        if (r.bin(q) != f) continue;
+        const unsigned long long c = place_in_order(r.l[q], r.index(q), shift);
+        first = min(first, c);
+        last = max(last, c);
+    }
+    for (int o = 32; o; o >>= 1) {
+        first = min(first, __shfl_xor(first, o));
+        last = max(last, __shfl_xor(last, o));
+    }
+    if ((tid & 63) == 0) {
+        atomicMin(&s.lo, first);
+        atomicMax(&s.hi, last);
+    }
+    __syncthreads();
+    lo = s.lo;
+    hi = s.hi;
+    uint32_t n;
+    do {
+        const int sh = max(0, 53 - __clzll(hi - lo));  // (hi - lo) >> sh is less than kFine
+        const uint32_t c0 = s.before_cnt;
+        const uint64_t w0 = s.before_sum;
+#pragma unroll
+        for (int e = 0; e < kFine / kRowThreads; ++e) {
+            s.pcnt[tid + e * kRowThreads] = 0;
+            s.psum[tid + e * kRowThreads] = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            if (r.bin(q) != f) continue;
+            const uint64_t c = place_in_order(r.l[q], r.index(q), shift);
+            if (c < lo || c > hi) continue;
+            atomicAdd(&s.pcnt[(c - lo) >> sh], 1u);
+            atomicAdd(&s.psum[(c - lo) >> sh], r.w[q]);
+        }
+        __syncthreads();
+        BinPair p;
+        bin_prefix(s.pcnt, s.psum, c0, w0, p, s);
+        find_bin(p, by_count, x, s);
+        __syncthreads();
+        n = s.pcnt[s.f];
+        lo += (uint64_t)s.f << sh;
+        hi = min(hi, lo + ((1ull << sh) - 1));
+        __syncthreads();
+    } while (n > kLast);
+}
+
+// The token at which the running count or weight crosses x.
+template <int PER, bool LINE>
+__device__ __forceinline__ void cross(const LastRegs<PER, LINE>& r, int shift, bool by_count, uint64_t x, LastShared& s) {
+    const int tid = threadIdx.x;
+    BinPair p;
+#pragma unroll
+    for (int e = 0; e < kFine / kRowThreads; ++e) {
+        const int i = tid * (kFine / kRowThreads) + e;
+        p.c[e] = s.cnt[i];
+        p.ws[e] = s.sum[i];
+        p.cb[e] = e ? p.cb[e - 1] + p.c[e - 1] : s.base_cnt[tid];
+        p.wb[e] = e ? p.wb[e - 1] + p.ws[e - 1] : s.base_sum[tid];
+    }
+    find_bin(p, by_count, x, s);
+    if (tid == 0) {
+        s.ne = 0;
+        s.lo = ~0ull;
+        s.hi = 0;
+    }
+    __syncthreads();
+    const int f = s.f;
+    uint64_t lo = 0, hi = ~0ull;
+    if (s.cnt[f] > kLast) narrow(r, shift, by_count, x, f, lo, hi, s);
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        if (r.bin(q) != f) continue;
+        const uint64_t c = place_in_order(r.l[q], r.index(q), shift);
+        if (c < lo || c > hi) continue;
         const int e = atomicAdd(&s.ne, 1);
         s.el[e] = r.l[q];
-        s.ei[e] = r.i[q];
+        s.ei[e] = r.index(q);
         s.ew[e] = r.w[q];
     }
     __syncthreads();
@@ -686,48 +829,12 @@ __device__ bool cross(const LastRegs<PER>& r, bool by_count, uint64_t x, LastSha
         if (before <= x && x < before + mine) s.rl = l, s.ri = id, s.through = bsum + s.ew[tid];
     }
     __syncthreads();
-    return true;
 }
 
-// The prefix of the fine histogram, two bins per thread.
-template <int PER>
-__device__ __forceinline__ void fine_prefix(LastRegs<PER>& r, LastShared& s) {
-    constexpr int E = kFine / kRowThreads;
-    const int tid = threadIdx.x, lane = tid & 63;
-    uint32_t c = 0;
-    uint64_t w = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        r.c[e] = s.cnt[E * tid + e];
-        r.ws[e] = s.sum[E * tid + e];
-        c += r.c[e];
-        w += r.ws[e];
-    }
-    const uint32_t c0 = c;
-    const uint64_t w0 = w;
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t cu = __shfl_up(c, o);
-        const uint64_t wu = __shfl_up((unsigned long long)w, o);
-        if (lane >= o) c += cu, w += wu;
-    }
-    if (lane == 63) s.wcnt[tid >> 6] = c, s.wsum[tid >> 6] = w;
-    __syncthreads();
-    c -= c0;
-    w -= w0;
-    for (int i = 0; i < (tid >> 6); ++i) c += s.wcnt[i], w += s.wsum[i];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        r.cb[e] = c;
-        r.wb[e] = w;
-        c += r.c[e];
-        w += r.ws[e];
-    }
-}
-
-// The three crossings and the token; false where a fine bin holds too many. Z:
-// the weight of all (cut: of which top-k leaves some out), Sm of what min-p keeps.
-template <int PER>
-__device__ __forceinline__ bool finish(const SampleArgs& a, int b, const RowParams& rp, const LastRegs<PER>& r, float m,
+// The three crossings and the token. Z: the weight of all (cut: of which top-k
+// leaves some out), Sm of what min-p keeps.
+template <int PER, bool LINE>
+__device__ __forceinline__ void finish(const SampleArgs& a, int b, const RowParams& rp, const LastRegs<PER, LINE>& r, float m,
                                        uint64_t Z, uint64_t Sm, bool cut, LastShared& s) {
     const int tid = threadIdx.x;
     const double scale = __builtin_ldexp(1.0, a.shift);
@@ -745,14 +852,13 @@ __device__ __forceinline__ bool finish(const SampleArgs& a, int b, const RowPara
             Z = min(Z, Sm);
             x = draw_target(rp.u, Z);
         }
-        if (!cross(r, step == 0, x, s)) return false;
+        cross(r, a.shift, step == 0, x, s);
         if (step < 2) Z = min(Z, (uint64_t)s.through);
     }
     if (tid == 0) {
         a.token[b] = s.ri;
         if (a.prob) a.prob[b] = (float)(weight(s.rl, m, rp.inv_t) / ((double)Z / scale));
     }
-    return true;
 }
 
 // The token from what was collected; false where that is too much.
@@ -829,7 +935,7 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
         }
         return true;
     }
-    LastRegs<kPer> r;
+    LastRegs<kPer, false> r;
     float place[kPer];
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
@@ -860,29 +966,31 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
     };
     int slots = 0;
     for (int i = 0; i < kCoarse / 32; ++i) slots += __popc(s.want[i]);
-    const int F = kFine / slots;
+    const int F = kFine / slots & ~1;  // (a thread's two fine bins are of one collected one)
     if (s.want[tid >> 5] >> (tid & 31) & 1) {
         const int k = rank(tid);
         s.base_cnt[k] = bc;
         s.base_sum[k] = bs;
     }
+    r.no_bins();
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-        r.f[q] = -1;
         if (place[q] < 0.0f) continue;
         const int bin = (int)place[q];
-        r.f[q] = rank(bin) * F + min((int)((place[q] - (float)bin) * (float)F), F - 1);
-        atomicAdd(&s.cnt[r.f[q]], 1u);
-        atomicAdd(&s.sum[r.f[q]], r.w[q]);
+        const int f = rank(bin) * F + min((int)((place[q] - (float)bin) * (float)F), F - 1);
+        r.set_bin(q, f);
+        atomicAdd(&s.cnt[f], 1u);
+        atomicAdd(&s.sum[f], r.w[q]);
     }
     __syncthreads();
-    fine_prefix(r, s);
+    BinPair p;
+    bin_prefix(s.cnt, s.sum, 0, 0, p, s);
     {
         constexpr int E = kFine / kRowThreads;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            s.pcnt[E * tid + e] = r.cb[e];
-            s.psum[E * tid + e] = r.wb[e];
+            s.pcnt[E * tid + e] = p.cb[e];
+            s.psum[E * tid + e] = p.wb[e];
         }
         __syncthreads();
         // From the sum over the collected bins to the one over the row's.
@@ -890,28 +998,32 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
         for (int e = 0; e < E; ++e) {
             const int k = (E * tid + e) / F;
             if (k >= slots) continue;  // (holds nothing)
-            r.cb[e] += s.base_cnt[k] - s.pcnt[k * F];
-            r.wb[e] += s.base_sum[k] - s.psum[k * F];
+            p.cb[e] += s.base_cnt[k] - s.pcnt[k * F];
+            p.wb[e] += s.base_sum[k] - s.psum[k * F];
         }
     }
-    return finish(a, b, rp, r, rr.m, Z, Sm, cut, s);
+    __syncthreads();
+    s.base_cnt[tid] = p.cb[0];
+    s.base_sum[tid] = p.wb[0];
+    finish(a, b, rp, r, rr.m, Z, Sm, cut, s);
+    return true;
 }
 
 // A row by one workgroup, PER logits of it in each thread's registers: the fine
 // histogram over the whole range at once. One launch, bound by its chain of barriers:
 // 4096 logits with cuts 13 us (sample_row 44), 16384 21 (the four launches above 24),
-// 256 such rows 24 (48). False where a bin holds too many.
+// 256 such rows 24 (48).
 template <int PER>
-__device__ __forceinline__ bool sample_small(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
+__device__ __forceinline__ void sample_small(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* row = a.logits + b * a.ld;
-    LastRegs<PER> r;
+    LastRegs<PER, true> r;
+    r.i[0] = tid;
     float m = -__builtin_inff(), lo = __builtin_inff();
     int at = 0x7FFFFFFF;
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
         const int i = tid + q * kRowThreads;
-        r.i[q] = i;
         r.l[q] = i < a.V ? row[i] : -__builtin_inff();
         if (i < a.V && ahead(r.l[q], i, m, at)) m = r.l[q], at = i;
         if (r.l[q] > -__builtin_inff()) lo = fminf(lo, r.l[q]);
@@ -939,27 +1051,28 @@ __device__ __forceinline__ bool sample_small(const SampleArgs& a, int b, const R
             a.token[b] = none ? -1 : at;
             if (a.prob) a.prob[b] = m != m ? m : (none ? 0.0f : 1.0f);
         }
-        return true;
+        return;
     }
     const double scale = __builtin_ldexp(1.0, a.shift);
     const float end = weightless(a);
     const float bins = (float)kFine / fmaxf(fminf((float)(((double)m - (double)lo) * rp.inv_t), end), 1e-30f);
     uint64_t Z = 0, Sm = 0;
     uint32_t all = 0;
+    r.no_bins();
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
         const double x = r.l[q] == m ? 0.0 : ((double)m - (double)r.l[q]) * rp.inv_t;
-        r.f[q] = -1;
         r.w[q] = 0;
-        if (r.i[q] >= a.V || !(x < end)) continue;
+        if (!(x < end)) continue;
         const double w = exp(-x);
         r.w[q] = fixed(w, scale);
-        r.f[q] = min((int)((float)x * bins), kFine - 1);
+        const int f = min((int)((float)x * bins), kFine - 1);
+        r.set_bin(q, f);
         Z += r.w[q];
         if (w >= rp.minp) Sm += r.w[q];
         ++all;
-        atomicAdd(&s.cnt[r.f[q]], 1u);
-        atomicAdd(&s.sum[r.f[q]], r.w[q]);
+        atomicAdd(&s.cnt[f], 1u);
+        atomicAdd(&s.sum[f], r.w[q]);
     }
     for (int o = 32; o; o >>= 1) {
         Z += __shfl_xor((unsigned long long)Z, o);
@@ -967,21 +1080,21 @@ __device__ __forceinline__ bool sample_small(const SampleArgs& a, int b, const R
         all += __shfl_xor(all, o);
     }
     __syncthreads();  // and every wave has read el
-    if (lane == 0) s.base_sum[wave] = Z, s.base_sum[64 + wave] = Sm, s.base_cnt[wave] = all;
-    fine_prefix(r, s);
+    if (lane == 0) s.psum[wave] = Z, s.psum[64 + wave] = Sm, s.pcnt[wave] = all;
+    BinPair p;
+    bin_prefix(s.cnt, s.sum, 0, 0, p, s);
+    s.base_cnt[tid] = p.cb[0];
+    s.base_sum[tid] = p.wb[0];
     Z = Sm = 0;
     all = 0;
-    for (int i = 0; i < kRowThreads / 64; ++i) Z += s.base_sum[i], Sm += s.base_sum[64 + i], all += s.base_cnt[i];
-    return finish(a, b, rp, r, m, Z, Sm, (uint32_t)rp.topk < all, s);
+    for (int i = 0; i < kRowThreads / 64; ++i) Z += s.psum[i], Sm += s.psum[64 + i], all += s.pcnt[i];
+    finish(a, b, rp, r, m, Z, Sm, (uint32_t)rp.topk < all, s);
 }
 template <int PER>
 __global__ void __launch_bounds__(kRowThreads) sample_small_kernel(SampleArgs a) {
-    __shared__ SampleShared sh;
+    __shared__ LastShared sh;
     const int b = blockIdx.x;
-    const RowParams rp = row_params(a, b);
-    if (sample_small<PER>(a, b, rp, sh.last)) return;
-    __syncthreads();
-    sample_row(a, b, rp, sh.row);
+    sample_small<PER>(a, b, row_params(a, b), sh);
 }
 
 // One workgroup per row: the token.

@@ -224,3 +224,55 @@ def test_sizes_around_the_variants_ends(dev, V):
     check(dev, x, u, temperature=0.7, top_k=[0, 50, 0, 700, 0, 3], top_p=[0.95, 1.0, 0.6, 0.9, 0.999999, 0.5],
           min_p=[0.0, 0.0, 0.05, 0.0, 0.0, 0.2])
     check(dev, x, u)
+
+
+def bf16_rounded(B, V, seed, std=2.0):
+    """Logits as a bf16 product leaves them: hundreds of each value."""
+    return normal(B, V, seed, std).bfloat16().float()
+
+
+@pytest.mark.parametrize("V", [4000, 16384, 32000, 128256, 262144])
+def test_logits_that_were_bf16(dev, V):
+    for seed, std in ((1, 1.0), (2, 2.5)):
+        x = bf16_rounded(5, V, seed, std)
+        for kw in ({}, dict(top_p=0.92), dict(top_k=V // 3), dict(temperature=2.0, top_k=V // 6, top_p=0.95),
+                   dict(min_p=0.01, top_p=0.99, temperature=0.8)):
+            check(dev, x, [0.0, 0.2, 0.55, 0.9, 0.9999], **kw)
+
+
+def test_neighbouring_logits_of_which_each_is_held_by_many(dev):
+    """Runs of equal logits a last bit apart, around zero and the type's smallest among them."""
+    V = 49998
+    x = torch.full((4, V), -9.0)
+    x[0, ::2] = (1.0 + torch.arange(V // 2).remainder(5).float() * 2.0 ** -23)
+    x[1, 1::3] = torch.arange(V // 3).remainder(7).float() * 2.0 ** -149
+    x[1, 2::3] = -torch.arange(V // 3).remainder(3).float() * 2.0 ** -149
+    x[2] = (torch.arange(V) * 7919 % V).remainder(300).float() * 2.0 ** -12
+    x[3, :4000] = 2.0
+    x[3, 4000:] = 2.0 - torch.arange(V - 4000).remainder(200).float() * 2.0 ** -10
+    for kw in ({}, dict(top_p=0.7), dict(top_k=4001), dict(top_k=20000, top_p=0.6, min_p=0.3)):
+        for u in (0.0, 0.35, 0.8, 0.9999):
+            check(dev, x, [u] * 4, **kw)
+
+
+@pytest.mark.parametrize("V,B", [(16384, 256), (262144, 1), (128256, 48)])
+def test_ties_cost_no_second_way(dev, V, B):
+    """A row of tied logits takes the launches of any other (and, at the crossings, two or three rounds of a
+    histogram in shared memory): less than three times its time, not the twenty of a row read again by one workgroup."""
+    import alveare_amd as aa
+
+    def us(x):
+        u = torch.full((B,), 0.7, device=dev)
+        best = math.inf
+        for turn in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                aa.sample(x, u, top_p=0.92)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b)) if turn else best
+        return best * 100
+
+    free, tied = us(normal(B, V, 1, 2.0).to(dev)), us(bf16_rounded(B, V, 1).to(dev))
+    assert tied < 3 * free, (free, tied)
