@@ -88,173 +88,6 @@ __device__ __forceinline__ uint64_t topp_target(double p, uint64_t S) { return m
 __device__ __forceinline__ uint64_t draw_target(double u, uint64_t Z) { return min((uint64_t)(u * (double)Z), Z - 1); }
 
 constexpr int kRowThreads = 1024;
-constexpr int kBins = 2048;
-
-struct RowShared {
-    uint32_t cnt[kBins];
-    unsigned long long sum[kBins];
-    unsigned long long wsum[kRowThreads / 64];
-    uint32_t wcnt[kRowThreads / 64];
-    float wmax[kRowThreads / 64];
-    int widx[kRowThreads / 64];
-    uint32_t bin;
-    uint32_t before_cnt;
-    unsigned long long before_sum;
-};
-
-struct Pick {
-    uint32_t key;       // the crossing value's
-    uint32_t cnt;       // tokens before the first that has it
-    uint64_t sum;       // their weight
-};
-
-// The value at which the running count (by_count) or weight crosses: the one r
-// with before_r <= x < before_r + own. Three passes of 11, 11 and 10 bits.
-__device__ Pick pick(const float* l, int V, float m, double inv_t, double scale, bool by_count, uint64_t x, RowShared& s) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    Pick p{0, 0, 0};
-    uint32_t mask = 0;
-    for (int level = 0; level < 3; ++level) {
-        const int sh = level == 0 ? 21 : (level == 1 ? 10 : 0);
-        const uint32_t bits = level == 2 ? 0x3FFu : 0x7FFu;
-        for (int i = tid; i < kBins; i += kRowThreads) {
-            s.cnt[i] = 0;
-            s.sum[i] = 0;
-        }
-        __syncthreads();
-        for (int i = tid; i < V; i += kRowThreads) {
-            const uint32_t k = key_of(l[i]);
-            if ((k & mask) != p.key) continue;
-            const uint32_t bin = bits - ((k >> sh) & bits);  // descending
-            atomicAdd(&s.cnt[bin], 1u);
-            atomicAdd(&s.sum[bin], (unsigned long long)fixed(weight(l[i], m, inv_t), scale));
-        }
-        __syncthreads();
-        // Each thread two bins: the exclusive prefix before them.
-        const uint32_t c0 = s.cnt[2 * tid], c1 = s.cnt[2 * tid + 1];
-        const uint64_t w0 = s.sum[2 * tid], w1 = s.sum[2 * tid + 1];
-        uint32_t c = c0 + c1;
-        uint64_t w = w0 + w1;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t cu = __shfl_up(c, o);
-            const uint64_t wu = __shfl_up((unsigned long long)w, o);
-            if (lane >= o) c += cu, w += wu;
-        }
-        if (lane == 63) s.wcnt[wave] = c, s.wsum[wave] = w;
-        __syncthreads();
-        uint32_t cb = p.cnt + c - c0 - c1;
-        uint64_t wb = p.sum + w - w0 - w1;
-        for (int i = 0; i < wave; ++i) cb += s.wcnt[i], wb += s.wsum[i];
-        const uint64_t b0 = by_count ? cb : wb, i0 = by_count ? c0 : w0, i1 = by_count ? c1 : w1;
-        if (b0 <= x && x < b0 + i0) s.bin = 2 * tid, s.before_cnt = cb, s.before_sum = wb;
-        if (b0 + i0 <= x && x < b0 + i0 + i1) s.bin = 2 * tid + 1, s.before_cnt = cb + c0, s.before_sum = wb + w0;
-        __syncthreads();
-        p.key |= (bits - s.bin) << sh;
-        p.cnt = s.before_cnt;
-        p.sum = s.before_sum;
-        mask |= bits << sh;
-        __syncthreads();
-    }
-    return p;
-}
-
-// A row by one workgroup from the logits alone, whatever their values.
-__device__ void sample_row(const SampleArgs& a, int b, const RowParams& rp, RowShared& s) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float* l = a.logits + b * a.ld;
-    // The largest logit and its first index; a NaN counts as largest.
-    float m = -__builtin_inff();
-    int mi = a.V;
-    for (int i = tid; i < a.V; i += kRowThreads) {
-        const float v = l[i];
-        if (mi == a.V || v > m || (v != v && m == m)) m = v, mi = i;
-    }
-    for (int o = 32; o; o >>= 1) {
-        const float v = __shfl_xor(m, o);
-        const int vi = __shfl_xor(mi, o);
-        const bool nan = v != v, mnan = m != m;
-        if (nan != mnan ? nan : (v > m || ((v == m || nan) && vi < mi))) m = v, mi = vi;
-    }
-    if (lane == 0) s.wmax[wave] = m, s.widx[wave] = mi;
-    __syncthreads();
-    m = s.wmax[0], mi = s.widx[0];
-    for (int i = 1; i < kRowThreads / 64; ++i) {
-        const float v = s.wmax[i];
-        const int vi = s.widx[i];
-        const bool nan = v != v, mnan = m != m;
-        if (vi < a.V && (nan != mnan ? nan : (v > m || ((v == m || nan) && vi < mi)))) m = v, mi = vi;
-    }
-    if (m != m || m == -__builtin_inff() || rp.topk == 1) {
-        if (tid == 0) {
-            a.token[b] = m == -__builtin_inff() ? -1 : mi;
-            if (a.prob) a.prob[b] = m != m ? m : (m == -__builtin_inff() ? 0.0f : 1.0f);
-        }
-        return;
-    }
-    const double scale = __builtin_ldexp(1.0, a.shift);
-    // The whole row's weight, and that of the tokens min-p keeps.
-    uint64_t S = 0, Sm = 0;
-    for (int i = tid; i < a.V; i += kRowThreads) {
-        const double w = weight(l[i], m, rp.inv_t);
-        const uint64_t f = fixed(w, scale);
-        S += f;
-        if (w >= rp.minp) Sm += f;
-    }
-    for (int o = 32; o; o >>= 1) {
-        S += __shfl_xor((unsigned long long)S, o);
-        Sm += __shfl_xor((unsigned long long)Sm, o);
-    }
-    __syncthreads();
-    if (lane == 0) s.wsum[wave] = S, s.sum[wave] = Sm;
-    __syncthreads();
-    S = Sm = 0;
-    for (int i = 0; i < kRowThreads / 64; ++i) S += s.wsum[i], Sm += s.sum[i];
-    __syncthreads();
-    uint64_t Z = S;
-    auto own_weight = [&](uint32_t key) { return fixed(weight(logit_of(key), m, rp.inv_t), scale); };
-    Pick p{};
-    uint64_t x = 0;
-#pragma unroll 1
-    for (int step = 0; step < 3; ++step) {  // top-k, top-p, the draw
-        if (step == 0) {
-            if (rp.topk >= a.V) continue;
-            x = (uint64_t)rp.topk - 1;
-        } else if (step == 1) {
-            const uint64_t target = topp_target(rp.topp, Z);
-            if (rp.topp >= 1.0 || target >= Z) continue;
-            x = target - 1;
-        } else {
-            Z = min(Z, Sm);
-            x = draw_target(rp.u, Z);
-        }
-        p = pick(l, a.V, m, rp.inv_t, scale, step == 0, x, s);
-        const uint64_t w = own_weight(p.key);
-        if (step == 0) Z = p.sum + (uint64_t)(rp.topk - (int)p.cnt) * w;
-        if (step == 1) Z = min(Z, p.sum + ((x - p.sum) / w + 1) * w);
-    }
-    const uint64_t w = own_weight(p.key);
-    int skip = (int)((x - p.sum) / w);  // equal logits ahead of the token, by index
-    // The token: the skip-th with that value.
-    for (int i0 = 0; i0 < a.V; i0 += kRowThreads) {
-        const int i = i0 + tid;
-        const bool is = i < a.V && key_of(l[i]) == p.key;
-        const uint64_t bal = __ballot(is);
-        if (lane == 0) s.wcnt[wave] = __popcll(bal);
-        __syncthreads();
-        int before = 0, total = 0;
-        for (int q = 0; q < kRowThreads / 64; ++q) {
-            if (q < wave) before += s.wcnt[q];
-            total += s.wcnt[q];
-        }
-        if (is && before + __popcll(bal & ((1ull << lane) - 1)) == skip) {
-            a.token[b] = i;
-            if (a.prob) a.prob[b] = (float)(weight(l[i], m, rp.inv_t) / ((double)Z / scale));
-        }
-        __syncthreads();
-        if (skip < total) break;
-        skip -= total;
-    }
-}
 
 // ---- several workgroups per row -----------------------------------------------------
 //
@@ -264,7 +97,7 @@ __device__ void sample_row(const SampleArgs& a, int b, const RowParams& rp, RowS
 // collection of those bins' tokens; the crossings among those, by comparison
 // where they are few, else by a finer histogram first. Every step moves integers,
 // so no order of atomics shows. A row whose bins hold more than kCand tokens (thousands
-// of one value, or more than a million logits) is done by sample_row.
+// of one value, or more than a million logits) is left to one workgroup (sample_over).
 //
 // What bounds it: one row is a chain of launches, each a trip or two to memory (one
 // row of 262144: 25 us, of them 4 + 8 + 9 + 4 in the kernels); many rows, the
@@ -392,7 +225,7 @@ __device__ __forceinline__ float weightless(const SampleArgs& a) { return (float
 
 // What a row's largest and smallest logits decide.
 struct RowRange {
-    float m;
+    float m, low;   // the largest, and the smallest above -infinity
     int at;
     bool done;      // the token is `at` (or there is none)
     float bins;     // bins per unit of x
@@ -413,6 +246,7 @@ __device__ __forceinline__ RowRange row_range(const SampleArgs& a, const RowWork
     }
     RowRange r;
     r.m = m;
+    r.low = lo;
     r.at = at;
     r.done = m != m || m == -__builtin_inff() || rp.topk == 1;
     r.end = weightless(a);
@@ -609,12 +443,20 @@ __global__ void __launch_bounds__(kPieceThreads) sample_collect_kernel(SampleArg
 }
 
 constexpr int kPer = kCand / kRowThreads;  // collected tokens of a thread
+constexpr int kLine = 256;
 struct LastShared {
-    // the collected bins, each cut into kFine / (their number) fine ones
-    uint32_t cnt[kFine], pcnt[kFine];
-    unsigned long long sum[kFine], psum[kFine];
-    uint32_t base_cnt[kCoarse];            // by collected bin: what comes before it
-    unsigned long long base_sum[kCoarse];
+    union {
+        struct {
+            // the collected bins, each cut into kFine / (their number) fine ones
+            uint32_t cnt[kFine];
+            unsigned long long sum[kFine];
+            uint32_t base_cnt[kCoarse];            // by collected bin: what comes before it
+            unsigned long long base_sum[kCoarse];
+        };
+        unsigned long long line[kRowThreads / 64][kLine];  // or the waves' tokens found in a row (OfRow)
+    };
+    uint32_t pcnt[kFine];
+    unsigned long long psum[kFine];
     uint32_t want[kCoarse / 32];
     unsigned long long wsum[kRowThreads / 64];
     uint32_t wcnt[kRowThreads / 64];
@@ -625,15 +467,11 @@ struct LastShared {
     int ne, f;
     uint32_t before_cnt;
     unsigned long long before_sum;
-    unsigned long long lo, hi;  // the first and last of its places in the order
+    unsigned long long lo, hi;  // the first and last of their places in the order
     // the token found, and the weight up to and with it
     float rl;
     int ri;
     unsigned long long through;
-};
-union SampleShared {
-    RowShared row;
-    LastShared last;
 };
 
 // A thread's two bins: counts and weights (c, ws), and what comes before them (cb, wb).
@@ -718,36 +556,98 @@ __device__ __forceinline__ uint64_t place_in_order(float l, int i, int shift) {
     return (uint64_t)~key_of(l) << (62 - shift) | (uint32_t)i;
 }
 
-// The tokens of fine bin f (logits that differ in their last bits, or not at all: those rounded to bf16 have
-// hundreds of each value) cut to at most kLast around the crossing: their places [lo, hi] into kFine equal parts,
-// until the one that holds it has no more. Places differ by one at least, so that ends; two or three times for a
-// bin of a few values. A row of 262144 logits with top-p, rounded to bf16 41 us (not rounded 34; by one workgroup
-// from the logits, which tied bins went to once, 700).
+// The collected tokens of fine bin f whose places are in [lo, hi].
 template <int PER, bool LINE>
-__device__ __forceinline__ void narrow(const LastRegs<PER, LINE>& r, int shift, bool by_count, uint64_t x, int f, uint64_t& lo,
-                                       uint64_t& hi, LastShared& s) {
-    const int tid = threadIdx.x;
-    unsigned long long first = ~0ull, last = 0;
+struct OfBin {
+    static constexpr bool kAlike = false;
+    const LastRegs<PER, LINE>& r;
+    int f, shift;
+    template <class F>
+    __device__ __forceinline__ void operator()(uint64_t lo, uint64_t hi, F each) const {
 #pragma unroll
-    for (int q = 0; q < PER; ++q) {
-        if (r.bin(q) != f) continue;
-        const unsigned long long c = place_in_order(r.l[q], r.index(q), shift);
-        first = min(first, c);
-        last = max(last, c);
+        for (int q = 0; q < PER; ++q) {
+            if (r.bin(q) != f) continue;
+            const uint64_t c = place_in_order(r.l[q], r.index(q), shift);
+            if (c >= lo && c <= hi) each(c, r.l[q], r.index(q), r.w[q]);
+        }
     }
-    for (int o = 32; o; o >>= 1) {
-        first = min(first, __shfl_xor(first, o));
-        last = max(last, __shfl_xor(last, o));
+};
+
+// The row's tokens whose places are in [lo, hi], from the logits: a wave lines up those it finds and takes them 64 at
+// a time, so that the exponential runs once for 64 tokens however few of the row they are, and not for a value it has.
+struct OfRow {
+    static constexpr bool kAlike = true;  // (a run of one value: 64 tokens of one bin, one after the other in an atomic)
+    static constexpr int kTurns = 4, kAtOnce = 3;
+    static_assert(64 * kAtOnce + 63 <= kLine, "what a turn finds, beside what is left");
+    const float* l;
+    int V, shift;
+    float m;
+    double inv_t;
+    unsigned long long (*line)[kLine];
+    template <class F>
+    __device__ __forceinline__ void operator()(uint64_t lo, uint64_t hi, F each) const {
+        const int tid = threadIdx.x, lane = tid & 63, bits = 62 - shift;
+        const double scale = __builtin_ldexp(1.0, shift);
+        const float top = logit_of(~(uint32_t)(lo >> bits)), least = logit_of(~(uint32_t)(hi >> bits));
+        unsigned long long* q = line[tid >> 6];
+        int i0 = 0, i1 = V, n = 0;
+        if (lo >> bits == hi >> bits) {  // one value: of these indices
+            i0 = (int)(lo & ((1u << bits) - 1));
+            i1 = min(V, (int)(hi & ((1u << bits) - 1)) + 1);
+        }
+        float had = __builtin_nanf("");
+        uint64_t its = 0;
+        // (the last k first: nothing moves)
+        auto take = [&](int k) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            n -= k;
+            if (lane < k) {
+                const uint64_t e = q[n + lane];
+                const float v = __builtin_bit_cast(float, (uint32_t)e);
+                if (v != had) had = v, its = fixed(weight(v, m, inv_t), scale);
+                const uint64_t c = place_in_order(v, (int)(e >> 32), shift);
+                if (c >= lo && c <= hi) each(c, v, (int)(e >> 32), its);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        };
+        constexpr int kAhead = kTurns * kAtOnce;
+        for (int base = i0; base < i1; base += kAhead * kRowThreads) {
+            float v[kAhead];
+#pragma unroll
+            for (int e = 0; e < kAhead; ++e) {
+                const int i = base + e * kRowThreads + tid;
+                v[e] = i < i1 ? l[i] : -__builtin_inff();  // (no place: m - infinity weighs nothing)
+            }
+#pragma unroll 1
+            for (int t = 0; t < kTurns; ++t) {
+#pragma unroll
+                for (int e = 0; e < kAtOnce; ++e) {
+                    const float ve = v[e];
+                    const int i = base + (t * kAtOnce + e) * kRowThreads + tid;
+                    const bool is = ve >= least && ve <= top;
+                    const uint64_t found = __ballot(is);
+                    if (is) q[n + __popcll(found & ((1ull << lane) - 1))] = (uint64_t)i << 32 | __builtin_bit_cast(uint32_t, ve);
+                    n += __popcll(found);
+                }
+#pragma unroll
+                for (int e = 0; e + kAtOnce < kAhead; ++e) v[e] = v[e + kAtOnce];
+#pragma unroll 1
+                while (n >= 64) take(64);
+            }
+        }
+        take(n);
     }
-    if ((tid & 63) == 0) {
-        atomicMin(&s.lo, first);
-        atomicMax(&s.hi, last);
-    }
-    __syncthreads();
-    lo = s.lo;
-    hi = s.hi;
-    uint32_t n;
-    do {
+};
+
+// n tokens with places in [lo, hi] cut to at most kLast around the crossing: the places into kFine equal parts, until
+// the part that holds it has no more. (Logits that differ in their last bits or not at all: rounded to bf16 there are
+// hundreds of each value.) Places differ by one at least, so that ends. A row of 262144 logits with top-p, rounded to
+// bf16, 41 us (not rounded 34).
+template <class M>
+__device__ __forceinline__ void narrow(uint32_t n, uint64_t& lo, uint64_t& hi, bool by_count, uint64_t x, const M& tokens,
+                                       LastShared& s) {
+    const int tid = threadIdx.x;
+    while (n > kLast) {
         const int sh = max(0, 53 - __clzll(hi - lo));  // (hi - lo) >> sh is less than kFine
         const uint32_t c0 = s.before_cnt;
         const uint64_t w0 = s.before_sum;
@@ -757,14 +657,28 @@ __device__ __forceinline__ void narrow(const LastRegs<PER, LINE>& r, int shift, 
             s.psum[tid + e * kRowThreads] = 0;
         }
         __syncthreads();
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            if (r.bin(q) != f) continue;
-            const uint64_t c = place_in_order(r.l[q], r.index(q), shift);
-            if (c < lo || c > hi) continue;
-            atomicAdd(&s.pcnt[(c - lo) >> sh], 1u);
-            atomicAdd(&s.psum[(c - lo) >> sh], r.w[q]);
-        }
+        tokens(lo, hi, [&](uint64_t c, float, int, uint64_t w) {
+            const uint32_t bin = (uint32_t)((c - lo) >> sh);
+            bool left = true;
+            if constexpr (M::kAlike)
+#pragma unroll 1
+                for (int turn = 0; turn < 4 && __any(left); ++turn)
+                    if (left) {
+                        const uint32_t bin0 = __builtin_amdgcn_readfirstlane(bin);
+                        const uint32_t w_lo = __builtin_amdgcn_readfirstlane((uint32_t)w);
+                        const uint32_t w_hi = __builtin_amdgcn_readfirstlane((uint32_t)(w >> 32));
+                        const bool alike = bin == bin0 && w == ((uint64_t)w_hi << 32 | w_lo);
+                        const uint64_t same = __ballot(alike);
+                        if (alike && (tid & 63) == __builtin_ctzll(same)) {
+                            atomicAdd(&s.pcnt[bin], (uint32_t)__popcll(same));
+                            atomicAdd(&s.psum[bin], (unsigned long long)(w * __popcll(same)));
+                        }
+                        left = !alike;
+                    }
+            if (!left) return;
+            atomicAdd(&s.pcnt[bin], 1u);
+            atomicAdd(&s.psum[bin], (unsigned long long)w);
+        });
         __syncthreads();
         BinPair p;
         bin_prefix(s.pcnt, s.psum, c0, w0, p, s);
@@ -774,42 +688,19 @@ __device__ __forceinline__ void narrow(const LastRegs<PER, LINE>& r, int shift, 
         lo += (uint64_t)s.f << sh;
         hi = min(hi, lo + ((1ull << sh) - 1));
         __syncthreads();
-    } while (n > kLast);
+    }
 }
 
-// The token at which the running count or weight crosses x.
-template <int PER, bool LINE>
-__device__ __forceinline__ void cross(const LastRegs<PER, LINE>& r, int shift, bool by_count, uint64_t x, LastShared& s) {
+// The token at which the running count or weight crosses x, by comparison of the few in [lo, hi].
+template <class M>
+__device__ __forceinline__ void pick(uint64_t lo, uint64_t hi, bool by_count, uint64_t x, const M& tokens, LastShared& s) {
     const int tid = threadIdx.x;
-    BinPair p;
-#pragma unroll
-    for (int e = 0; e < kFine / kRowThreads; ++e) {
-        const int i = tid * (kFine / kRowThreads) + e;
-        p.c[e] = s.cnt[i];
-        p.ws[e] = s.sum[i];
-        p.cb[e] = e ? p.cb[e - 1] + p.c[e - 1] : s.base_cnt[tid];
-        p.wb[e] = e ? p.wb[e - 1] + p.ws[e - 1] : s.base_sum[tid];
-    }
-    find_bin(p, by_count, x, s);
-    if (tid == 0) {
-        s.ne = 0;
-        s.lo = ~0ull;
-        s.hi = 0;
-    }
-    __syncthreads();
-    const int f = s.f;
-    uint64_t lo = 0, hi = ~0ull;
-    if (s.cnt[f] > kLast) narrow(r, shift, by_count, x, f, lo, hi, s);
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-        if (r.bin(q) != f) continue;
-        const uint64_t c = place_in_order(r.l[q], r.index(q), shift);
-        if (c < lo || c > hi) continue;
+    tokens(lo, hi, [&](uint64_t, float l, int i, uint64_t w) {
         const int e = atomicAdd(&s.ne, 1);
-        s.el[e] = r.l[q];
-        s.ei[e] = r.index(q);
-        s.ew[e] = r.w[q];
-    }
+        s.el[e] = l;
+        s.ei[e] = i;
+        s.ew[e] = w;
+    });
     __syncthreads();
     const int ne = s.ne;
     if (tid < ne) {
@@ -831,11 +722,56 @@ __device__ __forceinline__ void cross(const LastRegs<PER, LINE>& r, int shift, b
     __syncthreads();
 }
 
-// The three crossings and the token. Z: the weight of all (cut: of which top-k
-// leaves some out), Sm of what min-p keeps.
+// The same among the collected tokens.
 template <int PER, bool LINE>
-__device__ __forceinline__ void finish(const SampleArgs& a, int b, const RowParams& rp, const LastRegs<PER, LINE>& r, float m,
-                                       uint64_t Z, uint64_t Sm, bool cut, LastShared& s) {
+__device__ __forceinline__ void cross(const LastRegs<PER, LINE>& r, int shift, bool by_count, uint64_t x, LastShared& s) {
+    const int tid = threadIdx.x;
+    BinPair p;
+#pragma unroll
+    for (int e = 0; e < kFine / kRowThreads; ++e) {
+        const int i = tid * (kFine / kRowThreads) + e;
+        p.c[e] = s.cnt[i];
+        p.ws[e] = s.sum[i];
+        p.cb[e] = e ? p.cb[e - 1] + p.c[e - 1] : s.base_cnt[tid];
+        p.wb[e] = e ? p.wb[e - 1] + p.ws[e - 1] : s.base_sum[tid];
+    }
+    find_bin(p, by_count, x, s);
+    if (tid == 0) {
+        s.ne = 0;
+        s.lo = ~0ull;
+        s.hi = 0;
+    }
+    __syncthreads();
+    const int f = s.f;
+    const OfBin<PER, LINE> tokens{r, f, shift};
+    uint64_t lo = 0, hi = ~0ull;
+    if (s.cnt[f] > kLast) {
+        unsigned long long first = ~0ull, last = 0;
+        tokens(lo, hi, [&](uint64_t c, float, int, uint64_t) {
+            first = min(first, (unsigned long long)c);
+            last = max(last, (unsigned long long)c);
+        });
+        for (int o = 32; o; o >>= 1) {
+            first = min(first, __shfl_xor(first, o));
+            last = max(last, __shfl_xor(last, o));
+        }
+        if ((tid & 63) == 0) {
+            atomicMin(&s.lo, first);
+            atomicMax(&s.hi, last);
+        }
+        __syncthreads();
+        lo = s.lo;
+        hi = s.hi;
+        narrow(s.cnt[f], lo, hi, by_count, x, tokens, s);
+    }
+    pick(lo, hi, by_count, x, tokens, s);
+}
+
+// The three crossings and the token. Z: the weight of all (cut: of which top-k
+// leaves some out), Sm of what min-p keeps; at(by_count, x) finds a crossing.
+template <class At>
+__device__ __forceinline__ void finish(const SampleArgs& a, int b, const RowParams& rp, float m, uint64_t Z, uint64_t Sm,
+                                       bool cut, At at, LastShared& s) {
     const int tid = threadIdx.x;
     const double scale = __builtin_ldexp(1.0, a.shift);
 #pragma unroll 1
@@ -852,7 +788,7 @@ __device__ __forceinline__ void finish(const SampleArgs& a, int b, const RowPara
             Z = min(Z, Sm);
             x = draw_target(rp.u, Z);
         }
-        cross(r, a.shift, step == 0, x, s);
+        at(step == 0, x);
         if (step < 2) Z = min(Z, (uint64_t)s.through);
     }
     if (tid == 0) {
@@ -861,8 +797,48 @@ __device__ __forceinline__ void finish(const SampleArgs& a, int b, const RowPara
     }
 }
 
-// The token from what was collected; false where that is too much.
-__device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
+// A row of which more than kCand tokens are in the bins of the crossings (thousands of one value, or more than a
+// million logits), by one workgroup: the bins' prefix says in which bin a crossing is and a search over all values
+// from which to which logit that reaches; then parts of it as above, each a pass over the row, 20 to 60 us a pass of
+// 262144. With top-p, 262144 logits rounded to quarters 206 us, all alike 372; 48 rows of 128256, 172 and 255.
+__device__ __forceinline__ void sample_over(const SampleArgs& a, int b, const RowParams& rp, const RowWork& rw,
+                                            const RowRange& rr, uint64_t Z, uint64_t Sm, bool cut, LastShared& s) {
+    static_assert(kCoarse == kRowThreads, "a bin per thread");
+    const int tid = threadIdx.x, bits = 62 - a.shift;
+    const uint32_t* cnt = rw.cnt + kCoarse;
+    const unsigned long long* sum = rw.sum + kCoarse;
+    const OfRow tokens{a.logits + b * a.ld, a.V, a.shift, rr.m, rp.inv_t, s.line};
+    // The largest key of bin f or a later one (the row's own from f = 0 on).
+    auto edge = [&](int f) {
+        uint32_t in = key_of(-__builtin_inff()), out = key_of(rr.m);
+        if (f == 0) return out;
+        while (out - in > 1) {
+            const uint32_t k = in + (out - in) / 2;
+            const double x = x_of(logit_of(k), rr, rp.inv_t);
+            if (!(x < rr.end) || (int)place_of(x, rr) >= f)
+                in = k;
+            else
+                out = k;
+        }
+        return in;
+    };
+    finish(a, b, rp, rr.m, Z, Sm, cut, [&](bool by_count, uint64_t x) {
+        const uint64_t b0 = by_count ? cnt[tid] : sum[tid], b1 = by_count ? cnt[tid + 1] : sum[tid + 1];
+        if (b0 <= x && x < b1) s.f = tid, s.before_cnt = cnt[tid], s.before_sum = sum[tid];
+        if (tid == 0) s.ne = 0;
+        __syncthreads();
+        const int f = s.f;
+        const uint32_t e = edge(f + (tid & 1));
+        uint64_t lo = (uint64_t)~(uint32_t)__builtin_amdgcn_readlane((int)e, 0) << bits;
+        const uint32_t least = max((uint32_t)__builtin_amdgcn_readlane((int)e, 1) + 1, key_of(rr.low));
+        uint64_t hi = (uint64_t)~least << bits | ((1u << bits) - 1);
+        narrow(cnt[f + 1] - cnt[f], lo, hi, by_count, x, tokens, s);
+        pick(lo, hi, by_count, x, tokens, s);
+    }, s);
+}
+
+// The token from what was collected.
+__device__ __forceinline__ void sample_collected(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
     const int tid = threadIdx.x, lane = tid & 63;
     const RowWork rw = row_work(a, b);
     const RowRange rr = row_range(a, rw, rp, lane);
@@ -872,16 +848,16 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
             a.token[b] = none ? -1 : rr.at;
             if (a.prob) a.prob[b] = rr.m != rr.m ? rr.m : (none ? 0.0f : 1.0f);
         }
-        return true;
+        return;
     }
     const uint32_t n = *rw.n, over = *rw.over;
     const uint32_t all = rw.cnt[2 * kCoarse];
     uint64_t Z = rw.sum[2 * kCoarse], Sm = 0;
     for (int g = lane; g < a.pieces; g += 64) Sm += rw.minp[g];
-    if (over) return false;
     const double scale = __builtin_ldexp(1.0, a.shift);
     for (int o = 32; o; o >>= 1) Sm += __shfl_xor((unsigned long long)Sm, o);
     const bool cut = (uint32_t)rp.topk < all;
+    if (over) return sample_over(a, b, rp, rw, rr, Z, Sm, cut, s);
     if (n <= kLast) {
         // Few: each token's place among all, hence what comes before it, at once.
         const uint32_t* cnt = rw.cnt + kCoarse;
@@ -933,7 +909,7 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
             a.token[b] = id;
             if (a.prob) a.prob[b] = (float)(weight(l, rr.m, rp.inv_t) / ((double)Z / scale));
         }
-        return true;
+        return;
     }
     LastRegs<kPer, false> r;
     float place[kPer];
@@ -1005,13 +981,12 @@ __device__ __forceinline__ bool sample_collected(const SampleArgs& a, int b, con
     __syncthreads();
     s.base_cnt[tid] = p.cb[0];
     s.base_sum[tid] = p.wb[0];
-    finish(a, b, rp, r, rr.m, Z, Sm, cut, s);
-    return true;
+    finish(a, b, rp, rr.m, Z, Sm, cut, [&](bool by_count, uint64_t x) { cross(r, a.shift, by_count, x, s); }, s);
 }
 
 // A row by one workgroup, PER logits of it in each thread's registers: the fine
 // histogram over the whole range at once. One launch, bound by its chain of barriers:
-// 4096 logits with cuts 13 us (sample_row 44), 16384 21 (the four launches above 24),
+// 4096 logits with cuts 13 us, 16384 21 (the four launches above 24),
 // 256 such rows 24 (48).
 template <int PER>
 __device__ __forceinline__ void sample_small(const SampleArgs& a, int b, const RowParams& rp, LastShared& s) {
@@ -1088,7 +1063,7 @@ __device__ __forceinline__ void sample_small(const SampleArgs& a, int b, const R
     Z = Sm = 0;
     all = 0;
     for (int i = 0; i < kRowThreads / 64; ++i) Z += s.psum[i], Sm += s.psum[64 + i], all += s.pcnt[i];
-    finish(a, b, rp, r, m, Z, Sm, (uint32_t)rp.topk < all, s);
+    finish(a, b, rp, m, Z, Sm, (uint32_t)rp.topk < all, [&](bool by_count, uint64_t x) { cross(r, a.shift, by_count, x, s); }, s);
 }
 template <int PER>
 __global__ void __launch_bounds__(kRowThreads) sample_small_kernel(SampleArgs a) {
@@ -1099,12 +1074,9 @@ __global__ void __launch_bounds__(kRowThreads) sample_small_kernel(SampleArgs a)
 
 // One workgroup per row: the token.
 __global__ void __launch_bounds__(kRowThreads) sample_last_kernel(SampleArgs a) {
-    __shared__ SampleShared sh;
+    __shared__ LastShared sh;
     const int b = blockIdx.x;
-    const RowParams rp = row_params(a, b);
-    if (sample_collected(a, b, rp, sh.last)) return;
-    __syncthreads();
-    sample_row(a, b, rp, sh.row);
+    sample_collected(a, b, row_params(a, b), sh);
 }
 }  // namespace
 

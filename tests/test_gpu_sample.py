@@ -255,24 +255,46 @@ def test_neighbouring_logits_of_which_each_is_held_by_many(dev):
             check(dev, x, [u] * 4, **kw)
 
 
+def us_with_top_p(dev, x):
+    import alveare_amd as aa
+
+    x, u = x.to(dev), torch.full((x.shape[0],), 0.7, device=dev)
+    best = math.inf
+    for turn in range(6):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(10):
+            aa.sample(x, u, top_p=0.92)
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b)) if turn else best
+    return best * 100
+
+
 @pytest.mark.parametrize("V,B", [(16384, 256), (262144, 1), (128256, 48)])
 def test_ties_cost_no_second_way(dev, V, B):
     """A row of tied logits takes the launches of any other (and, at the crossings, two or three rounds of a
     histogram in shared memory): less than three times its time, not the twenty of a row read again by one workgroup."""
-    import alveare_amd as aa
-
-    def us(x):
-        u = torch.full((B,), 0.7, device=dev)
-        best = math.inf
-        for turn in range(6):
-            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
-            a.record()
-            for _ in range(10):
-                aa.sample(x, u, top_p=0.92)
-            b.record()
-            torch.cuda.synchronize()
-            best = min(best, a.elapsed_time(b)) if turn else best
-        return best * 100
-
-    free, tied = us(normal(B, V, 1, 2.0).to(dev)), us(bf16_rounded(B, V, 1).to(dev))
+    free, tied = us_with_top_p(dev, normal(B, V, 1, 2.0)), us_with_top_p(dev, bf16_rounded(B, V, 1))
     assert tied < 3 * free, (free, tied)
+
+
+@pytest.mark.parametrize("V,B,step,times", [(128256, 48, 0.25, 6), (262144, 1, 0.25, 12), (262144, 1, 1e9, 25)])
+def test_what_thousands_of_ties_cost(dev, V, B, step, times):
+    """One workgroup reads such a row a few times over for each crossing (measured 2.8, 6 and 11 times a row without
+    ties; nine passes of atomics for each were 9, 24 and 82)."""
+    x = normal(B, V, 1, 2.0)
+    free, tied = us_with_top_p(dev, x), us_with_top_p(dev, (x / step).round() * step)
+    assert tied < times * free, (free, tied)
+
+
+@pytest.mark.parametrize("V,step", [(40000, 1.0), (262144, 0.25), (262144, 4.0), (300001, 1e9), (1500000, 0.0), (3000001, 2.0 ** -7)])
+def test_thousands_of_tokens_at_a_border(dev, V, step):
+    """More tokens in the bins of the crossings than are collected: logits of a few values, and very many."""
+    x = normal(3, V, seed=V, std=2.0)
+    x = (x / step).round() * step if step else x
+    x[1, V // 3: V // 2] = -math.inf
+    x[2, ::5] = x[2].max() + 0.5
+    for kw in ({}, dict(top_p=0.9), dict(top_k=V // 2, top_p=0.8, temperature=1.5), dict(top_k=V // 50, min_p=0.2)):
+        for u in (0.0, 0.43, 0.99999):
+            check(dev, x, [u] * 3, **kw)
