@@ -137,9 +137,11 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
     dev = _need_gpu(qkv)
     (pages, kv_heads, S, D), ks, vs, B, W, ldt, T, width, ldqkv = _args(qkv, "qkv", kpages, vpages, page_table, q_start,
                                                                         kv_len, dev)
-    v_off = max(v_off, -1)
-    if max(heads, k_off, v_off) > _INT_MAX or min(heads, k_off, half or 0) < -_INT_MAX:
-        _far(heads=heads, k_off=k_off, v_off=v_off, half=half)
+    if v_off < 0:
+        v_off = -1
+    if not (0 < heads <= _INT_MAX and 0 < k_off <= _INT_MAX and v_off <= _INT_MAX and (half is None or half > 0)):
+        if max(heads, k_off, v_off) > _INT_MAX or min(heads, k_off, half or 0) < -_INT_MAX:
+            _far(heads=heads, k_off=k_off, v_off=v_off, half=half)
     if width < (k_off if v_off < 0 else v_off) + kv_heads * D:
         _narrow("qkv", width, (k_off if v_off < 0 else v_off) + kv_heads * D)
     ldq = heads * D
@@ -181,9 +183,10 @@ def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     ldo = heads * D
     if width < ldo:
         _narrow("q", width, ldo)
-    window, sinks, max_q = min(window, _INT_MAX), min(sinks, _INT_MAX), min(max_q, _INT_MAX)
-    if min(heads, window, sinks, max_q) < -_INT_MAX:
-        _far(heads=heads, window=window, sinks=sinks, max_q=max_q)
+    if not (0 < heads and 0 <= window <= _INT_MAX and 0 <= sinks <= _INT_MAX and 0 <= max_q <= _INT_MAX):
+        window, sinks, max_q = min(window, _INT_MAX), min(sinks, _INT_MAX), min(max_q, _INT_MAX)
+        if min(heads, window, sinks, max_q) < -_INT_MAX:
+            _far(heads=heads, window=window, sinks=sinks, max_q=max_q)
     if out is None:
         out = torch.empty_like(q) if width == ldo == ldq else q.new_empty((T, ldo))
     else:
