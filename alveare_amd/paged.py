@@ -326,15 +326,16 @@ class PagedCache:
                 last = self._table[s][-1]
                 left[last] = left.get(last, self._shared[last]) - 1
                 copied = left[last] > 0  # the last to write keeps the page
-            plan.append((s, m, copied, more))
-            need += copied + more
+            if copied or more:
+                plan.append((self._table[s], copied, more))
+                need += copied + more
         if need > len(self._free):
             raise MemoryError(f"{need} pages needed, {len(self._free)} free")
         taken = [heapq.heappop(self._free) for _ in range(need)]
         src, dst, at = [], [], 0  # (a slot's copy, then the pages it grows by)
-        for s, m, copied, more in plan:
+        for t, copied, more in plan:
             if copied:
-                src.append(self._table[s][-1])
+                src.append(t[-1])
                 dst.append(taken[at])
             at += copied + more
         if src:
@@ -349,12 +350,12 @@ class PagedCache:
         for p in taken:
             self._shared[p] = 1
         at = 0
-        for s, m, copied, more in plan:
-            t = self._table[s]
+        for t, copied, more in plan:
             if copied:
                 t.pop()
             t += taken[at:at + copied + more]
             at += copied + more
+        for s, m in zip(slots, n):
             self._len[s] += m
 
     def fork(self, src: int, dst: int) -> None:
