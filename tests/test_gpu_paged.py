@@ -794,3 +794,29 @@ def test_attention_mostly_padding(dev, D, pad):
     (pad = 100: few enough that it takes the batch alone)."""
     b = R.Batch([1, 2, 0, 1], [300, 2, 40, 1], kv_heads=8, D=D, page=16, dev=dev, extra_rows=pad)
     check_attention(b, 64 if D <= 128 else 8, dev, max_q=0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,D", [(32, 8, 64), (16, 8, 128), (16, 8, 256), (16, 1, 512)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (257, 5)])
+def test_attention_whole_tiles_beside_single_tokens(dev, heads, kv_heads, D, window, sinks):
+    """Tiles enough that none is split, of two chunks, and sequences of one and two rows in the same call."""
+    from alveare_amd import attention_paged
+
+    n, past = [1400, 1, 900, 2], [100, 611, 0, 64]
+    total = [a + b for a, b in zip(n, past)]
+    b = R.Batch(n, total, kv_heads=kv_heads, D=D, page=32, dev=dev)
+    q = rows(b.T, heads * D, dev)
+    scale = 1.5 / math.sqrt(D)
+    for mq in (0, 1400):
+        out = attention_paged(q, *b.args(), heads=heads, window=window, sinks=sinks, scale=scale, max_q=mq)
+        at = 0
+        for s, (m, L) in enumerate(zip(n, total)):
+            for i in sorted({0, 1, 31, 32, 127, 128, 500, 899, m // 2, m - 1}):
+                if i >= m:
+                    continue
+                one = R.Batch([1], [L - m + i + 1], kv_heads=kv_heads, D=D, page=16, dev="cpu")
+                one.k[0], one.v[0] = b.k[s][:L - m + i + 1], b.v[s][:L - m + i + 1]
+                want, tol = R.attention(q[at + i:at + i + 1], one, heads, window, sinks, scale)
+                got = out[at + i].double().cpu().view_as(want[0])
+                assert ((got - want[0]).abs() <= tol[0]).all(), (mq, s, i)
+            at += m
