@@ -51,7 +51,8 @@ struct PostPagedArgs {
 //
 // What bounds it: one token, three dependent trips to memory (the sequence, its
 // page and RoPE row, the stores), 5 us; many, the bytes. 16 + 2 x 8 heads of 256,
-// 4939 tokens: 48 us, 3.4 TB/s (a wave per head and two-byte accesses: 101 us).
+// 4939 tokens: 48 us, 3.4 TB/s (a wave per head and two-byte accesses: 101 us);
+// 42 where the same rows come again and are partly in the last cache.
 constexpr int kPostMaxWaves = 8;
 constexpr int kLeafPad = 8;  // floats: leaves then start eight banks apart
 
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
 
 // A workgroup copies 16 KB of one page of one cache, four 16-byte pieces per
 // thread; pointers and pairs come in the kernel's arguments, so a call is one
-// launch and no transfer. Bound by memory: 450 pages of 64 KB in 64
+// launch and no transfer. Bound by memory: 450 pages of 64 KB in 32
 // caches 370 us, 5.1 TB/s read and written; 6 pages of 64 KB in 24 caches, 4.4 us,
 // by the launch (14 us with the checks of 24 tensors on the host).
 constexpr int kCopyCaches = 128;  // per launch

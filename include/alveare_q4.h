@@ -471,17 +471,20 @@ int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off
 /*
  * out[t, h] = softmax(scale * K q[t, h]) V for every row t of a batch over the
  * positions p <= the row's own that its window holds: all of them, or with
- * window > 0 the last `window` and the first `sinks`. float32 scores and
- * softmax; bf16 out. A row that sees no position (all its pages are missing)
- * gets zeros. K and V of a position that a row does not see do not reach it,
+ * window > 0 the last `window` and the first `sinks`. float32 scores, maxima and
+ * sums; the weights are rounded to bf16 (half a step each, 2^-8 relative) for the
+ * product with V, whose sums are float32; bf16 out. A row that sees no position
+ * (all its pages are missing) gets zeros. K and V of a position that a row does not see do not reach it,
  * whatever they hold. Scores that are all -infinity count as unseen. D one of
  * 64, 128, 256, 512; scale finite, not negative; q, its rows, the pages and
  * their strides 16-byte aligned, out and its rows 8-byte; T * heads at most
  * 2^30; out does not overlap q.
  *
  * max_q: the most rows that any sequence owns, if the caller knows (0: not
- * known). It decides how the work is spread, not what is computed: a value too
- * small costs time. workspace: alv_attention_paged_workspace bytes for the same
+ * known). It decides how the work is spread: a value too small costs time. How it
+ * is spread, by max_q and by the lengths of all sequences of the call, decides in
+ * what order a row's sums are rounded, so its last bits may differ between calls
+ * that differ in those; equal calls give equal bits. workspace: alv_attention_paged_workspace bytes for the same
  * arguments, 16-byte aligned (NULL if that is 0); contents are not kept between
  * calls, and calls that may run at the same time need one each, graph replays
  * included.

@@ -298,3 +298,51 @@ def test_thousands_of_tokens_at_a_border(dev, V, step):
     for kw in ({}, dict(top_p=0.9), dict(top_k=V // 2, top_p=0.8, temperature=1.5), dict(top_k=V // 50, min_p=0.2)):
         for u in (0.0, 0.43, 0.99999):
             check(dev, x, [u] * 3, **kw)
+
+
+@pytest.mark.parametrize("V", [3000, 20000, 262144])
+def test_many_infinities_and_zeros(dev, V):
+    """Infinities, or zeros of both signs, more than a border's tokens are compared or collected."""
+    import alveare_amd as aa
+
+    x = normal(4, V, seed=V)
+    x[0, ::2] = math.inf
+    x[1, V // 3:] = math.inf
+    x[1, :V // 4] = -math.inf
+    x[2, ::2] = 0.0
+    x[2, 1::2] = -0.0
+    x[3, ::2] = -0.0
+    x[3, 1::4] = 0.0
+    for kw in ({}, dict(top_p=0.6), dict(top_k=V // 3)):
+        for u in (0.0, 0.5, 0.97):
+            check(dev, x, [u] * 4, **kw)
+    # An infinite temperature: as 3e38, of which every finite (l - l_0) / T here leaves exp 1 in 64 bits too, and
+    # -infinity 0 (the plain form's own -infinity / infinity is no number).
+    for u in (0.0, 0.5, 0.97):
+        token, prob = aa.sample(x.to(dev), torch.full((4,), u, device=dev), temperature=math.inf, top_k=V - 7, top_p=0.9)
+        for b in range(4):
+            want, p = R.sample(x[b], u, temperature=3e38, top_k=V - 7, top_p=0.9)
+            assert int(token[b]) == want and abs(float(prob[b]) - p) <= p * (2.0 ** -24 + 2.0 ** -35)
+
+
+def test_ties_replayed(dev):
+    """A captured call over rows that change between free, tied and constant ones."""
+    import alveare_amd as aa
+
+    V = 262144
+    x, u = normal(3, V, 1).to(dev), torch.tensor([0.2, 0.6, 0.95], device=dev)
+    aa.sample(x, u, top_p=0.9)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = aa.sample(x, u, top_p=0.9)
+    for seed in range(4):
+        y = normal(3, V, 10 + seed)
+        y[seed % 3] = y[seed % 3].bfloat16().float()
+        y[(seed + 1) % 3] = (y[(seed + 1) % 3] * 4).round() / 4 if seed else 0.25
+        x.copy_(y)
+        g.replay()
+        torch.cuda.synchronize()
+        want = aa.sample(x, u, top_p=0.9)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        for b in range(3):
+            assert int(out[0][b]) == R.sample(y[b], float(u[b]), top_p=0.9)[0]
