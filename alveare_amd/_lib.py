@@ -76,6 +76,16 @@ SIGNATURES: dict[str, tuple] = {
     "alv_attention_paged_workspace": (ctypes.c_uint64, [_i, _i, _i, _i, _i, _i]),
     "alv_attention_paged": (_i, [_vp, _l, _vp, _vp, _l, _l, _i, _i, _vp, _l, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i,
                                  _f, _vp, _l, _vp, ctypes.c_uint64, _vp]),
+    "alv_qkv_post_paged8": (_i, [_vp, _l, _i, _i, _i, _i, _i, _vp, _vp, _i, _i, _i, _f, _vp, _i, _l, _i, _i, _i, _vp, _l,
+                                 _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _l, _l, _vp, _l, _vp, _l, _vp]),
+    "alv_attention_paged8_workspace": (ctypes.c_uint64, [_i, _i, _i, _i, _i, _i]),
+    "alv_attention_paged8": (_i, [_vp, _l, _vp, _vp, _l, _l, _vp, _l, _i, _i, _vp, _l, _i, _vp, _vp, _i, _i, _i, _i, _i, _i,
+                                  _i, _i, _f, _vp, _l, _vp, ctypes.c_uint64, _vp]),
+    "alv_attention_shared_workspace": (ctypes.c_uint64, [_i, _i, _i, _i, _i, _i, _i]),
+    "alv_attention_shared": (_i, [_vp, _l, _vp, _vp, _l, _l, _vp, _l, _i, _i, _vp, _l, _i, _vp, _vp, _i, _i, _i, _vp, _vp,
+                                  _i, _i, _i, _i, _i, _i, _f, _vp, _l, _vp, ctypes.c_uint64, _vp]),
+    "alv_adjust_logits": (_i, [_vp, _l, _vp, _l, _i, _i, _vp, _l, _i, _vp, _vp, _vp, _f, _vp, _f, _vp, _f, _vp, _l, _vp, _l,
+                               _i, _vp, _l, _vp]),
     "alv_copy_pages": (_i, [_vp, _i, _l, _l, _i, _vp, _vp, _i, _vp]),
     "alv_sample_workspace": (ctypes.c_uint64, [_i, _i]),
     "alv_sample": (_i, [_vp, _l, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _vp, _vp, _vp, ctypes.c_uint64, _vp]),

@@ -10,6 +10,9 @@
 // or whose length does not fit its table row, is malformed: its rows get zeros.
 // Rows outside every sequence or past the batch's T are never touched, so any
 // contents of q_start, kv_len and the table stay in bounds.
+//
+// 8-bit pages hold e4m3 codes instead, and scales (page, kv head, slot, [k, v])
+// a biased exponent each: a value is code * 2^(scale - 127).
 #pragma once
 
 #include <stdint.h>
@@ -31,6 +34,14 @@ constexpr int kPageMin = 16, kPageMax = 1024;
 constexpr int kMaxRows = 1 << 22;  // 512 threads a row stay within a launch's 2^32 threads
 
 constexpr int kMaxHeads = 1 << 16;  // a row's offsets stay within 32 bits
+
+// Groups of sequences: group j is the sequences start[j] .. start[j + 1] - 1, whose
+// first len[j] positions (whole pages of them) are those of the group's first one.
+struct PagedGroups {
+    const int32_t* start;  // n + 1
+    const int32_t* len;    // n
+    int n;
+};
 
 inline int page_shift(int page_size) { return 31 - __builtin_clz((unsigned)page_size); }
 
@@ -94,6 +105,36 @@ __device__ __forceinline__ SeqRows find_row(const PagedBatch& a, int t, int lane
         }
     }
     return SeqRows{-1, 0, 0, 0, false};
+}
+
+// The positions that group j (start .. end) shares: whole pages, no more than its
+// first sequence has.
+__device__ __forceinline__ int group_len(const PagedBatch& a, int start, int end, int len) {
+    if (start < 0 || start >= end || end > a.B) return 0;
+    return max(0, min(min(len, a.kv_len[start]), a.max_pos)) >> a.shift << a.shift;
+}
+
+// The positions that sequence b shares with its group, and the group's first
+// sequence (b itself where it is in none), by the whole wave (b uniform).
+__device__ __forceinline__ int find_group(const PagedBatch& a, const PagedGroups& gr, int b, int lane, int* first) {
+    for (int j0 = 0; j0 < gr.n; j0 += 64) {
+        const int j = j0 + lane;
+        int lo = 0, hi = 0, len = 0;
+        if (j < gr.n) {
+            lo = gr.start[j];
+            hi = gr.start[j + 1];
+            len = gr.len[j];
+        }
+        const uint64_t m = __ballot(j < gr.n && lo <= b && b < hi);
+        if (m) {
+            const int l = __builtin_ctzll(m);
+            lo = __builtin_amdgcn_readlane(lo, l);
+            *first = lo;
+            return group_len(a, lo, __builtin_amdgcn_readlane(hi, l), __builtin_amdgcn_readlane(len, l));
+        }
+    }
+    *first = b;
+    return 0;
 }
 
 // The page of position p (0 <= p < max_pos) of sequence b, or -1.

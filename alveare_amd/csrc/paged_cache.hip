@@ -3,6 +3,7 @@
 //   alv_qkv_post_paged  per-head q/k/v norms, RoPE of q and k, insert of k and
 //                       v into their pages, for every new token of a batch
 //                       (alv_qkv_post's arithmetic, bit for bit)
+//   alv_qkv_post_paged8 the same into 8-bit pages
 //   alv_copy_pages      pages copied within each of many caches
 #include <limits.h>
 
@@ -37,9 +38,11 @@ struct PostPagedArgs {
     int cos_off, sin_off, half;
     uint16_t* q_out;
     int64_t ld_q;
-    uint16_t* kpages;
-    uint16_t* vpages;
+    void* kpages;  // bf16, or e4m3 codes
+    void* vpages;
     int64_t k_stride, v_stride;
+    uint8_t* scales;  // of codes
+    int64_t s_stride;
 };
 
 // One workgroup per packed row (token). Eight lanes per 128 columns (per head of
@@ -67,8 +70,43 @@ struct PostGeom {
     static __device__ __forceinline__ int at(int c) { return c + (c / Leaf) * kLeafPad; }
 };
 
-// WIDE: every row 16-byte aligned, a rotated half whole octets.
-template <int D, bool WIDE>
+// ---- 8-bit pages ---------------------------------------------------------------------
+//
+// A head's power of two is the smallest that brings its largest finite magnitude
+// to 448 = 1.75 * 2^8 (e4m3's largest) or less. A power of two costs e4m3 nothing
+// against a finer scale but the place of its smallest values (codes below 2^-6 are
+// 2^-14.8 of the largest at most), products with it are exact, and it is one byte.
+// Codes are rounded to nearest even, half a step, 2^-4 relative; what is not
+// finite becomes NaN.
+
+// The biased exponent, 1 .. 254, from the largest finite magnitude's bf16 bits.
+__device__ __forceinline__ int power_of(int bits) {
+    return max(1, (bits >> 7) - 8 + ((bits & 0x7F) > 0x60 ? 1 : 0));
+}
+
+__device__ __forceinline__ int finite_magnitude(uint16_t bits) {
+    const int m = bits & 0x7FFF;
+    return m < 0x7F80 ? m : 0;
+}
+
+// Eight bf16 values as codes. (v_cvt_pk_fp8_f32: to nearest even; infinities, like NaN, give NaN.)
+__device__ __forceinline__ uint2 encode8(const uint16_t (&v)[8], int power) {
+    const float up = __builtin_bit_cast(float, (uint32_t)(254 - power) << 23);  // 2^(127 - power)
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = bf16_bits_to_f32(v[4 * i + e]) * up;
+        const int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], c, true);
+    }
+    return uint2{w[0], w[1]};
+}
+
+// WIDE: every row 16-byte aligned (8-bit pages: 8), a rotated half whole octets.
+// E8: 8-bit pages.
+template <int D, bool WIDE, bool E8>
 __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post_paged_kernel(PostPagedArgs a) {
     using G = PostGeom<D>;
     __shared__ __align__(16) float rows[kPostMaxWaves][G::Heads * G::Row];
@@ -158,14 +196,8 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
                 p[1] = float4{f[e][4], f[e][5], f[e][6], f[e][7]};
             }
         }
-        uint16_t* dst = d.role == 0 ? a.q_out + (int64_t)t * a.ld_q + d.h * D
-                                    : (d.role == 1 ? a.kpages + max(page, 0) * a.k_stride : a.vpages + max(page, 0) * a.v_stride) +
-                                          (((int64_t)d.h << a.b.shift) + slot) * D;
-        const bool put = d.in && (d.role == 0 || page >= 0);
-#pragma unroll
-        for (int e = 0; e < G::Oct; ++e) {
+        auto rotated = [&](int e, uint16_t (&out)[8]) __attribute__((always_inline)) {
             const int c0 = 8 * (hl + G::Lanes * e);
-            uint16_t out[8];
             if (rot && c0 < 2 * a.half) {
                 // run_rope_cpu_gemma (model.py:549-575): y1 = x1 c - x2 s, y2 = x2 c + x1 s.
                 if constexpr (WIDE) {
@@ -202,12 +234,56 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
             if (!ok)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) out[i] = 0;
+        };
+        const bool put = d.in && (d.role == 0 || page >= 0);
+        const int64_t at = (((int64_t)d.h << a.b.shift) + slot) * D;  // in its page
+        if constexpr (E8) {
+            uint16_t out[G::Oct][8];
+            int top = 0;
+#pragma unroll
+            for (int e = 0; e < G::Oct; ++e) {
+                rotated(e, out[e]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max(top, finite_magnitude(out[e][i]));
+            }
+#pragma unroll
+            for (int k = 1; k < G::Lanes; k <<= 1) top = max(top, __shfl_xor(top, k));
             if (!put) continue;
-            const uint4 o8 = pack8(out);
-            if constexpr (WIDE)
-                *reinterpret_cast<uint4*>(dst + c0) = o8;
-            else
-                __builtin_memcpy(dst + c0, &o8, sizeof(o8));
+            const int power = power_of(top);
+#pragma unroll
+            for (int e = 0; e < G::Oct; ++e) {
+                const int c0 = 8 * (hl + G::Lanes * e);
+                if (d.role == 0) {
+                    const uint4 o8 = pack8(out[e]);
+                    __builtin_memcpy(a.q_out + (int64_t)t * a.ld_q + d.h * D + c0, &o8, sizeof(o8));
+                } else {
+                    uint8_t* dst = d.role == 1 ? static_cast<uint8_t*>(a.kpages) + page * a.k_stride
+                                               : static_cast<uint8_t*>(a.vpages) + page * a.v_stride;
+                    const uint2 o8 = encode8(out[e], power);
+                    if constexpr (WIDE)
+                        *reinterpret_cast<uint2*>(dst + at + c0) = o8;
+                    else
+                        __builtin_memcpy(dst + at + c0, &o8, sizeof(o8));
+                }
+            }
+            if (d.role && hl == 0)
+                a.scales[page * a.s_stride + 2 * (((int64_t)d.h << a.b.shift) + slot) + d.role - 1] = (uint8_t)power;
+        } else {
+            uint16_t* dst = d.role == 0 ? a.q_out + (int64_t)t * a.ld_q + d.h * D
+                                        : at + (d.role == 1 ? static_cast<uint16_t*>(a.kpages) + max(page, 0) * a.k_stride
+                                                            : static_cast<uint16_t*>(a.vpages) + max(page, 0) * a.v_stride);
+#pragma unroll
+            for (int e = 0; e < G::Oct; ++e) {
+                uint16_t out[8];
+                rotated(e, out);
+                if (!put) continue;
+                const uint4 o8 = pack8(out);
+                const int c0 = 8 * (hl + G::Lanes * e);
+                if constexpr (WIDE)
+                    *reinterpret_cast<uint4*>(dst + c0) = o8;
+                else
+                    __builtin_memcpy(dst + c0, &o8, sizeof(o8));
+            }
         }
     }
 }
@@ -246,43 +322,45 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(CopyArgs a) {
 
 using namespace alv;
 
-extern "C" int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off, int heads, int kv_heads,
-                                  int D, const float* q_w, const float* k_w, int norm_q, int norm_k, int norm_v,
-                                  float eps, const uint16_t* rope, int rope_rows, int64_t rope_stride, int cos_off,
-                                  int sin_off, int half, const int32_t* page_table, int64_t ld_table, int max_pages,
-                                  const int32_t* q_start, const int32_t* kv_len, int B, int T, int pages,
-                                  int page_size, uint16_t* kpages, uint16_t* vpages, int64_t k_stride,
-                                  int64_t v_stride, uint16_t* q_out, int64_t ld_q, void* stream) {
-    PostPagedArgs a{};
+namespace alv {
+namespace {
+
+// Both kinds of pages: 8-bit ones where scales are given (E8).
+template <bool E8>
+int post_paged(PostPagedArgs a, int64_t ld_table, int max_pages, const int32_t* page_table, const int32_t* q_start,
+               const int32_t* kv_len, int B, int T, int pages, int page_size, int D, int rope_rows, void* stream) {
     if (int rc = paged_batch(page_table, ld_table, max_pages, q_start, kv_len, B, T, pages, page_size, &a.b)) return rc;
-    if (!kpages || !vpages || (T > 0 && (!qkv || !q_out))) return fail(ALV_ERR_ARG, "null pointer");
+    if (!a.kpages || !a.vpages || (E8 && !a.scales) || (T > 0 && (!a.qkv || !a.q_out))) return fail(ALV_ERR_ARG, "null pointer");
+    const int heads = a.heads, kv_heads = a.kv_heads, k_off = a.k_off, v_off = a.v_off;
     const int64_t qw = (int64_t)heads * D, kw = (int64_t)kv_heads * D;
     if (heads < 1 || kv_heads < 1 || heads % kv_heads || (D != 64 && D != 128 && D != 256 && D != 512) || k_off < qw ||
-        (v_off >= 0 && v_off < k_off + kw) || ld_qkv < (v_off < 0 ? k_off : v_off) + kw || ld_q < qw)
+        (v_off >= 0 && v_off < k_off + kw) || a.ld_qkv < (v_off < 0 ? k_off : v_off) + kw || a.ld_q < qw)
         return fail(ALV_ERR_ARG, "bad qkv layout heads=%d kv_heads=%d D=%d k_off=%d v_off=%d (D one of 64, 128, 256, 512)",
                     heads, kv_heads, D, k_off, v_off);
     if (heads > kMaxHeads) return fail(ALV_ERR_RANGE, "%d heads (at most %d)", heads, kMaxHeads);
     const int64_t page_values = (int64_t)kv_heads * page_size * D;
-    if (k_stride < page_values || v_stride < page_values)
-        return fail(ALV_ERR_ARG, "page strides %lld and %lld hold fewer than the page's %lld values", (long long)k_stride,
-                    (long long)v_stride, (long long)page_values);
-    if (rope && (half < 1 || 2 * half > D || rope_rows < 1 || rope_stride < 1 || cos_off < 0 || sin_off < 0 ||
-                 cos_off + half > rope_stride || sin_off + half > rope_stride))
+    if (a.k_stride < page_values || a.v_stride < page_values)
+        return fail(ALV_ERR_ARG, "page strides %lld and %lld hold fewer than the page's %lld values", (long long)a.k_stride,
+                    (long long)a.v_stride, (long long)page_values);
+    if (E8 && a.s_stride < 2 * (int64_t)kv_heads * page_size)
+        return fail(ALV_ERR_ARG, "scales %lld apart hold fewer than a page's %lld", (long long)a.s_stride,
+                    2ll * kv_heads * page_size);
+    if (a.rope && (a.half < 1 || 2 * (int64_t)a.half > D || rope_rows < 1 || a.rope_stride < 1 || a.cos_off < 0 ||
+                   a.sin_off < 0 || a.cos_off + (int64_t)a.half > a.rope_stride || a.sin_off + (int64_t)a.half > a.rope_stride))
         return fail(ALV_ERR_ARG, "bad rope table layout rows=%d stride=%lld cos_off=%d sin_off=%d half=%d for D=%d",
-                    rope_rows, (long long)rope_stride, cos_off, sin_off, half, D);
+                    rope_rows, (long long)a.rope_stride, a.cos_off, a.sin_off, a.half, D);
     if (T == 0) return ALV_OK;
-    a.qkv = qkv, a.ld_qkv = ld_qkv, a.k_off = k_off, a.v_off = v_off, a.heads = heads, a.kv_heads = kv_heads;
-    a.q_w = q_w, a.k_w = k_w, a.norm_q = norm_q, a.norm_k = norm_k, a.norm_v = norm_v, a.eps = eps;
-    a.rope = rope, a.rope_stride = rope_stride, a.cos_off = cos_off, a.sin_off = sin_off, a.half = half;
-    a.q_out = q_out, a.ld_q = ld_q, a.kpages = kpages, a.vpages = vpages, a.k_stride = k_stride, a.v_stride = v_stride;
-    a.rope_rows = rope ? rope_rows : INT_MAX;
+    a.rope_rows = a.rope ? rope_rows : INT_MAX;
     auto rows16 = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
-    const bool wide = rows16(qkv, ld_qkv) && rows16(q_out, ld_q) && rows16(kpages, k_stride) && rows16(vpages, v_stride) &&
-             k_off % 8 == 0 && (v_off < 0 || v_off % 8 == 0) &&
-                      (!rope || (rows16(rope, rope_stride) && cos_off % 8 == 0 && sin_off % 8 == 0 && half % 8 == 0));
-    if (reinterpret_cast<uintptr_t>(qkv) % 2 || reinterpret_cast<uintptr_t>(q_out) % 2 || reinterpret_cast<uintptr_t>(rope) % 2 ||
-        reinterpret_cast<uintptr_t>(kpages) % 2 || reinterpret_cast<uintptr_t>(vpages) % 2 ||
-        reinterpret_cast<uintptr_t>(q_w) % 16 || reinterpret_cast<uintptr_t>(k_w) % 16)
+    auto rows8 = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 8 == 0 && ld % 8 == 0; };
+    const bool wide = rows16(a.qkv, a.ld_qkv) && rows16(a.q_out, a.ld_q) &&
+                      (E8 ? rows8(a.kpages, a.k_stride) && rows8(a.vpages, a.v_stride)
+                          : rows16(a.kpages, a.k_stride) && rows16(a.vpages, a.v_stride)) &&
+                      k_off % 8 == 0 && (v_off < 0 || v_off % 8 == 0) &&
+                      (!a.rope || (rows16(a.rope, a.rope_stride) && a.cos_off % 8 == 0 && a.sin_off % 8 == 0 && a.half % 8 == 0));
+    if (reinterpret_cast<uintptr_t>(a.qkv) % 2 || reinterpret_cast<uintptr_t>(a.q_out) % 2 || reinterpret_cast<uintptr_t>(a.rope) % 2 ||
+        (!E8 && (reinterpret_cast<uintptr_t>(a.kpages) % 2 || reinterpret_cast<uintptr_t>(a.vpages) % 2)) ||
+        reinterpret_cast<uintptr_t>(a.q_w) % 16 || reinterpret_cast<uintptr_t>(a.k_w) % 16)
         return fail(ALV_ERR_ALIGN, "q_w and k_w need 16-byte alignment, the bf16 arrays 2-byte");
     const int per_wave = D <= 128 ? 8 : 1024 / D;  // heads
     const int threads = 64 * std::min(kPostMaxWaves, (heads + 2 * kv_heads + per_wave - 1) / per_wave);
@@ -291,11 +369,47 @@ extern "C" int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off
         return hip_check(hipGetLastError(), "qkv_post_paged_kernel launch");
     };
     switch (D) {
-        case 64: return wide ? go(qkv_post_paged_kernel<64, true>) : go(qkv_post_paged_kernel<64, false>);
-        case 128: return wide ? go(qkv_post_paged_kernel<128, true>) : go(qkv_post_paged_kernel<128, false>);
-        case 256: return wide ? go(qkv_post_paged_kernel<256, true>) : go(qkv_post_paged_kernel<256, false>);
-        default: return wide ? go(qkv_post_paged_kernel<512, true>) : go(qkv_post_paged_kernel<512, false>);
+        case 64: return wide ? go(qkv_post_paged_kernel<64, true, E8>) : go(qkv_post_paged_kernel<64, false, E8>);
+        case 128: return wide ? go(qkv_post_paged_kernel<128, true, E8>) : go(qkv_post_paged_kernel<128, false, E8>);
+        case 256: return wide ? go(qkv_post_paged_kernel<256, true, E8>) : go(qkv_post_paged_kernel<256, false, E8>);
+        default: return wide ? go(qkv_post_paged_kernel<512, true, E8>) : go(qkv_post_paged_kernel<512, false, E8>);
     }
+}
+
+}  // namespace
+}  // namespace alv
+
+extern "C" int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off, int heads, int kv_heads,
+                                  int D, const float* q_w, const float* k_w, int norm_q, int norm_k, int norm_v,
+                                  float eps, const uint16_t* rope, int rope_rows, int64_t rope_stride, int cos_off,
+                                  int sin_off, int half, const int32_t* page_table, int64_t ld_table, int max_pages,
+                                  const int32_t* q_start, const int32_t* kv_len, int B, int T, int pages,
+                                  int page_size, uint16_t* kpages, uint16_t* vpages, int64_t k_stride,
+                                  int64_t v_stride, uint16_t* q_out, int64_t ld_q, void* stream) {
+    PostPagedArgs a{};
+    a.qkv = qkv, a.ld_qkv = ld_qkv, a.k_off = k_off, a.v_off = v_off, a.heads = heads, a.kv_heads = kv_heads;
+    a.q_w = q_w, a.k_w = k_w, a.norm_q = norm_q, a.norm_k = norm_k, a.norm_v = norm_v, a.eps = eps;
+    a.rope = rope, a.rope_stride = rope_stride, a.cos_off = cos_off, a.sin_off = sin_off, a.half = half;
+    a.q_out = q_out, a.ld_q = ld_q, a.kpages = kpages, a.vpages = vpages, a.k_stride = k_stride, a.v_stride = v_stride;
+    return post_paged<false>(a, ld_table, max_pages, page_table, q_start, kv_len, B, T, pages, page_size, D, rope_rows,
+                             stream);
+}
+
+extern "C" int alv_qkv_post_paged8(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off, int heads, int kv_heads,
+                                   int D, const float* q_w, const float* k_w, int norm_q, int norm_k, int norm_v,
+                                   float eps, const uint16_t* rope, int rope_rows, int64_t rope_stride, int cos_off,
+                                   int sin_off, int half, const int32_t* page_table, int64_t ld_table, int max_pages,
+                                   const int32_t* q_start, const int32_t* kv_len, int B, int T, int pages,
+                                   int page_size, uint8_t* kpages, uint8_t* vpages, int64_t k_stride, int64_t v_stride,
+                                   uint8_t* scales, int64_t s_stride, uint16_t* q_out, int64_t ld_q, void* stream) {
+    PostPagedArgs a{};
+    a.qkv = qkv, a.ld_qkv = ld_qkv, a.k_off = k_off, a.v_off = v_off, a.heads = heads, a.kv_heads = kv_heads;
+    a.q_w = q_w, a.k_w = k_w, a.norm_q = norm_q, a.norm_k = norm_k, a.norm_v = norm_v, a.eps = eps;
+    a.rope = rope, a.rope_stride = rope_stride, a.cos_off = cos_off, a.sin_off = sin_off, a.half = half;
+    a.q_out = q_out, a.ld_q = ld_q, a.kpages = kpages, a.vpages = vpages, a.k_stride = k_stride, a.v_stride = v_stride;
+    a.scales = scales, a.s_stride = s_stride;
+    return post_paged<true>(a, ld_table, max_pages, page_table, q_start, kv_len, B, T, pages, page_size, D, rope_rows,
+                            stream);
 }
 
 extern "C" int alv_copy_pages(void* const* caches, int ncaches, int64_t page_bytes, int64_t stride_bytes, int pages,

@@ -462,6 +462,76 @@ def _per_row(v, name: str, B: int, dtype: torch.dtype, dev: torch.device):
     return None, max(-1, min(int(v), 2 ** 31 - 1)) if dtype == torch.int32 else float(v)
 
 
+def _token_rows(t, name: str, dtype: torch.dtype, B: int, width: int, dev: torch.device):
+    """(address, row stride, columns) of a (B, >= width) tensor or one row for all."""
+    if t is None:
+        return None, 0, 0
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != dev or t.dim() not in (1, 2):
+        raise TypeError(f"{name} must be a {str(dtype)[6:]} tensor of one or {B} rows on the logits' device")
+    n, ld = t.shape[-1], 0 if t.dim() == 1 or t.shape[0] == 1 else t.stride(0)
+    if t.dim() == 2 and t.shape[0] not in (1, B) or n < width:
+        raise ValueError(f"{name} of shape {tuple(t.shape)} for {B} rows of at least {width}")
+    if n > 1 and t.stride(-1) != 1 or ld < 0:
+        raise ValueError(f"{name} must be contiguous along its rows")
+    return t.data_ptr(), ld, n
+
+
+def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, n_tokens: torch.Tensor | None = None,
+                  n_prompt: torch.Tensor | None = None, repetition=1.0, frequency=0.0, presence=0.0,
+                  bias_tokens: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                  allowed: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """What is done to rows of logits (float32, (B, vocab) or (vocab,)) before
+    ``sample``; in this order, for each token:
+
+    - if it is among the row's ``tokens``, l / ``repetition`` where l > 0, else l *
+      ``repetition``;
+    - if it is c > 0 times among those from ``n_prompt`` on, less ``frequency`` * c
+      + ``presence``;
+    - plus the ``bias`` of every time it is in ``bias_tokens``;
+    - -inf if bit t % 32 of word t // 32 of ``allowed`` (int32) is clear.
+
+    ``tokens`` (int32, (B, L)): prompt and generated tokens, of which the first
+    ``n_tokens`` (int32, one per row, by default all) count, the first ``n_prompt``
+    (by default none) of them as prompt. ``bias_tokens`` (int32) with ``bias``
+    (float32) and ``allowed`` are rows of (B, ...) or one for all; tokens outside
+    the vocabulary count for nothing. The penalties are numbers or one float32
+    value per row on the device. Float64 where something applies, rounded once.
+    Returns a new tensor, or ``out``, which may be ``logits`` itself: then only
+    what changes is read and written."""
+    dev = _need_gpu(logits)
+    if logits.dtype != torch.float32 or logits.dim() not in (1, 2) or logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        raise TypeError("logits must be float32, (B, vocab) or (vocab,), contiguous along the vocabulary")
+    B, V = (1, logits.shape[0]) if logits.dim() == 1 else logits.shape
+    ld = V if logits.dim() == 1 or B <= 1 else logits.stride(0)
+    if (bias is None) != (bias_tokens is None):
+        raise ValueError("bias_tokens and bias come together")
+    t, ldt, L = _token_rows(tokens, "tokens", torch.int32, B, 0, dev)
+    if tokens is not None and B > 1 and (tokens.dim() == 1 or tokens.shape[0] != B):
+        raise ValueError(f"tokens must be {B} rows")
+    bt, ldbt, M = _token_rows(bias_tokens, "bias_tokens", torch.int32, B, 0, dev)
+    bv, ldb, _ = _token_rows(bias, "bias", torch.float32, B, M, dev)
+    al, lda, _ = _token_rows(allowed, "allowed", torch.int32, B, (V + 31) // 32, dev)
+    for v, name in ((n_tokens, "n_tokens"), (n_prompt, "n_prompt")):
+        if v is not None and (not isinstance(v, torch.Tensor) or v.dtype != torch.int32 or v.device != dev or
+                              v.dim() != 1 or not v.is_contiguous() or v.numel() < B):
+            raise TypeError(f"{name} must be a contiguous int32 tensor of {B} on the logits' device")
+    params = (*_per_row(repetition, "repetition", B, torch.float32, dev),
+              *_per_row(frequency, "frequency", B, torch.float32, dev),
+              *_per_row(presence, "presence", B, torch.float32, dev))
+    if out is None:
+        out, ldo = torch.empty(logits.shape, dtype=torch.float32, device=dev), V
+    elif out.dtype != torch.float32 or out.device != dev or out.shape != logits.shape or V > 1 and out.stride(-1) != 1:
+        raise TypeError(f"out must be a float32 tensor of shape {tuple(logits.shape)} on the logits' device")
+    else:
+        ldo = V if out.dim() == 1 or B <= 1 else out.stride(0)
+    with _on(dev):
+        check(lib().alv_adjust_logits(logits.data_ptr(), ld, out.data_ptr(), ldo, B, V, t, ldt, L,
+                                      n_tokens.data_ptr() if n_tokens is not None else None,
+                                      n_prompt.data_ptr() if n_prompt is not None else None, *params, bt, ldbt, bv, ldb, M,
+                                      al, lda, _stream(logits)), "alv_adjust_logits")
+    return out
+
+
 def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
            token: torch.Tensor | None = None, prob: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """One token per row of ``logits`` (float32, (B, vocab) or (vocab,), rows

@@ -10,15 +10,21 @@ the kernels, so a captured step replays with whatever they hold then. Pages are
 entry outside ``[0, pages)`` holds no positions (pages a window has left behind
 may be given up by writing -1 there).
 
-===================  ========================================================
-``qkv_post_paged``   q/k/v norms + RoPE + insert of every new token, in the
-                     bits of ``layer.qkv_post``
-``attention_paged``  attention of every new token: causal, sliding window,
-                     first tokens that stay visible
-``copy_pages``       pages copied within each of many caches
-``PagedCache``       the layers' pages and the tables of a set of sequences:
-                     reserve, fork, truncate, free, compact
-===================  ========================================================
+With ``scales`` the pages are 8-bit, half the bytes: ``torch.float8_e4m3fn``
+codes, and ``scales`` ``(pages, kv_heads, S, 2)`` ``torch.float8_e8m0fnu`` a power
+of two for each slot's k and v; a value is code times power.
+
+==========================  =================================================
+``qkv_post_paged``          q/k/v norms + RoPE + insert of every new token, in
+                            the bits of ``layer.qkv_post``
+``attention_paged``         attention of every new token: causal, sliding
+                            window, first tokens that stay visible
+``attention_shared_paged``  the same where groups of sequences have their
+                            first pages in common: those once per group
+``copy_pages``              pages copied within each of many caches
+``PagedCache``              the layers' pages and the tables of a set of
+                            sequences: reserve, fork, truncate, free, compact
+==========================  =================================================
 """
 from __future__ import annotations
 
@@ -44,18 +50,19 @@ def _rows(t: torch.Tensor, name: str, width: int, dev: torch.device) -> int:
     return ld if T > 1 else w
 
 
-def _page_stride(t: torch.Tensor, name: str, dev: torch.device) -> int:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 4 or t.device != dev:
-        raise TypeError(f"{name} must be a (pages, kv_heads, page_size, D) bfloat16 tensor on {dev}")
+def _page_stride(t: torch.Tensor, name: str, dev: torch.device, dtype: torch.dtype = torch.bfloat16) -> int:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 4 or t.device != dev:
+        last = "2" if name == "scales" else "D"
+        raise TypeError(f"{name} must be a (pages, kv_heads, page_size, {last}) {str(dtype)[6:]} tensor on {dev}")
     (n, H, S, D), (s0, s1, s2, s3) = t.shape, t.stride()
     if s3 != 1 or s2 != D or s1 != S * D and H > 1:
         raise ValueError(f"{name}: each page must be contiguous, got strides {t.stride()}")
     return s0 if n > 1 else H * S * D
 
 
-def _pages(kpages: torch.Tensor, vpages: torch.Tensor, dev: torch.device):
+def _pages(kpages: torch.Tensor, vpages: torch.Tensor, dev: torch.device, dtype: torch.dtype):
     """(shape, page strides) of the two pools: each page contiguous in itself."""
-    ks, vs = _page_stride(kpages, "kpages", dev), _page_stride(vpages, "vpages", dev)
+    ks, vs = _page_stride(kpages, "kpages", dev, dtype), _page_stride(vpages, "vpages", dev, dtype)
     if kpages.shape != vpages.shape:
         raise ValueError(f"kpages and vpages differ: {tuple(kpages.shape)} and {tuple(vpages.shape)}")
     return kpages.shape, ks, vs
@@ -76,17 +83,18 @@ def _batch(page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor
 
 
 _BF16, _I32 = torch.bfloat16, torch.int32
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _INT_MAX = 2 ** 31 - 1
 
 
 def _args(t: torch.Tensor, name: str, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
-          q_start: torch.Tensor, kv_len: torch.Tensor, dev: torch.device):
+          q_start: torch.Tensor, kv_len: torch.Tensor, dev: torch.device, dtype: torch.dtype = _BF16):
     """((pages, kv_heads, S, D), page strides, B, max_pages, table's row stride, T, t's width and row stride): the
-    checks that every call shares. Contiguous tensors, as most are, take one test each (the others' take 6 us of a
-    call whose kernel may take 5)."""
+    checks that every call shares (dtype: the pages'). Contiguous tensors, as most are, take one test each (the
+    others' take 6 us of a call whose kernel may take 5)."""
     i = dev.index
     try:
-        if (t.dtype is _BF16 and kpages.dtype is _BF16 and vpages.dtype is _BF16 and page_table.dtype is _I32
+        if (t.dtype is _BF16 and kpages.dtype is dtype and vpages.dtype is dtype and page_table.dtype is _I32
                 and q_start.dtype is _I32 and kv_len.dtype is _I32 and t.is_contiguous() and kpages.is_contiguous()
                 and vpages.is_contiguous() and page_table.is_contiguous() and q_start.is_contiguous()
                 and kv_len.is_contiguous() and kpages.get_device() == i and vpages.get_device() == i
@@ -101,12 +109,20 @@ def _args(t: torch.Tensor, name: str, kpages: torch.Tensor, vpages: torch.Tensor
                 return shape, n, n, B, W, W, T, w, w
     except (AttributeError, ValueError):
         pass
-    return *_pages(kpages, vpages, dev), *_batch(page_table, q_start, kv_len, dev), *_shape2(t, name, dev)
+    return *_pages(kpages, vpages, dev, dtype), *_batch(page_table, q_start, kv_len, dev), *_shape2(t, name, dev)
 
 
 def _shape2(t: torch.Tensor, name: str, dev: torch.device):
     ld = _rows(t, name, 0, dev)
     return *t.shape, ld
+
+
+def _scales(scales: torch.Tensor, shape, dev: torch.device) -> int:
+    """How many bytes the scales of two pages of an 8-bit pool of `shape` are apart."""
+    ss = _page_stride(scales, "scales", dev, _E8M0)
+    if scales.shape != (*shape[:3], 2):
+        raise ValueError(f"scales of pages {tuple(shape)} are {(*shape[:3], 2)}, got {tuple(scales.shape)}")
+    return ss
 
 
 def _far(**numbers: int) -> None:
@@ -127,16 +143,21 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
                    q_start: torch.Tensor, kv_len: torch.Tensor, *, heads: int, k_off: int, v_off: int, q_w=None,
                    k_w=None, norm_q: bool = True, norm_k: bool = True, norm_v: bool = True, eps: float = _GEMMA_EPS,
                    rope: torch.Tensor | None = None, cos_off: int = 0, sin_off: int | None = None,
-                   half: int | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor:
+                   half: int | None = None, q_out: torch.Tensor | None = None,
+                   scales: torch.Tensor | None = None) -> torch.Tensor:
     """``layer.qkv_post`` for every row of ``qkv`` (T, [q | k | v]): per-head
-    norms, RoPE of q and k at the row's position, k and v into their pages.
+    norms, RoPE of q and k at the row's position, k and v into their pages. With
+    ``scales`` the pages are 8-bit: each head's k (v) gets the smallest power of two
+    that brings its largest finite magnitude to 448 or less, its values the nearest
+    codes (half a step, 2^-4 relative); what is not finite becomes NaN.
     ``rope`` is the (positions, width) bfloat16 table, by default [cos | sin]
     halves of its rows. Returns q (T, heads * D); rows past the last sequence are
     left as they are in ``q_out``, zeros for a sequence that does not fit its
     table (or the rope table)."""
     dev = _need_gpu(qkv)
-    (pages, kv_heads, S, D), ks, vs, B, W, ldt, T, width, ldqkv = _args(qkv, "qkv", kpages, vpages, page_table, q_start,
-                                                                        kv_len, dev)
+    shape, ks, vs, B, W, ldt, T, width, ldqkv = _args(qkv, "qkv", kpages, vpages, page_table, q_start, kv_len, dev,
+                                                      _BF16 if scales is None else _E4M3)
+    pages, kv_heads, S, D = shape
     if v_off < 0:
         v_off = -1
     if not (0 < heads <= _INT_MAX and 0 < k_off <= _INT_MAX and v_off <= _INT_MAX and (half is None or half > 0)):
@@ -159,30 +180,26 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
         ldq = _rows(q_out, "q_out", ldq, dev)
         if q_out.shape[0] < T:
             raise ValueError(f"q_out has {q_out.shape[0]} rows, qkv {T}")
+    args = (qkv.data_ptr(), ldqkv, k_off, v_off, heads, kv_heads, D, _ptr(q_w), _ptr(k_w), norm_q, norm_k, norm_v, eps,
+            _ptr(rope), rope_rows, ldr, cos_off, sin_off or 0, half or 0, page_table.data_ptr(), ldt, W,
+            q_start.data_ptr(), kv_len.data_ptr(), B, T, pages, S, kpages.data_ptr(), vpages.data_ptr(), ks, vs)
     with _on(dev):
-        check(lib().alv_qkv_post_paged(qkv.data_ptr(), ldqkv, k_off, v_off, heads, kv_heads, D, _ptr(q_w), _ptr(k_w),
-                                       norm_q, norm_k, norm_v, eps, _ptr(rope), rope_rows, ldr, cos_off, sin_off or 0,
-                                       half or 0, page_table.data_ptr(), ldt, W, q_start.data_ptr(), kv_len.data_ptr(),
-                                       B, T, pages, S, kpages.data_ptr(), vpages.data_ptr(), ks, vs, q_out.data_ptr(),
-                                       ldq, _stream(qkv)), "alv_qkv_post_paged")
+        if scales is None:
+            check(lib().alv_qkv_post_paged(*args, q_out.data_ptr(), ldq, _stream(qkv)), "alv_qkv_post_paged")
+        else:
+            ss = _scales(scales, shape, dev)
+            check(lib().alv_qkv_post_paged8(*args, scales.data_ptr(), ss, q_out.data_ptr(), ldq, _stream(qkv)),
+                  "alv_qkv_post_paged8")
     return q_out
 
 
-def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
-                    q_start: torch.Tensor, kv_len: torch.Tensor, *, heads: int, window: int = 0, sinks: int = 0,
-                    scale: float = 1.0, max_q: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Attention of every row of ``q`` (T, heads * D) over the positions up to
-    its own: all of them, or with ``window`` the last ``window`` and the first
-    ``sinks``. A row that sees no position gets zeros; rows past the last
-    sequence are left as they are in ``out``, which does not overlap ``q``.
-    Scores, maxima and sums are float32; the weights are rounded to bfloat16 for
-    the product with V. ``max_q``, the most rows any sequence owns, where the
-    caller knows it, lets the call choose how to spread the work (1 for a decode
-    step): like the other sequences' lengths it may change a row's last bits, by
-    the order in which its sums are rounded, and nothing else."""
+def _attention(q, kpages, vpages, page_table, q_start, kv_len, heads, window, sinks, max_q, out, scales):
+    """The checks that both attentions share: (arguments of the C calls up to the batch's, from heads to sinks, out,
+    its row stride, the numbers that a workspace's size goes by)."""
     dev = _need_gpu(q)
-    (pages, kv_heads, S, D), ks, vs, B, W, ldt, T, width, ldq = _args(q, "q", kpages, vpages, page_table, q_start, kv_len,
-                                                                      dev)
+    shape, ks, vs, B, W, ldt, T, width, ldq = _args(q, "q", kpages, vpages, page_table, q_start, kv_len, dev,
+                                                    _BF16 if scales is None else _E4M3)
+    pages, kv_heads, S, D = shape
     ldo = heads * D
     if width < ldo:
         _narrow("q", width, ldo)
@@ -196,13 +213,67 @@ def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
         ldo = _rows(out, "out", ldo, dev)
         if out.shape[0] < T:
             raise ValueError(f"out has {out.shape[0]} rows, q {T}")
+    batch = (pages, S, page_table.data_ptr(), ldt, W, q_start.data_ptr(), kv_len.data_ptr(), B, T, max_q)
+    pools = (q.data_ptr(), ldq, kpages.data_ptr(), vpages.data_ptr(), ks, vs)
+    if scales is not None:
+        pools += scales.data_ptr(), _scales(scales, shape, dev)
+    return dev, pools, batch, (heads, kv_heads, D, window, sinks), out, ldo
+
+
+def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
+                    q_start: torch.Tensor, kv_len: torch.Tensor, *, heads: int, window: int = 0, sinks: int = 0,
+                    scale: float = 1.0, max_q: int = 0, out: torch.Tensor | None = None,
+                    scales: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of every row of ``q`` (T, heads * D) over the positions up to
+    its own: all of them, or with ``window`` the last ``window`` and the first
+    ``sinks``. A row that sees no position gets zeros; rows past the last
+    sequence are left as they are in ``out``, which does not overlap ``q``.
+    Scores, maxima and sums are float32; the weights are rounded to bfloat16 for
+    the product with V. ``max_q``, the most rows any sequence owns, where the
+    caller knows it, lets the call choose how to spread the work (1 for a decode
+    step): like the other sequences' lengths it may change a row's last bits, by
+    the order in which its sums are rounded, and nothing else. With ``scales`` the
+    pages are 8-bit."""
+    dev, pools, batch, shape, out, ldo = _attention(q, kpages, vpages, page_table, q_start, kv_len, heads, window, sinks,
+                                                    max_q, out, scales)
     L = lib()
+    run, size = ((L.alv_attention_paged, L.alv_attention_paged_workspace) if scales is None else
+                 (L.alv_attention_paged8, L.alv_attention_paged8_workspace))
     with _on(dev):
-        ws = _workspace(L.alv_attention_paged_workspace(heads, kv_heads, D, B, T, max_q), dev)
-        check(L.alv_attention_paged(q.data_ptr(), ldq, kpages.data_ptr(), vpages.data_ptr(), ks, vs, pages, S,
-                                    page_table.data_ptr(), ldt, W, q_start.data_ptr(), kv_len.data_ptr(), B, T, max_q,
-                                    heads, kv_heads, D, window, sinks, scale, out.data_ptr(), ldo, *ws[1:],
-                                    _stream(q)), "alv_attention_paged")
+        ws = _workspace(size(*shape[:3], *batch[-3:]), dev)
+        check(run(*pools, *batch, *shape, scale, out.data_ptr(), ldo, *ws[1:], _stream(q)),
+              "alv_attention_paged" if scales is None else "alv_attention_paged8")
+    return out
+
+
+def attention_shared_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, page_table: torch.Tensor,
+                           q_start: torch.Tensor, kv_len: torch.Tensor, group_start: torch.Tensor,
+                           shared_len: torch.Tensor, *, heads: int, window: int = 0, sinks: int = 0, scale: float = 1.0,
+                           max_q: int = 0, out: torch.Tensor | None = None,
+                           scales: torch.Tensor | None = None) -> torch.Tensor:
+    """``attention_paged`` of a batch whose sequences come in groups with the same
+    first pages (``PagedCache.shared`` finds them), which are read and multiplied
+    once for all of a group's rows. Group j is the sequences ``group_start[j] ..
+    group_start[j + 1] - 1``; the first ``shared_len[j]`` positions of each (whole
+    pages of them, and no more than the group's first sequence has) are taken from
+    its first sequence's pages. Both are int32 tensors on the device, of groups + 1
+    and groups values, read by the kernels. Every row sees what it sees in
+    ``attention_paged``, its last bits may differ."""
+    dev, pools, batch, shape, out, ldo = _attention(q, kpages, vpages, page_table, q_start, kv_len, heads, window, sinks,
+                                                    max_q, out, scales)
+    for t, name in ((group_start, "group_start"), (shared_len, "shared_len")):
+        if not isinstance(t, torch.Tensor) or t.dtype != _I32 or t.dim() != 1 or t.device != dev or not t.is_contiguous():
+            raise TypeError(f"{name} must be a contiguous 1-D int32 tensor on {dev}")
+    G = shared_len.shape[0]
+    if group_start.shape[0] != G + 1:
+        raise ValueError(f"{G} shared lengths need group_start of {G + 1}, got {group_start.shape[0]}")
+    L = lib()
+    if scales is None:
+        pools += None, 0
+    with _on(dev):
+        ws = _workspace(L.alv_attention_shared_workspace(*shape[:3], *batch[-3:], G), dev)
+        check(L.alv_attention_shared(*pools, *batch, group_start.data_ptr(), shared_len.data_ptr(), G, *shape, scale,
+                                     out.data_ptr(), ldo, *ws[1:], _stream(q)), "alv_attention_shared")
     return out
 
 
@@ -260,7 +331,8 @@ def copy_pages(caches, src, dst) -> None:
 
 class PagedCache:
     """The K and V pages of a model's layers and the tables of up to ``slots``
-    sequences. One page number stands for that page of every layer, K and V:
+    sequences; ``dtype`` torch.float8_e4m3fn: 8-bit pages, whose ``scales`` are a
+    tensor per layer (None of bfloat16 ones). One page number stands for that page of every layer, K and V:
     layers of another head layout are another cache's, and a page stays its
     sequence's until that is truncated or freed, whatever a window has left behind.
 
@@ -273,16 +345,23 @@ class PagedCache:
     nothing, nor does one whose copies raise."""
 
     def __init__(self, *, layers: int, kv_heads: int, D: int, pages: int, page_size: int, slots: int, max_pages: int,
-                 device):
+                 device, dtype: torch.dtype = torch.bfloat16):
         if min(layers, kv_heads, D, pages, slots, max_pages) < 1:
             raise ValueError("layers, kv_heads, D, pages, slots and max_pages must be positive")
         if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
             raise ValueError(f"page_size={page_size}: a power of two from 16 to 1024")
         self.page_size, self.pages, self.slots, self.max_pages = page_size, pages, slots, max_pages
-        self.pool = torch.zeros((layers, 2, pages, kv_heads, page_size, D), dtype=torch.bfloat16, device=device)
-        self.device = self.pool.device
+        if dtype not in (_BF16, _E4M3):
+            raise ValueError(f"dtype={dtype}: torch.bfloat16 or torch.float8_e4m3fn")
+        self.pool = torch.zeros((layers, 2, pages, kv_heads, page_size, D), dtype=dtype, device=device)
+        self.device, self.dtype = self.pool.device, dtype
         self.k = [self.pool[i, 0] for i in range(layers)]
         self.v = [self.pool[i, 1] for i in range(layers)]
+        self.scales: list = [None] * layers
+        if dtype == _E4M3:
+            # (zeros would be 2^-127; of zero codes any power is one)
+            powers = torch.full((layers, pages, kv_heads, page_size, 2), 127, dtype=torch.uint8, device=device)
+            self.scales = list(powers.view(_E8M0).unbind(0))
         self._table: list[list[int]] = [[] for _ in range(slots)]
         self._len = [0] * slots
         self._shared = [0] * pages  # slots that hold the page
@@ -306,6 +385,8 @@ class PagedCache:
 
     def _copy(self, src: list[int], dst: list[int]) -> None:
         copy_pages(self.k + self.v, src, dst)
+        if self.dtype == _E4M3:
+            copy_pages(self.scales, src, dst)
 
     def _drop(self, page: int) -> None:
         self._shared[page] -= 1
@@ -428,3 +509,42 @@ class PagedCache:
         d = host.to(self.device)
         t, q, k = d.split([B * self.max_pages, B + 1, B])
         return t.view(B, self.max_pages), q, k
+
+    def shared(self, slots):
+        """(group_start, shared_len) on the device for ``attention_shared_paged`` of a
+        batch of these slots in this order: neighbours that have their first pages
+        in common, grouped so that the fewest pages are read. They hold until a
+        slot is forked, truncated, freed or its last shared page copied."""
+        slots = [self._slot(s) for s in slots]
+        if len(set(slots)) != len(slots):
+            raise ValueError("each slot once")
+        B, S = len(slots), self.page_size
+        common = []  # whole pages that neighbours share
+        for a, b in zip(slots, slots[1:]):
+            ta, tb = self._table[a], self._table[b]
+            most = min(self._len[a], self._len[b]) // S
+            lo, hi = 0, min(most, len(ta), len(tb))
+            if ta[:hi] != tb[:hi]:
+                while lo + 1 < hi:  # ta[:lo] == tb[:lo], ta[:hi] != tb[:hi]
+                    mid = (lo + hi) // 2
+                    lo, hi = (mid, hi) if ta[:mid] == tb[:mid] else (lo, mid)
+                hi = lo
+            common.append(hi)
+        # best[j]: (pages not read again among the first j slots, first slot of the last group, its shared pages)
+        best = [(0, 0, 0)]
+        for j in range(1, B + 1):
+            least, top = None, (best[j - 1][0], j - 1, 0)
+            for i in range(j - 2, -1, -1):
+                least = common[i] if least is None else min(least, common[i])
+                if least == 0:
+                    break
+                top = max(top, (best[i][0] + (j - 1 - i) * least, i, least), key=lambda v: v[0])
+            best.append(top)
+        start, length, j = [B], [], B
+        while j:
+            _, i, pages = best[j]
+            start.append(i)
+            length.append(pages * S)
+            j = i
+        host = torch.tensor(start[::-1] + length[::-1], dtype=torch.int32)
+        return host.to(self.device).split([len(start), len(length)])

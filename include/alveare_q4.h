@@ -469,6 +469,23 @@ int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off
                        void* stream);
 
 /*
+ * The same into 8-bit pages: kpages and vpages (page, kv head, slot, column) hold
+ * e4m3 codes (OCP: largest 448, NaN 0x7F and 0xFF), strides in codes, and scales (page, kv
+ * head, slot, [k, v]), pages s_stride bytes apart, a biased exponent of each slot's
+ * k and v: a value is code * 2^(scale - 127). The power is the smallest that brings
+ * the largest finite magnitude of the head's D bf16 values to 448 or less, at least
+ * 2^-126; codes are the values over it, to nearest even; what is not finite becomes
+ * NaN. Scales written are 1 to 254; one of 255 makes a slot's values infinite or NaN.
+ */
+int alv_qkv_post_paged8(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off, int heads, int kv_heads, int D,
+                        const float* q_w, const float* k_w, int norm_q, int norm_k, int norm_v, float eps,
+                        const uint16_t* rope, int rope_rows, int64_t rope_stride, int cos_off, int sin_off, int half,
+                        const int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* q_start,
+                        const int32_t* kv_len, int B, int T, int pages, int page_size, uint8_t* kpages,
+                        uint8_t* vpages, int64_t k_stride, int64_t v_stride, uint8_t* scales, int64_t s_stride,
+                        uint16_t* q_out, int64_t ld_q, void* stream);
+
+/*
  * out[t, h] = softmax(scale * K q[t, h]) V for every row t of a batch over the
  * positions p <= the row's own that its window holds: all of them, or with
  * window > 0 the last `window` and the first `sinks`. float32 scores, maxima and
@@ -497,6 +514,41 @@ int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16_t* kpages,
                         int64_t ld_out, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /*
+ * The same over 8-bit pages (alv_qkv_post_paged8): strides in codes, multiples of
+ * 16; scales 16-byte aligned and s_stride a multiple of 16.
+ */
+uint64_t alv_attention_paged8_workspace(int heads, int kv_heads, int D, int B, int T, int max_q);
+int alv_attention_paged8(const uint16_t* q, int64_t ld_q, const uint8_t* kpages, const uint8_t* vpages,
+                         int64_t k_stride, int64_t v_stride, const uint8_t* scales, int64_t s_stride, int pages,
+                         int page_size, const int32_t* page_table, int64_t ld_table, int max_pages,
+                         const int32_t* q_start, const int32_t* kv_len, int B, int T, int max_q, int heads,
+                         int kv_heads, int D, int window, int sinks, float scale, uint16_t* out, int64_t ld_out,
+                         void* workspace, uint64_t workspace_bytes, void* stream);
+
+/*
+ * alv_attention_paged, or with scales alv_attention_paged8 (NULL: bf16 pages), of a
+ * batch whose sequences come in groups with the same first positions, which are
+ * read and multiplied once for all rows of a group. Group j < groups is the
+ * sequences group_start[j] .. group_start[j + 1] - 1 (groups + 1 entries, not
+ * decreasing); the first shared_len[j] positions of each, whole pages of them and
+ * no more than the group's first sequence has, are those of its first sequence:
+ * the others' table entries for them are not read. A sequence in no group shares
+ * nothing. group_start and shared_len are int32 device memory, read by the
+ * kernels. Every row sees what alv_attention_paged lets it see; what the two
+ * parts of a row give is joined by their maxima and sums in float32, so its last
+ * bits may differ from that call's. workspace: alv_attention_shared_workspace
+ * bytes for the same arguments, as for alv_attention_paged.
+ */
+uint64_t alv_attention_shared_workspace(int heads, int kv_heads, int D, int B, int T, int max_q, int groups);
+int alv_attention_shared(const uint16_t* q, int64_t ld_q, const void* kpages, const void* vpages, int64_t k_stride,
+                         int64_t v_stride, const uint8_t* scales, int64_t s_stride, int pages, int page_size,
+                         const int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* q_start,
+                         const int32_t* kv_len, int B, int T, int max_q, const int32_t* group_start,
+                         const int32_t* shared_len, int groups, int heads, int kv_heads, int D, int window, int sinks,
+                         float scale, uint16_t* out, int64_t ld_out, void* workspace, uint64_t workspace_bytes,
+                         void* stream);
+
+/*
  * In each of `ncaches` caches (host array of device pointers; pages of
  * page_bytes bytes, stride_bytes apart, both multiples of 16, caches 16-byte
  * aligned, none overlapping): page dst[i] = page src[i], i < npairs. src and dst are HOST
@@ -506,6 +558,31 @@ int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16_t* kpages,
  */
 int alv_copy_pages(void* const* caches, int ncaches, int64_t page_bytes, int64_t stride_bytes, int pages,
                    const int32_t* src, const int32_t* dst, int npairs, void* stream);
+
+/*
+ * What is done to a row of float32 logits between the head and alv_sample, for B
+ * rows (ld and ld_out apart; out == logits with ld == ld_out: in place, else the
+ * two do not overlap). For token t with logit l, in this order:
+ *   x = l > 0 ? l / repetition : l * repetition    if t is among the row's tokens
+ *   x -= frequency * c + presence                  if it is c > 0 times among those
+ *                                                  from n_prompt on
+ *   x += its biases                                 each time t is on the row's list
+ *   x = -infinity                                   if bit t % 32 of word t / 32 is clear
+ * in float64 where any of the first three applies, rounded once; other logits keep
+ * their bits. tokens: L int32 a row (ld_tokens apart), of which the first
+ * n_tokens[b] count (NULL: all L; taken to be within [0, L]), and of these the
+ * first n_prompt[b] as prompt (NULL: none). bias_tokens, bias: M entries a row;
+ * allowed: (V + 31) / 32 words a row, NULL: all are allowed. Rows of the last four
+ * may be 0 apart: the same for all. Tokens outside [0, V) count for nothing.
+ * repetition (above 0), frequency and presence come as device arrays of B values,
+ * or (NULL) as one number. B <= 65535, V <= 2^24, L <= 2^30, B * V <= 2^35.
+ */
+int alv_adjust_logits(const float* logits, int64_t ld, float* out, int64_t ld_out, int B, int V,
+                      const int32_t* tokens, int64_t ld_tokens, int L, const int32_t* n_tokens,
+                      const int32_t* n_prompt, const float* repetition_dev, float repetition,
+                      const float* frequency_dev, float frequency, const float* presence_dev, float presence,
+                      const int32_t* bias_tokens, int64_t ld_bias_tokens, const float* bias, int64_t ld_bias, int M,
+                      const uint32_t* allowed, int64_t ld_allowed, void* stream);
 
 /*
  * One token per row of float32 logits (rows ld apart) from the row's uniform
