@@ -14,6 +14,12 @@
 
 namespace alv {
 
+int shared8_simple(const uint16_t* q, int64_t ld_q, const void* kpages, const void* vpages, int64_t k_stride, int64_t v_stride,
+                   const uint8_t* scales, int64_t s_stride, int pages, int page_size, const int32_t* page_table,
+                   int64_t ld_table, int max_pages, const int32_t* q_start, const int32_t* kv_len, int B, int T, int max_q,
+                   const int32_t* group_start, const int32_t* shared_len, int groups, int heads, int kv_heads, int D,
+                   int window, int sinks, float scale, uint16_t* out, int64_t ld_out, void* stream);
+
 namespace {
 
 struct SimpleArgs {
@@ -165,25 +171,16 @@ extern "C" int alv_attention_paged8(const uint16_t* q, int64_t ld_q, const uint8
     return attention_simple(a, true, page_table, ld_table, max_pages, q_start, kv_len, B, T, pages, page_size, max_q, D, stream);
 }
 
-extern "C" uint64_t alv_attention_shared_workspace(int heads, int kv_heads, int D, int B, int T, int max_q, int groups) {
-    return 0;
-}
-
-extern "C" int alv_attention_shared(const uint16_t* q, int64_t ld_q, const void* kpages, const void* vpages, int64_t k_stride,
-                                    int64_t v_stride, const uint8_t* scales, int64_t s_stride, int pages, int page_size,
-                                    const int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* q_start,
-                                    const int32_t* kv_len, int B, int T, int max_q, const int32_t* group_start,
-                                    const int32_t* shared_len, int groups, int heads, int kv_heads, int D, int window,
-                                    int sinks, float scale, uint16_t* out, int64_t ld_out, void* workspace,
-                                    uint64_t workspace_bytes, void* stream) {
-    if (groups < 0 || (groups > 0 && (!group_start || !shared_len))) return fail(ALV_ERR_ARG, "bad groups: %d", groups);
-    if (reinterpret_cast<uintptr_t>(group_start) % 4 || reinterpret_cast<uintptr_t>(shared_len) % 4)
-        return fail(ALV_ERR_ALIGN, "group_start and shared_len need 4-byte alignment");
+int alv::shared8_simple(const uint16_t* q, int64_t ld_q, const void* kpages, const void* vpages, int64_t k_stride,
+                        int64_t v_stride, const uint8_t* scales, int64_t s_stride, int pages, int page_size,
+                        const int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* q_start,
+                        const int32_t* kv_len, int B, int T, int max_q, const int32_t* group_start,
+                        const int32_t* shared_len, int groups, int heads, int kv_heads, int D, int window, int sinks,
+                        float scale, uint16_t* out, int64_t ld_out, void* stream) {
     SimpleArgs a{};
     a.gr = PagedGroups{group_start, shared_len, groups};
     a.q = q, a.ld_q = ld_q, a.kpages = kpages, a.vpages = vpages, a.k_stride = k_stride, a.v_stride = v_stride;
     a.scales = scales, a.s_stride = s_stride, a.heads = heads, a.kv_heads = kv_heads, a.window = window, a.sinks = sinks;
     a.scale = scale, a.out = out, a.ld_out = ld_out;
-    return attention_simple(a, scales != nullptr, page_table, ld_table, max_pages, q_start, kv_len, B, T, pages, page_size,
-                            max_q, D, stream);
+    return attention_simple(a, true, page_table, ld_table, max_pages, q_start, kv_len, B, T, pages, page_size, max_q, D, stream);
 }

@@ -532,7 +532,7 @@ int alv_attention_paged8(const uint16_t* q, int64_t ld_q, const uint8_t* kpages,
  * sequences group_start[j] .. group_start[j + 1] - 1 (groups + 1 entries, not
  * decreasing); the first shared_len[j] positions of each, whole pages of them and
  * no more than the group's first sequence has, are those of its first sequence:
- * the others' table entries for them are not read. A sequence in no group shares
+ * the others' table entries for them do not matter. A sequence in no group shares
  * nothing. group_start and shared_len are int32 device memory, read by the
  * kernels. Every row sees what alv_attention_paged lets it see; what the two
  * parts of a row give is joined by their maxima and sums in float32, so its last
