@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "paged.h"
 #include "q4_device.h"
@@ -41,9 +42,11 @@ struct PagedAttnArgs {
     PagedGroups gr;
     const uint16_t* q;
     int64_t ld_q;
-    const uint16_t* kpages;
-    const uint16_t* vpages;
+    const void* kpages;  // bf16, or codes (E8)
+    const void* vpages;
     int64_t k_stride, v_stride;
+    const uint8_t* scales;
+    int64_t s_stride;
     int heads, kv_heads, g;
     int window, sinks;
     float scale;
@@ -59,8 +62,13 @@ struct PagedAttnArgs {
     float* pre_ml;      // and its maximum and sum
 };
 
+template <bool E8>
+using PageValue = std::conditional_t<E8, uint8_t, uint16_t>;
+
 typedef short s16x4 __attribute__((__vector_size__(4 * sizeof(short))));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+typedef int i32x2 __attribute__((__vector_size__(2 * sizeof(int))));
+typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
 
 // ---- the matrix products' operands ---------------------------------------------------
 //
@@ -82,6 +90,15 @@ __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, uint32_t vo
                  : "v"(voff), "s"(r), "s"(soff), "s"(lds)
                  : "memory", "m0");
 }
+// The same of 4 bytes for each of the first N lanes.
+template <int N>
+__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds) {
+    if ((threadIdx.x & 63) < N)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                     :
+                     : "v"(voff), "s"(r), "s"(lds)
+                     : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // At most N of this wave's loads are still in flight.
@@ -91,7 +108,7 @@ __device__ __forceinline__ void wait_vm() {
 }
 
 // A buffer over [base, base + bytes), the same for the whole wave.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t wave_rsrc(const uint16_t* base, uint32_t bytes) {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t wave_rsrc(const void* base, uint32_t bytes) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
     const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
@@ -161,6 +178,56 @@ __device__ __forceinline__ constexpr uint32_t piece_far(int c) {
 
 __device__ __forceinline__ s16x4 read_tr(const unsigned char* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
+}
+
+// ---- 8-bit pages ---------------------------------------------------------------------
+//
+// Codes become bf16 operands in registers (two per instruction; e4m3's four bits fit
+// bf16's eight, so nothing is rounded). K's power is a factor of its score, V's of
+// the weight that multiplies it; where a workgroup shares tiles they go into the
+// conversion instead, a power of two being exact there too.
+
+// Eight codes times a power of two.
+__device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float power) {
+    typedef __bf16 bf16x2 __attribute__((__vector_size__(2 * sizeof(__bf16))));
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, true);
+    return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2,
+                                   3, 4, 5, 6, 7);
+}
+
+// The power of two of byte i of a word of biased exponents.
+template <int I>
+__device__ __forceinline__ float power_of_byte(uint32_t w) {
+    const uint32_t b = I == 3 ? w >> 1 : w << (23 - 8 * I);
+    return __builtin_bit_cast(float, b & 0x7F800000u);
+}
+
+// The streaming kernel keeps codes in LDS, 32 positions of a wave at a time; a row's
+// 16-byte pieces (D / 16) stand at (piece ^ swizzle of the row): the 16 rows (of 32)
+// that K's reads and the 32 (0 .. 3, 16 .. 19, 4 .. 7, 20 .. 23 by the first half of
+// the lanes) that V's touch at once then fall on different banks.
+template <int D>
+__device__ __forceinline__ constexpr int k8_swz(int row) {
+    return D == 64 ? (row >> 2) & 3 : (D == 128 ? (row >> 1) & 7 : row & 15);
+}
+template <int D>
+__device__ __forceinline__ constexpr int v8_swz(int row) {
+    return D == 64 ? ((row >> 2) & 1) | ((row >> 3) & 2)
+                   : (D == 128 ? ((row >> 1) & 3) | ((row >> 2) & 4) : (row & 7) | ((row >> 1) & 8));
+}
+template <int D>
+__device__ __forceinline__ constexpr uint32_t piece8(int c) {
+    return (c & (D >= 256 ? 15 : D / 16 - 1)) * 16;
+}
+template <int D>
+__device__ __forceinline__ constexpr uint32_t piece8_far(int c) {
+    return (c & ~(D >= 256 ? 15 : D / 16 - 1)) * 16;
+}
+__device__ __forceinline__ i32x2 read_tr8(const unsigned char* p) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(p));
 }
 
 // What a row sees of its launch's positions: from .. cap, of these the window of its
@@ -359,10 +426,11 @@ constexpr float kSlack = 8.0f;
 // value of V that is infinite or NaN to every row they compute, seen or not (0
 // times it is NaN, and no later step makes that a number again); a wave that ends
 // with such an output does its rows again with this.
-template <int D>
+template <int D, bool E8>
 __device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16_t* q, const Sight pos, int us, int ulo, int unit,
                           int u0, int u1, int lane, float (&acc)[D / 64], float& m, float& l) {
     constexpr int RW = D / 64;
+    using T = PageValue<E8>;
     const float c = fmaxf(a.scale * kLog2e, kMinScale);
     m = kNoMax;
     l = 0.0f;
@@ -374,19 +442,31 @@ __device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16
             const int p = pb + lane;
             int page = -1;
             if (p < base + unit && sees(a, p, pos)) page = page_of(a.b, seq, p);
-            float s = -__builtin_inff();
-            const int64_t off = (((int64_t)kvh << a.b.shift) + (p & ((1 << a.b.shift) - 1))) * D;
+            float s = -__builtin_inff(), up = 1.0f;
+            const int64_t slot = ((int64_t)kvh << a.b.shift) + (p & ((1 << a.b.shift) - 1));
             if (page >= 0) {
-                const u32x4* k = reinterpret_cast<const u32x4*>(a.kpages + page * a.k_stride + off);
+                const T* row = static_cast<const T*>(a.kpages) + page * a.k_stride + slot * D;
                 s = 0.0f;
                 for (int i = 0; i < D / 8; ++i) {
-                    const u32x4 kv = k[i], qv = reinterpret_cast<const u32x4*>(q)[i];
+                    const u32x4 qv = reinterpret_cast<const u32x4*>(q)[i];
+                    u32x4 kv;
+                    if constexpr (E8) {
+                        const uint2 codes = reinterpret_cast<const uint2*>(row)[i];
+                        kv = __builtin_bit_cast(u32x4, widen8(codes.x, codes.y, 1.0f));
+                    } else {
+                        kv = reinterpret_cast<const u32x4*>(row)[i];
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t kw = kv[e], qw = qv[e];
                         s = __builtin_fmaf(bf16_bits_to_f32(kw & 0xFFFFu), bf16_bits_to_f32(qw & 0xFFFFu), s);
                         s = __builtin_fmaf(bf16_bits_to_f32(kw >> 16), bf16_bits_to_f32(qw >> 16), s);
                     }
+                }
+                if constexpr (E8) {
+                    const uint32_t e = *reinterpret_cast<const uint16_t*>(a.scales + page * a.s_stride + 2 * slot);
+                    s *= power_of_byte<0>(e);
+                    up = power_of_byte<1>(e);
                 }
             }
             float top = s;
@@ -398,13 +478,15 @@ __device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16
             l = l * fac + sum;
 #pragma unroll
             for (int e = 0; e < RW; ++e) acc[e] *= fac;
+            if constexpr (E8) w *= up;
             for (uint64_t left = __ballot(page >= 0); left; left &= left - 1) {
                 const int j = __builtin_ctzll(left), pj = pb + j;
                 const float wj = __shfl(w, j);
-                const uint16_t* v = a.vpages + __shfl(page, j) * a.v_stride +
-                                    (((int64_t)kvh << a.b.shift) + (pj & ((1 << a.b.shift) - 1))) * D + RW * lane;
+                const T* v = static_cast<const T*>(a.vpages) + __shfl(page, j) * a.v_stride +
+                             (((int64_t)kvh << a.b.shift) + (pj & ((1 << a.b.shift) - 1))) * D + RW * lane;
 #pragma unroll
-                for (int e = 0; e < RW; ++e) acc[e] = __builtin_fmaf(wj, bf16_bits_to_f32(v[e]), acc[e]);
+                for (int e = 0; e < RW; ++e)
+                    acc[e] = __builtin_fmaf(wj, E8 ? __builtin_amdgcn_cvt_f32_fp8(v[e], 0) : bf16_bits_to_f32(v[e]), acc[e]);
             }
         }
     }
@@ -440,21 +522,23 @@ struct RowsSeq {
 };
 
 constexpr int rows_waves(int D) { return D == 512 ? 2 : (D == 64 ? 8 : 4); }
-constexpr int rows_stage(int D) { return 64 * D; }  // bytes of 16 positions' K and V
-constexpr int rows_stages(int D) { return 131072 / (rows_waves(D) * rows_stage(D)); }
-constexpr int rows_unit(int D) { return 16 * rows_waves(D); }
+// A wave's block: 16 positions' K and V, or 32 of 8-bit ones and their powers.
+constexpr int rows_block(bool E8) { return E8 ? 32 : 16; }
+constexpr int rows_stage(int D, bool E8) { return 64 * D + (E8 ? 64 : 0); }
+constexpr int rows_stages(int D) { return 131072 / (rows_waves(D) * 64 * D); }
+constexpr int rows_unit(int D, bool E8) { return rows_block(E8) * rows_waves(D); }
 // The waves' outputs at a tile's end, rows padded to spread over the banks.
 constexpr int rows_out_ld(int D) { return D + 4; }
 // Whether q's operands stay in LDS rather than registers: where they and the
 // output take more than half of a wave's 256 (the rest would spill).
 constexpr bool rows_q_lds(int D, int QT) { return QT * D > 256; }
-constexpr int rows_lds(int D, int QT) {
-    const int ring = rows_waves(D) * rows_stages(D) * rows_stage(D);
+constexpr int rows_lds(int D, int QT, bool E8) {
+    const int ring = rows_waves(D) * rows_stages(D) * rows_stage(D, E8);
     const int outs = rows_waves(D) * 16 * QT * (rows_out_ld(D) * 4);
     return (ring > outs ? ring : outs) + 2 * rows_waves(D) * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0) + 16;
 }
-constexpr int rows_mls(int D, int QT) {  // where the waves' maxima and sums stand; q behind them
-    return rows_lds(D, QT) - 16 - 2 * rows_waves(D) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
+constexpr int rows_mls(int D, int QT, bool E8) {  // where the waves' maxima and sums stand; q behind them
+    return rows_lds(D, QT, E8) - 16 - 2 * rows_waves(D) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
 }
 // Floats of one workspace place: outputs, maxima, sums.
 constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
@@ -590,13 +674,17 @@ __device__ __forceinline__ uint32_t part_count(uint64_t total, const Scan& sc, i
     return (uint32_t)min(min((uint64_t)grid, (uint64_t)sc.tiles * kPartsPerTile), total);
 }
 
-template <int D, int QT, int MODE>
+template <int D, int QT, bool E8, int MODE>
 __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kernel(PagedAttnArgs a) {
-    constexpr int NW = rows_waves(D), NS = rows_stages(D), UNIT = rows_unit(D), ROWS = 16 * QT;
-    constexpr int NC = D / 8;             // 16-byte pieces of a row
-    constexpr int NI = D / 32;            // loads of 64 pieces for 16 positions of K (of V)
-    constexpr int HALF = 32 * D;          // bytes of 16 positions' K
-    constexpr int RPL = 512 / D;          // rows of one load
+    constexpr int NW = rows_waves(D), NS = rows_stages(D), UNIT = rows_unit(D, E8), ROWS = 16 * QT;
+    constexpr int BP = rows_block(E8), NH = BP / 16;  // positions of a block, 16 at a time (within a page)
+    constexpr int STAGE = rows_stage(D, E8);
+    constexpr int NC = E8 ? D / 16 : D / 8;  // 16-byte pieces of a row
+    constexpr int NI = NC / 4;            // loads of 64 pieces for 16 positions of K (of V)
+    constexpr int HALF = 32 * D;          // bytes of a block's K
+    constexpr int RPL = 64 / NC;          // rows of one load
+    constexpr int LOADS = NH * (2 * NI + E8);  // of a block
+    using T = PageValue<E8>;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -608,19 +696,22 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
     uint64_t x = cut.begin(blockIdx.x);
     const uint64_t end = cut.begin(blockIdx.x + 1);
 
-    unsigned char* ring = smem + wave * NS * rows_stage(D);
+    unsigned char* ring = smem + wave * NS * STAGE;
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
-    float* mls = reinterpret_cast<float*>(smem + rows_mls(D, QT));  // [wave][max | sum][row]
-    int* odds = reinterpret_cast<int*>(smem + rows_lds(D, QT) - 16);
+    float* mls = reinterpret_cast<float*>(smem + rows_mls(D, QT, E8));  // [wave][max | sum][row]
+    int* odds = reinterpret_cast<int*>(smem + rows_lds(D, QT, E8) - 16);
     const float c = fmaxf(a.scale * kLog2e, kMinScale);
     const int S = 1 << a.b.shift;
     // Byte offsets that stay: this lane's piece of a load (memory side), of a K
     // read and of a V read (LDS side).
-    const uint32_t dma_k = (lane / NC) * (2 * D) + ((lane % NC) ^ k_swz<D>(lane / NC)) * 16;
-    const uint32_t dma_v = (lane / NC) * (2 * D) + ((lane % NC) ^ v_swz<D>(lane / NC)) * 16;
-    const uint32_t rd_k = col * (2 * D) + (G ^ k_swz<D>(col)) * 16;
-    const int vrow = 4 * G + (col >> 2);
-    const uint32_t rd_v = vrow * (2 * D) + (((col >> 1) & 1) ^ v_swz<D>(vrow)) * 16 + (col & 1) * 8;
+    constexpr auto kz = [](int row) { return E8 ? k8_swz<D>(row) : k_swz<D>(row); };
+    constexpr auto vz = [](int row) { return E8 ? v8_swz<D>(row) : v_swz<D>(row); };
+    const uint32_t dma_k = (lane / NC) * (16 * NC) + ((lane % NC) ^ kz(lane / NC)) * 16;
+    const uint32_t dma_v = (lane / NC) * (16 * NC) + ((lane % NC) ^ vz(lane / NC)) * 16;
+    const uint32_t rd_k = col * (16 * NC) + (G ^ kz(col)) * 16;
+    // V's transposing reads: 4 rows of a lane group's, or 8, the ones whose scores it has.
+    const int vrow = E8 ? 4 * G + (col >> 1 & 3) + 16 * (col >> 3) : 4 * G + (col >> 2);
+    const uint32_t rd_v = vrow * (16 * NC) + ((E8 ? 0 : (col >> 1) & 1) ^ vz(vrow)) * 16 + (col & 1) * 8;
 
     while (x < end) {
         const Found f = scan_find<ROWS, UNIT, MODE>(a, lane, sc, x);
@@ -630,38 +721,48 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
         const int nblk = f.s.len > 0 ? u1 - u0 : 0;  // this wave's blocks
         auto block_pos = [&](int j) {
             const int u = u0 + j;
-            return (u < f.s.us ? u : u - f.s.us + f.s.ulo) * UNIT + 16 * wave;
+            return (u < f.s.us ? u : u - f.s.us + f.s.ulo) * UNIT + BP * wave;
         };
         // The pages of this wave's blocks, 64 at a time, one per lane.
         const int32_t* table = a.b.table + (int64_t)f.seq * a.b.ld_table;
-        int pages = -1, pages0 = 0;
-        uint32_t gone_bits = 0;  // by buffer: its page is missing
+        int pages[NH], pages0 = 0;
+        uint32_t gone_bits = 0;  // by buffer: its page (of the first 16, of the others) is missing
         auto load_pages = [&](int j0) {
             pages0 = j0;
-            const int j = j0 + lane, p = block_pos(j);
-            pages = j < nblk && p < f.s.len ? table[p >> a.b.shift] : -1;
-            if ((unsigned)pages >= (unsigned)a.b.pages) pages = -1;
+            const int j = j0 + lane;
+#pragma unroll
+            for (int hf = 0; hf < NH; ++hf) {
+                const int p = block_pos(j) + 16 * hf;
+                pages[hf] = j < nblk && p < f.s.len ? table[p >> a.b.shift] : -1;
+                if ((unsigned)pages[hf] >= (unsigned)a.b.pages) pages[hf] = -1;
+            }
         };
-        auto page_at = [&](int j) { return __builtin_amdgcn_readlane(pages, j - pages0); };
         auto issue = [&](int j) {
             if (j - pages0 >= 64) load_pages(j);
-            const int page = page_at(j), p = block_pos(j);
-            // Past the sequence's end, and where the page is missing, zeros arrive.
-            const uint32_t bytes = page < 0 ? 0u : (uint32_t)max(0, min(16, f.s.len - p)) * (2 * D);
-            const int64_t off = (((int64_t)f.kvh << a.b.shift) + (p & (S - 1))) * D;
-            const __amdgpu_buffer_rsrc_t rk = wave_rsrc(a.kpages + max(page, 0) * a.k_stride + off, bytes);
-            const __amdgpu_buffer_rsrc_t rv = wave_rsrc(a.vpages + max(page, 0) * a.v_stride + off, bytes);
-            gone_bits = (gone_bits & ~(1u << (j % NS))) | ((uint32_t)(page < 0) << (j % NS));
-            const uint32_t dst = ring_lds + (uint32_t)(j % NS) * rows_stage(D);
-            // Load i brings rows RPL i .. of RPL each; the swizzles are exclusive
-            // ors of the row's bits, so the lane's offset within the rows of one
-            // load serves all, with the load's own bits applied.
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-                load_lds16(rk, dma_k ^ (k_swz<D>(RPL * i) * 16), 1024 * i, dst + 1024 * i);
+            for (int hf = 0; hf < NH; ++hf) {
+                const int page = __builtin_amdgcn_readlane(pages[hf], j - pages0), p = block_pos(j) + 16 * hf;
+                // Past the sequence's end, and where the page is missing, zeros arrive.
+                const uint32_t bytes = page < 0 ? 0u : (uint32_t)max(0, min(16, f.s.len - p)) * (16 * NC);
+                const int64_t slot = ((int64_t)f.kvh << a.b.shift) + (p & (S - 1));
+                const __amdgpu_buffer_rsrc_t rk = wave_rsrc(static_cast<const T*>(a.kpages) + max(page, 0) * a.k_stride + slot * D, bytes);
+                const __amdgpu_buffer_rsrc_t rv = wave_rsrc(static_cast<const T*>(a.vpages) + max(page, 0) * a.v_stride + slot * D, bytes);
+                const int bit = NH * (j % NS) + hf;
+                gone_bits = (gone_bits & ~(1u << bit)) | ((uint32_t)(page < 0) << bit);
+                const uint32_t dst = ring_lds + (uint32_t)(j % NS) * STAGE + hf * (16 * D);
+                // Load i brings rows RPL i .. of RPL each; the swizzles are exclusive
+                // ors of the row's bits, so the lane's offset within the rows of one
+                // load serves all, with the load's own bits applied.
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-                load_lds16(rv, dma_v ^ (v_swz<D>(RPL * i) * 16), 1024 * i, dst + HALF + 1024 * i);
+                for (int i = 0; i < NI; ++i)
+                    load_lds16(rk, dma_k ^ (kz(16 * hf + RPL * i) * 16), 1024 * i, dst + 1024 * i);
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    load_lds16(rv, dma_v ^ (vz(16 * hf + RPL * i) * 16), 1024 * i, dst + HALF + 1024 * i);
+                if constexpr (E8)  // the slots' 16 pairs of powers
+                    load_lds4<8>(wave_rsrc(a.scales + max(page, 0) * a.s_stride + 2 * slot, bytes ? 32 : 0), lane * 4,
+                                 ring_lds + (uint32_t)(j % NS) * STAGE + 64 * D + 32 * hf);
+            }
         };
 
         // This lane's rows of q, the B operand: row col of each 16, 8 columns of each 32.
@@ -669,7 +770,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
         int row_t[QT];
         constexpr bool QL = rows_q_lds(D, QT);
         bf16x8 q[QL ? 1 : QT][QL ? 1 : D / 32];
-        u32x4* qs = reinterpret_cast<u32x4*>(smem + rows_mls(D, QT) + 2 * NW * ROWS * 4) + lane;
+        u32x4* qs = reinterpret_cast<u32x4*>(smem + rows_mls(D, QT, E8) + 2 * NW * ROWS * 4) + lane;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const int r = min(16 * t + col, nrows - 1) + f.rt * ROWS;
@@ -677,13 +778,15 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
             row_t[t] = f.s.first + tok;
             pos[t].pos = pos[t].cap = f.s.len - f.s.n + tok;
             pos[t].from = MODE == kSuf ? f.s.from : 0;
-            const uint16_t* qr = a.q + (int64_t)(f.s.first + tok) * a.ld_q + h * D + 8 * G;
+            // (of codes, 16 bytes of a lane's are two operands: 16 columns of each 64)
+            const uint16_t* qr = a.q + (int64_t)(f.s.first + tok) * a.ld_q + h * D + (E8 ? 16 : 8) * G;
+            constexpr auto q_at = [](int i) { return E8 ? 64 * (i / 2) + 8 * (i % 2) : 32 * i; };
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
                 if constexpr (QL) {
-                    if (i % NW == wave) qs[(t * (D / 32) + i) * 64] = *reinterpret_cast<const u32x4*>(qr + 32 * i);
+                    if (i % NW == wave) qs[(t * (D / 32) + i) * 64] = *reinterpret_cast<const u32x4*>(qr + q_at(i));
                 } else {
-                    q[t][i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qr + 32 * i));
+                    q[t][i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qr + q_at(i)));
                 }
             }
         }
@@ -728,42 +831,79 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
         for (int j = 0; j < nblk; ++j) {
             // Blocks j + 1 .. j + NS - 1 may be in flight.
             if (j + NS <= nblk)
-                wait_vm<(NS - 1) * 2 * NI>();
+                wait_vm<(NS - 1) * LOADS>();
             else
                 wait_vm<0>();
-            const unsigned char* kt = ring + (j % NS) * rows_stage(D);
+            const unsigned char* kt = ring + (j % NS) * STAGE;
             const unsigned char* vt = kt + HALF;
-            f32x4 s[QT];
+            f32x4 s[NH][QT];
+            constexpr int KB = QT * D >= 512 ? (QT == 4 ? 1 : 2) : 0;  // K reads of codes at once, where registers are short
+            [[maybe_unused]] i32x2 powers[NH];  // of this lane's positions: k's, v's in turn
 #pragma unroll
-            for (int t = 0; t < QT; ++t) s[t] = f32x4{0, 0, 0, 0};
+            for (int hf = 0; hf < NH; ++hf) {
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const bf16x8 k = __builtin_bit_cast(
-                    bf16x8, *reinterpret_cast<const u32x4*>(kt + (rd_k ^ piece<D>(4 * i)) + piece_far<D>(4 * i)));
+                for (int t = 0; t < QT; ++t) s[hf][t] = f32x4{0, 0, 0, 0};
+                auto product = [&](bf16x8 k, int i) __attribute__((always_inline)) {
 #pragma unroll
-                for (int t = 0; t < QT; ++t) {
-                    if constexpr (QL)
-                        s[t] = mfma16x16x32(k, __builtin_bit_cast(bf16x8, qs[(t * (D / 32) + i) * 64]), s[t]);
-                    else
-                        s[t] = mfma16x16x32(k, q[t][i], s[t]);
+                    for (int t = 0; t < QT; ++t) {
+                        if constexpr (QL)
+                            s[hf][t] = mfma16x16x32(k, __builtin_bit_cast(bf16x8, qs[(t * (D / 32) + i) * 64]), s[hf][t]);
+                        else
+                            s[hf][t] = mfma16x16x32(k, q[t][i], s[hf][t]);
+                    }
+                };
+                if constexpr (E8) {
+                    powers[hf] = *reinterpret_cast<const i32x2*>(kt + 64 * D + 32 * hf + 8 * G);
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i) {
+                        if (KB > 0 && i % KB == 0) asm volatile("" ::: "memory");
+                        const u32x4 k = *reinterpret_cast<const u32x4*>(kt + hf * (16 * D) + (rd_k ^ piece8<D>(4 * i)) + piece8_far<D>(4 * i));
+                        product(widen8(k[0], k[1], 1.0f), 2 * i);
+                        product(widen8(k[2], k[3], 1.0f), 2 * i + 1);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)
+                        product(__builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
+                                                               kt + (rd_k ^ piece<D>(4 * i)) + piece_far<D>(4 * i))), i);
+                }
+            }
+            float vp[NH][4];  // V's powers
+            if constexpr (E8) {
+#pragma unroll
+                for (int hf = 0; hf < NH; ++hf) {
+                    const uint32_t p0 = powers[hf][0], p1 = powers[hf][1];
+                    const f32x4 kp{power_of_byte<0>(p0), power_of_byte<2>(p0), power_of_byte<0>(p1), power_of_byte<2>(p1)};
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) s[hf][t] *= kp;
+                    vp[hf][0] = power_of_byte<1>(p0), vp[hf][1] = power_of_byte<3>(p0);
+                    vp[hf][2] = power_of_byte<1>(p1), vp[hf][3] = power_of_byte<3>(p1);
                 }
             }
             const int p0 = block_pos(j);
-            const bool gone = (gone_bits >> (j % NS)) & 1;
-            const bool masked = gone || p0 + 15 > pos_lo || (MODE == kSuf && p0 < f.s.from) ||
-                                (a.window > 0 && p0 <= pos_hi - a.window && p0 + 15 >= a.sinks);
+            const uint32_t gone = gone_bits >> (NH * (j % NS)) & ((1u << NH) - 1);
+            const bool masked = gone || p0 + BP - 1 > pos_lo || (MODE == kSuf && p0 < f.s.from) ||
+                                (a.window > 0 && p0 <= pos_hi - a.window && p0 + BP - 1 >= a.sinks);
             if (masked) {
 #pragma unroll
-                for (int t = 0; t < QT; ++t)
+                for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!sees(a, p0 + 4 * G + i, pos[t]) || gone) s[t][i] = -__builtin_inff();
+                    for (int t = 0; t < QT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!sees(a, p0 + 16 * hf + 4 * G + i, pos[t]) || (gone >> hf & 1)) s[hf][t][i] = -__builtin_inff();
             }
-            s16x4 pw[QT];
+            typedef __bf16 Weights __attribute__((__vector_size__(4 * NH * sizeof(__bf16))));
+            Weights pw[QT];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float s0 = s[t][0], s1 = s[t][1], s2 = s[t][2], s3 = s[t][3];
-                const float top = fmaxf(fmaxf(s0, s1), fmaxf(s2, s3));
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int hf = 0; hf < NH; ++hf) {
+                    const float s0 = s[hf][t][0], s1 = s[hf][t][1], s2 = s[hf][t][2], s3 = s[hf][t][3];
+                    const float most = fmaxf(fmaxf(s0, s1), fmaxf(s2, s3));
+                    top = hf ? fmaxf(top, most) : most;
+                }
                 if (__any(__builtin_fmaf(top, c, -m[t]) > kSlack)) {
                     const float mn = fmaxf(m[t], max_groups(top) * c);
                     const float fac = __builtin_amdgcn_exp2f(m[t] - mn);
@@ -772,32 +912,49 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d) o[t][d] *= fac;
                 }
-                const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s0, c, -m[t]));
-                const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s1, c, -m[t]));
-                const float w2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s2, c, -m[t]));
-                const float w3 = __builtin_amdgcn_exp2f(__builtin_fmaf(s3, c, -m[t]));
-                l[t] += (w0 + w1) + (w2 + w3);
                 // Weights as bf16, the matrix cores' type: half a step, 2^-8
                 // relative each, as much as the output's own rounding (the outputs'
                 // mean error against 64 bits: 0.0021 to 0.0024, of which their own
                 // rounding is 0.0017).
-                pw[t] = pack4(w0, w1, w2, w3);
+#pragma unroll
+                for (int hf = 0; hf < NH; ++hf) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float si = s[hf][t][i];
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(si, c, -m[t]));
+                    }
+                    l[t] += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) pw[t][4 * hf + i] = (__bf16)(E8 ? w[i] * vp[hf][i] : w[i]);
+                }
             }
             auto read_v = [&](int d) __attribute__((always_inline)) {
-                return read_tr(vt + (rd_v ^ piece<D>(2 * d)) + piece_far<D>(2 * d));
+                if constexpr (E8)
+                    return read_tr8(vt + (rd_v ^ piece8<D>(d)) + piece8_far<D>(d));
+                else
+                    return read_tr(vt + (rd_v ^ piece<D>(2 * d)) + piece_far<D>(2 * d));
             };
-            constexpr int VB = D / 16 < 8 ? D / 16 : 8;  // V reads on their way at once
+            constexpr int VB = D / 16 < 8 ? D / 16 : (E8 && QT * D >= 512 ? (QT == 4 ? 2 : 4) : 8);  // V reads on their way at once
 #pragma unroll
             for (int d0 = 0; d0 < D / 16; d0 += VB) {
-                s16x4 v[VB];
+                std::conditional_t<E8, i32x2, s16x4> v[VB];
 #pragma unroll
                 for (int d = 0; d < VB; ++d) v[d] = read_v(d0 + d);
                 asm volatile("" ::: "memory");
 #pragma unroll
-                for (int d = 0; d < VB; ++d)
+                for (int d = 0; d < VB; ++d) {
+                    if constexpr (E8) {
+                        const bf16x8 vb = widen8(v[d][0], v[d][1], 1.0f);
 #pragma unroll
-                    for (int t = 0; t < QT; ++t)
-                        o[t][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v[d], pw[t], o[t][d0 + d], 0, 0, 0);
+                        for (int t = 0; t < QT; ++t) o[t][d0 + d] = mfma16x16x32(vb, pw[t], o[t][d0 + d]);
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < QT; ++t)
+                            o[t][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v[d], __builtin_bit_cast(s16x4, pw[t]),
+                                                                                     o[t][d0 + d], 0, 0, 0);
+                    }
+                }
             }
             // The buffer's reads are done before it is filled again.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -839,7 +996,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
                     row_positions<1>(a, f.seq, f.s.from, one, p);
                     at.pos = p[0], at.cap = min(p[0], f.s.len - 1);
                 }
-                plain_row<D>(a, f.seq, f.kvh, a.q + (int64_t)(f.s.first + tok) * a.ld_q + h * D, at, f.s.us, f.s.ulo, UNIT, u0, u1,
+                plain_row<D, E8>(a, f.seq, f.kvh, a.q + (int64_t)(f.s.first + tok) * a.ld_q + h * D, at, f.s.us, f.s.ulo, UNIT, u0, u1,
                              lane, acc, mr, lr);
                 if (whole) {
                     finish_row<D, MODE>(a, f.s.first + tok, h, lane, acc, mr, lr, f.s.from > 0);
@@ -933,9 +1090,9 @@ __device__ __forceinline__ void join_parts(int n, int lane, ML ml, int gap, O o,
 
 // The cut tiles: wave (boundary, row) joins the parts of the tile in which
 // boundary blockIdx.x + 1 is the first, in the order of the line.
-template <int D, int QT, int MODE>
+template <int D, int QT, bool E8, int MODE>
 __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArgs a, int grid) {
-    constexpr int UNIT = rows_unit(D), ROWS = 16 * QT, RW = D / 64;
+    constexpr int UNIT = rows_unit(D, E8), ROWS = 16 * QT, RW = D / 64;
     const int lane = threadIdx.x & 63;
     const int r = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
     Scan sc;
@@ -1145,7 +1302,7 @@ __device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, i
     return INT_MAX / 2;
 }
 
-template <int D, int MODE>
+template <int D, bool E8, int MODE>
 __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan& sc0, int gt, int kvh, int split, int nsplit, int entry, int* tab, unsigned char* smem) {
     constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D);
     constexpr int DW = D / DS;            // this wave's columns of the output (and of its scores' products)
@@ -1199,7 +1356,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     const uint32_t dma_k = (lane / NC) * (2 * D) + ((lane % NC) ^ k_swz<D>(wave * LR + lane / NC)) * 16;
     const uint32_t dma_v = (lane / NC) * (2 * D) + ((lane % NC) ^ v_swz<D>(wave * LR + lane / NC)) * 16;
     // Starts unit u's K (then its V) on the way to LDS; K before V, units in order.
-    auto issue = [&](int u, bool v) __attribute__((always_inline)) {
+    [[maybe_unused]] auto issue = [&](int u, bool v) __attribute__((always_inline)) {
         if (u - pages0 >= 64) load_pages(u);
         const int page = __builtin_amdgcn_readlane(pages, u - pages0), p = unit_pos(u) + wave * LR;
         const uint32_t bytes = page < 0 ? 0u : (uint32_t)max(0, min(LR, len - p)) * (2 * D);
@@ -1211,13 +1368,57 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
             const int at = NB * (u & 3);
             holes = (holes & ~(((1u << NB) - 1) << at)) | (now << at);
         }
-        const uint16_t* src = v ? a.vpages + max(page, 0) * a.v_stride : a.kpages + max(page, 0) * a.k_stride;
+        const uint16_t* src = v ? static_cast<const uint16_t*>(a.vpages) + max(page, 0) * a.v_stride
+                                : static_cast<const uint16_t*>(a.kpages) + max(page, 0) * a.k_stride;
         const __amdgpu_buffer_rsrc_t r = wave_rsrc(src + off, bytes);
         const uint32_t dst = (v ? vb_lds : kb_lds) + (u & 1) * TB, at = here(v ? dma_v : dma_k);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const uint32_t x = v ? (uint32_t)v_swz<D>(RPL * i) : (uint32_t)k_swz<D>(RPL * i);
             load_lds16(r, at ^ (x * 16), 1024 * i, dst + 1024 * i);
+        }
+    };
+
+    // 8-bit pages: a wave's share of a unit goes through registers, where codes become
+    // bf16 times their power, so that what LDS holds and the products are the same.
+    constexpr int NP = E8 ? LR * D / 1024 : 1;  // pieces of 16 codes of a lane, of K (of V)
+    struct Codes {
+        u32x4 c[NP];
+        int e[NP];
+    };
+    [[maybe_unused]] auto fetch = [&](int u, bool v, Codes& x) __attribute__((always_inline)) {
+        if (u - pages0 >= 64) load_pages(u);
+        const int page = __builtin_amdgcn_readlane(pages, u - pages0), p = unit_pos(u) + wave * LR;
+        const uint32_t have = page < 0 ? 0u : (uint32_t)max(0, min(LR, len - p));
+        const int64_t slot = ((int64_t)kvh << a.b.shift) + (p & ((1 << a.b.shift) - 1));
+        if (!v) {
+            uint32_t now = 0;
+#pragma unroll
+            for (int k = 0; k < NB; ++k) now |= (uint32_t)(gone[k] >> (u - pages0) & 1) << k;
+            const int at = NB * (u & 3);
+            holes = (holes & ~(((1u << NB) - 1) << at)) | (now << at);
+        }
+        const uint8_t* src = v ? static_cast<const uint8_t*>(a.vpages) + max(page, 0) * a.v_stride
+                               : static_cast<const uint8_t*>(a.kpages) + max(page, 0) * a.k_stride;
+        const __amdgpu_buffer_rsrc_t r = wave_rsrc(src + slot * D, have * D);
+        const __amdgpu_buffer_rsrc_t rs = wave_rsrc(a.scales + max(page, 0) * a.s_stride + 2 * slot, have * 2);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const uint32_t at = 64 * i + lane;
+            x.c[i] = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * at, 0, 0);
+            x.e[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, at / (D / 16) * 2 + v, 0, 0);
+        }
+    };
+    [[maybe_unused]] auto commit = [&](int u, bool v, const Codes& x) __attribute__((always_inline)) {
+        unsigned char* buf = (v ? vbuf : kbuf) + (u & 1) * TB;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int at = 64 * i + lane, row = wave * LR + at / (D / 16), pc = 2 * (at % (D / 16));
+            const int z = v ? v_swz<D>(row) : k_swz<D>(row);
+            const float power = power_of_byte<0>(x.e[i]);
+            const uint32_t c0 = x.c[i][0], c1 = x.c[i][1], c2 = x.c[i][2], c3 = x.c[i][3];
+            *reinterpret_cast<bf16x8*>(buf + row * (2 * D) + (pc ^ z) * 16) = widen8(c0, c1, power);
+            *reinterpret_cast<bf16x8*>(buf + row * (2 * D) + ((pc + 1) ^ z) * 16) = widen8(c2, c3, power);
         }
     };
 
@@ -1355,19 +1556,43 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         if constexpr (DS == 1) __builtin_amdgcn_s_setprio(0);
     };
 
+    // (what is fetched is one unit ahead of what is in LDS, with DS = 2 one phase)
+    [[maybe_unused]] Codes kx, vx;
     if (u1 > u0) {
         load_pages(u0);
-        issue(u0, false);
-        issue(u0, true);
+        if constexpr (E8) {
+            fetch(u0, false, kx);
+            fetch(u0, true, vx);
+            commit(u0, false, kx);
+            if constexpr (DS == 1) {
+                commit(u0, true, vx);
+                if (u0 + 1 < u1) {
+                    fetch(u0 + 1, false, kx);
+                    fetch(u0 + 1, true, vx);
+                }
+            }
+        } else {
+            issue(u0, false);
+            issue(u0, true);
+        }
     }
     if constexpr (DS == 1) {
 #pragma unroll 1
         for (int u = u0; u < u1; ++u) {
-            wait_vm<0>();
+            if constexpr (!E8) wait_vm<0>();
             __syncthreads();
             if (u + 1 < u1) {
-                issue(u + 1, false);
-                issue(u + 1, true);
+                if constexpr (E8) {
+                    commit(u + 1, false, kx);
+                    commit(u + 1, true, vx);
+                    if (u + 2 < u1) {
+                        fetch(u + 2, false, kx);
+                        fetch(u + 2, true, vx);
+                    }
+                } else {
+                    issue(u + 1, false);
+                    issue(u + 1, true);
+                }
             }
             const int pt = unit_pos(u);
             const unsigned char* kt = kbuf + (u & 1) * TB;
@@ -1388,7 +1613,15 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         const int grp = wave / (NW / 2), nu = u1 - u0;
         f32x4* mine = reinterpret_cast<f32x4*>(xch + wave * 1024) + lane;
         const f32x4* other = reinterpret_cast<const f32x4*>(xch + (wave ^ 1) * 1024) + lane;
+        // (codes become LDS's one phase ahead: phase + 1's buffer has had its last reader
+        // two phases ago)
         auto begin = [&](int phase) __attribute__((always_inline)) {
+            if constexpr (E8) {
+                __syncthreads();
+                if (phase + 1 < 2 * nu) commit(u0 + ((phase + 1) >> 1), (phase + 1) & 1, vx);
+                if (phase + 2 < 2 * nu) fetch(u0 + ((phase + 2) >> 1), phase & 1, vx);
+                return;
+            }
             if (phase + 1 < 2 * nu)
                 wait_vm<NL>();  // the loads issued in the last phase may still be on their way
             else
@@ -1441,7 +1674,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
             const int rr = r0 + r, tk = rr / a.g, hd = kvh * a.g + rr % a.g;
             float acc[D / 64], mr, lr;
             const Sight at{__builtin_amdgcn_readlane(pos, r), __builtin_amdgcn_readlane(cap, r), MODE == kSuf ? from : 0};
-            plain_row<D>(a, seq, kvh, a.q + (int64_t)(first + tk) * a.ld_q + hd * D, at, sp.us, sp.ulo, BN, u0, u1, lane, acc,
+            plain_row<D, E8>(a, seq, kvh, a.q + (int64_t)(first + tk) * a.ld_q + hd * D, at, sp.us, sp.ulo, BN, u0, u1, lane, acc,
                          mr, lr);
             if (nsplit == 1) {
                 finish_row<D, MODE>(a, first + tk, hd, lane, acc, mr, lr, from > 0);
@@ -1481,7 +1714,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     }
 }
 
-template <int D, int MODE>
+template <int D, bool E8, int MODE>
 __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kernel(PagedAttnArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int TR = tile_rows(D), BN = tile_bn(D);
@@ -1529,7 +1762,7 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
         kvh = item - gt * a.kv_heads;
     }
     // (tiles of more rows than max_q told of may be more than tab has entries for: they are not split)
-    tile_item<D, MODE>(a, sc0, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), split ? a.tab : nullptr, smem);
+    tile_item<D, E8, MODE>(a, sc0, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), split ? a.tab : nullptr, smem);
 }
 
 // The parts of the tiles joined, `groups` workgroups to a tile, merge_rows(D) of
@@ -1669,25 +1902,25 @@ __attribute__((unused)) int allow_lds(const void* k, int lds, std::atomic<uint64
     return ALV_OK;
 }
 
-template <int D, int QT, int MODE>
+template <int D, int QT, bool E8, int MODE>
 int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    constexpr int lds = rows_lds(D, QT);
+    constexpr int lds = rows_lds(D, QT, E8);
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, MODE>), lds, done)) return rc;
-    hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, MODE>), dim3(p.grid), dim3(64 * rows_waves(D)), lds, s, a);
+    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, E8, MODE>), lds, done)) return rc;
+    hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MODE>), dim3(p.grid), dim3(64 * rows_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_rows_kernel launch")) return rc;
-    hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT, MODE>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a, p.grid);
+    hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT, E8, MODE>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a, p.grid);
     return hip_check(hipGetLastError(), "attn_paged_rows_merge_kernel launch");
 }
 
-template <int D, int MODE>
+template <int D, bool E8, int MODE>
 int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     constexpr int lds = tile_lds(D);
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D, MODE>), lds, done)) return rc;
-    hipLaunchKernelGGL((attn_paged_tile_kernel<D, MODE>), dim3((uint32_t)std::max(p.grid_tiles, (int64_t)p.slots * 2)), dim3(64 * tile_waves(D)), lds, s, a);
+    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D, E8, MODE>), lds, done)) return rc;
+    hipLaunchKernelGGL((attn_paged_tile_kernel<D, E8, MODE>), dim3((uint32_t)std::max(p.grid_tiles, (int64_t)p.slots * 2)), dim3(64 * tile_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_tile_kernel launch")) return rc;
     if (p.slots == 0) return ALV_OK;
     // Few tiles are joined by as many workgroups as they have rows for, many by fewer
@@ -1702,7 +1935,7 @@ int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     return hip_check(hipGetLastError(), "attn_paged_tile_merge_kernel launch");
 }
 
-template <int D, int MODE>
+template <int D, bool E8, int MODE>
 int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
     a.row_limit = p.row_limit;
     a.slots = p.slots;
@@ -1712,19 +1945,19 @@ int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
     if (p.grid_tiles) {
         if (p.slots) a.tab = reinterpret_cast<int*>(part + p.rows_bytes / sizeof(float));
         a.part = part + (p.rows_bytes + p.tab_bytes) / sizeof(float);
-        if (int rc = launch_tiles<D, MODE>(a, p, s)) return rc;
+        if (int rc = launch_tiles<D, E8, MODE>(a, p, s)) return rc;
     }
     a.part = part;
-    if (p.qt == 1) return launch_rows<D, 1, MODE>(a, p, s);
+    if (p.qt == 1) return launch_rows<D, 1, E8, MODE>(a, p, s);
     if constexpr (D <= 256)
-        if (p.qt == 2) return launch_rows<D, 2, MODE>(a, p, s);
+        if (p.qt == 2) return launch_rows<D, 2, E8, MODE>(a, p, s);
     if constexpr (D <= 128)
-        if (p.qt == 4) return launch_rows<D, 4, MODE>(a, p, s);
+        if (p.qt == 4) return launch_rows<D, 4, E8, MODE>(a, p, s);
     return ALV_OK;
 }
 
 // The arguments' checks that all attention entries share, and what they fill in of
-// `a` (which holds pools, strides, heads, window, sinks, scale and out). codes: 8-bit pages.
+// `a` (which holds pools, strides, heads, window, sinks, scale, out and, of 8-bit pages, scales).
 __attribute__((unused)) int attn_check(PagedAttnArgs* a, int D, const int32_t* page_table, int64_t ld_table, int max_pages,
                                        const int32_t* q_start, const int32_t* kv_len, int B, int T, int pages, int page_size,
                                        int max_q) {
@@ -1742,8 +1975,14 @@ __attribute__((unused)) int attn_check(PagedAttnArgs* a, int D, const int32_t* p
     if (a->k_stride < page_values || a->v_stride < page_values)
         return fail(ALV_ERR_ARG, "page strides %lld and %lld hold fewer than the page's %lld values", (long long)a->k_stride,
                     (long long)a->v_stride, (long long)page_values);
-    if (reinterpret_cast<uintptr_t>(a->kpages) % 16 || reinterpret_cast<uintptr_t>(a->vpages) % 16 || a->k_stride % 8 ||
-        a->v_stride % 8 || reinterpret_cast<uintptr_t>(a->q) % 16 || a->ld_q % 8 || reinterpret_cast<uintptr_t>(a->out) % 8 ||
+    if (a->scales && a->s_stride < 2 * (int64_t)kv_heads * page_size)
+        return fail(ALV_ERR_ARG, "scales %lld apart hold fewer than a page's %lld", (long long)a->s_stride,
+                    2ll * kv_heads * page_size);
+    const int per = a->scales ? 16 : 8;  // values of 16 bytes
+    if (a->scales && (reinterpret_cast<uintptr_t>(a->scales) % 16 || a->s_stride % 16))
+        return fail(ALV_ERR_ALIGN, "scales and their pages need 16-byte alignment");
+    if (reinterpret_cast<uintptr_t>(a->kpages) % 16 || reinterpret_cast<uintptr_t>(a->vpages) % 16 || a->k_stride % per ||
+        a->v_stride % per || reinterpret_cast<uintptr_t>(a->q) % 16 || a->ld_q % 8 || reinterpret_cast<uintptr_t>(a->out) % 8 ||
         a->ld_out % 4)
         return fail(ALV_ERR_ALIGN, "q, kpages and vpages and their rows need 16-byte alignment, out and its rows 8-byte");
     if (T == 0) return ALV_OK;
@@ -1767,13 +2006,13 @@ __attribute__((unused)) int attn_workspace(const void* workspace, uint64_t have,
     return ALV_OK;
 }
 
-template <int MODE>
+template <bool E8, int MODE>
 int attn_launch(const PagedAttnArgs& a, int D, const AttnPlan& p, hipStream_t s) {
     switch (D) {
-        case 64: return launch_d<64, MODE>(a, p, s);
-        case 128: return launch_d<128, MODE>(a, p, s);
-        case 256: return launch_d<256, MODE>(a, p, s);
-        default: return launch_d<512, MODE>(a, p, s);
+        case 64: return launch_d<64, E8, MODE>(a, p, s);
+        case 128: return launch_d<128, E8, MODE>(a, p, s);
+        case 256: return launch_d<256, E8, MODE>(a, p, s);
+        default: return launch_d<512, E8, MODE>(a, p, s);
     }
 }
 
