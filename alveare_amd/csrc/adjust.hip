@@ -10,8 +10,9 @@
 //
 // A workgroup takes kRange tokens of one row: it counts the history's tokens among
 // them in LDS (integers: their order does not show), notes which list entry is a
-// token's first bias, and passes once over the logits. In place, only what changes
-// is read and written.
+// token's first bias, and passes once over the logits, which are on their way
+// meanwhile. In place, only what changes is read and written.
+//
 #include <algorithm>
 
 #include "q4_device.h"
@@ -43,82 +44,193 @@ struct AdjustArgs {
     int64_t ld_allowed;
 };
 
-constexpr int kRange = 4096;     // tokens of a workgroup
-constexpr int kThreads = 256;
-constexpr uint32_t kPrompt = 1u << 31;  // a count's bit: the token occurred (in the prompt, where nothing else is set)
+constexpr int kThreads = 512;
+constexpr int kGroups = 4;                        // of 4 tokens, per thread
+constexpr int kRange = 4 * kGroups * kThreads;    // tokens of a workgroup
 
+// What is known of a token: how often it was generated, whether it was in the
+// prompt, whether it is on the list again, and in the upper bits `entries - i` of its
+// first list entry i (0: none). While the upper bits are set the lower ones stay, so
+// a maximum of whole words takes the first entry. 32 bits for histories and lists
+// that fit, else 64.
+template <class Word>
+struct Fields;
+template <>
+struct Fields<uint32_t> {
+    static constexpr int kCount = 17, kFirst = 19;
+};
+template <>
+struct Fields<unsigned long long> {
+    static constexpr int kCount = 31, kFirst = 33;
+};
+constexpr int kMostCount = (1 << 17) - 1, kMostEntries = (1 << 13) - 1;
+
+// WIDE: rows 16-byte aligned. COPY: out is elsewhere.
+template <class Word, bool WIDE, bool COPY>
 __global__ void __launch_bounds__(kThreads) adjust_kernel(AdjustArgs a) {
-    __shared__ uint32_t count[kRange];
-    __shared__ uint32_t owner[kRange];  // index of a token's first list entry, ~0: none
-    __shared__ int twice;               // a token is on the list again
+    using F = Fields<Word>;
+    constexpr Word kPrompt = (Word)1 << F::kCount, kTwice = 2 * kPrompt, kCountMask = kPrompt - 1, kLower = 4 * kPrompt - 1;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Word* const what = reinterpret_cast<Word*>(smem);
     const int tid = threadIdx.x, b = blockIdx.y;
     const int64_t t0 = (int64_t)blockIdx.x * kRange;
     const int n = (int)min((int64_t)kRange, a.V - t0);
+    const float* in = a.logits + b * a.ld + t0;
+    float* out = a.out + b * a.ld_out + t0;
+    const uint32_t* allowed = a.allowed ? a.allowed + b * a.ld_allowed + t0 / 32 : nullptr;
+    float4 x[kGroups] = {};
+    uint32_t keep[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int i = 4 * (tid + kThreads * g);
+        keep[g] = 15;
+        if (i < n) {
+            if (COPY) {
+                if (WIDE && i + 4 <= n) {
+                    x[g] = *reinterpret_cast<const float4*>(in + i);
+                } else {
+                    x[g].x = in[i];
+                    x[g].y = in[min(i + 1, n - 1)];
+                    x[g].z = in[min(i + 2, n - 1)];
+                    x[g].w = in[min(i + 3, n - 1)];
+                }
+            }
+            if (allowed) keep[g] = allowed[i >> 5] >> (i & 31) & 15;
+        }
+    }
     const float r = a.rep_dev ? a.rep_dev[b] : a.rep, f = a.freq_dev ? a.freq_dev[b] : a.freq;
     const float p = a.pres_dev ? a.pres_dev[b] : a.pres;
     const bool history = a.L > 0 && (r != 1.0f || f != 0.0f || p != 0.0f);
-    const bool biased = a.M > 0;
-    if (history)
-        for (int i = tid; i < kRange; i += kThreads) count[i] = 0;
-    if (biased)
-        for (int i = tid; i < kRange; i += kThreads) owner[i] = ~0u;
-    if (tid == 0) twice = 0;
-    __syncthreads();
+    const bool known = history || a.M > 0;
+    const int32_t* list = a.M > 0 ? a.bias_tokens + b * a.ld_bias_tokens : nullptr;
+    const float* bias = a.M > 0 ? a.bias + b * a.ld_bias : nullptr;
+    if (known) {
+        for (int i = tid; i < (int)(kRange * sizeof(Word) / 16); i += kThreads) reinterpret_cast<uint4*>(smem)[i] = uint4{0, 0, 0, 0};
+    }
     if (history) {
         const int32_t* row = a.tokens + b * a.ld_tokens;
         const int have = a.n_tokens ? max(0, min(a.n_tokens[b], a.L)) : a.L;
         const int prompt = a.n_prompt ? a.n_prompt[b] : 0;
-        for (int i = tid; i < have; i += kThreads) {
-            const int64_t x = row[i] - t0;
-            if (x >= 0 && x < n) {
+        // 16-byte pieces from the first aligned token on, four of a thread on their way at once.
+        const int lead = min(have, (int)(-(reinterpret_cast<uintptr_t>(row) >> 2) & 3)), pieces = (have - lead) >> 2;
+        const int tail = lead + 4 * pieces;
+        int single = -1;
+        if (tid < lead) single = tid;
+        if (tid >= 64 && tail + tid - 64 < have) single = tail + tid - 64;
+        const int st = single >= 0 ? row[single] : -1;
+        auto note = [&](int token, int i) __attribute__((always_inline)) {
+            const int64_t at = token - t0;
+            if (at >= 0 && at < n) {
                 if (i < prompt)
-                    atomicOr(&count[x], kPrompt);
+                    atomicOr(&what[at], kPrompt);
                 else
-                    atomicAdd(&count[x], 1u);
+                    atomicAdd(&what[at], (Word)1);
+            }
+        };
+        const int4* piece = reinterpret_cast<const int4*>(row + lead);
+        int4 v[4];
+        auto load = [&](int q0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int q = q0 + tid + kThreads * u;
+                v[u] = q < pieces ? piece[q] : int4{-1, -1, -1, -1};
+            }
+        };
+        load(0);
+        __syncthreads();
+        for (int q0 = 0; q0 < pieces; q0 += 4 * kThreads) {
+            if (q0) load(q0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = lead + 4 * (q0 + tid + kThreads * u);
+                note(v[u].x, i);
+                note(v[u].y, i + 1);
+                note(v[u].z, i + 2);
+                note(v[u].w, i + 3);
             }
         }
+        if (single >= 0) note(st, single);
     }
-    const int32_t* list = biased ? a.bias_tokens + b * a.ld_bias_tokens : nullptr;
-    const float* bias = biased ? a.bias + b * a.ld_bias : nullptr;
-    if (biased) {
+    if (a.M > 0) {
+        __syncthreads();
         for (int i = tid; i < a.M; i += kThreads) {
-            const int64_t x = list[i] - t0;
-            if (x >= 0 && x < n) atomicMin(&owner[x], (uint32_t)i);
+            const int64_t at = list[i] - t0;
+            if (at >= 0 && at < n) atomicMax(&what[at], (Word)(a.M - i) << F::kFirst | (what[at] & kLower));
         }
         __syncthreads();
         for (int i = tid; i < a.M; i += kThreads) {
-            const int64_t x = list[i] - t0;
-            if (x >= 0 && x < n && owner[x] != (uint32_t)i) twice = 1;
+            const int64_t at = list[i] - t0;
+            if (at >= 0 && at < n && what[at] >> F::kFirst != (Word)(a.M - i)) atomicOr(&what[at], kTwice);
         }
     }
-    __syncthreads();
-    const float* in = a.logits + b * a.ld + t0;
-    float* out = a.out + b * a.ld_out + t0;
-    const uint32_t* allowed = a.allowed ? a.allowed + b * a.ld_allowed + t0 / 32 : nullptr;
-    const bool copy = a.out != a.logits;
-    for (int i = tid; i < n; i += kThreads) {
-        const uint32_t c = history ? count[i] : 0, o = biased ? owner[i] : ~0u;
-        const bool gone = allowed && !(allowed[i >> 5] >> (i & 31) & 1);
-        if (!copy && !c && o == ~0u && !gone) continue;
-        float x = -__builtin_inff();
-        if (!gone) {
-            x = in[i];
-            if (c || o != ~0u) {
-                double y = x;
-                if (c) y = y > 0 ? y / (double)r : y * (double)r;
-                const uint32_t made = c & ~kPrompt;
-                if (made) y -= (double)f * made + (double)p;
-                if (o != ~0u) {
-                    double s = bias[o];
-                    if (twice)
-                        for (int j = o + 1; j < a.M; ++j)
-                            if (list[j] == t0 + i) s += bias[j];
-                    y += s;
-                }
-                x = (float)y;
-            }
+    if (known) __syncthreads();
+    // The pass over the logits; what is known of a token, few of them, comes after.
+    uint32_t left = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int i = 4 * (tid + kThreads * g);
+        if (i >= n) continue;
+        const uint32_t k = keep[g];
+        if (known) {
+            Word w[4];
+            __builtin_memcpy(w, __builtin_assume_aligned(what + i, 16), sizeof(w));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) left |= (uint32_t)(w[e] != 0 && i + e < n) << (4 * g + e);
+            left &= ~(15u << (4 * g)) | k << (4 * g);
         }
-        out[i] = x;
+        if (!COPY && k == 15) continue;
+        const float gone = -__builtin_inff();
+        if (WIDE && i + 4 <= n && (COPY || k == 0)) {
+            float4 v;
+            v.x = k & 1 ? x[g].x : gone;
+            v.y = k & 2 ? x[g].y : gone;
+            v.z = k & 4 ? x[g].z : gone;
+            v.w = k & 8 ? x[g].w : gone;
+            *reinterpret_cast<float4*>(out + i) = v;
+        } else {
+            const float l[4] = {x[g].x, x[g].y, x[g].z, x[g].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < n && (COPY || !(k >> e & 1))) out[i + e] = k >> e & 1 ? l[e] : gone;
+        }
+    }
+    while (__any(left != 0)) {  // the whole wave, a token of each lane's at a time
+        const bool mine = left != 0;
+        const int at = mine ? __builtin_ctz(left) : 0, i = mine ? 4 * (tid + kThreads * (at >> 2)) + (at & 3) : 0;
+        left &= left - 1;
+        float l = 0.0f;
+        if (COPY) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const float x0 = x[g].x, x1 = x[g].y, x2 = x[g].z, x3 = x[g].w;
+                const float lo = at & 1 ? x1 : x0, hi = at & 1 ? x3 : x2;
+                if (at >> 2 == g) l = at & 2 ? hi : lo;
+            }
+        } else if (mine) {
+            l = in[i];
+        }
+        const Word w = mine ? what[i] : 0;
+        double y = l;
+        if (w & (kPrompt | kCountMask)) y = y > 0 ? y / (double)r : y * (double)r;
+        const Word made = w & kCountMask;
+        if (made) y -= (double)f * made + (double)p;
+        const int first = a.M - (int)(w >> F::kFirst);
+        double sum = w >> F::kFirst ? bias[first] : 0.0;
+        // A token that is on the list again: all its biases in order, 64 entries at a time.
+        for (uint64_t more = __ballot((w & kTwice) != 0); more; more &= more - 1) {
+            const int lane = __builtin_ctzll(more);
+            const int token = (int)t0 + __builtin_amdgcn_readlane(i, lane);
+            const int o = __builtin_amdgcn_readlane(first, lane);
+            double s = bias[o];
+            for (int j0 = o + 1; j0 < a.M; j0 += 64) {
+                const int j = j0 + (tid & 63);
+                for (uint64_t hit = __ballot(j < a.M && list[min(j, a.M - 1)] == token); hit; hit &= hit - 1)
+                    s += bias[j0 + __builtin_ctzll(hit)];
+            }
+            if ((tid & 63) == lane) sum = s;
+        }
+        if (w >> F::kFirst) y += sum;
+        if (mine) out[i] = (float)y;
     }
 }
 
@@ -164,6 +276,19 @@ extern "C" int alv_adjust_logits(const float* logits, int64_t ld, float* out, in
     a.rep = repetition, a.freq = frequency, a.pres = presence;
     a.bias_tokens = bias_tokens, a.ld_bias_tokens = ld_bias_tokens, a.bias = bias, a.ld_bias = ld_bias, a.M = M;
     a.allowed = allowed, a.ld_allowed = ld_allowed;
-    hipLaunchKernelGGL(adjust_kernel, dim3((V + kRange - 1) / kRange, B), dim3(kThreads), 0, (hipStream_t)stream, a);
-    return hip_check(hipGetLastError(), "adjust_kernel launch");
+    const bool small = L <= kMostCount && M <= kMostEntries;
+    const bool wide = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                      (B == 1 || (ld % 4 == 0 && ld_out % 4 == 0));
+    const size_t lds = L > 0 || M > 0 ? kRange * (small ? 4 : 8) : 0;
+    auto go = [&](auto k) {
+        hipLaunchKernelGGL(k, dim3((V + kRange - 1) / kRange, B), dim3(kThreads), lds, (hipStream_t)stream, a);
+        return hip_check(hipGetLastError(), "adjust_kernel launch");
+    };
+    using Large = unsigned long long;
+    if (out != logits) {
+        if (wide) return small ? go(adjust_kernel<uint32_t, true, true>) : go(adjust_kernel<Large, true, true>);
+        return small ? go(adjust_kernel<uint32_t, false, true>) : go(adjust_kernel<Large, false, true>);
+    }
+    if (wide) return small ? go(adjust_kernel<uint32_t, true, false>) : go(adjust_kernel<Large, true, false>);
+    return small ? go(adjust_kernel<uint32_t, false, false>) : go(adjust_kernel<Large, false, false>);
 }
