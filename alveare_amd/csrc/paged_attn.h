@@ -1140,7 +1140,19 @@ constexpr int tile_rows(int D) { return 32 * tile_waves(D) / tile_ds(D); }
 constexpr int tile_bn(int D) { return D <= 128 ? 64 : 32; }
 constexpr int tile_bytes(int D) { return tile_bn(D) * 2 * D; }  // of K, of V
 constexpr int tile_xch(int D) { return D == 512 ? tile_waves(D) * 4096 : 0; }
-constexpr int tile_lds(int D) { return 4 * tile_bytes(D) + tile_xch(D); }
+// 8-bit pages: whether LDS holds codes, widened at each read, and how many units of
+// them; else they are widened on their way there. Codes halve what LDS delivers, which
+// bounds D >= 256 (with the products), for two vector instructions per matrix one;
+// D <= 128 is bound by the vector ALUs already.
+constexpr bool tile_codes(int D, bool E8) { return E8 && D >= 256; }
+constexpr int tile_stages(int D) { return D == 512 ? 3 : 4; }
+constexpr int kPowers = 4;  // units whose powers are kept (V's are read when the next K's buffer is filled again)
+constexpr int tile_lds(int D, bool E8) {
+    return (tile_codes(D, E8) ? tile_stages(D) * 2 * tile_bn(D) * D + kPowers * 2 * tile_bn(D) : 4 * tile_bytes(D)) + tile_xch(D);
+}
+// The swizzle of V's codes there: the 8 rows (0 .. 3, 8 .. 11) of two pieces that half
+// the lanes read at once on different banks.
+__device__ __forceinline__ constexpr int vt8_swz(int row) { return ((row & 3) | ((row >> 1) & 4)) << 1; }
 
 typedef float f32x16 __attribute__((__vector_size__(16 * sizeof(float))));
 
@@ -1311,9 +1323,12 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     constexpr int NL = LR / RPL;          // its loads of K (of V)
     constexpr int NB = BN / 16;
     constexpr int KR = 4, VR = 4;         // operands of K, of V on their way from LDS
+    constexpr bool LC = tile_codes(D, E8);
+    constexpr int TC = BN * D, NST = tile_stages(D);  // bytes of a unit's K as codes; units in LDS
     unsigned char* kbuf = smem;
-    unsigned char* vbuf = smem + 2 * TB;
-    float* xch = reinterpret_cast<float*>(smem + 4 * TB);
+    unsigned char* vbuf = smem + (LC ? NST * TC : 2 * TB);
+    [[maybe_unused]] unsigned char* pow = smem + 2 * NST * TC;  // pairs of powers, of kPowers units
+    float* xch = reinterpret_cast<float*>(smem + tile_lds(D, E8) - tile_xch(D));
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = wave / DS, dh = wave % DS;
@@ -1349,8 +1364,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         }
     };
     uint32_t holes = 0;  // NB bits by unit modulo 4
-    const uint32_t kb_lds = __builtin_amdgcn_readfirstlane(lds_addr(kbuf)) + wave * LR * (2 * D);
-    const uint32_t vb_lds = __builtin_amdgcn_readfirstlane(lds_addr(vbuf)) + wave * LR * (2 * D);
+    const uint32_t kb_lds = __builtin_amdgcn_readfirstlane(lds_addr(kbuf)) + wave * LR * (LC ? D : 2 * D);
+    const uint32_t vb_lds = __builtin_amdgcn_readfirstlane(lds_addr(vbuf)) + wave * LR * (LC ? D : 2 * D);
     // The wave's rows start at a multiple of 4, not of 16: their bits of the
     // swizzles are part of the lane's offset.
     const uint32_t dma_k = (lane / NC) * (2 * D) + ((lane % NC) ^ k_swz<D>(wave * LR + lane / NC)) * 16;
@@ -1379,8 +1394,40 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         }
     };
 
-    // 8-bit pages: a wave's share of a unit goes through registers, where codes become
-    // bf16 times their power, so that what LDS holds and the products are the same.
+    // Codes to LDS as they are, with K the slots' powers.
+    constexpr int NCC = D / 16, RPC = 1024 / D;  // pieces of a row; rows of one load
+    constexpr int NLC = LC ? LR / RPC : 1;       // a wave's loads of K (of V)
+    const uint32_t dma_kc = (lane / NCC) * D + ((lane % NCC) ^ k8_swz<D>(wave * LR + lane / NCC)) * 16;
+    const uint32_t dma_vc = (lane / NCC) * D + ((lane % NCC) ^ vt8_swz(wave * LR + lane / NCC)) * 16;
+    auto slot_of = [&](int u) __attribute__((always_inline)) { return (uint32_t)(u - u0) % NST; };
+    [[maybe_unused]] auto issue_codes = [&](int u, bool v) __attribute__((always_inline)) {
+        if (u - pages0 >= 64) load_pages(u);
+        const int page = __builtin_amdgcn_readlane(pages, u - pages0), p = unit_pos(u) + wave * LR;
+        const int have = page < 0 ? 0 : max(0, min(LR, len - p));
+        const int64_t at0 = ((int64_t)kvh << a.b.shift) + (p & ((1 << a.b.shift) - 1));
+        if (!v) {
+            uint32_t now = 0;
+#pragma unroll
+            for (int k = 0; k < NB; ++k) now |= (uint32_t)(gone[k] >> (u - pages0) & 1) << k;
+            const int bit = NB * (u & 3);
+            holes = (holes & ~(((1u << NB) - 1) << bit)) | (now << bit);
+        }
+        const uint8_t* src = v ? static_cast<const uint8_t*>(a.vpages) + max(page, 0) * a.v_stride
+                               : static_cast<const uint8_t*>(a.kpages) + max(page, 0) * a.k_stride;
+        const __amdgpu_buffer_rsrc_t r = wave_rsrc(src + at0 * D, have * D);
+        const uint32_t slot = slot_of(u), dst = (v ? vb_lds : kb_lds) + slot * TC, at = here(v ? dma_vc : dma_kc);
+#pragma unroll
+        for (int i = 0; i < NLC; ++i) {
+            const uint32_t x = v ? (uint32_t)vt8_swz(RPC * i) : (uint32_t)k8_swz<D>(RPC * i);
+            load_lds16(r, at ^ (x * 16), 1024 * i, dst + 1024 * i);
+        }
+        if (!v)
+            load_lds4<LR / 2>(wave_rsrc(a.scales + max(page, 0) * a.s_stride + 2 * at0, have > 0 ? 2 * LR : 0), lane * 4,
+                              __builtin_amdgcn_readfirstlane(lds_addr(pow)) + (uint32_t)(u - u0) % kPowers * (2 * BN) + wave * (2 * LR));
+    };
+
+    // Or a wave's share of a unit goes through registers, where codes become bf16
+    // times their power, so that what LDS holds and the products are the same.
     constexpr int NP = E8 ? LR * D / 1024 : 1;  // pieces of 16 codes of a lane, of K (of V)
     struct Codes {
         u32x4 c[NP];
@@ -1441,9 +1488,11 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     const float c = fmaxf(a.scale * kLog2e, kMinScale);
     bf16x8 q[DW / 16];
     {
-        const uint16_t* qr = a.q + (int64_t)(first + tok) * a.ld_q + head * D + dh * DW + 8 * h;
+        // (a lane's 16 bytes of codes are two operands: 16 columns of each 32)
+        const uint16_t* qr = a.q + (int64_t)(first + tok) * a.ld_q + head * D + dh * DW + (LC ? 16 : 8) * h;
 #pragma unroll
-        for (int i = 0; i < DW / 16; ++i) q[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qr + 16 * i));
+        for (int i = 0; i < DW / 16; ++i)
+            q[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qr + (LC ? 32 * (i / 2) + 8 * (i % 2) : 16 * i)));
         // Waited for here: the compiler would else wait at their first use, in
         // the loop, each time, for whatever is on its way to LDS by then.
 #pragma unroll
@@ -1454,16 +1503,38 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     for (int d = 0; d < DW / 32; ++d) o[d] = f32x16{};
     float m = kNoMax, l = 0.0f;
 
-    const int vrow = 4 * h + ((lane & 15) >> 2);
-    const uint32_t rd_k = col * (2 * D) + (h ^ k_swz<D>(col)) * 16;
-    const uint32_t rd_v = vrow * (2 * D) + ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_swz<D>(vrow)) * 16 + (lane & 1) * 8;
+    const int vrow = LC ? 4 * h + ((lane >> 1) & 3) + 8 * ((lane >> 3) & 1) : 4 * h + ((lane & 15) >> 2);
+    const uint32_t rd_k = LC ? col * D + (h ^ k8_swz<D>(col)) * 16 : col * (2 * D) + (h ^ k_swz<D>(col)) * 16;
+    const uint32_t rd_v = LC ? vrow * D + (((lane >> 4) & 1) ^ vt8_swz(vrow)) * 16 + (lane & 1) * 8
+                             : vrow * (2 * D) + ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_swz<D>(vrow)) * 16 + (lane & 1) * 8;
 
     // Rows that see nothing of 32 positions at p0 (or are none) are done with them.
     auto skip = [&](int p0) { return nrows == 0 || p0 > wpos_hi; };
     // K q of the 32 positions whose rows begin at ks, over this wave's columns.
-    auto scores = [&](const unsigned char* ks) __attribute__((always_inline)) {
+    auto scores = [&](const unsigned char* ks, [[maybe_unused]] const unsigned char* pw) __attribute__((always_inline)) {
         f32x16 s{};
         const uint32_t at = here(rd_k);
+        if constexpr (LC) {
+            constexpr int NK = DW / 32, R = 3;  // pieces of two operands; on their way
+            const float power = power_of_byte<0>(*reinterpret_cast<const uint16_t*>(pw + 2 * col));
+            auto read_k = [&](int i) __attribute__((always_inline)) {
+                return *reinterpret_cast<const u32x4*>(ks + (at ^ piece8<D>(2 * i)) + dh * DW);
+            };
+            u32x4 k[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) k[i] = read_k(i);
+            if constexpr (DS == 1) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                const uint32_t c0 = k[i % R][0], c1 = k[i % R][1], c2 = k[i % R][2], c3 = k[i % R][3];
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen8(c0, c1, power), q[2 * i], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen8(c2, c3, power), q[2 * i + 1], s, 0, 0, 0);
+                if (i + R < NK) k[i % R] = read_k(i + R);
+            }
+            if constexpr (DS == 1) __builtin_amdgcn_s_setprio(0);
+            return s;
+        }
         auto read_k = [&](int i) __attribute__((always_inline)) {
             return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
                 ks + (at ^ piece<D>(2 * i)) + piece_far<D>((dh * DW + 16 * i) / 8 & ~15)));
@@ -1485,7 +1556,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         return s;
     };
     // Their weights, and the output's share of V.
-    auto absorb = [&](const f32x16& sv, int p0, const unsigned char* vs, uint32_t hole) __attribute__((always_inline)) {
+    auto absorb = [&](const f32x16& sv, int p0, const unsigned char* vs, [[maybe_unused]] const unsigned char* pwr, uint32_t hole)
+                      __attribute__((always_inline)) {
         hole &= 3;  // of its two blocks of 16
         float s[16];
 #pragma unroll
@@ -1530,27 +1602,48 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         l += (((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]))) +
              (((w[8] + w[9]) + (w[10] + w[11])) + ((w[12] + w[13]) + (w[14] + w[15])));
         // Weights as bf16, the matrix cores' type (see the streaming kernel).
+        if constexpr (LC) {  // times V's powers
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const i32x2 pairs = *reinterpret_cast<const i32x2*>(pwr + 16 * g + 8 * h);
+                const uint32_t a0 = pairs[0], a1 = pairs[1];
+                w[4 * g] *= power_of_byte<1>(a0);
+                w[4 * g + 1] *= power_of_byte<3>(a0);
+                w[4 * g + 2] *= power_of_byte<1>(a1);
+                w[4 * g + 3] *= power_of_byte<3>(a1);
+            }
+        }
         bf16x8 pw[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) pw[i >> 3][i & 7] = (__bf16)w[i];
         // Columns 32 d .. of this wave, positions 16 k + 8 e + 4 h .. + 3.
         const uint32_t at = here(rd_v);
         auto read_v = [&](int d, int k) __attribute__((always_inline)) {
+            if constexpr (LC) {
+                return read_tr8(vs + (at ^ piece8<D>(2 * d)) + dh * DW + k * 16 * D);
+            } else {
             const unsigned char* v = vs + (at ^ piece<D>(4 * d)) + piece_far<D>((dh * DW + 32 * d) / 8 & ~15) + k * 32 * D;
             const s16x4 lo = read_tr(v), hi = read_tr(v + 16 * D);
             return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+        };
+        auto operand = [](auto v) __attribute__((always_inline)) {
+            if constexpr (LC)
+                return widen8(v[0], v[1], 1.0f);
+            else
+                return v;
         };
         // Operand j: two blocks of columns in turn, then their second 16 positions.
         constexpr int NV = DW / 16;
         auto blk = [](int j) { return (j & ~3) / 2 + (j & 1); };
-        bf16x8 v[VR];
+        std::conditional_t<LC, i32x2, bf16x8> v[VR];
 #pragma unroll
         for (int j = 0; j < VR; ++j) v[j] = read_v(blk(j), j >> 1 & 1);
         if constexpr (DS == 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             __builtin_amdgcn_sched_barrier(0);
-            o[blk(j)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[j % VR], pw[j >> 1 & 1], o[blk(j)], 0, 0, 0);
+            o[blk(j)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(v[j % VR]), pw[j >> 1 & 1], o[blk(j)], 0, 0, 0);
             if (j + VR < NV) v[j % VR] = read_v(blk(j + VR), (j + VR) >> 1 & 1);
         }
         if constexpr (DS == 1) __builtin_amdgcn_s_setprio(0);
@@ -1560,7 +1653,16 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     [[maybe_unused]] Codes kx, vx;
     if (u1 > u0) {
         load_pages(u0);
-        if constexpr (E8) {
+        if constexpr (LC) {
+            // (DS = 1: three units ahead, of four; DS = 2: four phases, of three units)
+            constexpr int ahead = DS == 1 ? 3 : 2;
+#pragma unroll
+            for (int i = 0; i < ahead; ++i)
+                if (u0 + i < u1) {
+                    issue_codes(u0 + i, false);
+                    issue_codes(u0 + i, true);
+                }
+        } else if constexpr (E8) {
             fetch(u0, false, kx);
             fetch(u0, true, vx);
             commit(u0, false, kx);
@@ -1579,9 +1681,21 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     if constexpr (DS == 1) {
 #pragma unroll 1
         for (int u = u0; u < u1; ++u) {
-            if constexpr (!E8) wait_vm<0>();
+            if constexpr (LC) {
+                if (u + 2 < u1)
+                    wait_vm<2 * (2 * NLC + 1)>();
+                else
+                    wait_vm<0>();
+            } else if constexpr (!E8) {
+                wait_vm<0>();
+            }
             __syncthreads();
-            if (u + 1 < u1) {
+            if constexpr (LC) {
+                if (u + 3 < u1) {
+                    issue_codes(u + 3, false);
+                    issue_codes(u + 3, true);
+                }
+            } else if (u + 1 < u1) {
                 if constexpr (E8) {
                     commit(u + 1, false, kx);
                     commit(u + 1, true, vx);
@@ -1595,11 +1709,13 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
                 }
             }
             const int pt = unit_pos(u);
-            const unsigned char* kt = kbuf + (u & 1) * TB;
-            const unsigned char* vt = vbuf + (u & 1) * TB;
+            const uint32_t slot = LC ? slot_of(u) : u & 1;
+            const unsigned char* kt = kbuf + slot * (LC ? TC : TB);
+            const unsigned char* vt = vbuf + slot * (LC ? TC : TB);
+            const unsigned char* pw = pow + (uint32_t)(u - u0) % kPowers * (2 * BN);
 #pragma unroll 1
             for (int sub = 0; sub < BN / 32 && !skip(pt + 32 * sub); ++sub)
-                absorb(scores(kt + sub * 64 * D), pt + 32 * sub, vt + sub * 64 * D, holes >> (NB * (u & 3) + 2 * sub));
+                absorb(scores(kt + sub * 64 * D, pw), pt + 32 * sub, vt + sub * 64 * D, pw, holes >> (NB * (u & 3) + 2 * sub));
         }
     } else {
         // Two groups of waves, one of each per SIMD, half a unit apart: while one
@@ -1616,6 +1732,21 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         // (codes become LDS's one phase ahead: phase + 1's buffer has had its last reader
         // two phases ago)
         auto begin = [&](int phase) __attribute__((always_inline)) {
+            if constexpr (LC) {
+                // Phases phase + 1 .. + 3 may still be on their way: two of K, one of V, or
+                // the reverse. A buffer's last reader was two phases ago.
+                if (phase + 3 < 2 * nu) {
+                    if (phase & 1)
+                        wait_vm<3 * NLC + 2>();
+                    else
+                        wait_vm<3 * NLC + 1>();
+                } else {
+                    wait_vm<0>();
+                }
+                __syncthreads();
+                if (phase + 4 < 2 * nu) issue_codes(u0 + ((phase + 4) >> 1), phase & 1);
+                return;
+            }
             if constexpr (E8) {
                 __syncthreads();
                 if (phase + 1 < 2 * nu) commit(u0 + ((phase + 1) >> 1), (phase + 1) & 1, vx);
@@ -1636,7 +1767,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
             f32x16 s{};
             begin(2 * (u - u0) + grp);
             if (!skip(p0)) {
-                s = scores(kbuf + (u & 1) * TB);
+                const uint32_t slot = LC ? slot_of(u) : u & 1;
+                s = scores(kbuf + slot * (LC ? TC : TB), pow + (uint32_t)(u - u0) % kPowers * (2 * BN));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mine[64 * i] = f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
             }
@@ -1649,7 +1781,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[4 * i + e] += x[e];
                 }
-                absorb(s, p0, vbuf + (u & 1) * TB, holes >> (NB * (u & 3)));
+                const uint32_t slot = LC ? slot_of(u) : u & 1;
+                absorb(s, p0, vbuf + slot * (LC ? TC : TB), pow + (uint32_t)(u - u0) % kPowers * (2 * BN), holes >> (NB * (u & 3)));
             }
         }
         if (nu > 0 && grp == 0) begin(2 * nu);
@@ -1718,7 +1851,7 @@ template <int D, bool E8, int MODE>
 __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kernel(PagedAttnArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int TR = tile_rows(D), BN = tile_bn(D);
-    static_assert(tile_lds(D) >= 4 * kSplitTiles, "the tiles' units");
+    static_assert(tile_lds(D, E8) >= 4 * kSplitTiles, "the tiles' units");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const TileScan sc0 = tile_scan<TR, MODE>(a, 0, lane);
     const int tiles = tile_count<TR, MODE>(a, sc0, lane), items = tiles * a.kv_heads;
@@ -1916,7 +2049,7 @@ int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
 
 template <int D, bool E8, int MODE>
 int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    constexpr int lds = tile_lds(D);
+    constexpr int lds = tile_lds(D, E8);
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D, E8, MODE>), lds, done)) return rc;
