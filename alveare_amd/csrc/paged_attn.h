@@ -183,9 +183,10 @@ __device__ __forceinline__ s16x4 read_tr(const unsigned char* p) {
 // ---- 8-bit pages ---------------------------------------------------------------------
 //
 // Codes become bf16 operands in registers (two per instruction; e4m3's four bits fit
-// bf16's eight, so nothing is rounded). K's power is a factor of its score, V's of
-// the weight that multiplies it; where a workgroup shares tiles they go into the
-// conversion instead, a power of two being exact there too.
+// bf16's eight, so nothing is rounded), times a power of two at no cost: K's, of the
+// lane's position. A lane's codes of V are several positions': V's powers are factors of
+// the weights instead (exact in float32; where tiles are widened ahead of LDS, they too
+// go into the conversion).
 
 // Eight codes times a power of two.
 __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float power) {
@@ -521,24 +522,25 @@ struct RowsSeq {
     int us, ulo, nu;  // units of first tokens; first unit of the window; units in all
 };
 
-constexpr int rows_waves(int D) { return D == 512 ? 2 : (D == 64 ? 8 : 4); }
+constexpr int rows_groups(int D, bool E8) { return E8 && D <= 256 ? 2 : 1; }  // workgroups per CU
+constexpr int rows_waves(int D, bool E8) { return (D == 512 ? 2 : (D == 64 ? 8 : 4)) / rows_groups(D, E8); }
 // A wave's block: 16 positions' K and V, or 32 of 8-bit ones and their powers.
 constexpr int rows_block(bool E8) { return E8 ? 32 : 16; }
 constexpr int rows_stage(int D, bool E8) { return 64 * D + (E8 ? 64 : 0); }
-constexpr int rows_stages(int D) { return 131072 / (rows_waves(D) * 64 * D); }
-constexpr int rows_unit(int D, bool E8) { return rows_block(E8) * rows_waves(D); }
+constexpr int rows_stages(int D) { return 131072 / (rows_waves(D, false) * 64 * D); }
+constexpr int rows_unit(int D, bool E8) { return rows_block(E8) * rows_waves(D, E8); }
 // The waves' outputs at a tile's end, rows padded to spread over the banks.
 constexpr int rows_out_ld(int D) { return D + 4; }
 // Whether q's operands stay in LDS rather than registers: where they and the
 // output take more than half of a wave's 256 (the rest would spill).
 constexpr bool rows_q_lds(int D, int QT) { return QT * D > 256; }
 constexpr int rows_lds(int D, int QT, bool E8) {
-    const int ring = rows_waves(D) * rows_stages(D) * rows_stage(D, E8);
-    const int outs = rows_waves(D) * 16 * QT * (rows_out_ld(D) * 4);
-    return (ring > outs ? ring : outs) + 2 * rows_waves(D) * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0) + 16;
+    const int ring = rows_waves(D, E8) * rows_stages(D) * rows_stage(D, E8);
+    const int outs = rows_waves(D, E8) * 16 * QT * (rows_out_ld(D) * 4);
+    return (ring > outs ? ring : outs) + 2 * rows_waves(D, E8) * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0) + 16;
 }
 constexpr int rows_mls(int D, int QT, bool E8) {  // where the waves' maxima and sums stand; q behind them
-    return rows_lds(D, QT, E8) - 16 - 2 * rows_waves(D) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
+    return rows_lds(D, QT, E8) - 16 - 2 * rows_waves(D, E8) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
 }
 // Floats of one workspace place: outputs, maxima, sums.
 constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
@@ -675,15 +677,15 @@ __device__ __forceinline__ uint32_t part_count(uint64_t total, const Scan& sc, i
 }
 
 template <int D, int QT, bool E8, int MODE>
-__global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kernel(PagedAttnArgs a) {
-    constexpr int NW = rows_waves(D), NS = rows_stages(D), UNIT = rows_unit(D, E8), ROWS = 16 * QT;
+__global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_kernel(PagedAttnArgs a) {
+    constexpr int NW = rows_waves(D, E8), NS = rows_stages(D), UNIT = rows_unit(D, E8), ROWS = 16 * QT;
     constexpr int BP = rows_block(E8), NH = BP / 16;  // positions of a block, 16 at a time (within a page)
     constexpr int STAGE = rows_stage(D, E8);
     constexpr int NC = E8 ? D / 16 : D / 8;  // 16-byte pieces of a row
     constexpr int NI = NC / 4;            // loads of 64 pieces for 16 positions of K (of V)
     constexpr int HALF = 32 * D;          // bytes of a block's K
     constexpr int RPL = 64 / NC;          // rows of one load
-    constexpr int LOADS = NH * (2 * NI + E8);  // of a block
+    constexpr int LOADS = NH * 2 * NI + E8;   // of a block, at least
     using T = PageValue<E8>;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -725,43 +727,74 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
         };
         // The pages of this wave's blocks, 64 at a time, one per lane.
         const int32_t* table = a.b.table + (int64_t)f.seq * a.b.ld_table;
-        int pages[NH], pages0 = 0;
+        int pages0 = 0;
         uint32_t gone_bits = 0;  // by buffer: its page (of the first 16, of the others) is missing
+        int pages = -1;                        // bf16
+        [[maybe_unused]] uint64_t ka = 0, va = 0, sa = 0;  // 8-bit: where a block's K, V and powers begin
+        [[maybe_unused]] int have = 0;         // and how many positions there are; bit 8: its page is missing
+        // (pages of 16: a block's halves each)
+        const int halves = E8 && a.b.shift < 5 ? 1 : 0;
         auto load_pages = [&](int j0) {
             pages0 = j0;
-            const int j = j0 + lane;
-#pragma unroll
-            for (int hf = 0; hf < NH; ++hf) {
-                const int p = block_pos(j) + 16 * hf;
-                pages[hf] = j < nblk && p < f.s.len ? table[p >> a.b.shift] : -1;
-                if ((unsigned)pages[hf] >= (unsigned)a.b.pages) pages[hf] = -1;
+            const int j = j0 + (lane >> halves), p = block_pos(j) + 16 * (lane & halves);
+            pages = j < nblk && p < f.s.len ? table[p >> a.b.shift] : -1;
+            if ((unsigned)pages >= (unsigned)a.b.pages) pages = -1;
+            if constexpr (E8) {
+                const int64_t slot = ((int64_t)f.kvh << a.b.shift) + (p & (S - 1));
+                const int64_t page = max(pages, 0);
+                ka = reinterpret_cast<uint64_t>(a.kpages) + page * a.k_stride + slot * D;
+                va = reinterpret_cast<uint64_t>(a.vpages) + page * a.v_stride + slot * D;
+                sa = reinterpret_cast<uint64_t>(a.scales) + page * a.s_stride + slot * 2;
+                have = pages < 0 ? 256 : max(0, min(halves ? 16 : 32, f.s.len - p));
             }
         };
+        // Load i brings rows RPL i .. of RPL each; the swizzles are exclusive ors of the
+        // row's bits, so the lane's offset within the rows of one load serves all, with
+        // the load's own bits applied.
+        // Past the sequence's end, and where the page is missing, zeros arrive.
         auto issue = [&](int j) {
-            if (j - pages0 >= 64) load_pages(j);
+            const uint32_t dst = ring_lds + (uint32_t)(j % NS) * STAGE;
+            if constexpr (E8) {
+                if (j - pages0 >= 64 >> halves) load_pages(j);
+                auto part = [&](auto count, int at, uint32_t half) __attribute__((always_inline)) {
+                    constexpr int N = decltype(count)::value;  // rows: 16, or all 32
+                    const uint64_t k = lane_u64(ka, at), v = lane_u64(va, at), s = lane_u64(sa, at);
+                    const int n = __builtin_amdgcn_readlane(have, at);
+                    const uint32_t rows = n & 63;
+                    gone_bits |= (uint32_t)(n >> 8) * (N == 32 ? 3u : 1u << half) << (NH * (j % NS));
+                    const __amdgpu_buffer_rsrc_t rk = make_rsrc(reinterpret_cast<const void*>(k), rows * D);
+                    const __amdgpu_buffer_rsrc_t rv = make_rsrc(reinterpret_cast<const void*>(v), rows * D);
+                    const uint32_t to = dst + half * (16 * D);
 #pragma unroll
-            for (int hf = 0; hf < NH; ++hf) {
-                const int page = __builtin_amdgcn_readlane(pages[hf], j - pages0), p = block_pos(j) + 16 * hf;
-                // Past the sequence's end, and where the page is missing, zeros arrive.
-                const uint32_t bytes = page < 0 ? 0u : (uint32_t)max(0, min(16, f.s.len - p)) * (16 * NC);
-                const int64_t slot = ((int64_t)f.kvh << a.b.shift) + (p & (S - 1));
-                const __amdgpu_buffer_rsrc_t rk = wave_rsrc(static_cast<const T*>(a.kpages) + max(page, 0) * a.k_stride + slot * D, bytes);
-                const __amdgpu_buffer_rsrc_t rv = wave_rsrc(static_cast<const T*>(a.vpages) + max(page, 0) * a.v_stride + slot * D, bytes);
-                const int bit = NH * (j % NS) + hf;
-                gone_bits = (gone_bits & ~(1u << bit)) | ((uint32_t)(page < 0) << bit);
-                const uint32_t dst = ring_lds + (uint32_t)(j % NS) * STAGE + hf * (16 * D);
-                // Load i brings rows RPL i .. of RPL each; the swizzles are exclusive
-                // ors of the row's bits, so the lane's offset within the rows of one
-                // load serves all, with the load's own bits applied.
+                    for (int i = 0; i < N / RPL; ++i)
+                        load_lds16(rk, dma_k ^ (kz(RPL * i) * 16), 1024 * i, to + 1024 * i);
+#pragma unroll
+                    for (int i = 0; i < N / RPL; ++i)
+                        load_lds16(rv, dma_v ^ ((vz(RPL * i) ^ (half ? vz(16) : 0)) * 16), 1024 * i, to + HALF + 1024 * i);
+                    // (a page's powers, 16 pairs at least, are there whatever its positions)
+                    load_lds4<N / 2>(make_rsrc(reinterpret_cast<const void*>(s), rows ? 2 * N : 0), lane * 4, dst + 64 * D + 32 * half);
+                };
+                gone_bits &= ~(3u << (NH * (j % NS)));
+                if (halves) {
+                    part(std::integral_constant<int, 16>(), 2 * (j - pages0), 0);
+                    part(std::integral_constant<int, 16>(), 2 * (j - pages0) + 1, 1);
+                } else {
+                    part(std::integral_constant<int, 32>(), j - pages0, 0);
+                }
+            } else {
+                if (j - pages0 >= 64) load_pages(j);
+                const int page = __builtin_amdgcn_readlane(pages, j - pages0), p = block_pos(j);
+                const uint32_t bytes = page < 0 ? 0u : (uint32_t)max(0, min(16, f.s.len - p)) * (2 * D);
+                const int64_t off = (((int64_t)f.kvh << a.b.shift) + (p & (S - 1))) * D;
+                const __amdgpu_buffer_rsrc_t rk = wave_rsrc(static_cast<const T*>(a.kpages) + max(page, 0) * a.k_stride + off, bytes);
+                const __amdgpu_buffer_rsrc_t rv = wave_rsrc(static_cast<const T*>(a.vpages) + max(page, 0) * a.v_stride + off, bytes);
+                gone_bits = (gone_bits & ~(1u << (j % NS))) | ((uint32_t)(page < 0) << (j % NS));
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
-                    load_lds16(rk, dma_k ^ (kz(16 * hf + RPL * i) * 16), 1024 * i, dst + 1024 * i);
+                    load_lds16(rk, dma_k ^ (kz(RPL * i) * 16), 1024 * i, dst + 1024 * i);
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
-                    load_lds16(rv, dma_v ^ (vz(16 * hf + RPL * i) * 16), 1024 * i, dst + HALF + 1024 * i);
-                if constexpr (E8)  // the slots' 16 pairs of powers
-                    load_lds4<8>(wave_rsrc(a.scales + max(page, 0) * a.s_stride + 2 * slot, bytes ? 32 : 0), lane * 4,
-                                 ring_lds + (uint32_t)(j % NS) * STAGE + 64 * D + 32 * hf);
+                    load_lds16(rv, dma_v ^ (vz(RPL * i) * 16), 1024 * i, dst + HALF + 1024 * i);
             }
         };
 
@@ -854,12 +887,13 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
                 };
                 if constexpr (E8) {
                     powers[hf] = *reinterpret_cast<const i32x2*>(kt + 64 * D + 32 * hf + 8 * G);
+                    const float kp = power_of_byte<0>(*reinterpret_cast<const uint16_t*>(kt + 64 * D + 32 * hf + 2 * col));
 #pragma unroll
                     for (int i = 0; i < D / 64; ++i) {
                         if (KB > 0 && i % KB == 0) asm volatile("" ::: "memory");
                         const u32x4 k = *reinterpret_cast<const u32x4*>(kt + hf * (16 * D) + (rd_k ^ piece8<D>(4 * i)) + piece8_far<D>(4 * i));
-                        product(widen8(k[0], k[1], 1.0f), 2 * i);
-                        product(widen8(k[2], k[3], 1.0f), 2 * i + 1);
+                        product(widen8(k[0], k[1], kp), 2 * i);
+                        product(widen8(k[2], k[3], kp), 2 * i + 1);
                     }
                 } else {
 #pragma unroll
@@ -873,9 +907,6 @@ __global__ void __launch_bounds__((64 * rows_waves(D)), 2) attn_paged_rows_kerne
 #pragma unroll
                 for (int hf = 0; hf < NH; ++hf) {
                     const uint32_t p0 = powers[hf][0], p1 = powers[hf][1];
-                    const f32x4 kp{power_of_byte<0>(p0), power_of_byte<2>(p0), power_of_byte<0>(p1), power_of_byte<2>(p1)};
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) s[hf][t] *= kp;
                     vp[hf][0] = power_of_byte<1>(p0), vp[hf][1] = power_of_byte<3>(p0);
                     vp[hf][2] = power_of_byte<1>(p1), vp[hf][3] = power_of_byte<3>(p1);
                 }
@@ -1976,7 +2007,7 @@ struct AttnPlan {
     uint64_t rows_bytes, tab_bytes, part_bytes;
 };
 
-__attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q) {
+__attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q, bool e8) {
     AttnPlan p{};
     const int64_t g = heads / kv_heads;
     max_q = std::min(max_q, T);  // (and its products stay within 64 bits)
@@ -2005,7 +2036,7 @@ __attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B
         const int64_t r = tiles ? g : rows;
         p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
         p.row_limit = tiles ? 16 * p.qt : INT64_MAX;
-        p.grid = device_cus();
+        p.grid = device_cus() * rows_groups(D, e8);
         p.rows_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
     }
     p.part_bytes = p.rows_bytes;
@@ -2041,7 +2072,7 @@ int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, E8, MODE>), lds, done)) return rc;
-    hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MODE>), dim3(p.grid), dim3(64 * rows_waves(D)), lds, s, a);
+    hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MODE>), dim3(p.grid), dim3(64 * rows_waves(D, E8)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_rows_kernel launch")) return rc;
     hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT, E8, MODE>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a, p.grid);
     return hip_check(hipGetLastError(), "attn_paged_rows_merge_kernel launch");

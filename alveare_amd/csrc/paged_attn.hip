@@ -5,7 +5,7 @@ using namespace alv;
 
 extern "C" uint64_t alv_attention_paged_workspace(int heads, int kv_heads, int D, int B, int T, int max_q) {
     if (heads < 1 || kv_heads < 1 || heads % kv_heads || D < 1 || B < 1 || T < 1 || max_q < 0) return 0;
-    return attn_plan(heads, kv_heads, D, B, T, max_q).part_bytes;
+    return attn_plan(heads, kv_heads, D, B, T, max_q, false).part_bytes;
 }
 
 extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16_t* kpages, const uint16_t* vpages,
@@ -20,7 +20,7 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
     a.out = out, a.ld_out = ld_out;
     if (int rc = attn_check(&a, D, page_table, ld_table, max_pages, q_start, kv_len, B, T, pages, page_size, max_q)) return rc;
     if (T == 0) return ALV_OK;
-    const AttnPlan p = attn_plan(heads, kv_heads, D, B, T, max_q);
+    const AttnPlan p = attn_plan(heads, kv_heads, D, B, T, max_q, false);
     if (int rc = attn_fits(p, T, heads, B)) return rc;
     if (int rc = attn_workspace(workspace, workspace_bytes, p.part_bytes)) return rc;
     a.part = static_cast<float*>(workspace);

@@ -44,12 +44,12 @@ struct SharedPlan {
     uint64_t pre_bytes, bytes;
 };
 
-__attribute__((unused)) SharedPlan shared_plan(int heads, int kv_heads, int D, int B, int T, int max_q, int groups) {
+__attribute__((unused)) SharedPlan shared_plan(int heads, int kv_heads, int D, int B, int T, int max_q, int groups, bool e8) {
     SharedPlan p{};
-    p.suf = attn_plan(heads, kv_heads, D, B, T, max_q);
+    p.suf = attn_plan(heads, kv_heads, D, B, T, max_q, e8);
     p.bytes = p.suf.part_bytes;
     if (groups > 0) {
-        p.pre = attn_plan(heads, kv_heads, D, groups, T, 0);
+        p.pre = attn_plan(heads, kv_heads, D, groups, T, 0, e8);
         p.pre_bytes = ((uint64_t)T * heads * (D + 2) * sizeof(float) + 15) / 16 * 16;
         p.bytes = p.pre_bytes + std::max(p.pre.part_bytes, p.suf.part_bytes);
     }
@@ -70,7 +70,7 @@ int attention_shared(const SharedCall& c) {
                             c.max_q))
         return rc;
     if (c.T == 0) return ALV_OK;
-    const SharedPlan p = shared_plan(c.heads, c.kv_heads, c.D, c.B, c.T, c.max_q, c.groups);
+    const SharedPlan p = shared_plan(c.heads, c.kv_heads, c.D, c.B, c.T, c.max_q, c.groups, E8);
     if (int rc = attn_fits(p.pre, c.T, c.heads, c.groups)) return rc;
     if (int rc = attn_fits(p.suf, c.T, c.heads, c.B)) return rc;
     if (int rc = attn_workspace(c.workspace, c.workspace_bytes, p.bytes)) return rc;

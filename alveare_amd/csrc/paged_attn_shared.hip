@@ -7,7 +7,8 @@ extern "C" uint64_t alv_attention_shared_workspace(int heads, int kv_heads, int 
     if (heads < 1 || heads > kMaxHeads || kv_heads < 1 || heads % kv_heads || D < 1 || D > 512 || B < 1 || T < 1 || max_q < 0 ||
         groups < 0)
         return 0;
-    return shared_plan(heads, kv_heads, D, B, T, max_q, groups).bytes;
+    return std::max(shared_plan(heads, kv_heads, D, B, T, max_q, groups, false).bytes,
+                    shared_plan(heads, kv_heads, D, B, T, max_q, groups, true).bytes);
 }
 
 extern "C" int alv_attention_shared(const uint16_t* q, int64_t ld_q, const void* kpages, const void* vpages, int64_t k_stride,
