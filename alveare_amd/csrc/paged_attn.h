@@ -57,6 +57,7 @@ struct PagedAttnArgs {
     int max_items;      // tiles (times kv heads) that may be split: no more than slots; 0: none
     int slots;          // parts that run at once
     int* tab;           // for the merge: how many tiles, then kTabInts for each
+    int* cuts;          // for the streaming kernel's: kTabInts for each workgroup
     float* part;
     float* pre;         // what kPre leaves of each (row, head): D values,
     float* pre_ml;      // and its maximum and sum
@@ -546,6 +547,7 @@ constexpr int rows_mls(int D, int QT, bool E8) {  // where the waves' maxima and
 constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
 
 constexpr int kPartsPerTile = 64;
+constexpr int kTabInts = 8;  // an entry of the merges' tables
 
 struct Scan {
     RowsSeq s;          // this lane's sequence
@@ -694,6 +696,10 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
     Scan sc;
     const uint64_t total = scan_all<ROWS, UNIT, MODE>(a, lane, sc);
     const Cut cut = make_cut(total, part_count(total, sc, gridDim.x));
+    // The tile that begins in this part and ends in a later one, for the merge: the last
+    // part it is in, first row of its sequence, tile, rows, kv head, shared.
+    int* const cut_tile = a.cuts + kTabInts * blockIdx.x;
+    if (threadIdx.x == 0) cut_tile[0] = 0;
     if (blockIdx.x >= cut.n) return;
     uint64_t x = cut.begin(blockIdx.x);
     const uint64_t end = cut.begin(blockIdx.x + 1);
@@ -823,6 +829,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
                 }
             }
         }
+        if (nblk) load_pages(0);  // (its trip to memory beside q's)
         if constexpr (QL) {
             __syncthreads();
         } else {
@@ -857,7 +864,6 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) o[t][d] = f32x4{0, 0, 0, 0};
         }
-        if (nblk) load_pages(0);
 #pragma unroll 1
         for (int j = 0; j < min(NS, nblk); ++j) issue(j);
 #pragma unroll 1
@@ -1015,6 +1021,10 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
 #pragma unroll
         for (int w = 0; w < NW; ++w) again |= odds[w] != 0;
         const bool whole = u0 == 0 && u1 == f.s.nu;
+        if (u0 == 0 && !whole && tid == 0) {
+            cut_tile[0] = (int)cut.part_of(f.tile0 + f.s.nu - 1);
+            cut_tile[1] = f.s.first, cut_tile[2] = f.rt, cut_tile[3] = nrows, cut_tile[4] = f.kvh, cut_tile[5] = f.s.from;
+        }
         float* part = a.part + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * rows_part(D, QT);
         if (again) {
             for (int r = wave; r < nrows; r += NW) {
@@ -1119,32 +1129,26 @@ __device__ __forceinline__ void join_parts(int n, int lane, ML ml, int gap, O o,
     }
 }
 
-// The cut tiles: wave (boundary, row) joins the parts of the tile in which
-// boundary blockIdx.x + 1 is the first, in the order of the line.
-template <int D, int QT, bool E8, int MODE>
-__global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArgs a, int grid) {
-    constexpr int UNIT = rows_unit(D, E8), ROWS = 16 * QT, RW = D / 64;
+// The cut tiles: a wave per row joins the parts of the tile that begins in part
+// blockIdx.x and ends in a later one, in the order of the line. (What the streaming
+// workgroups wrote of it is one trip to memory; the scan for it anew took 2 us.)
+template <int D, int QT, int MODE>
+__global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArgs a) {
+    constexpr int ROWS = 16 * QT, RW = D / 64;
     const int lane = threadIdx.x & 63;
     const int r = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
-    Scan sc;
-    const uint64_t total = scan_all<ROWS, UNIT, MODE>(a, lane, sc);
-    const Cut cut = make_cut(total, part_count(total, sc, grid));
-    const uint32_t w = blockIdx.x + 1;
-    if (w >= cut.n) return;
-    const Found f = scan_find<ROWS, UNIT, MODE>(a, lane, sc, cut.begin(w));
-    if (f.u == 0 || cut.begin(w - 1) > f.tile0) return;
-    if (r >= min(ROWS, f.s.n * a.g - f.rt * ROWS)) return;
-    // Part w - 1 holds the tile's begin in its second place, the later ones
-    // theirs in the first.
-    auto place = [&](uint32_t v) { return a.part + (size_t)(2 * v + (v == w - 1 ? 1 : 0)) * rows_part(D, QT); };
-    const uint32_t last = cut.part_of(f.tile0 + f.s.nu - 1);
-    const int n = (int)(last - w + 2);
+    const int w = blockIdx.x;
+    const int* e = a.cuts + kTabInts * w;
+    const int last = e[0], first = e[1], rt = e[2], nrows = e[3], kvh = e[4], from = e[5];
+    if (last == 0 || r >= nrows) return;
+    // Part w holds the tile's begin in its second place, the later ones theirs in the first.
+    auto place = [&](int v) { return a.part + (size_t)(2 * (w + v) + (v == 0 ? 1 : 0)) * rows_part(D, QT); };
     float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
     join_parts<RW>(
-        n, lane, [&](int v) { return place(w - 1 + v) + ROWS * D + r; }, ROWS,
-        [&](int v) { return place(w - 1 + v) + (size_t)r * D + RW * lane; }, acc, mx, ls);
-    const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
-    finish_row<D, MODE>(a, f.s.first + tok, h, lane, acc, mx, ls, f.s.from > 0);
+        last - w + 1, lane, [&](int v) { return place(v) + ROWS * D + r; }, ROWS,
+        [&](int v) { return place(v) + (size_t)r * D + RW * lane; }, acc, mx, ls);
+    const int rr = r + rt * ROWS, tok = rr / a.g, h = kvh * a.g + (rr - tok * a.g);
+    finish_row<D, MODE>(a, first + tok, h, lane, acc, mx, ls, from > 0);
 }
 
 // ---- many rows: a workgroup shares K and V tiles ------------------------------------------
@@ -1280,7 +1284,7 @@ struct TileAt {
 constexpr int kSplitTiles = 512;  // at most, of one kv head
 constexpr int kMaxParts = 64;     // of a tile: a lane each in the merge
 constexpr int kMinCap = 2;        // (4: 380 tokens of 32 heads of 64 in 3 sequences 27 us for 21)
-constexpr int kTabInts = 8;       // entry of part 0, parts, first row of the sequence, tile, rows, kv head, shared
+// (entries: that of part 0, parts, first row of the sequence, tile, rows, kv head, shared)
 
 __device__ __forceinline__ int sum64(int v) {
 #pragma unroll
@@ -2004,7 +2008,7 @@ struct AttnPlan {
     int64_t grid_tiles;  // tiles times kv heads of the tile kernel at most (0: not launched),
     int64_t tiles;       // and at most as far as max_q tells
     int slots;           // parts of tiles; 0: none is split
-    uint64_t rows_bytes, tab_bytes, part_bytes;
+    uint64_t cuts_bytes, rows_bytes, tab_bytes, part_bytes;
 };
 
 __attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B, int T, int max_q, bool e8) {
@@ -2037,7 +2041,8 @@ __attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B
         p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
         p.row_limit = tiles ? 16 * p.qt : INT64_MAX;
         p.grid = device_cus() * rows_groups(D, e8);
-        p.rows_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
+        p.cuts_bytes = (uint64_t)p.grid * kTabInts * sizeof(int);
+        p.rows_bytes = p.cuts_bytes + (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
     }
     p.part_bytes = p.rows_bytes;
     if (tiles) {
@@ -2074,7 +2079,7 @@ int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, E8, MODE>), lds, done)) return rc;
     hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MODE>), dim3(p.grid), dim3(64 * rows_waves(D, E8)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_rows_kernel launch")) return rc;
-    hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT, E8, MODE>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a, p.grid);
+    hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT, MODE>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "attn_paged_rows_merge_kernel launch");
 }
 
@@ -2111,7 +2116,8 @@ int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
         a.part = part + (p.rows_bytes + p.tab_bytes) / sizeof(float);
         if (int rc = launch_tiles<D, E8, MODE>(a, p, s)) return rc;
     }
-    a.part = part;
+    a.cuts = reinterpret_cast<int*>(part);
+    a.part = part + p.cuts_bytes / sizeof(float);
     if (p.qt == 1) return launch_rows<D, 1, E8, MODE>(a, p, s);
     if constexpr (D <= 256)
         if (p.qt == 2) return launch_rows<D, 2, E8, MODE>(a, p, s);
