@@ -17,6 +17,8 @@
 // groups, each a sequence of all its members' rows over the shared positions alone,
 // leaves every row's maximum, sum and output in memory, unnormalised (kPre); then
 // one over the sequences takes the positions behind them and joins the two (kSuf).
+// Where both are the streaming kernel's they are one line of work (kMix), joined by
+// its merge: two launches instead of four.
 #pragma once
 
 #include <limits.h>
@@ -35,7 +37,7 @@ namespace {
 
 // What a launch's sequences are: the batch's; the groups over what each shares; the
 // batch's over what is behind that.
-enum { kAll = 0, kPre = 1, kSuf = 2 };
+enum { kAll = 0, kPre = 1, kSuf = 2, kMix = 3 };  // kMix: the groups, then the batch's
 
 struct PagedAttnArgs {
     PagedBatch b;
@@ -61,6 +63,10 @@ struct PagedAttnArgs {
     float* part;
     float* pre;         // what kPre leaves of each (row, head): D values,
     float* pre_ml;      // and its maximum and sum
+    float* suf;         // kMix: the same of what is behind,
+    float* suf_ml;
+    int4* recs;         // and where both parts of a row are (Rec), those of `pre` first
+    int grid;           // streaming workgroups
 };
 
 template <bool E8>
@@ -271,6 +277,16 @@ __device__ __forceinline__ void finish4(const PagedAttnArgs& a, int64_t t, int h
     store4(a.out + t * a.ld_out + h * D + d, v, inverse(l));
 }
 
+// What a row's part comes to, kept (see kPre).
+template <int D>
+__device__ __forceinline__ void keep4(float* to, float* ml, int64_t row, int d, f32x4 v, float m, float l) {
+    *reinterpret_cast<f32x4*>(to + row * D + d) = v;
+    if (d == 0) {
+        ml[2 * row] = m;
+        ml[2 * row + 1] = l;
+    }
+}
+
 // The same of RW values per lane, a row per wave.
 template <int D, int MODE>
 __device__ __forceinline__ void finish_row(const PagedAttnArgs& a, int64_t t, int h, int lane, const float (&acc)[D / 64], float m,
@@ -309,9 +325,11 @@ struct SeqIn {
     bool here, ok;      // has rows in the batch; well formed
 };
 
+// kMix: the groups take whole steps of 64, the sequences follow.
+__device__ __forceinline__ int group_steps(const PagedAttnArgs& a) { return (a.gr.n + 63) & ~63; }
 template <int MODE>
 __device__ __forceinline__ int seq_count(const PagedAttnArgs& a) {
-    return MODE == kPre ? a.gr.n : a.b.B;
+    return MODE == kPre ? a.gr.n : (MODE == kMix ? group_steps(a) + a.b.B : a.b.B);
 }
 
 // Sequence b of the launch, a lane each (b0 + lane, b0 uniform).
@@ -549,6 +567,11 @@ constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
 constexpr int kPartsPerTile = 64;
 constexpr int kTabInts = 8;  // an entry of the merges' tables
 
+// kMix: where a row's part is: {part of the tile's begin, its last part, row of the
+// tile, positions shared}; no last part where the whole tile was one workgroup's, which
+// kept what it comes to, or (nothing shared) wrote the output.
+constexpr int kWhole = -1, kDone = -2;
+
 struct Scan {
     RowsSeq s;          // this lane's sequence
     uint64_t incl;      // work of the sequences of this step up to and with this lane's
@@ -566,7 +589,12 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
 
 template <int ROWS, int UNIT, int MODE>
 __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int lane, uint64_t base, Scan& sc) {
-    const SeqIn in = seq_in<MODE>(a, b0, lane);
+    const bool pre = MODE == kPre || (MODE == kMix && b0 < group_steps(a)), suf = MODE == kSuf || (MODE == kMix && !pre);
+    SeqIn in;
+    if constexpr (MODE == kMix)
+        in = pre ? seq_in<kPre>(a, b0, lane) : seq_in<kSuf>(a, b0 - group_steps(a), lane);
+    else
+        in = seq_in<MODE>(a, b0, lane);
     RowsSeq s{};
     s.first = in.first, s.n = in.n, s.len = in.len, s.seq = in.seq, s.from = in.from;
     uint64_t w = 0;
@@ -575,9 +603,9 @@ __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int la
         s.tiles = (int)((rows + ROWS - 1) / ROWS);
         if (in.ok) {
             int lo = a.window > 0 ? max(0, in.lo + 1 - a.window) : 0;
-            if (MODE == kSuf) lo = a.sinks > s.from ? s.from : max(lo, s.from);
+            if (suf) lo = a.sinks > s.from ? s.from : max(lo, s.from);
             s.ulo = lo / UNIT;
-            s.us = MODE == kSuf ? 0 : min((min(a.sinks, lo) + UNIT - 1) / UNIT, s.ulo);
+            s.us = suf ? 0 : min((min(a.sinks, lo) + UNIT - 1) / UNIT, s.ulo);
             // (one at least: kPre may leave nothing within the window, kSuf nothing behind what is shared)
             s.nu = s.us + max((s.len + UNIT - 1) / UNIT - s.ulo, MODE == kAll ? INT_MIN : s.us ? 0 : 1);
         } else {
@@ -623,6 +651,7 @@ __device__ __forceinline__ uint64_t div32(uint64_t a, uint64_t b) {  // (32 bits
 struct Found {
     RowsSeq s;
     int seq, kvh, rt;
+    bool pre;         // of a group, over what it shares
     int u;            // unit in the tile
     uint64_t tile0;   // the tile's place in the line
 };
@@ -634,7 +663,8 @@ __device__ __forceinline__ Found scan_find(const PagedAttnArgs& a, int lane, Sca
     const uint64_t m = __ballot(sc.base + sc.incl > x);
     const int l = __builtin_ctzll(m);
     Found f;
-    f.seq = MODE == kPre ? __builtin_amdgcn_readlane(sc.s.seq, l) : sc.b0 + l;
+    f.seq = MODE == kPre || MODE == kMix ? __builtin_amdgcn_readlane(sc.s.seq, l) : sc.b0 + l;
+    f.pre = MODE == kPre || (MODE == kMix && sc.b0 < group_steps(a));
     f.s.from = MODE == kAll ? 0 : __builtin_amdgcn_readlane(sc.s.from, l);
     f.s.first = __builtin_amdgcn_readlane(sc.s.first, l);
     f.s.n = __builtin_amdgcn_readlane(sc.s.n, l);
@@ -698,8 +728,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
     const Cut cut = make_cut(total, part_count(total, sc, gridDim.x));
     // The tile that begins in this part and ends in a later one, for the merge: the last
     // part it is in, first row of its sequence, tile, rows, kv head, shared.
-    int* const cut_tile = a.cuts + kTabInts * blockIdx.x;
-    if (threadIdx.x == 0) cut_tile[0] = 0;
+    [[maybe_unused]] int* const cut_tile = a.cuts + kTabInts * blockIdx.x;
+    if (MODE != kMix && threadIdx.x == 0) cut_tile[0] = 0;
     if (blockIdx.x >= cut.n) return;
     uint64_t x = cut.begin(blockIdx.x);
     const uint64_t end = cut.begin(blockIdx.x + 1);
@@ -727,6 +757,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
         x += u1 - u0;
         const int nrows = min(ROWS, f.s.n * a.g - f.rt * ROWS);
         const int nblk = f.s.len > 0 ? u1 - u0 : 0;  // this wave's blocks
+        const bool pre = MODE == kPre || (MODE == kMix && f.pre), suf = MODE == kSuf || (MODE == kMix && !f.pre);
         auto block_pos = [&](int j) {
             const int u = u0 + j;
             return (u < f.s.us ? u : u - f.s.us + f.s.ulo) * UNIT + BP * wave;
@@ -816,7 +847,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
             const int tok = r / a.g, h = f.kvh * a.g + (r - tok * a.g);
             row_t[t] = f.s.first + tok;
             pos[t].pos = pos[t].cap = f.s.len - f.s.n + tok;
-            pos[t].from = MODE == kSuf ? f.s.from : 0;
+            pos[t].from = suf ? f.s.from : 0;
             // (of codes, 16 bytes of a lane's are two operands: 16 columns of each 64)
             const uint16_t* qr = a.q + (int64_t)(f.s.first + tok) * a.ld_q + h * D + (E8 ? 16 : 8) * G;
             constexpr auto q_at = [](int i) { return E8 ? 64 * (i / 2) + 8 * (i % 2) : 32 * i; };
@@ -842,7 +873,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
         }
         int pos_lo = f.s.len - f.s.n + (f.rt * ROWS) / a.g;
         int pos_hi = f.s.len - f.s.n + (f.rt * ROWS + nrows - 1) / a.g;
-        if constexpr (MODE == kPre) {
+        if (pre) {
             int p[QT];
             row_positions<QT>(a, f.seq, f.s.from, row_t, p);
             int lo = INT_MAX, hi = -1;
@@ -866,6 +897,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
         }
 #pragma unroll 1
         for (int j = 0; j < min(NS, nblk); ++j) issue(j);
+        auto blocks = [&](auto count) __attribute__((always_inline)) {
+            constexpr int NT = decltype(count)::value;  // row tiles of 16 that there are
 #pragma unroll 1
         for (int j = 0; j < nblk; ++j) {
             // Blocks j + 1 .. j + NS - 1 may be in flight.
@@ -875,128 +908,146 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
                 wait_vm<0>();
             const unsigned char* kt = ring + (j % NS) * STAGE;
             const unsigned char* vt = kt + HALF;
-            f32x4 s[NH][QT];
-            constexpr int KB = QT * D >= 512 ? (QT == 4 ? 1 : 2) : 0;  // K reads of codes at once, where registers are short
-            [[maybe_unused]] i32x2 powers[NH];  // of this lane's positions: k's, v's in turn
-#pragma unroll
-            for (int hf = 0; hf < NH; ++hf) {
-#pragma unroll
-                for (int t = 0; t < QT; ++t) s[hf][t] = f32x4{0, 0, 0, 0};
-                auto product = [&](bf16x8 k, int i) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) {
-                        if constexpr (QL)
-                            s[hf][t] = mfma16x16x32(k, __builtin_bit_cast(bf16x8, qs[(t * (D / 32) + i) * 64]), s[hf][t]);
-                        else
-                            s[hf][t] = mfma16x16x32(k, q[t][i], s[hf][t]);
-                    }
-                };
-                if constexpr (E8) {
-                    powers[hf] = *reinterpret_cast<const i32x2*>(kt + 64 * D + 32 * hf + 8 * G);
-                    const float kp = power_of_byte<0>(*reinterpret_cast<const uint16_t*>(kt + 64 * D + 32 * hf + 2 * col));
-#pragma unroll
-                    for (int i = 0; i < D / 64; ++i) {
-                        if (KB > 0 && i % KB == 0) asm volatile("" ::: "memory");
-                        const u32x4 k = *reinterpret_cast<const u32x4*>(kt + hf * (16 * D) + (rd_k ^ piece8<D>(4 * i)) + piece8_far<D>(4 * i));
-                        product(widen8(k[0], k[1], kp), 2 * i);
-                        product(widen8(k[2], k[3], kp), 2 * i + 1);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i)
-                        product(__builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
-                                                               kt + (rd_k ^ piece<D>(4 * i)) + piece_far<D>(4 * i))), i);
-                }
-            }
-            float vp[NH][4];  // V's powers
-            if constexpr (E8) {
+                f32x4 s[NH][NT];
+                constexpr int KB = QT * D >= 512 ? (QT == 4 ? 1 : 2) : 0;  // K reads of codes at once, where registers are short
+                [[maybe_unused]] i32x2 powers[NH];  // of this lane's positions: k's, v's in turn
 #pragma unroll
                 for (int hf = 0; hf < NH; ++hf) {
-                    const uint32_t p0 = powers[hf][0], p1 = powers[hf][1];
-                    vp[hf][0] = power_of_byte<1>(p0), vp[hf][1] = power_of_byte<3>(p0);
-                    vp[hf][2] = power_of_byte<1>(p1), vp[hf][3] = power_of_byte<3>(p1);
-                }
-            }
-            const int p0 = block_pos(j);
-            const uint32_t gone = gone_bits >> (NH * (j % NS)) & ((1u << NH) - 1);
-            const bool masked = gone || p0 + BP - 1 > pos_lo || (MODE == kSuf && p0 < f.s.from) ||
-                                (a.window > 0 && p0 <= pos_hi - a.window && p0 + BP - 1 >= a.sinks);
-            if (masked) {
 #pragma unroll
-                for (int hf = 0; hf < NH; ++hf)
+                    for (int t = 0; t < NT; ++t) s[hf][t] = f32x4{0, 0, 0, 0};
+                    auto product = [&](bf16x8 k, int i) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int t = 0; t < QT; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (!sees(a, p0 + 16 * hf + 4 * G + i, pos[t]) || (gone >> hf & 1)) s[hf][t][i] = -__builtin_inff();
-            }
-            typedef __bf16 Weights __attribute__((__vector_size__(4 * NH * sizeof(__bf16))));
-            Weights pw[QT];
-#pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                float top = -__builtin_inff();
-#pragma unroll
-                for (int hf = 0; hf < NH; ++hf) {
-                    const float s0 = s[hf][t][0], s1 = s[hf][t][1], s2 = s[hf][t][2], s3 = s[hf][t][3];
-                    const float most = fmaxf(fmaxf(s0, s1), fmaxf(s2, s3));
-                    top = hf ? fmaxf(top, most) : most;
-                }
-                if (__any(__builtin_fmaf(top, c, -m[t]) > kSlack)) {
-                    const float mn = fmaxf(m[t], max_groups(top) * c);
-                    const float fac = __builtin_amdgcn_exp2f(m[t] - mn);
-                    m[t] = mn;
-                    l[t] *= fac;
-#pragma unroll
-                    for (int d = 0; d < D / 16; ++d) o[t][d] *= fac;
-                }
-                // Weights as bf16, the matrix cores' type: half a step, 2^-8
-                // relative each, as much as the output's own rounding (the outputs'
-                // mean error against 64 bits: 0.0021 to 0.0024, of which their own
-                // rounding is 0.0017).
-#pragma unroll
-                for (int hf = 0; hf < NH; ++hf) {
-                    float w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float si = s[hf][t][i];
-                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(si, c, -m[t]));
-                    }
-                    l[t] += (w[0] + w[1]) + (w[2] + w[3]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) pw[t][4 * hf + i] = (__bf16)(E8 ? w[i] * vp[hf][i] : w[i]);
-                }
-            }
-            auto read_v = [&](int d) __attribute__((always_inline)) {
-                if constexpr (E8)
-                    return read_tr8(vt + (rd_v ^ piece8<D>(d)) + piece8_far<D>(d));
-                else
-                    return read_tr(vt + (rd_v ^ piece<D>(2 * d)) + piece_far<D>(2 * d));
-            };
-            constexpr int VB = D / 16 < 8 ? D / 16 : (E8 && QT * D >= 512 ? (QT == 4 ? 2 : 4) : 8);  // V reads on their way at once
-#pragma unroll
-            for (int d0 = 0; d0 < D / 16; d0 += VB) {
-                std::conditional_t<E8, i32x2, s16x4> v[VB];
-#pragma unroll
-                for (int d = 0; d < VB; ++d) v[d] = read_v(d0 + d);
-                asm volatile("" ::: "memory");
-#pragma unroll
-                for (int d = 0; d < VB; ++d) {
+                        for (int t = 0; t < NT; ++t) {
+                            if constexpr (QL)
+                                s[hf][t] = mfma16x16x32(k, __builtin_bit_cast(bf16x8, qs[(t * (D / 32) + i) * 64]), s[hf][t]);
+                            else
+                                s[hf][t] = mfma16x16x32(k, q[t][i], s[hf][t]);
+                        }
+                    };
                     if constexpr (E8) {
-                        const bf16x8 vb = widen8(v[d][0], v[d][1], 1.0f);
+                        powers[hf] = *reinterpret_cast<const i32x2*>(kt + 64 * D + 32 * hf + 8 * G);
+                        const float kp = power_of_byte<0>(*reinterpret_cast<const uint16_t*>(kt + 64 * D + 32 * hf + 2 * col));
 #pragma unroll
-                        for (int t = 0; t < QT; ++t) o[t][d0 + d] = mfma16x16x32(vb, pw[t], o[t][d0 + d]);
+                        for (int i = 0; i < D / 64; ++i) {
+                            if (KB > 0 && i % (KB > 0 ? KB : 1) == 0) asm volatile("" ::: "memory");
+                            const u32x4 k = *reinterpret_cast<const u32x4*>(kt + hf * (16 * D) + (rd_k ^ piece8<D>(4 * i)) + piece8_far<D>(4 * i));
+                            product(widen8(k[0], k[1], kp), 2 * i);
+                            product(widen8(k[2], k[3], kp), 2 * i + 1);
+                        }
                     } else {
 #pragma unroll
-                        for (int t = 0; t < QT; ++t)
-                            o[t][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v[d], __builtin_bit_cast(s16x4, pw[t]),
-                                                                                     o[t][d0 + d], 0, 0, 0);
+                        for (int i = 0; i < D / 32; ++i)
+                            product(__builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
+                                                                   kt + (rd_k ^ piece<D>(4 * i)) + piece_far<D>(4 * i))), i);
                     }
                 }
-            }
+                float vp[NH][4];  // V's powers
+                if constexpr (E8) {
+#pragma unroll
+                    for (int hf = 0; hf < NH; ++hf) {
+                        const uint32_t p0 = powers[hf][0], p1 = powers[hf][1];
+                        vp[hf][0] = power_of_byte<1>(p0), vp[hf][1] = power_of_byte<3>(p0);
+                        vp[hf][2] = power_of_byte<1>(p1), vp[hf][3] = power_of_byte<3>(p1);
+                    }
+                }
+                const int p0 = block_pos(j);
+                const uint32_t gone = gone_bits >> (NH * (j % NS)) & ((1u << NH) - 1);
+                const bool masked = gone || p0 + BP - 1 > pos_lo || (suf && p0 < f.s.from) ||
+                                    (a.window > 0 && p0 <= pos_hi - a.window && p0 + BP - 1 >= a.sinks);
+                if (masked) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        // Relative to p0 + 4 G, so that positions are constants; selects, no branches.
+                        const int base = p0 + 4 * G, top = pos[t].cap - base, begin = pos[t].from - base;
+                        const int lo = a.window > 0 ? pos[t].pos - a.window - base : INT_MIN, sk = a.sinks - base;
+#pragma unroll
+                        for (int hf = 0; hf < NH; ++hf) {
+                            const int hi = gone >> hf & 1 ? INT_MIN : top;
+                            f32x4 v = s[hf][t];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int p = 16 * hf + i;
+                                bool seen = (p <= hi) & ((p > lo) | (p < sk));
+                                if (MODE == kSuf || MODE == kMix) seen &= p >= begin;
+                                const float x = v[i];
+                                v[i] = seen ? x : -__builtin_inff();
+                            }
+                            s[hf][t] = v;
+                        }
+                    }
+                }
+                typedef __bf16 Weights __attribute__((__vector_size__(4 * NH * sizeof(__bf16))));
+                Weights pw[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float top = -__builtin_inff();
+#pragma unroll
+                    for (int hf = 0; hf < NH; ++hf) {
+                        const float s0 = s[hf][t][0], s1 = s[hf][t][1], s2 = s[hf][t][2], s3 = s[hf][t][3];
+                        const float most = fmaxf(fmaxf(s0, s1), fmaxf(s2, s3));
+                        top = hf ? fmaxf(top, most) : most;
+                    }
+                    if (__any(__builtin_fmaf(top, c, -m[t]) > kSlack)) {
+                        const float mn = fmaxf(m[t], max_groups(top) * c);
+                        const float fac = __builtin_amdgcn_exp2f(m[t] - mn);
+                        m[t] = mn;
+                        l[t] *= fac;
+#pragma unroll
+                        for (int d = 0; d < D / 16; ++d) o[t][d] *= fac;
+                    }
+                    // Weights as bf16, the matrix cores' type: half a step, 2^-8
+                    // relative each, as much as the output's own rounding (the outputs'
+                    // mean error against 64 bits: 0.0021 to 0.0024, of which their own
+                    // rounding is 0.0017).
+#pragma unroll
+                    for (int hf = 0; hf < NH; ++hf) {
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float si = s[hf][t][i];
+                            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(si, c, -m[t]));
+                        }
+                        l[t] += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) pw[t][4 * hf + i] = (__bf16)(E8 ? w[i] * vp[hf][i] : w[i]);
+                    }
+                }
+                auto read_v = [&](int d) __attribute__((always_inline)) {
+                    if constexpr (E8)
+                        return read_tr8(vt + (rd_v ^ piece8<D>(d)) + piece8_far<D>(d));
+                    else
+                        return read_tr(vt + (rd_v ^ piece<D>(2 * d)) + piece_far<D>(2 * d));
+                };
+                constexpr int VB = D / 16 < 8 ? D / 16 : (E8 && QT * D >= 512 ? (QT == 4 ? 2 : 4) : 8);  // V reads on their way at once
+#pragma unroll
+                for (int d0 = 0; d0 < D / 16; d0 += VB) {
+                    std::conditional_t<E8, i32x2, s16x4> v[VB];
+#pragma unroll
+                    for (int d = 0; d < VB; ++d) v[d] = read_v(d0 + d);
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int d = 0; d < VB; ++d) {
+                        if constexpr (E8) {
+                            const bf16x8 vb = widen8(v[d][0], v[d][1], 1.0f);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) o[t][d0 + d] = mfma16x16x32(vb, pw[t], o[t][d0 + d]);
+                        } else {
+#pragma unroll
+                            for (int t = 0; t < NT; ++t)
+                                o[t][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v[d], __builtin_bit_cast(s16x4, pw[t]),
+                                                                                         o[t][d0 + d], 0, 0, 0);
+                        }
+                    }
+                }
             // The buffer's reads are done before it is filled again.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (j + NS < nblk) issue(j + NS);
         }
+        };
+        if (MODE == kMix && QT > 1 && nrows <= 16)
+            blocks(std::integral_constant<int, 1>());
+        else
+            blocks(std::integral_constant<int, QT>());
 
         // The waves' results: rescaled to the largest maximum and added in order.
 #pragma unroll
@@ -1021,7 +1072,15 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
 #pragma unroll
         for (int w = 0; w < NW; ++w) again |= odds[w] != 0;
         const bool whole = u0 == 0 && u1 == f.s.nu;
-        if (u0 == 0 && !whole && tid == 0) {
+        if constexpr (MODE == kMix) {
+            for (int r = u0 == 0 ? tid : nrows; r < nrows; r += 64 * NW) {
+                const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
+                const int64_t row = (int64_t)(f.s.first + tok) * a.heads + h;
+                const int done = !pre && f.s.from == 0 ? kDone : kWhole;
+                a.recs[(pre ? 0 : (int64_t)a.b.T * a.heads) + row] =
+                    int4{(int)blockIdx.x, whole ? done : (int)cut.part_of(f.tile0 + f.s.nu - 1), r, f.s.from};
+            }
+        } else if (u0 == 0 && !whole && tid == 0) {
             cut_tile[0] = (int)cut.part_of(f.tile0 + f.s.nu - 1);
             cut_tile[1] = f.s.first, cut_tile[2] = f.rt, cut_tile[3] = nrows, cut_tile[4] = f.kvh, cut_tile[5] = f.s.from;
         }
@@ -1030,8 +1089,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
             for (int r = wave; r < nrows; r += NW) {
                 const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
                 float acc[D / 64], mr, lr;
-                Sight at{f.s.len - f.s.n + tok, f.s.len - f.s.n + tok, MODE == kSuf ? f.s.from : 0};
-                if constexpr (MODE == kPre) {
+                Sight at{f.s.len - f.s.n + tok, f.s.len - f.s.n + tok, suf ? f.s.from : 0};
+                if (pre) {
                     const int one[1] = {f.s.first + tok};
                     int p[1];
                     row_positions<1>(a, f.seq, f.s.from, one, p);
@@ -1040,7 +1099,16 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
                 plain_row<D, E8>(a, f.seq, f.kvh, a.q + (int64_t)(f.s.first + tok) * a.ld_q + h * D, at, f.s.us, f.s.ulo, UNIT, u0, u1,
                              lane, acc, mr, lr);
                 if (whole) {
-                    finish_row<D, MODE>(a, f.s.first + tok, h, lane, acc, mr, lr, f.s.from > 0);
+                    if constexpr (MODE == kMix) {
+                        PagedAttnArgs to = a;  // (kPre keeps a row)
+                        to.pre = pre ? a.pre : a.suf, to.pre_ml = pre ? a.pre_ml : a.suf_ml;
+                        if (!pre && f.s.from == 0)
+                            finish_row<D, kAll>(a, f.s.first + tok, h, lane, acc, mr, lr, false);
+                        else
+                            finish_row<D, kPre>(to, f.s.first + tok, h, lane, acc, mr, lr, false);
+                    } else {
+                        finish_row<D, MODE>(a, f.s.first + tok, h, lane, acc, mr, lr, f.s.from > 0);
+                    }
                     continue;
                 }
 #pragma unroll
@@ -1079,7 +1147,14 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
             }
             if (whole) {
                 const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
-                finish4<D, MODE>(a, f.s.first + tok, h, d, v, mx, ls, f.s.from > 0);
+                if constexpr (MODE == kMix) {
+                    if (!pre && f.s.from == 0)
+                        finish4<D, kAll>(a, f.s.first + tok, h, d, v, mx, ls, false);
+                    else
+                        keep4<D>(pre ? a.pre : a.suf, pre ? a.pre_ml : a.suf_ml, (int64_t)(f.s.first + tok) * a.heads + h, d, v, mx, ls);
+                } else {
+                    finish4<D, MODE>(a, f.s.first + tok, h, d, v, mx, ls, f.s.from > 0);
+                }
             } else {
                 *reinterpret_cast<f32x4*>(part + (size_t)r * D + d) = v;
                 if (d == 0) {
@@ -1149,6 +1224,35 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
         [&](int v) { return place(v) + (size_t)r * D + RW * lane; }, acc, mx, ls);
     const int rr = r + rt * ROWS, tok = rr / a.g, h = kvh * a.g + (rr - tok * a.g);
     finish_row<D, MODE>(a, first + tok, h, lane, acc, mx, ls, from > 0);
+}
+
+// kMix: a wave per (row, head) joins its two parts, in the order shared, own. (Records of
+// sequences that are malformed may hold anything; they are not followed out of bounds.)
+template <int D, int QT>
+__global__ void __launch_bounds__(256) attn_paged_mix_merge_kernel(PagedAttnArgs a) {
+    constexpr int ROWS = 16 * QT, RW = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.b.T * a.heads;
+    if (row >= rows) return;
+    const int t = __builtin_amdgcn_readfirstlane((int)(row / a.heads)), h = __builtin_amdgcn_readfirstlane((int)(row % a.heads));
+    const int4 rp = a.recs[row], rs = a.recs[rows + row];
+    const SeqRows sr = find_row(a.b, t, lane);
+    if (sr.seq < 0 || sr.first < 0 || (int64_t)sr.first + sr.n > a.b.T) return;
+    if (uniform(rs.y) == kDone) return;
+    float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
+    auto add = [&](const int4& rec, const float* kept, const float* ml) {
+        const int w = uniform(rec.x), last = uniform(rec.y), r = uniform(rec.z);
+        if (w < 0 || w >= a.grid || r < 0 || r >= ROWS || last >= a.grid || (last != kWhole && last <= w)) return;
+        auto place = [&](int v) { return a.part + (size_t)(2 * (w + v) + (v == 0 ? 1 : 0)) * rows_part(D, QT); };
+        const bool whole = last == kWhole;
+        join_parts<RW>(
+            whole ? 1 : last - w + 1, lane, [&](int v) { return whole ? ml + 2 * row : place(v) + ROWS * D + r; },
+            whole ? 1 : ROWS, [&](int v) { return whole ? kept + row * D + RW * lane : place(v) + (size_t)r * D + RW * lane; },
+            acc, mx, ls);
+    };
+    if (uniform(rs.w) > 0) add(rp, a.pre, a.pre_ml);
+    add(rs, a.suf, a.suf_ml);
+    finish_row<D, kAll>(a, t, h, lane, acc, mx, ls, false);
 }
 
 // ---- many rows: a workgroup shares K and V tiles ------------------------------------------
@@ -2060,6 +2164,23 @@ __attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B
     return p;
 }
 
+// kMix: where the sequences' own rows are the streaming kernel's and a group's fill no
+// more than two of its tiles (so that what is shared is read twice at most), that
+// `rows` of the average group come to; else qt is 0.
+__attribute__((unused)) AttnPlan mix_plan(const AttnPlan& suf, int heads, int kv_heads, int D, int T, int max_q, int groups) {
+    AttnPlan p{};
+    const int64_t g = heads / kv_heads, rows = ((int64_t)T + groups - 1) / groups * g;
+    const int qt_max = D <= 128 ? 4 : (D == 256 ? 2 : 1);
+    if (suf.qt == 0 || suf.grid_tiles || rows > 32 * qt_max || (int64_t)T * heads > 1 << 24) return p;
+    p = suf;
+    const int64_t r = std::max(std::min(rows, (int64_t)16 * qt_max), (int64_t)16 * suf.qt);
+    p.qt = r <= 16 ? 1 : (r <= 32 ? 2 : 4);
+    p.row_limit = INT64_MAX;
+    p.cuts_bytes = 0;
+    p.rows_bytes = p.part_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
+    return p;
+}
+
 // Dynamic LDS past 64 KiB, asked for once per kernel and device.
 __attribute__((unused)) int allow_lds(const void* k, int lds, std::atomic<uint64_t>& done) {
     int dev = 0;
@@ -2079,6 +2200,10 @@ int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, E8, MODE>), lds, done)) return rc;
     hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MODE>), dim3(p.grid), dim3(64 * rows_waves(D, E8)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_rows_kernel launch")) return rc;
+    if constexpr (MODE == kMix) {
+        hipLaunchKernelGGL((attn_paged_mix_merge_kernel<D, QT>), dim3((uint32_t)(((int64_t)a.b.T * a.heads + 3) / 4)), dim3(256), 0, s, a);
+        return hip_check(hipGetLastError(), "attn_paged_mix_merge_kernel launch");
+    }
     hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT, MODE>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "attn_paged_rows_merge_kernel launch");
 }
@@ -2106,16 +2231,18 @@ int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
 
 template <int D, bool E8, int MODE>
 int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
+    a.grid = p.grid;
     a.row_limit = p.row_limit;
     a.slots = p.slots;
     a.max_items = p.slots ? (int)p.tiles : 0;
     a.max_tiles = (int)(p.grid_tiles / a.kv_heads);
     float* part = a.part;
-    if (p.grid_tiles) {
-        if (p.slots) a.tab = reinterpret_cast<int*>(part + p.rows_bytes / sizeof(float));
-        a.part = part + (p.rows_bytes + p.tab_bytes) / sizeof(float);
-        if (int rc = launch_tiles<D, E8, MODE>(a, p, s)) return rc;
-    }
+    if constexpr (MODE != kMix)
+        if (p.grid_tiles) {
+            if (p.slots) a.tab = reinterpret_cast<int*>(part + p.rows_bytes / sizeof(float));
+            a.part = part + (p.rows_bytes + p.tab_bytes) / sizeof(float);
+            if (int rc = launch_tiles<D, E8, MODE>(a, p, s)) return rc;
+        }
     a.cuts = reinterpret_cast<int*>(part);
     a.part = part + p.cuts_bytes / sizeof(float);
     if (p.qt == 1) return launch_rows<D, 1, E8, MODE>(a, p, s);

@@ -37,11 +37,12 @@ int attention_shared8(const SharedCall& c);  // of 8-bit pages
 
 namespace {
 
-// What kPre leaves (D values, a maximum and a sum for each row and head), then the
-// two runs' own workspace, one after the other's.
+// Two runs: what kPre leaves (D values, a maximum and a sum for each row and head),
+// then the runs' own workspace, one after the other's. One (mix.qt > 0): what is kept
+// of both parts of a row, where they are, then the line's parts.
 struct SharedPlan {
-    AttnPlan pre, suf;
-    uint64_t pre_bytes, bytes;
+    AttnPlan pre, suf, mix;
+    uint64_t rec_bytes, kept_bytes, bytes;
 };
 
 __attribute__((unused)) SharedPlan shared_plan(int heads, int kv_heads, int D, int B, int T, int max_q, int groups, bool e8) {
@@ -49,9 +50,15 @@ __attribute__((unused)) SharedPlan shared_plan(int heads, int kv_heads, int D, i
     p.suf = attn_plan(heads, kv_heads, D, B, T, max_q, e8);
     p.bytes = p.suf.part_bytes;
     if (groups > 0) {
-        p.pre = attn_plan(heads, kv_heads, D, groups, T, 0, e8);
-        p.pre_bytes = ((uint64_t)T * heads * (D + 2) * sizeof(float) + 15) / 16 * 16;
-        p.bytes = p.pre_bytes + std::max(p.pre.part_bytes, p.suf.part_bytes);
+        p.kept_bytes = ((uint64_t)T * heads * (D + 2) * sizeof(float) + 15) / 16 * 16;
+        p.mix = mix_plan(p.suf, heads, kv_heads, D, T, max_q, groups);
+        if (p.mix.qt) {
+            p.rec_bytes = 2 * (uint64_t)T * heads * sizeof(int4);
+            p.bytes = p.rec_bytes + 2 * p.kept_bytes + p.mix.part_bytes;
+        } else {
+            p.pre = attn_plan(heads, kv_heads, D, groups, T, 0, e8);
+            p.bytes = p.kept_bytes + std::max(p.pre.part_bytes, p.suf.part_bytes);
+        }
     }
     return p;
 }
@@ -78,9 +85,17 @@ int attention_shared(const SharedCall& c) {
     a.part = static_cast<float*>(c.workspace);
     if (c.groups == 0) return attn_launch<E8, kSuf>(a, c.D, p.suf, s);
     a.gr = PagedGroups{c.group_start, c.shared_len, c.groups};
-    a.pre = a.part;
-    a.pre_ml = a.pre + (int64_t)c.T * c.heads * c.D;
-    a.part = a.pre + p.pre_bytes / sizeof(float);
+    const int64_t rows = (int64_t)c.T * c.heads;
+    a.recs = reinterpret_cast<int4*>(c.workspace);
+    a.pre = a.part + p.rec_bytes / sizeof(float);
+    a.pre_ml = a.pre + rows * c.D;
+    a.suf = a.pre + p.kept_bytes / sizeof(float);
+    a.suf_ml = a.suf + rows * c.D;
+    if (p.mix.qt) {
+        a.part = a.suf + p.kept_bytes / sizeof(float);
+        return attn_launch<E8, kMix>(a, c.D, p.mix, s);
+    }
+    a.part = a.suf;
     if (int rc = attn_launch<E8, kPre>(a, c.D, p.pre, s)) return rc;
     return attn_launch<E8, kSuf>(a, c.D, p.suf, s);
 }
