@@ -13,12 +13,11 @@
 // the kernels sort the sequences by their own counts, so a batch may hold both
 // kinds; a small batch with more rows is the tile kernel's alone.
 //
-// Groups of sequences that share their first positions (MODE): one run over the
-// groups, each a sequence of all its members' rows over the shared positions alone,
-// leaves every row's maximum, sum and output in memory, unnormalised (kPre); then
-// one over the sequences takes the positions behind them and joins the two (kSuf).
-// Where both are the streaming kernel's they are one line of work (kMix), joined by
-// its merge: two launches instead of four.
+// Groups of sequences that share their first positions (MIX): each group is one more
+// sequence, of all its members' rows over the shared positions alone, and the batch's
+// own run over what is behind. The kernels take the groups and the sequences alike, by
+// their rows; what the parts of a row come to is kept, unnormalised, with its maximum
+// and sum, and a last launch joins them.
 #pragma once
 
 #include <limits.h>
@@ -34,10 +33,6 @@
 namespace alv {
 
 namespace {
-
-// What a launch's sequences are: the batch's; the groups over what each shares; the
-// batch's over what is behind that.
-enum { kAll = 0, kPre = 1, kSuf = 2, kMix = 3 };  // kMix: the groups, then the batch's
 
 struct PagedAttnArgs {
     PagedBatch b;
@@ -61,12 +56,13 @@ struct PagedAttnArgs {
     int* tab;           // for the merge: how many tiles, then kTabInts for each
     int* cuts;          // for the streaming kernel's: kTabInts for each workgroup
     float* part;
-    float* pre;         // what kPre leaves of each (row, head): D values,
-    float* pre_ml;      // and its maximum and sum
-    float* suf;         // kMix: the same of what is behind,
-    float* suf_ml;
-    int4* recs;         // and where both parts of a row are (Rec), those of `pre` first
-    int grid;           // streaming workgroups
+    // MIX: what a row's part comes to where one workgroup had all of it, D values and a
+    // maximum and sum for each (row, head): over what is shared, and behind,
+    float* kept[2];
+    float* kept_ml[2];
+    int4* recs;         // where the parts of each are (Rec), those over what is shared first,
+    float* tile_part;   // and the tiles' parts
+    int grid, tile_places;  // streaming workgroups; parts of tiles that there is room for
 };
 
 template <bool E8>
@@ -254,150 +250,147 @@ __device__ __forceinline__ void store4(uint16_t* dst, f32x4 v, float inv) {
     *reinterpret_cast<s16x4*>(dst) = pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
 }
 
-// Where a row's result goes: four values v at column d of head h of packed row t,
-// unnormalised, with the row's maximum and sum. kSuf, where `shared`: joined to what
-// kPre left of it.
-template <int D, int MODE>
-__device__ __forceinline__ void finish4(const PagedAttnArgs& a, int64_t t, int h, int d, f32x4 v, float m, float l, bool shared) {
-    const int64_t row = t * a.heads + h;
-    if constexpr (MODE == kPre) {
-        *reinterpret_cast<f32x4*>(a.pre + row * D + d) = v;
+// Where a row's part goes that one workgroup had all of: four values v at column d of
+// head h of packed row t, unnormalised, with the row's maximum and sum. `half`: over what
+// is shared 0, behind 1; `alone`: the row has no other part.
+template <int D, bool MIX>
+__device__ __forceinline__ void finish4(const PagedAttnArgs& a, int64_t t, int h, int d, f32x4 v, float m, float l, int half,
+                                        bool alone) {
+    if (MIX && !alone) {
+        const int64_t row = t * a.heads + h;
+        *reinterpret_cast<f32x4*>(a.kept[half] + row * D + d) = v;
         if (d == 0) {
-            a.pre_ml[2 * row] = m;
-            a.pre_ml[2 * row + 1] = l;
+            a.kept_ml[half][2 * row] = m;
+            a.kept_ml[half][2 * row + 1] = l;
         }
         return;
-    }
-    if (MODE == kSuf && shared) {
-        const float mp = a.pre_ml[2 * row], lp = a.pre_ml[2 * row + 1], mx = fmaxf(m, mp);
-        const float f = __builtin_amdgcn_exp2f(m - mx), fp = __builtin_amdgcn_exp2f(mp - mx);
-        v = v * f + *reinterpret_cast<const f32x4*>(a.pre + row * D + d) * fp;
-        l = l * f + lp * fp;
     }
     store4(a.out + t * a.ld_out + h * D + d, v, inverse(l));
 }
 
-// What a row's part comes to, kept (see kPre).
-template <int D>
-__device__ __forceinline__ void keep4(float* to, float* ml, int64_t row, int d, f32x4 v, float m, float l) {
-    *reinterpret_cast<f32x4*>(to + row * D + d) = v;
-    if (d == 0) {
-        ml[2 * row] = m;
-        ml[2 * row + 1] = l;
-    }
-}
-
 // The same of RW values per lane, a row per wave.
-template <int D, int MODE>
+template <int D, bool MIX>
 __device__ __forceinline__ void finish_row(const PagedAttnArgs& a, int64_t t, int h, int lane, const float (&acc)[D / 64], float m,
-                                           float l, bool shared) {
+                                           float l, int half, bool alone) {
     constexpr int RW = D / 64;
-    const int64_t row = t * a.heads + h;
-    if constexpr (MODE == kPre) {
+    if (MIX && !alone) {
+        const int64_t row = t * a.heads + h;
 #pragma unroll
-        for (int e = 0; e < RW; ++e) a.pre[row * D + RW * lane + e] = acc[e];
+        for (int e = 0; e < RW; ++e) a.kept[half][row * D + RW * lane + e] = acc[e];
         if (lane == 0) {
-            a.pre_ml[2 * row] = m;
-            a.pre_ml[2 * row + 1] = l;
+            a.kept_ml[half][2 * row] = m;
+            a.kept_ml[half][2 * row + 1] = l;
         }
         return;
-    }
-    float f = 1.0f, fp = 0.0f;
-    const bool join = MODE == kSuf && shared;
-    if (join) {
-        const float mp = a.pre_ml[2 * row], lp = a.pre_ml[2 * row + 1], mx = fmaxf(m, mp);
-        f = __builtin_amdgcn_exp2f(m - mx), fp = __builtin_amdgcn_exp2f(mp - mx);
-        l = l * f + lp * fp;
     }
     const float inv = inverse(l);
     uint16_t* dst = a.out + t * a.ld_out + h * D + RW * lane;
 #pragma unroll
-    for (int e = 0; e < RW; ++e)
-        dst[e] = bf16_rne_bits((join ? acc[e] * f + a.pre[row * D + RW * lane + e] * fp : acc[e]) * inv);
+    for (int e = 0; e < RW; ++e) dst[e] = bf16_rne_bits(acc[e] * inv);
 }
+
+// Where a row's part is: {first place, places, row of the tile, positions shared}. Places
+// are the streaming workgroups' (w's second, then the first ones of w + 1, ...) or, with
+// kTileRec in the row, the tiles' parts (a.kv_heads apart). No places: what it comes to
+// was kept, or (kDone) is the row's output.
+constexpr int kWhole = 0, kDone = -1, kTileRec = 1 << 16;
 
 // One sequence of a launch (lane's own): rows, positions and where they begin.
 struct SeqIn {
     int first, n, len;  // len: positions up to which it runs
     int seq;            // whose row of the table they are in
-    int from;           // kSuf: what precedes is shared; kPre: sequence behind the group's last
-    int lo;             // position of the first row (kPre: the lowest of any row, with a window)
+    int from;           // what precedes is shared; of a group: sequence behind its last
+    int lo;             // position of the first row (of a group: the lowest of any row, with a window)
     bool here, ok;      // has rows in the batch; well formed
 };
 
-// kMix: the groups take whole steps of 64, the sequences follow.
-__device__ __forceinline__ int group_steps(const PagedAttnArgs& a) { return (a.gr.n + 63) & ~63; }
-template <int MODE>
+// The groups take whole steps of 64, the sequences follow.
+template <bool MIX>
+__device__ __forceinline__ int group_steps(const PagedAttnArgs& a) {
+    return MIX ? (a.gr.n + 63) & ~63 : 0;
+}
+template <bool MIX>
 __device__ __forceinline__ int seq_count(const PagedAttnArgs& a) {
-    return MODE == kPre ? a.gr.n : (MODE == kMix ? group_steps(a) + a.b.B : a.b.B);
+    return group_steps<MIX>(a) + a.b.B;
 }
 
-// Sequence b of the launch, a lane each (b0 + lane, b0 uniform).
-template <int MODE>
-__device__ __forceinline__ SeqIn seq_in(const PagedAttnArgs& a, int b0, int lane) {
+// Group j0 + lane over what it shares (j0 uniform).
+__device__ __forceinline__ SeqIn group_in(const PagedAttnArgs& a, int j0, int lane) {
     SeqIn s{};
-    const int b = b0 + lane;
-    if constexpr (MODE == kPre) {
-        int end = 0;
-        if (b < a.gr.n) {
-            s.seq = a.gr.start[b];
-            end = a.gr.start[b + 1];
-            s.len = group_len(a.b, s.seq, end, a.gr.len[b]);
-            if (s.len > 0) {
-                s.first = a.b.q_start[s.seq];
-                s.n = a.b.q_start[end] - s.first;
-                s.here = s.first >= 0 && s.n > 0 && (int64_t)s.first + s.n <= a.b.T;
-                s.ok = true;
-                s.from = end;
-            }
-        }
-        if (a.window > 0) {
-            for (uint64_t left = __ballot(s.here); left; left &= left - 1) {
-                const int l = __builtin_ctzll(left);
-                const int hi = __builtin_amdgcn_readlane(end, l);
-                int low = INT_MAX;
-                for (int c = __builtin_amdgcn_readlane(s.seq, l) + lane; c < hi; c += 64) {
-                    const int n = a.b.q_start[c + 1] - a.b.q_start[c];
-                    if (n > 0) low = min(low, a.b.kv_len[c] - n);
-                }
-#pragma unroll
-                for (int o = 32; o; o >>= 1) low = min(low, __shfl_xor(low, o));
-                if (lane == l) s.lo = max(0, low);
-            }
-        }
-    } else {
-        if (b < a.b.B) {
-            s.seq = b;
-            s.first = a.b.q_start[b];
-            s.n = a.b.q_start[b + 1] - s.first;
-            s.len = a.b.kv_len[b];
+    const int j = j0 + lane;
+    int end = 0;
+    if (j < a.gr.n) {
+        s.seq = a.gr.start[j];
+        end = a.gr.start[j + 1];
+        s.len = group_len(a.b, s.seq, end, a.gr.len[j]);
+        if (s.len > 0) {
+            s.first = a.b.q_start[s.seq];
+            s.n = a.b.q_start[end] - s.first;
             s.here = s.first >= 0 && s.n > 0 && (int64_t)s.first + s.n <= a.b.T;
-            s.ok = s.n <= s.len && s.len <= a.b.max_pos;
-            s.lo = s.len - s.n;
+            s.ok = true;
+            s.from = end;
         }
-        if constexpr (MODE == kSuf) {
-            for (int j0 = 0; j0 < a.gr.n; j0 += 64) {
-                const int j = j0 + lane;
-                int lo = INT_MAX, hi = 0, len = 0;
-                if (j < a.gr.n) {
-                    lo = a.gr.start[j];
-                    hi = a.gr.start[j + 1];
-                    len = group_len(a.b, lo, hi, a.gr.len[j]);
-                }
-                int l = 0;  // the last group that begins at b or before
-#pragma unroll
-                for (int o = 32; o; o >>= 1)
-                    if (__shfl(lo, l + o) <= b) l += o;
-                const int end = __shfl(hi, l), shared = __shfl(len, l), begin = __shfl(lo, l);
-                if (begin <= b && b < end) s.from = shared;
+    }
+    if (a.window > 0) {
+        for (uint64_t left = __ballot(s.here); left; left &= left - 1) {
+            const int l = __builtin_ctzll(left);
+            const int hi = __builtin_amdgcn_readlane(end, l);
+            int low = INT_MAX;
+            for (int c = __builtin_amdgcn_readlane(s.seq, l) + lane; c < hi; c += 64) {
+                const int n = a.b.q_start[c + 1] - a.b.q_start[c];
+                if (n > 0) low = min(low, a.b.kv_len[c] - n);
             }
-            if (!s.ok) s.from = 0;
+#pragma unroll
+            for (int o = 32; o; o >>= 1) low = min(low, __shfl_xor(low, o));
+            if (lane == l) s.lo = max(0, low);
         }
     }
     return s;
 }
 
-// kPre: the positions of NR packed rows (lane's own each) of the sequences seq ..
+// Sequence b0 + lane of the batch (b0 uniform), behind what it shares.
+template <bool MIX>
+__device__ __forceinline__ SeqIn batch_in(const PagedAttnArgs& a, int b0, int lane) {
+    SeqIn s{};
+    const int b = b0 + lane;
+    if (b < a.b.B) {
+        s.seq = b;
+        s.first = a.b.q_start[b];
+        s.n = a.b.q_start[b + 1] - s.first;
+        s.len = a.b.kv_len[b];
+        s.here = s.first >= 0 && s.n > 0 && (int64_t)s.first + s.n <= a.b.T;
+        s.ok = s.n <= s.len && s.len <= a.b.max_pos;
+        s.lo = s.len - s.n;
+    }
+    if constexpr (MIX) {
+        for (int j0 = 0; j0 < a.gr.n; j0 += 64) {
+            const int j = j0 + lane;
+            int lo = INT_MAX, hi = 0, len = 0;
+            if (j < a.gr.n) {
+                lo = a.gr.start[j];
+                hi = a.gr.start[j + 1];
+                len = group_len(a.b, lo, hi, a.gr.len[j]);
+            }
+            int l = 0;  // the last group that begins at b or before
+#pragma unroll
+            for (int o = 32; o; o >>= 1)
+                if (__shfl(lo, l + o) <= b) l += o;
+            const int end = __shfl(hi, l), shared = __shfl(len, l), begin = __shfl(lo, l);
+            if (begin <= b && b < end) s.from = shared;
+        }
+        if (!s.ok) s.from = 0;
+    }
+    return s;
+}
+
+template <bool MIX>
+__device__ __forceinline__ SeqIn seq_in(const PagedAttnArgs& a, int b0, int lane) {
+    if constexpr (MIX)
+        if (b0 < group_steps<MIX>(a)) return group_in(a, b0, lane);
+    return batch_in<MIX>(a, b0 - group_steps<MIX>(a), lane);
+}
+
+// Of a group: the positions of NR packed rows (lane's own each) of the sequences seq ..
 // end - 1, by the whole wave.
 template <int NR>
 __device__ __forceinline__ void row_positions(const PagedAttnArgs& a, int seq, int end, const int (&t)[NR], int (&pos)[NR]) {
@@ -567,11 +560,6 @@ constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
 constexpr int kPartsPerTile = 64;
 constexpr int kTabInts = 8;  // an entry of the merges' tables
 
-// kMix: where a row's part is: {part of the tile's begin, its last part, row of the
-// tile, positions shared}; no last part where the whole tile was one workgroup's, which
-// kept what it comes to, or (nothing shared) wrote the output.
-constexpr int kWhole = -1, kDone = -2;
-
 struct Scan {
     RowsSeq s;          // this lane's sequence
     uint64_t incl;      // work of the sequences of this step up to and with this lane's
@@ -587,14 +575,10 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
     return ((uint64_t)hi << 32) | lo;
 }
 
-template <int ROWS, int UNIT, int MODE>
+template <int ROWS, int UNIT, bool MIX>
 __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int lane, uint64_t base, Scan& sc) {
-    const bool pre = MODE == kPre || (MODE == kMix && b0 < group_steps(a)), suf = MODE == kSuf || (MODE == kMix && !pre);
-    SeqIn in;
-    if constexpr (MODE == kMix)
-        in = pre ? seq_in<kPre>(a, b0, lane) : seq_in<kSuf>(a, b0 - group_steps(a), lane);
-    else
-        in = seq_in<MODE>(a, b0, lane);
+    const bool suf = MIX && b0 >= group_steps<MIX>(a);
+    const SeqIn in = seq_in<MIX>(a, b0, lane);
     RowsSeq s{};
     s.first = in.first, s.n = in.n, s.len = in.len, s.seq = in.seq, s.from = in.from;
     uint64_t w = 0;
@@ -606,8 +590,8 @@ __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int la
             if (suf) lo = a.sinks > s.from ? s.from : max(lo, s.from);
             s.ulo = lo / UNIT;
             s.us = suf ? 0 : min((min(a.sinks, lo) + UNIT - 1) / UNIT, s.ulo);
-            // (one at least: kPre may leave nothing within the window, kSuf nothing behind what is shared)
-            s.nu = s.us + max((s.len + UNIT - 1) / UNIT - s.ulo, MODE == kAll ? INT_MIN : s.us ? 0 : 1);
+            // (one at least: there may be nothing within the window, nothing behind what is shared)
+            s.nu = s.us + max((s.len + UNIT - 1) / UNIT - s.ulo, !MIX ? INT_MIN : s.us ? 0 : 1);
         } else {
             s.len = 0;  // malformed: one unit that sees nothing
             s.nu = 1;
@@ -628,14 +612,14 @@ __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int la
 }
 
 // The first step, and the work of the whole batch.
-template <int ROWS, int UNIT, int MODE>
+template <int ROWS, int UNIT, bool MIX>
 __device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, Scan& sc) {
-    scan_step<ROWS, UNIT, MODE>(a, 0, lane, 0, sc);
+    scan_step<ROWS, UNIT, MIX>(a, 0, lane, 0, sc);
     uint64_t total = sc.sum;
     uint32_t tiles = sc.s.nu ? min(sc.s.tiles, kPartsPerTile) : 0;
-    for (int b0 = 64; b0 < seq_count<MODE>(a); b0 += 64) {
+    for (int b0 = 64; b0 < seq_count<MIX>(a); b0 += 64) {
         Scan t;
-        scan_step<ROWS, UNIT, MODE>(a, b0, lane, 0, t);
+        scan_step<ROWS, UNIT, MIX>(a, b0, lane, 0, t);
         total = min(total + t.sum, (uint64_t)1 << 62);  // (sequences that overlap: no wrap)
         tiles = min(tiles + (t.s.nu ? min(t.s.tiles, kPartsPerTile) : 0), 1u << 24);
     }
@@ -657,15 +641,15 @@ struct Found {
 };
 
 // The tile and unit at place x of the line (x < total; calls with x rising).
-template <int ROWS, int UNIT, int MODE>
+template <int ROWS, int UNIT, bool MIX>
 __device__ __forceinline__ Found scan_find(const PagedAttnArgs& a, int lane, Scan& sc, uint64_t x) {
-    while (x >= sc.base + sc.sum) scan_step<ROWS, UNIT, MODE>(a, sc.b0 + 64, lane, sc.base + sc.sum, sc);
+    while (x >= sc.base + sc.sum) scan_step<ROWS, UNIT, MIX>(a, sc.b0 + 64, lane, sc.base + sc.sum, sc);
     const uint64_t m = __ballot(sc.base + sc.incl > x);
     const int l = __builtin_ctzll(m);
     Found f;
-    f.seq = MODE == kPre || MODE == kMix ? __builtin_amdgcn_readlane(sc.s.seq, l) : sc.b0 + l;
-    f.pre = MODE == kPre || (MODE == kMix && sc.b0 < group_steps(a));
-    f.s.from = MODE == kAll ? 0 : __builtin_amdgcn_readlane(sc.s.from, l);
+    f.seq = MIX ? __builtin_amdgcn_readlane(sc.s.seq, l) : sc.b0 + l;
+    f.pre = MIX && sc.b0 < group_steps<MIX>(a);
+    f.s.from = !MIX ? 0 : __builtin_amdgcn_readlane(sc.s.from, l);
     f.s.first = __builtin_amdgcn_readlane(sc.s.first, l);
     f.s.n = __builtin_amdgcn_readlane(sc.s.n, l);
     f.s.len = __builtin_amdgcn_readlane(sc.s.len, l);
@@ -708,7 +692,7 @@ __device__ __forceinline__ uint32_t part_count(uint64_t total, const Scan& sc, i
     return (uint32_t)min(min((uint64_t)grid, (uint64_t)sc.tiles * kPartsPerTile), total);
 }
 
-template <int D, int QT, bool E8, int MODE>
+template <int D, int QT, bool E8, bool MIX>
 __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_kernel(PagedAttnArgs a) {
     constexpr int NW = rows_waves(D, E8), NS = rows_stages(D), UNIT = rows_unit(D, E8), ROWS = 16 * QT;
     constexpr int BP = rows_block(E8), NH = BP / 16;  // positions of a block, 16 at a time (within a page)
@@ -724,12 +708,12 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, G = lane >> 4;
     Scan sc;
-    const uint64_t total = scan_all<ROWS, UNIT, MODE>(a, lane, sc);
+    const uint64_t total = scan_all<ROWS, UNIT, MIX>(a, lane, sc);
     const Cut cut = make_cut(total, part_count(total, sc, gridDim.x));
     // The tile that begins in this part and ends in a later one, for the merge: the last
-    // part it is in, first row of its sequence, tile, rows, kv head, shared.
+    // part it is in, first row of its sequence, tile, rows, kv head.
     [[maybe_unused]] int* const cut_tile = a.cuts + kTabInts * blockIdx.x;
-    if (MODE != kMix && threadIdx.x == 0) cut_tile[0] = 0;
+    if (!MIX && threadIdx.x == 0) cut_tile[0] = 0;
     if (blockIdx.x >= cut.n) return;
     uint64_t x = cut.begin(blockIdx.x);
     const uint64_t end = cut.begin(blockIdx.x + 1);
@@ -752,12 +736,12 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
     const uint32_t rd_v = vrow * (16 * NC) + ((E8 ? 0 : (col >> 1) & 1) ^ vz(vrow)) * 16 + (col & 1) * 8;
 
     while (x < end) {
-        const Found f = scan_find<ROWS, UNIT, MODE>(a, lane, sc, x);
+        const Found f = scan_find<ROWS, UNIT, MIX>(a, lane, sc, x);
         const int u0 = f.u, u1 = uniform((int)min((uint64_t)f.s.nu, u0 + (end - x)));
         x += u1 - u0;
         const int nrows = min(ROWS, f.s.n * a.g - f.rt * ROWS);
         const int nblk = f.s.len > 0 ? u1 - u0 : 0;  // this wave's blocks
-        const bool pre = MODE == kPre || (MODE == kMix && f.pre), suf = MODE == kSuf || (MODE == kMix && !f.pre);
+        const bool pre = MIX && f.pre, suf = MIX && !f.pre, alone = suf && f.s.from == 0;
         auto block_pos = [&](int j) {
             const int u = u0 + j;
             return (u < f.s.us ? u : u - f.s.us + f.s.ulo) * UNIT + BP * wave;
@@ -968,7 +952,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
                             for (int i = 0; i < 4; ++i) {
                                 const int p = 16 * hf + i;
                                 bool seen = (p <= hi) & ((p > lo) | (p < sk));
-                                if (MODE == kSuf || MODE == kMix) seen &= p >= begin;
+                                if (MIX) seen &= p >= begin;
                                 const float x = v[i];
                                 v[i] = seen ? x : -__builtin_inff();
                             }
@@ -1044,7 +1028,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
             if (j + NS < nblk) issue(j + NS);
         }
         };
-        if (MODE == kMix && QT > 1 && nrows <= 16)
+        if (MIX && QT > 1 && nrows <= 16)
             blocks(std::integral_constant<int, 1>());
         else
             blocks(std::integral_constant<int, QT>());
@@ -1072,17 +1056,17 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
 #pragma unroll
         for (int w = 0; w < NW; ++w) again |= odds[w] != 0;
         const bool whole = u0 == 0 && u1 == f.s.nu;
-        if constexpr (MODE == kMix) {
+        if constexpr (MIX) {
             for (int r = u0 == 0 ? tid : nrows; r < nrows; r += 64 * NW) {
                 const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
                 const int64_t row = (int64_t)(f.s.first + tok) * a.heads + h;
-                const int done = !pre && f.s.from == 0 ? kDone : kWhole;
+                const int places = (int)cut.part_of(f.tile0 + f.s.nu - 1) - (int)blockIdx.x + 1;
                 a.recs[(pre ? 0 : (int64_t)a.b.T * a.heads) + row] =
-                    int4{(int)blockIdx.x, whole ? done : (int)cut.part_of(f.tile0 + f.s.nu - 1), r, f.s.from};
+                    int4{(int)blockIdx.x, !whole ? places : (alone ? kDone : kWhole), r, f.s.from};
             }
         } else if (u0 == 0 && !whole && tid == 0) {
             cut_tile[0] = (int)cut.part_of(f.tile0 + f.s.nu - 1);
-            cut_tile[1] = f.s.first, cut_tile[2] = f.rt, cut_tile[3] = nrows, cut_tile[4] = f.kvh, cut_tile[5] = f.s.from;
+            cut_tile[1] = f.s.first, cut_tile[2] = f.rt, cut_tile[3] = nrows, cut_tile[4] = f.kvh;
         }
         float* part = a.part + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * rows_part(D, QT);
         if (again) {
@@ -1099,16 +1083,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
                 plain_row<D, E8>(a, f.seq, f.kvh, a.q + (int64_t)(f.s.first + tok) * a.ld_q + h * D, at, f.s.us, f.s.ulo, UNIT, u0, u1,
                              lane, acc, mr, lr);
                 if (whole) {
-                    if constexpr (MODE == kMix) {
-                        PagedAttnArgs to = a;  // (kPre keeps a row)
-                        to.pre = pre ? a.pre : a.suf, to.pre_ml = pre ? a.pre_ml : a.suf_ml;
-                        if (!pre && f.s.from == 0)
-                            finish_row<D, kAll>(a, f.s.first + tok, h, lane, acc, mr, lr, false);
-                        else
-                            finish_row<D, kPre>(to, f.s.first + tok, h, lane, acc, mr, lr, false);
-                    } else {
-                        finish_row<D, MODE>(a, f.s.first + tok, h, lane, acc, mr, lr, f.s.from > 0);
-                    }
+                    finish_row<D, MIX>(a, f.s.first + tok, h, lane, acc, mr, lr, !pre, alone);
                     continue;
                 }
 #pragma unroll
@@ -1147,14 +1122,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
             }
             if (whole) {
                 const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
-                if constexpr (MODE == kMix) {
-                    if (!pre && f.s.from == 0)
-                        finish4<D, kAll>(a, f.s.first + tok, h, d, v, mx, ls, false);
-                    else
-                        keep4<D>(pre ? a.pre : a.suf, pre ? a.pre_ml : a.suf_ml, (int64_t)(f.s.first + tok) * a.heads + h, d, v, mx, ls);
-                } else {
-                    finish4<D, MODE>(a, f.s.first + tok, h, d, v, mx, ls, f.s.from > 0);
-                }
+                finish4<D, MIX>(a, f.s.first + tok, h, d, v, mx, ls, !pre, alone);
             } else {
                 *reinterpret_cast<f32x4*>(part + (size_t)r * D + d) = v;
                 if (d == 0) {
@@ -1207,14 +1175,14 @@ __device__ __forceinline__ void join_parts(int n, int lane, ML ml, int gap, O o,
 // The cut tiles: a wave per row joins the parts of the tile that begins in part
 // blockIdx.x and ends in a later one, in the order of the line. (What the streaming
 // workgroups wrote of it is one trip to memory; the scan for it anew took 2 us.)
-template <int D, int QT, int MODE>
+template <int D, int QT>
 __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArgs a) {
     constexpr int ROWS = 16 * QT, RW = D / 64;
     const int lane = threadIdx.x & 63;
     const int r = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
     const int w = blockIdx.x;
     const int* e = a.cuts + kTabInts * w;
-    const int last = e[0], first = e[1], rt = e[2], nrows = e[3], kvh = e[4], from = e[5];
+    const int last = e[0], first = e[1], rt = e[2], nrows = e[3], kvh = e[4];
     if (last == 0 || r >= nrows) return;
     // Part w holds the tile's begin in its second place, the later ones theirs in the first.
     auto place = [&](int v) { return a.part + (size_t)(2 * (w + v) + (v == 0 ? 1 : 0)) * rows_part(D, QT); };
@@ -1223,36 +1191,60 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
         last - w + 1, lane, [&](int v) { return place(v) + ROWS * D + r; }, ROWS,
         [&](int v) { return place(v) + (size_t)r * D + RW * lane; }, acc, mx, ls);
     const int rr = r + rt * ROWS, tok = rr / a.g, h = kvh * a.g + (rr - tok * a.g);
-    finish_row<D, MODE>(a, first + tok, h, lane, acc, mx, ls, from > 0);
+    finish_row<D, false>(a, first + tok, h, lane, acc, mx, ls, 0, true);
 }
 
-// kMix: a wave per (row, head) joins its two parts, in the order shared, own. (Records of
-// sequences that are malformed may hold anything; they are not followed out of bounds.)
-template <int D, int QT>
-__global__ void __launch_bounds__(256) attn_paged_mix_merge_kernel(PagedAttnArgs a) {
-    constexpr int ROWS = 16 * QT, RW = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.b.T * a.heads;
-    if (row >= rows) return;
-    const int t = __builtin_amdgcn_readfirstlane((int)(row / a.heads)), h = __builtin_amdgcn_readfirstlane((int)(row % a.heads));
-    const int4 rp = a.recs[row], rs = a.recs[rows + row];
-    const SeqRows sr = find_row(a.b, t, lane);
-    if (sr.seq < 0 || sr.first < 0 || (int64_t)sr.first + sr.n > a.b.T) return;
-    if (uniform(rs.y) == kDone) return;
-    float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
-    auto add = [&](const int4& rec, const float* kept, const float* ml) {
-        const int w = uniform(rec.x), last = uniform(rec.y), r = uniform(rec.z);
-        if (w < 0 || w >= a.grid || r < 0 || r >= ROWS || last >= a.grid || (last != kWhole && last <= w)) return;
-        auto place = [&](int v) { return a.part + (size_t)(2 * (w + v) + (v == 0 ? 1 : 0)) * rows_part(D, QT); };
-        const bool whole = last == kWhole;
-        join_parts<RW>(
-            whole ? 1 : last - w + 1, lane, [&](int v) { return whole ? ml + 2 * row : place(v) + ROWS * D + r; },
-            whole ? 1 : ROWS, [&](int v) { return whole ? kept + row * D + RW * lane : place(v) + (size_t)r * D + RW * lane; },
-            acc, mx, ls);
-    };
-    if (uniform(rs.w) > 0) add(rp, a.pre, a.pre_ml);
-    add(rs, a.suf, a.suf_ml);
-    finish_row<D, kAll>(a, t, h, lane, acc, mx, ls, false);
+// MIX: the parts of every (row, head) joined, in the order shared, own: by a wave, or
+// (PG = 4: few rows, of many parts) by four, a quarter of each half's places each.
+// Records of sequences that are malformed may hold anything: they are not followed out
+// of bounds.
+template <int D, int QT, int PG>
+__global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
+    constexpr int ROWS = 16 * QT, RW = D / 64, TR = 128;
+    __shared__ float sums[PG > 1 ? PG : 1][D + 2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int part = PG > 1 ? wave : 0;
+    const int64_t rows = (int64_t)a.b.T * a.heads;
+    for (int64_t row = (int64_t)blockIdx.x * (4 / PG) + (PG > 1 ? 0 : wave); row < rows; row += (int64_t)gridDim.x * (4 / PG)) {
+        const int t = uniform((int)(row / a.heads)), h = uniform((int)(row % a.heads));
+        const int4 recs[2] = {a.recs[row], a.recs[rows + row]};
+        const SeqRows sr = find_row(a.b, t, lane);
+        if (sr.seq < 0 || sr.first < 0 || (int64_t)sr.first + sr.n > a.b.T || uniform(recs[1].y) == kDone) continue;
+        float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (half == 0 && uniform(recs[1].w) <= 0) continue;
+            const int w = uniform(recs[half].x), n = uniform(recs[half].y), r = uniform(recs[half].z) & (kTileRec - 1);
+            const bool tile = uniform(recs[half].z) & kTileRec, whole = n == kWhole;
+            const int last = tile ? w + (n - 1) * a.kv_heads : w + n - 1;
+            if (!whole && (n < 1 || w < 0 || r >= (tile ? TR : ROWS) || last < w || last >= (tile ? a.tile_places : a.grid))) continue;
+            const int lo = whole ? 0 : (int)((int64_t)n * part / PG), hi = whole ? part == 0 : (int)((int64_t)n * (part + 1) / PG);
+            auto at = [&](int v) {
+                return tile ? a.tile_part + (int64_t)(w + v * a.kv_heads) * (TR * (D + 2))
+                            : a.part + (size_t)(2 * (w + v) + (v == 0 ? 1 : 0)) * rows_part(D, QT);
+            };
+            join_parts<RW>(
+                hi - lo, lane, [&](int v) { return whole ? a.kept_ml[half] + 2 * row : at(lo + v) + (tile ? TR : ROWS) * D + r; },
+                whole ? 1 : (tile ? TR : ROWS),
+                [&](int v) { return (whole ? a.kept[half] + row * D : at(lo + v) + (size_t)r * D) + RW * lane; }, acc, mx, ls);
+        }
+        if constexpr (PG > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < RW; ++e) sums[wave][RW * lane + e] = acc[e];
+            if (lane == 0) {
+                sums[wave][D] = mx;
+                sums[wave][D + 1] = ls;
+            }
+            __syncthreads();
+            if (wave) continue;
+#pragma unroll
+            for (int e = 0; e < RW; ++e) acc[e] = 0.0f;
+            ls = 0.0f, mx = kNoMax;
+            join_parts<RW>(PG, lane, [&](int v) { return &sums[v][D]; }, 1, [&](int v) { return &sums[v][RW * lane]; }, acc, mx, ls);
+        }
+        finish_row<D, false>(a, t, h, lane, acc, mx, ls, 0, true);
+    }
 }
 
 // ---- many rows: a workgroup shares K and V tiles ------------------------------------------
@@ -1301,10 +1293,10 @@ struct TileScan {
     SeqIn s;
     int tiles, incl, sum;
 };
-template <int TR, int MODE>
+template <int TR, bool MIX>
 __device__ __forceinline__ TileScan tile_scan(const PagedAttnArgs& a, int b0, int lane) {
     TileScan t{};
-    t.s = seq_in<MODE>(a, b0, lane);
+    t.s = seq_in<MIX>(a, b0, lane);
     const int64_t rows = t.s.here ? (int64_t)t.s.n * a.g : 0;
     if (rows > a.row_limit) t.tiles = (int)((rows + TR - 1) / TR);
     int x = t.tiles;
@@ -1321,39 +1313,41 @@ __device__ __forceinline__ TileScan tile_scan(const PagedAttnArgs& a, int b0, in
 // The positions tile rt of a sequence runs over, in units of BN.
 struct TileSpan {
     int rows;            // of the tile
-    int pos_lo, pos_hi;  // of its first and last row (kPre: the lowest and the highest there can be)
+    int pos_lo, pos_hi;  // of its first and last row (of a group: the lowest and the highest there can be)
     int us, ulo, nu;
 };
-template <int TR, int BN, int MODE>
-__device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int len, bool ok, int from, int low, int rt) {
+template <int TR, int BN, bool MIX>
+__device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int len, bool ok, int from, int low, bool pre, int rt) {
     TileSpan s;
     const int r0 = rt * TR;  // (rows, of one kv head too, stay below 2^30)
     s.rows = min(TR, n * a.g - r0);
-    s.pos_lo = MODE == kPre ? low : len - n + r0 / a.g;
-    s.pos_hi = MODE == kPre ? len - 1 : len - n + (r0 + s.rows - 1) / a.g;
+    s.pos_lo = pre ? low : len - n + r0 / a.g;
+    s.pos_hi = pre ? len - 1 : len - n + (r0 + s.rows - 1) / a.g;
     int lo = a.window > 0 ? max(0, s.pos_lo + 1 - a.window) : 0;
-    if (MODE == kSuf) lo = a.sinks > from ? from : max(lo, from);
+    const bool suf = MIX && !pre;
+    if (suf) lo = a.sinks > from ? from : max(lo, from);
     s.ulo = lo / BN;
-    s.us = MODE == kSuf ? 0 : min((min(a.sinks, lo) + BN - 1) / BN, s.ulo);
-    s.nu = ok ? s.us + max(s.pos_hi / BN + 1 - s.ulo, MODE == kAll ? INT_MIN : 0) : 0;
+    s.us = suf ? 0 : min((min(a.sinks, lo) + BN - 1) / BN, s.ulo);
+    s.nu = ok ? s.us + max(s.pos_hi / BN + 1 - s.ulo, !MIX ? INT_MIN : 0) : 0;
     return s;
 }
 
 // Items (tiles times kv heads, times their parts) and where each is found: heaviest
 // (last) tiles first, kv heads side by side, so that the workgroups an XCD gets
 // in turn share theirs where there are eight.
-template <int TR, int MODE>
+template <int TR, bool MIX>
 __device__ __forceinline__ int tile_count(const PagedAttnArgs& a, const TileScan& sc0, int lane) {  // per kv head
     // (no more than there can be: sequences that overlap must not carry the sum away)
     int all = min(sc0.sum, a.max_tiles);
-    for (int b0 = 64; b0 < seq_count<MODE>(a); b0 += 64) all = min(all + tile_scan<TR, MODE>(a, b0, lane).sum, a.max_tiles);
+    for (int b0 = 64; b0 < seq_count<MIX>(a); b0 += 64) all = min(all + tile_scan<TR, MIX>(a, b0, lane).sum, a.max_tiles);
     return all;
 }
 
 // Where tile gt is (sc0: the first 64 sequences, read once for all that needs them).
-template <int TR, int BN, int MODE>
+template <int TR, int BN, bool MIX>
 struct TileAt {
     int seq, rt, first, n, len, from;
+    bool pre;
     TileSpan sp;
     __device__ __forceinline__ TileAt(const PagedAttnArgs& a, const TileScan& sc0, int gt, int lane) {
         int base = 0, b0 = 0;
@@ -1361,17 +1355,18 @@ struct TileAt {
         while (gt >= base + sc.sum) {
             base += sc.sum;
             b0 += 64;
-            sc = tile_scan<TR, MODE>(a, b0, lane);
+            sc = tile_scan<TR, MIX>(a, b0, lane);
         }
         const int l = __builtin_ctzll(__ballot(base + sc.incl > gt));
-        seq = MODE == kPre ? __builtin_amdgcn_readlane(sc.s.seq, l) : b0 + l;
+        seq = MIX ? __builtin_amdgcn_readlane(sc.s.seq, l) : b0 + l;
+        pre = MIX && b0 < group_steps<MIX>(a);
         first = __builtin_amdgcn_readlane(sc.s.first, l);
         n = __builtin_amdgcn_readlane(sc.s.n, l);
         len = __builtin_amdgcn_readlane(sc.s.len, l);
-        from = MODE == kAll ? 0 : __builtin_amdgcn_readlane(sc.s.from, l);
+        from = !MIX ? 0 : __builtin_amdgcn_readlane(sc.s.from, l);
         rt = gt - base - __builtin_amdgcn_readlane(sc.incl - sc.tiles, l);
-        sp = tile_span<TR, BN, MODE>(a, n, len, __builtin_amdgcn_readlane((int)sc.s.ok, l) != 0, from,
-                                     MODE == kPre ? __builtin_amdgcn_readlane(sc.s.lo, l) : 0, rt);
+        sp = tile_span<TR, BN, MIX>(a, n, len, __builtin_amdgcn_readlane((int)sc.s.ok, l) != 0, from,
+                                    MIX ? __builtin_amdgcn_readlane(sc.s.lo, l) : 0, pre, rt);
     }
 };
 
@@ -1388,7 +1383,7 @@ struct TileAt {
 constexpr int kSplitTiles = 512;  // at most, of one kv head
 constexpr int kMaxParts = 64;     // of a tile: a lane each in the merge
 constexpr int kMinCap = 2;        // (4: 380 tokens of 32 heads of 64 in 3 sequences 27 us for 21)
-// (entries: that of part 0, parts, first row of the sequence, tile, rows, kv head, shared)
+// (entries: that of part 0, parts, first row of the sequence, tile, rows, kv head)
 
 __device__ __forceinline__ int sum64(int v) {
 #pragma unroll
@@ -1397,11 +1392,11 @@ __device__ __forceinline__ int sum64(int v) {
 }
 
 // Units of every tile, into LDS, by all waves.
-template <int TR, int BN, int NW, int MODE>
+template <int TR, int BN, int NW, bool MIX>
 __device__ __forceinline__ void tile_units(const PagedAttnArgs& a, const TileScan& sc0, int tiles, int lane, int wave, int* nu) {
     int base = 0, turn = 0;
-    for (int b0 = 0; b0 < seq_count<MODE>(a) && base < tiles; b0 += 64) {
-        const TileScan sc = b0 ? tile_scan<TR, MODE>(a, b0, lane) : sc0;
+    for (int b0 = 0; b0 < seq_count<MIX>(a) && base < tiles; b0 += 64) {
+        const TileScan sc = b0 ? tile_scan<TR, MIX>(a, b0, lane) : sc0;
         for (int x0 = 0; x0 < sc.sum && base + x0 < tiles; x0 += 64, ++turn) {
             if (turn % NW != wave) continue;
             const int x = x0 + lane;
@@ -1412,9 +1407,9 @@ __device__ __forceinline__ void tile_units(const PagedAttnArgs& a, const TileSca
             l = min(l, 63);
             const int before = __shfl(sc.incl - sc.tiles, l), n = __shfl(sc.s.n, l), len = __shfl(sc.s.len, l);
             const bool ok = __shfl((int)sc.s.ok, l) != 0;
-            const int from = MODE == kSuf ? __shfl(sc.s.from, l) : 0, low = MODE == kPre ? __shfl(sc.s.lo, l) : 0;
+            const int from = MIX ? __shfl(sc.s.from, l) : 0, low = MIX ? __shfl(sc.s.lo, l) : 0;
             if (x < sc.sum && base + x < tiles)
-                nu[base + x] = tile_span<TR, BN, MODE>(a, n, len, ok, from, low, x - before).nu;
+                nu[base + x] = tile_span<TR, BN, MIX>(a, n, len, ok, from, low, MIX && b0 < group_steps<MIX>(a), x - before).nu;
         }
         base += sc.sum;
     }
@@ -1453,7 +1448,7 @@ __device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, i
     return INT_MAX / 2;
 }
 
-template <int D, bool E8, int MODE>
+template <int D, bool E8, bool MIX>
 __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan& sc0, int gt, int kvh, int split, int nsplit, int entry, int* tab, unsigned char* smem) {
     constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D);
     constexpr int DW = D / DS;            // this wave's columns of the output (and of its scores' products)
@@ -1473,15 +1468,23 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     const int rg = wave / DS, dh = wave % DS;
     const int col = lane & 31, h = lane >> 5;
 
-    const TileAt<TR, BN, MODE> at_item(a, sc0, gt, lane);
+    const TileAt<TR, BN, MIX> at_item(a, sc0, gt, lane);
     const int seq = at_item.seq, rt = at_item.rt;
     const int first = at_item.first, n = at_item.n, len = at_item.len, from = at_item.from;
+    const bool pre = MIX && at_item.pre, suf = MIX && !at_item.pre, alone = suf && from == 0;
     const TileSpan sp = at_item.sp;
     const int u0 = uniform((int)((int64_t)sp.nu * split / nsplit));
     const int u1 = uniform((int)((int64_t)sp.nu * (split + 1) / nsplit));
-    if (tab && split == 0 && tid == 0) {
+    if constexpr (MIX) {
+        for (int r = split == 0 ? tid : sp.rows; r < sp.rows; r += 64 * NW) {
+            const int rr = rt * TR + r;
+            const int64_t row = (int64_t)(first + rr / a.g) * a.heads + kvh * a.g + rr % a.g;
+            a.recs[(pre ? 0 : (int64_t)a.b.T * a.heads) + row] =
+                int4{entry, nsplit > 1 ? nsplit : (alone ? kDone : kWhole), r | kTileRec, from};
+        }
+    } else if (tab && split == 0 && tid == 0) {
         int* e = tab + kTabInts * (1 + gt * a.kv_heads + kvh);
-        e[0] = entry, e[1] = nsplit, e[2] = first, e[3] = rt, e[4] = sp.rows, e[5] = kvh, e[6] = from;
+        e[0] = entry, e[1] = nsplit, e[2] = first, e[3] = rt, e[4] = sp.rows, e[5] = kvh;
     }
 
     const int32_t* table = a.b.table + (int64_t)seq * a.b.ld_table;
@@ -1617,7 +1620,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     int wpos_lo = len - n + r0 / a.g;                        // lowest position up to which a row of the wave sees,
     int wpos_hi = len - n + (r0 + max(nrows, 1) - 1) / a.g;  // highest,
     int wpos_top = wpos_hi;                                  // and highest position of one
-    if constexpr (MODE == kPre) {
+    if (pre) {
         const int one[1] = {first + tok};
         int p[1];
         row_positions<1>(a, seq, from, one, p);
@@ -1701,17 +1704,17 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         float s[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = sv[i];
-        const bool masked = hole || p0 + 31 > wpos_lo || (MODE == kSuf && p0 < from) ||
+        const bool masked = hole || p0 + 31 > wpos_lo || (suf && p0 < from) ||
                             (a.window > 0 && p0 <= wpos_top - a.window && p0 + 31 >= a.sinks);
         if (masked) {
             // Relative to p0 + 4 h, so that positions are constants.
             const int at = cap - p0 - 4 * h, lo = a.window > 0 ? pos - p0 - 4 * h - a.window : INT_MIN, sk = a.sinks - p0 - 4 * h;
-            [[maybe_unused]] const int begin = from - p0 - 4 * h;
+            [[maybe_unused]] const int begin = (suf ? from : 0) - p0 - 4 * h;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int p = 8 * (i / 4) + i % 4, hi = hole >> (i / 8) & 1 ? -1 : at;
                 bool seen = (p <= hi) & ((p > lo) | (p < sk));
-                if constexpr (MODE == kSuf) seen &= p >= begin;
+                if constexpr (MIX) seen &= p >= begin;
                 s[i] = seen ? s[i] : -__builtin_inff();
             }
         }
@@ -1945,11 +1948,11 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         for (int r = 0; dh == 0 && r < nrows; ++r) {
             const int rr = r0 + r, tk = rr / a.g, hd = kvh * a.g + rr % a.g;
             float acc[D / 64], mr, lr;
-            const Sight at{__builtin_amdgcn_readlane(pos, r), __builtin_amdgcn_readlane(cap, r), MODE == kSuf ? from : 0};
+            const Sight at{__builtin_amdgcn_readlane(pos, r), __builtin_amdgcn_readlane(cap, r), suf ? from : 0};
             plain_row<D, E8>(a, seq, kvh, a.q + (int64_t)(first + tk) * a.ld_q + hd * D, at, sp.us, sp.ulo, BN, u0, u1, lane, acc,
                          mr, lr);
             if (nsplit == 1) {
-                finish_row<D, MODE>(a, first + tk, hd, lane, acc, mr, lr, from > 0);
+                finish_row<D, MIX>(a, first + tk, hd, lane, acc, mr, lr, !pre, alone);
                 continue;
             }
             float* pr = part + (32 * rg + r) * D + D / 64 * lane;
@@ -1969,8 +1972,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
         for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                finish4<D, MODE>(a, first + tok, head, dh * DW + 4 * h + 32 * d + 8 * k,
-                                 f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]}, m, l, from > 0);
+                finish4<D, MIX>(a, first + tok, head, dh * DW + 4 * h + 32 * d + 8 * k,
+                                f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]}, m, l, !pre, alone);
     } else {
         float* dst = part + (32 * rg + col) * D + dh * DW + 4 * h;
 #pragma unroll
@@ -1986,21 +1989,21 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     }
 }
 
-template <int D, bool E8, int MODE>
+template <int D, bool E8, bool MIX>
 __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kernel(PagedAttnArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int TR = tile_rows(D), BN = tile_bn(D);
     static_assert(tile_lds(D, E8) >= 4 * kSplitTiles, "the tiles' units");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const TileScan sc0 = tile_scan<TR, MODE>(a, 0, lane);
-    const int tiles = tile_count<TR, MODE>(a, sc0, lane), items = tiles * a.kv_heads;
+    const TileScan sc0 = tile_scan<TR, MIX>(a, 0, lane);
+    const int tiles = tile_count<TR, MIX>(a, sc0, lane), items = tiles * a.kv_heads;
     const bool split = items <= a.max_items;
     if (a.tab && blockIdx.x == 0 && tid == 0) a.tab[0] = split ? items : 0;
     if (items == 0) return;  // (the streaming kernel's all; there may be no slots to plan for)
     int gt, kvh, part = 0, parts = 1, entry = 0;
     if (split) {
         int* nu = reinterpret_cast<int*>(smem);
-        tile_units<TR, BN, tile_waves(D), MODE>(a, sc0, tiles, lane, wave, nu);
+        tile_units<TR, BN, tile_waves(D), MIX>(a, sc0, tiles, lane, wave, nu);
         int all;
         const int cap = tile_cap(a, nu, tiles, lane, all);
         const int e = all * a.kv_heads - 1 - (int)blockIdx.x;
@@ -2034,18 +2037,18 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
         kvh = item - gt * a.kv_heads;
     }
     // (tiles of more rows than max_q told of may be more than tab has entries for: they are not split)
-    tile_item<D, E8, MODE>(a, sc0, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), split ? a.tab : nullptr, smem);
+    tile_item<D, E8, MIX>(a, sc0, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), split ? a.tab : nullptr, smem);
 }
 
 // The parts of the tiles joined, `groups` workgroups to a tile, merge_rows(D) of
 // its rows at a time: the parts' factors first, a row per wave and a part per
 // lane, into LDS, then the outputs, 16 bytes per lane and part.
 constexpr int merge_rows(int D) { return 1024 / D; }
-template <int D, int PG, int MODE>
+template <int D, int PG>
 __global__ void __launch_bounds__((256 * PG)) attn_paged_tile_merge_kernel(PagedAttnArgs a, int groups) {
     constexpr int TR = tile_rows(D), R = merge_rows(D), C = D / 4;  // 16-byte pieces of a row
     __shared__ float fac[R][64];
-    __shared__ float tops[R], lsum[R];
+    __shared__ float inv[R];
     __shared__ f32x4 sums[PG > 1 ? PG - 1 : 1][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int item = blockIdx.x / groups;
@@ -2079,10 +2082,7 @@ __global__ void __launch_bounds__((256 * PG)) attn_paged_tile_merge_kernel(Paged
 #pragma unroll
             for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
             fac[w][lane] = f;
-            if (lane == 0) {
-                tops[w] = top;
-                lsum[w] = sum;
-            }
+            if (lane == 0) inv[w] = inverse(sum);
         }
         __syncthreads();
         for (int v0 = vlo; v0 < vhi; v0 += 8) {
@@ -2098,7 +2098,7 @@ __global__ void __launch_bounds__((256 * PG)) attn_paged_tile_merge_kernel(Paged
         }
         if (r < rows && tid < 256) {
             const int rr = rt * TR + r0 + r, tok = rr / a.g, head = kvh * a.g + rr % a.g;
-            finish4<D, MODE>(a, first + tok, head, 4 * c, acc, tops[r], lsum[r], e[6] > 0);
+            store4(a.out + (int64_t)(first + tok) * a.ld_out + head * D + 4 * c, acc, inv[r]);
         }
         __syncthreads();
     }
@@ -2164,20 +2164,41 @@ __attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B
     return p;
 }
 
-// kMix: where the sequences' own rows are the streaming kernel's and a group's fill no
-// more than two of its tiles (so that what is shared is read twice at most), that
-// `rows` of the average group come to; else qt is 0.
-__attribute__((unused)) AttnPlan mix_plan(const AttnPlan& suf, int heads, int kv_heads, int D, int T, int max_q, int groups) {
+// How the work of groups and sequences together (MIX) is spread: groups of few rows and
+// the sequences' own rows are streamed, more rows are tiles, which read K and V once for
+// 128 rows. (A streaming tile of more than 32 rows is bound by its products: 64 sequences
+// of three prompts, 88 rows of a group and kv head, 95 us streamed, 49 + 20 with tiles.)
+__attribute__((unused)) AttnPlan mix_plan(int heads, int kv_heads, int D, int B, int T, int max_q, int groups, bool e8) {
     AttnPlan p{};
-    const int64_t g = heads / kv_heads, rows = ((int64_t)T + groups - 1) / groups * g;
+    const int64_t g = heads / kv_heads, all = T * g;
+    max_q = std::min(max_q, T);
     const int qt_max = D <= 128 ? 4 : (D == 256 ? 2 : 1);
-    if (suf.qt == 0 || suf.grid_tiles || rows > 32 * qt_max || (int64_t)T * heads > 1 << 24) return p;
-    p = suf;
-    const int64_t r = std::max(std::min(rows, (int64_t)16 * qt_max), (int64_t)16 * suf.qt);
-    p.qt = r <= 16 ? 1 : (r <= 32 ? 2 : 4);
-    p.row_limit = INT64_MAX;
-    p.cuts_bytes = 0;
-    p.rows_bytes = p.part_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
+    const int64_t rows = (max_q > 0 ? max_q : ((int64_t)T + B - 1) / B) * g;  // of a sequence, as far as is known
+    const int64_t group_rows = ((int64_t)T + groups - 1) / groups * g;
+    const int64_t slots = (int64_t)device_cus() * (D == 512 ? 1 : 2), tr = 128;
+    auto tiles_of = [&](int64_t n, int64_t row_limit) { return (all / tr + std::min(n, all / (row_limit + 1) + 1)) * kv_heads; };
+    auto tiles_known = [&](int64_t n) { return max_q > 0 ? std::min(n, (int64_t)B * ((max_q * g + tr - 1) / tr) * kv_heads) : n; };
+    // (the sequences' rules are attn_plan's)
+    const bool few = tiles_known(tiles_of(B, 0)) <= slots / 2;
+    const bool seq_tiles = rows > (few ? (D == 512 ? 15 : 16) : 16 * qt_max);
+    const bool group_tiles = seq_tiles || group_rows > 16 * std::min(qt_max, 2);
+    if (!seq_tiles) {
+        const int64_t r = group_tiles ? rows : std::max(rows, group_rows);
+        p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
+        p.row_limit = group_tiles ? 16 * p.qt : INT64_MAX;
+        p.grid = device_cus() * rows_groups(D, e8);
+        p.rows_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
+    }
+    p.part_bytes = p.rows_bytes;
+    if (group_tiles) {
+        p.grid_tiles = tiles_of(groups, p.row_limit) + tiles_of(B, p.row_limit);
+        const bool own = seq_tiles || max_q == 0 || max_q * g > p.row_limit;  // sequences that are tiles
+        p.tiles = std::min(p.grid_tiles, tiles_of(groups, p.row_limit) + (own ? tiles_known(tiles_of(B, p.row_limit)) : 0));
+        if (p.tiles <= slots / 2 && p.tiles <= kSplitTiles) {
+            p.slots = (int)slots;
+            p.part_bytes += std::min((uint64_t)slots * 2, (uint64_t)p.tiles * kMaxParts) * tr * (D + 2) * sizeof(float);
+        }
+    }
     return p;
 }
 
@@ -2192,65 +2213,79 @@ __attribute__((unused)) int allow_lds(const void* k, int lds, std::atomic<uint64
     return ALV_OK;
 }
 
-template <int D, int QT, bool E8, int MODE>
+template <int D, int QT, bool E8, bool MIX>
 int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     constexpr int lds = rows_lds(D, QT, E8);
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, E8, MODE>), lds, done)) return rc;
-    hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MODE>), dim3(p.grid), dim3(64 * rows_waves(D, E8)), lds, s, a);
+    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, E8, MIX>), lds, done)) return rc;
+    hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MIX>), dim3(p.grid), dim3(64 * rows_waves(D, E8)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_rows_kernel launch")) return rc;
-    if constexpr (MODE == kMix) {
-        hipLaunchKernelGGL((attn_paged_mix_merge_kernel<D, QT>), dim3((uint32_t)(((int64_t)a.b.T * a.heads + 3) / 4)), dim3(256), 0, s, a);
-        return hip_check(hipGetLastError(), "attn_paged_mix_merge_kernel launch");
-    }
-    hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT, MODE>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a);
+    if (MIX) return ALV_OK;
+    hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "attn_paged_rows_merge_kernel launch");
 }
 
-template <int D, bool E8, int MODE>
+template <int D, bool E8, bool MIX>
 int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     constexpr int lds = tile_lds(D, E8);
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D, E8, MODE>), lds, done)) return rc;
-    hipLaunchKernelGGL((attn_paged_tile_kernel<D, E8, MODE>), dim3((uint32_t)std::max(p.grid_tiles, (int64_t)p.slots * 2)), dim3(64 * tile_waves(D)), lds, s, a);
+    if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D, E8, MIX>), lds, done)) return rc;
+    hipLaunchKernelGGL((attn_paged_tile_kernel<D, E8, MIX>), dim3((uint32_t)std::max(p.grid_tiles, (int64_t)p.slots * 2)), dim3(64 * tile_waves(D)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_tile_kernel launch")) return rc;
-    if (p.slots == 0) return ALV_OK;
+    if (MIX || p.slots == 0) return ALV_OK;
     // Few tiles are joined by as many workgroups as they have rows for, many by fewer
     // each (a tile in one part costs its workgroups two loads).
     const int groups = (int)std::max((int64_t)1, std::min((int64_t)tile_rows(D) / merge_rows(D), 4096 / p.tiles));
     // Four groups of threads share many parts (drafts over 4 long contexts, 64 parts:
     // 12.5 -> 10.5 us; 16 parts of 32 tiles, D = 256: 15.5 -> 21.4).
     if (p.slots / p.tiles >= 32)
-        hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D, 4, MODE>), dim3((uint32_t)p.tiles * groups), dim3(1024), 0, s, a, groups);
+        hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D, 4>), dim3((uint32_t)p.tiles * groups), dim3(1024), 0, s, a, groups);
     else
-        hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D, 1, MODE>), dim3((uint32_t)p.tiles * groups), dim3(256), 0, s, a, groups);
+        hipLaunchKernelGGL((attn_paged_tile_merge_kernel<D, 1>), dim3((uint32_t)p.tiles * groups), dim3(256), 0, s, a, groups);
     return hip_check(hipGetLastError(), "attn_paged_tile_merge_kernel launch");
 }
 
-template <int D, bool E8, int MODE>
+template <int D, bool E8, bool MIX>
 int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
     a.grid = p.grid;
+    a.tile_places = p.slots ? (int)std::min((int64_t)p.slots * 2, p.tiles * kMaxParts) : 0;
     a.row_limit = p.row_limit;
     a.slots = p.slots;
     a.max_items = p.slots ? (int)p.tiles : 0;
     a.max_tiles = (int)(p.grid_tiles / a.kv_heads);
     float* part = a.part;
-    if constexpr (MODE != kMix)
-        if (p.grid_tiles) {
-            if (p.slots) a.tab = reinterpret_cast<int*>(part + p.rows_bytes / sizeof(float));
-            a.part = part + (p.rows_bytes + p.tab_bytes) / sizeof(float);
-            if (int rc = launch_tiles<D, E8, MODE>(a, p, s)) return rc;
-        }
+    a.tile_part = part + (p.rows_bytes + p.tab_bytes) / sizeof(float);
+    if (p.grid_tiles) {
+        if (!MIX && p.slots) a.tab = reinterpret_cast<int*>(part + p.rows_bytes / sizeof(float));
+        a.part = a.tile_part;
+        if (int rc = launch_tiles<D, E8, MIX>(a, p, s)) return rc;
+    }
     a.cuts = reinterpret_cast<int*>(part);
     a.part = part + p.cuts_bytes / sizeof(float);
-    if (p.qt == 1) return launch_rows<D, 1, E8, MODE>(a, p, s);
+    auto join = [&](auto qt) {
+        if constexpr (!MIX) return ALV_OK;
+        // Four waves to a row where rows are few (8 samples of one prompt, 32 rows: 11 us, 6).
+        const int64_t rows = (int64_t)a.b.T * a.heads;
+        constexpr int QT = decltype(qt)::value;
+        if (rows <= 8192)
+            hipLaunchKernelGGL((attn_paged_join_kernel<D, QT, 4>), dim3((uint32_t)rows), dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL((attn_paged_join_kernel<D, QT, 1>), dim3((uint32_t)std::min((rows + 3) / 4, (int64_t)1 << 22)),
+                               dim3(256), 0, s, a);
+        return hip_check(hipGetLastError(), "attn_paged_join_kernel launch");
+    };
+    auto rows_run = [&](auto qt) {
+        if (p.qt)
+            if (int rc = launch_rows<D, decltype(qt)::value, E8, MIX>(a, p, s)) return rc;
+        return join(qt);
+    };
     if constexpr (D <= 256)
-        if (p.qt == 2) return launch_rows<D, 2, E8, MODE>(a, p, s);
+        if (p.qt == 2) return rows_run(std::integral_constant<int, 2>());
     if constexpr (D <= 128)
-        if (p.qt == 4) return launch_rows<D, 4, E8, MODE>(a, p, s);
-    return ALV_OK;
+        if (p.qt == 4) return rows_run(std::integral_constant<int, 4>());
+    return rows_run(std::integral_constant<int, 1>());
 }
 
 // The arguments' checks that all attention entries share, and what they fill in of
@@ -2303,13 +2338,13 @@ __attribute__((unused)) int attn_workspace(const void* workspace, uint64_t have,
     return ALV_OK;
 }
 
-template <bool E8, int MODE>
+template <bool E8, bool MIX>
 int attn_launch(const PagedAttnArgs& a, int D, const AttnPlan& p, hipStream_t s) {
     switch (D) {
-        case 64: return launch_d<64, E8, MODE>(a, p, s);
-        case 128: return launch_d<128, E8, MODE>(a, p, s);
-        case 256: return launch_d<256, E8, MODE>(a, p, s);
-        default: return launch_d<512, E8, MODE>(a, p, s);
+        case 64: return launch_d<64, E8, MIX>(a, p, s);
+        case 128: return launch_d<128, E8, MIX>(a, p, s);
+        case 256: return launch_d<256, E8, MIX>(a, p, s);
+        default: return launch_d<512, E8, MIX>(a, p, s);
     }
 }
 

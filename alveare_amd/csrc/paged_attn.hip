@@ -24,5 +24,5 @@ extern "C" int alv_attention_paged(const uint16_t* q, int64_t ld_q, const uint16
     if (int rc = attn_fits(p, T, heads, B)) return rc;
     if (int rc = attn_workspace(workspace, workspace_bytes, p.part_bytes)) return rc;
     a.part = static_cast<float*>(workspace);
-    return attn_launch<false, kAll>(a, D, p, (hipStream_t)stream);
+    return attn_launch<false, false>(a, D, p, (hipStream_t)stream);
 }

@@ -26,5 +26,5 @@ extern "C" int alv_attention_paged8(const uint16_t* q, int64_t ld_q, const uint8
     if (int rc = attn_fits(p, T, heads, B)) return rc;
     if (int rc = attn_workspace(workspace, workspace_bytes, p.part_bytes)) return rc;
     a.part = static_cast<float*>(workspace);
-    return attn_launch<true, kAll>(a, D, p, (hipStream_t)stream);
+    return attn_launch<true, false>(a, D, p, (hipStream_t)stream);
 }

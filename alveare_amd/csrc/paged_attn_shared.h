@@ -1,5 +1,4 @@
-// Attention of sequences that share their first pages (paged_attn.h): one run over
-// the groups, one over what is behind what they share.
+// Attention of sequences that share their first pages (paged_attn.h).
 #pragma once
 
 #include "paged_attn.h"
@@ -37,35 +36,25 @@ int attention_shared8(const SharedCall& c);  // of 8-bit pages
 
 namespace {
 
-// Two runs: what kPre leaves (D values, a maximum and a sum for each row and head),
-// then the runs' own workspace, one after the other's. One (mix.qt > 0): what is kept
-// of both parts of a row, where they are, then the line's parts.
+// The workspace: where the parts of each (row, head) are, what is kept of them (D values,
+// a maximum and a sum, for both halves), then the kernels' parts.
 struct SharedPlan {
-    AttnPlan pre, suf, mix;
+    AttnPlan p;
     uint64_t rec_bytes, kept_bytes, bytes;
 };
 
 __attribute__((unused)) SharedPlan shared_plan(int heads, int kv_heads, int D, int B, int T, int max_q, int groups, bool e8) {
-    SharedPlan p{};
-    p.suf = attn_plan(heads, kv_heads, D, B, T, max_q, e8);
-    p.bytes = p.suf.part_bytes;
-    if (groups > 0) {
-        p.kept_bytes = ((uint64_t)T * heads * (D + 2) * sizeof(float) + 15) / 16 * 16;
-        p.mix = mix_plan(p.suf, heads, kv_heads, D, T, max_q, groups);
-        if (p.mix.qt) {
-            p.rec_bytes = 2 * (uint64_t)T * heads * sizeof(int4);
-            p.bytes = p.rec_bytes + 2 * p.kept_bytes + p.mix.part_bytes;
-        } else {
-            p.pre = attn_plan(heads, kv_heads, D, groups, T, 0, e8);
-            p.bytes = p.kept_bytes + std::max(p.pre.part_bytes, p.suf.part_bytes);
-        }
-    }
-    return p;
+    SharedPlan s{};
+    s.p = mix_plan(heads, kv_heads, D, B, T, max_q, groups, e8);
+    s.rec_bytes = 2 * (uint64_t)T * heads * sizeof(int4);
+    s.kept_bytes = ((uint64_t)T * heads * (D + 2) * sizeof(float) + 15) / 16 * 16;
+    s.bytes = s.rec_bytes + 2 * s.kept_bytes + s.p.part_bytes;
+    return s;
 }
 
 template <bool E8>
-int attention_shared(const SharedCall& c) {
-    if (c.groups < 0 || (c.groups > 0 && (!c.group_start || !c.shared_len))) return fail(ALV_ERR_ARG, "bad groups: %d", c.groups);
+int attention_shared(const SharedCall& c) {  // of one group at least
+    if (!c.group_start || !c.shared_len) return fail(ALV_ERR_ARG, "null pointer");
     if (reinterpret_cast<uintptr_t>(c.group_start) % 4 || reinterpret_cast<uintptr_t>(c.shared_len) % 4)
         return fail(ALV_ERR_ALIGN, "group_start and shared_len need 4-byte alignment");
     PagedAttnArgs a{};
@@ -78,26 +67,20 @@ int attention_shared(const SharedCall& c) {
         return rc;
     if (c.T == 0) return ALV_OK;
     const SharedPlan p = shared_plan(c.heads, c.kv_heads, c.D, c.B, c.T, c.max_q, c.groups, E8);
-    if (int rc = attn_fits(p.pre, c.T, c.heads, c.groups)) return rc;
-    if (int rc = attn_fits(p.suf, c.T, c.heads, c.B)) return rc;
+    if (int rc = attn_fits(p.p, c.T, c.heads, c.B)) return rc;
     if (int rc = attn_workspace(c.workspace, c.workspace_bytes, p.bytes)) return rc;
     const hipStream_t s = (hipStream_t)c.stream;
     a.part = static_cast<float*>(c.workspace);
-    if (c.groups == 0) return attn_launch<E8, kSuf>(a, c.D, p.suf, s);
     a.gr = PagedGroups{c.group_start, c.shared_len, c.groups};
     const int64_t rows = (int64_t)c.T * c.heads;
     a.recs = reinterpret_cast<int4*>(c.workspace);
-    a.pre = a.part + p.rec_bytes / sizeof(float);
-    a.pre_ml = a.pre + rows * c.D;
-    a.suf = a.pre + p.kept_bytes / sizeof(float);
-    a.suf_ml = a.suf + rows * c.D;
-    if (p.mix.qt) {
-        a.part = a.suf + p.kept_bytes / sizeof(float);
-        return attn_launch<E8, kMix>(a, c.D, p.mix, s);
+    a.part += p.rec_bytes / sizeof(float);
+    for (int half = 0; half < 2; ++half) {
+        a.kept[half] = a.part;
+        a.kept_ml[half] = a.part + rows * c.D;
+        a.part += p.kept_bytes / sizeof(float);
     }
-    a.part = a.suf;
-    if (int rc = attn_launch<E8, kPre>(a, c.D, p.pre, s)) return rc;
-    return attn_launch<E8, kSuf>(a, c.D, p.suf, s);
+    return attn_launch<E8, true>(a, c.D, p.p, s);
 }
 
 }  // namespace

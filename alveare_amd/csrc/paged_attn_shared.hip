@@ -7,6 +7,9 @@ extern "C" uint64_t alv_attention_shared_workspace(int heads, int kv_heads, int 
     if (heads < 1 || heads > kMaxHeads || kv_heads < 1 || heads % kv_heads || D < 1 || D > 512 || B < 1 || T < 1 || max_q < 0 ||
         groups < 0)
         return 0;
+    if (groups == 0)
+        return std::max(alv_attention_paged_workspace(heads, kv_heads, D, B, T, max_q),
+                        alv_attention_paged8_workspace(heads, kv_heads, D, B, T, max_q));
     return std::max(shared_plan(heads, kv_heads, D, B, T, max_q, groups, false).bytes,
                     shared_plan(heads, kv_heads, D, B, T, max_q, groups, true).bytes);
 }
@@ -18,6 +21,16 @@ extern "C" int alv_attention_shared(const uint16_t* q, int64_t ld_q, const void*
                                     const int32_t* shared_len, int groups, int heads, int kv_heads, int D, int window,
                                     int sinks, float scale, uint16_t* out, int64_t ld_out, void* workspace,
                                     uint64_t workspace_bytes, void* stream) {
+    if (groups < 0) return fail(ALV_ERR_ARG, "bad groups: %d", groups);
+    if (groups == 0 && scales)
+        return alv_attention_paged8(q, ld_q, static_cast<const uint8_t*>(kpages), static_cast<const uint8_t*>(vpages), k_stride,
+                                    v_stride, scales, s_stride, pages, page_size, page_table, ld_table, max_pages, q_start,
+                                    kv_len, B, T, max_q, heads, kv_heads, D, window, sinks, scale, out, ld_out, workspace,
+                                    workspace_bytes, stream);
+    if (groups == 0)
+        return alv_attention_paged(q, ld_q, static_cast<const uint16_t*>(kpages), static_cast<const uint16_t*>(vpages), k_stride,
+                                   v_stride, pages, page_size, page_table, ld_table, max_pages, q_start, kv_len, B, T, max_q,
+                                   heads, kv_heads, D, window, sinks, scale, out, ld_out, workspace, workspace_bytes, stream);
     const SharedCall c{q, ld_q, kpages, vpages, k_stride, v_stride, scales, s_stride, pages, page_size, page_table, ld_table,
                        max_pages, q_start, kv_len, B, T, max_q, group_start, shared_len, groups, heads, kv_heads, D, window,
                        sinks, scale, out, ld_out, workspace, workspace_bytes, stream};
