@@ -534,25 +534,25 @@ struct RowsSeq {
     int us, ulo, nu;  // units of first tokens; first unit of the window; units in all
 };
 
-constexpr int rows_groups(int D, bool E8) { return E8 && D <= 256 ? 2 : 1; }  // workgroups per CU
-constexpr int rows_waves(int D, bool E8) { return (D == 512 ? 2 : (D == 64 ? 8 : 4)) / rows_groups(D, E8); }
+constexpr bool rows_two(int D, bool E8) { return E8 && D <= 256; }  // two workgroups per CU, else one
+constexpr int rows_waves(int D, bool TWO) { return (D == 512 ? 2 : (D == 64 ? 8 : 4)) / (TWO ? 2 : 1); }
 // A wave's block: 16 positions' K and V, or 32 of 8-bit ones and their powers.
 constexpr int rows_block(bool E8) { return E8 ? 32 : 16; }
 constexpr int rows_stage(int D, bool E8) { return 64 * D + (E8 ? 64 : 0); }
 constexpr int rows_stages(int D) { return 131072 / (rows_waves(D, false) * 64 * D); }
-constexpr int rows_unit(int D, bool E8) { return rows_block(E8) * rows_waves(D, E8); }
+constexpr int rows_unit(int D, bool E8, bool TWO) { return rows_block(E8) * rows_waves(D, TWO); }
 // The waves' outputs at a tile's end, rows padded to spread over the banks.
 constexpr int rows_out_ld(int D) { return D + 4; }
 // Whether q's operands stay in LDS rather than registers: where they and the
 // output take more than half of a wave's 256 (the rest would spill).
 constexpr bool rows_q_lds(int D, int QT) { return QT * D > 256; }
-constexpr int rows_lds(int D, int QT, bool E8) {
-    const int ring = rows_waves(D, E8) * rows_stages(D) * rows_stage(D, E8);
-    const int outs = rows_waves(D, E8) * 16 * QT * (rows_out_ld(D) * 4);
-    return (ring > outs ? ring : outs) + 2 * rows_waves(D, E8) * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0) + 16;
+constexpr int rows_lds(int D, int QT, bool E8, bool TWO) {
+    const int NW = rows_waves(D, TWO), ring = NW * rows_stages(D) * rows_stage(D, E8);
+    const int outs = NW * 16 * QT * (rows_out_ld(D) * 4);
+    return (ring > outs ? ring : outs) + 2 * NW * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0) + 16;
 }
-constexpr int rows_mls(int D, int QT, bool E8) {  // where the waves' maxima and sums stand; q behind them
-    return rows_lds(D, QT, E8) - 16 - 2 * rows_waves(D, E8) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
+constexpr int rows_mls(int D, int QT, bool E8, bool TWO) {  // where the waves' maxima and sums stand; q behind them
+    return rows_lds(D, QT, E8, TWO) - 16 - 2 * rows_waves(D, TWO) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
 }
 // Floats of one workspace place: outputs, maxima, sums.
 constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
@@ -693,8 +693,9 @@ __device__ __forceinline__ uint32_t part_count(uint64_t total, const Scan& sc, i
 }
 
 template <int D, int QT, bool E8, bool MIX>
-__global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_kernel(PagedAttnArgs a) {
-    constexpr int NW = rows_waves(D, E8), NS = rows_stages(D), UNIT = rows_unit(D, E8), ROWS = 16 * QT;
+__global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn_paged_rows_kernel(PagedAttnArgs a) {
+    constexpr bool TWO = rows_two(D, E8);
+    constexpr int NW = rows_waves(D, TWO), NS = rows_stages(D), UNIT = rows_unit(D, E8, TWO), ROWS = 16 * QT;
     constexpr int BP = rows_block(E8), NH = BP / 16;  // positions of a block, 16 at a time (within a page)
     constexpr int STAGE = rows_stage(D, E8);
     constexpr int NC = E8 ? D / 16 : D / 8;  // 16-byte pieces of a row
@@ -720,8 +721,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
 
     unsigned char* ring = smem + wave * NS * STAGE;
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
-    float* mls = reinterpret_cast<float*>(smem + rows_mls(D, QT, E8));  // [wave][max | sum][row]
-    int* odds = reinterpret_cast<int*>(smem + rows_lds(D, QT, E8) - 16);
+    float* mls = reinterpret_cast<float*>(smem + rows_mls(D, QT, E8, TWO));  // [wave][max | sum][row]
+    int* odds = reinterpret_cast<int*>(smem + rows_lds(D, QT, E8, TWO) - 16);
     const float c = fmaxf(a.scale * kLog2e, kMinScale);
     const int S = 1 << a.b.shift;
     // Byte offsets that stay: this lane's piece of a load (memory side), of a K
@@ -824,7 +825,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
         int row_t[QT];
         constexpr bool QL = rows_q_lds(D, QT);
         bf16x8 q[QL ? 1 : QT][QL ? 1 : D / 32];
-        u32x4* qs = reinterpret_cast<u32x4*>(smem + rows_mls(D, QT, E8) + 2 * NW * ROWS * 4) + lane;
+        u32x4* qs = reinterpret_cast<u32x4*>(smem + rows_mls(D, QT, E8, TWO) + 2 * NW * ROWS * 4) + lane;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const int r = min(16 * t + col, nrows - 1) + f.rt * ROWS;
@@ -1136,18 +1137,17 @@ __global__ void __launch_bounds__((64 * rows_waves(D, E8)), 2) attn_paged_rows_k
 }
 
 // acc, l of n parts rescaled to the largest maximum and added in order, by one
-// wave: the maxima and sums 64 parts at a time, a part per lane (ml(v) points to
-// part v's maximum, its sum `gap` floats behind), then eight parts' outputs (o(v)
-// points to this lane's) on their way at once.
-template <int RW, class ML, class O>
-__device__ __forceinline__ void join_parts(int n, int lane, ML ml, int gap, O o, float (&acc)[RW], float& mx, float& l) {
+// wave: the maxima and sums 64 parts at a time, a part per lane (top(v) points to
+// part v's maximum, sum(v) to its sum), then eight parts' outputs (o(v) points to
+// this lane's) on their way at once.
+template <int RW, class M, class L, class O>
+__device__ __forceinline__ void join_parts(int n, int lane, M top_of, L sum_of, O o, float (&acc)[RW], float& mx, float& l) {
     for (int v0 = 0; v0 < n; v0 += 64) {
         const int c = min(64, n - v0);
         float m = kNoMax, s = 0.0f;
         if (lane < c) {
-            const float* p = ml(v0 + lane);
-            m = p[0];
-            s = p[gap];
+            m = *top_of(v0 + lane);
+            s = *sum_of(v0 + lane);
         }
         float top = m;
         for (int k = 32; k; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
@@ -1188,7 +1188,7 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
     auto place = [&](int v) { return a.part + (size_t)(2 * (w + v) + (v == 0 ? 1 : 0)) * rows_part(D, QT); };
     float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
     join_parts<RW>(
-        last - w + 1, lane, [&](int v) { return place(v) + ROWS * D + r; }, ROWS,
+        last - w + 1, lane, [&](int v) { return place(v) + ROWS * D + r; }, [&](int v) { return place(v) + ROWS * (D + 1) + r; },
         [&](int v) { return place(v) + (size_t)r * D + RW * lane; }, acc, mx, ls);
     const int rr = r + rt * ROWS, tok = rr / a.g, h = kvh * a.g + (rr - tok * a.g);
     finish_row<D, false>(a, first + tok, h, lane, acc, mx, ls, 0, true);
@@ -1211,23 +1211,46 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
         const SeqRows sr = find_row(a.b, t, lane);
         if (sr.seq < 0 || sr.first < 0 || (int64_t)sr.first + sr.n > a.b.T || uniform(recs[1].y) == kDone) continue;
         float acc[RW] = {}, ls = 0.0f, mx = kNoMax;
+        // The places of both halves as one list (a whole part is one place).
+        struct {
+            int w, n, r, rows;
+            bool tile, whole;
+        } x[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            if (half == 0 && uniform(recs[1].w) <= 0) continue;
-            const int w = uniform(recs[half].x), n = uniform(recs[half].y), r = uniform(recs[half].z) & (kTileRec - 1);
-            const bool tile = uniform(recs[half].z) & kTileRec, whole = n == kWhole;
-            const int last = tile ? w + (n - 1) * a.kv_heads : w + n - 1;
-            if (!whole && (n < 1 || w < 0 || r >= (tile ? TR : ROWS) || last < w || last >= (tile ? a.tile_places : a.grid))) continue;
-            const int lo = whole ? 0 : (int)((int64_t)n * part / PG), hi = whole ? part == 0 : (int)((int64_t)n * (part + 1) / PG);
-            auto at = [&](int v) {
-                return tile ? a.tile_part + (int64_t)(w + v * a.kv_heads) * (TR * (D + 2))
-                            : a.part + (size_t)(2 * (w + v) + (v == 0 ? 1 : 0)) * rows_part(D, QT);
-            };
-            join_parts<RW>(
-                hi - lo, lane, [&](int v) { return whole ? a.kept_ml[half] + 2 * row : at(lo + v) + (tile ? TR : ROWS) * D + r; },
-                whole ? 1 : (tile ? TR : ROWS),
-                [&](int v) { return (whole ? a.kept[half] + row * D : at(lo + v) + (size_t)r * D) + RW * lane; }, acc, mx, ls);
+            auto& p = x[half];
+            p.w = uniform(recs[half].x), p.n = uniform(recs[half].y), p.r = uniform(recs[half].z) & (kTileRec - 1);
+            p.tile = uniform(recs[half].z) & kTileRec, p.whole = p.n == kWhole;
+            p.rows = p.tile ? TR : ROWS;
+            const int last = p.tile ? p.w + (p.n - 1) * a.kv_heads : p.w + p.n - 1;
+            if (p.whole)
+                p.n = 1;
+            else if (p.n < 1 || p.w < 0 || p.r >= p.rows || last < p.w || last >= (p.tile ? a.tile_places : a.grid))
+                p.n = 0;
         }
+        if (uniform(recs[1].w) <= 0) x[0].n = 0;
+        const int n = x[0].n + x[1].n;
+        auto from = [&](int half, int v) {
+            const auto& p = x[half];
+            return p.tile ? a.tile_part + (int64_t)(p.w + v * a.kv_heads) * (TR * (D + 2))
+                          : a.part + (size_t)(2 * (p.w + v) + (v == 0 ? 1 : 0)) * rows_part(D, QT);
+        };
+        auto top_of = [&](int half, int v) {
+            const auto& p = x[half];
+            return p.whole ? a.kept_ml[half] + 2 * row : from(half, v) + p.rows * D + p.r;
+        };
+        auto out_of = [&](int half, int v) {
+            const auto& p = x[half];
+            return (p.whole ? a.kept[half] + row * D : from(half, v) + (size_t)p.r * D) + RW * lane;
+        };
+        const int lo = (int)((int64_t)n * part / PG), hi = (int)((int64_t)n * (part + 1) / PG), n0 = x[0].n;
+        join_parts<RW>(
+            hi - lo, lane, [&](int v) { return lo + v < n0 ? top_of(0, lo + v) : top_of(1, lo + v - n0); },
+            [&](int v) {
+                return lo + v < n0 ? top_of(0, lo + v) + (x[0].whole ? 1 : x[0].rows)
+                                   : top_of(1, lo + v - n0) + (x[1].whole ? 1 : x[1].rows);
+            },
+            [&](int v) { return lo + v < n0 ? out_of(0, lo + v) : out_of(1, lo + v - n0); }, acc, mx, ls);
         if constexpr (PG > 1) {
             __syncthreads();
 #pragma unroll
@@ -1241,7 +1264,7 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
 #pragma unroll
             for (int e = 0; e < RW; ++e) acc[e] = 0.0f;
             ls = 0.0f, mx = kNoMax;
-            join_parts<RW>(PG, lane, [&](int v) { return &sums[v][D]; }, 1, [&](int v) { return &sums[v][RW * lane]; }, acc, mx, ls);
+            join_parts<RW>(PG, lane, [&](int v) { return &sums[v][D]; }, [&](int v) { return &sums[v][D + 1]; }, [&](int v) { return &sums[v][RW * lane]; }, acc, mx, ls);
         }
         finish_row<D, false>(a, t, h, lane, acc, mx, ls, 0, true);
     }
@@ -2144,7 +2167,7 @@ __attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B
         const int64_t r = tiles ? g : rows;
         p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
         p.row_limit = tiles ? 16 * p.qt : INT64_MAX;
-        p.grid = device_cus() * rows_groups(D, e8);
+        p.grid = device_cus() * (rows_two(D, e8) ? 2 : 1);
         p.cuts_bytes = (uint64_t)p.grid * kTabInts * sizeof(int);
         p.rows_bytes = p.cuts_bytes + (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
     }
@@ -2186,7 +2209,7 @@ __attribute__((unused)) AttnPlan mix_plan(int heads, int kv_heads, int D, int B,
         const int64_t r = group_tiles ? rows : std::max(rows, group_rows);
         p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
         p.row_limit = group_tiles ? 16 * p.qt : INT64_MAX;
-        p.grid = device_cus() * rows_groups(D, e8);
+        p.grid = device_cus() * (rows_two(D, e8) ? 2 : 1);
         p.rows_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
     }
     p.part_bytes = p.rows_bytes;
@@ -2215,11 +2238,12 @@ __attribute__((unused)) int allow_lds(const void* k, int lds, std::atomic<uint64
 
 template <int D, int QT, bool E8, bool MIX>
 int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    constexpr int lds = rows_lds(D, QT, E8);
+    constexpr bool TWO = rows_two(D, E8);
+    constexpr int lds = rows_lds(D, QT, E8, TWO);
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, E8, MIX>), lds, done)) return rc;
-    hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MIX>), dim3(p.grid), dim3(64 * rows_waves(D, E8)), lds, s, a);
+    hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MIX>), dim3(p.grid), dim3(64 * rows_waves(D, TWO)), lds, s, a);
     if (int rc = hip_check(hipGetLastError(), "attn_paged_rows_kernel launch")) return rc;
     if (MIX) return ALV_OK;
     hipLaunchKernelGGL((attn_paged_rows_merge_kernel<D, QT>), dim3(p.grid - 1, 4 * QT), dim3(256), 0, s, a);
@@ -2269,7 +2293,7 @@ int launch_d(PagedAttnArgs a, const AttnPlan& p, hipStream_t s) {
         // Four waves to a row where rows are few (8 samples of one prompt, 32 rows: 11 us, 6).
         const int64_t rows = (int64_t)a.b.T * a.heads;
         constexpr int QT = decltype(qt)::value;
-        if (rows <= 8192)
+        if (rows <= 1024)
             hipLaunchKernelGGL((attn_paged_join_kernel<D, QT, 4>), dim3((uint32_t)rows), dim3(256), 0, s, a);
         else
             hipLaunchKernelGGL((attn_paged_join_kernel<D, QT, 1>), dim3((uint32_t)std::min((rows + 3) / 4, (int64_t)1 << 22)),

@@ -30,7 +30,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import ALV_ACT_GELU_TANH, ALV_ACT_SILU, check, lib
+from ._lib import ALV_ACT_GELU_TANH, ALV_ACT_SILU, call, check, lib
 
 _ACTS = {"gelu": ALV_ACT_GELU_TANH, "gelu_tanh": ALV_ACT_GELU_TANH, "silu": ALV_ACT_SILU}
 
@@ -465,7 +465,11 @@ def _per_row(v, name: str, B: int, dtype: torch.dtype, dev: torch.device):
 def _token_rows(t, name: str, dtype: torch.dtype, B: int, width: int, dev: torch.device):
     """(address, row stride, columns) of a (B, >= width) tensor or one row for all."""
     if t is None:
-        return None, 0, 0
+        return 0, 0, 0
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_contiguous() and t.get_device() == dev.index:
+        shape = t.shape  # (one test each for what most are)
+        if len(shape) == 2 and shape[0] == B and shape[1] >= width:
+            return t.data_ptr(), shape[1] if B > 1 else 0, shape[1]
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != dev or t.dim() not in (1, 2):
         raise TypeError(f"{name} must be a {str(dtype)[6:]} tensor of one or {B} rows on the logits' device")
     n, ld = t.shape[-1], 0 if t.dim() == 1 or t.shape[0] == 1 else t.stride(0)
@@ -506,7 +510,7 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, n
     if (bias is None) != (bias_tokens is None):
         raise ValueError("bias_tokens and bias come together")
     t, ldt, L = _token_rows(tokens, "tokens", torch.int32, B, 0, dev)
-    if tokens is not None and B > 1 and (tokens.dim() == 1 or tokens.shape[0] != B):
+    if B > 1 and ldt == 0 and tokens is not None and (tokens.dim() == 1 or tokens.shape[0] != B):
         raise ValueError(f"tokens must be {B} rows")
     bt, ldbt, M = _token_rows(bias_tokens, "bias_tokens", torch.int32, B, 0, dev)
     bv, ldb, _ = _token_rows(bias, "bias", torch.float32, B, M, dev)
@@ -515,9 +519,10 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, n
         if v is not None and (not isinstance(v, torch.Tensor) or v.dtype != torch.int32 or v.device != dev or
                               v.dim() != 1 or not v.is_contiguous() or v.numel() < B):
             raise TypeError(f"{name} must be a contiguous int32 tensor of {B} on the logits' device")
-    params = (*_per_row(repetition, "repetition", B, torch.float32, dev),
-              *_per_row(frequency, "frequency", B, torch.float32, dev),
-              *_per_row(presence, "presence", B, torch.float32, dev))
+    params = []
+    for v, name in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence")):
+        p, x = _per_row(v, name, B, torch.float32, dev)
+        params += p or 0, x
     if out is None:
         out, ldo = torch.empty(logits.shape, dtype=torch.float32, device=dev), V
     elif out.dtype != torch.float32 or out.device != dev or out.shape != logits.shape or V > 1 and out.stride(-1) != 1:
@@ -525,10 +530,9 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, n
     else:
         ldo = V if out.dim() == 1 or B <= 1 else out.stride(0)
     with _on(dev):
-        check(lib().alv_adjust_logits(logits.data_ptr(), ld, out.data_ptr(), ldo, B, V, t, ldt, L,
-                                      n_tokens.data_ptr() if n_tokens is not None else None,
-                                      n_prompt.data_ptr() if n_prompt is not None else None, *params, bt, ldbt, bv, ldb, M,
-                                      al, lda, _stream(logits)), "alv_adjust_logits")
+        call(lib(), "alv_adjust_logits", logits.data_ptr(), ld, out.data_ptr(), ldo, B, V, t, ldt, L,
+             n_tokens.data_ptr() if n_tokens is not None else 0, n_prompt.data_ptr() if n_prompt is not None else 0, *params,
+             bt, ldbt, bv, ldb, M, al, lda, _stream(logits))
     return out
 
 

@@ -29,12 +29,13 @@ of two for each slot's k and v; a value is code times power.
 from __future__ import annotations
 
 import array
+import functools
 import heapq
 
 import numpy as np
 import torch
 
-from ._lib import check, lib
+from ._lib import call, check, lib
 from .layer import _GEMMA_EPS, _f32, _ptr
 from .ops import _need_gpu, _on, _stream, _workspace
 
@@ -119,6 +120,9 @@ def _shape2(t: torch.Tensor, name: str, dev: torch.device):
 
 def _scales(scales: torch.Tensor, shape, dev: torch.device) -> int:
     """How many bytes the scales of two pages of an 8-bit pool of `shape` are apart."""
+    if (isinstance(scales, torch.Tensor) and scales.dtype is _E8M0 and scales.is_contiguous() and
+            scales.get_device() == dev.index and scales.shape == (*shape[:3], 2)):
+        return shape[1] * shape[2] * 2
     ss = _page_stride(scales, "scales", dev, _E8M0)
     if scales.shape != (*shape[:3], 2):
         raise ValueError(f"scales of pages {tuple(shape)} are {(*shape[:3], 2)}, got {tuple(scales.shape)}")
@@ -185,12 +189,18 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
             q_start.data_ptr(), kv_len.data_ptr(), B, T, pages, S, kpages.data_ptr(), vpages.data_ptr(), ks, vs)
     with _on(dev):
         if scales is None:
-            check(lib().alv_qkv_post_paged(*args, q_out.data_ptr(), ldq, _stream(qkv)), "alv_qkv_post_paged")
+            call(lib(), "alv_qkv_post_paged", *args, q_out.data_ptr(), ldq, _stream(qkv))
         else:
             ss = _scales(scales, shape, dev)
-            check(lib().alv_qkv_post_paged8(*args, scales.data_ptr(), ss, q_out.data_ptr(), ldq, _stream(qkv)),
-                  "alv_qkv_post_paged8")
+            call(lib(), "alv_qkv_post_paged8", *args, scales.data_ptr(), ss, q_out.data_ptr(), ldq, _stream(qkv))
     return q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _size(device: int, name: str, *numbers: int) -> int:
+    """Bytes of a call's workspace, a function of its numbers (asking the library is 1 us of a call). The device is
+    the current one."""
+    return getattr(lib(), name + "_workspace")(*numbers)
 
 
 def _attention(q, kpages, vpages, page_table, q_start, kv_len, heads, window, sinks, max_q, out, scales):
@@ -236,13 +246,10 @@ def attention_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     pages are 8-bit."""
     dev, pools, batch, shape, out, ldo = _attention(q, kpages, vpages, page_table, q_start, kv_len, heads, window, sinks,
                                                     max_q, out, scales)
-    L = lib()
-    run, size = ((L.alv_attention_paged, L.alv_attention_paged_workspace) if scales is None else
-                 (L.alv_attention_paged8, L.alv_attention_paged8_workspace))
+    name = "alv_attention_paged" if scales is None else "alv_attention_paged8"
     with _on(dev):
-        ws = _workspace(size(*shape[:3], *batch[-3:]), dev)
-        check(run(*pools, *batch, *shape, scale, out.data_ptr(), ldo, *ws[1:], _stream(q)),
-              "alv_attention_paged" if scales is None else "alv_attention_paged8")
+        _, ws, n = _workspace(_size(dev.index, name, *shape[:3], *batch[-3:]), dev)
+        call(lib(), name, *pools, *batch, *shape, scale, out.data_ptr(), ldo, ws or 0, n, _stream(q))
     return out
 
 
@@ -267,13 +274,12 @@ def attention_shared_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.
     G = shared_len.shape[0]
     if group_start.shape[0] != G + 1:
         raise ValueError(f"{G} shared lengths need group_start of {G + 1}, got {group_start.shape[0]}")
-    L = lib()
     if scales is None:
-        pools += None, 0
+        pools += 0, 0
     with _on(dev):
-        ws = _workspace(L.alv_attention_shared_workspace(*shape[:3], *batch[-3:], G), dev)
-        check(L.alv_attention_shared(*pools, *batch, group_start.data_ptr(), shared_len.data_ptr(), G, *shape, scale,
-                                     out.data_ptr(), ldo, *ws[1:], _stream(q)), "alv_attention_shared")
+        _, ws, n = _workspace(_size(dev.index, "alv_attention_shared", *shape[:3], *batch[-3:], G), dev)
+        call(lib(), "alv_attention_shared", *pools, *batch, group_start.data_ptr(), shared_len.data_ptr(), G, *shape, scale,
+             out.data_ptr(), ldo, ws or 0, n, _stream(q))
     return out
 
 

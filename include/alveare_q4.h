@@ -610,6 +610,21 @@ int alv_sample(const float* logits, int64_t ld, int B, int V, const float* u, co
                uint64_t workspace_bytes, void* stream);
 
 /*
+ * Some entry points (ALV_CALL_ and their name) called with their n arguments as 64-bit words, in order:
+ * pointers and integers as they are (an int within 32 bits, else ALV_ERR_RANGE),
+ * floats as doubles. For callers whose foreign calls pay for each argument (Python's
+ * ctypes: 5 us for the 29 of alv_attention_paged8, 1 us so). `words` is host memory,
+ * read before the call returns.
+ */
+#define ALV_CALL_QKV_POST_PAGED 0
+#define ALV_CALL_QKV_POST_PAGED8 1
+#define ALV_CALL_ATTENTION_PAGED 2
+#define ALV_CALL_ATTENTION_PAGED8 3
+#define ALV_CALL_ATTENTION_SHARED 4
+#define ALV_CALL_ADJUST_LOGITS 5
+int alv_call(int entry, const uint64_t* words, int n);
+
+/*
  * One op of a chain: a registered projection (y = W x) or a registered FFN
  * layer (y = ffn(x)); exactly one of `weight` and `ffn` is set. x and y are
  * device fp32 buffers of M rows (leading dimension K, resp. N or H). dep is

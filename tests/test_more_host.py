@@ -222,3 +222,40 @@ def test_reference_of_codes():
     assert M.decode(*M.encode(x))[0].tolist() == [448.0, 16.0, 20.0, -16.0, 0.0, 2.0 ** -8, 1.0]
     assert int(M.encode(torch.tensor([[449.0]]))[1]) == 128
     assert int(M.encode(torch.tensor([[2.0 ** -133]]))[1]) == 1
+
+
+def test_packed_calls(L):
+    """alv_call gives what the entry itself gives; what it cannot pass it refuses."""
+    from alveare_amd import _lib
+
+    assert set(_lib.PACKED) <= set(_lib.SIGNATURES)
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "alveare_q4.h")).read()
+    for name, (entry, n, words) in _lib.PACKED.items():
+        assert f"#define ALV_CALL_{name[4:].upper()} {entry}\n" in header
+        zeros = words.pack(*[0] * n)
+        assert len(zeros) == 8 * n
+        rc = L.alv_call(entry, zeros, n)
+        message = L.alv_last_error()
+        assert rc == getattr(L, name)(*[0] * n) and (rc == _lib.ALV_OK or message == L.alv_last_error())
+        assert L.alv_call(entry, zeros, n - 1) == _lib.ALV_ERR_ARG
+        types = _lib.SIGNATURES[name][1]
+        for i, t in enumerate(types):
+            if t is ctypes.c_int:
+                for far in (2 ** 31, -2 ** 31 - 1, 2 ** 40):
+                    assert L.alv_call(entry, words.pack(*[far if j == i else 0 for j in range(n)]), n) == _lib.ALV_ERR_RANGE
+    assert L.alv_call(99, b"", 0) == _lib.ALV_ERR_ARG
+    assert L.alv_call(-1, b"", 0) == _lib.ALV_ERR_ARG
+    assert L.alv_call(0, None, 0) == _lib.ALV_ERR_ARG
+    # every argument in its place: refused for the one that is wrong, whatever the others
+    good = dict(q=1 << 20, ld_q=256, k=1 << 20, v=1 << 20, ks=2048, vs=2048, sc=1 << 20, ss=64, pages=9, S=16, table=1 << 20,
+                ldt=4, W=4, qs=1 << 20, kl=1 << 20, B=2, T=0, mq=0, heads=4, kv=2, D=64, window=0, sinks=0, scale=1.0,
+                out=1 << 20, ldo=256, ws=0, wb=0, st=0)
+    entry, n, words = _lib.PACKED["alv_attention_paged8"]
+    run = lambda **ch: L.alv_call(entry, words.pack(*{**good, **ch}.values()), n)  # noqa: E731
+    assert run() == _lib.ALV_OK
+    for ch in (*BAD, dict(sc=None), dict(ss=63)):
+        if None not in ch.values() and "T" not in ch:
+            assert run(**ch) == attn8(L, T=0, **ch) == _lib.ALV_ERR_ARG, ch
+    assert run(scale=1e300) == _lib.ALV_ERR_ARG
+    with pytest.raises(_lib.Q4ValueError):
+        _lib.call(L, "alv_attention_paged8", *{**good, "D": 96}.values())
