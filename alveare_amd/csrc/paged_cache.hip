@@ -110,6 +110,7 @@ template <int D, bool WIDE, bool E8>
 __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post_paged_kernel(PostPagedArgs a) {
     using G = PostGeom<D>;
     __shared__ __align__(16) float rows[kPostMaxWaves][G::Heads * G::Row];
+    __shared__ __align__(16) uint16_t angles[WIDE ? kPostMaxWaves : 1][WIDE ? D : 8];  // a wave's cosines, its sines
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = blockDim.x >> 6;
@@ -157,11 +158,21 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
     const int page = ok ? page_of(a.b, sr.seq, pos) : -1;
     const int slot = pos & ((1 << a.b.shift) - 1);
     const uint16_t* rr = ok && a.rope ? a.rope + pos * a.rope_stride : nullptr;
+    // The row's angles, four of each per lane, on their way beside the page's number.
+    [[maybe_unused]] uint2 cosines{}, sines{};
+    if constexpr (WIDE)
+        if (rr && 4 * lane < a.half) {
+            cosines = *reinterpret_cast<const uint2*>(rr + a.cos_off + 4 * lane);
+            sines = *reinterpret_cast<const uint2*>(rr + a.sin_off + 4 * lane);
+        }
 
     for (int r0 = wave; r0 * G::Heads < total; r0 += nw) {
         if (r0 != wave) {
             d = head(r0);
             load_x(d, x);
+        } else if (WIDE && 4 * lane < a.half && rr) {
+            *reinterpret_cast<uint2*>(&angles[wave][4 * lane]) = cosines;
+            *reinterpret_cast<uint2*>(&angles[wave][D / 2 + 4 * lane]) = sines;
         }
         float f[G::Oct][8];
         const int norm = d.role == 0 ? a.norm_q : (d.role == 1 ? a.norm_k : a.norm_v);
@@ -207,8 +218,8 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
                     const float4 o0 = op[0], o1 = op[1];
                     const float o[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
                     float cr[8], sn[8];
-                    unpack8(*reinterpret_cast<const uint4*>(rr + a.cos_off + i0), cr);
-                    unpack8(*reinterpret_cast<const uint4*>(rr + a.sin_off + i0), sn);
+                    unpack8(*reinterpret_cast<const uint4*>(&angles[wave][i0]), cr);
+                    unpack8(*reinterpret_cast<const uint4*>(&angles[wave][D / 2 + i0]), sn);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float xc = mul_rn(f[e][i], cr[i]), os = mul_rn(o[i], sn[i]);
