@@ -611,15 +611,17 @@ __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int la
     sc.b0 = b0;
 }
 
-// The first step, and the work of the whole batch.
+// The first step (and `next`, the second: the first of sequences behind up to 64
+// groups), and the work of the whole batch.
 template <int ROWS, int UNIT, bool MIX>
-__device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, Scan& sc) {
+__device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, Scan& sc, Scan& next) {
     scan_step<ROWS, UNIT, MIX>(a, 0, lane, 0, sc);
     uint64_t total = sc.sum;
     uint32_t tiles = sc.s.nu ? min(sc.s.tiles, kPartsPerTile) : 0;
     for (int b0 = 64; b0 < seq_count<MIX>(a); b0 += 64) {
         Scan t;
-        scan_step<ROWS, UNIT, MIX>(a, b0, lane, 0, t);
+        scan_step<ROWS, UNIT, MIX>(a, b0, lane, total, t);
+        if (MIX && b0 == 64) next = t;
         total = min(total + t.sum, (uint64_t)1 << 62);  // (sequences that overlap: no wrap)
         tiles = min(tiles + (t.s.nu ? min(t.s.tiles, kPartsPerTile) : 0), 1u << 24);
     }
@@ -708,8 +710,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, G = lane >> 4;
-    Scan sc;
-    const uint64_t total = scan_all<ROWS, UNIT, MIX>(a, lane, sc);
+    Scan sc, next;
+    const uint64_t total = scan_all<ROWS, UNIT, MIX>(a, lane, sc, next);
     const Cut cut = make_cut(total, part_count(total, sc, gridDim.x));
     // The tile that begins in this part and ends in a later one, for the merge: the last
     // part it is in, first row of its sequence, tile, rows, kv head.
@@ -717,6 +719,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
     if (!MIX && threadIdx.x == 0) cut_tile[0] = 0;
     if (blockIdx.x >= cut.n) return;
     uint64_t x = cut.begin(blockIdx.x);
+    if (MIX && seq_count<MIX>(a) > 64 && x >= next.base) sc = next;  // (a step anew is 3 us)
     const uint64_t end = cut.begin(blockIdx.x + 1);
 
     unsigned char* ring = smem + wave * NS * STAGE;
@@ -1358,27 +1361,39 @@ __device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int
 // Items (tiles times kv heads, times their parts) and where each is found: heaviest
 // (last) tiles first, kv heads side by side, so that the workgroups an XCD gets
 // in turn share theirs where there are eight.
+// Step b0 / 64: the first two are read once for all that needs them (a step behind
+// groups is 3 us).
+struct TileSteps {
+    TileScan s0, s1;
+};
 template <int TR, bool MIX>
-__device__ __forceinline__ int tile_count(const PagedAttnArgs& a, const TileScan& sc0, int lane) {  // per kv head
+__device__ __forceinline__ TileScan tile_step(const PagedAttnArgs& a, const TileSteps& s, int b0, int lane) {
+    if (b0 == 0) return s.s0;
+    if (MIX && b0 == 64) return s.s1;
+    return tile_scan<TR, MIX>(a, b0, lane);
+}
+
+template <int TR, bool MIX>
+__device__ __forceinline__ int tile_count(const PagedAttnArgs& a, const TileSteps& steps, int lane) {  // per kv head
     // (no more than there can be: sequences that overlap must not carry the sum away)
-    int all = min(sc0.sum, a.max_tiles);
-    for (int b0 = 64; b0 < seq_count<MIX>(a); b0 += 64) all = min(all + tile_scan<TR, MIX>(a, b0, lane).sum, a.max_tiles);
+    int all = min(steps.s0.sum, a.max_tiles);
+    for (int b0 = 64; b0 < seq_count<MIX>(a); b0 += 64) all = min(all + tile_step<TR, MIX>(a, steps, b0, lane).sum, a.max_tiles);
     return all;
 }
 
-// Where tile gt is (sc0: the first 64 sequences, read once for all that needs them).
+// Where tile gt is.
 template <int TR, int BN, bool MIX>
 struct TileAt {
     int seq, rt, first, n, len, from;
     bool pre;
     TileSpan sp;
-    __device__ __forceinline__ TileAt(const PagedAttnArgs& a, const TileScan& sc0, int gt, int lane) {
+    __device__ __forceinline__ TileAt(const PagedAttnArgs& a, const TileSteps& steps, int gt, int lane) {
         int base = 0, b0 = 0;
-        TileScan sc = sc0;
+        TileScan sc = steps.s0;
         while (gt >= base + sc.sum) {
             base += sc.sum;
             b0 += 64;
-            sc = tile_scan<TR, MIX>(a, b0, lane);
+            sc = tile_step<TR, MIX>(a, steps, b0, lane);
         }
         const int l = __builtin_ctzll(__ballot(base + sc.incl > gt));
         seq = MIX ? __builtin_amdgcn_readlane(sc.s.seq, l) : b0 + l;
@@ -1416,10 +1431,10 @@ __device__ __forceinline__ int sum64(int v) {
 
 // Units of every tile, into LDS, by all waves.
 template <int TR, int BN, int NW, bool MIX>
-__device__ __forceinline__ void tile_units(const PagedAttnArgs& a, const TileScan& sc0, int tiles, int lane, int wave, int* nu) {
+__device__ __forceinline__ void tile_units(const PagedAttnArgs& a, const TileSteps& steps, int tiles, int lane, int wave, int* nu) {
     int base = 0, turn = 0;
     for (int b0 = 0; b0 < seq_count<MIX>(a) && base < tiles; b0 += 64) {
-        const TileScan sc = b0 ? tile_scan<TR, MIX>(a, b0, lane) : sc0;
+        const TileScan sc = tile_step<TR, MIX>(a, steps, b0, lane);
         for (int x0 = 0; x0 < sc.sum && base + x0 < tiles; x0 += 64, ++turn) {
             if (turn % NW != wave) continue;
             const int x = x0 + lane;
@@ -1472,7 +1487,7 @@ __device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, i
 }
 
 template <int D, bool E8, bool MIX>
-__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan& sc0, int gt, int kvh, int split, int nsplit, int entry, int* tab, unsigned char* smem) {
+__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileSteps& steps, int gt, int kvh, int split, int nsplit, int entry, int* tab, unsigned char* smem) {
     constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D);
     constexpr int DW = D / DS;            // this wave's columns of the output (and of its scores' products)
     constexpr int TB = tile_bytes(D), NC = D / 8, RPL = 512 / D;
@@ -1491,7 +1506,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileScan
     const int rg = wave / DS, dh = wave % DS;
     const int col = lane & 31, h = lane >> 5;
 
-    const TileAt<TR, BN, MIX> at_item(a, sc0, gt, lane);
+    const TileAt<TR, BN, MIX> at_item(a, steps, gt, lane);
     const int seq = at_item.seq, rt = at_item.rt;
     const int first = at_item.first, n = at_item.n, len = at_item.len, from = at_item.from;
     const bool pre = MIX && at_item.pre, suf = MIX && !at_item.pre, alone = suf && from == 0;
@@ -2018,15 +2033,17 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
     constexpr int TR = tile_rows(D), BN = tile_bn(D);
     static_assert(tile_lds(D, E8) >= 4 * kSplitTiles, "the tiles' units");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const TileScan sc0 = tile_scan<TR, MIX>(a, 0, lane);
-    const int tiles = tile_count<TR, MIX>(a, sc0, lane), items = tiles * a.kv_heads;
+    TileSteps steps;
+    steps.s0 = tile_scan<TR, MIX>(a, 0, lane);
+    if (MIX && seq_count<MIX>(a) > 64) steps.s1 = tile_scan<TR, MIX>(a, 64, lane);
+    const int tiles = tile_count<TR, MIX>(a, steps, lane), items = tiles * a.kv_heads;
     const bool split = items <= a.max_items;
     if (a.tab && blockIdx.x == 0 && tid == 0) a.tab[0] = split ? items : 0;
     if (items == 0) return;  // (the streaming kernel's all; there may be no slots to plan for)
     int gt, kvh, part = 0, parts = 1, entry = 0;
     if (split) {
         int* nu = reinterpret_cast<int*>(smem);
-        tile_units<TR, BN, tile_waves(D), MIX>(a, sc0, tiles, lane, wave, nu);
+        tile_units<TR, BN, tile_waves(D), MIX>(a, steps, tiles, lane, wave, nu);
         int all;
         const int cap = tile_cap(a, nu, tiles, lane, all);
         const int e = all * a.kv_heads - 1 - (int)blockIdx.x;
@@ -2060,7 +2077,7 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
         kvh = item - gt * a.kv_heads;
     }
     // (tiles of more rows than max_q told of may be more than tab has entries for: they are not split)
-    tile_item<D, E8, MIX>(a, sc0, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), split ? a.tab : nullptr, smem);
+    tile_item<D, E8, MIX>(a, steps, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), split ? a.tab : nullptr, smem);
 }
 
 // The parts of the tiles joined, `groups` workgroups to a tile, merge_rows(D) of
