@@ -44,7 +44,7 @@ struct PagedAttnArgs {
     int64_t k_stride, v_stride;
     const uint8_t* scales;
     int64_t s_stride;
-    int heads, kv_heads, g;
+    int heads, kv_heads, g, g_shift;  // g: q heads of a kv head; its logarithm, -1: not a power of two
     int window, sinks;
     float scale;
     uint16_t* out;
@@ -109,6 +109,10 @@ template <int N>
 __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+
+// A barrier for what is in LDS: the waves' stores to memory go on (__syncthreads waits for
+// them, 1 us and more at a tile's end).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // A buffer over [base, base + bytes), the same for the whole wave.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t wave_rsrc(const void* base, uint32_t bytes) {
@@ -569,6 +573,9 @@ struct Scan {
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// The token that row r (tokens times q heads of the group) belongs to: a division is 25
+// instructions, one after the other, several times a tile.
+__device__ __forceinline__ int per_head(const PagedAttnArgs& a, int r) { return a.g_shift >= 0 ? r >> a.g_shift : r / a.g; }
 __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, l);
     const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l);
@@ -665,7 +672,7 @@ __device__ __forceinline__ Found scan_find(const PagedAttnArgs& a, int lane, Sca
     const uint64_t tile = div32(in, (uint32_t)f.s.nu);
     f.u = uniform((int)(in - tile * f.s.nu));
     f.tile0 = start + tile * f.s.nu;
-    f.kvh = uniform((int)((uint32_t)tile / (uint32_t)f.s.tiles));
+    f.kvh = f.s.tiles == 1 ? uniform((int)tile) : uniform((int)((uint32_t)tile / (uint32_t)f.s.tiles));
     f.rt = uniform((int)((uint32_t)tile - (uint32_t)f.kvh * f.s.tiles));
     return f;
 }
@@ -832,7 +839,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const int r = min(16 * t + col, nrows - 1) + f.rt * ROWS;
-            const int tok = r / a.g, h = f.kvh * a.g + (r - tok * a.g);
+            const int tok = per_head(a, r), h = f.kvh * a.g + (r - tok * a.g);
             row_t[t] = f.s.first + tok;
             pos[t].pos = pos[t].cap = f.s.len - f.s.n + tok;
             pos[t].from = suf ? f.s.from : 0;
@@ -859,8 +866,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) asm volatile("" : "+v"(q[t][i]));
         }
-        int pos_lo = f.s.len - f.s.n + (f.rt * ROWS) / a.g;
-        int pos_hi = f.s.len - f.s.n + (f.rt * ROWS + nrows - 1) / a.g;
+        int pos_lo = f.s.len - f.s.n + per_head(a, f.rt * ROWS);
+        int pos_hi = f.s.len - f.s.n + per_head(a, f.rt * ROWS + nrows - 1);
         if (pre) {
             int p[QT];
             row_positions<QT>(a, f.seq, f.s.from, row_t, p);
@@ -1061,10 +1068,10 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
         for (int w = 0; w < NW; ++w) again |= odds[w] != 0;
         const bool whole = u0 == 0 && u1 == f.s.nu;
         if constexpr (MIX) {
+            const int places = whole ? 0 : (int)cut.part_of(f.tile0 + f.s.nu - 1) - (int)blockIdx.x + 1;
             for (int r = u0 == 0 ? tid : nrows; r < nrows; r += 64 * NW) {
-                const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
+                const int rr = r + f.rt * ROWS, tok = per_head(a, rr), h = f.kvh * a.g + (rr - tok * a.g);
                 const int64_t row = (int64_t)(f.s.first + tok) * a.heads + h;
-                const int places = (int)cut.part_of(f.tile0 + f.s.nu - 1) - (int)blockIdx.x + 1;
                 a.recs[(pre ? 0 : (int64_t)a.b.T * a.heads) + row] =
                     int4{(int)blockIdx.x, !whole ? places : (alone ? kDone : kWhole), r, f.s.from};
             }
@@ -1075,7 +1082,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
         float* part = a.part + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * rows_part(D, QT);
         if (again) {
             for (int r = wave; r < nrows; r += NW) {
-                const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
+                const int rr = r + f.rt * ROWS, tok = per_head(a, rr), h = f.kvh * a.g + (rr - tok * a.g);
                 float acc[D / 64], mr, lr;
                 Sight at{f.s.len - f.s.n + tok, f.s.len - f.s.n + tok, suf ? f.s.from : 0};
                 if (pre) {
@@ -1125,7 +1132,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
                 mx = mn;
             }
             if (whole) {
-                const int rr = r + f.rt * ROWS, tok = rr / a.g, h = f.kvh * a.g + (rr - tok * a.g);
+                const int rr = r + f.rt * ROWS, tok = per_head(a, rr), h = f.kvh * a.g + (rr - tok * a.g);
                 finish4<D, MIX>(a, f.s.first + tok, h, d, v, mx, ls, !pre, alone);
             } else {
                 *reinterpret_cast<f32x4*>(part + (size_t)r * D + d) = v;
@@ -1135,7 +1142,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
                 }
             }
         }
-        __syncthreads();  // the ring and mls are free again
+        lds_barrier();  // the ring and mls are free again
     }
 }
 
@@ -1193,7 +1200,7 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
     join_parts<RW>(
         last - w + 1, lane, [&](int v) { return place(v) + ROWS * D + r; }, [&](int v) { return place(v) + ROWS * (D + 1) + r; },
         [&](int v) { return place(v) + (size_t)r * D + RW * lane; }, acc, mx, ls);
-    const int rr = r + rt * ROWS, tok = rr / a.g, h = kvh * a.g + (rr - tok * a.g);
+    const int rr = r + rt * ROWS, tok = per_head(a, rr), h = kvh * a.g + (rr - tok * a.g);
     finish_row<D, false>(a, first + tok, h, lane, acc, mx, ls, 0, true);
 }
 
@@ -2137,7 +2144,7 @@ __global__ void __launch_bounds__((256 * PG)) attn_paged_tile_merge_kernel(Paged
             for (int k = 0; k < PG - 1; ++k) acc += sums[k][tid % 256];
         }
         if (r < rows && tid < 256) {
-            const int rr = rt * TR + r0 + r, tok = rr / a.g, head = kvh * a.g + rr % a.g;
+            const int rr = rt * TR + r0 + r, tok = per_head(a, rr), head = kvh * a.g + rr % a.g;
             store4(a.out + (int64_t)(first + tok) * a.ld_out + head * D + 4 * c, acc, inv[r]);
         }
         __syncthreads();
@@ -2360,6 +2367,7 @@ __attribute__((unused)) int attn_check(PagedAttnArgs* a, int D, const int32_t* p
         return fail(ALV_ERR_ALIGN, "q, kpages and vpages and their rows need 16-byte alignment, out and its rows 8-byte");
     if (T == 0) return ALV_OK;
     a->g = heads / kv_heads;
+    a->g_shift = a->g & (a->g - 1) ? -1 : __builtin_ctz((unsigned)a->g);
     a->window = a->window < a->b.max_pos ? a->window : 0;  // (all positions are within it)
     if ((int64_t)T * heads > (int64_t)1 << 30)  // (the largest launch: 2^32 threads)
         return fail(ALV_ERR_RANGE, "%d rows of %d heads in one call (at most 2^30 rows times heads)", T, heads);
