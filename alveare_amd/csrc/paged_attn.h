@@ -112,7 +112,11 @@ __device__ __forceinline__ void wait_vm() {
 
 // A barrier for what is in LDS: the waves' stores to memory go on (__syncthreads waits for
 // them, 1 us and more at a tile's end).
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 // A buffer over [base, base + bytes), the same for the whole wave.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t wave_rsrc(const void* base, uint32_t bytes) {
@@ -352,9 +356,10 @@ __device__ __forceinline__ SeqIn group_in(const PagedAttnArgs& a, int j0, int la
     return s;
 }
 
-// Sequence b0 + lane of the batch (b0 uniform), behind what it shares.
+// Sequence b0 + lane of the batch (b0 uniform), behind what it shares. groups: the first
+// 64 as group_in gave them, where the caller has them (two trips to memory less).
 template <bool MIX>
-__device__ __forceinline__ SeqIn batch_in(const PagedAttnArgs& a, int b0, int lane) {
+__device__ __forceinline__ SeqIn batch_in(const PagedAttnArgs& a, int b0, int lane, const SeqIn* groups = nullptr) {
     SeqIn s{};
     const int b = b0 + lane;
     if (b < a.b.B) {
@@ -370,7 +375,9 @@ __device__ __forceinline__ SeqIn batch_in(const PagedAttnArgs& a, int b0, int la
         for (int j0 = 0; j0 < a.gr.n; j0 += 64) {
             const int j = j0 + lane;
             int lo = INT_MAX, hi = 0, len = 0;
-            if (j < a.gr.n) {
+            if (j0 == 0 && groups) {
+                if (j < a.gr.n) lo = groups->seq, hi = groups->from, len = groups->len;  // (none shared: no end)
+            } else if (j < a.gr.n) {
                 lo = a.gr.start[j];
                 hi = a.gr.start[j + 1];
                 len = group_len(a.b, lo, hi, a.gr.len[j]);
@@ -388,10 +395,10 @@ __device__ __forceinline__ SeqIn batch_in(const PagedAttnArgs& a, int b0, int la
 }
 
 template <bool MIX>
-__device__ __forceinline__ SeqIn seq_in(const PagedAttnArgs& a, int b0, int lane) {
+__device__ __forceinline__ SeqIn seq_in(const PagedAttnArgs& a, int b0, int lane, const SeqIn* groups = nullptr) {
     if constexpr (MIX)
         if (b0 < group_steps<MIX>(a)) return group_in(a, b0, lane);
-    return batch_in<MIX>(a, b0 - group_steps<MIX>(a), lane);
+    return batch_in<MIX>(a, b0 - group_steps<MIX>(a), lane, groups);
 }
 
 // Of a group: the positions of NR packed rows (lane's own each) of the sequences seq ..
@@ -583,9 +590,10 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
 }
 
 template <int ROWS, int UNIT, bool MIX>
-__device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int lane, uint64_t base, Scan& sc) {
+__device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int lane, uint64_t base, Scan& sc,
+                                          const SeqIn* groups = nullptr) {
     const bool suf = MIX && b0 >= group_steps<MIX>(a);
-    const SeqIn in = seq_in<MIX>(a, b0, lane);
+    const SeqIn in = seq_in<MIX>(a, b0, lane, groups);
     RowsSeq s{};
     s.first = in.first, s.n = in.n, s.len = in.len, s.seq = in.seq, s.from = in.from;
     uint64_t w = 0;
@@ -627,7 +635,9 @@ __device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, S
     uint32_t tiles = sc.s.nu ? min(sc.s.tiles, kPartsPerTile) : 0;
     for (int b0 = 64; b0 < seq_count<MIX>(a); b0 += 64) {
         Scan t;
-        scan_step<ROWS, UNIT, MIX>(a, b0, lane, total, t);
+        SeqIn groups{};
+        groups.seq = sc.s.seq, groups.from = sc.s.from, groups.len = sc.s.len;
+        scan_step<ROWS, UNIT, MIX>(a, b0, lane, total, t, MIX ? &groups : nullptr);
         if (MIX && b0 == 64) next = t;
         total = min(total + t.sum, (uint64_t)1 << 62);  // (sequences that overlap: no wrap)
         tiles = min(tiles + (t.s.nu ? min(t.s.tiles, kPartsPerTile) : 0), 1u << 24);
@@ -675,6 +685,17 @@ __device__ __forceinline__ Found scan_find(const PagedAttnArgs& a, int lane, Sca
     f.kvh = f.s.tiles == 1 ? uniform((int)tile) : uniform((int)((uint32_t)tile / (uint32_t)f.s.tiles));
     f.rt = uniform((int)((uint32_t)tile - (uint32_t)f.kvh * f.s.tiles));
     return f;
+}
+
+// The tile behind f in the line, if it is the same sequence's.
+__device__ __forceinline__ bool scan_next(const PagedAttnArgs& a, Found& f) {
+    const bool last = f.rt + 1 == f.s.tiles;
+    if (last && f.kvh + 1 == a.kv_heads) return false;
+    f.kvh += last;
+    f.rt = last ? 0 : f.rt + 1;
+    f.u = 0;
+    f.tile0 += f.s.nu;
+    return true;
 }
 
 // The line of `total` units cut into n parts, the first r of them a unit longer.
@@ -746,8 +767,9 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
     const int vrow = E8 ? 4 * G + (col >> 1 & 3) + 16 * (col >> 3) : 4 * G + (col >> 2);
     const uint32_t rd_v = vrow * (16 * NC) + ((E8 ? 0 : (col >> 1) & 1) ^ vz(vrow)) * 16 + (col & 1) * 8;
 
-    while (x < end) {
-        const Found f = scan_find<ROWS, UNIT, MIX>(a, lane, sc, x);
+    Found f;
+    for (bool begun = false; x < end; begun = true) {
+        if (!begun || !scan_next(a, f)) f = scan_find<ROWS, UNIT, MIX>(a, lane, sc, x);
         const int u0 = f.u, u1 = uniform((int)min((uint64_t)f.s.nu, u0 + (end - x)));
         x += u1 - u0;
         const int nrows = min(ROWS, f.s.n * a.g - f.rt * ROWS);
@@ -1067,18 +1089,20 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
 #pragma unroll
         for (int w = 0; w < NW; ++w) again |= odds[w] != 0;
         const bool whole = u0 == 0 && u1 == f.s.nu;
-        if constexpr (MIX) {
-            const int places = whole ? 0 : (int)cut.part_of(f.tile0 + f.s.nu - 1) - (int)blockIdx.x + 1;
-            for (int r = u0 == 0 ? tid : nrows; r < nrows; r += 64 * NW) {
-                const int rr = r + f.rt * ROWS, tok = per_head(a, rr), h = f.kvh * a.g + (rr - tok * a.g);
-                const int64_t row = (int64_t)(f.s.first + tok) * a.heads + h;
-                a.recs[(pre ? 0 : (int64_t)a.b.T * a.heads) + row] =
-                    int4{(int)blockIdx.x, !whole ? places : (alone ? kDone : kWhole), r, f.s.from};
+        auto note = [&]() __attribute__((always_inline)) {  // where this tile's parts are
+            if constexpr (MIX) {
+                const int places = whole ? 0 : (int)cut.part_of(f.tile0 + f.s.nu - 1) - (int)blockIdx.x + 1;
+                for (int r = u0 == 0 ? tid : nrows; r < nrows; r += 64 * NW) {
+                    const int rr = r + f.rt * ROWS, tok = per_head(a, rr), h = f.kvh * a.g + (rr - tok * a.g);
+                    const int64_t row = (int64_t)(f.s.first + tok) * a.heads + h;
+                    a.recs[(pre ? 0 : (int64_t)a.b.T * a.heads) + row] =
+                        int4{(int)blockIdx.x, !whole ? places : (alone ? kDone : kWhole), r, f.s.from};
+                }
+            } else if (u0 == 0 && !whole && tid == 0) {
+                cut_tile[0] = (int)cut.part_of(f.tile0 + f.s.nu - 1);
+                cut_tile[1] = f.s.first, cut_tile[2] = f.rt, cut_tile[3] = nrows, cut_tile[4] = f.kvh;
             }
-        } else if (u0 == 0 && !whole && tid == 0) {
-            cut_tile[0] = (int)cut.part_of(f.tile0 + f.s.nu - 1);
-            cut_tile[1] = f.s.first, cut_tile[2] = f.rt, cut_tile[3] = nrows, cut_tile[4] = f.kvh;
-        }
+        };
         float* part = a.part + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * rows_part(D, QT);
         if (again) {
             for (int r = wave; r < nrows; r += NW) {
@@ -1104,6 +1128,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
                     part[ROWS * (D + 1) + r] = lr;
                 }
             }
+            note();
             __syncthreads();
             continue;
         }
@@ -1118,7 +1143,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(row + 16 * d) = o[t][d] * fac;
         }
-        __syncthreads();
+        lds_barrier();
         for (int e = tid; e < nrows * (D / 4); e += 64 * NW) {
             const int r = e / (D / 4), d = 4 * (e - r * (D / 4));
             f32x4 v = *reinterpret_cast<const f32x4*>(outs + (size_t)r * rows_out_ld(D) + d);
@@ -1142,6 +1167,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
                 }
             }
         }
+        note();
         lds_barrier();  // the ring and mls are free again
     }
 }
@@ -1327,9 +1353,9 @@ struct TileScan {
     int tiles, incl, sum;
 };
 template <int TR, bool MIX>
-__device__ __forceinline__ TileScan tile_scan(const PagedAttnArgs& a, int b0, int lane) {
+__device__ __forceinline__ TileScan tile_scan(const PagedAttnArgs& a, int b0, int lane, const SeqIn* groups = nullptr) {
     TileScan t{};
-    t.s = seq_in<MIX>(a, b0, lane);
+    t.s = seq_in<MIX>(a, b0, lane, groups);
     const int64_t rows = t.s.here ? (int64_t)t.s.n * a.g : 0;
     if (rows > a.row_limit) t.tiles = (int)((rows + TR - 1) / TR);
     int x = t.tiles;
@@ -1377,7 +1403,7 @@ template <int TR, bool MIX>
 __device__ __forceinline__ TileScan tile_step(const PagedAttnArgs& a, const TileSteps& s, int b0, int lane) {
     if (b0 == 0) return s.s0;
     if (MIX && b0 == 64) return s.s1;
-    return tile_scan<TR, MIX>(a, b0, lane);
+    return tile_scan<TR, MIX>(a, b0, lane, MIX ? &s.s0.s : nullptr);
 }
 
 template <int TR, bool MIX>
@@ -2042,7 +2068,7 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileSteps steps;
     steps.s0 = tile_scan<TR, MIX>(a, 0, lane);
-    if (MIX && seq_count<MIX>(a) > 64) steps.s1 = tile_scan<TR, MIX>(a, 64, lane);
+    if (MIX && seq_count<MIX>(a) > 64) steps.s1 = tile_scan<TR, MIX>(a, 64, lane, &steps.s0.s);
     const int tiles = tile_count<TR, MIX>(a, steps, lane), items = tiles * a.kv_heads;
     const bool split = items <= a.max_items;
     if (a.tab && blockIdx.x == 0 && tid == 0) a.tab[0] = split ? items : 0;
