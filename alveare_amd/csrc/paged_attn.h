@@ -537,6 +537,13 @@ __device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16
 // 512 on 1: 85 us); a large copy moves 4.9 on this card, reads alone more. One
 // sequence of 300 positions is two launches, 14 us with the host's part.
 
+// With groups or 8-bit pages a tile has kTileCost places in the line ahead of its units,
+// what its begin and end cost beside them: parts of many short tiles were the last to end
+// (64 sequences of 20 to 1500 own positions: 99 thousand cycles where the median took 66).
+// A part that ends among them leaves the tile to the next.
+constexpr int kTileCost = 3;
+constexpr int tile_cost(bool E8, bool MIX) { return E8 || MIX ? kTileCost : 0; }
+
 // A sequence's place in the line, per lane of the scan.
 struct RowsSeq {
     int first, n, len;
@@ -589,7 +596,7 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
     return ((uint64_t)hi << 32) | lo;
 }
 
-template <int ROWS, int UNIT, bool MIX>
+template <int ROWS, int UNIT, int COST, bool MIX>
 __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int lane, uint64_t base, Scan& sc,
                                           const SeqIn* groups = nullptr) {
     const bool suf = MIX && b0 >= group_steps<MIX>(a);
@@ -611,7 +618,7 @@ __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int la
             s.len = 0;  // malformed: one unit that sees nothing
             s.nu = 1;
         }
-        w = (uint64_t)s.tiles * a.kv_heads * s.nu;
+        w = (uint64_t)s.tiles * a.kv_heads * (COST + s.nu);
     }
     uint64_t x = w;
 #pragma unroll
@@ -628,16 +635,16 @@ __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int la
 
 // The first step (and `next`, the second: the first of sequences behind up to 64
 // groups), and the work of the whole batch.
-template <int ROWS, int UNIT, bool MIX>
+template <int ROWS, int UNIT, int COST, bool MIX>
 __device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, Scan& sc, Scan& next) {
-    scan_step<ROWS, UNIT, MIX>(a, 0, lane, 0, sc);
+    scan_step<ROWS, UNIT, COST, MIX>(a, 0, lane, 0, sc);
     uint64_t total = sc.sum;
     uint32_t tiles = sc.s.nu ? min(sc.s.tiles, kPartsPerTile) : 0;
     for (int b0 = 64; b0 < seq_count<MIX>(a); b0 += 64) {
         Scan t;
         SeqIn groups{};
         groups.seq = sc.s.seq, groups.from = sc.s.from, groups.len = sc.s.len;
-        scan_step<ROWS, UNIT, MIX>(a, b0, lane, total, t, MIX ? &groups : nullptr);
+        scan_step<ROWS, UNIT, COST, MIX>(a, b0, lane, total, t, MIX ? &groups : nullptr);
         if (MIX && b0 == 64) next = t;
         total = min(total + t.sum, (uint64_t)1 << 62);  // (sequences that overlap: no wrap)
         tiles = min(tiles + (t.s.nu ? min(t.s.tiles, kPartsPerTile) : 0), 1u << 24);
@@ -655,14 +662,14 @@ struct Found {
     RowsSeq s;
     int seq, kvh, rt;
     bool pre;         // of a group, over what it shares
-    int u;            // unit in the tile
+    int at;           // place in the tile: COST, then its units
     uint64_t tile0;   // the tile's place in the line
 };
 
 // The tile and unit at place x of the line (x < total; calls with x rising).
-template <int ROWS, int UNIT, bool MIX>
+template <int ROWS, int UNIT, int COST, bool MIX>
 __device__ __forceinline__ Found scan_find(const PagedAttnArgs& a, int lane, Scan& sc, uint64_t x) {
-    while (x >= sc.base + sc.sum) scan_step<ROWS, UNIT, MIX>(a, sc.b0 + 64, lane, sc.base + sc.sum, sc);
+    while (x >= sc.base + sc.sum) scan_step<ROWS, UNIT, COST, MIX>(a, sc.b0 + 64, lane, sc.base + sc.sum, sc);
     const uint64_t m = __ballot(sc.base + sc.incl > x);
     const int l = __builtin_ctzll(m);
     Found f;
@@ -676,25 +683,27 @@ __device__ __forceinline__ Found scan_find(const PagedAttnArgs& a, int lane, Sca
     f.s.us = __builtin_amdgcn_readlane(sc.s.us, l);
     f.s.ulo = __builtin_amdgcn_readlane(sc.s.ulo, l);
     f.s.nu = __builtin_amdgcn_readlane(sc.s.nu, l);
-    const uint64_t seq_work = (uint64_t)f.s.tiles * a.kv_heads * f.s.nu;
+    const uint32_t places = COST + f.s.nu;
+    const uint64_t seq_work = (uint64_t)f.s.tiles * a.kv_heads * places;
     const uint64_t start = sc.base + lane_u64(sc.incl, l) - seq_work;
     const uint64_t in = x - start;
-    const uint64_t tile = div32(in, (uint32_t)f.s.nu);
-    f.u = uniform((int)(in - tile * f.s.nu));
-    f.tile0 = start + tile * f.s.nu;
+    const uint64_t tile = div32(in, places);
+    f.at = uniform((int)(in - tile * places));
+    f.tile0 = start + tile * places;
     f.kvh = f.s.tiles == 1 ? uniform((int)tile) : uniform((int)((uint32_t)tile / (uint32_t)f.s.tiles));
     f.rt = uniform((int)((uint32_t)tile - (uint32_t)f.kvh * f.s.tiles));
     return f;
 }
 
 // The tile behind f in the line, if it is the same sequence's.
+template <int COST>
 __device__ __forceinline__ bool scan_next(const PagedAttnArgs& a, Found& f) {
     const bool last = f.rt + 1 == f.s.tiles;
     if (last && f.kvh + 1 == a.kv_heads) return false;
     f.kvh += last;
     f.rt = last ? 0 : f.rt + 1;
-    f.u = 0;
-    f.tile0 += f.s.nu;
+    f.at = 0;
+    f.tile0 += COST + f.s.nu;
     return true;
 }
 
@@ -733,13 +742,14 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
     constexpr int HALF = 32 * D;          // bytes of a block's K
     constexpr int RPL = 64 / NC;          // rows of one load
     constexpr int LOADS = NH * 2 * NI + E8;   // of a block, at least
+    constexpr int COST = tile_cost(E8, MIX);
     using T = PageValue<E8>;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, G = lane >> 4;
     Scan sc, next;
-    const uint64_t total = scan_all<ROWS, UNIT, MIX>(a, lane, sc, next);
+    const uint64_t total = scan_all<ROWS, UNIT, COST, MIX>(a, lane, sc, next);
     const Cut cut = make_cut(total, part_count(total, sc, gridDim.x));
     // The tile that begins in this part and ends in a later one, for the merge: the last
     // part it is in, first row of its sequence, tile, rows, kv head.
@@ -769,9 +779,10 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
 
     Found f;
     for (bool begun = false; x < end; begun = true) {
-        if (!begun || !scan_next(a, f)) f = scan_find<ROWS, UNIT, MIX>(a, lane, sc, x);
-        const int u0 = f.u, u1 = uniform((int)min((uint64_t)f.s.nu, u0 + (end - x)));
-        x += u1 - u0;
+        if (!begun || !scan_next<COST>(a, f)) f = scan_find<ROWS, UNIT, COST, MIX>(a, lane, sc, x);
+        const int u0 = max(0, f.at - COST), u1 = uniform((int)min((int64_t)f.s.nu, (int64_t)(end - f.tile0) - COST));
+        if (COST > 0 && u1 <= 0) break;
+        x = f.tile0 + COST + u1;
         const int nrows = min(ROWS, f.s.n * a.g - f.rt * ROWS);
         const int nblk = f.s.len > 0 ? u1 - u0 : 0;  // this wave's blocks
         const bool pre = MIX && f.pre, suf = MIX && !f.pre, alone = suf && f.s.from == 0;
@@ -1091,7 +1102,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
         const bool whole = u0 == 0 && u1 == f.s.nu;
         auto note = [&]() __attribute__((always_inline)) {  // where this tile's parts are
             if constexpr (MIX) {
-                const int places = whole ? 0 : (int)cut.part_of(f.tile0 + f.s.nu - 1) - (int)blockIdx.x + 1;
+                const int places = whole ? 0 : (int)cut.part_of(f.tile0 + COST + f.s.nu - 1) - (int)blockIdx.x + 1;
                 for (int r = u0 == 0 ? tid : nrows; r < nrows; r += 64 * NW) {
                     const int rr = r + f.rt * ROWS, tok = per_head(a, rr), h = f.kvh * a.g + (rr - tok * a.g);
                     const int64_t row = (int64_t)(f.s.first + tok) * a.heads + h;
@@ -1099,7 +1110,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
                         int4{(int)blockIdx.x, !whole ? places : (alone ? kDone : kWhole), r, f.s.from};
                 }
             } else if (u0 == 0 && !whole && tid == 0) {
-                cut_tile[0] = (int)cut.part_of(f.tile0 + f.s.nu - 1);
+                cut_tile[0] = (int)cut.part_of(f.tile0 + COST + f.s.nu - 1);
                 cut_tile[1] = f.s.first, cut_tile[2] = f.rt, cut_tile[3] = nrows, cut_tile[4] = f.kvh;
             }
         };
