@@ -53,9 +53,11 @@ struct PostPagedArgs {
 // a rotated pair's other half.
 //
 // What bounds it: one token, three dependent trips to memory (the sequence, its
-// page and RoPE row, the stores), 5 us; many, the bytes. 16 + 2 x 8 heads of 256,
-// 4939 tokens: 48 us, 3.4 TB/s (a wave per head and two-byte accesses: 101 us);
-// 42 where the same rows come again and are partly in the last cache.
+// page and RoPE row, the stores), 5 us; many, those trips again, six waves per SIMD
+// at a time (more would spill), and the arithmetic between them, by numpy's order and
+// two roundings some 25 instructions a value. 16 + 2 x 8 heads of 256, 4939 tokens: 44 us,
+// 3.7 TB/s, into bf16 pages and 42 into 8-bit ones (rounding and coding value by value 48
+// and 49; a wave per head and two-byte accesses: 101).
 constexpr int kPostMaxWaves = 8;
 constexpr int kLeafPad = 8;  // floats: leaves then start eight banks apart
 
@@ -79,29 +81,59 @@ struct PostGeom {
 // Codes are rounded to nearest even, half a step, 2^-4 relative; what is not
 // finite becomes NaN.
 
-// The biased exponent, 1 .. 254, from the largest finite magnitude's bf16 bits.
+// The biased exponent, 1 .. 247, from the largest finite magnitude's bf16 bits.
 __device__ __forceinline__ int power_of(int bits) {
     return max(1, (bits >> 7) - 8 + ((bits & 0x7F) > 0x60 ? 1 : 0));
 }
 
-__device__ __forceinline__ int finite_magnitude(uint16_t bits) {
-    const int m = bits & 0x7FFF;
-    return m < 0x7F80 ? m : 0;
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+constexpr int kInfBits = 0x7F80;
+
+// The larger of `top` and the octet's magnitudes by their bits; those of what is not
+// finite, from kInfBits on, left out if FINITE.
+template <bool FINITE>
+__device__ __forceinline__ u16x2 larger_magnitude(u16x2 top, const uint32_t (&w)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        u16x2 m = __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu);
+        if constexpr (FINITE) m = u16x2{m.x < kInfBits ? m.x : (uint16_t)0, m.y < kInfBits ? m.y : (uint16_t)0};
+        top = __builtin_elementwise_max(top, m);
+    }
+    return top;
 }
 
-// Eight bf16 values as codes. (v_cvt_pk_fp8_f32: to nearest even; infinities, like NaN, give NaN.)
-__device__ __forceinline__ uint2 encode8(const uint16_t (&v)[8], int power) {
-    const float up = __builtin_bit_cast(float, (uint32_t)(254 - power) << 23);  // 2^(127 - power)
-    uint32_t w[2];
+// Eight bf16 values as codes. (v_cvt_scalef32_pk_fp8_bf16 divides by the power and rounds to
+// nearest even; infinities, like NaN, give NaN. Against v_cvt_pk_fp8_f32 of each product: the
+// same codes for every bf16 value and power, a third of the instructions.)
+__device__ __forceinline__ uint2 encode8(const uint32_t (&w)[4], int power) {
+    const float scale = __builtin_bit_cast(float, (uint32_t)power << 23);
+    uint32_t c[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = bf16_bits_to_f32(v[4 * i + e]) * up;
-        const int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-        w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], c, true);
+        s16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(s16x2{}, __builtin_bit_cast(bf16x2, w[2 * i]), scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, w[2 * i + 1]), scale, true);
+        c[i] = __builtin_bit_cast(uint32_t, r);
     }
-    return uint2{w[0], w[1]};
+    return uint2{c[0], c[1]};
+}
+
+// ---- both kinds ------------------------------------------------------------------------
+
+// bf16_rne_bits of eight values, in pairs; NaN, which the conversion passes on, is looked
+// for once in all eight.
+__device__ __forceinline__ void round8(const float (&f)[8], uint32_t (&w)[4]) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{f[2 * i], f[2 * i + 1]}), bf16x2));
+        nan |= __builtin_isunordered(f[2 * i], f[2 * i + 1]);
+    }
+    if (nan)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = bf16_rne_bits(f[2 * i]) | ((uint32_t)bf16_rne_bits(f[2 * i + 1]) << 16);
 }
 
 // WIDE: every row 16-byte aligned (8-bit pages: 8), a rotated half whole octets.
@@ -193,13 +225,13 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
         for (int e = 0; e < G::Oct; ++e) {
             const int c0 = 8 * (hl + G::Lanes * e);
             if (norm) {
-                float w[8];
-                load_w8(d.w, c0 / 8, w);
+                float w[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};  // (a product with 1 is its value)
+                if (d.w) load_w8(d.w, c0 / 8, w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = mul_rn(f[e][i], inv);
-                    f[e][i] = bf16r(d.w ? mul_rn(v, w[i]) : v);
-                }
+                for (int i = 0; i < 8; ++i) w[i] = mul_rn(mul_rn(f[e][i], inv), w[i]);
+                uint32_t r[4];
+                round8(w, r);
+                unpack8(uint4{r[0], r[1], r[2], r[3]}, f[e]);
             }
             if (rr) {  // the whole wave: a head's rows hold what its pairs read
                 float4* p = reinterpret_cast<float4*>(row + G::at(c0));
@@ -207,66 +239,77 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
                 p[1] = float4{f[e][4], f[e][5], f[e][6], f[e][7]};
             }
         }
-        auto rotated = [&](int e, uint16_t (&out)[8]) __attribute__((always_inline)) {
+        auto rotated = [&](int e, uint32_t (&out)[4]) __attribute__((always_inline)) {
             const int c0 = 8 * (hl + G::Lanes * e);
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = f[e][i];
             if (rot && c0 < 2 * a.half) {
                 // run_rope_cpu_gemma (model.py:549-575): y1 = x1 c - x2 s, y2 = x2 c + x1 s.
                 if constexpr (WIDE) {
                     const bool low = c0 < a.half;
                     const int i0 = low ? c0 : c0 - a.half;
+                    const uint32_t sign = low ? 0x80008000u : 0u;  // (x1 c - x2 s = x1 c + x2 (-s), bit for bit)
                     const float4* op = reinterpret_cast<const float4*>(row + G::at(low ? c0 + a.half : i0));
                     const float4 o0 = op[0], o1 = op[1];
                     const float o[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
                     float cr[8], sn[8];
                     unpack8(*reinterpret_cast<const uint4*>(&angles[wave][i0]), cr);
-                    unpack8(*reinterpret_cast<const uint4*>(&angles[wave][D / 2 + i0]), sn);
+                    const uint4 s8 = *reinterpret_cast<const uint4*>(&angles[wave][D / 2 + i0]);
+                    unpack8(uint4{s8.x ^ sign, s8.y ^ sign, s8.z ^ sign, s8.w ^ sign}, sn);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float xc = mul_rn(f[e][i], cr[i]), os = mul_rn(o[i], sn[i]);
-                        out[i] = bf16_rne_bits(low ? sub_rn(xc, os) : add_rn(xc, os));
-                    }
+                    for (int i = 0; i < 8; ++i) y[i] = add_rn(mul_rn(y[i], cr[i]), mul_rn(o[i], sn[i]));
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int c = c0 + i, k = c < a.half ? c : c - a.half;
-                        float y = f[e][i];
                         if (c < 2 * a.half) {
-                            const float xc = mul_rn(y, bf16_bits_to_f32(rr[a.cos_off + k]));
+                            const float xc = mul_rn(y[i], bf16_bits_to_f32(rr[a.cos_off + k]));
                             const float os = mul_rn(row[G::at(c < a.half ? c + a.half : k)], bf16_bits_to_f32(rr[a.sin_off + k]));
-                            y = c < a.half ? sub_rn(xc, os) : add_rn(xc, os);
+                            y[i] = c < a.half ? sub_rn(xc, os) : add_rn(xc, os);
                         }
-                        out[i] = bf16_rne_bits(y);
                     }
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) out[i] = bf16_rne_bits(f[e][i]);
             }
+            round8(y, out);
             if (!ok)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) out[i] = 0;
+                for (int i = 0; i < 4; ++i) out[i] = 0;
         };
         const bool put = d.in && (d.role == 0 || page >= 0);
         const int64_t at = (((int64_t)d.h << a.b.shift) + slot) * D;  // in its page
         if constexpr (E8) {
-            uint16_t out[G::Oct][8];
-            int top = 0;
+            uint32_t out[G::Oct][4];
+            u16x2 top2{};
 #pragma unroll
             for (int e = 0; e < G::Oct; ++e) {
                 rotated(e, out[e]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = max(top, finite_magnitude(out[e][i]));
+                top2 = larger_magnitude<false>(top2, out[e]);
             }
+            auto over_head = [&](u16x2 m) __attribute__((always_inline)) {
+                int top = max(m.x, m.y);
 #pragma unroll
-            for (int k = 1; k < G::Lanes; k <<= 1) top = max(top, __shfl_xor(top, k));
+                for (int k = 1; k < G::Lanes; k <<= 1) top = max(top, __shfl_xor(top, k));
+                return top;
+            };
+            int top = over_head(top2);
+            if (__any(top >= kInfBits)) {  // (of any head of the wave: its lanes stay together)
+                top2 = u16x2{};
+#pragma unroll
+                for (int e = 0; e < G::Oct; ++e) top2 = larger_magnitude<true>(top2, out[e]);
+                top = over_head(top2);
+            }
             if (!put) continue;
             const int power = power_of(top);
 #pragma unroll
             for (int e = 0; e < G::Oct; ++e) {
                 const int c0 = 8 * (hl + G::Lanes * e);
                 if (d.role == 0) {
-                    const uint4 o8 = pack8(out[e]);
-                    __builtin_memcpy(a.q_out + (int64_t)t * a.ld_q + d.h * D + c0, &o8, sizeof(o8));
+                    uint16_t* dst = a.q_out + (int64_t)t * a.ld_q + d.h * D + c0;
+                    if constexpr (WIDE)
+                        *reinterpret_cast<uint4*>(dst) = uint4{out[e][0], out[e][1], out[e][2], out[e][3]};
+                    else
+                        __builtin_memcpy(dst, out[e], sizeof(out[e]));
                 } else {
                     uint8_t* dst = d.role == 1 ? static_cast<uint8_t*>(a.kpages) + page * a.k_stride
                                                : static_cast<uint8_t*>(a.vpages) + page * a.v_stride;
@@ -285,15 +328,14 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
                                                             : static_cast<uint16_t*>(a.vpages) + max(page, 0) * a.v_stride);
 #pragma unroll
             for (int e = 0; e < G::Oct; ++e) {
-                uint16_t out[8];
+                uint32_t out[4];
                 rotated(e, out);
                 if (!put) continue;
-                const uint4 o8 = pack8(out);
                 const int c0 = 8 * (hl + G::Lanes * e);
                 if constexpr (WIDE)
-                    *reinterpret_cast<uint4*>(dst + c0) = o8;
+                    *reinterpret_cast<uint4*>(dst + c0) = uint4{out[0], out[1], out[2], out[3]};
                 else
-                    __builtin_memcpy(dst + c0, &o8, sizeof(o8));
+                    __builtin_memcpy(dst + c0, out, sizeof(out));
             }
         }
     }
