@@ -1504,6 +1504,7 @@ __device__ __forceinline__ int tile_parts_sum(const int* nu, int tiles, int lane
     for (int t = lane; t < tiles; t += 64) c += tile_parts(nu[t], cap);
     return sum64(c);
 }
+template <bool MIX>
 __device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, int tiles, int lane, int& parts) {
     int total = 0, most = 0;
     for (int t = lane; t < tiles; t += 64) {
@@ -1519,7 +1520,25 @@ __device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, i
     if ((int64_t)total * 5 <= (int64_t)most * tiles * 3) {  // uneven: the light ones fill in behind the heavy
         const int cap = max(least, (int)((int64_t)total * 3 / (4 * slots)) + 5);
         parts = tile_parts_sum(nu, tiles, lane, cap);
-        if (parts <= 2 * slots) return cap;
+        if (parts <= (MIX ? slots : 2 * slots)) return cap;
+        // A group's tile's parts are as long as can be: no second turn, but the smallest cap of
+        // 64, a lane each, whose parts all run at once (drafts of 16 sequences over 20032 shared
+        // positions and up to 3000 of their own, heads of 512: 150 -> 105 us; this search for
+        // every call costs 64 tokens over 4 prompts of 4000 3 us of 60).
+        if constexpr (MIX) {
+            const int lo = max(least, (total + slots - 1) / slots), mine = lo + lane * (1 + lo / 48);
+            const float inv = 1.0f / (float)mine;
+            int n = 0;
+#pragma unroll 4
+            for (int t = 0; t < tiles; ++t)  // (one off at millions of units only)
+                n += (int)(((float)max(1, nu[t]) + (float)mine - 0.5f) * inv);
+            const uint64_t fit = __ballot(n <= slots);
+            if (fit) {
+                const int best = __builtin_amdgcn_readlane(mine, __builtin_ctzll(fit));
+                parts = tile_parts_sum(nu, tiles, lane, best);
+                if (parts <= slots) return best;
+            }
+        }
     }
     int cap = max(least, (total + slots - tiles / 2 - 1) / max(1, slots - tiles / 2));
     for (int turn = 0; turn < 2; ++turn, cap += cap / 2) {
@@ -2089,9 +2108,10 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
         int* nu = reinterpret_cast<int*>(smem);
         tile_units<TR, BN, tile_waves(D), MIX>(a, steps, tiles, lane, wave, nu);
         int all;
-        const int cap = tile_cap(a, nu, tiles, lane, all);
-        const int e = all * a.kv_heads - 1 - (int)blockIdx.x;
-        if (e < 0) return;
+        const int cap = tile_cap<MIX>(a, nu, tiles, lane, all);
+        // (MIX: groups' parts before sequences'; else a prompt's last tiles before its first)
+        const int e = MIX ? (int)blockIdx.x : all * a.kv_heads - 1 - (int)blockIdx.x;
+        if (e < 0 || e >= all * a.kv_heads) return;
         int base = 0, t0 = 0, p, incl;
         while (true) {
             p = t0 + lane < tiles ? tile_parts(nu[t0 + lane], cap) : 0;
