@@ -131,6 +131,46 @@ def test_shared_what_is_masked_reaches_no_row(dev, D, bits, n):
     assert ((got - want).abs() <= tol)[~poisoned].all()
 
 
+@pytest.mark.parametrize("heads,kv_heads,D,B", [(8, 8, 64, 5), (32, 8, 64, 7), (16, 2, 64, 7), (32, 8, 64, 40), (6, 2, 128, 30),
+                                                (16, 8, 256, 30), (16, 1, 512, 6), (2, 2, 512, 12), (2, 2, 512, 40)])
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("window,sinks", [(5, 0), (60, 3), (150, 70)])
+def test_shared_window_decode(dev, heads, kv_heads, D, B, bits, window, sinks):
+    """One token each, few rows of a group and many: all of them streamed, groups in tiles beside streamed
+    sequences, and all in tiles."""
+    own = [1 + (i * 29) % 67 for i in range(B)]
+    b = batch([1] * B, own, [(B - 2, 176), (1, 64)], kv_heads=kv_heads, D=D, page=16, dev=dev, bits=bits, extra_rows=1)
+    check(b, heads, dev, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1200, 9)])
+def test_shared_one_long_tile_beside_short_ones(dev, window, sinks):
+    """A group's long tile and sequences' shorter ones in as many parts as run at once."""
+    b = batch([17] * 5, [900 + 77 * i for i in range(5)], [(5, 8192)], kv_heads=32, D=64, page=128, dev=dev, bits=16)
+    check(b, 32, dev, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("D", [64, 256, 512])
+@pytest.mark.parametrize("n", [1, 9])
+def test_shared_same_bits_and_apart(dev, D, n):
+    """The same bits from call to call; the same answer in groups of one, in none and by attention that shares nothing."""
+    from alveare_amd import attention_paged, attention_shared_paged
+
+    b = batch([n] * 4, [n + 700, n + 3, n + 64, n], [(4, 512)], kv_heads=2, D=D, page=64, dev=dev)
+    q = rows(b.T, 8 * D, dev)
+    kw = dict(heads=8, scale=0.1, max_q=n, scales=b.scales)
+    a = [attention_shared_paged(q, *b.args(), *b.groups(), **kw) for _ in range(3)]
+    assert torch.equal(a[0], a[1]) and torch.equal(a[0], a[2])
+    for s in range(1, 4):
+        b.table[s, :8] = b.table[0, :8]
+    want, tol = M.attention(q, b, 8, 0, 0, 0.1)
+    i32 = dict(dtype=torch.int32, device=dev)
+    for got in (a[0], attention_paged(q, *b.args(), **kw),
+                attention_shared_paged(q, *b.args(), torch.arange(5, **i32), torch.full((4,), 512, **i32), **kw),
+                attention_shared_paged(q, *b.args(), torch.zeros(1, **i32), torch.zeros(0, **i32), **kw)):
+        assert ((got.double().cpu().view_as(want) - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 def test_shared_missing_pages(dev, bits):
     """Shared pages that are gone are gone for all; a row with none left gets zeros."""
