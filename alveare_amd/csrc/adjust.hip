@@ -249,8 +249,12 @@ extern "C" int alv_adjust_logits(const float* logits, int64_t ld, float* out, in
     if (B < 0 || V < 1 || L < 0 || M < 0) return fail(ALV_ERR_ARG, "bad shape B=%d V=%d L=%d M=%d", B, V, L, M);
     if (B > 0 && (!logits || !out || (L > 0 && !tokens) || (M > 0 && (!bias_tokens || !bias))))
         return fail(ALV_ERR_ARG, "null pointer");
-    if (B > 65535 || V > 1 << 24 || L > 1 << 30 || (int64_t)B * V > (int64_t)1 << 35)
-        return fail(ALV_ERR_RANGE, "%d rows of %d logits, %d tokens each (at most 65535, 2^24, 2^30; 2^35 logits)", B, V, L);
+    // (a list entry that is there again looks through the list: 2^16 of them take a wave 0.1 s at most)
+    if (B > 65535 || V > 1 << 24 || L > 1 << 30 || M > 1 << 16 || (int64_t)B * V > (int64_t)1 << 35)
+        return fail(ALV_ERR_RANGE, "%d rows of %d logits, %d tokens and %d biases each (at most 65535, 2^24, 2^30, 2^16; 2^35 logits)",
+                    B, V, L, M);
+    if (B > 1 && std::max(ld, ld_out) > (int64_t)1 << 40)
+        return fail(ALV_ERR_RANGE, "rows %lld and %lld apart (at most 2^40)", (long long)ld, (long long)ld_out);
     if (!repetition_dev && !(repetition > 0.0f)) return fail(ALV_ERR_ARG, "repetition %g: above 0", (double)repetition);
     if (B > 1 && (ld < V || ld_out < V || ld_tokens < 0 || ld_bias_tokens < 0 || ld_bias < 0 || ld_allowed < 0))
         return fail(ALV_ERR_ARG, "rows of %d logits, %lld and %lld apart", V, (long long)ld, (long long)ld_out);
@@ -258,10 +262,10 @@ extern "C" int alv_adjust_logits(const float* logits, int64_t ld, float* out, in
     // Rows that are elsewhere: none of one's within another's (both may be columns of one array).
     if (B > 0 && out != logits) {
         const int64_t in0 = (int64_t)reinterpret_cast<uintptr_t>(logits), out0 = (int64_t)reinterpret_cast<uintptr_t>(out);
-        const int64_t in1 = in0 + 4 * ((B - 1) * ld + V), out1 = out0 + 4 * ((B - 1) * ld_out + V);
+        const int64_t in1 = in0 + 4 * ((B > 1 ? (B - 1) * ld : 0) + V), out1 = out0 + 4 * ((B > 1 ? (B - 1) * ld_out : 0) + V);
         if (in0 < out1 && out0 < in1) {
-            const int64_t d = ((out0 - in0) / 4 % ld + ld) % ld;
-            if (B == 1 || ld != ld_out || d < V || d + V > ld) return fail(ALV_ERR_ARG, "out overlaps logits");
+            const int64_t d = B == 1 ? 0 : ((out0 - in0) / 4 % ld + ld) % ld;
+            if (ld != ld_out || d < V || d + V > ld) return fail(ALV_ERR_ARG, "out overlaps logits");
         }
     }
     for (const void* p : {(const void*)logits, (const void*)out, (const void*)tokens, (const void*)n_tokens, (const void*)n_prompt,

@@ -575,7 +575,8 @@ int alv_copy_pages(void* const* caches, int ncaches, int64_t page_bytes, int64_t
  * allowed: (V + 31) / 32 words a row, NULL: all are allowed. Rows of the last four
  * may be 0 apart: the same for all. Tokens outside [0, V) count for nothing.
  * repetition (above 0), frequency and presence come as device arrays of B values,
- * or (NULL) as one number. B <= 65535, V <= 2^24, L <= 2^30, B * V <= 2^35.
+ * or (NULL) as one number. B <= 65535, V <= 2^24, L <= 2^30, M <= 2^16,
+ * B * V <= 2^35.
  */
 int alv_adjust_logits(const float* logits, int64_t ld, float* out, int64_t ld_out, int B, int V,
                       const int32_t* tokens, int64_t ld_tokens, int L, const int32_t* n_tokens,

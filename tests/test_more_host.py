@@ -117,6 +117,23 @@ def test_adjust_arguments(L):
     assert adjust(B=0, l=None, out=None) == ALV_OK
 
 
+def test_adjust_one_row_has_no_stride(L):
+    """The distance between rows counts for nothing where there is one, a zero neither; far rows and long lists of
+    biases are refused."""
+    from alveare_amd._lib import ALV_ERR_ARG, ALV_ERR_RANGE
+
+    def adjust(out, ld, B=1, M=0):
+        return L.alv_adjust_logits(P, ld, ctypes.c_void_p(out), ld, B, 100, None, 0, 0, None, None, None, 1.0, None, 0.0,
+                                   None, 0.0, P, 0, P, 0, M, None, 0, None)
+
+    for ld in (0, -1, 1, 100, 1000, 2 ** 62):
+        assert adjust((1 << 20) + 40, ld) == ALV_ERR_ARG, ld  # within the row
+        assert adjust((1 << 20) - 396, ld) == ALV_ERR_ARG, ld
+    assert adjust(1 << 30, 2 ** 62, B=2) == ALV_ERR_RANGE
+    assert adjust(1 << 30, 2 ** 40 + 1, B=2) == ALV_ERR_RANGE
+    assert adjust(1 << 30, 100, M=2 ** 16 + 1) == ALV_ERR_RANGE
+
+
 class _Host:
     """PagedCache with its pools on the host and page copies left out."""
 
