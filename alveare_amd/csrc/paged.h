@@ -114,29 +114,6 @@ __device__ __forceinline__ int group_len(const PagedBatch& a, int start, int end
     return max(0, min(min(len, a.kv_len[start]), a.max_pos)) >> a.shift << a.shift;
 }
 
-// The positions that sequence b shares with its group, and the group's first
-// sequence (b itself where it is in none), by the whole wave (b uniform).
-__device__ __forceinline__ int find_group(const PagedBatch& a, const PagedGroups& gr, int b, int lane, int* first) {
-    for (int j0 = 0; j0 < gr.n; j0 += 64) {
-        const int j = j0 + lane;
-        int lo = 0, hi = 0, len = 0;
-        if (j < gr.n) {
-            lo = gr.start[j];
-            hi = gr.start[j + 1];
-            len = gr.len[j];
-        }
-        const uint64_t m = __ballot(j < gr.n && lo <= b && b < hi);
-        if (m) {
-            const int l = __builtin_ctzll(m);
-            lo = __builtin_amdgcn_readlane(lo, l);
-            *first = lo;
-            return group_len(a, lo, __builtin_amdgcn_readlane(hi, l), __builtin_amdgcn_readlane(len, l));
-        }
-    }
-    *first = b;
-    return 0;
-}
-
 // The page of position p (0 <= p < max_pos) of sequence b, or -1.
 __device__ __forceinline__ int page_of(const PagedBatch& a, int b, int p) {
     const int e = a.table[(int64_t)b * a.ld_table + (p >> a.shift)];

@@ -1269,10 +1269,11 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
             p.w = uniform(recs[half].x), p.n = uniform(recs[half].y), p.r = uniform(recs[half].z) & (kTileRec - 1);
             p.tile = uniform(recs[half].z) & kTileRec, p.whole = p.n == kWhole;
             p.rows = p.tile ? TR : ROWS;
-            const int last = p.tile ? p.w + (p.n - 1) * a.kv_heads : p.w + p.n - 1;
+            const int most = p.tile ? a.tile_places : a.grid;
+            const int64_t last = p.w + (int64_t)(p.n - 1) * (p.tile ? a.kv_heads : 1);
             if (p.whole)
                 p.n = 1;
-            else if (p.n < 1 || p.w < 0 || p.r >= p.rows || last < p.w || last >= (p.tile ? a.tile_places : a.grid))
+            else if (p.n < 1 || p.w < 0 || p.r >= p.rows || last >= most)
                 p.n = 0;
         }
         if (uniform(recs[1].w) <= 0) x[0].n = 0;

@@ -475,7 +475,8 @@ int alv_qkv_post_paged(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off
  * k and v: a value is code * 2^(scale - 127). The power is the smallest that brings
  * the largest finite magnitude of the head's D bf16 values to 448 or less, at least
  * 2^-126; codes are the values over it, to nearest even; what is not finite becomes
- * NaN. Scales written are 1 to 254; one of 255 makes a slot's values infinite or NaN.
+ * NaN. Scales written are 1 to 247. One of 0 may count as 2^-127 or as 0, one of
+ * 255 makes a slot's values infinite or NaN.
  */
 int alv_qkv_post_paged8(const uint16_t* qkv, int64_t ld_qkv, int k_off, int v_off, int heads, int kv_heads, int D,
                         const float* q_w, const float* k_w, int norm_q, int norm_k, int norm_v, float eps,
@@ -537,7 +538,8 @@ int alv_attention_paged8(const uint16_t* q, int64_t ld_q, const uint8_t* kpages,
  * kernels. Every row sees what alv_attention_paged lets it see; what the two
  * parts of a row give is joined by their maxima and sums in float32, so its last
  * bits may differ from that call's. workspace: alv_attention_shared_workspace
- * bytes for the same arguments, as for alv_attention_paged.
+ * bytes for the same arguments (8 D + 48 for each row and head, and the parts of cut
+ * tiles), as for alv_attention_paged.
  */
 uint64_t alv_attention_shared_workspace(int heads, int kv_heads, int D, int B, int T, int max_q, int groups);
 int alv_attention_shared(const uint16_t* q, int64_t ld_q, const void* kpages, const void* vpages, int64_t k_stride,
