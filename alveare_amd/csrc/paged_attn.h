@@ -958,7 +958,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
 #pragma unroll
                         for (int i = 0; i < D / 64; ++i) {
                             if (KB > 0 && i % (KB > 0 ? KB : 1) == 0) asm volatile("" ::: "memory");
-                            const u32x4 k = *reinterpret_cast<const u32x4*>(kt + hf * (16 * D) + (rd_k ^ piece8<D>(4 * i)) + piece8_far<D>(4 * i));
+                            const u32x4 k = *reinterpret_cast<const u32x4*>(kt + hf * (16 * D) + (rd_k ^ piece8<D>(4 * i)) +
+                                                                            piece8_far<D>(4 * i));
                             product(widen8(k[0], k[1], kp), 2 * i);
                             product(widen8(k[2], k[3], kp), 2 * i + 1);
                         }
@@ -1312,7 +1313,9 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
 #pragma unroll
             for (int e = 0; e < RW; ++e) acc[e] = 0.0f;
             ls = 0.0f, mx = kNoMax;
-            join_parts<RW>(PG, lane, [&](int v) { return &sums[v][D]; }, [&](int v) { return &sums[v][D + 1]; }, [&](int v) { return &sums[v][RW * lane]; }, acc, mx, ls);
+            join_parts<RW>(
+                PG, lane, [&](int v) { return &sums[v][D]; }, [&](int v) { return &sums[v][D + 1]; },
+                [&](int v) { return &sums[v][RW * lane]; }, acc, mx, ls);
         }
         finish_row<D, false>(a, t, h, lane, acc, mx, ls, 0, true);
     }
@@ -1551,7 +1554,8 @@ __device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, i
 }
 
 template <int D, bool E8, bool MIX>
-__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileSteps& steps, int gt, int kvh, int split, int nsplit, int entry, int* tab, unsigned char* smem) {
+__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileSteps& steps, int gt, int kvh, int split, int nsplit,
+                                          int entry, int* tab, unsigned char* smem) {
     constexpr int DS = tile_ds(D), NW = tile_waves(D), TR = tile_rows(D), BN = tile_bn(D);
     constexpr int DW = D / DS;            // this wave's columns of the output (and of its scores' products)
     constexpr int TB = tile_bytes(D), NC = D / 8, RPL = 512 / D;
@@ -2142,7 +2146,8 @@ __global__ void __launch_bounds__((64 * tile_waves(D)), 2) attn_paged_tile_kerne
         kvh = item - gt * a.kv_heads;
     }
     // (tiles of more rows than max_q told of may be more than tab has entries for: they are not split)
-    tile_item<D, E8, MIX>(a, steps, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry), split ? a.tab : nullptr, smem);
+    tile_item<D, E8, MIX>(a, steps, uniform(gt), uniform(kvh), uniform(part), uniform(parts), uniform(entry),
+                          split ? a.tab : nullptr, smem);
 }
 
 // The parts of the tiles joined, `groups` workgroups to a tile, merge_rows(D) of

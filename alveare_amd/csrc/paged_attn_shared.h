@@ -65,6 +65,9 @@ int attention_shared(const SharedCall& c) {  // of one group at least
     if (int rc = attn_check(&a, c.D, c.page_table, c.ld_table, c.max_pages, c.q_start, c.kv_len, c.B, c.T, c.pages, c.page_size,
                             c.max_q))
         return rc;
+    // (groups and sequences are counted together, and every workgroup looks at all)
+    if (c.groups > kMaxRows || c.B > kMaxRows)
+        return fail(ALV_ERR_RANGE, "%d groups of %d sequences (at most 2^22 of each)", c.groups, c.B);
     if (c.T == 0) return ALV_OK;
     const SharedPlan p = shared_plan(c.heads, c.kv_heads, c.D, c.B, c.T, c.max_q, c.groups, E8);
     if (int rc = attn_fits(p.p, c.T, c.heads, c.B)) return rc;

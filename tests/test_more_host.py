@@ -73,6 +73,13 @@ def test_shared_arguments(L):
     assert shared(L, T=0, q=None, out=None) == ALV_OK
 
 
+def test_shared_too_many_groups(L):
+    from alveare_amd._lib import ALV_ERR_RANGE
+
+    for ch in (dict(G=(1 << 22) + 1), dict(G=2 ** 31 - 1), dict(B=(1 << 22) + 1), dict(G=2 ** 31 - 1, B=2 ** 31 - 1)):
+        assert shared(L, **ch) == ALV_ERR_RANGE, ch
+
+
 def test_post8_arguments(L):
     from alveare_amd._lib import ALV_ERR_ARG, ALV_ERR_RANGE, ALV_OK
 
