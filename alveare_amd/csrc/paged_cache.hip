@@ -55,9 +55,10 @@ struct PostPagedArgs {
 // What bounds it: one token, three dependent trips to memory (the sequence, its
 // page and RoPE row, the stores), 5 us; many, those trips again, six waves per SIMD
 // at a time (more would spill), and the arithmetic between them, by numpy's order and
-// two roundings some 25 instructions a value. 16 + 2 x 8 heads of 256, 4939 tokens: 44 us,
-// 3.7 TB/s, into bf16 pages and 42 into 8-bit ones (rounding and coding value by value 48
-// and 49; a wave per head and two-byte accesses: 101).
+// two roundings some 30 instructions a value (8-bit pages: the vector ALUs are busy 73 %
+// of the time). 16 + 2 x 8 heads of 256, 4939 tokens: 43.5 us, 3.8 TB/s, into bf16 pages
+// and 43.4, 3.3 TB/s, into 8-bit ones (rounding and coding value by value 47.6 and 49.3; a
+// wave per head and two-byte accesses: 101).
 constexpr int kPostMaxWaves = 8;
 constexpr int kLeafPad = 8;  // floats: leaves then start eight banks apart
 
@@ -219,18 +220,24 @@ __global__ void __launch_bounds__((64 * kPostMaxWaves), (WIDE ? 6 : 2)) qkv_post
         float sum = leaf8_sq_n<G::Leaf / 8>(row + (hl >> 3) * (G::Leaf + kLeafPad), hl & 7);
         if (G::Leaves > 1) sum = add_rn(sum, dpp_f<0x140>(sum));
         if (G::Leaves > 2) sum = add_rn(sum, __shfl_xor(sum, 16));
-        const float inv = __fdiv_rn(1.0f, sqrtf(add_rn(__fdiv_rn(sum, (float)D), a.eps)));
+        const float inv = __fdiv_rn(1.0f, sqrtf(add_rn(mul_rn(sum, 1.0f / D), a.eps)));  // (D: a power of two)
         const bool rot = d.role < 2 && rr;
 #pragma unroll
         for (int e = 0; e < G::Oct; ++e) {
             const int c0 = 8 * (hl + G::Lanes * e);
             if (norm) {
-                float w[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};  // (a product with 1 is its value)
-                if (d.w) load_w8(d.w, c0 / 8, w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = mul_rn(mul_rn(f[e][i], inv), w[i]);
+                for (int i = 0; i < 8; ++i) f[e][i] = mul_rn(f[e][i], inv);
+                if (d.w) {
+                    const float4* w = reinterpret_cast<const float4*>(d.w + c0);
+                    const float4 w0 = w[0], w1 = w[1];
+                    f[e][0] = mul_rn(f[e][0], w0.x), f[e][1] = mul_rn(f[e][1], w0.y);
+                    f[e][2] = mul_rn(f[e][2], w0.z), f[e][3] = mul_rn(f[e][3], w0.w);
+                    f[e][4] = mul_rn(f[e][4], w1.x), f[e][5] = mul_rn(f[e][5], w1.y);
+                    f[e][6] = mul_rn(f[e][6], w1.z), f[e][7] = mul_rn(f[e][7], w1.w);
+                }
                 uint32_t r[4];
-                round8(w, r);
+                round8(f[e], r);
                 unpack8(uint4{r[0], r[1], r[2], r[3]}, f[e]);
             }
             if (rr) {  // the whole wave: a head's rows hold what its pairs read
