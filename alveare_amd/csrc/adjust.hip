@@ -13,6 +13,11 @@
 // token's first bias, and passes once over the logits, which are on their way
 // meanwhile. In place, only what changes is read and written.
 //
+// Bound by memory where there are rows enough: 64 rows of 262144, 1 % allowed, in place
+// 14.7 us, 4.7 TB/s of words and -infinities; 48 rows of 128256 with histories of up to
+// 8000 tokens and 300 biases 16.3 us, 3.1 TB/s, by the 16 workgroups of a row that each
+// read its whole history (smaller ranges read it more often, larger ones leave CUs idle).
+// One row of 262144 with 1500 tokens: 7.3 us, three trips to memory one after the other.
 #include <algorithm>
 
 #include "q4_device.h"

@@ -536,6 +536,11 @@ __device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16
 // us), 5.2 (16 of 128 on 8: 128 us), 5.6 (16 of 256 on 8: 240 us) and 4.0 (16 of
 // 512 on 1: 85 us); a large copy moves 4.9 on this card, reads alone more. One
 // sequence of 300 positions is two launches, 14 us with the host's part.
+//
+// 8-bit pages: half the bytes, so twice the positions in each block and two workgroups
+// per CU, one computing while the other waits (D <= 256; a CU's LDS holds no more at
+// 512). 64 sequences of 100 to 8000 positions, 32 q heads of 64 on 8: 63 us, 4.5 TB/s, of
+// them 2 for the merge; the same over bf16 pages 114.
 
 // With groups or 8-bit pages a tile has kTileCost places in the line ahead of its units,
 // what its begin and end cost beside them: parts of many short tiles were the last to end
@@ -1245,7 +1250,8 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
 // MIX: the parts of every (row, head) joined, in the order shared, own: by a wave, or
 // (PG = 4: few rows, of many parts) by four, a quarter of each half's places each.
 // Records of sequences that are malformed may hold anything: they are not followed out
-// of bounds.
+// of bounds. Few rows: three trips to memory, 7 us; 576 rows of 512 in 45 parts 13 us, 4.5
+// TB/s.
 template <int D, int QT, int PG>
 __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
     constexpr int ROWS = 16 * QT, RW = D / 64, TR = 128;
@@ -1339,6 +1345,12 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
 // (1100), 16 of 512 on 1 1220 us (900). BN = 32 at D = 128 gains there (310 us)
 // and loses on the shorter ones (4096 tokens 120 -> 134 us, 2048 in a 1024 window
 // 52 -> 58); reading K ahead of the next loads' addresses costs 2 to 8 % at D <= 128.
+//
+// 8-bit pages: the widening is 2 vector instructions a matrix one more, 4096 tokens of 16
+// heads of 512 on one behind 2048 714 us (770 TFLOP/s): matrix cores busy 30 % of the
+// time, vector ALUs 46 %, the waves waiting 36 %. Groups: drafts of 16 sequences (0 to 5
+// tokens) over 20032 shared positions, 5 tiles in 45 parts each, 68 us, and 13 for the
+// join of 60 MB of parts.
 constexpr int tile_ds(int D) { return D == 512 ? 2 : 1; }      // waves that share 32 rows
 constexpr int tile_waves(int D) { return D == 512 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D) / tile_ds(D); }
