@@ -171,6 +171,32 @@ def test_shared_same_bits_and_apart(dev, D, n):
         assert ((got.double().cpu().view_as(want) - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("heads,kv_heads,D", [(32, 8, 64), (6, 2, 128), (16, 8, 256), (16, 1, 512)])
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("mq", [1, 2, 20, 100000])
+def test_shared_any_hint(dev, heads, kv_heads, D, bits, mq):
+    """max_q spreads the work; one that is wrong changes no row beyond its last bits, shared or not."""
+    from alveare_amd import attention_paged, attention_shared_paged
+
+    for n, own, groups in (([40, 1, 3, 0, 150], [60, 1, 90, 5, 170], [(4, 160), (1, 80)]), ([7], [40], [(1, 96)]),
+                           ([1] * 30, [1 + 3 * i for i in range(30)], [(30, 96)])):
+        b = batch(n, own, groups, kv_heads=kv_heads, D=D, page=16, dev=dev, bits=bits, extra_rows=2)
+        q = rows(b.T, heads * D, dev)
+        want, tol = M.attention(q, b, heads, 50, 3, 0.1)
+        kw = dict(heads=heads, window=50, sinks=3, scale=0.1, max_q=mq, scales=b.scales)
+        m = want.shape[0]
+        got = attention_shared_paged(q, *b.args(), *b.groups(), out=torch.full_like(q, 7.0), **kw)
+        assert ((got[:m].double().cpu().view_as(want) - want).abs() <= tol).all() and (got[m:] == 7.0).all()
+        at = 0
+        for count, s in groups:  # every sequence's own table names the shared pages too
+            s = min(s, b.total[at]) // 16
+            for c in range(at, at + count):
+                b.table[c, :s] = b.table[at, :s]
+            at += count
+        got = attention_paged(q, *b.args(), out=torch.full_like(q, 7.0), **kw)
+        assert ((got[:m].double().cpu().view_as(want) - want).abs() <= tol).all() and (got[m:] == 7.0).all()
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 def test_shared_missing_pages(dev, bits):
     """Shared pages that are gone are gone for all; a row with none left gets zeros."""
