@@ -1729,11 +1729,42 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileStep
         }
     };
 
+    // The first units' way begins ahead of q's, a trip to memory less. (What is fetched is
+    // one unit ahead of what is in LDS, with DS = 2 one phase.)
+    [[maybe_unused]] Codes kx, vx;
+    if (u1 > u0) {
+        load_pages(u0);
+        if constexpr (LC) {
+            // (DS = 1: three units ahead, of four; DS = 2: four phases, of three units)
+            constexpr int ahead = DS == 1 ? 3 : 2;
+#pragma unroll
+            for (int i = 0; i < ahead; ++i)
+                if (u0 + i < u1) {
+                    issue_codes(u0 + i, false);
+                    issue_codes(u0 + i, true);
+                }
+        } else if constexpr (E8) {
+            fetch(u0, false, kx);
+            fetch(u0, true, vx);
+        } else {
+            issue(u0, false);
+            issue(u0, true);
+        }
+    }
+
     // This lane's row: column col of the wave's 32.
     const int r0 = rt * TR + 32 * rg;
     const int nrows = max(0, min(32, n * a.g - r0));
     const int row = r0 + min(col, max(nrows - 1, 0));
     const int tok = min(row / a.g, n - 1), head = kvh * a.g + row % a.g;
+    bf16x8 q[DW / 16];
+    {
+        // (a lane's 16 bytes of codes are two operands: 16 columns of each 32)
+        const uint16_t* qr = a.q + (int64_t)(first + tok) * a.ld_q + head * D + dh * DW + (LC ? 16 : 8) * h;
+#pragma unroll
+        for (int i = 0; i < DW / 16; ++i)
+            q[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qr + (LC ? 32 * (i / 2) + 8 * (i % 2) : 16 * i)));
+    }
     int pos = len - n + tok, cap = pos;
     int wpos_lo = len - n + r0 / a.g;                        // lowest position up to which a row of the wave sees,
     int wpos_hi = len - n + (r0 + max(nrows, 1) - 1) / a.g;  // highest,
@@ -1746,18 +1777,10 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileStep
         wpos_lo = min64(cap), wpos_hi = max64(cap), wpos_top = max64(pos);
     }
     const float c = fmaxf(a.scale * kLog2e, kMinScale);
-    bf16x8 q[DW / 16];
-    {
-        // (a lane's 16 bytes of codes are two operands: 16 columns of each 32)
-        const uint16_t* qr = a.q + (int64_t)(first + tok) * a.ld_q + head * D + dh * DW + (LC ? 16 : 8) * h;
+    // Waited for here: the compiler would else wait at their first use, in
+    // the loop, each time, for whatever is on its way to LDS by then.
 #pragma unroll
-        for (int i = 0; i < DW / 16; ++i)
-            q[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qr + (LC ? 32 * (i / 2) + 8 * (i % 2) : 16 * i)));
-        // Waited for here: the compiler would else wait at their first use, in
-        // the loop, each time, for whatever is on its way to LDS by then.
-#pragma unroll
-        for (int i = 0; i < DW / 16; ++i) asm volatile("" : "+v"(q[i]));
-    }
+    for (int i = 0; i < DW / 16; ++i) asm volatile("" : "+v"(q[i]));
     f32x16 o[DW / 32];
 #pragma unroll
     for (int d = 0; d < DW / 32; ++d) o[d] = f32x16{};
@@ -1909,22 +1932,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileStep
         if constexpr (DS == 1) __builtin_amdgcn_s_setprio(0);
     };
 
-    // (what is fetched is one unit ahead of what is in LDS, with DS = 2 one phase)
-    [[maybe_unused]] Codes kx, vx;
-    if (u1 > u0) {
-        load_pages(u0);
-        if constexpr (LC) {
-            // (DS = 1: three units ahead, of four; DS = 2: four phases, of three units)
-            constexpr int ahead = DS == 1 ? 3 : 2;
-#pragma unroll
-            for (int i = 0; i < ahead; ++i)
-                if (u0 + i < u1) {
-                    issue_codes(u0 + i, false);
-                    issue_codes(u0 + i, true);
-                }
-        } else if constexpr (E8) {
-            fetch(u0, false, kx);
-            fetch(u0, true, vx);
+    if constexpr (E8 && !LC)
+        if (u1 > u0) {
             commit(u0, false, kx);
             if constexpr (DS == 1) {
                 commit(u0, true, vx);
@@ -1933,11 +1942,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileStep
                     fetch(u0 + 1, true, vx);
                 }
             }
-        } else {
-            issue(u0, false);
-            issue(u0, true);
         }
-    }
     if constexpr (DS == 1) {
 #pragma unroll 1
         for (int u = u0; u < u1; ++u) {
