@@ -1347,9 +1347,9 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
 // 52 -> 58); reading K ahead of the next loads' addresses costs 2 to 8 % at D <= 128.
 //
 // 8-bit pages: the widening is 2 vector instructions a matrix one more, 4096 tokens of 16
-// heads of 512 on one behind 2048 714 us (770 TFLOP/s): matrix cores busy 30 % of the
+// heads of 512 on one behind 2048 706 us (780 TFLOP/s): matrix cores busy 30 % of the
 // time, vector ALUs 46 %, the waves waiting 36 %. Groups: drafts of 16 sequences (0 to 5
-// tokens) over 20032 shared positions, 5 tiles in 45 parts each, 68 us, and 13 for the
+// tokens) over 20032 shared positions, 5 tiles in 45 parts each, 63 us, and 13 for the
 // join of 60 MB of parts.
 constexpr int tile_ds(int D) { return D == 512 ? 2 : 1; }      // waves that share 32 rows
 constexpr int tile_waves(int D) { return D == 512 ? 8 : 4; }
@@ -1539,7 +1539,7 @@ __device__ __forceinline__ int tile_cap(const PagedAttnArgs& a, const int* nu, i
         if (parts <= (MIX ? slots : 2 * slots)) return cap;
         // A group's tile's parts are as long as can be: no second turn, but the smallest cap of
         // 64, a lane each, whose parts all run at once (drafts of 16 sequences over 20032 shared
-        // positions and up to 3000 of their own, heads of 512: 150 -> 105 us; this search for
+        // positions and up to 3000 of their own, heads of 512: 150 -> 106 us; this search for
         // every call costs 64 tokens over 4 prompts of 4000 3 us of 60).
         if constexpr (MIX) {
             const int lo = max(least, (total + slots - 1) / slots), mine = lo + lane * (1 + lo / 48);
