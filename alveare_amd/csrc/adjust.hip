@@ -221,16 +221,23 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(AdjustArgs a) {
         if (made) y -= (double)f * made + (double)p;
         const int first = a.M - (int)(w >> F::kFirst);
         double sum = w >> F::kFirst ? bias[first] : 0.0;
-        // A token that is on the list again: all its biases in order, 64 entries at a time.
+        // A token that is on the list again: all its biases in order, 4 x 64 entries at a time.
         for (uint64_t more = __ballot((w & kTwice) != 0); more; more &= more - 1) {
             const int lane = __builtin_ctzll(more);
             const int token = (int)t0 + __builtin_amdgcn_readlane(i, lane);
             const int o = __builtin_amdgcn_readlane(first, lane);
             double s = bias[o];
-            for (int j0 = o + 1; j0 < a.M; j0 += 64) {
-                const int j = j0 + (tid & 63);
-                for (uint64_t hit = __ballot(j < a.M && list[min(j, a.M - 1)] == token); hit; hit &= hit - 1)
-                    s += bias[j0 + __builtin_ctzll(hit)];
+            for (int j0 = o + 1; j0 < a.M; j0 += 256) {
+                int entry[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int j = j0 + 64 * u + (tid & 63);
+                    entry[u] = j < a.M ? list[j] : -1;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    for (uint64_t hit = __ballot(entry[u] == token); hit; hit &= hit - 1)
+                        s += bias[j0 + 64 * u + __builtin_ctzll(hit)];
             }
             if ((tid & 63) == lane) sum = s;
         }
@@ -254,7 +261,7 @@ extern "C" int alv_adjust_logits(const float* logits, int64_t ld, float* out, in
     if (B < 0 || V < 1 || L < 0 || M < 0) return fail(ALV_ERR_ARG, "bad shape B=%d V=%d L=%d M=%d", B, V, L, M);
     if (B > 0 && (!logits || !out || (L > 0 && !tokens) || (M > 0 && (!bias_tokens || !bias))))
         return fail(ALV_ERR_ARG, "null pointer");
-    // (a list entry that is there again looks through the list: 2^16 of them take a wave 0.1 s at most)
+    // (a list entry that is there again looks through the list: 2^16 of them are tens of milliseconds at most)
     if (B > 65535 || V > 1 << 24 || L > 1 << 30 || M > 1 << 16 || (int64_t)B * V > (int64_t)1 << 35)
         return fail(ALV_ERR_RANGE, "%d rows of %d logits, %d tokens and %d biases each (at most 65535, 2^24, 2^30, 2^16; 2^35 logits)",
                     B, V, L, M);

@@ -132,6 +132,18 @@ def test_adjust_counts(dev):
     assert torch.equal(got, adjust_logits(logits, tokens=t.to(dev), n_tokens=over, frequency=1.0))
 
 
+@pytest.mark.parametrize("V,L,Mb", [(50000, 140000, 0), (3000, 131071, 8191), (3000, 131072, 8191), (3000, 40, 8192),
+                                    (262144, 140000, 65536)])
+def test_adjust_long_histories_and_lists(dev, V, L, Mb):
+    """On both sides of what 32 bits a token hold."""
+    c = make(2, V, L, Mb, dev, seed=L)
+    if V == 3000:
+        c["tokens"][0] = 7  # as often as there are tokens
+        c["n_prompt"][0] = 0
+    check(c, frequency=0.001)
+    check(c, in_place=True, frequency=0.001)
+
+
 def test_adjust_strides_and_alignment(dev):
     """Rows that start anywhere, columns of wider arrays, logits and out side by side in one array."""
     c = make(4, 2051, 90, 6, dev)
