@@ -569,13 +569,17 @@ constexpr int rows_out_ld(int D) { return D + 4; }
 // Whether q's operands stay in LDS rather than registers: where they and the
 // output take more than half of a wave's 256 (the rest would spill).
 constexpr bool rows_q_lds(int D, int QT) { return QT * D > 256; }
+// The waves' flags of outputs that are not finite, an int each, at the end.
+constexpr int rows_flags(int D, bool TWO) { return (4 * rows_waves(D, TWO) + 15) / 16 * 16; }
 constexpr int rows_lds(int D, int QT, bool E8, bool TWO) {
     const int NW = rows_waves(D, TWO), ring = NW * rows_stages(D) * rows_stage(D, E8);
     const int outs = NW * 16 * QT * (rows_out_ld(D) * 4);
-    return (ring > outs ? ring : outs) + 2 * NW * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0) + 16;
+    return (ring > outs ? ring : outs) + 2 * NW * 16 * QT * 4 + (rows_q_lds(D, QT) ? 32 * QT * D : 0) +
+           rows_flags(D, TWO);
 }
 constexpr int rows_mls(int D, int QT, bool E8, bool TWO) {  // where the waves' maxima and sums stand; q behind them
-    return rows_lds(D, QT, E8, TWO) - 16 - 2 * rows_waves(D, TWO) * 16 * QT * 4 - (rows_q_lds(D, QT) ? 32 * QT * D : 0);
+    return rows_lds(D, QT, E8, TWO) - rows_flags(D, TWO) - 2 * rows_waves(D, TWO) * 16 * QT * 4 -
+           (rows_q_lds(D, QT) ? 32 * QT * D : 0);
 }
 // Floats of one workspace place: outputs, maxima, sums.
 constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
@@ -768,7 +772,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn
     unsigned char* ring = smem + wave * NS * STAGE;
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
     float* mls = reinterpret_cast<float*>(smem + rows_mls(D, QT, E8, TWO));  // [wave][max | sum][row]
-    int* odds = reinterpret_cast<int*>(smem + rows_lds(D, QT, E8, TWO) - 16);
+    int* odds = reinterpret_cast<int*>(smem + rows_lds(D, QT, E8, TWO) - rows_flags(D, TWO));
     const float c = fmaxf(a.scale * kLog2e, kMinScale);
     const int S = 1 << a.b.shift;
     // Byte offsets that stay: this lane's piece of a load (memory side), of a K
