@@ -322,6 +322,15 @@ __device__ __forceinline__ int seq_count(const PagedAttnArgs& a) {
     return group_steps<MIX>(a) + a.b.B;
 }
 
+// The packed rows of group `start` .. end - 1 that are the batch's (none: nothing is shared).
+struct GroupRows {
+    int first, n;
+};
+__device__ __forceinline__ GroupRows group_rows(const PagedAttnArgs& a, int start, int end) {
+    const int first = max(0, a.b.q_start[start]), last = min(a.b.T, a.b.q_start[end]);
+    return {first, last > first ? last - first : 0};
+}
+
 // Group j0 + lane over what it shares (j0 uniform).
 __device__ __forceinline__ SeqIn group_in(const PagedAttnArgs& a, int j0, int lane) {
     SeqIn s{};
@@ -332,11 +341,11 @@ __device__ __forceinline__ SeqIn group_in(const PagedAttnArgs& a, int j0, int la
         end = a.gr.start[j + 1];
         s.len = group_len(a.b, s.seq, end, a.gr.len[j]);
         if (s.len > 0) {
-            s.first = a.b.q_start[s.seq];
-            s.n = a.b.q_start[end] - s.first;
-            s.here = s.first >= 0 && s.n > 0 && (int64_t)s.first + s.n <= a.b.T;
-            s.ok = true;
-            s.from = end;
+            const GroupRows r = group_rows(a, s.seq, end);
+            s.first = r.first, s.n = r.n;
+            s.here = s.ok = r.n > 0;
+            s.len = s.here ? s.len : 0;
+            s.from = s.here ? end : 0;
         }
     }
     if (a.window > 0) {
@@ -375,19 +384,26 @@ __device__ __forceinline__ SeqIn batch_in(const PagedAttnArgs& a, int b0, int la
         for (int j0 = 0; j0 < a.gr.n; j0 += 64) {
             const int j = j0 + lane;
             int lo = INT_MAX, hi = 0, len = 0;
+            GroupRows rows{};
             if (j0 == 0 && groups) {
-                if (j < a.gr.n) lo = groups->seq, hi = groups->from, len = groups->len;  // (none shared: no end)
+                if (j < a.gr.n) {  // (none shared: no end)
+                    lo = groups->seq, hi = groups->from, len = groups->len;
+                    rows = {groups->first, groups->n};
+                }
             } else if (j < a.gr.n) {
                 lo = a.gr.start[j];
                 hi = a.gr.start[j + 1];
                 len = group_len(a.b, lo, hi, a.gr.len[j]);
+                if (len > 0) rows = group_rows(a, lo, hi);
             }
             int l = 0;  // the last group that begins at b or before
 #pragma unroll
             for (int o = 32; o; o >>= 1)
                 if (__shfl(lo, l + o) <= b) l += o;
             const int end = __shfl(hi, l), shared = __shfl(len, l), begin = __shfl(lo, l);
-            if (begin <= b && b < end) s.from = shared;
+            const int first = __shfl(rows.first, l), n = __shfl(rows.n, l);
+            // (beside members that are malformed the group's rows may not be all of this one's)
+            if (begin <= b && b < end && s.here && first <= s.first && s.first - first <= n - s.n) s.from = shared;
         }
         if (!s.ok) s.from = 0;
     }
@@ -653,6 +669,7 @@ __device__ __forceinline__ uint64_t scan_all(const PagedAttnArgs& a, int lane, S
         Scan t;
         SeqIn groups{};
         groups.seq = sc.s.seq, groups.from = sc.s.from, groups.len = sc.s.len;
+        groups.first = sc.s.first, groups.n = sc.s.n;
         scan_step<ROWS, UNIT, COST, MIX>(a, b0, lane, total, t, MIX ? &groups : nullptr);
         if (MIX && b0 == 64) next = t;
         total = min(total + t.sum, (uint64_t)1 << 62);  // (sequences that overlap: no wrap)

@@ -40,3 +40,42 @@ def test_masked_nan_in_each_waves_block(dev, bits, heads):
         for got in (attention_paged(q, *b.args(), **kw), attention_shared_paged(q, *b.args(), *b.groups(), **kw)):
             close(got, want.view(2 * heads, 64), tol.view(2 * heads, 64), seen)
             assert torch.isnan(got.view(2 * heads, 64)[seen.stop:]).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("heads,kv_heads,D", [(8, 2, 128), (4, 1, 256), (16, 1, 512)])
+@pytest.mark.parametrize("n", [[2, 3, 1, 2], [50, 3, 1, 70]])
+@pytest.mark.parametrize("window", [0, 30])
+def test_members_beside_malformed_ones(dev, bits, heads, kv_heads, D, n, window):
+    """A member whose rows do not fit the batch takes its group along with it nowhere: the others' outputs are what
+    they are without it. Where no rows of a group are the batch's, or not those of a member, that shares nothing."""
+    from alveare_amd import attention_paged, attention_shared_paged
+    from alveare_amd._lib import lib
+
+    total = [v + 64 + i for i, v in enumerate(n)]
+    at = [sum(n[:i]) for i in range(5)]
+    kw = dict(heads=heads, window=window, sinks=2 if window else 0, scale=0.1)
+
+    def run(b, q, q_start, mq):
+        size = lib().alv_attention_shared_workspace(heads, kv_heads, D, 4, len(q), mq, 1)
+        stale = torch.full((size,), 255, dtype=torch.uint8, device=dev)  # what the call's workspace holds
+        del stale
+        b.q_start.copy_(torch.tensor(q_start))
+        return attention_shared_paged(q, *b.args(), *b.groups(), max_q=mq, scales=b.scales,
+                                      out=torch.full_like(q, 7.0), **kw)
+
+    b = M.Batch(n, total, kv_heads=kv_heads, D=D, page=16, dev=dev, bits=bits, groups=[(4, 64)])
+    q = rows(b.T, heads * D, dev)
+    want, tol = M.attention(q, b, heads, window, kw["sinks"], 0.1)
+    for mq in (0, max(n)):
+        close(run(b, q[:-1], at, mq), want[:at[3]], tol[:at[3]])                      # the last one's end past the rows
+        close(run(b, q, [*at[:4], 2 ** 31 - 1], mq), want[:at[3]], tol[:at[3]])
+        out = run(b, q, [-1, *at[1:]], mq)                                            # the first begins ahead of them
+        close(out[n[0]:], want[n[0]:], tol[n[0]:])
+    # with pages of their own
+    b = M.Batch(n, total, kv_heads=kv_heads, D=D, page=16, dev=dev, bits=bits)
+    want, tol = M.attention(q, b, heads, window, kw["sinks"], 0.1)
+    b.group_start, b.shared_len = (torch.tensor(v, dtype=torch.int32, device=dev) for v in ([0, 4], [64]))
+    for mq in (0, max(n)):
+        close(run(b, q, [*at[:4], -5], mq), want[:at[3]], tol[:at[3]])               # the group has no rows
+        close(run(b, q, [0, at[1], at[2], at[3], 1], mq)[at[2]:], want[at[2]:at[3]], tol[at[2]:at[3]])  # or one
