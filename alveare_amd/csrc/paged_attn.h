@@ -553,10 +553,12 @@ __device__ void plain_row(const PagedAttnArgs& a, int seq, int kvh, const uint16
 // 512 on 1: 85 us); a large copy moves 4.9 on this card, reads alone more. One
 // sequence of 300 positions is two launches, 14 us with the host's part.
 //
-// 8-bit pages: half the bytes, so twice the positions in each block and two workgroups
-// per CU, one computing while the other waits (D <= 256; a CU's LDS holds no more at
-// 512). 64 sequences of 100 to 8000 positions, 32 q heads of 64 on 8: 63 us, 4.5 TB/s, of
-// them 2 for the merge; the same over bf16 pages 114.
+// 8-bit pages: half the bytes, so twice the positions in each block and, where its LDS
+// holds both, two workgroups per CU, one computing while the other waits (not at 512, nor
+// with q in LDS too: there as many waves in one, where half of them were left when two
+// were counted on: 16 tokens of 64 sequences of 116 to 3016 positions, 16 heads of 256 on 8
+// 205 -> 131 us, 32 of 128 on 8 220 -> 128). 64 sequences of 100 to 8000 positions, 32 q
+// heads of 64 on 8: 63 us, 4.5 TB/s, of them 2 for the merge; the same over bf16 pages 114.
 
 // With groups or 8-bit pages a tile has kTileCost places in the line ahead of its units,
 // what its begin and end cost beside them: parts of many short tiles were the last to end
@@ -573,7 +575,7 @@ struct RowsSeq {
     int us, ulo, nu;  // units of first tokens; first unit of the window; units in all
 };
 
-constexpr bool rows_two(int D, bool E8) { return E8 && D <= 256; }  // two workgroups per CU, else one
+// TWO: two workgroups per CU (rows_two), else one.
 constexpr int rows_waves(int D, bool TWO) { return (D == 512 ? 2 : (D == 64 ? 8 : 4)) / (TWO ? 2 : 1); }
 // A wave's block: 16 positions' K and V, or 32 of 8-bit ones and their powers.
 constexpr int rows_block(bool E8) { return E8 ? 32 : 16; }
@@ -597,6 +599,9 @@ constexpr int rows_mls(int D, int QT, bool E8, bool TWO) {  // where the waves' 
     return rows_lds(D, QT, E8, TWO) - rows_flags(D, TWO) - 2 * rows_waves(D, TWO) * 16 * QT * 4 -
            (rows_q_lds(D, QT) ? 32 * QT * D : 0);
 }
+// Whether two workgroups share a CU: 8-bit pages, and where both fit its LDS.
+constexpr int kCuLds = 160 * 1024;
+constexpr bool rows_two(int D, int QT, bool E8) { return E8 && D <= 256 && 2 * rows_lds(D, QT, E8, true) <= kCuLds; }
 // Floats of one workspace place: outputs, maxima, sums.
 constexpr int rows_part(int D, int QT) { return 16 * QT * (D + 2); }
 
@@ -758,8 +763,8 @@ __device__ __forceinline__ uint32_t part_count(uint64_t total, const Scan& sc, i
 }
 
 template <int D, int QT, bool E8, bool MIX>
-__global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, E8))), 2) attn_paged_rows_kernel(PagedAttnArgs a) {
-    constexpr bool TWO = rows_two(D, E8);
+__global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, QT, E8))), 2) attn_paged_rows_kernel(PagedAttnArgs a) {
+    constexpr bool TWO = rows_two(D, QT, E8);
     constexpr int NW = rows_waves(D, TWO), NS = rows_stages(D), UNIT = rows_unit(D, E8, TWO), ROWS = 16 * QT;
     constexpr int BP = rows_block(E8), NH = BP / 16;  // positions of a block, 16 at a time (within a page)
     constexpr int STAGE = rows_stage(D, E8);
@@ -2292,7 +2297,7 @@ __attribute__((unused)) AttnPlan attn_plan(int heads, int kv_heads, int D, int B
         const int64_t r = tiles ? g : rows;
         p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
         p.row_limit = tiles ? 16 * p.qt : INT64_MAX;
-        p.grid = device_cus() * (rows_two(D, e8) ? 2 : 1);
+        p.grid = device_cus() * (rows_two(D, p.qt, e8) ? 2 : 1);
         p.cuts_bytes = (uint64_t)p.grid * kTabInts * sizeof(int);
         p.rows_bytes = p.cuts_bytes + (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
     }
@@ -2334,7 +2339,7 @@ __attribute__((unused)) AttnPlan mix_plan(int heads, int kv_heads, int D, int B,
         const int64_t r = group_tiles ? rows : std::max(rows, group_rows);
         p.qt = std::min(qt_max, r <= 16 ? 1 : (r <= 32 ? 2 : 4));
         p.row_limit = group_tiles ? 16 * p.qt : INT64_MAX;
-        p.grid = device_cus() * (rows_two(D, e8) ? 2 : 1);
+        p.grid = device_cus() * (rows_two(D, p.qt, e8) ? 2 : 1);
         p.rows_bytes = (uint64_t)p.grid * 2 * 16 * p.qt * (D + 2) * sizeof(float);
     }
     p.part_bytes = p.rows_bytes;
@@ -2363,9 +2368,9 @@ __attribute__((unused)) int allow_lds(const void* k, int lds, std::atomic<uint64
 
 template <int D, int QT, bool E8, bool MIX>
 int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    constexpr bool TWO = rows_two(D, E8);
+    constexpr bool TWO = rows_two(D, QT, E8);
     constexpr int lds = rows_lds(D, QT, E8, TWO);
-    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    static_assert(lds <= kCuLds, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_rows_kernel<D, QT, E8, MIX>), lds, done)) return rc;
     hipLaunchKernelGGL((attn_paged_rows_kernel<D, QT, E8, MIX>), dim3(p.grid), dim3(64 * rows_waves(D, TWO)), lds, s, a);
@@ -2378,7 +2383,7 @@ int launch_rows(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
 template <int D, bool E8, bool MIX>
 int launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     constexpr int lds = tile_lds(D, E8);
-    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    static_assert(lds <= kCuLds, "LDS of a CU");
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_paged_tile_kernel<D, E8, MIX>), lds, done)) return rc;
     hipLaunchKernelGGL((attn_paged_tile_kernel<D, E8, MIX>), dim3((uint32_t)std::max(p.grid_tiles, (int64_t)p.slots * 2)), dim3(64 * tile_waves(D)), lds, s, a);

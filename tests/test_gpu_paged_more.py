@@ -79,3 +79,19 @@ def test_members_beside_malformed_ones(dev, bits, heads, kv_heads, D, n, window)
     for mq in (0, max(n)):
         close(run(b, q, [*at[:4], -5], mq), want[:at[3]], tol[:at[3]])               # the group has no rows
         close(run(b, q, [0, at[1], at[2], at[3], 1], mq)[at[2]:], want[at[2]:at[3]], tol[at[2]:at[3]])  # or one
+
+
+@pytest.mark.parametrize("heads,D", [(32, 64), (64, 64), (128, 64), (128, 128), (64, 256)])
+@pytest.mark.parametrize("page", [16, 64])
+def test_streaming_of_many_rows_over_8_bit_pages(dev, heads, D, page):
+    """Up to 64 rows of a sequence and kv head (32 at D = 256) in a batch too large for tiles."""
+    from alveare_amd import attention_paged
+
+    B = 140
+    n = [i % 2 if i > 130 else 1 for i in range(B)]
+    total = [1 + (i * 29) % 140 + (800 if i == 7 else 0) for i in range(B)]
+    b = M.Batch(n, total, kv_heads=2, D=D, page=page, dev=dev)
+    q = rows(b.T, heads * D, dev)
+    for window in (0, 50):
+        want, tol = M.attention(q, b, heads, window, 0, 0.1)
+        close(attention_paged(q, *b.args(), heads=heads, window=window, scale=0.1, max_q=1, scales=b.scales), want, tol)

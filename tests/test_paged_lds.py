@@ -33,3 +33,11 @@ def test_every_wave_has_a_flag(tmp_path):
     static_assert(rows_lds(D, QT, E8, {two}) - used >= 4 * waves, "a flag for each wave");
     static_assert(used % 4 == 0, "aligned");
 """)
+
+
+def test_workgroups_that_share_a_cu_fit_its_lds(tmp_path):
+    """The streaming kernel's grid counts on two workgroups a CU where rows_two says so, else on one."""
+    compiles(tmp_path, """
+    static_assert((rows_two(D, QT, E8) ? 2 : 1) * rows_lds(D, QT, E8, rows_two(D, QT, E8)) <= 160 * 1024, "LDS of a CU");
+    static_assert(E8 || !rows_two(D, QT, E8), "bf16 rings are a CU's");
+""")
