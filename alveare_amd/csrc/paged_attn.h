@@ -453,6 +453,21 @@ __device__ __forceinline__ int min64(int v) {
 }
 __device__ __forceinline__ int max64(int v) { return -min64(-v); }
 
+// The units of positions that a run begins with, before it goes on from `lo`, the first
+// that a window holds: `us` units of first tokens from 0 on, then from unit `ulo` on. own:
+// behind the `from` positions that a group shares; where the gap is no more units than they
+// are, straight from there.
+struct Begin {
+    int us, ulo;
+};
+template <int UNIT>
+__device__ __forceinline__ Begin begin_units(const PagedAttnArgs& a, int lo, bool own, int from) {
+    if (own && a.sinks <= from) return {0, max(lo, from) / UNIT};
+    const int ulo = lo / UNIT, us = min((min(a.sinks, lo) + UNIT - 1) / UNIT, ulo);
+    if (own && us + from / UNIT >= ulo) return {0, from / UNIT};
+    return {us, ulo};
+}
+
 constexpr float kNoMax = -3.0e38f;  // running maximum of a row that has seen nothing
 constexpr float kMinScale = 1e-37f;  // -infinity times it is -infinity, a score times it 0
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -638,10 +653,9 @@ __device__ __forceinline__ void scan_step(const PagedAttnArgs& a, int b0, int la
     if (in.here && rows <= a.row_limit) {
         s.tiles = (int)((rows + ROWS - 1) / ROWS);
         if (in.ok) {
-            int lo = a.window > 0 ? max(0, in.lo + 1 - a.window) : 0;
-            if (suf) lo = a.sinks > s.from ? s.from : max(lo, s.from);
-            s.ulo = lo / UNIT;
-            s.us = suf ? 0 : min((min(a.sinks, lo) + UNIT - 1) / UNIT, s.ulo);
+            const int lo = a.window > 0 ? max(0, in.lo + 1 - a.window) : 0;
+            const Begin at = begin_units<UNIT>(a, lo, suf, s.from);
+            s.us = at.us, s.ulo = at.ulo;
             // (one at least: there may be nothing within the window, nothing behind what is shared)
             s.nu = s.us + max((s.len + UNIT - 1) / UNIT - s.ulo, !MIX ? INT_MIN : s.us ? 0 : 1);
         } else {
@@ -1435,11 +1449,9 @@ __device__ __forceinline__ TileSpan tile_span(const PagedAttnArgs& a, int n, int
     s.rows = min(TR, n * a.g - r0);
     s.pos_lo = pre ? low : len - n + r0 / a.g;
     s.pos_hi = pre ? len - 1 : len - n + (r0 + s.rows - 1) / a.g;
-    int lo = a.window > 0 ? max(0, s.pos_lo + 1 - a.window) : 0;
-    const bool suf = MIX && !pre;
-    if (suf) lo = a.sinks > from ? from : max(lo, from);
-    s.ulo = lo / BN;
-    s.us = suf ? 0 : min((min(a.sinks, lo) + BN - 1) / BN, s.ulo);
+    const int lo = a.window > 0 ? max(0, s.pos_lo + 1 - a.window) : 0;
+    const Begin at = begin_units<BN>(a, lo, MIX && !pre, from);
+    s.us = at.us, s.ulo = at.ulo;
     s.nu = ok ? s.us + max(s.pos_hi / BN + 1 - s.ulo, !MIX ? INT_MIN : 0) : 0;
     return s;
 }

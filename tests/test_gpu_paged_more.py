@@ -95,3 +95,54 @@ def test_streaming_of_many_rows_over_8_bit_pages(dev, heads, D, page):
     for window in (0, 50):
         want, tol = M.attention(q, b, heads, window, 0, 0.1)
         close(attention_paged(q, *b.args(), heads=heads, window=window, scale=0.1, max_q=1, scales=b.scales), want, tol)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("heads,kv_heads,D", [(4, 2, 64), (8, 2, 128), (4, 1, 256), (16, 1, 512)])
+@pytest.mark.parametrize("n", [[1, 1, 1, 1, 1], [1, 3, 70, 0, 140]])
+def test_first_tokens_on_both_sides_of_what_is_shared(dev, bits, heads, kv_heads, D, n):
+    """A window, and first tokens that end ahead of a group's shared positions, within and behind them."""
+    from alveare_amd import attention_shared_paged
+
+    own = [700, 430, 500, 90, 810]
+    total = [o + s for o, s in zip(own, (64, 64, 0, 208, 208))]
+    b = M.Batch(n, total, kv_heads=kv_heads, D=D, page=16, dev=dev, bits=bits, groups=[(2, 64), (1, 0), (2, 208)])
+    q = rows(b.T, heads * D, dev)
+    for window, sinks in ((100, 1), (100, 64), (100, 65), (30, 150), (100, 300), (600, 4), (1, 900)):
+        want, tol = M.attention(q, b, heads, window, sinks, 0.1)
+        for mq in (0, max(n)):
+            close(attention_shared_paged(q, *b.args(), *b.groups(), heads=heads, window=window, sinks=sinks, scale=0.1,
+                                         max_q=mq, scales=b.scales), want, tol)
+
+
+@pytest.mark.parametrize("D,n", [(64, 1), (256, 1), (128, 64), (512, 64)])
+def test_a_window_with_first_tokens_bounds_what_is_read(dev, D, n):
+    """Sequences that share nothing, 40000 positions behind a window of 512: the time is attention_paged's, which
+    reads some 600 (all of them would take tens of times as long)."""
+    from alveare_amd import attention_paged, attention_shared_paged
+
+    B, L, S = 16, 40000, 64
+    need = (L + S - 1) // S
+    k, v = (torch.randn(B * need, 1, S, D, device=dev).to(bf) for _ in range(2))
+    i32 = dict(dtype=torch.int32, device=dev)
+    table = torch.arange(B * need, **i32).view(B, need)
+    q = rows(B * n, 4 * D, dev)
+    args = q, k, v, table, torch.arange(0, B * n + 1, n, **i32), torch.full((B,), L, **i32)
+    groups = torch.arange(B + 1, **i32), torch.zeros(B, **i32)
+    kw = dict(heads=4, window=512, sinks=4, scale=0.1, max_q=n)
+
+    def least(call):
+        times = []
+        for _ in range(8):
+            a, z = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                call()
+            z.record()
+            z.synchronize()
+            times.append(a.elapsed_time(z))
+        return min(times)
+
+    plain = least(lambda: attention_paged(*args, **kw))
+    shared = least(lambda: attention_shared_paged(*args, *groups, **kw))
+    assert shared < 4 * plain, (shared, plain)
