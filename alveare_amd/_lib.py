@@ -155,7 +155,11 @@ def call(L, name: str, *args) -> None:
         check(getattr(L, name)(*args), name)
         return
     entry, n, words = PACKED[name]
-    check(packed(entry, words.pack(*args), n), name)
+    try:
+        array = words.pack(*args)
+    except (struct.error, TypeError) as e:  # (what is no number of its kind: as ctypes has it)
+        raise ctypes.ArgumentError(f"{name}: {e}") from None
+    check(packed(entry, array, n), name)
 
 
 def check(rc: int, what: str) -> None:
