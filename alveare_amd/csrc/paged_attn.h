@@ -242,6 +242,16 @@ __device__ __forceinline__ i32x2 read_tr8(const unsigned char* p) {
     return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(p));
 }
 
+// Of N slots' powers in LDS V's from slot `have` on, behind the end, cleared: any byte may be
+// there, and a weight of 0 times an infinite power is NaN. (K's make scores that the mask
+// drops.)
+template <int N>
+__device__ __forceinline__ void clear_powers(unsigned char* pairs, int have) {
+    const int i = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, here(0)));  // (the lane, no register kept)
+    if (i < N && i >= have) pairs[2 * i + 1] = 0;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
 // What a row sees of its launch's positions: from .. cap, of these the window of its
 // own position `pos` and the first tokens.
 struct Sight {
@@ -981,6 +991,7 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, QT, E8))), 2) 
                 wait_vm<0>();
             const unsigned char* kt = ring + (j % NS) * STAGE;
             const unsigned char* vt = kt + HALF;
+            if (E8 && j + 1 == nblk) clear_powers<BP>(ring + (j % NS) * STAGE + 64 * D, f.s.len - block_pos(j));
                 f32x4 s[NH][NT];
                 constexpr int KB = QT * D >= 512 ? (QT == 4 ? 1 : 2) : 0;  // K reads of codes at once, where registers are short
                 [[maybe_unused]] i32x2 powers[NH];  // of this lane's positions: k's, v's in turn
@@ -1724,6 +1735,12 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileStep
                               __builtin_amdgcn_readfirstlane(lds_addr(pow)) + (uint32_t)(u - u0) % kPowers * (2 * BN) + wave * (2 * LR));
     };
 
+    // The last unit, u1 - 1, may end behind len: its powers there.
+    [[maybe_unused]] const int tail = u1 > u0 ? len - unit_pos(u1 - 1) : BN;
+    [[maybe_unused]] auto powers_end = [&](int u) __attribute__((always_inline)) {
+        if (u + 1 == u1 && tail < BN) clear_powers<BN>(pow + (uint32_t)(u - u0) % kPowers * (2 * BN), tail);
+    };
+
     // Or a wave's share of a unit goes through registers, where codes become bf16
     // times their power, so that what LDS holds and the products are the same.
     constexpr int NP = E8 ? LR * D / 1024 : 1;  // pieces of 16 codes of a lane, of K (of V)
@@ -2005,6 +2022,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileStep
                     issue_codes(u + 3, false);
                     issue_codes(u + 3, true);
                 }
+                powers_end(u);  // (each wave for itself)
             } else if (u + 1 < u1) {
                 if constexpr (E8) {
                     commit(u + 1, false, kx);
@@ -2076,6 +2094,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileStep
             const int p0 = unit_pos(u);
             f32x16 s{};
             begin(2 * (u - u0) + grp);
+            if constexpr (LC)
+                if (wave == 0) powers_end(u);  // (for all: V's are read from the next phase on)
             if (!skip(p0)) {
                 const uint32_t slot = LC ? slot_of(u) : u & 1;
                 s = scores(kbuf + slot * (LC ? TC : TB), pow + (uint32_t)(u - u0) % kPowers * (2 * BN));

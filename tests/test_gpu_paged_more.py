@@ -146,3 +146,41 @@ def test_a_window_with_first_tokens_bounds_what_is_read(dev, D, n):
     plain = least(lambda: attention_paged(*args, **kw))
     shared = least(lambda: attention_shared_paged(*args, *groups, **kw))
     assert shared < 4 * plain, (shared, plain)
+
+
+@pytest.mark.parametrize("heads,kv_heads,D", [(8, 2, 64), (8, 2, 128), (4, 1, 256), (16, 1, 512)])
+@pytest.mark.parametrize("n", [[1, 1, 1, 1], [3, 70, 0, 5], [130, 1, 150, 40]])
+def test_powers_behind_the_end_do_not_matter(dev, heads, kv_heads, D, n):
+    """Slots that no sequence holds have the largest power byte; the output is the same to the bit, and no wave
+    does its rows again for it (which takes tens of times as long)."""
+    from alveare_amd import attention_paged, attention_shared_paged
+
+    total = [v + p for v, p in zip(n, (2001, 1999, 640, 830))]
+    b = M.Batch(n, total, kv_heads=kv_heads, D=D, page=64, dev=dev, groups=[(2, 512), (2, 0)])
+    q = rows(b.T, heads * D, dev)
+    kw = dict(heads=heads, scale=0.1, max_q=max(n), scales=b.scales)
+    bytes_ = b.scales.view(torch.uint8)
+    held = torch.zeros(b.pages, 64, dtype=torch.bool)
+    for s, t in enumerate(total):
+        for p in range(b.shared[s] if b.leader[s] != s else 0, t):
+            held[int(b.table[s, p // 64]), p % 64] = True
+    free = (~held)[:, None, :, None].expand(bytes_.shape).to(dev)
+    made = []
+    for power in (127, 255):
+        bytes_[free] = power
+        calls = (lambda: attention_paged(q, *b.args(), **kw), lambda: attention_shared_paged(q, *b.args(), *b.groups(), **kw))
+        for call in calls:
+            times = []
+            out = call()
+            for _ in range(6):
+                a, z = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+                a.record()
+                for _ in range(5):
+                    call()
+                z.record()
+                z.synchronize()
+                times.append(a.elapsed_time(z))
+            made.append((out, min(times)))
+    for (a, ta), (z, tz) in zip(made[:2], made[2:]):
+        assert torch.equal(a.view(torch.int16), z.view(torch.int16))
+        assert tz < 3 * ta, (ta, tz)
