@@ -857,7 +857,8 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, QT, E8))), 2) 
         auto load_pages = [&](int j0) {
             pages0 = j0;
             const int j = j0 + (lane >> halves), p = block_pos(j) + 16 * (lane & halves);
-            pages = j < nblk && p < f.s.len ? table[p >> a.b.shift] : -1;
+            // (what a group shares is not this sequence's to read: its entries may be any)
+            pages = j < nblk && p < f.s.len && (!suf || p >= f.s.from) ? table[p >> a.b.shift] : -1;
             if ((unsigned)pages >= (unsigned)a.b.pages) pages = -1;
             if constexpr (E8) {
                 const int64_t slot = ((int64_t)f.kvh << a.b.shift) + (p & (S - 1));
@@ -1665,7 +1666,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, const TileStep
         const int p = unit_pos(v0 + lane);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const bool in = v0 + lane < u1 && p + 16 * k < len;
+            const bool in = v0 + lane < u1 && p + 16 * k < len && (!suf || p + 16 * k >= from);  // (else any entry may be there)
             int e = in ? table[(p + 16 * k) >> a.b.shift] : -1;
             if ((unsigned)e >= (unsigned)a.b.pages) e = -1;
             gone[k] = __ballot(in && e < 0);

@@ -184,3 +184,40 @@ def test_powers_behind_the_end_do_not_matter(dev, heads, kv_heads, D, n):
     for (a, ta), (z, tz) in zip(made[:2], made[2:]):
         assert torch.equal(a.view(torch.int16), z.view(torch.int16))
         assert tz < 3 * ta, (ta, tz)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("heads,kv_heads,D", [(8, 2, 64), (8, 2, 128), (4, 1, 256), (16, 1, 512)])
+@pytest.mark.parametrize("n", [[1, 1, 1, 1], [3, 70, 0, 5], [130, 1, 150, 40]])
+def test_table_entries_of_what_is_shared_do_not_matter(dev, bits, heads, kv_heads, D, n):
+    """The members' own entries for shared positions name no page, or one of NaN: the same bits, and no wave does
+    its rows again for it (which takes tens of times as long)."""
+    from alveare_amd import attention_shared_paged
+
+    total = [v + p for v, p in zip(n, (2001, 1999, 840, 2830))]
+    b = M.Batch(n, total, kv_heads=kv_heads, D=D, page=16, dev=dev, bits=bits, groups=[(2, 528), (2, 528)])
+    q = rows(b.T, heads * D, dev)
+    kw = dict(heads=heads, scale=0.1, max_q=max(n), scales=b.scales)
+    used = set(b.table[(b.table >= 0) & (b.table < b.pages)].tolist())
+    spare = next(p for p in range(b.pages) if p not in used)
+    if bits == 8:
+        b.scales.view(torch.uint8)[spare] = 255
+    for window, sinks in ((0, 0), (700, 600)):
+        made = []
+        for entry in (-1, spare):
+            b.table[1, :33] = b.table[3, :33] = entry
+            call = lambda: attention_shared_paged(q, *b.args(), *b.groups(), window=window, sinks=sinks, **kw)  # noqa: E731
+            out = call()
+            times = []
+            for _ in range(6):
+                a, z = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+                a.record()
+                for _ in range(5):
+                    call()
+                z.record()
+                z.synchronize()
+                times.append(a.elapsed_time(z))
+            made.append((out, min(times)))
+        (a, ta), (z, tz) = made
+        assert torch.equal(a.view(torch.int16), z.view(torch.int16))
+        assert tz < 3 * ta, (ta, tz)
