@@ -984,15 +984,15 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, QT, E8))), 2) 
         auto blocks = [&](auto count) __attribute__((always_inline)) {
             constexpr int NT = decltype(count)::value;  // row tiles of 16 that there are
 #pragma unroll 1
-        for (int j = 0; j < nblk; ++j) {
-            // Blocks j + 1 .. j + NS - 1 may be in flight.
-            if (j + NS <= nblk)
-                wait_vm<(NS - 1) * LOADS>();
-            else
-                wait_vm<0>();
-            const unsigned char* kt = ring + (j % NS) * STAGE;
-            const unsigned char* vt = kt + HALF;
-            if (E8 && j + 1 == nblk) clear_powers<BP>(ring + (j % NS) * STAGE + 64 * D, f.s.len - block_pos(j));
+            for (int j = 0; j < nblk; ++j) {
+                // Blocks j + 1 .. j + NS - 1 may be in flight.
+                if (j + NS <= nblk)
+                    wait_vm<(NS - 1) * LOADS>();
+                else
+                    wait_vm<0>();
+                const unsigned char* kt = ring + (j % NS) * STAGE;
+                const unsigned char* vt = kt + HALF;
+                if (E8 && j + 1 == nblk) clear_powers<BP>(ring + (j % NS) * STAGE + 64 * D, f.s.len - block_pos(j));
                 f32x4 s[NH][NT];
                 constexpr int KB = QT * D >= 512 ? (QT == 4 ? 1 : 2) : 0;  // K reads of codes at once, where registers are short
                 [[maybe_unused]] i32x2 powers[NH];  // of this lane's positions: k's, v's in turn
@@ -1125,10 +1125,10 @@ __global__ void __launch_bounds__((64 * rows_waves(D, rows_two(D, QT, E8))), 2) 
                         }
                     }
                 }
-            // The buffer's reads are done before it is filled again.
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (j + NS < nblk) issue(j + NS);
-        }
+                // The buffer's reads are done before it is filled again.
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (j + NS < nblk) issue(j + NS);
+            }
         };
         if (MIX && QT > 1 && nrows <= 16)
             blocks(std::integral_constant<int, 1>());
