@@ -1302,7 +1302,7 @@ __global__ void __launch_bounds__(256) attn_paged_rows_merge_kernel(PagedAttnArg
 // MIX: the parts of every (row, head) joined, in the order shared, own: by a wave, or
 // (PG = 4: few rows, of many parts) by four, a quarter of each half's places each.
 // Records of sequences that are malformed may hold anything: they are not followed out
-// of bounds. Few rows: three trips to memory, 7 us; 576 rows of 512 in 45 parts 13 us, 4.5
+// of bounds. Few rows: three trips to memory, 7 us; 576 rows of 512 in 45 parts 16 us, 3.7
 // TB/s.
 template <int D, int QT, int PG>
 __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
@@ -1401,7 +1401,7 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a) {
 // 8-bit pages: the widening is 2 vector instructions a matrix one more, 4096 tokens of 16
 // heads of 512 on one behind 2048 706 us (780 TFLOP/s): matrix cores busy 30 % of the
 // time, vector ALUs 46 %, the waves waiting 36 %. Groups: drafts of 16 sequences (0 to 5
-// tokens) over 20032 shared positions, 5 tiles in 45 parts each, 63 us, and 13 for the
+// tokens) over 20032 shared positions, 5 tiles in 45 parts each, 65 us, and 16 for the
 // join of 60 MB of parts.
 constexpr int tile_ds(int D) { return D == 512 ? 2 : 1; }      // waves that share 32 rows
 constexpr int tile_waves(int D) { return D == 512 ? 8 : 4; }

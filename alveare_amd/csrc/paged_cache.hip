@@ -79,8 +79,8 @@ struct PostGeom {
 // to 448 = 1.75 * 2^8 (e4m3's largest) or less. A power of two costs e4m3 nothing
 // against a finer scale but the place of its smallest values (codes below 2^-6 are
 // 2^-14.8 of the largest at most), products with it are exact, and it is one byte.
-// Codes are rounded to nearest even, half a step, 2^-4 relative; what is not
-// finite becomes NaN.
+// Codes are rounded to nearest even, half a step: max(2^-4 of the value, 2^-10 of the
+// power); what is not finite becomes NaN.
 
 // The biased exponent, 1 .. 247, from the largest finite magnitude's bf16 bits.
 __device__ __forceinline__ int power_of(int bits) {

@@ -20,7 +20,7 @@ of two for each slot's k and v; a value is code times power.
 ``attention_paged``         attention of every new token: causal, sliding
                             window, first tokens that stay visible
 ``attention_shared_paged``  the same where groups of sequences have their
-                            first pages in common: those once per group
+                            first pages in common: those for many rows at once
 ``copy_pages``              pages copied within each of many caches
 ``PagedCache``              the layers' pages and the tables of a set of
                             sequences: reserve, fork, truncate, free, compact
@@ -153,7 +153,7 @@ def qkv_post_paged(qkv: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
     norms, RoPE of q and k at the row's position, k and v into their pages. With
     ``scales`` the pages are 8-bit: each head's k (v) gets the smallest power of two
     that brings its largest finite magnitude to 448 or less, its values the nearest
-    codes (half a step, 2^-4 relative); what is not finite becomes NaN.
+    codes (off by at most max(2^-4 |x|, 2^-10 power)); what is not finite becomes NaN.
     ``rope`` is the (positions, width) bfloat16 table, by default [cos | sin]
     halves of its rows. Returns q (T, heads * D); rows past the last sequence are
     left as they are in ``q_out``, zeros for a sequence that does not fit its
@@ -260,7 +260,7 @@ def attention_shared_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.
                            scales: torch.Tensor | None = None) -> torch.Tensor:
     """``attention_paged`` of a batch whose sequences come in groups with the same
     first pages (``PagedCache.shared`` finds them), which are read and multiplied
-    once for all of a group's rows. Group j is the sequences ``group_start[j] ..
+    for many of a group's rows at once. Group j is the sequences ``group_start[j] ..
     group_start[j + 1] - 1``; the first ``shared_len[j]`` positions of each (whole
     pages of them, and no more than the group's first sequence has) are taken from
     its first sequence's pages. Both are int32 tensors on the device, of groups + 1

@@ -529,12 +529,13 @@ int alv_attention_paged8(const uint16_t* q, int64_t ld_q, const uint8_t* kpages,
 /*
  * alv_attention_paged, or with scales alv_attention_paged8 (NULL: bf16 pages), of a
  * batch whose sequences come in groups with the same first positions, which are
- * read and multiplied once for all rows of a group. Group j < groups is the
+ * read and multiplied for many rows of a group at once. Group j < groups is the
  * sequences group_start[j] .. group_start[j + 1] - 1 (groups + 1 entries, not
  * decreasing); the first shared_len[j] positions of each, whole pages of them and
  * no more than the group's first sequence has, are those of its first sequence:
  * the others' table entries for them do not matter. A sequence in no group shares
- * nothing. group_start and shared_len are int32 device memory, read by the
+ * nothing; nor does, beside malformed ones, one whose rows are not among its group's
+ * (group_start[j]'s first to group_start[j + 1]'s, as far as within T). group_start and shared_len are int32 device memory, read by the
  * kernels. Every row sees what alv_attention_paged lets it see; what the two
  * parts of a row give is joined by their maxima and sums in float32, so its last
  * bits may differ from that call's. workspace: alv_attention_shared_workspace
