@@ -535,7 +535,8 @@ int alv_attention_paged8(const uint16_t* q, int64_t ld_q, const uint8_t* kpages,
  * no more than the group's first sequence has, are those of its first sequence:
  * the others' table entries for them do not matter. A sequence in no group shares
  * nothing; nor does, beside malformed ones, one whose rows are not among its group's
- * (group_start[j]'s first to group_start[j + 1]'s, as far as within T). group_start and shared_len are int32 device memory, read by the
+ * (the first of group_start[j] up to the first of group_start[j + 1], as far as within
+ * T). group_start and shared_len are int32 device memory, read by the
  * kernels. Every row sees what alv_attention_paged lets it see; what the two
  * parts of a row give is joined by their maxima and sums in float32, so its last
  * bits may differ from that call's. workspace: alv_attention_shared_workspace
